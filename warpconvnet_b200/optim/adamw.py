@@ -1,0 +1,283 @@
+"""AdamW over many tensors in one launch (``csrc/adamw.cu``), moments in 32 bits or in 8.
+
+The moments of all tensors are one flat tensor each: a tensor's moments begin at its *slot*, a multiple of 256 elements, and fill
+whole blocks of 256.  With 8 bits they are codes of a logarithmic scale, 8 values to an octave, with one int16 base per block:
+the code ``k > 0`` stands for the fp32 number with the bits ``(k + base) << 20``, 0 for zero; the first moment has a sign in its
+top bit.  Numbers are rounded to a neighbouring code at random (a hash of the tensor's step and the element's place), so that the
+second moment, which moves by a thousandth per step, keeps its mean.
+"""
+from __future__ import annotations
+
+import functools
+import struct
+from array import array
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from .._native import check, dtype_code, lib, ptr, require_cuda, stream_ptr
+from ..nn.functional.batch_norm import _counter
+
+BLOCK = 256
+
+
+@functools.lru_cache(maxsize=256)
+def _bits(value: float) -> int:
+    """A number as the 64 bits of a double (calls pass integers only)."""
+    return struct.unpack("<q", struct.pack("<d", value))[0]
+
+
+def moment_slots(sizes: Sequence[int]) -> Tuple[List[int], int]:
+    """(first element of each tensor's moments, length of the flat moments) for tensors of these sizes in order."""
+    at, out = 0, []
+    for n in sizes:
+        out.append(at)
+        at += -(-n // BLOCK) * BLOCK
+    return out, at
+
+
+def _one(values, what: str):
+    kinds = set(values)
+    if len(kinds) != 1:
+        raise ValueError(f"{what} differ: {sorted(map(str, kinds))}")
+    return kinds.pop()
+
+
+def _scalar(t: Optional[Tensor], name: str, device: torch.device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.device != device or t.dtype != torch.float32 or t.numel() != 1:
+        raise ValueError(f"{name} must be one float32 on {device}, got {t.numel()} x {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _moments(m: Tensor, v: Tensor, m_base: Optional[Tensor], v_base: Optional[Tensor], device: torch.device) -> int:
+    """The length of the flat moments, which are checked."""
+    if (m_base is None) != (v_base is None):
+        raise ValueError("both moments have bases (8 bits) or none (32 bits)")
+    dtype = torch.float32 if m_base is None else torch.uint8
+    n = m.numel()
+    for t, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
+        if t.dtype != dtype or t.device != device or t.dim() != 1 or not t.is_contiguous() or t.numel() != n or n % BLOCK or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be a contiguous, 16-byte aligned 1-d {dtype} tensor of a multiple of {BLOCK} elements on {device}, "
+                             f"as long as the other moment; got {tuple(t.shape)} {t.dtype} on {t.device}")
+    for t, name in ((m_base, "exp_avg_base"), (v_base, "exp_avg_sq_base")):
+        if t is not None and (t.dtype != torch.int16 or t.device != device or t.numel() != n // BLOCK or not t.is_contiguous()):
+            raise ValueError(f"{name} must be {n // BLOCK} contiguous int16 on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return n
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tensor, exp_avg_sq: Tensor, steps: Tensor, *,
+               lr: Union[float, Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+               exp_avg_base: Optional[Tensor] = None, exp_avg_sq_base: Optional[Tensor] = None, slots: Optional[Sequence[int]] = None,
+               step_index: Optional[Sequence[int]] = None, grad_scale: Optional[Tensor] = None, found_inf: Optional[Tensor] = None) -> None:
+    """One AdamW step of ``params`` in place, computed in fp32.
+
+    ``params`` (contiguous, one dtype) and ``grads`` (one dtype, which may be another) are float32, float16 or bfloat16 CUDA
+    tensors of one device.  ``exp_avg`` / ``exp_avg_sq`` are the flat moments: float32, or uint8 codes with their int16 bases
+    (zeros to begin with).  ``slots`` are the tensors' places in them, one after the other (:func:`moment_slots`) where not
+    given.  ``steps`` (int32, on the device) counts each tensor's steps and is advanced; ``step_index`` are the tensors' places
+    in it.  ``lr`` may be a float32 device tensor, which a captured step reads at every replay.  Gradients are divided by
+    ``grad_scale``; the step is cancelled where ``found_inf`` is not zero."""
+    if len(params) != len(grads):
+        raise ValueError(f"{len(params)} parameters but {len(grads)} gradients")
+    if not params:
+        return
+    device, dtype = _one([p.device for p in params], "devices of the parameters"), _one([p.dtype for p in params], "dtypes of the parameters")
+    require_cuda(params[0], "params")
+    if _one([g.device for g in grads], "devices of the gradients") != device:
+        raise ValueError(f"gradients must be on {device}")
+    if any(g.layout != torch.strided for g in grads):
+        raise TypeError("gradients must be dense")
+    grad_dtype = _one([g.dtype for g in grads], "dtypes of the gradients")
+    codes = dtype_code(dtype), dtype_code(grad_dtype)
+    if not all([p.is_contiguous() for p in params]):
+        raise ValueError("parameters must be contiguous: they are updated in place")
+    if [p.shape for p in params] != [g.shape for g in grads]:
+        raise ValueError("a gradient has another shape than its parameter")
+    sizes = [p.numel() for p in params]
+    length = _moments(exp_avg, exp_avg_sq, exp_avg_base, exp_avg_sq_base, device)
+    if slots is None:
+        slots, need = moment_slots(sizes)
+    else:
+        if len(slots) != len(params) or any(s % BLOCK or s < 0 for s in slots):
+            raise ValueError(f"slots must be {len(params)} multiples of {BLOCK}")
+        need = max([s + -(-n // BLOCK) * BLOCK for s, n in zip(slots, sizes)])
+    if need > length:
+        raise ValueError(f"the moments have {length} elements, the tensors need {need}")
+    if step_index is None:
+        step_index = range(len(params))
+    if steps.dtype != torch.int32 or steps.device != device or not steps.is_contiguous():
+        raise ValueError(f"steps must be contiguous int32 on {device}, got {steps.dtype} on {steps.device}")
+    if len(step_index) != len(params) or min(step_index) < 0 or max(step_index) >= steps.numel():
+        raise ValueError(f"steps has {steps.numel()} elements: not a place for each of {len(params)} tensors")
+    lr_at = None
+    if isinstance(lr, Tensor):
+        if lr.is_cuda:
+            lr_at, lr = _scalar(lr, "lr", device), 0.0
+        else:
+            lr = float(lr)
+    if not all([g.is_contiguous() for g in grads]):
+        grads = [g.contiguous() for g in grads]
+    table = array("q")
+    for row in zip([p.data_ptr() for p in params], [g.data_ptr() for g in grads], sizes, slots, step_index):
+        table.extend(row)
+    stream = stream_ptr(device)
+    with torch.cuda.device(device):
+        check(lib().wcn_adamw_step(table.buffer_info()[0], len(params), *codes, ptr(exp_avg), ptr(exp_avg_base), ptr(exp_avg_sq),
+                                   ptr(exp_avg_sq_base), ptr(steps), _bits(lr), _bits(betas[0]), _bits(betas[1]), _bits(eps),
+                                   _bits(weight_decay), lr_at, _scalar(grad_scale, "grad_scale", device),
+                                   _scalar(found_inf, "found_inf", device), ptr(_counter(device, stream)), stream), "wcn_adamw_step")
+    torch.autograd.graph.increment_version(list(params))
+
+
+def decode_moments(exp_avg: Tensor, exp_avg_base: Tensor, exp_avg_sq: Tensor, exp_avg_sq_base: Tensor) -> Tuple[Tensor, Tensor]:
+    """The numbers that 8-bit moments stand for, as flat fp32 tensors."""
+    require_cuda(exp_avg, "exp_avg")
+    device = exp_avg.device
+    n = _moments(exp_avg, exp_avg_sq, exp_avg_base, exp_avg_sq_base, device)
+    m, v = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
+    with torch.cuda.device(device):
+        check(lib().wcn_adamw_decode(ptr(exp_avg), ptr(exp_avg_base), ptr(exp_avg_sq), ptr(exp_avg_sq_base), n, ptr(m), ptr(v),
+                                     stream_ptr(device)), "wcn_adamw_decode")
+    return m, v
+
+
+class _Arena:
+    """The flat moments and step counts of some parameters."""
+
+    def __init__(self, params: Sequence[Tensor], bits: int):
+        device = params[0].device
+        slots, length = moment_slots([p.numel() for p in params])
+        dtype = torch.float32 if bits == 32 else torch.uint8
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(length, dtype=dtype, device=device) for _ in range(2))
+        self.exp_avg_base = self.exp_avg_sq_base = None
+        if bits == 8:
+            self.exp_avg_base, self.exp_avg_sq_base = (torch.zeros(length // BLOCK, dtype=torch.int16, device=device) for _ in range(2))
+        self.steps = torch.zeros(len(params), dtype=torch.int32, device=device)
+        self.place = {p: (i, s) for i, (p, s) in enumerate(zip(params, slots))}
+
+    def state(self, p: Tensor) -> dict:
+        """Views of what is kept for a parameter."""
+        i, s = self.place[p]
+        blocks = -(-p.numel() // BLOCK)
+        if self.exp_avg_base is None:
+            return {"step": self.steps[i], "exp_avg": self.exp_avg[s:s + p.numel()].view(p.shape), "exp_avg_sq": self.exp_avg_sq[s:s + p.numel()].view(p.shape)}
+        base = slice(s // BLOCK, s // BLOCK + blocks)
+        return {"step": self.steps[i], "exp_avg": self.exp_avg[s:s + blocks * BLOCK], "exp_avg_base": self.exp_avg_base[base],
+                "exp_avg_sq": self.exp_avg_sq[s:s + blocks * BLOCK], "exp_avg_sq_base": self.exp_avg_sq_base[base]}
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` as one launch per group and dtype.
+
+    ``state_bits``: 32, or 8 for moments of a byte each (a quarter of the memory, and 16 instead of 28 bytes of traffic per
+    fp32 parameter).  The moments live in flat tensors; ``state[p]`` are views of them.  Nothing is read back to the host:
+    steps can be captured in a CUDA graph (with a float32 device tensor as ``lr`` where that changes), and ``torch.amp.GradScaler``
+    hands its scale and its infinity flag to the kernel.  Parameters are float32, float16 or bfloat16, contiguous and on CUDA
+    devices at the first step."""
+
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32):
+        if not isinstance(lr, Tensor) and not 0.0 <= lr:
+            raise ValueError(f"invalid learning rate: {lr}")
+        if isinstance(lr, Tensor) and lr.numel() != 1:
+            raise ValueError("a learning rate is one number")
+        if not 0.0 <= eps:
+            raise ValueError(f"invalid epsilon: {eps}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"invalid betas: {betas}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"invalid weight decay: {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, got {state_bits}")
+        self._arena_of: dict = {}
+        self.state_bits = state_bits
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if self.param_groups[-1]["state_bits"] != self.state_bits:
+            self.param_groups.pop()
+            raise ValueError(f"all groups of this optimizer have moments of {self.state_bits} bits")
+
+    def _make_room(self, params: Sequence[Tensor]) -> None:
+        """Moments for the parameters that have none."""
+        by_device: dict = {}
+        for p in params:
+            by_device.setdefault(p.device, []).append(p)
+        for group in by_device.values():
+            arena = _Arena(group, self.state_bits)
+            for p in group:
+                self._arena_of[p] = arena
+                self.state[p] = arena.state(p)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        for group in self.param_groups:
+            buckets: dict = {}
+            params = [p for p in group["params"] if p.grad is not None]
+            missing = [p for p in params if p not in self._arena_of]
+            if missing:
+                self._make_room([p for p in group["params"] if p not in self._arena_of])
+            for p in params:
+                buckets.setdefault((id(self._arena_of[p]), p.dtype, p.grad.dtype), []).append(p)
+            for (_, _, _), some in buckets.items():
+                arena = self._arena_of[some[0]]
+                places = [arena.place[p] for p in some]
+                adamw_step(some, [p.grad for p in some], arena.exp_avg, arena.exp_avg_sq, arena.steps, lr=group["lr"], betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"], exp_avg_base=arena.exp_avg_base,
+                           exp_avg_sq_base=arena.exp_avg_sq_base, slots=[s for _, s in places], step_index=[i for i, _ in places],
+                           grad_scale=scale, found_inf=found)
+        return loss
+
+    # -- what is kept travels as the views of ``state``: copies are put into flat tensors again
+
+    def _take_state(self, state: dict) -> None:
+        """Moments and steps from ``{parameter: entries}``."""
+        self._arena_of = {}
+        self.state.clear()
+        known = [p for g in self.param_groups for p in g["params"] if p in state]
+        for p in known:
+            if not p.is_cuda:
+                raise ValueError("move the parameters to their device before their optimizer's state is loaded")
+        self._make_room(known)
+        for p in known:
+            mine = self.state[p]
+            if set(mine) != set(state[p]):
+                raise ValueError(f"state with {sorted(state[p])} cannot be loaded into an optimizer with moments of {self.state_bits} bits")
+            for name, view in mine.items():
+                value = torch.as_tensor(state[p][name])
+                if value.numel() != view.numel():
+                    raise ValueError(f"{name} of a parameter with {p.numel()} elements has {value.numel()}")
+                view.copy_(value.to(view.device).view(view.shape))
+
+    def load_state_dict(self, state_dict):
+        """Takes the state of an optimizer of this class with the same ``state_bits``, and with 32 bits one of ``torch.optim.AdamW``."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        names = [i for g in state_dict["param_groups"] for i in g["params"]]
+        entries = {p: state_dict["state"][i] for p, i in zip(params, names) if i in state_dict["state"]}
+        bits = {g.get("state_bits", 32) for g in state_dict["param_groups"]}
+        if bits - {self.state_bits}:
+            raise ValueError(f"moments of {sorted(bits)} bits cannot be loaded into an optimizer with moments of {self.state_bits} bits")
+        groups = [{**own, **g} for own, g in zip(({k: v for k, v in g.items() if k != "params"} for g in self.param_groups), state_dict["param_groups"])]
+        if len(groups) != len(self.param_groups) or len(state_dict["param_groups"]) != len(self.param_groups):
+            raise ValueError("loaded state dict has a different number of parameter groups")
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self._take_state(entries)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.state_bits = self.defaults["state_bits"]
+        self._arena_of = {}
+        if "state" in state:
+            self._take_state({p: dict(entries) for p, entries in self.state.items()})
