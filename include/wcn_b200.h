@@ -587,6 +587,26 @@ int wcn_batch_norm_backward(const void* x, const void* dy, const void* y, int64_
                             const float* gamma, const float* beta, const float* mean, const float* rstd, int relu, void* dx,
                             void* dresidual, float* sums, void* workspace, uint32_t* counter, void* stream);
 
+/* ------------------------------------------------------------------ group normalisation per scene */
+
+/* y = act(gamma * (x - mean) / sqrt(var + eps) + beta) of rows [offsets[scenes], channels], x with rows x_ld elements apart, y
+ * contiguous; mean and (biased) variance are those of a scene's rows offsets[b] .. offsets[b + 1] (a host array that rises from
+ * 0) and a group's channels / groups channels.  gamma, beta: fp32 [channels] or NULL; act: 0 none, 1 ReLU, 2 SiLU, 3 GELU (of
+ * the error function); eps as the bits of a float.  mean / rstd [scenes, groups] (both or neither) are left for the backward
+ * pass; those of empty scenes are not written.
+ * backward: dx contiguous (may be NULL), sums [2, channels] = d beta, d gamma (may be NULL).
+ * workspace: 16-byte aligned, the bytes that the query gives.  At most 4096 channels and 2^31 - 2^16 rows.
+ * The reference normalises per row (warpconvnet/nn/modules/normalizations.py) and has segment statistics as torch operations. */
+int wcn_group_norm_workspace_bytes(const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups, int dtype,
+                                   int backward, int64_t* bytes);
+int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups, int dtype,
+                   const float* gamma, const float* beta, uint32_t eps_bits, int act, void* y, float* mean, float* rstd,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const int64_t* offsets, int64_t scenes,
+                            int32_t channels, int32_t groups, int dtype, const float* gamma, const float* beta,
+                            const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ AdamW over many tensors */
 
 /* One tensor of wcn_adamw_step: n elements of a parameter and its gradient (contiguous), the first element of its moments
