@@ -607,6 +607,30 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
                             const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ cross entropy of a linear layer */
+
+/* loss_rows[i] = log sum_j exp(z_ij) - z_iy of z = x w^T + bias, x [n, channels], w [classes, channels] of one dtype (rows x_ld and
+ * w_ld elements apart; in 16 bits: 16-byte aligned, the distances multiples of 8), bias [classes] of bias_dtype or NULL, one
+ * int64 label a row; z is not kept.  A row whose label is `ignore` has the loss 0; so has one whose label names no class, for
+ * which WCN_ERR_BOUNDS is stored.  reduction: 0 none, 1 mean over the *count rows that count, 2 sum (*loss).
+ * Left for the backward pass: lse2 [n] (log-sum-exp in units of ln 2), loss_rows, count, and with a bias bias2
+ * [classes rounded up to 256, + 256] (16-byte aligned).  counter: one zero word, zero again afterwards (one per stream).
+ * backward: gradients of x [n, channels] and w [classes, channels] (contiguous, 16-byte aligned, of dtype) and of the bias (of
+ * bias_dtype), each of which may be NULL.  grad: one number; or, with row_max (their largest magnitude), one a row's loss.
+ * count: of a mean, else NULL.  Few launches for small problems, some for every piece of 256 MB of the logits' gradient.
+ * workspace: 16-byte aligned; `what` of the query: 0 forward, else the sum of 1 (dx), 2 (dw), 4 (dbias).
+ * Stands for a 1x1x1 convolution to classes (examples/mink_unet.py:405-413) and torch.nn.functional.cross_entropy behind it. */
+int wcn_linear_ce_workspace_bytes(int64_t n, int32_t channels, int64_t classes, int dtype, int what, int64_t* bytes);
+int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t channels, const void* w, int64_t w_ld, int64_t classes,
+                  const void* bias, int bias_dtype, const int64_t* labels, int64_t ignore, int dtype, int reduction, float* lse2,
+                  float* loss_rows, float* bias2, int32_t* count, float* loss, void* workspace, int64_t workspace_bytes,
+                  uint32_t* counter, int32_t* dev_status, void* stream);
+int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, int32_t channels, const void* w, int64_t w_ld, int64_t classes,
+                           const float* bias2, const int64_t* labels, int64_t ignore, int dtype, const float* lse2,
+                           const float* loss_rows, const int32_t* count, const float* grad, const float* row_max, void* dx,
+                           void* dw, void* dbias, int bias_dtype, void* workspace, int64_t workspace_bytes, int32_t* dev_status,
+                           void* stream);
+
 /* ------------------------------------------------------------------ AdamW over many tensors */
 
 /* One tensor of wcn_adamw_step: n elements of a parameter and its gradient (contiguous), the first element of its moments

@@ -16,11 +16,13 @@ from .geometry.coords.search.torch_hashmap import HashMethod, TorchHashTable
 from .geometry.features.cat import CatFeatures
 from .geometry.types.voxels import Voxels
 from .nn.functional.group_norm import segmented_group_norm
+from .nn.functional.linear_cross_entropy import linear_cross_entropy
 from .nn.functional.sparse_conv import (SPARSE_CONV_BWD_ALGO_MODE, SPARSE_CONV_FWD_ALGO_MODE, STRIDED_CONV_MODE,
                                         ConvEpilogue, spatially_sparse_conv)
 from .nn.functional.sparse_pool import sparse_avg_pool, sparse_max_pool, sparse_reduce, sparse_unpool
 from .nn.functional.transforms import cat
 from .nn.modules.activations import ReLU
+from .nn.modules.loss import LinearCrossEntropy
 from .nn.modules.normalizations import BatchNorm, SegmentedGroupNorm
 from .nn.modules.sequential import Sequential
 from .nn.modules.sparse_conv import SparseConv2d, SparseConv3d, SpatiallySparseConv

@@ -26,9 +26,8 @@
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, drains
 // its copies and frees its tensor memory.
-#include <cuda.h>
-
 #include "tcgen05_common.cuh"
+#include "tma_common.cuh"
 
 namespace {
 
@@ -79,21 +78,6 @@ struct RowsControl {
   int32_t skip;
   float sc[MAX_COLS], sh[MAX_COLS];
 };
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-
-// 32 bytes in one request: a whole sector per lane, so that rows scattered over the output cost the
-// L2 one full-sector write each instead of two half-sector ones.
-__device__ __forceinline__ void st_global_32B(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 
 // One 16-column piece of a row: convert and store columns [c0, c0 + 16) that exist (< c_store).
 template <typename TO>
@@ -452,24 +436,6 @@ bool plan_rows(int K, int c_in, int c_out, RowsParams* p, size_t* smem) {
   p->nacc = 512 / (q * c_out) < MAX_ACC ? 512 / (q * c_out) : MAX_ACC;  // q * c_out <= 256: at least two
   *smem = (size_t)(nbuf * q * per_offset + stages * a_bytes + fixed);
   return true;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult res;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &res) == cudaSuccess &&
-        res == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(sym);
-    tried = true;
-  }
-  return fn;
 }
 
 template <int BK, bool BF16, typename TO, bool GROUPED>

@@ -1,0 +1,590 @@
+// Cross entropy of a linear layer's logits z = x w^T + b [n rows, v classes] against one label per row, without keeping z:
+//     loss_i = log sum_j exp(z_ij) - z_iy                       over rows whose label is not `ignore`: mean, sum, or each
+//     g = s_i (softmax(z_i) - onehot(y_i))      dx = g w      dw = g^T x      db = sums of g's columns
+//
+// Forward: one pass over tiles of z, of which each row keeps a running (largest, sum of exponentials); then a warp a row puts
+// the pieces of its classes together and takes z_iy from a product of its own, in fp32 (the label's logit would cost the tiles a
+// comparison each).  Backward: z again, piece by piece of rows x classes; a piece's g goes to the workspace in x's type and is
+// multiplied by w and by x from there.  Products whose sums over k are divided, or that several pieces add to, are put together
+// in fp32 in a fixed order: the same bits on every run.
+// g is rounded to 16 bits as softmax - onehot, without the rows' factor, which the results are multiplied by in fp32: labels'
+// entries are the largest ones and keep 8 (11) bits whatever the number of rows.  (In fp16 it is raised by 2^14: a probability
+// of 2^-28 is still a normal number.)
+//
+// 16-bit types run on the tensor cores (linear_ce_tcgen05.cu); fp32 on the FMA pipes here, in tiles of 64 x 64, sums of 128
+// products at a time.
+#include "linear_ce.cuh"
+
+int wcn_ce_logits_splits(int rows, int classes);
+int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st);
+int wcn_ce_product_splits(int m, int n, int k);
+int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, int dtype, int32_t* dev_status, cudaStream_t st);
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LN2 = 0.6931471805599453;
+constexpr int64_t PIECE_BYTES = 256ll << 20;   // of g
+constexpr int PIECE_ROWS = 148 * 128;
+
+inline float lift_of(int dtype) { return dtype == WCN_F16 ? 14.f : 0.f; }
+
+// ------------------------------------------------------------------ around the products
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) ce_bias_kernel(const T* bias, int64_t v, int64_t padded, float* bias2) {
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < padded; i += (int64_t)gridDim.x * THREADS)
+    bias2[i] = i < v ? wcn_to_float<T>(bias[i]) * LOG2E : -INFINITY;
+}
+
+struct LossParams {
+  const void* x;
+  const void* w;
+  int64_t x_ld, w_ld, n, v;
+  int c, parts, reduction;
+  const float* bias2;
+  const int64_t* labels;
+  int64_t ignore;
+  const float2* part;      // [parts][n]
+  float* lse2;
+  float* loss_rows;
+  float* loss;
+  int32_t* count;
+  double* block_sums;      // [blocks]
+  int32_t* block_counts;   // [blocks]
+  unsigned* counter;
+  int32_t* dev_status;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant__ LossParams p) {
+  __shared__ double s_sum[THREADS / 32];
+  __shared__ int s_count[THREADS / 32];
+  __shared__ bool last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool failed = *(volatile int32_t*)p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
+  double total = 0;
+  int counted = 0;
+  bool bad = false;
+  for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < p.n; r += (int64_t)gridDim.x * (THREADS / 32)) {
+    const int64_t y = __ldg(&p.labels[r]);
+    const bool counts = y != p.ignore && y >= 0 && y < p.v;
+    bad |= y != p.ignore && !counts;
+    float dot = 0.f;
+    if (counts) {
+      const T *const xr = reinterpret_cast<const T*>(p.x) + r * p.x_ld, *const wr = reinterpret_cast<const T*>(p.w) + y * p.w_ld;
+      for (int c = lane; c < p.c; c += 32) dot = fmaf(wcn_to_float<T>(xr[c]), wcn_to_float<T>(wr[c]), dot);
+    }
+    float top = -INFINITY, sum = 0.f;
+    for (int i = lane; i < p.parts; i += 32) {
+      const float2 q = __ldg(&p.part[(int64_t)i * p.n + r]);
+      const float now = fmaxf(top, q.x), by = now == -INFINITY ? 0.f : now;
+      sum = sum * exp2f(top - by) + q.y * exp2f(q.x - by);
+      top = now;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+      const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      const float now = fmaxf(top, t), by = now == -INFINITY ? 0.f : now;
+      sum = sum * exp2f(top - by) + s * exp2f(t - by);
+      top = now;
+    }
+    const float lse2 = top + log2f(sum);
+    float loss = 0.f;
+    if (counts) {
+      const float z = p.bias2 ? fmaf(dot, LOG2E, __ldg(&p.bias2[y])) : dot * LOG2E;
+      loss = (lse2 - z) * (float)LN2;
+      if (loss < 0.f) loss = 0.f;                       // (roundings of a probability of one)
+    }
+    if (failed) loss = __int_as_float(0x7FC00000);
+    total += (double)loss;
+    counted += counts;
+    if (lane == 0) {
+      p.lse2[r] = lse2;
+      p.loss_rows[r] = loss;
+    }
+  }
+  if (bad && lane == 0) wcn_report_bounds(p.dev_status);
+  if (!p.loss) return;
+  if (lane == 0) { s_sum[warp] = total; s_count[warp] = counted; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < THREADS / 32; ++i) { total += s_sum[i]; counted += s_count[i]; }
+    p.block_sums[blockIdx.x] = total;
+    p.block_counts[blockIdx.x] = counted;
+    __threadfence();
+    last = atomicAdd(p.counter, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  total = 0;
+  counted = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) {
+    total += __ldcg(&p.block_sums[i]);
+    counted += __ldcg(&p.block_counts[i]);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    counted += __shfl_xor_sync(0xFFFFFFFFu, counted, o);
+  }
+  if (lane == 0) { s_sum[warp] = total; s_count[warp] = counted; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < THREADS / 32; ++i) { total += s_sum[i]; counted += s_count[i]; }
+    *p.loss = (float)(p.reduction == 1 ? total / (double)counted : total);
+    *p.count = counted;
+    *p.counter = 0;
+  }
+}
+
+// acc (+)= sums of the splits, or the finished result.  Four columns a thread, SIDE threads that share the splits.
+struct JoinParams {
+  const float* slab;       // [splits][m][ld]
+  float* acc;              // [m][ld] (null: nothing before, nothing after)
+  bool add;                // acc has something already
+  void* out;               // [m][n]; null: acc is written
+  int64_t m;
+  int n, ld, splits;
+  wcn_ce_scale scale;
+  const int32_t* dev_status;
+};
+
+template <typename TO, int SIDE>
+__global__ void __launch_bounds__(THREADS) ce_join_kernel(const __grid_constant__ JoinParams p) {
+  constexpr int QUADS = THREADS / SIDE;
+  __shared__ double part[SIDE > 1 ? THREADS : 1][4];
+  const int side = threadIdx.x / QUADS, at = threadIdx.x % QUADS;
+  const int quads = p.ld / 4;
+  const int64_t all = p.m * quads, q = (int64_t)blockIdx.x * QUADS + at;
+  double v[4] = {0, 0, 0, 0};
+  if (q < all) {
+    const float4* const from = reinterpret_cast<const float4*>(p.slab) + q;
+#pragma unroll 4
+    for (int s = side; s < p.splits; s += SIDE) {
+      const float4 t = __ldg(from + (int64_t)s * all);
+      v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+    }
+  }
+  if (SIDE > 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[threadIdx.x][i] = v[i];
+    __syncthreads();
+    if (side) return;
+    for (int s = 1; s < SIDE; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += part[s * QUADS + at][i];
+  }
+  if (q >= all) return;
+  const int64_t row = q / quads;
+  const int col = (int)(q % quads) * 4;
+  if (p.add) {
+    const float4 t = reinterpret_cast<const float4*>(p.acc)[q];
+    v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+  }
+  if (!p.out) {
+    reinterpret_cast<float4*>(p.acc)[q] = make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+    return;
+  }
+  const int count = p.scale.count ? *p.scale.count : 1;
+  float scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
+  if (*p.dev_status == (int)WCN_ERR_WAIT_EXPIRED) scale = __int_as_float(0x7FC00000);
+  TO* const out = reinterpret_cast<TO*>(p.out) + row * p.n + col;
+  __align__(16) TO r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = wcn_from_float<TO>((float)v[i] * scale);
+  if (p.n % 4 == 0) {   // (the result is a tensor's memory: its rows of whole quads start on their boundaries)
+    if (col < p.n) {
+      if (sizeof(TO) == 2) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(r);
+      else *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(r);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < p.n) out[i] = r[i];
+  }
+}
+
+// The same of one number a class: 32 classes a block, eight threads that share the splits.
+template <typename TO>
+__global__ void __launch_bounds__(THREADS) ce_join_sums_kernel(const __grid_constant__ JoinParams p) {
+  __shared__ double part[THREADS / 32][33];
+  const int lane = threadIdx.x & 31, side = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  double v = 0;
+  if (i < p.m)
+#pragma unroll 4
+    for (int s = side; s < p.splits; s += THREADS / 32) v += (double)__ldg(&p.slab[(int64_t)s * p.m + i]);
+  part[side][lane] = v;
+  __syncthreads();
+  if (side || i >= p.m) return;
+  for (int s = 1; s < THREADS / 32; ++s) v += part[s][lane];
+  if (p.add) v += (double)p.acc[i];
+  if (!p.out) {
+    p.acc[i] = (float)v;
+    return;
+  }
+  const int count = p.scale.count ? *p.scale.count : 1;
+  float scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
+  if (*p.dev_status == (int)WCN_ERR_WAIT_EXPIRED) scale = __int_as_float(0x7FC00000);
+  reinterpret_cast<TO*>(p.out)[i] = wcn_from_float<TO>((float)v * scale);
+}
+
+template <typename TO> int join_as(const JoinParams& p, cudaStream_t st) {
+  if (p.ld == 1) {
+    ce_join_sums_kernel<TO><<<(unsigned)((p.m + 31) / 32), THREADS, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+  }
+  const int64_t all = p.m * (p.ld / 4);
+  if (p.splits >= 16) ce_join_kernel<TO, 8><<<(unsigned)((all + THREADS / 8 - 1) / (THREADS / 8)), THREADS, 0, st>>>(p);
+  else ce_join_kernel<TO, 1><<<(unsigned)((all + THREADS - 1) / THREADS), THREADS, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+int join(const JoinParams& p, int dtype, cudaStream_t st) {
+  if (dtype == WCN_F32) return join_as<float>(p, st);
+  if (dtype == WCN_F16) return join_as<__half>(p, st);
+  return join_as<__nv_bfloat16>(p, st);
+}
+
+// ------------------------------------------------------------------ fp32
+
+constexpr int TILE = 64, DEPTH = 16, CHAIN = 128;   // a chain of 128 products has a sum of its own
+
+enum Layout { LOGITS = 0, ROWS_BY_CLASSES = 1, CLASSES_BY_ROWS = 2 };   // A[m][k] B[n][k]; A[m][k] B[k][n]; A[k][m] B[k][n]
+
+// One tile of 64 x 64 sums over k in [k0, k1): a thread has rows ty * 4 .. and columns tx * 4 ..; `sums`: A's row sums (tx = 0).
+template <int LAYOUT>
+__device__ __forceinline__ void fp32_tile(const float* a, int64_t a_ld, const float* b, int64_t b_ld, int m0, int n0, int m, int n, int k0, int k1,
+                                          float (&out)[4][4], float (&sums)[4]) {
+  __shared__ __align__(16) float sa[DEPTH][TILE + 4], sb[DEPTH][TILE + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4], part[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sums[i] = part[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = out[i][j] = 0.f;
+  }
+  int chain = 0;
+  for (int k = k0; k < k1; k += DEPTH) {
+#pragma unroll
+    for (int i = threadIdx.x; i < TILE * DEPTH; i += THREADS) {
+      {
+        const int kk = LAYOUT == CLASSES_BY_ROWS ? i / TILE : i % DEPTH, r = LAYOUT == CLASSES_BY_ROWS ? i % TILE : i / DEPTH;
+        const bool in = k + kk < k1 && m0 + r < m;
+        sa[kk][r] = in ? __ldg(LAYOUT == CLASSES_BY_ROWS ? a + (int64_t)(k + kk) * a_ld + m0 + r : a + (int64_t)(m0 + r) * a_ld + k + kk) : 0.f;
+      }
+      {
+        const int kk = LAYOUT == LOGITS ? i % DEPTH : i / TILE, r = LAYOUT == LOGITS ? i / DEPTH : i % TILE;
+        const bool in = k + kk < k1 && n0 + r < n;
+        sb[kk][r] = in ? __ldg(LAYOUT == LOGITS ? b + (int64_t)(n0 + r) * b_ld + k + kk : b + (int64_t)(k + kk) * b_ld + n0 + r) : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < DEPTH; ++kk) {
+      const float4 u = *reinterpret_cast<const float4*>(&sa[kk][ty * 4]), v = *reinterpret_cast<const float4*>(&sb[kk][tx * 4]);
+      const float x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[i] += x[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+      }
+    }
+    __syncthreads();
+    if (++chain == CHAIN / DEPTH || k + DEPTH >= k1) {
+      chain = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sums[i] += part[i];
+        part[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { out[i][j] += acc[i][j]; acc[i][j] = 0.f; }
+      }
+    }
+  }
+}
+
+template <bool GRAD>
+__global__ void __launch_bounds__(THREADS) ce_logits_fp32_kernel(const __grid_constant__ wcn_ce_piece q) {
+  const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float z[4][4], unused[4];
+  fp32_tile<LOGITS>((const float*)q.x, q.x_ld, (const float*)q.w, q.w_ld, m0, n0, q.rows, q.classes, 0, q.channels, z, unused);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = n0 + tx * 4 + j;
+      z[i][j] = col >= q.classes ? -INFINITY : q.bias2 ? fmaf(z[i][j], LOG2E, __ldg(&q.bias2[col])) : z[i][j] * LOG2E;
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m0 + ty * 4 + i;
+    if (!GRAD) {
+      float top = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3])), by = top == -INFINITY ? 0.f : top, sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += exp2f(z[i][j] - by);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) {   // the 16 threads of a row
+        const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const float now = fmaxf(top, t);
+        by = now == -INFINITY ? 0.f : now;
+        sum = sum * exp2f(top - by) + s * exp2f(t - by);
+        top = now;
+      }
+      if (tx == 0 && row < q.rows) q.part[(int64_t)blockIdx.y * q.rows + row] = make_float2(top, sum);
+    } else if (row < q.rows) {
+      const int64_t y = __ldg(&q.labels[row]);
+      const bool counts = y != q.ignore && y >= 0 && y < q.all_classes;
+      float scale = 1.f;
+      if (q.row_scale) {
+        const float most = __ldg(q.row_max);
+        scale = most > 0.f ? __ldg(&q.row_scale[row]) / most : most == most ? 0.f : most;
+      }
+      const float lse2 = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = n0 + tx * 4 + j;
+        if (col >= q.classes) continue;
+        float g = 0.f;
+        if (counts) g = scale * (y - q.first_class == col ? expm1f(-loss) : exp2f(z[i][j] - lse2));
+        reinterpret_cast<float*>(q.g)[(int64_t)row * q.g_ld + col] = g;
+      }
+    }
+  }
+}
+
+template <bool TRANS>
+__global__ void __launch_bounds__(THREADS) ce_product_fp32_kernel(const __grid_constant__ wcn_ce_product q, int per) {
+  const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, split = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float d[4][4], sums[4];
+  const int k0 = split * per, k1 = min(k0 + per, q.k);
+  fp32_tile<TRANS ? CLASSES_BY_ROWS : ROWS_BY_CLASSES>((const float*)q.a, q.a_ld, (const float*)q.b, q.b_ld, m0, n0, q.m, q.n, k0, k1, d, sums);
+  const int ld = wcn_ce_round(q.n, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m0 + ty * 4 + i;
+    if (row >= q.m) continue;
+    if (n0 + tx * 4 < ld)
+      *reinterpret_cast<float4*>(q.slab + ((int64_t)split * q.m + row) * ld + n0 + tx * 4) = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
+    if (q.slab_ones && n0 == 0 && tx == 0) q.slab_ones[(int64_t)split * q.m + row] = sums[i];
+  }
+}
+
+int fp32_splits(int m, int n, int k) {
+  const int64_t tiles = (int64_t)((m + TILE - 1) / TILE) * ((n + TILE - 1) / TILE), want = (8 * (int64_t)wcn_num_sms() + tiles - 1) / tiles;
+  const int chains = (k + CHAIN - 1) / CHAIN;
+  const int s = (int)(want < chains ? want : chains), per = (chains + s - 1) / s;
+  return (chains + per - 1) / per;
+}
+
+int fp32_product(const wcn_ce_product& q, bool transposed, cudaStream_t st) {
+  const int chains = (q.k + CHAIN - 1) / CHAIN, per = (chains + q.splits - 1) / q.splits * CHAIN;
+  const dim3 grid((q.m + TILE - 1) / TILE, (q.n + TILE - 1) / TILE, q.splits);
+  if (transposed) ce_product_fp32_kernel<true><<<grid, THREADS, 0, st>>>(q, per);
+  else ce_product_fp32_kernel<false><<<grid, THREADS, 0, st>>>(q, per);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+// ------------------------------------------------------------------ plans
+
+int logit_parts(int64_t n, int64_t v, int dtype) {
+  return dtype == WCN_F32 ? (int)((v + TILE - 1) / TILE) : 2 * wcn_ce_logits_splits((int)n, (int)v);
+}
+int loss_blocks(int64_t n) {
+  const int64_t want = (n + THREADS / 32 - 1) / (THREADS / 32), most = 8 * (int64_t)wcn_num_sms();
+  return (int)(want < most ? want : most);
+}
+int product_splits(int m, int n, int k, int dtype) { return dtype == WCN_F32 ? fp32_splits(m, n, k) : wcn_ce_product_splits(m, n, k); }
+
+// How the gradient of the logits is cut into pieces, and where everything is in the workspace.
+struct Pieces {
+  int64_t n, v;
+  int c, ld, dtype;
+  int rows, classes, row_pieces, class_pieces;
+  int64_t g, slab_x, slab_w, slab_b, acc_x, acc_w, acc_b, bytes;
+  int64_t g_ld;
+};
+
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
+  Pieces p = {};
+  p.n = n; p.v = v; p.c = c; p.dtype = dtype;
+  p.ld = wcn_ce_round(c, 16);
+  const int e = wcn_dtype_size(dtype);
+  p.row_pieces = (int)((n + PIECE_ROWS - 1) / PIECE_ROWS);
+  if (v <= 1024) {   // few classes: all of them with as many rows as there is room for
+    const int64_t most = PIECE_BYTES / (e * ((v + 63) / 64 * 64)) / 128 * 128;
+    p.row_pieces = (int)((n + most - 1) / most);
+  }
+  p.rows = wcn_ce_round((n + p.row_pieces - 1) / p.row_pieces, 128);
+  p.row_pieces = (int)((n + p.rows - 1) / p.rows);
+  if (p.rows > n) p.rows = (int)n;
+  int64_t most = PIECE_BYTES / ((int64_t)p.rows * e) / 256 * 256;
+  if (most < 1024) most = 1024;
+  p.class_pieces = (int)((v + most - 1) / most);
+  p.classes = p.class_pieces == 1 ? (int)v : wcn_ce_round((v + p.class_pieces - 1) / p.class_pieces, 256);
+  p.class_pieces = (int)((v + p.classes - 1) / p.classes);
+  p.g_ld = wcn_ce_round(p.classes, 64);
+  // the largest slabs of any piece (the last ones are smaller, and their sums divided otherwise)
+  int64_t sx = 0, sw = 0, sb = 0;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j) {
+      const int64_t r = i ? n - (int64_t)(p.row_pieces - 1) * p.rows : p.rows, k = j ? v - (int64_t)(p.class_pieces - 1) * p.classes : p.classes;
+      const int64_t fx = product_splits((int)r, c, (int)k, dtype) * r * p.ld * 4, s = product_splits((int)k, c, (int)r, dtype);
+      if (fx > sx) sx = fx;
+      if (s * k * p.ld * 4 > sw) sw = s * k * p.ld * 4;
+      if (s * k * 4 > sb) sb = s * k * 4;
+    }
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t here = at; at += aligned(bytes); return here; };
+  p.g = take((int64_t)p.rows * p.g_ld * e);
+  p.slab_x = take(x ? sx : 0);
+  p.slab_w = take(w || b ? sw : 0);
+  p.slab_b = take(b ? (sb + 15) / 16 * 16 : 0);
+  p.acc_x = take(x && p.class_pieces > 1 ? (int64_t)p.rows * p.ld * 4 : 0);
+  p.acc_w = take(w && p.row_pieces > 1 ? v * p.ld * 4 : 0);
+  p.acc_b = take(b && p.row_pieces > 1 ? (v + 16) * 4 : 0);
+  p.bytes = at;
+  return p;
+}
+
+bool sizes_ok(int64_t n, int32_t c, int64_t v, int dtype) {
+  return n > 0 && n < 0x7FFFFF00ll && v > 0 && v < 0x7FFFFF00ll && v / TILE < 65535 && c > 0 && c <= 32768 && dtype >= WCN_F32 && dtype <= WCN_BF16;
+}
+
+bool matrix_ok(const void* p, int64_t ld, int c, int dtype) {
+  if (!p || ld < c) return false;
+  return dtype == WCN_F32 ? reinterpret_cast<uintptr_t>(p) % 4 == 0 : reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0;
+}
+
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+extern "C" int wcn_linear_ce_workspace_bytes(int64_t n, int32_t channels, int64_t classes, int dtype, int what, int64_t* bytes) {
+  if (!bytes || !sizes_ok(n, channels, classes, dtype)) return WCN_ERR_INVALID_PARAMETERS;
+  if (what) *bytes = cut(n, channels, classes, dtype, what & 1, what & 2, what & 4).bytes;
+  else *bytes = aligned((int64_t)logit_parts(n, classes, dtype) * n * 8) + (int64_t)loss_blocks(n) * 16;
+  return WCN_OK;
+}
+
+extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t channels, const void* w, int64_t w_ld, int64_t classes,
+                             const void* bias, int bias_dtype, const int64_t* labels, int64_t ignore, int dtype, int reduction,
+                             float* lse2, float* loss_rows, float* bias2, int32_t* count, float* loss, void* workspace,
+                             int64_t workspace_bytes, uint32_t* counter, int32_t* dev_status, void* stream) {
+  if (!sizes_ok(n, channels, classes, dtype) || !matrix_ok(x, x_ld, channels, dtype) || !matrix_ok(w, w_ld, channels, dtype) || !labels ||
+      !lse2 || !loss_rows || !workspace || !on16(workspace) || !counter || !dev_status || (bias && (!bias2 || !on16(bias2))) ||
+      reduction < 0 || reduction > 2 || (reduction && (!loss || !count)) || bias_dtype < WCN_F32 || bias_dtype > WCN_BF16)
+    return WCN_ERR_INVALID_PARAMETERS;
+  int64_t need = 0;
+  wcn_linear_ce_workspace_bytes(n, channels, classes, dtype, 0, &need);
+  if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  cudaStream_t st = wcn_stream(stream);
+  if (bias) {
+    const int64_t padded = (classes + 255) / 256 * 256 + 256;
+    const unsigned blocks = (unsigned)((padded + THREADS - 1) / THREADS < 1024 ? (padded + THREADS - 1) / THREADS : 1024);
+    if (bias_dtype == WCN_F32) ce_bias_kernel<float><<<blocks, THREADS, 0, st>>>((const float*)bias, classes, padded, bias2);
+    else if (bias_dtype == WCN_F16) ce_bias_kernel<__half><<<blocks, THREADS, 0, st>>>((const __half*)bias, classes, padded, bias2);
+    else ce_bias_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>((const __nv_bfloat16*)bias, classes, padded, bias2);
+  }
+  const int parts = logit_parts(n, classes, dtype);
+  wcn_ce_piece q = {};
+  q.x = x; q.w = w; q.x_ld = x_ld; q.w_ld = w_ld; q.rows = (int)n; q.classes = (int)classes; q.channels = channels;
+  q.bias2 = bias ? bias2 : nullptr;
+  q.part = (float2*)workspace;
+  if (dtype == WCN_F32) {
+    ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)((classes + TILE - 1) / TILE)), THREADS, 0, st>>>(q);
+  } else {
+    const int rc = wcn_ce_logits(q, dtype, false, 0.f, dev_status, st);
+    if (rc != WCN_OK) return rc;
+  }
+  LossParams p = {};
+  p.x = x; p.w = w; p.x_ld = x_ld; p.w_ld = w_ld; p.n = n; p.v = classes; p.c = channels; p.parts = parts; p.reduction = reduction;
+  p.bias2 = q.bias2; p.labels = labels; p.ignore = ignore; p.part = q.part; p.lse2 = lse2; p.loss_rows = loss_rows;
+  p.loss = reduction ? loss : nullptr; p.count = count; p.counter = counter; p.dev_status = dev_status;
+  const int blocks = loss_blocks(n);
+  p.block_sums = (double*)((char*)workspace + aligned((int64_t)parts * n * 8));
+  p.block_counts = (int32_t*)(p.block_sums + blocks);
+  if (dtype == WCN_F32) ce_loss_kernel<float><<<blocks, THREADS, 0, st>>>(p);
+  else if (dtype == WCN_F16) ce_loss_kernel<__half><<<blocks, THREADS, 0, st>>>(p);
+  else ce_loss_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, int32_t channels, const void* w, int64_t w_ld,
+                                      int64_t classes, const float* bias2, const int64_t* labels, int64_t ignore, int dtype,
+                                      const float* lse2, const float* loss_rows, const int32_t* count, const float* grad,
+                                      const float* row_max, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
+                                      int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+  if (!sizes_ok(n, channels, classes, dtype) || !matrix_ok(x, x_ld, channels, dtype) || !matrix_ok(w, w_ld, channels, dtype) || !labels ||
+      !lse2 || !loss_rows || !grad || !workspace || !on16(workspace) || !on16(dx) || !on16(dw) || !dev_status || bias_dtype < WCN_F32 ||
+      bias_dtype > WCN_BF16)
+    return WCN_ERR_INVALID_PARAMETERS;
+  if (!dx && !dw && !dbias) return WCN_OK;
+  const Pieces p = cut(n, channels, classes, dtype, dx, dw, dbias);
+  if (p.bytes > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  cudaStream_t st = wcn_stream(stream);
+  char* const ws = (char*)workspace;
+  const int e = wcn_dtype_size(dtype);
+  const float lift = lift_of(dtype);
+  const wcn_ce_scale scale = {row_max ? row_max : grad, count, dtype == WCN_F16 ? 1.f / 16384.f : 1.f};
+  for (int i = 0; i < p.row_pieces; ++i) {
+    const int64_t r0 = (int64_t)i * p.rows;
+    const int rows = (int)(n - r0 < p.rows ? n - r0 : p.rows);
+    for (int j = 0; j < p.class_pieces; ++j) {
+      const int64_t v0 = (int64_t)j * p.classes;
+      const int vs = (int)(classes - v0 < p.classes ? classes - v0 : p.classes);
+      wcn_ce_piece q = {};
+      q.x = (const char*)x + r0 * x_ld * e; q.w = (const char*)w + v0 * w_ld * e; q.x_ld = x_ld; q.w_ld = w_ld;
+      q.rows = rows; q.classes = vs; q.channels = channels; q.bias2 = bias2 ? bias2 + v0 : nullptr;
+      q.lse2 = lse2 + r0; q.loss = loss_rows + r0; q.labels = labels + r0; q.ignore = ignore; q.first_class = v0; q.all_classes = classes;
+      q.row_scale = row_max ? grad + r0 : nullptr; q.row_max = row_max;
+      q.g = ws + p.g; q.g_ld = p.g_ld;
+      int rc = WCN_OK;
+      if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q);
+      else rc = wcn_ce_logits(q, dtype, true, lift, dev_status, st);
+      if (rc != WCN_OK) return rc;
+      if (dx) {
+        wcn_ce_product d = {};
+        d.a = q.g; d.a_ld = p.g_ld; d.b = q.w; d.b_ld = w_ld; d.m = rows; d.n = channels; d.k = vs;
+        d.splits = product_splits(rows, channels, vs, dtype); d.slab = (float*)(ws + p.slab_x); d.scale = scale;
+        char* const out = (char*)dx + r0 * channels * e;
+        const bool whole = p.class_pieces == 1 && d.splits == 1 && dtype != WCN_F32;
+        if (whole) d.out = out;
+        rc = dtype == WCN_F32 ? fp32_product(d, false, st) : wcn_ce_product_run(d, false, dtype, dev_status, st);
+        if (rc != WCN_OK) return rc;
+        if (!whole) {
+          JoinParams jp = {d.slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? out : nullptr, rows, channels, p.ld, d.splits, scale, dev_status};
+          rc = join(jp, dtype, st);
+          if (rc != WCN_OK) return rc;
+        }
+      }
+      if (dw || dbias) {
+        wcn_ce_product d = {};
+        d.a = q.g; d.a_ld = p.g_ld; d.b = q.x; d.b_ld = x_ld; d.m = vs; d.n = channels; d.k = rows;
+        d.splits = product_splits(vs, channels, rows, dtype); d.slab = (float*)(ws + p.slab_w); d.scale = scale;
+        d.slab_ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
+        rc = dtype == WCN_F32 ? fp32_product(d, true, st) : wcn_ce_product_run(d, true, dtype, dev_status, st);
+        if (rc != WCN_OK) return rc;
+        const bool done = i == p.row_pieces - 1;
+        if (dw) {
+          JoinParams jp = {d.slab, (float*)(ws + p.acc_w) + v0 * p.ld, i > 0, done ? (char*)dw + v0 * channels * e : nullptr, vs, channels, p.ld, d.splits, scale, dev_status};
+          rc = join(jp, dtype, st);
+          if (rc != WCN_OK) return rc;
+        }
+        if (dbias) {
+          JoinParams jp = {d.slab_ones, (float*)(ws + p.acc_b) + v0, i > 0, done ? (char*)dbias + v0 * wcn_dtype_size(bias_dtype) : nullptr, vs, 1, 1, d.splits, scale, dev_status};
+          rc = join(jp, bias_dtype, st);
+          if (rc != WCN_OK) return rc;
+        }
+      }
+    }
+  }
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}

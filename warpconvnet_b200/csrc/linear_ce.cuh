@@ -1,0 +1,45 @@
+// What the kernels of the linear cross entropy (linear_ce.cu, linear_ce_tcgen05.cu) share.
+#pragma once
+#include "wcn_common.cuh"
+
+// What a gradient is multiplied by as it is finished: *g / *count * factor (0 where no row counts).
+struct wcn_ce_scale {
+  const float* g;
+  const int32_t* count;   // null: 1
+  float factor;
+};
+
+// The logits of a piece of rows x classes, as they are used: sums of exponentials (forward) or gradients (backward).
+struct wcn_ce_piece {
+  const void* x;            // first row of the piece
+  const void* w;            // first class
+  int64_t x_ld, w_ld;
+  int rows, classes, channels;
+  const float* bias2;       // bias / ln 2 from the first class on, -inf from the last class to a multiple of 256; null: none
+  // forward: [2 * splits][rows] of (largest, sum of 2^(z - largest)), z in units of ln 2
+  float2* part;
+  // backward
+  const float* lse2;        // of the piece's rows, in units of ln 2
+  const float* loss;
+  const int64_t* labels;
+  const float* row_scale;   // gradient of each row's loss (null: 1), divided by *row_max
+  const float* row_max;
+  int64_t ignore, first_class, all_classes;
+  void* g;                  // [rows][g_ld]
+  int64_t g_ld;
+};
+
+// D[m][n] = sum over k of A[m][k] B[k][n]: the sums of each split of k, or the finished result.
+struct wcn_ce_product {
+  const void* a;            // [k][m] (transposed) or [m][k]
+  const void* b;            // [k][n]
+  int64_t a_ld, b_ld;
+  int m, n, k;
+  int splits;
+  float* slab;              // [splits][m][n rounded up to 16]
+  float* slab_ones;         // [splits][m]: the sums of A alone; null: not wanted
+  void* out;                // [m][n]: written instead of the slab (one split)
+  wcn_ce_scale scale;
+};
+
+__host__ __device__ static inline int wcn_ce_round(int64_t v, int to) { return (int)((v + to - 1) / to * to); }

@@ -1,0 +1,618 @@
+// The matrix products of the linear cross entropy in 16 bits on the tensor cores.
+//
+// ce_logits_kernel computes tiles of 128 rows x up to 256 classes of z = x w^T + b and uses them as they leave tensor memory:
+//   forward   running (largest, sum of exponentials) of each row over the classes of a unit, one pair per half tile column;
+//   backward  g = (softmax - onehot) in 16 bits, a piece of the gradient of the logits, from the saved log-sum-exp.
+// ce_product_kernel multiplies such a piece by the weights (dX = g W) or by the rows (dW = g^T X).
+//
+// Logits are kept in units of ln 2, so that an exponential is one instruction.  Both kernels are persistent: one thread issues
+// TMA tile loads into a ring, one the matrix instructions, eight warps empty one of two accumulators while the other is filled.
+// Where they fit, the rows of a tile (up to 384 channels) or the classes (up to 256 of them) stay in shared memory and only the
+// other operand passes: a multiprocessor receives about 80 bytes a clock, and a tile whose operands both arrived anew would
+// wait for them (192 KB against 2 048 clocks of matrix instructions at 256 channels).
+//
+// Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix
+// instructions and frees its tensor memory; what was to come of it is then filled with NaN (linear_ce.cu).
+#include "linear_ce.cuh"
+#include "tcgen05_common.cuh"
+#include "tma_common.cuh"
+
+namespace {
+
+constexpr int TILE_M = 128, SLICE = 64;                   // rows of a tile; channels (elements of k) of a stage
+constexpr int A_BYTES = TILE_M * SLICE * 2;
+constexpr int MAX_STAGES = 12;
+constexpr int EPI_WARPS = 8, EPI_WARP0 = 2, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+constexpr int SMEM_BUDGET = 222 * 1024;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Ring {
+  int slot, phase, depth;
+  __device__ __forceinline__ void advance() {
+    if (++slot == depth) { slot = 0; phase ^= 1; }
+  }
+};
+
+struct Control {
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t res_full, res_empty;
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t done;
+  uint32_t tmem_holder;
+  int32_t skip;
+};
+
+__device__ __forceinline__ uint32_t bar(uint64_t* b) { return smem_u32(b); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Barriers, tensor memory and the look at the status word that both kernels begin with; false: an earlier launch gave up.
+__device__ __forceinline__ bool begin(Control* ctl, int stages, int tmem_cols, int32_t* dev_status) {
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) return false;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(bar(&ctl->full[s]), 1); mbar_init(bar(&ctl->empty[s]), 1); }
+    mbar_init(bar(&ctl->res_full), 1);
+    mbar_init(bar(&ctl->res_empty), 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), EPI_WARPS); }
+    mbar_init(bar(&ctl->done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return true;
+}
+
+// A producer that gave up: the copies it has issued land before the block's shared memory is given back.  (The ring stands
+// behind the last fill; fill i of a slot completes phase i & 1 of its barrier.)
+__device__ void drain_ring(Control* ctl, Ring r, int issued) {
+  for (int i = 0; i < issued && i < r.depth; ++i) {
+    if (--r.slot < 0) { r.slot = r.depth - 1; r.phase ^= 1; }
+    for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->full[r.slot]), (uint32_t)r.phase); ++k) {}
+  }
+}
+
+// ------------------------------------------------------------------ logits
+
+enum Resident { NOTHING = 0, ROWS = 1, CLASSES = 2 };
+
+struct LogitParams {
+  wcn_ce_piece q;
+  int KB;                 // slices of 64 channels
+  int NT;                 // classes of a tile
+  int m_tiles, n_tiles, splits, per, units, stages, tmem_cols;
+  float lift;             // exponent that gradients are raised by (fp16: see wcn_ce_lift)
+  int32_t* dev_status;
+};
+
+// A thread's row over the classes of a unit.
+struct RowSum { float top, sum; };
+
+template <int RES, bool GRAD, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ LogitParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int B_BYTES = p.NT * SLICE * 2;
+  const int stage_bytes = RES == ROWS ? B_BYTES : RES == CLASSES ? A_BYTES : A_BYTES + B_BYTES;
+  const int res_slice = RES == ROWS ? A_BYTES : B_BYTES;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t res = base + (uint32_t)(p.stages * stage_bytes);
+  Control* ctl = reinterpret_cast<Control*>(smem_raw + (base - smem_u32(smem_raw)) + p.stages * stage_bytes + (RES == NOTHING ? 0 : p.KB * res_slice));
+  if (!begin(ctl, p.stages, p.tmem_cols, p.dev_status)) return;
+  const uint32_t tmem = ctl->tmem_holder;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      Ring r{0, 0, p.stages};
+      int issued = 0, res_phase = 0;
+      bool have = false;
+      for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+        const int m = u % p.m_tiles, n0 = u / p.m_tiles * p.per, n1 = min(n0 + p.per, p.n_tiles);
+        if (RES == ROWS || (RES == CLASSES && !have)) {
+          if (!mbar_wait(bar(&ctl->res_empty), res_phase ^ 1, p.dev_status)) { ok = false; break; }
+          res_phase ^= 1;
+          have = true;
+          const uint32_t full = bar(&ctl->res_full);
+          mbar_expect_tx(full, (uint32_t)(p.KB * res_slice));
+          for (int s = 0; s < p.KB; ++s)
+            tma_load_2d(res + (uint32_t)(s * res_slice), RES == ROWS ? &x_map : &w_map, s * SLICE, RES == ROWS ? m * TILE_M : 0, full);
+        }
+        for (int n = n0; n < n1 && ok; ++n)
+          for (int s = 0; s < p.KB; ++s) {
+            if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
+            const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
+            mbar_expect_tx(full, (uint32_t)stage_bytes);
+            if (RES != ROWS) tma_load_2d(at, &x_map, s * SLICE, m * TILE_M, full);
+            if (RES != CLASSES) tma_load_2d(RES == NOTHING ? at + A_BYTES : at, &w_map, s * SLICE, n * p.NT, full);
+            r.advance();
+            ++issued;
+          }
+      }
+      if (!ok) {
+        drain_ring(ctl, r, issued);
+        for (int k = 0; have && k < 100000 && !mbar_try_wait(bar(&ctl->res_full), (uint32_t)(res_phase ^ 1)); ++k) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(p.NT >> 3) << 17) |
+                             ((uint32_t)(TILE_M >> 4) << 24);
+      Ring r{0, 0, p.stages};
+      int ab = 0, aphase = 0, res_phase = 0;
+      bool have = false;
+      const uint64_t ring0 = smem_desc<128>(base), res0 = smem_desc<128>(res);
+      for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+        const int n0 = u / p.m_tiles * p.per, n1 = min(n0 + p.per, p.n_tiles);
+        if (RES == ROWS || (RES == CLASSES && !have)) {
+          if (!mbar_wait(bar(&ctl->res_full), res_phase, p.dev_status)) { ok = false; break; }
+          res_phase ^= 1;
+          have = true;
+        }
+        for (int n = n0; n < n1 && ok; ++n) {
+          if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(ab * p.NT);
+          for (int s = 0; s < p.KB; ++s) {
+            if (!mbar_wait(bar(&ctl->full[r.slot]), r.phase, p.dev_status)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t ring = ring0 + (uint64_t)((r.slot * stage_bytes) >> 4), kept = res0 + (uint64_t)((s * res_slice) >> 4);
+            const uint64_t a = RES == ROWS ? kept : ring, b = RES == CLASSES ? kept : RES == NOTHING ? ring + (A_BYTES >> 4) : ring;
+#pragma unroll
+            for (int k = 0; k < SLICE / 16; ++k) umma_f16(d, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc, (s | k) ? 1u : 0u);
+            umma_commit(bar(&ctl->empty[r.slot]));
+            r.advance();
+          }
+          if (!ok) break;
+          umma_commit(bar(&ctl->acc_full[ab]));
+          if (++ab == 2) { ab = 0; aphase ^= 1; }
+        }
+        if (RES == ROWS) umma_commit(bar(&ctl->res_empty));
+      }
+      umma_commit(bar(&ctl->done));
+      (void)mbar_wait(bar(&ctl->done), 0, p.dev_status);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
+    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;   // of 16 columns
+    int ab = 0, aphase = 0;
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
+      const int m = u % p.m_tiles, split = u / p.m_tiles, n0 = split * p.per, n1 = min(n0 + p.per, p.n_tiles);
+      const int row = m * TILE_M + quarter * 32 + lane;
+      const bool live = row < p.q.rows;
+      float top = -INFINITY, sum = 0.f;                  // forward
+      float minus = -INFINITY, scale = 1.f;              // backward: exponent of the row, gradient of its loss
+      int label = -1;
+      if (GRAD && live) {
+        const int64_t y = __ldg(&p.q.labels[row]);
+        if (y != p.q.ignore && y >= 0 && y < p.q.all_classes) {
+          minus = p.lift - __ldg(&p.q.lse2[row]);
+          const int64_t in = y - p.q.first_class;
+          label = in >= 0 && in < p.q.classes ? (int)in : -1;
+          if (p.q.row_scale) {
+            const float most = __ldg(p.q.row_max);
+            scale = most > 0.f ? __ldg(&p.q.row_scale[row]) / most : most == most ? 0.f : most;
+          }
+        }
+      }
+      for (int n = n0; n < n1; ++n) {
+        if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
+        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.NT);
+        const int col0 = n * p.NT;
+        auto use = [&](auto& r, int c) {   // columns c .. of the tile
+          constexpr int W = sizeof(r) / 4;
+          __syncwarp();
+          tmem_load(t + (uint32_t)c, r);
+          tmem_ld_wait();
+          float z[W];
+          const int col = col0 + c;
+          if (p.q.bias2) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+              const float4 b = __ldg(reinterpret_cast<const float4*>(p.q.bias2 + col + i));
+              z[i] = fmaf(__uint_as_float(r[i]), LOG2E, b.x);
+              z[i + 1] = fmaf(__uint_as_float(r[i + 1]), LOG2E, b.y);
+              z[i + 2] = fmaf(__uint_as_float(r[i + 2]), LOG2E, b.z);
+              z[i + 3] = fmaf(__uint_as_float(r[i + 3]), LOG2E, b.w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) z[i] = __uint_as_float(r[i]) * LOG2E;
+            if (col + W > p.q.classes) {
+#pragma unroll
+              for (int i = 0; i < W; ++i)
+                if (col + i >= p.q.classes) z[i] = -INFINITY;
+            }
+          }
+          if (!GRAD) {
+            float m8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m8[i] = z[i];
+#pragma unroll
+            for (int i = 8; i < W; ++i) m8[i & 7] = fmaxf(m8[i & 7], z[i]);
+#pragma unroll
+            for (int o = 4; o; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < o; ++i) m8[i] = fmaxf(m8[i], m8[i + o]);
+            const float now = fmaxf(top, m8[0]), by = now == -INFINITY ? 0.f : now;   // (a row of -inf so far: sums of zeros)
+            float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < W; ++i) s4[i & 3] += exp2_fast(z[i] - by);
+            sum = fmaf(sum, exp2_fast(top - by), (s4[0] + s4[1]) + (s4[2] + s4[3]));
+            top = now;
+          } else {
+            uint32_t out[W / 2];
+#pragma unroll
+            for (int i = 0; i < W; i += 2) {
+              float a = exp2_fast(z[i] + minus), b = exp2_fast(z[i + 1] + minus);
+              if (p.q.row_scale) { a *= scale; b *= scale; }
+              out[i / 2] = minus == -INFINITY ? 0u : pack2<BF16>(a, b);   // (a row that does not count, whatever is in it)
+            }
+            uint16_t* const g = reinterpret_cast<uint16_t*>(p.q.g) + (int64_t)row * p.q.g_ld + col;
+#pragma unroll
+            for (int i = 0; i < W / 16; ++i)
+              if (live && col + 16 * i < p.q.g_ld) st_global_32B(g + 16 * i, out + 8 * i);
+            const int in = label - col;
+            if (in >= 0 && in < W) {
+              // softmax - 1 at the label's class, from the row's loss: no difference of nearly equal numbers
+              const float d = expm1f(-__ldg(&p.q.loss[row])) * scale * exp2f(p.lift);
+              const uint32_t v = pack2<BF16>(d, d);
+              g[in] = (uint16_t)v;
+            }
+          }
+        };
+        int c = first;
+        for (; c + 2 <= last; c += 2) { uint32_t r[32]; use(r, c * 16); }
+        if (c < last) { uint32_t r[16]; use(r, c * 16); }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[ab]));
+        if (++ab == 2) { ab = 0; aphase ^= 1; }
+      }
+      if (!ok) break;
+      if (!GRAD && live) p.q.part[(int64_t)(split * 2 + half) * p.q.rows + row] = make_float2(top, sum);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+}
+
+// ------------------------------------------------------------------ products
+
+struct ProductParams {
+  wcn_ce_product q;
+  int NT, NB;             // columns of a tile, chunks of 64 of them
+  int m_tiles, n_tiles, units, ksteps, per, stages, accs, stride, tmem_cols;
+  int vec;                // rows of `out` start on 32-byte boundaries
+  int32_t* dev_status;
+};
+
+template <bool TRANS, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ ProductParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int CHUNK = SLICE * 128;                      // 64 rows of k x 64 columns
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stage_bytes = A_BYTES + p.NB * CHUNK;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ones = base + (uint32_t)(p.stages * stage_bytes);
+  uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw)) + p.stages * stage_bytes;
+  Control* ctl = reinterpret_cast<Control*>(gen + CHUNK);
+  const bool with_ones = p.q.slab_ones != nullptr;
+  auto split_of = [&](int u) { return u / (p.m_tiles * p.n_tiles); };
+  auto m_of = [&](int u) { return u / p.n_tiles % p.m_tiles; };
+  auto n_of = [&](int u) { return u % p.n_tiles; };
+  auto mark = [&]() {   // the finished result of this block's units, where it has none
+    if (!p.q.out) return;
+    const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x)
+      for (int i = threadIdx.x; i < TILE_M * p.NT; i += THREADS) {
+        const int row = m_of(u) * TILE_M + i / p.NT, col = n_of(u) * p.NT + i % p.NT;
+        if (row < p.q.m && col < p.q.n) reinterpret_cast<uint16_t*>(p.q.out)[(int64_t)row * p.q.n + col] = nan;
+      }
+  };
+  if (with_ones) {   // a chunk of ones: the sums of A's rows are another 16 columns of the product
+    const uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u;
+    for (int i = threadIdx.x; i < CHUNK / 4; i += THREADS) reinterpret_cast<uint32_t*>(gen)[i] = one;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (!begin(ctl, p.stages, p.tmem_cols, p.dev_status)) { mark(); return; }
+  const uint32_t tmem = ctl->tmem_holder;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      Ring r{0, 0, p.stages};
+      int issued = 0;
+      for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+        const int m = m_of(u) * TILE_M, n = n_of(u) * p.NT, k0 = split_of(u) * p.per, k1 = min(k0 + p.per, p.ksteps);
+        for (int k = k0; k < k1; ++k) {
+          if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
+          const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
+          mbar_expect_tx(full, (uint32_t)stage_bytes);
+          if (TRANS) {
+            tma_load_2d(at, &a_map, m, k * SLICE, full);
+            tma_load_2d(at + CHUNK, &a_map, m + 64, k * SLICE, full);
+          } else {
+            tma_load_2d(at, &a_map, k * SLICE, m, full);
+          }
+          for (int c = 0; c < p.NB; ++c) tma_load_2d(at + A_BYTES + (uint32_t)(c * CHUNK), &b_map, n + 64 * c, k * SLICE, full);
+          r.advance();
+          ++issued;
+        }
+      }
+      if (!ok) drain_ring(ctl, r, issued);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t flags = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | (TRANS ? 1u << 15 : 0u) | (1u << 16) |
+                             ((uint32_t)(TILE_M >> 4) << 24);
+      const uint32_t idesc = flags | ((uint32_t)(p.NT >> 3) << 17), idesc_ones = flags | ((uint32_t)(16 >> 3) << 17);
+      const uint64_t a0 = TRANS ? smem_desc_mn<128>(base, CHUNK) : smem_desc<128>(base), b0 = smem_desc_mn<128>(base + A_BYTES, CHUNK);
+      const uint64_t ones0 = smem_desc_mn<128>(ones, CHUNK);
+      constexpr int A_STEP = TRANS ? 128 : 2;             // 16 of k further, in units of 16 bytes
+      Ring r{0, 0, p.stages};
+      int ab = 0, aphase = 0;
+      for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+        const int k0 = split_of(u) * p.per, k1 = min(k0 + p.per, p.ksteps);
+        const bool sums = with_ones && n_of(u) == 0;
+        if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(ab * p.stride);
+        for (int k = k0; k < k1; ++k) {
+          if (!mbar_wait(bar(&ctl->full[r.slot]), r.phase, p.dev_status)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t at = (uint64_t)((r.slot * stage_bytes) >> 4);
+#pragma unroll
+          for (int i = 0; i < SLICE / 16; ++i)
+            umma_f16(d, a0 + at + (uint64_t)(i * A_STEP), b0 + at + (uint64_t)(i * 128), idesc, (k > k0 || i) ? 1u : 0u);
+          if (sums)
+#pragma unroll
+            for (int i = 0; i < SLICE / 16; ++i)
+              umma_f16(d + (uint32_t)p.NT, a0 + at + (uint64_t)(i * A_STEP), ones0 + (uint64_t)(i * 128), idesc_ones, (k > k0 || i) ? 1u : 0u);
+          umma_commit(bar(&ctl->empty[r.slot]));
+          r.advance();
+        }
+        if (!ok) break;
+        umma_commit(bar(&ctl->acc_full[ab]));
+        if (++ab == p.accs) { ab = 0; aphase ^= 1; }
+      }
+      umma_commit(bar(&ctl->done));
+      (void)mbar_wait(bar(&ctl->done), 0, p.dev_status);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
+    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;
+    const int64_t slab_ld = wcn_ce_round(p.q.n, 16);
+    float scale = 0.f;
+    if (p.q.out) {
+      const int count = p.q.scale.count ? *p.q.scale.count : 1;
+      scale = count ? *p.q.scale.g / (float)count * p.q.scale.factor : 0.f;
+    }
+    int ab = 0, aphase = 0;
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
+      if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      const int row = m_of(u) * TILE_M + quarter * 32 + lane, n = n_of(u) * p.NT, split = split_of(u);
+      const bool live = row < p.q.m;
+      const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.stride);
+      float* const slab = p.q.slab + ((int64_t)split * p.q.m + row) * slab_ld + n;
+      uint16_t* const out = reinterpret_cast<uint16_t*>(p.q.out) + (int64_t)row * p.q.n + n;
+      for (int c = first; c < last; ++c) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld16(t + (uint32_t)(c * 16), r);
+        tmem_ld_wait();
+        if (!live) continue;
+        if (p.q.out) {
+          uint32_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = pack2<BF16>(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
+          if (p.vec && n + c * 16 + 16 <= p.q.n) {
+            st_global_32B(out + c * 16, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n + c * 16 + i < p.q.n) out[c * 16 + i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+          }
+        } else if (n + c * 16 < slab_ld) {
+          st_global_32B(slab + c * 16, r);
+          st_global_32B(slab + c * 16 + 8, r + 8);
+        }
+      }
+      if (with_ones && n == 0 && half) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld16(t + (uint32_t)p.NT, r);
+        tmem_ld_wait();
+        if (live) p.q.slab_ones[(int64_t)split * p.q.m + row] = __uint_as_float(r[0]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[ab]));
+      if (++ab == p.accs) { ab = 0; aphase ^= 1; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) mark();
+}
+
+template <auto KERNEL> bool allow_smem() {
+  static bool configured[64] = {};   // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    configured[dev] = true;
+  }
+  return true;
+}
+
+int columns_pow2(int cols) {
+  int v = 32;
+  while (v < cols) v <<= 1;
+  return v;
+}
+
+// Classes of a tile and how many tiles of a row of them make a unit.
+void plan_logits(int rows, int classes, LogitParams* p) {
+  p->m_tiles = (rows + TILE_M - 1) / TILE_M;
+  p->n_tiles = (classes + 255) / 256;
+  p->NT = p->n_tiles <= 4 ? wcn_ce_round((classes + p->n_tiles - 1) / p->n_tiles, 16) : 256;
+  // As few rounds of the grid as there can be, counted in tiles; a unit costs the loads of its rows, about a tile.
+  const int sms = wcn_num_sms();
+  int64_t best = INT64_MAX;
+  for (int per = p->n_tiles; per >= 1; --per) {
+    const int splits = (p->n_tiles + per - 1) / per;
+    if (splits > 64) break;
+    const int64_t rounds = ((int64_t)p->m_tiles * splits + sms - 1) / sms, cost = rounds * (per + 1);
+    if (cost < best) { best = cost; p->per = per; p->splits = splits; }
+  }
+  p->units = p->m_tiles * p->splits;
+}
+
+template <int RES, bool GRAD, bool BF16>
+int launch_logits(LogitParams& p, size_t fixed, cudaStream_t st) {
+  const int b_bytes = p.NT * SLICE * 2;
+  const int stage = RES == ROWS ? b_bytes : RES == CLASSES ? A_BYTES : A_BYTES + b_bytes;
+  const size_t kept = RES == NOTHING ? 0 : (size_t)p.KB * (RES == ROWS ? A_BYTES : b_bytes);
+  p.stages = (int)((SMEM_BUDGET - fixed - kept) / stage);
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  p.tmem_cols = columns_pow2(2 * p.NT);
+  CUtensorMap xm, wm;
+  if (!matrix_map(&xm, p.q.x, p.q.rows, p.q.channels, p.q.x_ld * 2, TILE_M, BF16) ||
+      !matrix_map(&wm, p.q.w, p.q.classes, p.q.channels, p.q.w_ld * 2, p.NT, BF16))
+    return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = ce_logits_kernel<RES, GRAD, BF16>;
+  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
+  const int sms = wcn_num_sms();
+  kern<<<p.units < sms ? p.units : sms, THREADS, fixed + kept + (size_t)p.stages * stage, st>>>(xm, wm, p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+template <bool GRAD, bool BF16> int by_resident(LogitParams& p, cudaStream_t st) {
+  const size_t fixed = sizeof(Control) + 1024 + 128;
+  const int64_t b_bytes = (int64_t)p.NT * SLICE * 2;
+  if (p.n_tiles == 1 && p.KB * b_bytes + 4 * A_BYTES + (int64_t)fixed <= SMEM_BUDGET) return launch_logits<CLASSES, GRAD, BF16>(p, fixed, st);
+  if (p.KB * (int64_t)A_BYTES + 3 * b_bytes + (int64_t)fixed <= SMEM_BUDGET) return launch_logits<ROWS, GRAD, BF16>(p, fixed, st);
+  return launch_logits<NOTHING, GRAD, BF16>(p, fixed, st);
+}
+
+template <bool TRANS, bool BF16>
+int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st) {
+  ProductParams p = {};
+  p.q = q;
+  p.dev_status = dev_status;
+  const int most = q.slab_ones ? 240 : 256;
+  p.n_tiles = (q.n + most - 1) / most;
+  p.NT = wcn_ce_round((q.n + p.n_tiles - 1) / p.n_tiles, 16);
+  p.NB = (p.NT + 63) / 64;
+  p.m_tiles = (q.m + TILE_M - 1) / TILE_M;
+  p.ksteps = (q.k + SLICE - 1) / SLICE;
+  p.per = (p.ksteps + q.splits - 1) / q.splits;
+  if ((p.ksteps + p.per - 1) / p.per != q.splits) return WCN_ERR_INVALID_PARAMETERS;
+  p.units = p.m_tiles * p.n_tiles * q.splits;
+  p.stride = p.NT + (q.slab_ones ? 16 : 0);
+  p.accs = 2 * p.stride <= 512 ? 2 : 1;
+  p.tmem_cols = columns_pow2(p.accs * p.stride);
+  p.vec = q.out && reinterpret_cast<uintptr_t>(q.out) % 32 == 0 && (q.n * 2) % 32 == 0;
+  const size_t fixed = sizeof(Control) + 1024 + 128 + SLICE * 128;
+  const int stage = A_BYTES + p.NB * SLICE * 128;
+  p.stages = (int)((SMEM_BUDGET - fixed) / stage);
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  CUtensorMap am, bm;
+  if (!matrix_map(&am, q.a, TRANS ? q.k : q.m, TRANS ? q.m : q.k, q.a_ld * 2, TRANS ? SLICE : TILE_M, BF16) ||
+      !matrix_map(&bm, q.b, q.k, q.n, q.b_ld * 2, SLICE, BF16))
+    return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = ce_product_kernel<TRANS, BF16>;
+  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
+  const int sms = wcn_num_sms();
+  kern<<<p.units < sms ? p.units : sms, THREADS, fixed + (size_t)p.stages * stage, st>>>(am, bm, p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+}  // namespace
+
+int wcn_ce_logits_splits(int rows, int classes) {
+  LogitParams p = {};
+  plan_logits(rows, classes, &p);
+  return p.splits;
+}
+
+int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st) {
+  LogitParams p = {};
+  p.q = q;
+  p.lift = lift;
+  p.dev_status = dev_status;
+  p.KB = (q.channels + SLICE - 1) / SLICE;
+  plan_logits(q.rows, q.classes, &p);
+  if (dtype == WCN_BF16) return gradient ? by_resident<true, true>(p, st) : by_resident<false, true>(p, st);
+  return gradient ? by_resident<true, false>(p, st) : by_resident<false, false>(p, st);
+}
+
+// Splits of k with which the product's tiles keep every multiprocessor busy.
+int wcn_ce_product_splits(int m, int n, int k) {
+  const int tiles = ((m + TILE_M - 1) / TILE_M) * ((n + 239) / 240), ksteps = (k + SLICE - 1) / SLICE, sms = wcn_num_sms();
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= sms && s <= ksteps; ++s) {
+    const int per = (ksteps + s - 1) / s;
+    if ((ksteps + per - 1) / per != s) continue;
+    // rounds of the grid in steps of k, a unit's start and its sums' way out and back counted as some more
+    const double cost = (double)((tiles * (int64_t)s + sms - 1) / sms) * (per + 6) + 0.02 * tiles * s;
+    if (cost < least) { least = cost; best = s; }
+  }
+  return best;
+}
+
+int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, int dtype, int32_t* dev_status, cudaStream_t st) {
+  if (dtype == WCN_BF16) return transposed ? launch_product<true, true>(q, dev_status, st) : launch_product<false, true>(q, dev_status, st);
+  return transposed ? launch_product<true, false>(q, dev_status, st) : launch_product<false, false>(q, dev_status, st);
+}
