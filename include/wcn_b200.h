@@ -642,7 +642,7 @@ typedef struct {
 } wcn_adamw_tensor;
 
 /* One decoupled-weight-decay Adam step of all tensors (a host array, read during the call), in fp32.  exp_avg / exp_avg_sq hold
- * the moments of all tensors, 16-byte aligned: fp32, or with the two base arrays (one int16 per 256 elements) 8-bit codes: the
+ * the moments of all tensors, 32-byte aligned: fp32, or with the two base arrays (one int16 per 256 elements) 8-bit codes: the
  * code k > 0 stands for the fp32 number with the bits (k + base) << 20, 0 for zero; exp_avg has a sign in its top bit.  Codes
  * are rounded at random with a hash of step and place; the elements behind a tensor's end must be zero codes and stay so.
  * steps (device): the steps made before this one, advanced by it.  lr_bits .. weight_decay_bits: the bits of doubles; lr (a

@@ -6,6 +6,7 @@ PyTorch is used for device memory and streams only.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import importlib.util
@@ -237,6 +238,11 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(idx)
 
 
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: launches are made for that (costs a comparison where it is already)."""
+    return _HERE_ALREADY if device.index is None or device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
 def small_to_device(t: torch.Tensor, device, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """A small host tensor (batch offsets, a few sizes) on ``device`` WITHOUT synchronising the
     stream: staged through pinned memory and copied asynchronously.  (A plain ``.to(device)`` of
@@ -260,6 +266,7 @@ def require_cuda(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
 
 
+_HERE_ALREADY = contextlib.nullcontext()
 _status_words = {}
 
 

@@ -56,30 +56,46 @@ struct Hyper {
   float lr, wd, eps, b1, b1c, b2, b2c, log_b1, log_b2;
 };
 
+// Eight elements of a lane; fp32 ones in one request of 32 bytes (two of 16 touch every line twice).
 template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, bool vec, float (&x)[8]) {
   if (vec && left >= 8) {
-    __align__(16) T v[8];
+    __align__(32) T v[8];
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "l"(p));
+    } else {
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = wcn_to_float<T>(v[i]);
+      for (int i = 0; i < 8; ++i) x[i] = wcn_to_float<T>(v[i]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = i < left ? wcn_to_float<T>(p[i]) : 0.f;
   }
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, int64_t left, bool vec, const float (&x)[8]) {
-  __align__(16) T v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = wcn_from_float<T>(x[i]);
   if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]),
+                   "f"(x[5]), "f"(x[6]), "f"(x[7]) : "memory");
+    } else {
+      __align__(16) T v[8];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+      for (int i = 0; i < 8; ++i) v[i] = wcn_from_float<T>(x[i]);
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < left) p[i] = v[i];
+      if (i < left) p[i] = wcn_from_float<T>(x[i]);
   }
+}
+
+// (one part in 2^22 of an update)
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ float code_value(uint32_t k, uint32_t base) { return k ? __uint_as_float((k + base) << 20) : 0.f; }
@@ -125,7 +141,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
   const int64_t s = t.slot + e;
   P* const param = reinterpret_cast<P*>(t.param) + e;
   const G* const grad = reinterpret_cast<const G*>(t.grad) + e;
-  const bool pvec = (reinterpret_cast<uintptr_t>(t.param) & 15) == 0, gvec = (reinterpret_cast<uintptr_t>(t.grad) & 15) == 0;
+  const bool pvec = reinterpret_cast<uintptr_t>(t.param) % (8 * sizeof(P)) == 0, gvec = reinterpret_cast<uintptr_t>(t.grad) % (8 * sizeof(G)) == 0;
 
   float p[8], g[8], m[8], v[8];
   if (mine) {
@@ -171,7 +187,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     const float d = h.grad_scale ? g[i] * inv : g[i];
     m[i] = __fadd_rn(__fmul_rn(m[i], h.b1), __fmul_rn(d, h.b1c));
     v[i] = __fadd_rn(__fmul_rn(v[i], h.b2), __fmul_rn(__fmul_rn(d, d), h.b2c));
-    p[i] = p[i] * keep - size * __fdividef(m[i], fmaf(sqrtf(v[i]), root, h.eps));
+    p[i] = p[i] * keep - size * __fdividef(m[i], fmaf(sqrt_fast(v[i]), root, h.eps));
     m_top = max(m_top, __float_as_uint(m[i]) & 0x7FFFFFFFu);
     v_top = max(v_top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
   }
@@ -264,7 +280,7 @@ int by_param(int dtype, int grad_dtype, const wcn_adamw_tensor* t, int64_t count
   return by_grad<__nv_bfloat16, EIGHT>(grad_dtype, t, count, h, st);
 }
 
-bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool on32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 double number(int64_t bits) {
   double d;
@@ -279,7 +295,7 @@ extern "C" int wcn_adamw_step(const wcn_adamw_tensor* tensors, int64_t count, in
                               int64_t beta1_bits, int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits,
                               const float* lr, const float* grad_scale, const float* found_inf, uint32_t* counter, void* stream) {
   if (count < 0 || (count && (!tensors || !exp_avg || !exp_avg_sq || !steps || !counter)) || dtype < WCN_F32 || dtype > WCN_BF16 ||
-      grad_dtype < WCN_F32 || grad_dtype > WCN_BF16 || !on16(exp_avg) || !on16(exp_avg_sq) || !exp_avg_base != !exp_avg_sq_base)
+      grad_dtype < WCN_F32 || grad_dtype > WCN_BF16 || !on32(exp_avg) || !on32(exp_avg_sq) || !exp_avg_base != !exp_avg_sq_base)
     return WCN_ERR_INVALID_PARAMETERS;
   const double b1 = number(beta1_bits), b2 = number(beta2_bits);
   if (!(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1)) return WCN_ERR_INVALID_PARAMETERS;
@@ -302,8 +318,8 @@ extern "C" int wcn_adamw_decode(const void* exp_avg, const int16_t* exp_avg_base
                                 const int16_t* exp_avg_sq_base, int64_t n, float* exp_avg_out, float* exp_avg_sq_out, void* stream) {
   if (n < 0 || n % CODES || n / CODES > 0x7FFFFFFFll) return WCN_ERR_INVALID_PARAMETERS;
   if (!n) return WCN_OK;
-  if (!exp_avg || !exp_avg_sq || !exp_avg_base || !exp_avg_sq_base || !exp_avg_out || !exp_avg_sq_out || !on16(exp_avg) ||
-      !on16(exp_avg_sq) || !on16(exp_avg_out) || !on16(exp_avg_sq_out))
+  if (!exp_avg || !exp_avg_sq || !exp_avg_base || !exp_avg_sq_base || !exp_avg_out || !exp_avg_sq_out || !on32(exp_avg) ||
+      !on32(exp_avg_sq) || !on32(exp_avg_out) || !on32(exp_avg_sq_out))
     return WCN_ERR_INVALID_PARAMETERS;
   const int64_t blocks = (n + THREADS * 8 - 1) / (THREADS * 8);
   decode_moments_kernel<<<(unsigned)blocks, THREADS, 0, wcn_stream(stream)>>>((const uint8_t*)exp_avg, exp_avg_base, (const uint8_t*)exp_avg_sq,

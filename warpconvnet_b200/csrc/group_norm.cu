@@ -18,18 +18,18 @@
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512;
 constexpr int ROWS = 8;                          // rows of a thread at a time
-constexpr int FEW = 24, MANY = 1000;             // scenes of a launch: 0.3 and 12 KB of parameters
+constexpr int SCENES = 250;                      // of a launch: 2 KB of parameters
 constexpr int MAX_C = 4096;
 constexpr int64_t GROUP_BYTES = 48ll << 20;
 
 enum Act { NONE = 0, RELU = 1, SILU = 2, GELU = 3 };
 
-template <int M> struct Scenes {
+struct Scenes {
   int count;
-  int row0[M + 1];    // first row, from the launch's first row on
-  int tile0[M + 1];   // first tile
+  int row0[SCENES + 1];    // first row, from the launch's first row on
+  int tile0[SCENES + 1];   // first tile
 };
 
 struct Params {
@@ -80,8 +80,8 @@ template <int ACT> __device__ __forceinline__ float through(float dy, float z) {
 }
 
 // The scene and the rows of a block's tile.
-struct Tile { int scene, lo, hi, first, last; };   // first, last + 1: tiles of the scene
-template <int M> __device__ __forceinline__ Tile find_tile(const Scenes<M>& s, int rows) {
+struct Tile { int scene, lo, hi, first, last; };   // first, last: tiles of the scene
+__device__ __forceinline__ Tile find_tile(const Scenes& s, int rows) {
   int at = 0;
   for (int hi = s.count; hi - at > 1;) {
     const int mid = (at + hi) / 2;
@@ -105,8 +105,31 @@ struct Place {
   }
 };
 
-template <typename T, int V, int M>
-__global__ void __launch_bounds__(THREADS) group_stats_kernel(const __grid_constant__ Scenes<M> scenes, const __grid_constant__ Params p) {
+// Sums of a value over the rows' threads, for each of the W channels side by side: as many neighbouring threads a channel as there
+// are, V values each.  f(channel, y0, step, sum) is called by all threads that share a channel (y0, y0 + step, .. are theirs;
+// sum adds over them), last with the threads of channels beyond W.
+template <typename F> __device__ __forceinline__ void per_channel(int W, F&& f) {
+  int share = 1;
+  while (share < 32 && share * 2 * W <= THREADS) share *= 2;
+  for (int c0 = 0; c0 < W; c0 += THREADS / share) f(c0 + (int)threadIdx.x / share, (int)threadIdx.x % share, share);
+}
+__device__ __forceinline__ float sum_over(float v, int share) {
+  for (int o = share >> 1; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ double sum_over(double v, int share) {
+  for (int o = share >> 1; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+// f(group, lane, lanes) by as many neighbouring threads a group as there are, at most a warp.
+template <typename F> __device__ __forceinline__ void per_group(int G, F&& f) {
+  int width = 32;
+  while (width > 1 && width * G > THREADS) width >>= 1;
+  for (int g0 = 0; g0 < G; g0 += THREADS / width) f(g0 + (int)threadIdx.x / width, (int)threadIdx.x % width, width);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS, 2) group_stats_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float smem[];
   const Place at(p.C, V);
   const int W = at.txs * V;                       // channels side by side
@@ -115,41 +138,44 @@ __global__ void __launch_bounds__(THREADS) group_stats_kernel(const __grid_const
   float* const c_mean = s_m2 + at.tys * W;        // [C]
   float* const c_m2 = c_mean + p.C;               // [C]
   const Tile t = find_tile(scenes, p.rows);
-  const int n_tile = t.hi - t.lo;
+  const int n_tile = t.hi - t.lo, n_each = n_tile / at.tys, n_more = n_tile % at.tys;   // rows of a thread: one more for the first
   const T* const x = reinterpret_cast<const T*>(p.x);
   for (int pc = at.tx; pc - at.tx < at.pieces; pc += at.txs) {
-    const bool live = at.ty < at.tys && pc < at.pieces;
-    float mean[V], m2[V];
+    if (at.ty < at.tys && pc < at.pieces) {
+      float mean[V], m2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
-    if (live) {
+      for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
+      const int64_t step = (int64_t)at.tys * p.x_ld;
+      const T* from = x + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
       int n = 0;
-      for (int r = t.lo + at.ty; r < t.hi; r += ROWS * at.tys) {
+      const int mine = n_each + (at.ty < n_more);
+      for (; n + ROWS <= mine; n += ROWS, from += ROWS * step) {
         Piece<T, V> q[ROWS];
-        int k = 0;
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-          if (r + u * at.tys < t.hi) {
-            q[u] = load_piece<T, V>(x + (int64_t)(r + u * at.tys) * p.x_ld + pc * V);
-            k = u + 1;
-          }
-        const float inv = 1.f / (float)k, share = (float)k / (float)(n + k);
+        for (int u = 0; u < ROWS; ++u) q[u] = load_piece<T, V>(from + u * step);
+        const float share = (float)ROWS / (float)(n + ROWS), both = share * (float)n;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float sum = 0.f, d2 = 0.f;
+          float f[ROWS], sum = 0.f, d2 = 0.f;
 #pragma unroll
-          for (int u = 0; u < ROWS; ++u) sum += u < k ? wcn_to_float<T>(q[u].v[i]) : 0.f;
-          const float mb = sum * inv;
+          for (int u = 0; u < ROWS; ++u) { f[u] = wcn_to_float<T>(q[u].v[i]); sum += f[u]; }
+          const float mb = sum * (1.f / ROWS);
 #pragma unroll
-          for (int u = 0; u < ROWS; ++u) {
-            const float d = u < k ? wcn_to_float<T>(q[u].v[i]) - mb : 0.f;
-            d2 = fmaf(d, d, d2);
-          }
+          for (int u = 0; u < ROWS; ++u) { const float d = f[u] - mb; d2 = fmaf(d, d, d2); }
           const float delta = mb - mean[i];
           mean[i] = fmaf(delta, share, mean[i]);
-          m2[i] += d2 + delta * delta * (share * (float)n);
+          m2[i] += fmaf(delta * delta, both, d2);
         }
-        n += k;
+      }
+      for (; n < mine; ++n, from += step) {       // the last rows one by one
+        const Piece<T, V> q = load_piece<T, V>(from);
+        const float share = 1.f / (float)(n + 1), both = share * (float)n;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float delta = wcn_to_float<T>(q.v[i]) - mean[i];
+          mean[i] = fmaf(delta, share, mean[i]);
+          m2[i] = fmaf(delta * delta, both, m2[i]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -159,51 +185,43 @@ __global__ void __launch_bounds__(THREADS) group_stats_kernel(const __grid_const
     }
     __syncthreads();
     const int c0 = (pc - at.tx) * V;
-    for (int c = threadIdx.x; c < W && c0 + c < p.C; c += THREADS) {
-      float sum = 0.f, m2c = 0.f;
-      // rows ty, ty + tys, ... of the tile
-      for (int y = 0; y < at.tys; ++y) sum = fmaf(s_mean[y * W + c], (float)((n_tile - y + at.tys - 1) / at.tys), sum);
-      const float m = sum / (float)n_tile;
-      for (int y = 0; y < at.tys; ++y) {
-        const float d = s_mean[y * W + c] - m;
-        m2c += s_m2[y * W + c] + d * d * (float)((n_tile - y + at.tys - 1) / at.tys);
+    per_channel(W, [&](int c, int y0, int share) {
+      const bool live = c < W && c0 + c < p.C;
+      float sum = 0.f, m2 = 0.f;
+      if (live)
+        for (int y = y0; y < at.tys; y += share) sum = fmaf(s_mean[y * W + c], (float)(n_each + (y < n_more)), sum);
+      const float m = sum_over(sum, share) / (float)n_tile;
+      if (live)
+        for (int y = y0; y < at.tys; y += share) {
+          const float d = s_mean[y * W + c] - m;
+          m2 += fmaf(d * d, (float)(n_each + (y < n_more)), s_m2[y * W + c]);
+        }
+      m2 = sum_over(m2, share);
+      if (live && y0 == 0) {
+        c_mean[c0 + c] = m;
+        c_m2[c0 + c] = m2;
       }
-      c_mean[c0 + c] = m;
-      c_m2[c0 + c] = m2c;
-    }
+    });
     __syncthreads();
   }
-  // a warp puts the channels of a group together
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int g = warp; g < p.G; g += THREADS / 32) {
-    float sum = 0.f, m2g = 0.f;
-    for (int c = lane; c < p.per; c += 32) sum += c_mean[g * p.per + c];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const float m = sum / (float)p.per;
-    for (int c = lane; c < p.per; c += 32) {
-      const float d = c_mean[g * p.per + c] - m;
-      m2g += c_m2[g * p.per + c] + d * d * (float)n_tile;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m2g += __shfl_xor_sync(0xFFFFFFFFu, m2g, o);
-    if (lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(m, m2g);
-  }
+  per_group(p.G, [&](int g, int lane, int width) {
+    float sum = 0.f, m2 = 0.f;
+    if (g < p.G)
+      for (int c = lane; c < p.per; c += width) sum += c_mean[g * p.per + c];
+    const float m = sum_over(sum, width) / (float)p.per;
+    if (g < p.G)
+      for (int c = lane; c < p.per; c += width) {
+        const float d = c_mean[g * p.per + c] - m;
+        m2 += fmaf(d * d, (float)n_tile, c_m2[g * p.per + c]);
+      }
+    m2 = sum_over(m2, width);
+    if (g < p.G && lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(m, m2);
+  });
 }
 
-// What each group's tiles come to together, by as many threads a group as there are, lanes of one warp.
-template <typename F> __device__ __forceinline__ void per_group(int G, F&& f) {
-  int width = 32;
-  while (width > 1 && width * G > THREADS) width >>= 1;
-  for (int g0 = 0; g0 < G; g0 += THREADS / width) f(g0 + (int)threadIdx.x / width, (int)threadIdx.x % width, width);
-}
-__device__ __forceinline__ double sum_over(double v, int width) {
-  for (int o = width >> 1; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-
-template <typename T, int V, int ACT, int M>
-__global__ void __launch_bounds__(THREADS) group_apply_kernel(const __grid_constant__ Scenes<M> scenes, const __grid_constant__ Params p) {
+// A piece has SUB groups side by side (V / SUB channels of one group each; V: any).
+template <typename T, int V, int ACT, int SUB>
+__global__ void __launch_bounds__(THREADS, 2) group_apply_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float smem[];
   float* const s_mean = smem;       // [G]
   float* const s_rstd = smem + p.G;
@@ -212,25 +230,29 @@ __global__ void __launch_bounds__(THREADS) group_apply_kernel(const __grid_const
   const int n_scene = scenes.row0[t.scene + 1] - scenes.row0[t.scene];
   const int n_last = n_scene - (t.last - t.first - 1) * p.rows;
   per_group(p.G, [&](int g, int lane, int width) {
-    double sum = 0, m2 = 0;
-    const bool live = g < p.G;
-    if (live)
-      for (int i = t.first + lane; i < t.last; i += width)
-        sum += (double)__ldg(&p.part[(int64_t)i * p.G + g]).x * (i == t.last - 1 ? n_last : p.rows);
-    const double mean = sum_over(sum, width) / n_scene;
-    if (live)
+    // in one pass, about the first tile's mean: what the tiles' means differ by is no more than the spread
+    double n = 0, d1 = 0, d2 = 0;
+    float about = 0.f;
+    if (g < p.G) {
+      about = __ldg(&p.part[(int64_t)t.first * p.G + g]).x;
+#pragma unroll 4
       for (int i = t.first + lane; i < t.last; i += width) {
         const float2 v = __ldg(&p.part[(int64_t)i * p.G + g]);
-        const double d = (double)v.x - mean;
-        m2 += (double)v.y + d * d * ((double)(i == t.last - 1 ? n_last : p.rows) * p.per);
+        const double k = (double)(i == t.last - 1 ? n_last : p.rows), d = (double)v.x - (double)about;
+        d1 += k * d;
+        d2 += (double)v.y + k * d * d * p.per;
       }
-    m2 = sum_over(m2, width);
-    if (live && lane == 0) {
-      const float rstd = (float)(1.0 / sqrt(m2 / ((double)n_scene * p.per) + (double)p.eps));
-      s_mean[g] = (float)mean;
+    }
+    n = (double)n_scene;
+    d1 = sum_over(d1, width) / n;
+    d2 = sum_over(d2, width);
+    if (g < p.G && lane == 0) {
+      const double var = d2 / (n * p.per) - d1 * d1;
+      const float mean = (float)((double)about + d1), rstd = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps));
+      s_mean[g] = mean;
       s_rstd[g] = rstd;
       if ((int)blockIdx.x == t.first && p.mean) {
-        p.mean[(int64_t)t.scene * p.G + g] = (float)mean;
+        p.mean[(int64_t)t.scene * p.G + g] = mean;
         p.rstd[(int64_t)t.scene * p.G + g] = rstd;
       }
     }
@@ -240,11 +262,11 @@ __global__ void __launch_bounds__(THREADS) group_apply_kernel(const __grid_const
   const T* const x = reinterpret_cast<const T*>(p.x);
   T* const y = reinterpret_cast<T*>(p.out);
   for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
-    float mean[V], scale[V], beta[V];
+    float mean[SUB], scale[V], beta[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = pc * V + i, g = c / p.per;
-      mean[i] = s_mean[g];
+      mean[i * SUB / V] = s_mean[g];
       scale[i] = s_rstd[g] * (p.gamma ? __ldg(&p.gamma[c]) : 1.f);
       beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
     }
@@ -258,15 +280,15 @@ __global__ void __launch_bounds__(THREADS) group_apply_kernel(const __grid_const
         if (r + u * at.tys >= t.hi) break;
         Piece<T, V> o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = wcn_from_float<T>(activate<ACT>(fmaf(wcn_to_float<T>(q[u].v[i]) - mean[i], scale[i], beta[i])));
+        for (int i = 0; i < V; ++i) o.v[i] = wcn_from_float<T>(activate<ACT>(fmaf(wcn_to_float<T>(q[u].v[i]) - mean[i * SUB / V], scale[i], beta[i])));
         store_piece<T, V>(y + (int64_t)(r + u * at.tys) * p.C + pc * V, o);
       }
     }
   }
 }
 
-template <typename T, int V, int ACT, int M>
-__global__ void __launch_bounds__(THREADS) group_grad_sums_kernel(const __grid_constant__ Scenes<M> scenes, const __grid_constant__ Params p) {
+template <typename T, int V, int ACT, int SUB>
+__global__ void __launch_bounds__(THREADS, 1) group_grad_sums_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float smem[];
   const Place at(p.C, V);
   const int W = at.txs * V;
@@ -277,16 +299,15 @@ __global__ void __launch_bounds__(THREADS) group_grad_sums_kernel(const __grid_c
   const Tile t = find_tile(scenes, p.rows);
   const T *const x = reinterpret_cast<const T*>(p.x), *const dy = reinterpret_cast<const T*>(p.dy);
   for (int pc = at.tx; pc - at.tx < at.pieces; pc += at.txs) {
-    const bool live = at.ty < at.tys && pc < at.pieces;
-    if (live) {
-      float a[V], b[V], mean[V], rstd[V], gamma[V], beta[V];
+    if (at.ty < at.tys && pc < at.pieces) {
+      float a[V], b[V], mean[SUB], rstd[SUB], gamma[V], beta[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int c = pc * V + i;
         const int64_t g = (int64_t)t.scene * p.G + c / p.per;
         a[i] = b[i] = 0.f;
-        mean[i] = __ldg(&p.mean[g]);
-        rstd[i] = __ldg(&p.rstd[g]);
+        mean[i * SUB / V] = __ldg(&p.mean[g]);
+        rstd[i * SUB / V] = __ldg(&p.rstd[g]);
         gamma[i] = p.gamma ? __ldg(&p.gamma[c]) : 1.f;
         beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
       }
@@ -303,7 +324,7 @@ __global__ void __launch_bounds__(THREADS) group_grad_sums_kernel(const __grid_c
           if (r + u * at.tys >= t.hi) break;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[i]) * rstd[i];
+            const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[i * SUB / V]) * rstd[i * SUB / V];
             const float dz = through<ACT>(wcn_to_float<T>(d[u].v[i]), fmaf(xhat, gamma[i], beta[i]));
             a[i] += dz;
             b[i] = fmaf(dz, xhat, b[i]);
@@ -318,12 +339,17 @@ __global__ void __launch_bounds__(THREADS) group_grad_sums_kernel(const __grid_c
     }
     __syncthreads();
     const int c0 = (pc - at.tx) * V;
-    for (int c = threadIdx.x; c < W && c0 + c < p.C; c += THREADS) {
+    per_channel(W, [&](int c, int y0, int share) {
+      const bool live = c < W && c0 + c < p.C;
       float a = 0.f, b = 0.f;
-      for (int y = 0; y < at.tys; ++y) {
-        a += s_a[y * W + c];
-        b += s_b[y * W + c];
-      }
+      if (live)
+        for (int y = y0; y < at.tys; y += share) {
+          a += s_a[y * W + c];
+          b += s_b[y * W + c];
+        }
+      a = sum_over(a, share);
+      b = sum_over(b, share);
+      if (!live || y0) return;
       const float gamma = p.gamma ? __ldg(&p.gamma[c0 + c]) : 1.f;
       if (p.channels) {
         p.channels[(int64_t)blockIdx.x * 2 * p.C + c0 + c] = a;
@@ -331,27 +357,24 @@ __global__ void __launch_bounds__(THREADS) group_grad_sums_kernel(const __grid_c
       }
       c_a[c0 + c] = gamma * a;
       c_b[c0 + c] = gamma * b;
-    }
+    });
     __syncthreads();
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int g = warp; g < p.G; g += THREADS / 32) {
+  per_group(p.G, [&](int g, int lane, int width) {
     float a = 0.f, b = 0.f;
-    for (int c = lane; c < p.per; c += 32) {
-      a += c_a[g * p.per + c];
-      b += c_b[g * p.per + c];
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-      b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
-    }
-    if (lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(a, b);
-  }
+    if (g < p.G)
+      for (int c = lane; c < p.per; c += width) {
+        a += c_a[g * p.per + c];
+        b += c_b[g * p.per + c];
+      }
+    a = sum_over(a, width);
+    b = sum_over(b, width);
+    if (g < p.G && lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(a, b);
+  });
 }
 
-template <typename T, int V, int ACT, int M>
-__global__ void __launch_bounds__(THREADS) group_grad_apply_kernel(const __grid_constant__ Scenes<M> scenes, const __grid_constant__ Params p) {
+template <typename T, int V, int ACT, int SUB>
+__global__ void __launch_bounds__(THREADS, 1) group_grad_apply_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float smem[];
   float* const s_a = smem;          // [G]
   float* const s_b = smem + p.G;
@@ -361,6 +384,7 @@ __global__ void __launch_bounds__(THREADS) group_grad_apply_kernel(const __grid_
   per_group(p.G, [&](int g, int lane, int width) {
     double a = 0, b = 0;
     if (g < p.G)
+#pragma unroll 4
       for (int i = t.first + lane; i < t.last; i += width) {
         const float2 v = __ldg(&p.part[(int64_t)i * p.G + g]);
         a += (double)v.x;
@@ -379,34 +403,35 @@ __global__ void __launch_bounds__(THREADS) group_grad_apply_kernel(const __grid_
   const T *const x = reinterpret_cast<const T*>(p.x), *const dy = reinterpret_cast<const T*>(p.dy);
   T* const dx = reinterpret_cast<T*>(p.out);
   for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
-    float mean[V], rstd[V], gamma[V], beta[V], a[V], b[V];
+    float mean[SUB], rstd[SUB], gamma[V], beta[V], a[SUB], b[SUB];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = pc * V + i, g = c / p.per;
-      mean[i] = __ldg(&p.mean[(int64_t)t.scene * p.G + g]);
-      rstd[i] = __ldg(&p.rstd[(int64_t)t.scene * p.G + g]);
+      mean[i * SUB / V] = __ldg(&p.mean[(int64_t)t.scene * p.G + g]);
+      rstd[i * SUB / V] = __ldg(&p.rstd[(int64_t)t.scene * p.G + g]);
       gamma[i] = p.gamma ? __ldg(&p.gamma[c]) : 1.f;
       beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
-      a[i] = s_a[g];
-      b[i] = s_b[g];
+      a[i * SUB / V] = s_a[g];
+      b[i * SUB / V] = s_b[g];
     }
-    for (int r = t.lo + at.ty; r < t.hi; r += 2 * at.tys) {
-      Piece<T, V> q[2], d[2];
+    for (int r = t.lo + at.ty; r < t.hi; r += 4 * at.tys) {
+      Piece<T, V> q[4], d[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 4; ++u)
         if (r + u * at.tys < t.hi) {
           q[u] = load_piece<T, V>(x + (int64_t)(r + u * at.tys) * p.x_ld + pc * V);
           d[u] = load_piece<T, V>(dy + (int64_t)(r + u * at.tys) * p.dy_ld + pc * V);
         }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 4; ++u) {
         if (r + u * at.tys >= t.hi) break;
         Piece<T, V> o;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[i]) * rstd[i];
+          const int k = i * SUB / V;
+          const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[k]) * rstd[k];
           const float dz = through<ACT>(wcn_to_float<T>(d[u].v[i]), fmaf(xhat, gamma[i], beta[i]));
-          o.v[i] = wcn_from_float<T>(rstd[i] * (fmaf(gamma[i], dz, -a[i]) - xhat * b[i]));
+          o.v[i] = wcn_from_float<T>(rstd[k] * (fmaf(gamma[i], dz, -a[k]) - xhat * b[k]));
         }
         store_piece<T, V>(dx + (int64_t)(r + u * at.tys) * p.C + pc * V, o);
       }
@@ -414,47 +439,41 @@ __global__ void __launch_bounds__(THREADS) group_grad_apply_kernel(const __grid_
   }
 }
 
-// Sums over the tiles: 32 channels a block, eight tiles side by side, in double.
-__global__ void __launch_bounds__(THREADS) group_param_grads_kernel(const float* part, int64_t tiles, int n, float* out) {
-  __shared__ double s[THREADS / 32][33];
+// Sums over the tiles: 32 channels a block, 32 tiles side by side, in double.
+__global__ void __launch_bounds__(1024) group_param_grads_kernel(const float* part, int64_t tiles, int n, float* out) {
+  __shared__ double s[32][33];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   double v = 0;
   if (c < n) {
-    int64_t i = y;
-    for (; i + 3 * (THREADS / 32) < tiles; i += 4 * (THREADS / 32)) {
-      float q[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) q[u] = __ldg(&part[(i + u * (THREADS / 32)) * n + c]);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v += (double)q[u];
-    }
-    for (; i < tiles; i += THREADS / 32) v += (double)__ldg(&part[i * n + c]);
+#pragma unroll 8
+    for (int64_t i = y; i < tiles; i += 32) v += (double)__ldg(&part[i * n + c]);
   }
   s[y][lane] = v;
   __syncthreads();
-  if (y == 0 && c < n) {
-    for (int k = 1; k < THREADS / 32; ++k) v += s[k][lane];
-    out[c] = (float)v;
-  }
+  v = sum_over(s[lane][y], 32);   // (a warp a channel)
+  if (lane == 0 && blockIdx.x * 32 + y < n) out[blockIdx.x * 32 + y] = (float)v;
 }
 
 // ------------------------------------------------------------------ launches
 
 struct Plan {
   int vec;       // elements of a piece
-  int rows;      // rows of a tile
+  int tys;       // rows of a block side by side
 };
 
-Plan plan(int64_t n, int C, int elem, bool aligned) {
+Plan plan(int C, int elem, bool aligned) {
   Plan q;
   q.vec = aligned && C % (16 / elem) == 0 ? 16 / elem : 1;
-  const int pieces = C / q.vec, tys = THREADS / (pieces < THREADS ? pieces : THREADS);
-  // four blocks an SM, one to 64 rows a thread
-  int64_t per = n / ((int64_t)tys * 4 * wcn_num_sms());
-  per = per < 1 ? 1 : per > 64 ? 64 : per;
-  if (per > ROWS) per = per / ROWS * ROWS;
-  q.rows = (int)(per * tys);
+  const int pieces = C / q.vec;
+  q.tys = THREADS / (pieces < THREADS ? pieces : THREADS);
   return q;
+}
+
+// Rows of a tile, for a launch over n rows: as many blocks as run at once (three times as many where scenes are short, whose
+// last tiles are smaller ones), at least four rows a thread.
+int tile_rows(int64_t n, int64_t scenes, int tys, int blocks_per_sm) {
+  const int64_t side = (int64_t)tys * blocks_per_sm * wcn_num_sms() * (scenes > 16 ? 3 : 1), per = (n + side - 1) / side;
+  return (int)((per < 4 ? 4 : per) * tys);
 }
 
 size_t sums_smem(int C, int vec) {
@@ -462,77 +481,76 @@ size_t sums_smem(int C, int vec) {
   return ((size_t)2 * tys * txs * vec + 2 * C) * sizeof(float);
 }
 
-// All launches of one direction over one group of scenes: f(scenes, tiles).
-template <int M, typename F> int launch_group(const int64_t* offsets, int64_t first, int64_t last, int rows, F&& f) {
-  Scenes<M> s;
-  s.count = (int)(last - first);
-  int tiles = 0;
-  for (int64_t i = first; i <= last; ++i) {
-    s.row0[i - first] = (int)(offsets[i] - offsets[first]);
-    s.tile0[i - first] = tiles;
-    if (i < last) tiles += (int)((offsets[i + 1] - offsets[i] + rows - 1) / rows);
-  }
-  if (!tiles) return WCN_OK;
-  return f(s, tiles);
-}
-
-// The scenes in groups that stay in L2.
-template <typename F> int in_groups(const int64_t* offsets, int64_t scenes, int64_t row_bytes, F&& f) {
+// The scenes in groups that stay in L2: f(first, behind the last, rows of a tile, tiles).
+template <typename F> int in_groups(const int64_t* offsets, int64_t scenes, int64_t row_bytes, bool back, int tys, F&& f) {
   for (int64_t i = 0; i < scenes;) {
     int64_t j = i + 1;
-    while (j < scenes && j - i < MANY && (offsets[j + 1] - offsets[i]) * row_bytes <= GROUP_BYTES) ++j;
-    const int rc = f(i, j);
+    while (j < scenes && j - i < SCENES && (offsets[j + 1] - offsets[i]) * row_bytes <= GROUP_BYTES) ++j;
+    const int rows = tile_rows(offsets[j] - offsets[i], j - i, tys, back ? 1 : 2);
+    int64_t tiles = 0;
+    for (int64_t k = i; k < j; ++k) tiles += (offsets[k + 1] - offsets[k] + rows - 1) / rows;
+    const int rc = tiles ? f(i, j, rows, (int)tiles) : WCN_OK;
     if (rc != WCN_OK) return rc;
     i = j;
   }
   return WCN_OK;
 }
 
-template <typename T, int V, int ACT, int M> int forward_group(const Scenes<M>& s, int tiles, const Params& p, cudaStream_t st) {
-  group_stats_kernel<T, V, M><<<tiles, THREADS, sums_smem(p.C, V), st>>>(s, p);
-  group_apply_kernel<T, V, ACT, M><<<tiles, THREADS, (size_t)2 * p.G * sizeof(float), st>>>(s, p);
-  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
-}
-template <typename T, int V, int ACT, int M> int backward_group(const Scenes<M>& s, int tiles, const Params& p, cudaStream_t st) {
-  group_grad_sums_kernel<T, V, ACT, M><<<tiles, THREADS, sums_smem(p.C, V), st>>>(s, p);
-  if (p.out) group_grad_apply_kernel<T, V, ACT, M><<<tiles, THREADS, (size_t)2 * p.G * sizeof(float), st>>>(s, p);
-  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
-}
-
-template <typename T, int V, int ACT> int all_groups(bool back, Params p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
+template <typename T, int V, int ACT, int SUB> int all_groups(bool back, Params p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
   const int64_t row_bytes = (int64_t)p.C * sizeof(T) * (back ? 2 : 1);
   const Params base = p;
-  return in_groups(offsets, scenes, row_bytes, [&](int64_t i, int64_t j) {
+  const size_t sums = sums_smem(p.C, V), apply = (size_t)2 * p.G * sizeof(float);
+  const int pieces = p.C / V, tys = THREADS / (pieces < THREADS ? pieces : THREADS);
+  if (sums > 48 * 1024) {
+    auto a = group_stats_kernel<T, V>;
+    auto b = group_grad_sums_kernel<T, V, ACT, SUB>;
+    if (cudaFuncSetAttribute(a, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums) != cudaSuccess ||
+        cudaFuncSetAttribute(b, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums) != cudaSuccess)
+      return WCN_ERR_INITIALIZATION;
+  }
+  return in_groups(offsets, scenes, row_bytes, back, tys, [&](int64_t i, int64_t j, int rows, int tiles) {
     const int64_t r = offsets[i];
+    Scenes s;
+    s.count = (int)(j - i);
+    int at = 0;
+    for (int64_t k = i; k <= j; ++k) {
+      s.row0[k - i] = (int)(offsets[k] - r);
+      s.tile0[k - i] = at;
+      if (k < j) at += (int)((offsets[k + 1] - offsets[k] + rows - 1) / rows);
+    }
+    p.rows = rows;
     p.x = reinterpret_cast<const T*>(base.x) + r * p.x_ld;
     if (back) p.dy = reinterpret_cast<const T*>(base.dy) + r * p.dy_ld;
     p.out = base.out ? reinterpret_cast<T*>(base.out) + r * p.C : nullptr;
     p.mean = base.mean ? base.mean + i * p.G : nullptr;
     p.rstd = base.rstd ? base.rstd + i * p.G : nullptr;
-    auto go = [&](const auto& s, int tiles) {
-      constexpr int M = sizeof(s) == sizeof(Scenes<FEW>) ? FEW : MANY;
-      const int rc = back ? backward_group<T, V, ACT, M>(s, tiles, p, st) : forward_group<T, V, ACT, M>(s, tiles, p, st);
-      if (back) {  // (the forward's tiles are done with once its second launch is)
-        p.part += (int64_t)tiles * p.G;
-        if (p.channels) p.channels += (int64_t)tiles * 2 * p.C;
-      }
-      return rc;
-    };
-    return j - i <= FEW ? launch_group<FEW>(offsets, i, j, p.rows, go) : launch_group<MANY>(offsets, i, j, p.rows, go);
+    if (!back) {
+      group_stats_kernel<T, V><<<tiles, THREADS, sums, st>>>(s, p);
+      group_apply_kernel<T, V, ACT, SUB><<<tiles, THREADS, apply, st>>>(s, p);
+    } else {
+      group_grad_sums_kernel<T, V, ACT, SUB><<<tiles, THREADS, sums, st>>>(s, p);
+      if (p.out) group_grad_apply_kernel<T, V, ACT, SUB><<<tiles, THREADS, apply, st>>>(s, p);
+      if (p.channels) p.channels += (int64_t)tiles * 2 * p.C;   // (the groups' sums are done with, these are not)
+    }
+    return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
   });
 }
 
-template <typename T, int V> int by_act(int act, bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
+template <typename T, int V, int SUB> int by_act(int act, bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
   switch (act) {
-    case NONE: return all_groups<T, V, NONE>(back, p, offsets, scenes, st);
-    case RELU: return all_groups<T, V, RELU>(back, p, offsets, scenes, st);
-    case SILU: return all_groups<T, V, SILU>(back, p, offsets, scenes, st);
-    default: return all_groups<T, V, GELU>(back, p, offsets, scenes, st);
+    case NONE: return all_groups<T, V, NONE, SUB>(back, p, offsets, scenes, st);
+    case RELU: return all_groups<T, V, RELU, SUB>(back, p, offsets, scenes, st);
+    case SILU: return all_groups<T, V, SILU, SUB>(back, p, offsets, scenes, st);
+    default: return all_groups<T, V, GELU, SUB>(back, p, offsets, scenes, st);
   }
 }
 
 template <typename T> int by_vec(int vec, int act, bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
-  return vec == 1 ? by_act<T, 1>(act, back, p, offsets, scenes, st) : by_act<T, 16 / (int)sizeof(T)>(act, back, p, offsets, scenes, st);
+  constexpr int V = 16 / (int)sizeof(T);
+  if (vec == 1) return by_act<T, 1, 1>(act, back, p, offsets, scenes, st);
+  if (p.per % V == 0) return by_act<T, V, 1>(act, back, p, offsets, scenes, st);
+  if (p.per % (V / 2) == 0) return by_act<T, V, 2>(act, back, p, offsets, scenes, st);
+  return by_act<T, V, V>(act, back, p, offsets, scenes, st);
 }
 
 int by_dtype(int dtype, int vec, int act, bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
@@ -549,10 +567,14 @@ bool norm_ok(int64_t scenes, const int64_t* offsets, int C, int G, int dtype) {
   return true;
 }
 
-int64_t count_tiles(const int64_t* offsets, int64_t scenes, int rows) {
-  int64_t tiles = 0;
-  for (int64_t i = 0; i < scenes; ++i) tiles += (offsets[i + 1] - offsets[i] + rows - 1) / rows;
-  return tiles;
+// Tiles of all launches together, and of the largest one.
+void count_tiles(const int64_t* offsets, int64_t scenes, int64_t row_bytes, bool back, int tys, int64_t* all, int64_t* most) {
+  *all = *most = 0;
+  in_groups(offsets, scenes, row_bytes, back, tys, [&](int64_t, int64_t, int, int tiles) {
+    *all += tiles;
+    if (tiles > *most) *most = tiles;
+    return (int)WCN_OK;
+  });
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -564,8 +586,14 @@ float from_bits(uint32_t b) {
   return f;
 }
 
-// Bytes of the groups' sums, then of the channels' (backward).
-int64_t part_bytes(int64_t tiles, int G) { return (tiles * G * (int64_t)sizeof(float2) + 15) / 16 * 16; }
+// Bytes of the groups' sums (of a launch), then of the channels' (of all of them).
+int64_t part_bytes(const int64_t* offsets, int64_t scenes, int C, int G, int elem, bool back, bool channels, int tys, int64_t* total) {
+  int64_t all, most;
+  count_tiles(offsets, scenes, (int64_t)C * elem * (back ? 2 : 1), back, tys, &all, &most);
+  const int64_t first = (most * G * (int64_t)sizeof(float2) + 15) / 16 * 16;
+  *total = first + (channels ? all * 2 * C * 4 : 0);
+  return first;
+}
 
 }  // namespace
 
@@ -574,8 +602,9 @@ extern "C" int wcn_group_norm_workspace_bytes(const int64_t* offsets, int64_t sc
   if (!bytes || !norm_ok(scenes, offsets, channels, groups, dtype)) return WCN_ERR_INVALID_PARAMETERS;
   int64_t most = 0;
   for (int v = 0; v < 2; ++v) {   // (whatever the rows' alignment will be)
-    const int64_t tiles = count_tiles(offsets, scenes, plan(offsets[scenes], channels, wcn_dtype_size(dtype), v).rows);
-    const int64_t need = part_bytes(tiles, groups) + (backward ? tiles * 2 * channels * 4 : 0);
+    int64_t need;
+    const int elem = wcn_dtype_size(dtype);
+    part_bytes(offsets, scenes, channels, groups, elem, backward, backward, plan(channels, elem, v).tys, &need);
     if (need > most) most = need;
   }
   *bytes = most;
@@ -590,11 +619,13 @@ extern "C" int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offset
   if (!offsets[scenes]) return WCN_OK;
   if (!x || !y || !workspace || !on16(workspace)) return WCN_ERR_INVALID_PARAMETERS;
   const int elem = wcn_dtype_size(dtype);
-  const Plan q = plan(offsets[scenes], channels, elem, rows_on16(x, x_ld, elem) && rows_on16(y, channels, elem));
-  if (part_bytes(count_tiles(offsets, scenes, q.rows), groups) > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  const Plan q = plan(channels, elem, rows_on16(x, x_ld, elem) && rows_on16(y, channels, elem));
+  int64_t need;
+  part_bytes(offsets, scenes, channels, groups, elem, false, false, q.tys, &need);
+  if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   Params p = {};
   p.x = x; p.out = y; p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)workspace;
-  p.x_ld = x_ld; p.C = channels; p.G = groups; p.per = channels / groups; p.rows = q.rows; p.eps = from_bits(eps_bits);
+  p.x_ld = x_ld; p.C = channels; p.G = groups; p.per = channels / groups; p.eps = from_bits(eps_bits);
   return by_dtype(dtype, q.vec, act, false, p, offsets, scenes, wcn_stream(stream));
 }
 
@@ -608,16 +639,17 @@ extern "C" int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* 
   if (!offsets[scenes]) return !sums || cudaMemsetAsync(sums, 0, (size_t)2 * channels * 4, st) == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
   if (!x || !dy || !mean || !rstd || !workspace || !on16(workspace)) return WCN_ERR_INVALID_PARAMETERS;
   const int elem = wcn_dtype_size(dtype);
-  const Plan q = plan(offsets[scenes], channels, elem, rows_on16(x, x_ld, elem) && rows_on16(dy, dy_ld, elem) && rows_on16(dx, channels, elem));
-  const int64_t tiles = count_tiles(offsets, scenes, q.rows);
-  if (part_bytes(tiles, groups) + (sums ? tiles * 2 * channels * 4 : 0) > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  const Plan q = plan(channels, elem, rows_on16(x, x_ld, elem) && rows_on16(dy, dy_ld, elem) && rows_on16(dx, channels, elem));
+  int64_t need;
+  const int64_t first = part_bytes(offsets, scenes, channels, groups, elem, true, sums, q.tys, &need);
+  if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   Params p = {};
   p.x = x; p.dy = dy; p.out = dx; p.gamma = gamma; p.beta = beta; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
   p.part = (float2*)workspace;
-  p.channels = sums ? (float*)((char*)workspace + part_bytes(tiles, groups)) : nullptr;
-  p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = channels; p.G = groups; p.per = channels / groups; p.rows = q.rows;
+  p.channels = sums ? (float*)((char*)workspace + first) : nullptr;
+  p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = channels; p.G = groups; p.per = channels / groups;
   const int rc = by_dtype(dtype, q.vec, act, true, p, offsets, scenes, st);
   if (rc != WCN_OK || !sums) return rc;
-  group_param_grads_kernel<<<(2 * channels + 31) / 32, THREADS, 0, st>>>(p.channels, tiles, 2 * channels, sums);
+  group_param_grads_kernel<<<(2 * channels + 31) / 32, 1024, 0, st>>>(p.channels, (need - first) / (2 * channels * 4), 2 * channels, sums);
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }

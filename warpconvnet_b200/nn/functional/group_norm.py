@@ -4,12 +4,13 @@ An addition to the reference, whose ``GroupNorm`` is ``nn.GroupNorm`` of ``[N, C
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Optional, Sequence, Union
 
 import torch
 from torch import Tensor
 
-from ..._native import check, dtype_code, lib, ptr, require_cuda, stream_ptr
+from ..._native import check, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
 from .batch_norm import _bits, reverse_mode_only
 
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
@@ -22,13 +23,21 @@ def check_activation(activation: Optional[str]) -> int:
         raise ValueError(f"activation is one of {list(_ACTIVATIONS)}, got {activation!r}") from None
 
 
-def _host_offsets(offsets: Union[Tensor, Sequence[int], None], n: int) -> Tensor:
+def _host_offsets(offsets: Union[Tensor, Sequence[int], None], n: int) -> array:
+    """[scenes + 1] 64-bit integers on the host."""
     if offsets is None:
-        return torch.tensor([0, n], dtype=torch.int64)
-    offsets = torch.as_tensor(offsets)
-    if offsets.dim() != 1 or not len(offsets) or offsets.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"offsets must be a 1-d integer tensor [scenes + 1], got {tuple(offsets.shape)} {offsets.dtype}")
-    return offsets.detach().to(device="cpu", dtype=torch.int64).contiguous()
+        return array("q", (0, n))
+    if isinstance(offsets, Tensor):
+        if offsets.dim() != 1 or offsets.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"offsets must be a 1-d integer tensor [scenes + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+        offsets = offsets.tolist()
+    try:
+        at = array("q", offsets)
+    except (TypeError, OverflowError):
+        raise ValueError("offsets must be integers [scenes + 1]") from None
+    if not at or at[-1] != n:
+        raise ValueError(f"offsets must end at the {n} rows of x, got {list(at[-4:])}")
+    return at
 
 
 def _rows(t: Tensor):
@@ -39,14 +48,14 @@ def _rows(t: Tensor):
     return t, max(t.stride(0), c)
 
 
-def _workspace(offsets: Tensor, c: int, groups: int, dtype: int, backward: bool, device) -> Tensor:
+def _workspace(offsets: array, c: int, groups: int, dtype: int, backward: bool, device) -> Tensor:
     size = ctypes.c_int64(0)
-    if lib().wcn_group_norm_workspace_bytes(offsets.data_ptr(), len(offsets) - 1, c, groups, dtype, int(backward), ctypes.addressof(size)):
-        raise ValueError(f"offsets must rise from 0 to a number of rows, with at most 4096 channels: got {offsets.tolist()[:8]} ..., {c} channels")
+    if lib().wcn_group_norm_workspace_bytes(offsets.buffer_info()[0], len(offsets) - 1, c, groups, dtype, int(backward), ctypes.addressof(size)):
+        raise ValueError(f"offsets must rise from 0, and at most 4096 channels are taken: got {list(offsets[:8])} ... and {c} channels")
     return torch.empty(max(16, size.value), dtype=torch.uint8, device=device)
 
 
-def _forward(x: Tensor, offsets: Tensor, groups: int, weight, bias, eps: float, act: int, keep: bool):
+def _forward(x: Tensor, offsets: array, groups: int, weight, bias, eps: float, act: int, keep: bool):
     """(y, mean and 1 / std of each scene and group, or None)"""
     n, c = x.shape
     dev, dc = x.device, dtype_code(x.dtype)
@@ -56,16 +65,16 @@ def _forward(x: Tensor, offsets: Tensor, groups: int, weight, bias, eps: float, 
     saved = torch.empty((2, scenes, groups), dtype=torch.float32, device=dev) if keep else None
     x, ld = _rows(x)
     at = saved.data_ptr() if keep else None
-    with torch.cuda.device(dev):
-        check(lib().wcn_group_norm(ptr(x), ld, offsets.data_ptr(), scenes, c, groups, dc, ptr(weight), ptr(bias), _bits(eps), act, ptr(y),
+    with on_device(dev):
+        check(lib().wcn_group_norm(ptr(x), ld, offsets.buffer_info()[0], scenes, c, groups, dc, ptr(weight), ptr(bias), _bits(eps), act, ptr(y),
                                    at, at + 4 * scenes * groups if keep else None, ptr(ws), ws.numel(), stream_ptr(dev)), "wcn_group_norm")
     return y, saved
 
 
-def formula(x: Tensor, offsets: Tensor, groups: int, weight, bias, eps: float, activation: Optional[str]) -> Tensor:
+def formula(x: Tensor, offsets: Sequence[int], groups: int, weight, bias, eps: float, activation: Optional[str]) -> Tensor:
     """The same through torch, scene by scene: for a graph of the gradient, forward-mode differentiation and function transforms."""
-    at, out = offsets.tolist(), []
-    for lo, hi in zip(at, at[1:]):
+    out = []
+    for lo, hi in zip(offsets, offsets[1:]):
         if hi > lo:
             xs = x[lo:hi].float().reshape(hi - lo, groups, -1)
             var, mean = torch.var_mean(xs, dim=(0, 2), keepdim=True, correction=0)
@@ -81,10 +90,10 @@ def formula(x: Tensor, offsets: Tensor, groups: int, weight, bias, eps: float, a
 
 class _SegmentedGroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], offsets: Tensor, groups: int, eps: float, activation):
+    def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], offsets: array, groups: int, eps: float, activation):
         y, saved = _forward(x, offsets, groups, _vector(weight), _vector(bias), eps, _ACTIVATIONS[activation], True)
         ctx.save_for_backward(x, weight, bias, saved)
-        ctx.offsets, ctx.groups, ctx.eps, ctx.activation = offsets.clone(), groups, eps, activation
+        ctx.offsets, ctx.groups, ctx.eps, ctx.activation = offsets, groups, eps, activation
         return y
 
     @staticmethod
@@ -104,15 +113,17 @@ class _SegmentedGroupNorm(torch.autograd.Function):
         sums = torch.empty((2, c), dtype=torch.float32, device=dev) if need_w or need_b else None
         ws = _workspace(ctx.offsets, c, ctx.groups, dc, True, dev)
         gamma, beta, at = _vector(weight), _vector(bias), saved.data_ptr()
-        with torch.cuda.device(dev):
-            check(lib().wcn_group_norm_backward(ptr(x), x_ld, ptr(dy), dy_ld, ctx.offsets.data_ptr(), scenes, c, ctx.groups, dc, ptr(gamma),
+        with on_device(dev):
+            check(lib().wcn_group_norm_backward(ptr(x), x_ld, ptr(dy), dy_ld, ctx.offsets.buffer_info()[0], scenes, c, ctx.groups, dc, ptr(gamma),
                                                 ptr(beta), at, at + 4 * scenes * ctx.groups, _ACTIVATIONS[ctx.activation], ptr(dx), ptr(sums),
                                                 ptr(ws), ws.numel(), stream_ptr(dev)), "wcn_group_norm_backward")
         return (dx, sums[1].to(weight.dtype) if need_w else None, sums[0].to(bias.dtype) if need_b else None) + (None,) * 4
 
 
 def _vector(t: Optional[Tensor]) -> Optional[Tensor]:
-    return None if t is None else t.detach().float().contiguous()
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
 
 
 def segmented_group_norm(x: Tensor, offsets: Union[Tensor, Sequence[int], None], num_groups: int, weight: Optional[Tensor] = None,
@@ -135,8 +146,6 @@ def segmented_group_norm(x: Tensor, offsets: Union[Tensor, Sequence[int], None],
         if t is not None and (t.shape != (c,) or t.device != x.device or not t.is_floating_point()):
             raise ValueError(f"{name} must be {c} floating-point numbers on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     offsets = _host_offsets(offsets, n)
-    if int(offsets[-1]) != n:
-        raise ValueError(f"offsets end at {int(offsets[-1])}, x has {n} rows")
     if not reverse_mode_only():
         return formula(x, offsets, num_groups, weight, bias, eps, activation)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):

@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from ..._native import check, device_status, dtype_code, lib, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import check, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import _counter, reverse_mode_only
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -40,23 +40,29 @@ def _workspace(n: int, c: int, v: int, code: int, what: int, device) -> Tensor:
     return torch.empty(query_bytes("wcn_linear_ce_workspace_bytes", n, c, v, code, what), dtype=torch.uint8, device=device)
 
 
+def _kept(n: int, v: int, bias: bool):
+    """Places of the count and of the bias in what is kept, and its length."""
+    at_bias = (2 * n + 1 + 3) // 4 * 4
+    return 2 * n, at_bias, at_bias + (-(-v // 256) * 256 + 256 if bias else 0)
+
+
 def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: int):
-    """(loss or losses, what the backward pass needs)"""
+    """(loss or losses, what the backward pass needs: log-sum-exp and loss of each row, the count, the bias in units of ln 2)"""
     (n, c), v, dev = x.shape, weight.shape[0], x.device
     code, stream = dtype_code(x.dtype), stream_ptr(dev)
     x, x_ld = _matrix(x)
     weight, w_ld = _matrix(weight)
-    rows = torch.empty((2, n), dtype=torch.float32, device=dev)        # log-sum-exp and loss of each row
-    bias2 = None if bias is None else torch.empty(-(-v // 256) * 256 + 256, dtype=torch.float32, device=dev)
-    count = torch.empty(1, dtype=torch.int32, device=dev)
+    at_count, at_bias, length = _kept(n, v, bias is not None)
+    kept = torch.empty(length, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
+    base = kept.data_ptr()
     ws = _workspace(n, c, v, code, 0, dev)
-    with torch.cuda.device(dev):
+    with on_device(dev):
         check(lib().wcn_linear_ce(ptr(x), x_ld, n, c, ptr(weight), w_ld, v, ptr(bias), dtype_code(bias.dtype) if bias is not None else 0,
-                                  ptr(labels), ignore_index, code, reduction, ptr(rows), rows.data_ptr() + 4 * n, ptr(bias2), ptr(count),
-                                  ptr(loss), ptr(ws), ws.numel(), ptr(_counter(dev, stream)), ptr(device_status(dev)), stream),
+                                  ptr(labels), ignore_index, code, reduction, base, base + 4 * n, base + 4 * at_bias if bias is not None else None,
+                                  base + 4 * at_count, ptr(loss), ptr(ws), ws.numel(), ptr(_counter(dev, stream)), ptr(device_status(dev)), stream),
               "wcn_linear_ce")
-    return (loss if reduction else rows[1]), (rows, bias2, count)
+    return (loss if reduction else kept[n:2 * n]), kept
 
 
 def formula(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: str) -> Tensor:
@@ -69,14 +75,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], labels: Tensor, ignore_index: int, reduction: str):
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        loss, (rows, bias2, count) = _forward(x.detach(), weight.detach(), labels, None if bias is None else bias.detach().contiguous(),
-                                              ignore_index, _REDUCTIONS[reduction])
-        ctx.save_for_backward(x, weight, bias, labels, rows, bias2, count)
+        loss, kept = _forward(x.detach(), weight.detach(), labels, None if bias is None else bias.detach().contiguous(),
+                              ignore_index, _REDUCTIONS[reduction])
+        ctx.save_for_backward(x, weight, bias, labels, kept)
         return loss.clone() if reduction == "none" else loss   # (the row losses are kept: the caller's are its own)
 
     @staticmethod
     def backward(ctx, grad: Tensor):
-        x, weight, bias, labels, rows, bias2, count = ctx.saved_tensors
+        x, weight, bias, labels, kept = ctx.saved_tensors
         if torch.is_grad_enabled():  # a graph of the gradient is wanted
             loss = formula(x, weight, labels, bias, ctx.ignore_index, ctx.reduction)
             wanted = [t for t, need in zip((x, weight, bias), ctx.needs_input_grad) if need]
@@ -89,13 +95,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dw = torch.empty((v, c), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(v, dtype=bias.dtype, device=dev) if need_b else None
         grad = grad.float().contiguous()
+        at_count, at_bias, _ = _kept(n, v, bias is not None)
+        base = kept.data_ptr()
         row_max = grad.abs().amax() if ctx.reduction == "none" else None
         x, x_ld = _matrix(x)
         weight, w_ld = _matrix(weight)
         ws = _workspace(n, c, v, code, need_x + 2 * need_w + 4 * need_b, dev)
-        with torch.cuda.device(dev):
-            check(lib().wcn_linear_ce_backward(ptr(x), x_ld, n, c, ptr(weight), w_ld, v, ptr(bias2), ptr(labels), ctx.ignore_index, code,
-                                               ptr(rows), rows.data_ptr() + 4 * n, ptr(count) if ctx.reduction == "mean" else None, ptr(grad),
+        with on_device(dev):
+            check(lib().wcn_linear_ce_backward(ptr(x), x_ld, n, c, ptr(weight), w_ld, v, base + 4 * at_bias if bias is not None else None,
+                                               ptr(labels), ctx.ignore_index, code, base, base + 4 * n,
+                                               base + 4 * at_count if ctx.reduction == "mean" else None, ptr(grad),
                                                ptr(row_max), ptr(dx), ptr(dw), ptr(db), dtype_code(bias.dtype) if need_b else 0, ptr(ws),
                                                ws.numel(), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear_ce_backward")
         return dx, dw, db, None, None, None

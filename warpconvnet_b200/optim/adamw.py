@@ -11,12 +11,14 @@ from __future__ import annotations
 import functools
 import struct
 from array import array
+from itertools import accumulate, chain
+from operator import attrgetter, eq
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
 
-from .._native import check, dtype_code, lib, ptr, require_cuda, stream_ptr
+from .._native import check, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
 from ..nn.functional.batch_norm import _counter
 
 BLOCK = 256
@@ -30,15 +32,14 @@ def _bits(value: float) -> int:
 
 def moment_slots(sizes: Sequence[int]) -> Tuple[List[int], int]:
     """(first element of each tensor's moments, length of the flat moments) for tensors of these sizes in order."""
-    at, out = 0, []
-    for n in sizes:
-        out.append(at)
-        at += -(-n // BLOCK) * BLOCK
-    return out, at
+    out = list(accumulate([-(-n // BLOCK) * BLOCK for n in sizes], initial=0))
+    return out[:-1], out[-1]
 
 
-def _one(values, what: str):
-    kinds = set(values)
+_dtype, _layout, _shape = attrgetter("dtype"), attrgetter("layout"), attrgetter("shape")
+
+
+def _one(kinds: set, what: str):
     if len(kinds) != 1:
         raise ValueError(f"{what} differ: {sorted(map(str, kinds))}")
     return kinds.pop()
@@ -59,8 +60,8 @@ def _moments(m: Tensor, v: Tensor, m_base: Optional[Tensor], v_base: Optional[Te
     dtype = torch.float32 if m_base is None else torch.uint8
     n = m.numel()
     for t, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
-        if t.dtype != dtype or t.device != device or t.dim() != 1 or not t.is_contiguous() or t.numel() != n or n % BLOCK or t.data_ptr() % 16:
-            raise ValueError(f"{name} must be a contiguous, 16-byte aligned 1-d {dtype} tensor of a multiple of {BLOCK} elements on {device}, "
+        if t.dtype != dtype or t.device != device or t.dim() != 1 or not t.is_contiguous() or t.numel() != n or n % BLOCK or t.data_ptr() % 32:
+            raise ValueError(f"{name} must be a contiguous, 32-byte aligned 1-d {dtype} tensor of a multiple of {BLOCK} elements on {device}, "
                              f"as long as the other moment; got {tuple(t.shape)} {t.dtype} on {t.device}")
     for t, name in ((m_base, "exp_avg_base"), (v_base, "exp_avg_sq_base")):
         if t is not None and (t.dtype != torch.int16 or t.device != device or t.numel() != n // BLOCK or not t.is_contiguous()):
@@ -85,19 +86,20 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tenso
         raise ValueError(f"{len(params)} parameters but {len(grads)} gradients")
     if not params:
         return
-    device, dtype = _one([p.device for p in params], "devices of the parameters"), _one([p.dtype for p in params], "dtypes of the parameters")
+    # (a network has hundreds of tensors: each look at all of them is one pass of a C function)
+    device, dtype = params[0].device, _one(set(map(_dtype, params)), "dtypes of the parameters")
     require_cuda(params[0], "params")
-    if _one([g.device for g in grads], "devices of the gradients") != device:
-        raise ValueError(f"gradients must be on {device}")
-    if any(g.layout != torch.strided for g in grads):
+    if set(map(_layout, grads)) != {torch.strided}:
         raise TypeError("gradients must be dense")
-    grad_dtype = _one([g.dtype for g in grads], "dtypes of the gradients")
+    grad_dtype = _one(set(map(_dtype, grads)), "dtypes of the gradients")
     codes = dtype_code(dtype), dtype_code(grad_dtype)
-    if not all([p.is_contiguous() for p in params]):
+    if set(map(Tensor.get_device, params)) != {device.index} or set(map(Tensor.get_device, grads)) != {device.index}:
+        raise ValueError(f"all parameters and gradients must be on {device}")
+    if not all(map(Tensor.is_contiguous, params)):
         raise ValueError("parameters must be contiguous: they are updated in place")
-    if [p.shape for p in params] != [g.shape for g in grads]:
+    if not all(map(eq, map(_shape, params), map(_shape, grads))):
         raise ValueError("a gradient has another shape than its parameter")
-    sizes = [p.numel() for p in params]
+    sizes = list(map(Tensor.numel, params))
     length = _moments(exp_avg, exp_avg_sq, exp_avg_base, exp_avg_sq_base, device)
     if slots is None:
         slots, need = moment_slots(sizes)
@@ -119,18 +121,16 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tenso
             lr_at, lr = _scalar(lr, "lr", device), 0.0
         else:
             lr = float(lr)
-    if not all([g.is_contiguous() for g in grads]):
+    if not all(map(Tensor.is_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
-    table = array("q")
-    for row in zip([p.data_ptr() for p in params], [g.data_ptr() for g in grads], sizes, slots, step_index):
-        table.extend(row)
+    table = array("q", chain.from_iterable(zip(map(Tensor.data_ptr, params), map(Tensor.data_ptr, grads), sizes, slots, step_index)))
     stream = stream_ptr(device)
-    with torch.cuda.device(device):
+    with on_device(device):
         check(lib().wcn_adamw_step(table.buffer_info()[0], len(params), *codes, ptr(exp_avg), ptr(exp_avg_base), ptr(exp_avg_sq),
                                    ptr(exp_avg_sq_base), ptr(steps), _bits(lr), _bits(betas[0]), _bits(betas[1]), _bits(eps),
                                    _bits(weight_decay), lr_at, _scalar(grad_scale, "grad_scale", device),
                                    _scalar(found_inf, "found_inf", device), ptr(_counter(device, stream)), stream), "wcn_adamw_step")
-    torch.autograd.graph.increment_version(list(params))
+    torch.autograd.graph.increment_version(params)
 
 
 def decode_moments(exp_avg: Tensor, exp_avg_base: Tensor, exp_avg_sq: Tensor, exp_avg_sq_base: Tensor) -> Tuple[Tensor, Tensor]:
@@ -139,7 +139,7 @@ def decode_moments(exp_avg: Tensor, exp_avg_base: Tensor, exp_avg_sq: Tensor, ex
     device = exp_avg.device
     n = _moments(exp_avg, exp_avg_sq, exp_avg_base, exp_avg_sq_base, device)
     m, v = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
-    with torch.cuda.device(device):
+    with on_device(device):
         check(lib().wcn_adamw_decode(ptr(exp_avg), ptr(exp_avg_base), ptr(exp_avg_sq), ptr(exp_avg_sq_base), n, ptr(m), ptr(v),
                                      stream_ptr(device)), "wcn_adamw_decode")
     return m, v
