@@ -595,17 +595,19 @@ int wcn_batch_norm_backward(const void* x, const void* dy, const void* y, int64_
  * the error function); eps as the bits of a float.  mean / rstd [scenes, groups] (both or neither) are left for the backward
  * pass; those of empty scenes are not written.
  * backward: dx contiguous (may be NULL), sums [2, channels] = d beta, d gamma (may be NULL).
- * workspace: 16-byte aligned, the bytes that the query gives.  At most 4096 channels and 2^31 - 2^16 rows.
+ * workspace: 16-byte aligned, the bytes that the query gives.  sync: zeroed device memory of the size that its query gives, zero
+ * again afterwards (one per stream).  At most 4096 channels and 2^31 - 2^16 rows.  A launch for every 250 scenes that have rows.
  * The reference normalises per row (warpconvnet/nn/modules/normalizations.py) and has segment statistics as torch operations. */
 int wcn_group_norm_workspace_bytes(const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups, int dtype,
                                    int backward, int64_t* bytes);
+int wcn_group_norm_sync_bytes(int64_t* bytes);
 int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups, int dtype,
                    const float* gamma, const float* beta, uint32_t eps_bits, int act, void* y, float* mean, float* rstd,
-                   void* workspace, int64_t workspace_bytes, void* stream);
+                   void* workspace, int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream);
 int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const int64_t* offsets, int64_t scenes,
                             int32_t channels, int32_t groups, int dtype, const float* gamma, const float* beta,
                             const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
-                            int64_t workspace_bytes, void* stream);
+                            int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream);
 
 /* ------------------------------------------------------------------ cross entropy of a linear layer */
 

@@ -5,31 +5,44 @@
 //     dbeta = sum dz,  dgamma = sum dz xhat,  dx = (gamma dz - sum(gamma dz) / M - xhat sum(gamma dz xhat) / M) / std.
 //
 // Bound by HBM where the rows are larger than L2, by L2 and latency below.  Each direction looks at the rows twice, first for
-// sums, then to write the result.  The scenes are worked through in groups of up to GROUP_BYTES, a launch per look, so that the
-// second one finds the rows in L2: HBM sees them once (scenes larger than that twice).  A thread owns 16 bytes of channels and
-// walks the rows of a tile of its scene; a tile leaves one mean and one sum of squared distances from it per group (backward:
-// two sums), and each block of the second look puts the tiles of its scene together itself, in their order and in double: no
-// block waits for another and the bits are the same on every run.
-// Variances are never differences of large numbers: eight rows of a thread at a time have a mean of their own, and means are
-// put together by their differences.  A row far from all others or a mean that is large against the spread costs no precision.
+// sums, then to write the result, in ONE launch: tiles of both looks are items that blocks claim in order, a scene's second look
+// following its first one at a distance of `lag` tiles, so that it finds the rows in L2 while other blocks are at the next
+// scene's first look: HBM sees the rows once (those of scenes that do not fit L2 twice) and no multiprocessor waits between
+// looks.  (A launch a look and group of scenes of 48 MB took 529 us instead of the 869 of many short tiles for 8 x 150 000 rows
+// of 96 channels fp16, forward and backward, of which the launches' starts and ends were half.)
+// A thread owns 16 bytes of channels and walks the rows of a tile of its scene; a tile leaves one mean and one sum of squared
+// distances from it per group (backward: two sums, and two per channel); the block that leaves a scene's last tile puts the
+// tiles together, in their order and in double, and raises the scene's flag: the same bits on every run.
+// What an item waits for has been claimed before it, by blocks that are running: there is always one that can go on.  Waits are
+// bounded all the same; one that runs out sets the status word, and what could not be computed is filled with NaN.
+// Variances are never differences of large numbers: a thread's few rows of a tile have a mean of their own, about the first of
+// them, and means are put together by their differences.  A row far from all others or a mean that is large against the spread costs no precision.
 #include <string.h>
 
-#include "wcn_common.cuh"
+#include <type_traits>
+
+#include "tcgen05_common.cuh"
 
 namespace {
 
-constexpr int THREADS = 512;
-constexpr int ROWS = 8;                          // rows of a thread at a time
+constexpr int THREADS = 256;
+constexpr int BLOCKS_FORWARD = 2, BLOCKS_BACKWARD = 2;   // of a multiprocessor (128 registers a thread)
 constexpr int SCENES = 250;                      // of a launch: 2 KB of parameters
 constexpr int MAX_C = 4096;
-constexpr int64_t GROUP_BYTES = 48ll << 20;
 
 enum Act { NONE = 0, RELU = 1, SILU = 2, GELU = 3 };
 
 struct Scenes {
-  int count;
+  int count;               // with rows
+  int scene[SCENES];       // its place among all of them
   int row0[SCENES + 1];    // first row, from the launch's first row on
   int tile0[SCENES + 1];   // first tile
+};
+
+// What the blocks of a launch share, all zero before and after it.
+struct Sync {
+  int ticket, done, scenes;      // items claimed, blocks that have ended, scenes whose sums are complete
+  int tiles[SCENES], flag[SCENES];
 };
 
 struct Params {
@@ -41,14 +54,20 @@ struct Params {
   float* mean;            // [scenes][G]
   float* rstd;
   float2* part;           // [tiles][G]: (mean, sum of squared distances); backward: (sum gamma dz, sum gamma dz xhat)
-  float* channels;        // [tiles][2][C] backward: sum dz, sum dz xhat
+  float2* whole;          // [scenes][G] of all tiles: (mean, 1 / std); backward: the two sums over M
+  float* channels;        // [tiles][2][C] backward: sum dz, sum dz xhat (null: not wanted)
+  float* sums;            // [2][C] of all tiles: added to from the second launch on
   int64_t x_ld, dy_ld;
   int C, G, per;          // per: channels of a group
-  int rows;               // rows of a tile
+  int rows, each;         // rows of a tile, and of each of its threads
+  int tiles, lag, items;
+  int add;                // `sums` has something already
   float eps;
+  Sync* sync;
+  int32_t* dev_status;
 };
 
-template <typename T, int V> struct Piece { T v[V]; };
+template <typename T, int V> struct alignas(V * sizeof(T)) Piece { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ Piece<T, V> load_piece(const T* p) {
   Piece<T, V> q;
   if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(q.v) = __ldg(reinterpret_cast<const uint4*>(p));
@@ -56,39 +75,99 @@ template <typename T, int V> __device__ __forceinline__ Piece<T, V> load_piece(c
     for (int i = 0; i < V; ++i) q.v[i] = p[i];
   return q;
 }
+// Rounded two at a time (a conversion of one number goes through the slow pipe of the special functions).
+template <typename T, int V> __device__ __forceinline__ Piece<T, V> rounded(const float2 (&f)[(V + 1) / 2]) {
+  Piece<T, V> q;
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) {
+    if constexpr (V == 1) q.v[0] = wcn_from_float<T>(f[i].x);
+    else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(q.v + 2 * i) = __float22half2_rn(f[i]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(q.v + 2 * i) = __float22bfloat162_rn(f[i]);
+    else { q.v[2 * i] = f[i].x; q.v[2 * i + 1] = f[i].y; }
+  }
+  return q;
+}
+
+// The last look at a piece and what is written: not kept in L2 at the cost of rows that are to be looked at again.
+template <typename T, int V> __device__ __forceinline__ Piece<T, V> load_last(const T* p) {
+  Piece<T, V> q;
+  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(q.v) = __ldcs(reinterpret_cast<const uint4*>(p));
+  else
+    for (int i = 0; i < V; ++i) q.v[i] = p[i];
+  return q;
+}
 template <typename T, int V> __device__ __forceinline__ void store_piece(T* p, const Piece<T, V>& q) {
-  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(q.v);
+  if constexpr (V * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(q.v));
   else
     for (int i = 0; i < V; ++i) p[i] = q.v[i];
 }
 
-template <int ACT> __device__ __forceinline__ float activate(float z) {
-  if (ACT == RELU) return z > 0.f || z != z ? z : 0.f;
-  if (ACT == SILU) return __fdividef(z, 1.f + __expf(-z));
-  if (ACT == GELU) return z * 0.5f * (1.f + erff(z * 0.70710678118654752f));
+// Pairs of numbers, one instruction each.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+template <typename T, int V> __device__ __forceinline__ float2 pair_of(const Piece<T, V>& q, int i) {
+  if constexpr (V == 1) return make_float2(wcn_to_float<T>(q.v[0]), 0.f);
+  else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(q.v + 2 * i));
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(q.v + 2 * i));
+  else return make_float2(q.v[2 * i], q.v[2 * i + 1]);
+}
+// Per-channel values of a piece, from channel c on.
+template <int V> __device__ __forceinline__ float2 pair_at(const float* p, int c, float none) {
+  return p ? make_float2(__ldg(p + c), V == 1 ? none : __ldg(p + c + (V > 1))) : both(none);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + exp(-z))
+__device__ __forceinline__ float2 logistic(float2 z) {
+  const float2 e = __fmul2_rn(z, both(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(both(1.f), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+  return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+}
+// (1 + erf(z / sqrt(2))) / 2
+__device__ __forceinline__ float2 normal(float2 z) {
+  const float2 h = __fmul2_rn(z, both(0.70710678118654752f));
+  return __ffma2_rn(make_float2(erff(h.x), erff(h.y)), both(0.5f), both(0.5f));
+}
+
+template <int ACT> __device__ __forceinline__ float2 activate(float2 z) {
+  if (ACT == RELU) return make_float2(z.x > 0.f || z.x != z.x ? z.x : 0.f, z.y > 0.f || z.y != z.y ? z.y : 0.f);
+  if (ACT == SILU) return __fmul2_rn(z, logistic(z));
+  if (ACT == GELU) return __fmul2_rn(z, normal(z));
   return z;
 }
 // dy act'(z)
-template <int ACT> __device__ __forceinline__ float through(float dy, float z) {
-  if (ACT == RELU) return z > 0.f || z != z ? dy : 0.f;
+template <int ACT> __device__ __forceinline__ float2 through(float2 dy, float2 z) {
+  if (ACT == RELU) return make_float2(z.x > 0.f || z.x != z.x ? dy.x : 0.f, z.y > 0.f || z.y != z.y ? dy.y : 0.f);
   if (ACT == SILU) {
-    const float p = __fdividef(1.f, 1.f + __expf(-z));
-    return dy * (p * fmaf(z, 1.f - p, 1.f));
+    const float2 p = logistic(z), q = __ffma2_rn(p, both(-1.f), both(1.f));
+    return __fmul2_rn(dy, __fmul2_rn(p, __ffma2_rn(z, q, both(1.f))));
   }
-  if (ACT == GELU) return dy * (0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z));
+  if (ACT == GELU) {
+    const float2 e = __fmul2_rn(__fmul2_rn(z, z), both(-0.72134752044448170f));
+    const float2 density = make_float2(0.3989422804014327f * exp2_fast(e.x), 0.3989422804014327f * exp2_fast(e.y));
+    return __fmul2_rn(dy, __ffma2_rn(z, density, normal(z)));
+  }
   return dy;
 }
 
-// The scene and the rows of a block's tile.
-struct Tile { int scene, lo, hi, first, last; };   // first, last: tiles of the scene
-__device__ __forceinline__ Tile find_tile(const Scenes& s, int rows) {
+// The scene and the rows of a tile.
+struct Tile { int scene, place, lo, hi, first, last; };   // scene of the launch, its place among all; first, last: its tiles
+__device__ __forceinline__ Tile find_tile(const Scenes& s, int tile, int rows) {
   int at = 0;
   for (int hi = s.count; hi - at > 1;) {
     const int mid = (at + hi) / 2;
-    if (s.tile0[mid] <= (int)blockIdx.x) at = mid; else hi = mid;
+    if (s.tile0[mid] <= tile) at = mid; else hi = mid;
   }
-  Tile t{at, 0, 0, s.tile0[at], s.tile0[at + 1]};
-  t.lo = s.row0[at] + ((int)blockIdx.x - t.first) * rows;
+  Tile t{at, s.scene[at], 0, 0, s.tile0[at], s.tile0[at + 1]};
+  t.lo = s.row0[at] + (tile - t.first) * rows;
   t.hi = min(t.lo + rows, s.row0[at + 1]);
   return t;
 }
@@ -128,59 +207,112 @@ template <typename F> __device__ __forceinline__ void per_group(int G, F&& f) {
   for (int g0 = 0; g0 < G; g0 += THREADS / width) f(g0 + (int)threadIdx.x / width, (int)threadIdx.x % width, width);
 }
 
+// f(j, what load(j) gives) for a thread's rows, U of them loaded while the U before are worked on.
+template <int U, typename L, typename F> __device__ __forceinline__ void walk(int rows, L&& load, F&& f) {
+  decltype(load(0)) a[U], b[U];
+  int j = 0;
+  if (rows >= U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) a[u] = load(u);
+    for (;;) {
+      const bool more = j + 2 * U <= rows;
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) b[u] = load(j + U + u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(j + u, a[u]);
+      j += U;
+      if (!more) break;
+      const bool again = j + 2 * U <= rows;
+      if (again) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[u] = load(j + U + u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(j + u, b[u]);
+      j += U;
+      if (!again) break;
+    }
+  }
+  if (j == rows) return;
+#pragma unroll
+  for (int u = 0; u < U - 1; ++u)
+    if (j + u < rows) a[u] = load(j + u);
+#pragma unroll
+  for (int u = 0; u < U - 1; ++u)
+    if (j + u < rows) f(j + u, a[u]);
+}
+// Rows of a thread in a tile of n.
+__device__ __forceinline__ int rows_of(const Params& p, const Place& at, int n) {
+  return n == p.rows ? p.each : n / at.tys + (at.ty < n % at.tys);
+}
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_release(int* p, int v) { asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
+
+// Waits (one thread) until *p is `want`; false: the limit has passed, here or elsewhere.
+__device__ __noinline__ bool wait_for(const int* p, int want, int32_t* dev_status) {
+  const long long t0 = clock64();
+  for (int i = 0;; ++i) {
+    if (load_acquire(p) == want) return true;
+    if ((i & 255) == 255) {
+      if (*(volatile int32_t*)dev_status == (int)WCN_ERR_WAIT_EXPIRED) return false;
+      if (clock64() - t0 > kWaitCycles) {
+        atomicExch(dev_status, (int)WCN_ERR_WAIT_EXPIRED);
+        return false;
+      }
+    }
+  }
+}
+
 template <typename T, int V>
-__global__ void __launch_bounds__(THREADS, 2) group_stats_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) float smem[];
-  const Place at(p.C, V);
+__device__ __forceinline__ void tile_stats(const Params& p, const Place& at, const Tile& t, int tile, float* smem) {
   const int W = at.txs * V;                       // channels side by side
   float* const s_mean = smem;                     // [tys][W]
   float* const s_m2 = smem + at.tys * W;          // [tys][W]
   float* const c_mean = s_m2 + at.tys * W;        // [C]
   float* const c_m2 = c_mean + p.C;               // [C]
-  const Tile t = find_tile(scenes, p.rows);
-  const int n_tile = t.hi - t.lo, n_each = n_tile / at.tys, n_more = n_tile % at.tys;   // rows of a thread: one more for the first
+  const int n_tile = t.hi - t.lo, n_each = n_tile == p.rows ? p.each : n_tile / at.tys, n_more = n_tile - n_each * at.tys;   // rows of a thread: one more for the first
   const T* const x = reinterpret_cast<const T*>(p.x);
   for (int pc = at.tx; pc - at.tx < at.pieces; pc += at.txs) {
     if (at.ty < at.tys && pc < at.pieces) {
-      float mean[V], m2[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.f;
+      // About the thread's first row: at most 64 rows, of which a far first one spoils the others' distances by no more than
+      // its own distance counts for.
+      constexpr int P = (V + 1) / 2;
+      float2 first[P], s1[P], s2[P];     // (its negative)
+      const int rows = rows_of(p, at, n_tile);
       const int64_t step = (int64_t)at.tys * p.x_ld;
-      const T* from = x + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
-      int n = 0;
-      const int mine = n_each + (at.ty < n_more);
-      for (; n + ROWS <= mine; n += ROWS, from += ROWS * step) {
-        Piece<T, V> q[ROWS];
+      const T* const from = x + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) q[u] = load_piece<T, V>(from + u * step);
-        const float share = (float)ROWS / (float)(n + ROWS), both = share * (float)n;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float f[ROWS], sum = 0.f, d2 = 0.f;
-#pragma unroll
-          for (int u = 0; u < ROWS; ++u) { f[u] = wcn_to_float<T>(q[u].v[i]); sum += f[u]; }
-          const float mb = sum * (1.f / ROWS);
-#pragma unroll
-          for (int u = 0; u < ROWS; ++u) { const float d = f[u] - mb; d2 = fmaf(d, d, d2); }
-          const float delta = mb - mean[i];
-          mean[i] = fmaf(delta, share, mean[i]);
-          m2[i] += fmaf(delta * delta, both, d2);
-        }
-      }
-      for (; n < mine; ++n, from += step) {       // the last rows one by one
+      for (int i = 0; i < P; ++i) first[i] = s1[i] = s2[i] = both(0.f);
+      if (rows) {
         const Piece<T, V> q = load_piece<T, V>(from);
-        const float share = 1.f / (float)(n + 1), both = share * (float)n;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float delta = wcn_to_float<T>(q.v[i]) - mean[i];
-          mean[i] = fmaf(delta, share, mean[i]);
-          m2[i] = fmaf(delta * delta, both, m2[i]);
-        }
+        for (int i = 0; i < P; ++i) first[i] = __fmul2_rn(pair_of<T, V>(q, i), both(-1.f));
       }
+      walk<4>(rows, [&](int j) { return load_piece<T, V>(from + j * step); }, [&](int, const Piece<T, V>& q) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        s_mean[at.ty * W + at.tx * V + i] = mean[i];
-        s_m2[at.ty * W + at.tx * V + i] = m2[i];
+        for (int i = 0; i < P; ++i) {
+          const float2 d = __fadd2_rn(pair_of<T, V>(q, i), first[i]);
+          s1[i] = __fadd2_rn(s1[i], d);
+          s2[i] = __ffma2_rn(d, d, s2[i]);
+        }
+      });
+      const float inv = rows ? 1.f / (float)rows : 0.f;
+      auto leave = [&](int c, float first, float s1, float s2) {
+        const float d = s1 * inv;
+        s_mean[at.ty * W + at.tx * V + c] = d - first;
+        s_m2[at.ty * W + at.tx * V + c] = fmaxf(fmaf(-s1, d, s2), 0.f) + (s1 - s1);   // (NaN stays NaN)
+      };
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        leave(2 * i, first[i].x, s1[i].x, s2[i].x);
+        if (V > 1) leave(2 * i + 1, first[i].y, s1[i].y, s2[i].y);
       }
     }
     __syncthreads();
@@ -215,126 +347,160 @@ __global__ void __launch_bounds__(THREADS, 2) group_stats_kernel(const __grid_co
         m2 += fmaf(d * d, (float)n_tile, c_m2[g * p.per + c]);
       }
     m2 = sum_over(m2, width);
-    if (g < p.G && lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(m, m2);
+    if (g < p.G && lane == 0) p.part[(int64_t)tile * p.G + g] = make_float2(m, m2);
   });
 }
 
-// A piece has SUB groups side by side (V / SUB channels of one group each; V: any).
-template <typename T, int V, int ACT, int SUB>
-__global__ void __launch_bounds__(THREADS, 2) group_apply_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) float smem[];
-  float* const s_mean = smem;       // [G]
-  float* const s_rstd = smem + p.G;
-  const Place at(p.C, V);
-  const Tile t = find_tile(scenes, p.rows);
-  const int n_scene = scenes.row0[t.scene + 1] - scenes.row0[t.scene];
+// The tiles of a scene together: f(group, lane, lanes) leaves the group's values in `whole`.
+template <typename T, int V>
+__device__ __forceinline__ void join_stats(const Params& p, const Tile& t, int n_scene) {
   const int n_last = n_scene - (t.last - t.first - 1) * p.rows;
   per_group(p.G, [&](int g, int lane, int width) {
     // in one pass, about the first tile's mean: what the tiles' means differ by is no more than the spread
-    double n = 0, d1 = 0, d2 = 0;
+    double d1 = 0, d2 = 0;
     float about = 0.f;
     if (g < p.G) {
-      about = __ldg(&p.part[(int64_t)t.first * p.G + g]).x;
+      about = __ldcg(&p.part[(int64_t)t.first * p.G + g]).x;
 #pragma unroll 4
       for (int i = t.first + lane; i < t.last; i += width) {
-        const float2 v = __ldg(&p.part[(int64_t)i * p.G + g]);
+        const float2 v = __ldcg(&p.part[(int64_t)i * p.G + g]);
         const double k = (double)(i == t.last - 1 ? n_last : p.rows), d = (double)v.x - (double)about;
         d1 += k * d;
         d2 += (double)v.y + k * d * d * p.per;
       }
     }
-    n = (double)n_scene;
+    const double n = (double)n_scene;
     d1 = sum_over(d1, width) / n;
     d2 = sum_over(d2, width);
     if (g < p.G && lane == 0) {
       const double var = d2 / (n * p.per) - d1 * d1;
       const float mean = (float)((double)about + d1), rstd = (float)(1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps));
-      s_mean[g] = mean;
-      s_rstd[g] = rstd;
-      if ((int)blockIdx.x == t.first && p.mean) {
-        p.mean[(int64_t)t.scene * p.G + g] = mean;
-        p.rstd[(int64_t)t.scene * p.G + g] = rstd;
+      p.whole[(int64_t)t.scene * p.G + g] = make_float2(mean, rstd);
+      if (p.mean) {
+        p.mean[(int64_t)t.place * p.G + g] = mean;
+        p.rstd[(int64_t)t.place * p.G + g] = rstd;
       }
     }
   });
-  __syncthreads();
-  if (at.ty >= at.tys) return;
-  const T* const x = reinterpret_cast<const T*>(p.x);
-  T* const y = reinterpret_cast<T*>(p.out);
-  for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
-    float mean[SUB], scale[V], beta[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = pc * V + i, g = c / p.per;
-      mean[i * SUB / V] = s_mean[g];
-      scale[i] = s_rstd[g] * (p.gamma ? __ldg(&p.gamma[c]) : 1.f);
-      beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
-    }
-    for (int r = t.lo + at.ty; r < t.hi; r += 4 * at.tys) {
-      Piece<T, V> q[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (r + u * at.tys < t.hi) q[u] = load_piece<T, V>(x + (int64_t)(r + u * at.tys) * p.x_ld + pc * V);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (r + u * at.tys >= t.hi) break;
-        Piece<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = wcn_from_float<T>(activate<ACT>(fmaf(wcn_to_float<T>(q[u].v[i]) - mean[i * SUB / V], scale[i], beta[i])));
-        store_piece<T, V>(y + (int64_t)(r + u * at.tys) * p.C + pc * V, o);
+}
+
+__device__ __forceinline__ void join_grad_sums(const Params& p, const Tile& t, int n_scene) {
+  per_group(p.G, [&](int g, int lane, int width) {
+    double a = 0, b = 0;
+    if (g < p.G)
+#pragma unroll 4
+      for (int i = t.first + lane; i < t.last; i += width) {
+        const float2 v = __ldcg(&p.part[(int64_t)i * p.G + g]);
+        a += (double)v.x;
+        b += (double)v.y;
       }
+    a = sum_over(a, width);
+    b = sum_over(b, width);
+    if (g < p.G && lane == 0) {
+      const double inv = 1.0 / ((double)n_scene * p.per);
+      p.whole[(int64_t)t.scene * p.G + g] = make_float2((float)(a * inv), (float)(b * inv));
     }
-  }
+  });
+}
+
+// A piece has SUB groups side by side (V / SUB channels of one group each; V: any).
+// (x - mean) * scale: of 16-bit numbers as one multiplication and addition, whose rounding is far below theirs.
+template <typename T> __device__ __forceinline__ float2 centred(float2 x, float2 mean, float2 scale, float2 minus) {
+  return sizeof(T) == 2 ? __ffma2_rn(x, scale, minus) : __fmul2_rn(__fadd2_rn(x, make_float2(-mean.x, -mean.y)), scale);
+}
+// The values of a pair of channels, which may be of two of a piece's SUB groups.
+template <int V, int SUB> __device__ __forceinline__ float2 of_pair(const float (&v)[SUB], int i) {
+  return make_float2(v[2 * i * SUB / V], v[V == 1 ? 0 : (2 * i + 1) * SUB / V]);
 }
 
 template <typename T, int V, int ACT, int SUB>
-__global__ void __launch_bounds__(THREADS, 1) group_grad_sums_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) float smem[];
-  const Place at(p.C, V);
+__device__ __forceinline__ void tile_apply(const Params& p, const Place& at, const Tile& t, bool ok) {
+  constexpr int P = (V + 1) / 2;
+  if (at.ty >= at.tys) return;
+  const int rows = rows_of(p, at, t.hi - t.lo);
+  const int64_t step = (int64_t)at.tys * p.x_ld, out_step = (int64_t)at.tys * p.C;
+  for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
+    const T* const from = reinterpret_cast<const T*>(p.x) + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
+    T* const to = reinterpret_cast<T*>(p.out) + (int64_t)(t.lo + at.ty) * p.C + pc * V;
+    float mean[SUB], rstd[SUB];
+    float2 scale[P], beta[P];
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) {
+      const int g = (pc * V + k * (V / SUB)) / p.per;
+      const float2 v = ok ? __ldcg(&p.whole[(int64_t)t.scene * p.G + g]) : make_float2(__int_as_float(0x7FC00000), 1.f);
+      mean[k] = v.x;
+      rstd[k] = v.y;
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), pair_at<V>(p.gamma, pc * V + 2 * i, 1.f));
+      beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
+      const float2 m = of_pair<V, SUB>(mean, i);
+      if (sizeof(T) == 2) beta[i] = __ffma2_rn(make_float2(-m.x, -m.y), scale[i], beta[i]);
+    }
+    walk<4>(rows, [&](int j) { return load_last<T, V>(from + j * step); }, [&](int j, const Piece<T, V>& q) {
+      float2 o[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        float2 x = pair_of<T, V>(q, i);
+        const float2 m = of_pair<V, SUB>(mean, i);
+        if (sizeof(T) == 4) x = __fadd2_rn(x, make_float2(-m.x, -m.y));
+        o[i] = activate<ACT>(__ffma2_rn(x, scale[i], beta[i]));
+      }
+      store_piece<T, V>(to + j * out_step, rounded<T, V>(o));
+    });
+  }
+}
+
+template <typename T, int V> struct Pair { Piece<T, V> x, dy; };
+
+template <typename T, int V, int ACT, int SUB>
+__device__ __forceinline__ void tile_grad_sums(const Params& p, const Place& at, const Tile& t, int tile, float* smem) {
   const int W = at.txs * V;
   float* const s_a = smem;                    // [tys][W]
   float* const s_b = smem + at.tys * W;       // [tys][W]
   float* const c_a = s_b + at.tys * W;        // [C] gamma dz
   float* const c_b = c_a + p.C;               // [C] gamma dz xhat
-  const Tile t = find_tile(scenes, p.rows);
-  const T *const x = reinterpret_cast<const T*>(p.x), *const dy = reinterpret_cast<const T*>(p.dy);
   for (int pc = at.tx; pc - at.tx < at.pieces; pc += at.txs) {
     if (at.ty < at.tys && pc < at.pieces) {
-      float a[V], b[V], mean[SUB], rstd[SUB], gamma[V], beta[V];
+      const T* const x = reinterpret_cast<const T*>(p.x) + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
+      const T* const dy = reinterpret_cast<const T*>(p.dy) + (int64_t)(t.lo + at.ty) * p.dy_ld + pc * V;
+      const int64_t step = (int64_t)at.tys * p.x_ld, dy_step = (int64_t)at.tys * p.dy_ld;
+      constexpr int P = (V + 1) / 2;
+      float2 a[P], b[P], gamma[P], beta[P];
+      float mean[SUB], rstd[SUB], minus[SUB];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = pc * V + i;
-        const int64_t g = (int64_t)t.scene * p.G + c / p.per;
-        a[i] = b[i] = 0.f;
-        mean[i * SUB / V] = __ldg(&p.mean[g]);
-        rstd[i * SUB / V] = __ldg(&p.rstd[g]);
-        gamma[i] = p.gamma ? __ldg(&p.gamma[c]) : 1.f;
-        beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
+      for (int k = 0; k < SUB; ++k) {
+        const int64_t g = (int64_t)t.place * p.G + (pc * V + k * (V / SUB)) / p.per;
+        mean[k] = __ldg(&p.mean[g]);
+        rstd[k] = __ldg(&p.rstd[g]);
+        minus[k] = -mean[k] * rstd[k];
       }
-      for (int r = t.lo + at.ty; r < t.hi; r += 4 * at.tys) {
-        Piece<T, V> q[4], d[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (r + u * at.tys < t.hi) {
-            q[u] = load_piece<T, V>(x + (int64_t)(r + u * at.tys) * p.x_ld + pc * V);
-            d[u] = load_piece<T, V>(dy + (int64_t)(r + u * at.tys) * p.dy_ld + pc * V);
-          }
+      for (int i = 0; i < P; ++i) {
+        a[i] = b[i] = both(0.f);
+        gamma[i] = pair_at<V>(p.gamma, pc * V + 2 * i, 1.f);
+        beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
+      }
+      walk<2>(rows_of(p, at, t.hi - t.lo), [&](int j) { return Pair<T, V>{load_piece<T, V>(x + j * step), load_piece<T, V>(dy + j * dy_step)}; },
+              [&](int, const Pair<T, V>& q) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (r + u * at.tys >= t.hi) break;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[i * SUB / V]) * rstd[i * SUB / V];
-            const float dz = through<ACT>(wcn_to_float<T>(d[u].v[i]), fmaf(xhat, gamma[i], beta[i]));
-            a[i] += dz;
-            b[i] = fmaf(dz, xhat, b[i]);
-          }
+        for (int i = 0; i < P; ++i) {
+          const float2 xhat = centred<T>(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i), of_pair<V, SUB>(rstd, i), of_pair<V, SUB>(minus, i));
+          const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(xhat, gamma[i], beta[i]));
+          a[i] = __fadd2_rn(a[i], dz);
+          b[i] = __ffma2_rn(dz, xhat, b[i]);
         }
-      }
+      });
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        s_a[at.ty * W + at.tx * V + i] = a[i];
-        s_b[at.ty * W + at.tx * V + i] = b[i];
+      for (int i = 0; i < P; ++i) {
+        const int c = at.ty * W + at.tx * V + 2 * i;
+        s_a[c] = a[i].x;
+        s_b[c] = b[i].x;
+        if (V > 1) {
+          s_a[c + 1] = a[i].y;
+          s_b[c + 1] = b[i].y;
+        }
       }
     }
     __syncthreads();
@@ -352,8 +518,8 @@ __global__ void __launch_bounds__(THREADS, 1) group_grad_sums_kernel(const __gri
       if (!live || y0) return;
       const float gamma = p.gamma ? __ldg(&p.gamma[c0 + c]) : 1.f;
       if (p.channels) {
-        p.channels[(int64_t)blockIdx.x * 2 * p.C + c0 + c] = a;
-        p.channels[(int64_t)blockIdx.x * 2 * p.C + p.C + c0 + c] = b;
+        p.channels[(int64_t)tile * 2 * p.C + c0 + c] = a;
+        p.channels[(int64_t)tile * 2 * p.C + p.C + c0 + c] = b;
       }
       c_a[c0 + c] = gamma * a;
       c_b[c0 + c] = gamma * b;
@@ -369,96 +535,146 @@ __global__ void __launch_bounds__(THREADS, 1) group_grad_sums_kernel(const __gri
       }
     a = sum_over(a, width);
     b = sum_over(b, width);
-    if (g < p.G && lane == 0) p.part[(int64_t)blockIdx.x * p.G + g] = make_float2(a, b);
+    if (g < p.G && lane == 0) p.part[(int64_t)tile * p.G + g] = make_float2(a, b);
   });
 }
 
 template <typename T, int V, int ACT, int SUB>
-__global__ void __launch_bounds__(THREADS, 1) group_grad_apply_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) float smem[];
-  float* const s_a = smem;          // [G]
-  float* const s_b = smem + p.G;
-  const Place at(p.C, V);
-  const Tile t = find_tile(scenes, p.rows);
-  const int n_scene = scenes.row0[t.scene + 1] - scenes.row0[t.scene];
-  per_group(p.G, [&](int g, int lane, int width) {
-    double a = 0, b = 0;
-    if (g < p.G)
-#pragma unroll 4
-      for (int i = t.first + lane; i < t.last; i += width) {
-        const float2 v = __ldg(&p.part[(int64_t)i * p.G + g]);
-        a += (double)v.x;
-        b += (double)v.y;
-      }
-    a = sum_over(a, width);
-    b = sum_over(b, width);
-    if (g < p.G && lane == 0) {
-      const double inv = 1.0 / ((double)n_scene * p.per);
-      s_a[g] = (float)(a * inv);
-      s_b[g] = (float)(b * inv);
-    }
-  });
-  __syncthreads();
+__device__ __forceinline__ void tile_grad_apply(const Params& p, const Place& at, const Tile& t, bool ok) {
   if (at.ty >= at.tys) return;
-  const T *const x = reinterpret_cast<const T*>(p.x), *const dy = reinterpret_cast<const T*>(p.dy);
-  T* const dx = reinterpret_cast<T*>(p.out);
+  const int64_t step = (int64_t)at.tys * p.x_ld, dy_step = (int64_t)at.tys * p.dy_ld, out_step = (int64_t)at.tys * p.C;
   for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
-    float mean[SUB], rstd[SUB], gamma[V], beta[V], a[SUB], b[SUB];
+    const T* const x = reinterpret_cast<const T*>(p.x) + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
+    const T* const dy = reinterpret_cast<const T*>(p.dy) + (int64_t)(t.lo + at.ty) * p.dy_ld + pc * V;
+    T* const dx = reinterpret_cast<T*>(p.out) + (int64_t)(t.lo + at.ty) * p.C + pc * V;
+    constexpr int P = (V + 1) / 2;
+    float mean[SUB], rstd[SUB], minus[SUB], a[SUB], b[SUB];   // (the sums' negatives)
+    float2 gamma[P], beta[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = pc * V + i, g = c / p.per;
-      mean[i * SUB / V] = __ldg(&p.mean[(int64_t)t.scene * p.G + g]);
-      rstd[i * SUB / V] = __ldg(&p.rstd[(int64_t)t.scene * p.G + g]);
-      gamma[i] = p.gamma ? __ldg(&p.gamma[c]) : 1.f;
-      beta[i] = p.beta ? __ldg(&p.beta[c]) : 0.f;
-      a[i * SUB / V] = s_a[g];
-      b[i * SUB / V] = s_b[g];
+    for (int i = 0; i < P; ++i) {
+      gamma[i] = pair_at<V>(p.gamma, pc * V + 2 * i, 1.f);
+      beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
     }
-    for (int r = t.lo + at.ty; r < t.hi; r += 4 * at.tys) {
-      Piece<T, V> q[4], d[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (r + u * at.tys < t.hi) {
-          q[u] = load_piece<T, V>(x + (int64_t)(r + u * at.tys) * p.x_ld + pc * V);
-          d[u] = load_piece<T, V>(dy + (int64_t)(r + u * at.tys) * p.dy_ld + pc * V);
-        }
+    for (int k = 0; k < SUB; ++k) {
+      const int g = (pc * V + k * (V / SUB)) / p.per;
+      mean[k] = __ldg(&p.mean[(int64_t)t.place * p.G + g]);
+      rstd[k] = __ldg(&p.rstd[(int64_t)t.place * p.G + g]);
+      minus[k] = -mean[k] * rstd[k];
+      const float2 v = ok ? __ldcg(&p.whole[(int64_t)t.scene * p.G + g]) : make_float2(__int_as_float(0x7FC00000), 0.f);
+      a[k] = -v.x;
+      b[k] = -v.y;
+    }
+    walk<2>(rows_of(p, at, t.hi - t.lo), [&](int j) { return Pair<T, V>{load_last<T, V>(x + j * step), load_last<T, V>(dy + j * dy_step)}; },
+            [&](int j, const Pair<T, V>& q) {
+      float2 o[P];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (r + u * at.tys >= t.hi) break;
-        Piece<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int k = i * SUB / V;
-          const float xhat = (wcn_to_float<T>(q[u].v[i]) - mean[k]) * rstd[k];
-          const float dz = through<ACT>(wcn_to_float<T>(d[u].v[i]), fmaf(xhat, gamma[i], beta[i]));
-          o.v[i] = wcn_from_float<T>(rstd[k] * (fmaf(gamma[i], dz, -a[k]) - xhat * b[k]));
-        }
-        store_piece<T, V>(dx + (int64_t)(r + u * at.tys) * p.C + pc * V, o);
+      for (int i = 0; i < P; ++i) {
+        const float2 r = of_pair<V, SUB>(rstd, i);
+        const float2 xhat = centred<T>(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i), r, of_pair<V, SUB>(minus, i));
+        const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(xhat, gamma[i], beta[i]));
+        o[i] = __fmul2_rn(r, __ffma2_rn(xhat, of_pair<V, SUB>(b, i), __ffma2_rn(gamma[i], dz, of_pair<V, SUB>(a, i))));
       }
-    }
+      store_piece<T, V>(dx + j * out_step, rounded<T, V>(o));
+    });
   }
 }
 
-// Sums over the tiles: 32 channels a block, 32 tiles side by side, in double.
-__global__ void __launch_bounds__(1024) group_param_grads_kernel(const float* part, int64_t tiles, int n, float* out) {
-  __shared__ double s[32][33];
-  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+// Sums of eight channels over all tiles, 32 tiles side by side, in double.
+constexpr int JOINED = 8;
+__device__ __forceinline__ void join_channels(const Params& p, int c0, bool ok, float* smem) {
+  constexpr int SIDE = THREADS / JOINED;
+  double (*const s)[JOINED + 1] = reinterpret_cast<double(*)[JOINED + 1]>(smem);
+  const int x = threadIdx.x % JOINED, y = threadIdx.x / JOINED, n = 2 * p.C, c = c0 + x;
   double v = 0;
   if (c < n) {
 #pragma unroll 8
-    for (int64_t i = y; i < tiles; i += 32) v += (double)__ldg(&part[i * n + c]);
+    for (int i = y; i < p.tiles; i += SIDE) v += (double)__ldcg(&p.channels[(int64_t)i * n + c]);
   }
-  s[y][lane] = v;
+  s[y][x] = v;
   __syncthreads();
-  v = sum_over(s[lane][y], 32);   // (a warp a channel)
-  if (lane == 0 && blockIdx.x * 32 + y < n) out[blockIdx.x * 32 + y] = (float)v;
+  if (y || c >= n) return;
+  for (int k = 1; k < SIDE; ++k) v += s[k][x];
+  if (p.add) v += (double)p.sums[c];
+  p.sums[c] = ok ? (float)v : __int_as_float(0x7FC00000);
+}
+
+// Item k of a launch: the first look at a tile, the second one, or (backward) sums of channels behind all of them.
+struct Item { int kind, at; };
+__device__ __forceinline__ Item item_of(const Params& p, int k, bool apply) {
+  if (!apply) return k < p.tiles ? Item{0, k} : Item{2, k - p.tiles};
+  if (k < p.lag) return {0, k};
+  const int j = k - p.lag, both = 2 * (p.tiles - p.lag);
+  if (j < both) return {j & 1, (j & 1 ? 0 : p.lag) + j / 2};
+  return j - both < p.lag ? Item{1, p.tiles - p.lag + j - both} : Item{2, j - both - p.lag};
+}
+
+template <typename T, int V, int ACT, int SUB, bool BACK>
+__global__ void __launch_bounds__(THREADS, BACK ? BLOCKS_BACKWARD : BLOCKS_FORWARD) group_norm_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ int s_item, s_last, s_ok;
+  const bool apply = p.out != nullptr;
+  const Place at(p.C, V);
+  if (threadIdx.x == 0) s_item = atomicAdd(&p.sync->ticket, 1);
+  __syncthreads();
+  for (;;) {
+    const int k = s_item;
+    if (k >= p.items) break;
+    int next = 0;
+    if (threadIdx.x == 0) next = atomicAdd(&p.sync->ticket, 1);   // (arrives while this item is worked on)
+    const Item it = item_of(p, k, apply);
+    if (it.kind == 2) {
+      if (threadIdx.x == 0) s_ok = wait_for(&p.sync->scenes, scenes.count, p.dev_status);
+      __syncthreads();
+      join_channels(p, it.at * JOINED, s_ok, smem);
+    } else {
+      const Tile t = find_tile(scenes, it.at, p.rows);
+      if (it.kind == 0) {
+        if constexpr (BACK) tile_grad_sums<T, V, ACT, SUB>(p, at, t, it.at, smem);
+        else tile_stats<T, V>(p, at, t, it.at, smem);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(&p.sync->tiles[t.scene], 1) == t.last - t.first - 1;
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          const int n = scenes.row0[t.scene + 1] - scenes.row0[t.scene];
+          if constexpr (BACK) join_grad_sums(p, t, n);
+          else join_stats<T, V>(p, t, n);
+          __threadfence();
+          __syncthreads();
+          if (threadIdx.x == 0) {
+            store_release(&p.sync->flag[t.scene], 1);
+            __threadfence();
+            atomicAdd(&p.sync->scenes, 1);
+          }
+        }
+      } else {
+        if (threadIdx.x == 0) s_ok = wait_for(&p.sync->flag[t.scene], 1, p.dev_status);
+        __syncthreads();
+        if constexpr (BACK) tile_grad_apply<T, V, ACT, SUB>(p, at, t, s_ok);
+        else tile_apply<T, V, ACT, SUB>(p, at, t, s_ok);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s_item = next;
+    __syncthreads();
+  }
+  // the last block leaves everything zero
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(&p.sync->done, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  for (int i = threadIdx.x; i < (int)(sizeof(Sync) / 4); i += THREADS) reinterpret_cast<int*>(p.sync)[i] = 0;
 }
 
 // ------------------------------------------------------------------ launches
 
 struct Plan {
   int vec;       // elements of a piece
-  int tys;       // rows of a block side by side
+  int tys;       // rows of a tile side by side
 };
 
 Plan plan(int C, int elem, bool aligned) {
@@ -469,79 +685,87 @@ Plan plan(int C, int elem, bool aligned) {
   return q;
 }
 
-// Rows of a tile, for a launch over n rows: as many blocks as run at once (three times as many where scenes are short, whose
-// last tiles are smaller ones), at least four rows a thread.
-int tile_rows(int64_t n, int64_t scenes, int tys, int blocks_per_sm) {
-  const int64_t side = (int64_t)tys * blocks_per_sm * wcn_num_sms() * (scenes > 16 ? 3 : 1), per = (n + side - 1) / side;
-  return (int)((per < 4 ? 4 : per) * tys);
-}
-
 size_t sums_smem(int C, int vec) {
   const int pieces = C / vec, txs = pieces < THREADS ? pieces : THREADS, tys = THREADS / txs;
-  return ((size_t)2 * tys * txs * vec + 2 * C) * sizeof(float);
+  const size_t bytes = ((size_t)2 * tys * txs * vec + 2 * C) * sizeof(float), channels = THREADS / JOINED * (JOINED + 1) * sizeof(double);
+  return bytes > channels ? bytes : channels;
 }
 
-// The scenes in groups that stay in L2: f(first, behind the last, rows of a tile, tiles).
-template <typename F> int in_groups(const int64_t* offsets, int64_t scenes, int64_t row_bytes, bool back, int tys, F&& f) {
+// Scenes [i, j) of a launch.
+struct Part { int64_t i, j; int rows, tiles, most; };   // rows of a tile; tiles of all scenes and of the longest one
+
+// f(part) for each launch.  Tiles of up to 64 rows a thread (32 backward, where there are two numbers for each), fewer where
+// there would not be one for each block.
+template <typename F> int in_launches(const int64_t* offsets, int64_t scenes, bool back, int tys, F&& f) {
   for (int64_t i = 0; i < scenes;) {
-    int64_t j = i + 1;
-    while (j < scenes && j - i < SCENES && (offsets[j + 1] - offsets[i]) * row_bytes <= GROUP_BYTES) ++j;
-    const int rows = tile_rows(offsets[j] - offsets[i], j - i, tys, back ? 1 : 2);
-    int64_t tiles = 0;
-    for (int64_t k = i; k < j; ++k) tiles += (offsets[k + 1] - offsets[k] + rows - 1) / rows;
-    const int rc = tiles ? f(i, j, rows, (int)tiles) : WCN_OK;
+    Part q = {i, i, 0, 0, 0};
+    int count = 0;   // scenes with rows
+    for (; q.j < scenes && count < SCENES; ++q.j) count += offsets[q.j + 1] > offsets[q.j];
+    const int64_t n = offsets[q.j] - offsets[i], side = (int64_t)tys * (back ? BLOCKS_BACKWARD : BLOCKS_FORWARD) * wcn_num_sms(), per = (n + side - 1) / side;
+    const int most = back ? 32 : 64, least = 2;
+    q.rows = (int)(per < least ? least : per > most ? most : per) * tys;
+    for (int64_t k = i; k < q.j; ++k) {
+      const int tiles = (int)((offsets[k + 1] - offsets[k] + q.rows - 1) / q.rows);
+      q.tiles += tiles;
+      if (tiles > q.most) q.most = tiles;
+    }
+    i = q.j;
+    const int rc = q.tiles ? f(q) : WCN_OK;
     if (rc != WCN_OK) return rc;
-    i = j;
   }
   return WCN_OK;
 }
 
-template <typename T, int V, int ACT, int SUB> int all_groups(bool back, Params p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
-  const int64_t row_bytes = (int64_t)p.C * sizeof(T) * (back ? 2 : 1);
+template <typename T, int V, int ACT, int SUB, bool BACK> int all_launches(Params p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
   const Params base = p;
-  const size_t sums = sums_smem(p.C, V), apply = (size_t)2 * p.G * sizeof(float);
+  const size_t smem = sums_smem(p.C, V);
   const int pieces = p.C / V, tys = THREADS / (pieces < THREADS ? pieces : THREADS);
-  if (sums > 48 * 1024) {
-    auto a = group_stats_kernel<T, V>;
-    auto b = group_grad_sums_kernel<T, V, ACT, SUB>;
-    if (cudaFuncSetAttribute(a, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums) != cudaSuccess ||
-        cudaFuncSetAttribute(b, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums) != cudaSuccess)
-      return WCN_ERR_INITIALIZATION;
+  auto kern = group_norm_kernel<T, V, ACT, SUB, BACK>;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return WCN_ERR_INITIALIZATION;
   }
-  return in_groups(offsets, scenes, row_bytes, back, tys, [&](int64_t i, int64_t j, int rows, int tiles) {
-    const int64_t r = offsets[i];
+  return in_launches(offsets, scenes, BACK, tys, [&](const Part& q) {
+    const int64_t r = offsets[q.i];
     Scenes s;
-    s.count = (int)(j - i);
-    int at = 0;
-    for (int64_t k = i; k <= j; ++k) {
-      s.row0[k - i] = (int)(offsets[k] - r);
-      s.tile0[k - i] = at;
-      if (k < j) at += (int)((offsets[k + 1] - offsets[k] + rows - 1) / rows);
+    s.count = 0;
+    int at = 0;   // (mean and rstd are those of all scenes, also of the empty ones, which a launch leaves out)
+    for (int64_t k = q.i; k < q.j; ++k) {
+      if (offsets[k + 1] == offsets[k]) continue;
+      s.scene[s.count] = (int)(k - q.i);
+      s.row0[s.count] = (int)(offsets[k] - r);
+      s.tile0[s.count++] = at;
+      at += (int)((offsets[k + 1] - offsets[k] + q.rows - 1) / q.rows);
     }
-    p.rows = rows;
+      s.row0[s.count] = (int)(offsets[q.j] - r);
+    s.tile0[s.count] = at;
+    const int grid_most = (BACK ? BLOCKS_BACKWARD : BLOCKS_FORWARD) * wcn_num_sms();
+    p.rows = q.rows;
+    p.each = q.rows / tys;
+    p.tiles = q.tiles;
+    const int lag = q.most + grid_most * 5 / 8;   // (two items for each tile: what was claimed a grid of items ago is done)
+    p.lag = lag < q.tiles ? lag : q.tiles;
     p.x = reinterpret_cast<const T*>(base.x) + r * p.x_ld;
-    if (back) p.dy = reinterpret_cast<const T*>(base.dy) + r * p.dy_ld;
+    if (BACK) p.dy = reinterpret_cast<const T*>(base.dy) + r * p.dy_ld;
     p.out = base.out ? reinterpret_cast<T*>(base.out) + r * p.C : nullptr;
-    p.mean = base.mean ? base.mean + i * p.G : nullptr;
-    p.rstd = base.rstd ? base.rstd + i * p.G : nullptr;
-    if (!back) {
-      group_stats_kernel<T, V><<<tiles, THREADS, sums, st>>>(s, p);
-      group_apply_kernel<T, V, ACT, SUB><<<tiles, THREADS, apply, st>>>(s, p);
-    } else {
-      group_grad_sums_kernel<T, V, ACT, SUB><<<tiles, THREADS, sums, st>>>(s, p);
-      if (p.out) group_grad_apply_kernel<T, V, ACT, SUB><<<tiles, THREADS, apply, st>>>(s, p);
-      if (p.channels) p.channels += (int64_t)tiles * 2 * p.C;   // (the groups' sums are done with, these are not)
-    }
+    p.mean = base.mean ? base.mean + q.i * p.G : nullptr;
+    p.rstd = base.rstd ? base.rstd + q.i * p.G : nullptr;
+    p.items = (p.out ? 2 : 1) * q.tiles + (p.sums ? (2 * p.C + JOINED - 1) / JOINED : 0);
+    kern<<<p.items < grid_most ? p.items : grid_most, THREADS, smem, st>>>(s, p);
+    p.add = 1;
     return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
   });
 }
 
+template <typename T, int V, int ACT, int SUB> int by_way(bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
+  return back ? all_launches<T, V, ACT, SUB, true>(p, offsets, scenes, st) : all_launches<T, V, ACT, SUB, false>(p, offsets, scenes, st);
+}
 template <typename T, int V, int SUB> int by_act(int act, bool back, const Params& p, const int64_t* offsets, int64_t scenes, cudaStream_t st) {
   switch (act) {
-    case NONE: return all_groups<T, V, NONE, SUB>(back, p, offsets, scenes, st);
-    case RELU: return all_groups<T, V, RELU, SUB>(back, p, offsets, scenes, st);
-    case SILU: return all_groups<T, V, SILU, SUB>(back, p, offsets, scenes, st);
-    default: return all_groups<T, V, GELU, SUB>(back, p, offsets, scenes, st);
+    case NONE: return by_way<T, V, NONE, SUB>(back, p, offsets, scenes, st);
+    case RELU: return by_way<T, V, RELU, SUB>(back, p, offsets, scenes, st);
+    case SILU: return by_way<T, V, SILU, SUB>(back, p, offsets, scenes, st);
+    default: return by_way<T, V, GELU, SUB>(back, p, offsets, scenes, st);
   }
 }
 
@@ -567,18 +791,8 @@ bool norm_ok(int64_t scenes, const int64_t* offsets, int C, int G, int dtype) {
   return true;
 }
 
-// Tiles of all launches together, and of the largest one.
-void count_tiles(const int64_t* offsets, int64_t scenes, int64_t row_bytes, bool back, int tys, int64_t* all, int64_t* most) {
-  *all = *most = 0;
-  in_groups(offsets, scenes, row_bytes, back, tys, [&](int64_t, int64_t, int, int tiles) {
-    *all += tiles;
-    if (tiles > *most) *most = tiles;
-    return (int)WCN_OK;
-  });
-}
-
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool rows_on16(const void* p, int64_t ld, int elem) { return on16(p) && ld * elem % 16 == 0; }
+bool in_pieces(const void* p, int64_t ld, int elem) { return on16(p) && ld * elem % 16 == 0; }
 
 float from_bits(uint32_t b) {
   float f;
@@ -586,13 +800,19 @@ float from_bits(uint32_t b) {
   return f;
 }
 
-// Bytes of the groups' sums (of a launch), then of the channels' (of all of them).
-int64_t part_bytes(const int64_t* offsets, int64_t scenes, int C, int G, int elem, bool back, bool channels, int tys, int64_t* total) {
-  int64_t all, most;
-  count_tiles(offsets, scenes, (int64_t)C * elem * (back ? 2 : 1), back, tys, &all, &most);
-  const int64_t first = (most * G * (int64_t)sizeof(float2) + 15) / 16 * 16;
-  *total = first + (channels ? all * 2 * C * 4 : 0);
-  return first;
+// Where a launch keeps what its tiles leave: sums of the groups, of whole scenes, of the channels (backward).
+struct Room { int64_t whole, channels, bytes; };
+Room room(const int64_t* offsets, int64_t scenes, int C, int G, bool back, bool channels, int tys) {
+  int64_t most = 0;
+  in_launches(offsets, scenes, back, tys, [&](const Part& q) {
+    if (q.tiles > most) most = q.tiles;
+    return (int)WCN_OK;
+  });
+  Room r;
+  r.whole = (most * G * (int64_t)sizeof(float2) + 255) / 256 * 256;
+  r.channels = r.whole + ((scenes < SCENES ? scenes : SCENES) * G * (int64_t)sizeof(float2) + 255) / 256 * 256;
+  r.bytes = r.channels + (channels ? most * 2 * C * 4 : 0);
+  return r;
 }
 
 }  // namespace
@@ -602,29 +822,33 @@ extern "C" int wcn_group_norm_workspace_bytes(const int64_t* offsets, int64_t sc
   if (!bytes || !norm_ok(scenes, offsets, channels, groups, dtype)) return WCN_ERR_INVALID_PARAMETERS;
   int64_t most = 0;
   for (int v = 0; v < 2; ++v) {   // (whatever the rows' alignment will be)
-    int64_t need;
-    const int elem = wcn_dtype_size(dtype);
-    part_bytes(offsets, scenes, channels, groups, elem, backward, backward, plan(channels, elem, v).tys, &need);
-    if (need > most) most = need;
+    const Room r = room(offsets, scenes, channels, groups, backward, backward, plan(channels, wcn_dtype_size(dtype), v).tys);
+    if (r.bytes > most) most = r.bytes;
   }
   *bytes = most;
   return WCN_OK;
 }
 
+extern "C" int wcn_group_norm_sync_bytes(int64_t* bytes) {
+  if (!bytes) return WCN_ERR_INVALID_PARAMETERS;
+  *bytes = sizeof(Sync);
+  return WCN_OK;
+}
+
 extern "C" int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups,
                               int dtype, const float* gamma, const float* beta, uint32_t eps_bits, int act, void* y, float* mean,
-                              float* rstd, void* workspace, int64_t workspace_bytes, void* stream) {
+                              float* rstd, void* workspace, int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream) {
   if (!norm_ok(scenes, offsets, channels, groups, dtype) || act < NONE || act > GELU || x_ld < channels || !mean != !rstd)
     return WCN_ERR_INVALID_PARAMETERS;
   if (!offsets[scenes]) return WCN_OK;
-  if (!x || !y || !workspace || !on16(workspace)) return WCN_ERR_INVALID_PARAMETERS;
+  if (!x || !y || !workspace || !on16(workspace) || !sync || !dev_status) return WCN_ERR_INVALID_PARAMETERS;
   const int elem = wcn_dtype_size(dtype);
-  const Plan q = plan(channels, elem, rows_on16(x, x_ld, elem) && rows_on16(y, channels, elem));
-  int64_t need;
-  part_bytes(offsets, scenes, channels, groups, elem, false, false, q.tys, &need);
-  if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  const Plan q = plan(channels, elem, in_pieces(x, x_ld, elem) && in_pieces(y, channels, elem));
+  const Room r = room(offsets, scenes, channels, groups, false, false, q.tys);
+  if (r.bytes > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   Params p = {};
-  p.x = x; p.out = y; p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.part = (float2*)workspace;
+  p.x = x; p.out = y; p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd;
+  p.part = (float2*)workspace; p.whole = (float2*)((char*)workspace + r.whole); p.sync = (Sync*)sync; p.dev_status = dev_status;
   p.x_ld = x_ld; p.C = channels; p.G = groups; p.per = channels / groups; p.eps = from_bits(eps_bits);
   return by_dtype(dtype, q.vec, act, false, p, offsets, scenes, wcn_stream(stream));
 }
@@ -632,24 +856,22 @@ extern "C" int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offset
 extern "C" int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const int64_t* offsets,
                                        int64_t scenes, int32_t channels, int32_t groups, int dtype, const float* gamma,
                                        const float* beta, const float* mean, const float* rstd, int act, void* dx, float* sums,
-                                       void* workspace, int64_t workspace_bytes, void* stream) {
+                                       void* workspace, int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream) {
   if (!norm_ok(scenes, offsets, channels, groups, dtype) || act < NONE || act > GELU || x_ld < channels || dy_ld < channels)
     return WCN_ERR_INVALID_PARAMETERS;
   cudaStream_t st = wcn_stream(stream);
   if (!offsets[scenes]) return !sums || cudaMemsetAsync(sums, 0, (size_t)2 * channels * 4, st) == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
-  if (!x || !dy || !mean || !rstd || !workspace || !on16(workspace)) return WCN_ERR_INVALID_PARAMETERS;
+  if (!x || !dy || !mean || !rstd || !workspace || !on16(workspace) || !sync || !dev_status) return WCN_ERR_INVALID_PARAMETERS;
   const int elem = wcn_dtype_size(dtype);
-  const Plan q = plan(channels, elem, rows_on16(x, x_ld, elem) && rows_on16(dy, dy_ld, elem) && rows_on16(dx, channels, elem));
-  int64_t need;
-  const int64_t first = part_bytes(offsets, scenes, channels, groups, elem, true, sums, q.tys, &need);
-  if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
+  const Plan q = plan(channels, elem, in_pieces(x, x_ld, elem) && in_pieces(dy, dy_ld, elem) && in_pieces(dx, channels, elem));
+  const Room r = room(offsets, scenes, channels, groups, true, sums, q.tys);
+  if (r.bytes > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   Params p = {};
   p.x = x; p.dy = dy; p.out = dx; p.gamma = gamma; p.beta = beta; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
-  p.part = (float2*)workspace;
-  p.channels = sums ? (float*)((char*)workspace + first) : nullptr;
+  p.part = (float2*)workspace; p.whole = (float2*)((char*)workspace + r.whole); p.sync = (Sync*)sync; p.dev_status = dev_status;
+  p.channels = sums ? (float*)((char*)workspace + r.channels) : nullptr;
+  p.sums = sums;
   p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = channels; p.G = groups; p.per = channels / groups;
-  const int rc = by_dtype(dtype, q.vec, act, true, p, offsets, scenes, st);
-  if (rc != WCN_OK || !sums) return rc;
-  group_param_grads_kernel<<<(2 * channels + 31) / 32, 1024, 0, st>>>(p.channels, (need - first) / (2 * channels * 4), 2 * channels, sums);
-  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+  if (!dx && !sums) return WCN_OK;
+  return by_dtype(dtype, q.vec, act, true, p, offsets, scenes, st);
 }

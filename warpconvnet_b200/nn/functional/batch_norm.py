@@ -19,17 +19,18 @@ _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _counters: dict = {}
 
 
-def _counter(device: torch.device, stream: int) -> Tensor:
-    """The block counter of the reductions: zero between launches of one stream.  A launch that is being captured gets one
-    of its own, zeroed by the graph: graphs replay in any order and on any stream, and the capture's memory is theirs."""
+def _counter(device: torch.device, stream: int, words: int = 1) -> Tensor:
+    """The block counter of the reductions (``words``: of launches that share more than one word): zero between launches of one
+    stream.  A launch that is being captured gets one of its own, zeroed by the graph: graphs replay in any order and on any
+    stream, and the capture's memory is theirs."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(1, dtype=torch.int32, device=device)
-    key = (device.index, stream)
+        return torch.zeros(words, dtype=torch.int32, device=device)
+    key = (device.index, stream, words)
     hit = _counters.get(key)
     if hit is None:
         if len(_counters) >= 256:  # streams come and go; the memory of a counter returns to its own stream
             _counters.pop(next(iter(_counters)), None)
-        hit = _counters[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        hit = _counters[key] = torch.zeros(words, dtype=torch.int32, device=device)
     return hit
 
 

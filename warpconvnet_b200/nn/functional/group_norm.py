@@ -10,8 +10,8 @@ from typing import Optional, Sequence, Union
 import torch
 from torch import Tensor
 
-from ..._native import check, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
-from .batch_norm import _bits, reverse_mode_only
+from ..._native import check, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from .batch_norm import _bits, _counter, reverse_mode_only
 
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -55,6 +55,10 @@ def _workspace(offsets: array, c: int, groups: int, dtype: int, backward: bool, 
     return torch.empty(max(16, size.value), dtype=torch.uint8, device=device)
 
 
+def _sync(device, stream: int) -> Tensor:
+    return _counter(device, stream, query_bytes("wcn_group_norm_sync_bytes") // 4)
+
+
 def _forward(x: Tensor, offsets: array, groups: int, weight, bias, eps: float, act: int, keep: bool):
     """(y, mean and 1 / std of each scene and group, or None)"""
     n, c = x.shape
@@ -64,10 +68,11 @@ def _forward(x: Tensor, offsets: array, groups: int, weight, bias, eps: float, a
     scenes = len(offsets) - 1
     saved = torch.empty((2, scenes, groups), dtype=torch.float32, device=dev) if keep else None
     x, ld = _rows(x)
-    at = saved.data_ptr() if keep else None
+    at, stream = saved.data_ptr() if keep else None, stream_ptr(dev)
     with on_device(dev):
         check(lib().wcn_group_norm(ptr(x), ld, offsets.buffer_info()[0], scenes, c, groups, dc, ptr(weight), ptr(bias), _bits(eps), act, ptr(y),
-                                   at, at + 4 * scenes * groups if keep else None, ptr(ws), ws.numel(), stream_ptr(dev)), "wcn_group_norm")
+                                   at, at + 4 * scenes * groups if keep else None, ptr(ws), ws.numel(), ptr(_sync(dev, stream)),
+                                   ptr(device_status(dev)), stream), "wcn_group_norm")
     return y, saved
 
 
@@ -112,11 +117,11 @@ class _SegmentedGroupNorm(torch.autograd.Function):
         dx = torch.empty((n, c), dtype=x.dtype, device=dev) if need_x else None
         sums = torch.empty((2, c), dtype=torch.float32, device=dev) if need_w or need_b else None
         ws = _workspace(ctx.offsets, c, ctx.groups, dc, True, dev)
-        gamma, beta, at = _vector(weight), _vector(bias), saved.data_ptr()
+        gamma, beta, at, stream = _vector(weight), _vector(bias), saved.data_ptr(), stream_ptr(dev)
         with on_device(dev):
             check(lib().wcn_group_norm_backward(ptr(x), x_ld, ptr(dy), dy_ld, ctx.offsets.buffer_info()[0], scenes, c, ctx.groups, dc, ptr(gamma),
                                                 ptr(beta), at, at + 4 * scenes * ctx.groups, _ACTIVATIONS[ctx.activation], ptr(dx), ptr(sums),
-                                                ptr(ws), ws.numel(), stream_ptr(dev)), "wcn_group_norm_backward")
+                                                ptr(ws), ws.numel(), ptr(_sync(dev, stream)), ptr(device_status(dev)), stream), "wcn_group_norm_backward")
         return (dx, sums[1].to(weight.dtype) if need_w else None, sums[0].to(bias.dtype) if need_b else None) + (None,) * 4
 
 
