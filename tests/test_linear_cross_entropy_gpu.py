@@ -1,4 +1,8 @@
 """Cross entropy of a linear layer without its logits, against the formula in 64 bits."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -75,9 +79,9 @@ def test_against_the_formula(dtype, bias, n, c, v):
     check_device_status(DEV)
 
 
-def test_many_pieces():
-    """Rows and classes beyond one piece of the logits' gradient."""
-    n, c, v = 40000, 64, 8000
+@pytest.mark.parametrize("n,c,v", [(40000, 64, 8000), (60000, 96, 200), (60000, 72, 20), (50001, 128, 130), (30000, 160, 40), (100000, 32, 600)])
+def test_many_pieces(n, c, v):
+    """Rows and classes beyond one piece of the logits' gradient, and many tiles for each block."""
     x, w, labels, b = inputs(n, c, v, torch.bfloat16, True)
     mine = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
     loss = linear_cross_entropy(mine[0], mine[1], labels.to(DEV), mine[2])
@@ -266,6 +270,17 @@ def test_captured_and_on_a_stream_of_its_own():
             t.zero_()
         graph.replay()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_the_first_thing_that_a_backward_thread_does():
+    """In a process of its own: the gradient's launch is the first CUDA call of autograd's thread."""
+    code = ("import torch\nfrom warpconvnet_b200 import linear_cross_entropy\n"
+            "x = torch.randn(2000, 96, device='cuda').bfloat16().requires_grad_(True)\nw = torch.randn(20, 96, device='cuda').bfloat16()\n"
+            "loss = linear_cross_entropy(x, w, torch.zeros(2000, dtype=torch.int64, device='cuda'))\n"
+            "assert torch.isfinite(torch.autograd.grad(loss, [x], torch.ones((), device='cuda'))[0]).all()\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_module_on_a_geometry_and_under_autocast():

@@ -17,6 +17,9 @@
 
 int wcn_ce_logits_splits(int rows, int classes);
 int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st);
+int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias);
+int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
+                int32_t* dev_status, cudaStream_t st);
 int wcn_ce_product_splits(int m, int n, int k);
 int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, int dtype, int32_t* dev_status, cudaStream_t st);
 
@@ -57,34 +60,58 @@ struct LossParams {
   int32_t* dev_status;
 };
 
-template <typename T>
+// The product of a row and its label's weights: eight lanes share it in pieces of 16 bytes (VEC: rows start on such boundaries).
+template <typename T, bool VEC> __device__ __forceinline__ float share_of_dot(const T* x, const T* w, int c, int lane) {
+  constexpr int N = 16 / (int)sizeof(T);
+  float dot = 0.f;
+  int i = lane * N;
+#pragma unroll 4
+  for (; i + N <= c; i += 8 * N) {
+    __align__(16) T a[N], b[N];
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(x + i));
+      *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(w + i));
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) { a[k] = x[i + k]; b[k] = w[i + k]; }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) dot = fmaf(wcn_to_float<T>(a[k]), wcn_to_float<T>(b[k]), dot);
+  }
+  for (; i < c; ++i) dot = fmaf(wcn_to_float<T>(x[i]), wcn_to_float<T>(w[i]), dot);   // (one lane's, the last)
+  return dot;
+}
+
+// Eight lanes a row: its loss from the sums of its classes' pieces and its label's logit.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant__ LossParams p) {
   __shared__ double s_sum[THREADS / 32];
   __shared__ int s_count[THREADS / 32];
   __shared__ bool last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7;
   const bool failed = *(volatile int32_t*)p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
   double total = 0;
   int counted = 0;
   bool bad = false;
-  for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + warp; r < p.n; r += (int64_t)gridDim.x * (THREADS / 32)) {
-    const int64_t y = __ldg(&p.labels[r]);
-    const bool counts = y != p.ignore && y >= 0 && y < p.v;
-    bad |= y != p.ignore && !counts;
-    float dot = 0.f;
-    if (counts) {
-      const T *const xr = reinterpret_cast<const T*>(p.x) + r * p.x_ld, *const wr = reinterpret_cast<const T*>(p.w) + y * p.w_ld;
-      for (int c = lane; c < p.c; c += 32) dot = fmaf(wcn_to_float<T>(xr[c]), wcn_to_float<T>(wr[c]), dot);
-    }
+  const int64_t step = (int64_t)gridDim.x * (THREADS / 8);
+  int64_t r = (int64_t)blockIdx.x * (THREADS / 8) + threadIdx.x / 8;
+  int64_t y = r < p.n ? __ldg(&p.labels[r]) : p.ignore;
+  for (int64_t first = r - lane / 8; first < p.n; first += step, r += step) {   // (a warp's four rows)
+    const int64_t ahead = r + step < p.n ? __ldg(&p.labels[r + step]) : p.ignore;
+    const bool live = r < p.n, counts = live && y != p.ignore && y >= 0 && y < p.v;
+    bad |= live && y != p.ignore && !counts;
+    float dot = counts ? share_of_dot<T, VEC>(reinterpret_cast<const T*>(p.x) + r * p.x_ld, reinterpret_cast<const T*>(p.w) + y * p.w_ld, p.c, l) : 0.f;
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < p.parts; i += 32) {
-      const float2 q = __ldg(&p.part[(int64_t)i * p.n + r]);
-      const float now = fmaxf(top, q.x), by = now == -INFINITY ? 0.f : now;
-      sum = sum * exp2f(top - by) + q.y * exp2f(q.x - by);
-      top = now;
-    }
+    if (live)
+#pragma unroll 4
+      for (int i = l; i < p.parts; i += 8) {
+        const float2 q = __ldg(&p.part[(int64_t)i * p.n + r]);
+        const float now = fmaxf(top, q.x), by = now == -INFINITY ? 0.f : now;
+        sum = sum * exp2f(top - by) + q.y * exp2f(q.x - by);
+        top = now;
+      }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = 4; o; o >>= 1) {
       dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
       const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
       const float now = fmaxf(top, t), by = now == -INFINITY ? 0.f : now;
@@ -99,14 +126,20 @@ __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant_
       if (loss < 0.f) loss = 0.f;                       // (roundings of a probability of one)
     }
     if (failed) loss = __int_as_float(0x7FC00000);
-    total += (double)loss;
-    counted += counts;
-    if (lane == 0) {
+    if (live && l == 0) {
+      total += (double)loss;
+      counted += counts;
       p.lse2[r] = lse2;
       p.loss_rows[r] = loss;
     }
+    y = ahead;
   }
-  if (bad && lane == 0) wcn_report_bounds(p.dev_status);
+#pragma unroll
+  for (int o = 16; o >= 8; o >>= 1) {
+    total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    counted += __shfl_xor_sync(0xFFFFFFFFu, counted, o);
+  }
+  if (bad && l == 0) wcn_report_bounds(p.dev_status);
   if (!p.loss) return;
   if (lane == 0) { s_sum[warp] = total; s_count[warp] = counted; }
   __syncthreads();
@@ -396,7 +429,7 @@ int logit_parts(int64_t n, int64_t v, int dtype) {
   return dtype == WCN_F32 ? (int)((v + TILE - 1) / TILE) : 2 * wcn_ce_logits_splits((int)n, (int)v);
 }
 int loss_blocks(int64_t n) {
-  const int64_t want = (n + THREADS / 32 - 1) / (THREADS / 32), most = 8 * (int64_t)wcn_num_sms();
+  const int64_t want = (n + THREADS / 8 - 1) / (THREADS / 8), most = 8 * (int64_t)wcn_num_sms();
   return (int)(want < most ? want : most);
 }
 int product_splits(int m, int n, int k, int dtype) { return dtype == WCN_F32 ? fp32_splits(m, n, k) : wcn_ce_product_splits(m, n, k); }
@@ -408,6 +441,7 @@ struct Pieces {
   int rows, classes, row_pieces, class_pieces;
   int64_t g, slab_x, slab_w, slab_b, acc_x, acc_w, acc_b, bytes;
   int64_t g_ld;
+  int head;              // blocks of the kernel that needs no pieces (few classes), 0: not taken
 };
 
 int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -417,6 +451,15 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
   p.n = n; p.v = v; p.c = c; p.dtype = dtype;
   p.ld = wcn_ce_round(c, 16);
   const int e = wcn_dtype_size(dtype);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t here = at; at += aligned(bytes); return here; };
+  p.head = dtype != WCN_F32 && v <= 256 ? wcn_ce_head_blocks(n, c, (int)v, b) : 0;
+  if (p.head) {
+    p.slab_w = take(w || b ? (int64_t)p.head * v * p.ld * 4 : 0);
+    p.slab_b = take(b ? (int64_t)p.head * v * 4 : 0);
+    p.bytes = at;
+    return p;
+  }
   p.row_pieces = (int)((n + PIECE_ROWS - 1) / PIECE_ROWS);
   if (v <= 1024) {   // few classes: all of them with as many rows as there is room for
     const int64_t most = PIECE_BYTES / (e * ((v + 63) / 64 * 64)) / 128 * 128;
@@ -441,8 +484,6 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
       if (s * k * p.ld * 4 > sw) sw = s * k * p.ld * 4;
       if (s * k * 4 > sb) sb = s * k * 4;
     }
-  int64_t at = 0;
-  auto take = [&](int64_t bytes) { const int64_t here = at; at += aligned(bytes); return here; };
   p.g = take((int64_t)p.rows * p.g_ld * e);
   p.slab_x = take(x ? sx : 0);
   p.slab_w = take(w || b ? sw : 0);
@@ -469,7 +510,7 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 extern "C" int wcn_linear_ce_workspace_bytes(int64_t n, int32_t channels, int64_t classes, int dtype, int what, int64_t* bytes) {
   if (!bytes || !sizes_ok(n, channels, classes, dtype)) return WCN_ERR_INVALID_PARAMETERS;
-  if (what) *bytes = cut(n, channels, classes, dtype, what & 1, what & 2, what & 4).bytes;
+  if (what) *bytes = cut(n, channels, classes, dtype, what & 1, what & 2, what & 4).bytes + 256;   // (never none)
   else *bytes = aligned((int64_t)logit_parts(n, classes, dtype) * n * 8) + (int64_t)loss_blocks(n) * 16;
   return WCN_OK;
 }
@@ -511,9 +552,10 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   const int blocks = loss_blocks(n);
   p.block_sums = (double*)((char*)workspace + aligned((int64_t)parts * n * 8));
   p.block_counts = (int32_t*)(p.block_sums + blocks);
-  if (dtype == WCN_F32) ce_loss_kernel<float><<<blocks, THREADS, 0, st>>>(p);
-  else if (dtype == WCN_F16) ce_loss_kernel<__half><<<blocks, THREADS, 0, st>>>(p);
-  else ce_loss_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>(p);
+  if (dtype == WCN_F16) ce_loss_kernel<__half, true><<<blocks, THREADS, 0, st>>>(p);
+  else if (dtype == WCN_BF16) ce_loss_kernel<__nv_bfloat16, true><<<blocks, THREADS, 0, st>>>(p);
+  else if (on16(x) && on16(w) && x_ld % 4 == 0 && w_ld % 4 == 0) ce_loss_kernel<float, true><<<blocks, THREADS, 0, st>>>(p);
+  else ce_loss_kernel<float, false><<<blocks, THREADS, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -534,6 +576,17 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
   const int e = wcn_dtype_size(dtype);
   const float lift = lift_of(dtype);
   const wcn_ce_scale scale = {row_max ? row_max : grad, count, dtype == WCN_F16 ? 1.f / 16384.f : 1.f};
+  if (p.head) {
+    wcn_ce_piece q = {};
+    q.x = x; q.w = w; q.x_ld = x_ld; q.w_ld = w_ld; q.rows = (int)n; q.classes = (int)classes; q.channels = channels; q.bias2 = bias2;
+    q.lse2 = lse2; q.loss = loss_rows; q.labels = labels; q.ignore = ignore; q.all_classes = classes;
+    q.row_scale = row_max ? grad : nullptr; q.row_max = row_max;
+    float *const slab = dw || dbias ? (float*)(ws + p.slab_w) : nullptr, *const ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
+    int rc = wcn_ce_head(q, scale, dx, slab, ones, dtype, lift, dev_status, st);
+    if (rc == WCN_OK && dw) rc = join({slab, nullptr, false, dw, classes, channels, p.ld, p.head, scale, dev_status}, dtype, st);
+    if (rc == WCN_OK && dbias) rc = join({ones, nullptr, false, dbias, classes, 1, 1, p.head, scale, dev_status}, bias_dtype, st);
+    return rc;
+  }
   for (int i = 0; i < p.row_pieces; ++i) {
     const int64_t r0 = (int64_t)i * p.rows;
     const int rows = (int)(n - r0 < p.rows ? n - r0 : p.rows);

@@ -116,8 +116,61 @@ struct LogitParams {
   int32_t* dev_status;
 };
 
-// A thread's row over the classes of a unit.
-struct RowSum { float top, sum; };
+// Logits in units of ln 2 from W accumulators, columns `col` on; -inf behind the last class.
+template <int W> __device__ __forceinline__ void to_logits(const wcn_ce_piece& q, const uint32_t (&r)[W], int col, float (&z)[W]) {
+  if (q.bias2) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(q.bias2 + col + i));
+      z[i] = fmaf(__uint_as_float(r[i]), LOG2E, b.x);
+      z[i + 1] = fmaf(__uint_as_float(r[i + 1]), LOG2E, b.y);
+      z[i + 2] = fmaf(__uint_as_float(r[i + 2]), LOG2E, b.z);
+      z[i + 3] = fmaf(__uint_as_float(r[i + 3]), LOG2E, b.w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) z[i] = __uint_as_float(r[i]) * LOG2E;
+    if (col + W > q.classes) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (col + i >= q.classes) z[i] = -INFINITY;
+    }
+  }
+}
+
+// What the gradient of a row's logits needs: the exponent's shift (-inf: the row does not count), the gradient of its loss, its
+// label's column of the piece (-1: elsewhere) and the gradient there.
+struct RowGrad {
+  float minus, scale;
+  int label;
+};
+__device__ __forceinline__ RowGrad row_grad(const wcn_ce_piece& q, int row, float lift) {
+  RowGrad g = {-INFINITY, 1.f, -1};
+  if (row >= q.rows) return g;
+  const int64_t y = __ldg(&q.labels[row]);
+  if (y == q.ignore || y < 0 || y >= q.all_classes) return g;
+  g.minus = lift - __ldg(&q.lse2[row]);
+  const int64_t in = y - q.first_class;
+  g.label = in >= 0 && in < q.classes ? (int)in : -1;
+  if (q.row_scale) {
+    const float most = __ldg(q.row_max);
+    g.scale = most > 0.f ? __ldg(&q.row_scale[row]) / most : most == most ? 0.f : most;
+  }
+  return g;
+}
+// softmax - 1 at the label's class, from the row's loss: no difference of nearly equal numbers.
+template <bool BF16> __device__ __forceinline__ uint16_t label_grad(const wcn_ce_piece& q, const RowGrad& g, int row, float lift) {
+  const float d = expm1f(-__ldg(&q.loss[row])) * g.scale * exp2f(lift);
+  return (uint16_t)pack2<BF16>(d, d);
+}
+template <int W, bool BF16> __device__ __forceinline__ void gradients(const wcn_ce_piece& q, const RowGrad& g, const float (&z)[W], uint32_t (&out)[W / 2]) {
+#pragma unroll
+  for (int i = 0; i < W; i += 2) {
+    float a = exp2_fast(z[i] + g.minus), b = exp2_fast(z[i + 1] + g.minus);
+    if (q.row_scale) { a *= g.scale; b *= g.scale; }
+    out[i / 2] = g.minus == -INFINITY ? 0u : pack2<BF16>(a, b);   // (a row that does not count, whatever is in it)
+  }
+}
 
 template <int RES, bool GRAD, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -215,20 +268,8 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
       const int row = m * TILE_M + quarter * 32 + lane;
       const bool live = row < p.q.rows;
       float top = -INFINITY, sum = 0.f;                  // forward
-      float minus = -INFINITY, scale = 1.f;              // backward: exponent of the row, gradient of its loss
-      int label = -1;
-      if (GRAD && live) {
-        const int64_t y = __ldg(&p.q.labels[row]);
-        if (y != p.q.ignore && y >= 0 && y < p.q.all_classes) {
-          minus = p.lift - __ldg(&p.q.lse2[row]);
-          const int64_t in = y - p.q.first_class;
-          label = in >= 0 && in < p.q.classes ? (int)in : -1;
-          if (p.q.row_scale) {
-            const float most = __ldg(p.q.row_max);
-            scale = most > 0.f ? __ldg(&p.q.row_scale[row]) / most : most == most ? 0.f : most;
-          }
-        }
-      }
+      RowGrad rg = {};                                   // backward
+      if (GRAD) rg = row_grad(p.q, row, p.lift);
       for (int n = n0; n < n1; ++n) {
         if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
@@ -242,24 +283,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
           tmem_ld_wait();
           float z[W];
           const int col = col0 + c;
-          if (p.q.bias2) {
-#pragma unroll
-            for (int i = 0; i < W; i += 4) {
-              const float4 b = __ldg(reinterpret_cast<const float4*>(p.q.bias2 + col + i));
-              z[i] = fmaf(__uint_as_float(r[i]), LOG2E, b.x);
-              z[i + 1] = fmaf(__uint_as_float(r[i + 1]), LOG2E, b.y);
-              z[i + 2] = fmaf(__uint_as_float(r[i + 2]), LOG2E, b.z);
-              z[i + 3] = fmaf(__uint_as_float(r[i + 3]), LOG2E, b.w);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) z[i] = __uint_as_float(r[i]) * LOG2E;
-            if (col + W > p.q.classes) {
-#pragma unroll
-              for (int i = 0; i < W; ++i)
-                if (col + i >= p.q.classes) z[i] = -INFINITY;
-            }
-          }
+          to_logits<W>(p.q, r, col, z);
           if (!GRAD) {
             float m8[8];
 #pragma unroll
@@ -278,23 +302,13 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
             top = now;
           } else {
             uint32_t out[W / 2];
-#pragma unroll
-            for (int i = 0; i < W; i += 2) {
-              float a = exp2_fast(z[i] + minus), b = exp2_fast(z[i + 1] + minus);
-              if (p.q.row_scale) { a *= scale; b *= scale; }
-              out[i / 2] = minus == -INFINITY ? 0u : pack2<BF16>(a, b);   // (a row that does not count, whatever is in it)
-            }
+            gradients<W, BF16>(p.q, rg, z, out);
             uint16_t* const g = reinterpret_cast<uint16_t*>(p.q.g) + (int64_t)row * p.q.g_ld + col;
 #pragma unroll
             for (int i = 0; i < W / 16; ++i)
               if (live && col + 16 * i < p.q.g_ld) st_global_32B(g + 16 * i, out + 8 * i);
-            const int in = label - col;
-            if (in >= 0 && in < W) {
-              // softmax - 1 at the label's class, from the row's loss: no difference of nearly equal numbers
-              const float d = expm1f(-__ldg(&p.q.loss[row])) * scale * exp2f(p.lift);
-              const uint32_t v = pack2<BF16>(d, d);
-              g[in] = (uint16_t)v;
-            }
+            const int in = rg.label - col;
+            if (in >= 0 && in < W) g[in] = label_grad<BF16>(p.q, rg, row, p.lift);
           }
         };
         int c = first;
@@ -481,6 +495,263 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
   if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) mark();
 }
 
+// ------------------------------------------------------------------ gradients of few classes
+
+// With at most 256 classes a tile's row of logits is whole, and both products can be made of g while it is in shared memory: x is
+// read once, dx written once, and g is never in global memory.  Per 128 rows: z = x w^T; the epilogue warps write g as an operand
+// tile; dx = g w and dw += g^T x, the latter in accumulators that stay in tensor memory until the block's last tile.  The same
+// images in shared memory serve every product: a tile of rows whose channels (classes) run along 128-byte lines is a K-major
+// operand with its rows on the M / N side, or an MN-major one with its rows on the K side.
+// 240 000 x 96 x 200 classes bf16: pieces of g through global memory took 64 (g) + 39 (dx) + 33 us (dw).
+struct HeadParams {
+  wcn_ce_piece q;
+  wcn_ce_scale scale;
+  void* dx;               // [rows][channels] (null: not wanted)
+  float* slab;            // [blocks][classes][channels rounded up to 16] (null: neither dw nor dbias)
+  float* slab_ones;       // [blocks][classes] (null: no dbias)
+  int KB, NT, CN, MB;     // slices of 64 channels; classes, channels rounded up to 16; blocks of 128 classes
+  int apart;              // dx has columns of its own
+  int acc, tmem_cols;     // first column of dw
+  int tiles, vec;
+  float lift;
+  int32_t* dev_status;
+};
+
+struct HeadControl {
+  uint64_t w_full, x_full[2], x_empty[2], s_full, g_full, g_empty, dx_full, dx_read, acc_full;
+  uint32_t tmem_holder;
+  int32_t skip;
+};
+
+constexpr int ONES_BYTES = 16 * 128;
+
+template <bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ HeadParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w_slice = p.NT * 128, x_stage = p.KB * A_BYTES;
+  const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
+  const int w_at = 0, x_at = w_at + p.KB * w_slice, g_at = x_at + 2 * x_stage, ones_at = g_at + p.MB * 2 * A_BYTES, ctl_at = ones_at + ONES_BYTES;
+  uint8_t* const gen = smem_raw + pad;
+  const uint32_t base = smem_u32(smem_raw) + pad;
+  HeadControl* ctl = reinterpret_cast<HeadControl*>(gen + ctl_at);
+  const bool sums = p.slab != nullptr, with_ones = p.slab_ones != nullptr;
+  auto mark = [&]() {
+    if (!p.dx) return;
+    const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x)
+      for (int i = threadIdx.x; i < TILE_M * p.q.channels; i += THREADS) {
+        const int row = t * TILE_M + i / p.q.channels;
+        if (row < p.q.rows) reinterpret_cast<uint16_t*>(p.dx)[(int64_t)row * p.q.channels + i % p.q.channels] = nan;
+      }
+  };
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) { mark(); return; }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->x_full[i]), 1); mbar_init(bar(&ctl->x_empty[i]), 1); }
+    mbar_init(bar(&ctl->w_full), 1);
+    mbar_init(bar(&ctl->s_full), 1);
+    mbar_init(bar(&ctl->g_full), EPI_WARPS);
+    mbar_init(bar(&ctl->g_empty), 1);
+    mbar_init(bar(&ctl->dx_full), 1);
+    mbar_init(bar(&ctl->dx_read), EPI_WARPS);
+    mbar_init(bar(&ctl->acc_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u;
+  for (int i = threadIdx.x; i < ONES_BYTES / 4; i += THREADS) reinterpret_cast<uint32_t*>(gen + ones_at)[i] = one;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_holder;
+  const uint32_t dx_col = p.apart ? (uint32_t)p.NT : 0u;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      mbar_expect_tx(bar(&ctl->w_full), (uint32_t)(p.KB * w_slice));
+      for (int s = 0; s < p.KB; ++s) tma_load_2d(base + w_at + (uint32_t)(s * w_slice), &w_map, s * SLICE, 0, bar(&ctl->w_full));
+      int i = 0;
+      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
+        if (!mbar_wait(bar(&ctl->x_empty[i & 1]), ((i >> 1) & 1) ^ 1, p.dev_status)) { ok = false; break; }
+        const uint32_t full = bar(&ctl->x_full[i & 1]);
+        mbar_expect_tx(full, (uint32_t)x_stage);
+        for (int s = 0; s < p.KB; ++s) tma_load_2d(base + x_at + (uint32_t)((i & 1) * x_stage + s * A_BYTES), &x_map, s * SLICE, t * TILE_M, full);
+      }
+      if (!ok) {   // what has been issued lands before the block's shared memory is given back
+        for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->w_full), 0); ++k) {}
+        for (int j = i - 2 < 0 ? 0 : i - 2; j < i; ++j)
+          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->x_full[j & 1]), (uint32_t)((j >> 1) & 1)); ++k) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t flags = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(TILE_M >> 4) << 24);
+      const uint32_t n_s = (uint32_t)(p.NT >> 3) << 17, n_c = (uint32_t)(p.CN >> 3) << 17, n_one = 2u << 17;
+      const uint32_t id_s = flags | n_s, id_dx = flags | (1u << 16) | n_c, id_dw = flags | (1u << 15) | (1u << 16) | n_c,
+                     id_one = flags | (1u << 15) | (1u << 16) | n_one;
+      const uint64_t w_k = smem_desc<128>(base + w_at), w_mn = smem_desc_mn<128>(base + w_at, (uint32_t)w_slice);
+      const uint64_t x_k = smem_desc<128>(base + x_at), x_mn = smem_desc_mn<128>(base + x_at, A_BYTES);
+      const uint64_t g_k = smem_desc<128>(base + g_at), g_mn = smem_desc_mn<128>(base + g_at, A_BYTES), ones = smem_desc_mn<128>(base + ones_at, ONES_BYTES);
+      auto logits = [&](int i) {
+        if (!mbar_wait(bar(&ctl->x_full[i & 1]), (i >> 1) & 1, p.dev_status)) { ok = false; return; }
+        tc_fence_after();
+        for (int s = 0; s < p.KB; ++s)
+#pragma unroll
+          for (int k = 0; k < SLICE / 16; ++k)
+            umma_f16(tmem, x_k + (uint64_t)(((i & 1) * x_stage + s * A_BYTES) >> 4) + (uint64_t)(k * 2), w_k + (uint64_t)((s * w_slice) >> 4) + (uint64_t)(k * 2),
+                     id_s, (s | k) ? 1u : 0u);
+        umma_commit(bar(&ctl->s_full));
+      };
+      ok = mbar_wait(bar(&ctl->w_full), 0, p.dev_status);
+      if (ok) logits(0);
+      int i = 0;
+      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++i) {
+        const bool more = t + (int)gridDim.x < p.tiles;
+        if (!mbar_wait(bar(&ctl->g_full), i & 1, p.dev_status)) { ok = false; break; }
+        tc_fence_after();
+        if (p.dx) {
+          for (int k = 0; k < p.NT / 16; ++k)   // 16 classes a step: a chunk of 64 is 16 KB of g and 64 lines of w
+            umma_f16(tmem + dx_col, g_k + (uint64_t)(((k >> 2) * A_BYTES) >> 4) + (uint64_t)((k & 3) * 2), w_mn + (uint64_t)(k * 128), id_dx, k ? 1u : 0u);
+          umma_commit(bar(&ctl->dx_full));
+        }
+        if (more && (p.apart || !p.dx)) {
+          logits(i + 1);
+          if (!ok) break;
+        }
+        if (sums) {
+          const uint64_t x = x_mn + (uint64_t)(((i & 1) * x_stage) >> 4);
+          for (int m = 0; m < p.MB; ++m) {
+            const uint64_t g = g_mn + (uint64_t)((m * 2 * A_BYTES) >> 4);
+            const uint32_t d = tmem + (uint32_t)(p.acc + m * p.CN);
+#pragma unroll
+            for (int k = 0; k < TILE_M / 16; ++k) umma_f16(d, g + (uint64_t)(k * 128), x + (uint64_t)(k * 128), id_dw, (i | k) ? 1u : 0u);
+            if (with_ones) {
+              const uint32_t d1 = tmem + (uint32_t)(p.acc + p.MB * p.CN + m * 16);
+#pragma unroll
+              for (int k = 0; k < TILE_M / 16; ++k) umma_f16(d1, g + (uint64_t)(k * 128), ones, id_one, (i | k) ? 1u : 0u);
+            }
+          }
+        }
+        umma_commit(bar(&ctl->x_empty[i & 1]));
+        umma_commit(bar(&ctl->g_empty));
+        if (more && !p.apart && p.dx) {
+          if (!mbar_wait(bar(&ctl->dx_read), i & 1, p.dev_status)) { ok = false; break; }
+          logits(i + 1);
+        }
+      }
+      umma_commit(bar(&ctl->acc_full));
+      (void)mbar_wait(bar(&ctl->acc_full), 0, p.dev_status);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2, in_tile = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;
+    const int c_pieces = p.CN / 16, c_first = half ? (c_pieces + 1) / 2 : 0, c_last = half ? c_pieces : (c_pieces + 1) / 2;
+    float scale = 0.f;
+    if (p.dx) {
+      const int count = p.scale.count ? *p.scale.count : 1;
+      scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
+    }
+    int i = 0;
+    RowGrad next = row_grad(p.q, (int)blockIdx.x * TILE_M + in_tile, p.lift);
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
+      const int row = t * TILE_M + in_tile;
+      const RowGrad rg = next;
+      next = row_grad(p.q, t + (int)gridDim.x < p.tiles ? row + (int)gridDim.x * TILE_M : p.q.rows, p.lift);
+      if (ok) ok = mbar_wait(bar(&ctl->s_full), i & 1, p.dev_status);
+      if (ok && i) ok = mbar_wait(bar(&ctl->g_empty), (i - 1) & 1, p.dev_status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      for (int c = first; c < last; ++c) {
+        uint32_t r[16], out[8];
+        float z[16];
+        __syncwarp();
+        tmem_ld16(lanes + (uint32_t)(c * 16), r);
+        tmem_ld_wait();
+        to_logits<16>(p.q, r, c * 16, z);
+        gradients<16, BF16>(p.q, rg, z, out);
+        uint8_t* const chunk = gen + g_at + (c >> 2) * A_BYTES;
+        const int piece = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(chunk + tile_offset<128>(in_tile, piece)) = make_uint4(out[0], out[1], out[2], out[3]);
+        *reinterpret_cast<uint4*>(chunk + tile_offset<128>(in_tile, piece + 1)) = make_uint4(out[4], out[5], out[6], out[7]);
+        const int in = rg.label - c * 16;
+        if (in >= 0 && in < 16)
+          reinterpret_cast<uint16_t*>(chunk + tile_offset<128>(in_tile, piece + (in >> 3)))[in & 7] = label_grad<BF16>(p.q, rg, row, p.lift);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->g_full));
+      if (!p.dx) continue;
+      if (ok) ok = mbar_wait(bar(&ctl->dx_full), i & 1, p.dev_status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      uint16_t* const out = reinterpret_cast<uint16_t*>(p.dx) + (int64_t)row * p.q.channels;
+      for (int c = c_first; c < c_last; ++c) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld16(lanes + dx_col + (uint32_t)(c * 16), r);
+        tmem_ld_wait();
+        if (row >= p.q.rows) continue;
+        uint32_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = pack2<BF16>(__uint_as_float(r[2 * k]) * scale, __uint_as_float(r[2 * k + 1]) * scale);
+        if (p.vec && c * 16 + 16 <= p.q.channels) {
+          st_global_32B(out + c * 16, v);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (c * 16 + k < p.q.channels) out[c * 16 + k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->dx_read));
+    }
+    if (sums) {
+      __syncwarp();
+      if (ok) ok = mbar_wait(bar(&ctl->acc_full), 0, p.dev_status);
+      if (__all_sync(0xFFFFFFFFu, ok)) {
+        tc_fence_after();
+        for (int m = 0; m < p.MB; ++m) {
+          const int cls = m * 128 + in_tile;
+          const bool live = cls < p.q.classes;
+          float* const to = p.slab + ((int64_t)blockIdx.x * p.q.classes + cls) * p.CN;
+          for (int c = c_first; c < c_last; ++c) {
+            uint32_t r[16];
+            __syncwarp();
+            tmem_ld16(lanes + (uint32_t)(p.acc + m * p.CN + c * 16), r);
+            tmem_ld_wait();
+            if (!live) continue;
+            st_global_32B(to + c * 16, r);
+            st_global_32B(to + c * 16 + 8, r + 8);
+          }
+          if (with_ones && half) {
+            uint32_t r[16];
+            __syncwarp();
+            tmem_ld16(lanes + (uint32_t)(p.acc + p.MB * p.CN + m * 16), r);
+            tmem_ld_wait();
+            if (live) p.slab_ones[(int64_t)blockIdx.x * p.q.classes + cls] = __uint_as_float(r[0]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) mark();
+}
+
 template <auto KERNEL> bool allow_smem() {
   static bool configured[64] = {};   // per device
   int dev = 0;
@@ -578,7 +849,55 @@ int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
+// Whether the shapes fit, and how.
+bool plan_head(int64_t rows, int channels, int classes, bool bias, HeadParams* p, size_t* smem) {
+  if (classes > 256 || channels > 256) return false;
+  p->KB = (channels + SLICE - 1) / SLICE;
+  p->NT = wcn_ce_round(classes, 16);
+  p->CN = wcn_ce_round(channels, 16);
+  p->MB = (classes + 127) / 128;
+  const int sums = p->MB * (p->CN + (bias ? 16 : 0)), both = p->NT + p->CN, one = p->NT > p->CN ? p->NT : p->CN;
+  p->apart = both + sums <= 512;
+  p->acc = p->apart ? both : one;
+  if (p->acc + sums > 512) return false;
+  p->tmem_cols = 512;
+  p->tiles = (int)((rows + TILE_M - 1) / TILE_M);
+  *smem = 1024 + (size_t)p->KB * p->NT * 128 + 2 * (size_t)p->KB * A_BYTES + (size_t)p->MB * 2 * A_BYTES + ONES_BYTES + sizeof(HeadControl) + 128;
+  return *smem <= SMEM_BUDGET;
+}
+
+template <bool BF16> int launch_head(HeadParams& p, size_t smem, int blocks, cudaStream_t st) {
+  CUtensorMap xm, wm;
+  if (!matrix_map(&xm, p.q.x, p.q.rows, p.q.channels, p.q.x_ld * 2, TILE_M, BF16) ||
+      !matrix_map(&wm, p.q.w, p.q.classes, p.q.channels, p.q.w_ld * 2, p.NT, BF16))
+    return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = ce_head_kernel<BF16>;
+  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
+  kern<<<blocks, THREADS, smem, st>>>(xm, wm, p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
 }  // namespace
+
+// Blocks, and with them slabs, of the kernel for few classes; 0: not taken.
+int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias) {
+  HeadParams p = {};
+  size_t smem;
+  if (!plan_head(rows, channels, classes, bias, &p, &smem)) return 0;
+  const int sms = wcn_num_sms();
+  return p.tiles < sms ? p.tiles : sms;
+}
+
+int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
+                int32_t* dev_status, cudaStream_t st) {
+  HeadParams p = {};
+  size_t smem;
+  if (!plan_head(q.rows, q.channels, q.classes, slab_ones, &p, &smem)) return WCN_ERR_UNSUPPORTED_CONFIG;
+  p.q = q; p.scale = scale; p.dx = dx; p.slab = slab; p.slab_ones = slab_ones; p.lift = lift; p.dev_status = dev_status;
+  p.vec = reinterpret_cast<uintptr_t>(dx) % 32 == 0 && q.channels * 2 % 32 == 0;
+  const int sms = wcn_num_sms(), blocks = p.tiles < sms ? p.tiles : sms;
+  return dtype == WCN_BF16 ? launch_head<true>(p, smem, blocks, st) : launch_head<false>(p, smem, blocks, st);
+}
 
 int wcn_ce_logits_splits(int rows, int classes) {
   LogitParams p = {};

@@ -37,6 +37,10 @@ inline EncodeTiledFn encode_tiled() {
       fn = reinterpret_cast<EncodeTiledFn>(sym);
     tried = true;
   }
+  // Driver calls want a context that is current to the calling thread, which a thread that has made no runtime call yet (one of
+  // autograd's) does not have.
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) (void)cudaSetDevice(dev);
   return fn;
 }
 
