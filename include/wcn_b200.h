@@ -635,26 +635,22 @@ int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, int32_t chann
 
 /* ------------------------------------------------------------------ AdamW over many tensors */
 
-/* One tensor of wcn_adamw_step: n elements of a parameter and its gradient (contiguous), the first element of its moments
- * (a multiple of 256; each tensor's moments fill whole blocks of 256) and its place in `steps`. */
-typedef struct {
-  void* param;
-  const void* grad;
-  int64_t n, slot, step;
-} wcn_adamw_tensor;
-
-/* One decoupled-weight-decay Adam step of all tensors (a host array, read during the call), in fp32.  exp_avg / exp_avg_sq hold
+/* One decoupled-weight-decay Adam step of `count` tensors, in fp32.  The host arrays, read during the call, hold the addresses of the
+ * parameters and gradients (contiguous), their elements, the first element of each tensor's moments (a multiple of 256; NULL: one
+ * after the other; each tensor's moments fill whole blocks of 256) and its place in `steps` (NULL: its own).  exp_avg / exp_avg_sq hold
  * the moments of all tensors, 32-byte aligned: fp32, or with the two base arrays (one int16 per 256 elements) 8-bit codes: the
  * code k > 0 stands for the fp32 number with the bits (k + base) << 20, 0 for zero; exp_avg has a sign in its top bit.  Codes
  * are rounded at random with a hash of step and place; the elements behind a tensor's end must be zero codes and stay so.
+ * WCN_ERR_BOUNDS: they need more than the `length` elements or `num_steps` steps that there are.
  * steps (device): the steps made before this one, advanced by it.  lr_bits .. weight_decay_bits: the bits of doubles; lr (a
  * device float, may be NULL) stands for lr_bits.  Gradients are divided by *grad_scale (NULL: 1); *found_inf != 0 cancels
  * the step.  counter: one zero word, zero again afterwards (one per stream).  More than 640 tensors are several launches.
  * The reference leaves the update to torch's optimizers; this stands for torch.optim.AdamW. */
-int wcn_adamw_step(const wcn_adamw_tensor* tensors, int64_t count, int dtype, int grad_dtype, void* exp_avg,
-                   int16_t* exp_avg_base, void* exp_avg_sq, int16_t* exp_avg_sq_base, int32_t* steps, int64_t lr_bits,
-                   int64_t beta1_bits, int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits, const float* lr,
-                   const float* grad_scale, const float* found_inf, uint32_t* counter, void* stream);
+int wcn_adamw_step(const int64_t* params, const int64_t* grads, const int64_t* sizes, const int64_t* slots, const int64_t* step_at,
+                   int64_t count, int dtype, int grad_dtype, void* exp_avg, int16_t* exp_avg_base, void* exp_avg_sq,
+                   int16_t* exp_avg_sq_base, int64_t length, int32_t* steps, int64_t num_steps, int64_t lr_bits, int64_t beta1_bits,
+                   int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits, const float* lr, const float* grad_scale,
+                   const float* found_inf, uint32_t* counter, void* stream);
 /* The numbers that n codes of either moment stand for (n: a multiple of 256). */
 int wcn_adamw_decode(const void* exp_avg, const int16_t* exp_avg_base, const void* exp_avg_sq, const int16_t* exp_avg_sq_base,
                      int64_t n, float* exp_avg_out, float* exp_avg_sq_out, void* stream);

@@ -29,7 +29,7 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int CODES = 256;                                   // elements of a code block: a warp's
 constexpr int CHUNK = THREADS / 32 * CODES;                  // elements of a thread block
-constexpr int FEW = 48, MANY = 640;                          // tensors of a launch: 2 KB and 26 KB of parameters
+constexpr int FEW = 48, SOME = 240, MANY = 640;              // tensors of a launch: 2, 10 and 26 KB of parameters
 
 struct Tensor {
   void* param;
@@ -91,11 +91,12 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int64_t left,
   }
 }
 
-// (one part in 2^22 of an update)
-__device__ __forceinline__ float sqrt_fast(float x) {
-  float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// m / (sqrt(v) * root + eps), to one part in 2^21 of an update.
+__device__ __forceinline__ float quotient(float m, float v, float root, float eps) {
+  float s, r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(s, root, eps)));
+  return m * r;
 }
 
 __device__ __forceinline__ float code_value(uint32_t k, uint32_t base) { return k ? __uint_as_float((k + base) << 20) : 0.f; }
@@ -108,20 +109,38 @@ __device__ __forceinline__ uint32_t code_base(uint32_t top_bits, uint32_t codes)
 }
 __device__ __forceinline__ uint32_t code_limit(uint32_t top_bits) { return top_bits < 0x7F800000u ? 0x7F7u : 0x7FFu; }
 
-__device__ __forceinline__ uint32_t pack_m(float x, uint32_t random, uint32_t base, uint32_t limit) {
-  const uint32_t bits = __float_as_uint(x) & 0x7FFFFFFFu;
-  const uint32_t q = min((bits + random) >> 20, limit);
-  uint32_t k = q - base;
-  if (q <= base && base) {
-    const float first = __uint_as_float((base + 1) << 20);
-    k = __uint_as_float(bits) > __fmul_rn(first, __fmul_rn((float)random, 9.5367431640625e-7f)) ? 1 : 0;   // 2^-20
+// Codes of a lane's eight numbers (bits of the magnitudes), one a byte, given 20 random bits for each.  `signs`: the first
+// moment, whose sign is the code's top bit.
+template <bool SIGNS> __device__ __forceinline__ uint2 pack8(const float (&x)[8], const uint32_t (&random)[8], uint32_t base, uint32_t top_bits) {
+  uint32_t k[8];
+  bool low = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu, q = (bits + random[i]) >> 20;
+    k[i] = q - base;
+    if (SIGNS) low |= q <= base;
+    else k[i] = bits ? (uint32_t)max((int)k[i], 1) : 0u;
   }
-  return k | (x < 0.f ? 128u : 0u);
-}
-__device__ __forceinline__ uint32_t pack_v(float x, uint32_t random, uint32_t base, uint32_t limit) {
-  const uint32_t bits = __float_as_uint(x) & 0x7FFFFFFFu;
-  const uint32_t q = min((bits + random) >> 20, limit);
-  return !bits ? 0u : q > base ? q - base : 1u;
+  // rare, and the same for a warp: numbers below the first code (first moment), numbers near the end of fp32
+  if (SIGNS && base && __any_sync(0xFFFFFFFFu, low)) {
+    const float first = __uint_as_float((base + 1) << 20);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+      if (((bits + random[i]) >> 20) <= base) k[i] = __uint_as_float(bits) > __fmul_rn(first, __fmul_rn((float)random[i], 9.5367431640625e-7f)) ? 1 : 0;   // 2^-20
+    }
+  }
+  if (top_bits >= 0x7F600000u) {
+    const uint32_t most = code_limit(top_bits) - base;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = min(k[i], most);
+  }
+  if (SIGNS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] |= (__float_as_uint(x[i]) >> 24) & 128u;
+  }
+  auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); };
+  return make_uint2(four(k[0], k[1], k[2], k[3]), four(k[4], k[5], k[6], k[7]));
 }
 
 template <typename P, typename G, bool EIGHT, int MAX>
@@ -187,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
     const float d = h.grad_scale ? g[i] * inv : g[i];
     m[i] = __fadd_rn(__fmul_rn(m[i], h.b1), __fmul_rn(d, h.b1c));
     v[i] = __fadd_rn(__fmul_rn(v[i], h.b2), __fmul_rn(__fmul_rn(d, d), h.b2c));
-    p[i] = p[i] * keep - size * __fdividef(m[i], fmaf(sqrt_fast(v[i]), root, h.eps));
+    p[i] = p[i] * keep - size * quotient(m[i], v[i], root, h.eps);
     m_top = max(m_top, __float_as_uint(m[i]) & 0x7FFFFFFFu);
     v_top = max(v_top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
   }
@@ -195,16 +214,16 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
   if (EIGHT) {
     m_top = __reduce_max_sync(0xFFFFFFFFu, m_top);
     v_top = __reduce_max_sync(0xFFFFFFFFu, v_top);
-    const uint32_t mb = code_base(m_top, 127), vb = code_base(v_top, 255), ml = code_limit(m_top), vl = code_limit(v_top);
-    uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+    const uint32_t mb = code_base(m_top, 127), vb = code_base(v_top, 255);
+    uint32_t for_m[8], for_v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t random = wcn_fmix32((uint32_t)(s + i) * 0x9E3779B9u ^ salt);
-      cm[i / 4] |= pack_m(m[i], random >> 12, mb, ml) << (i % 4 * 8);
-      cv[i / 4] |= pack_v(v[i], (random * 0x9E3779B1u) >> 12, vb, vl) << (i % 4 * 8);
+      for_m[i] = random >> 12;
+      for_v[i] = (random * 0x9E3779B1u) >> 12;
     }
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(h.m) + s) = make_uint2(cm[0], cm[1]);
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(h.v) + s) = make_uint2(cv[0], cv[1]);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(h.m) + s) = pack8<true>(m, for_m, mb, m_top);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(h.v) + s) = pack8<false>(v, for_v, vb, v_top);
     if ((threadIdx.x & 31) == 0) {
       h.m_base[s / CODES] = (int16_t)mb;
       h.v_base[s / CODES] = (int16_t)vb;
@@ -243,41 +262,49 @@ int launch(const Tensor* t, Hyper& h, int count, unsigned blocks, cudaStream_t s
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
+// What a call is given of its tensors.
+struct Given {
+  const int64_t *params, *grads, *sizes, *slots, *step_at;   // slots, step_at: null: one after the other
+  int64_t count;
+};
+
 template <typename P, typename G, bool EIGHT>
-int run(const wcn_adamw_tensor* tensors, int64_t count, Hyper& h, cudaStream_t st) {
+int run(const Given& a, Hyper& h, cudaStream_t st) {
   Tensor t[MANY];
-  for (int64_t i = 0; i < count;) {
+  int64_t slot = 0;
+  for (int64_t i = 0; i < a.count;) {
     int k = 0;
     int64_t blocks = 0;
-    for (; i < count && k < MANY; ++i) {
-      const int64_t need = (tensors[i].n + CHUNK - 1) / CHUNK;
-      if (!need) continue;
+    for (; i < a.count && k < MANY; ++i) {
+      const int64_t n = a.sizes[i], need = (n + CHUNK - 1) / CHUNK;
       if (blocks + need > 0x7FFFFFFF) break;
-      t[k++] = {tensors[i].param, tensors[i].grad, tensors[i].n, tensors[i].slot, (int32_t)tensors[i].step, (int32_t)blocks};
+      if (need) t[k++] = {(void*)a.params[i], (const void*)a.grads[i], n, a.slots ? a.slots[i] : slot, (int32_t)(a.step_at ? a.step_at[i] : i), (int32_t)blocks};
       blocks += need;
+      slot += (n + CODES - 1) / CODES * CODES;
     }
     if (!k) {
-      if (i < count) return WCN_ERR_INVALID_PARAMETERS;      // (one tensor of 2^42 elements)
+      if (i < a.count) return WCN_ERR_INVALID_PARAMETERS;    // (one tensor of 2^42 elements)
       break;
     }
-    const int rc = k <= FEW ? launch<P, G, EIGHT, FEW>(t, h, k, (unsigned)blocks, st) : launch<P, G, EIGHT, MANY>(t, h, k, (unsigned)blocks, st);
+    const int rc = k <= FEW ? launch<P, G, EIGHT, FEW>(t, h, k, (unsigned)blocks, st) : k <= SOME ? launch<P, G, EIGHT, SOME>(t, h, k, (unsigned)blocks, st)
+                                                                                                   : launch<P, G, EIGHT, MANY>(t, h, k, (unsigned)blocks, st);
     if (rc != WCN_OK) return rc;
   }
   return WCN_OK;
 }
 
 template <typename P, bool EIGHT>
-int by_grad(int dtype, const wcn_adamw_tensor* t, int64_t count, Hyper& h, cudaStream_t st) {
-  if (dtype == WCN_F32) return run<P, float, EIGHT>(t, count, h, st);
-  if (dtype == WCN_F16) return run<P, __half, EIGHT>(t, count, h, st);
-  return run<P, __nv_bfloat16, EIGHT>(t, count, h, st);
+int by_grad(int dtype, const Given& a, Hyper& h, cudaStream_t st) {
+  if (dtype == WCN_F32) return run<P, float, EIGHT>(a, h, st);
+  if (dtype == WCN_F16) return run<P, __half, EIGHT>(a, h, st);
+  return run<P, __nv_bfloat16, EIGHT>(a, h, st);
 }
 
 template <bool EIGHT>
-int by_param(int dtype, int grad_dtype, const wcn_adamw_tensor* t, int64_t count, Hyper& h, cudaStream_t st) {
-  if (dtype == WCN_F32) return by_grad<float, EIGHT>(grad_dtype, t, count, h, st);
-  if (dtype == WCN_F16) return by_grad<__half, EIGHT>(grad_dtype, t, count, h, st);
-  return by_grad<__nv_bfloat16, EIGHT>(grad_dtype, t, count, h, st);
+int by_param(int dtype, int grad_dtype, const Given& a, Hyper& h, cudaStream_t st) {
+  if (dtype == WCN_F32) return by_grad<float, EIGHT>(grad_dtype, a, h, st);
+  if (dtype == WCN_F16) return by_grad<__half, EIGHT>(grad_dtype, a, h, st);
+  return by_grad<__nv_bfloat16, EIGHT>(grad_dtype, a, h, st);
 }
 
 bool on32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
@@ -290,20 +317,27 @@ double number(int64_t bits) {
 
 }  // namespace
 
-extern "C" int wcn_adamw_step(const wcn_adamw_tensor* tensors, int64_t count, int dtype, int grad_dtype, void* exp_avg,
-                              int16_t* exp_avg_base, void* exp_avg_sq, int16_t* exp_avg_sq_base, int32_t* steps, int64_t lr_bits,
-                              int64_t beta1_bits, int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits,
+extern "C" int wcn_adamw_step(const int64_t* params, const int64_t* grads, const int64_t* sizes, const int64_t* slots,
+                              const int64_t* step_at, int64_t count, int dtype, int grad_dtype, void* exp_avg, int16_t* exp_avg_base,
+                              void* exp_avg_sq, int16_t* exp_avg_sq_base, int64_t length, int32_t* steps, int64_t num_steps,
+                              int64_t lr_bits, int64_t beta1_bits, int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits,
                               const float* lr, const float* grad_scale, const float* found_inf, uint32_t* counter, void* stream) {
-  if (count < 0 || (count && (!tensors || !exp_avg || !exp_avg_sq || !steps || !counter)) || dtype < WCN_F32 || dtype > WCN_BF16 ||
-      grad_dtype < WCN_F32 || grad_dtype > WCN_BF16 || !on32(exp_avg) || !on32(exp_avg_sq) || !exp_avg_base != !exp_avg_sq_base)
+  if (count < 0 || (count && (!params || !grads || !sizes || !counter || (length && (!exp_avg || !exp_avg_sq)) || (num_steps && !steps))) || dtype < WCN_F32 ||
+      dtype > WCN_BF16 || grad_dtype < WCN_F32 || grad_dtype > WCN_BF16 || !on32(exp_avg) || !on32(exp_avg_sq) || !exp_avg_base != !exp_avg_sq_base)
     return WCN_ERR_INVALID_PARAMETERS;
   const double b1 = number(beta1_bits), b2 = number(beta2_bits);
   if (!(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1)) return WCN_ERR_INVALID_PARAMETERS;
-  for (int64_t i = 0; i < count; ++i)
-    if (tensors[i].n < 0 || (tensors[i].n && (!tensors[i].param || !tensors[i].grad)) || tensors[i].slot < 0 || tensors[i].slot % CODES ||
-        tensors[i].step < 0 || tensors[i].step > 0x7FFFFFFF ||
-        reinterpret_cast<uintptr_t>(tensors[i].param) % wcn_dtype_size(dtype) || reinterpret_cast<uintptr_t>(tensors[i].grad) % wcn_dtype_size(grad_dtype))
+  int64_t slot = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t n = sizes[i], at = step_at ? step_at[i] : i;
+    if (slots) slot = slots[i];
+    if (n < 0 || (n && (!params[i] || !grads[i])) || params[i] % wcn_dtype_size(dtype) || grads[i] % wcn_dtype_size(grad_dtype) || slot < 0 ||
+        slot % CODES || at < 0 || at > 0x7FFFFFFF)
       return WCN_ERR_INVALID_PARAMETERS;
+    slot += (n + CODES - 1) / CODES * CODES;
+    if (slot > length || at >= num_steps) return WCN_ERR_BOUNDS;
+  }
+  const Given a = {params, grads, sizes, slots, step_at, count};
   Hyper h = {};
   h.m = exp_avg; h.v = exp_avg_sq; h.m_base = exp_avg_base; h.v_base = exp_avg_sq_base; h.steps = steps;
   h.lr_at = lr; h.grad_scale = grad_scale; h.found_inf = found_inf; h.counter = counter;
@@ -311,7 +345,7 @@ extern "C" int wcn_adamw_step(const wcn_adamw_tensor* tensors, int64_t count, in
   h.b1 = (float)b1; h.b1c = (float)(1 - b1); h.b2 = (float)b2; h.b2c = (float)(1 - b2);
   h.log_b1 = (float)log(b1); h.log_b2 = (float)log(b2);
   cudaStream_t st = wcn_stream(stream);
-  return exp_avg_base ? by_param<true>(dtype, grad_dtype, tensors, count, h, st) : by_param<false>(dtype, grad_dtype, tensors, count, h, st);
+  return exp_avg_base ? by_param<true>(dtype, grad_dtype, a, h, st) : by_param<false>(dtype, grad_dtype, a, h, st);
 }
 
 extern "C" int wcn_adamw_decode(const void* exp_avg, const int16_t* exp_avg_base, const void* exp_avg_sq,

@@ -30,7 +30,7 @@ def _host_offsets(offsets: Union[Tensor, Sequence[int], None], n: int) -> array:
     if isinstance(offsets, Tensor):
         if offsets.dim() != 1 or offsets.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"offsets must be a 1-d integer tensor [scenes + 1], got {tuple(offsets.shape)} {offsets.dtype}")
-        offsets = offsets.tolist()
+        offsets = offsets.detach().to(device="cpu", dtype=torch.int64).numpy().tobytes()
     try:
         at = array("q", offsets)
     except (TypeError, OverflowError):

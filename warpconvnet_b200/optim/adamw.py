@@ -36,7 +36,12 @@ def moment_slots(sizes: Sequence[int]) -> Tuple[List[int], int]:
     return out[:-1], out[-1]
 
 
-_dtype, _layout, _shape = attrgetter("dtype"), attrgetter("layout"), attrgetter("shape")
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_BOUNDS = -8   # a status of the library
+
+
+def _at(a: Optional[array]) -> Optional[int]:
+    return None if a is None else a.buffer_info()[0]
 
 
 def _one(kinds: set, what: str):
@@ -69,7 +74,6 @@ def _moments(m: Tensor, v: Tensor, m_base: Optional[Tensor], v_base: Optional[Te
     return n
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tensor, exp_avg_sq: Tensor, steps: Tensor, *,
                lr: Union[float, Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                exp_avg_base: Optional[Tensor] = None, exp_avg_sq_base: Optional[Tensor] = None, slots: Optional[Sequence[int]] = None,
@@ -89,47 +93,53 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tenso
     # (a network has hundreds of tensors: each look at all of them is one pass of a C function)
     device, dtype = params[0].device, _one(set(map(_dtype, params)), "dtypes of the parameters")
     require_cuda(params[0], "params")
-    if set(map(_layout, grads)) != {torch.strided}:
-        raise TypeError("gradients must be dense")
     grad_dtype = _one(set(map(_dtype, grads)), "dtypes of the gradients")
     codes = dtype_code(dtype), dtype_code(grad_dtype)
     if set(map(Tensor.get_device, params)) != {device.index} or set(map(Tensor.get_device, grads)) != {device.index}:
         raise ValueError(f"all parameters and gradients must be on {device}")
-    if not all(map(Tensor.is_contiguous, params)):
-        raise ValueError("parameters must be contiguous: they are updated in place")
     if not all(map(eq, map(_shape, params), map(_shape, grads))):
         raise ValueError("a gradient has another shape than its parameter")
-    sizes = list(map(Tensor.numel, params))
+    try:
+        if not all(map(Tensor.is_contiguous, params)):
+            raise ValueError("parameters must be contiguous: they are updated in place")
+        if not all(map(Tensor.is_contiguous, grads)):
+            grads = [g.detach().contiguous() for g in grads]
+        at_params, at_grads = array("q", map(Tensor.data_ptr, params)), array("q", map(Tensor.data_ptr, grads))
+    except (NotImplementedError, RuntimeError):
+        if all(t.layout == torch.strided for t in chain(params, grads)):
+            raise
+        raise TypeError("parameters and gradients must be dense") from None
+    sizes = array("q", map(Tensor.numel, params))
     length = _moments(exp_avg, exp_avg_sq, exp_avg_base, exp_avg_sq_base, device)
-    if slots is None:
-        slots, need = moment_slots(sizes)
-    else:
-        if len(slots) != len(params) or any(s % BLOCK or s < 0 for s in slots):
-            raise ValueError(f"slots must be {len(params)} multiples of {BLOCK}")
-        need = max([s + -(-n // BLOCK) * BLOCK for s, n in zip(slots, sizes)])
-    if need > length:
-        raise ValueError(f"the moments have {length} elements, the tensors need {need}")
-    if step_index is None:
-        step_index = range(len(params))
+    for places, name in ((slots, "slots"), (step_index, "step_index")):
+        if places is not None and len(places) != len(params):
+            raise ValueError(f"{name} has {len(places)} places for {len(params)} tensors")
+    if slots is not None:
+        slots = array("q", slots)
+        if any([s % BLOCK or s < 0 for s in slots]):
+            raise ValueError(f"slots must be multiples of {BLOCK}")
+    if step_index is not None:
+        step_index = array("q", step_index)
+        if min(step_index) < 0:
+            raise ValueError("step_index must not be negative")
     if steps.dtype != torch.int32 or steps.device != device or not steps.is_contiguous():
         raise ValueError(f"steps must be contiguous int32 on {device}, got {steps.dtype} on {steps.device}")
-    if len(step_index) != len(params) or min(step_index) < 0 or max(step_index) >= steps.numel():
-        raise ValueError(f"steps has {steps.numel()} elements: not a place for each of {len(params)} tensors")
     lr_at = None
     if isinstance(lr, Tensor):
         if lr.is_cuda:
             lr_at, lr = _scalar(lr, "lr", device), 0.0
         else:
             lr = float(lr)
-    if not all(map(Tensor.is_contiguous, grads)):
-        grads = [g.contiguous() for g in grads]
-    table = array("q", chain.from_iterable(zip(map(Tensor.data_ptr, params), map(Tensor.data_ptr, grads), sizes, slots, step_index)))
     stream = stream_ptr(device)
     with on_device(device):
-        check(lib().wcn_adamw_step(table.buffer_info()[0], len(params), *codes, ptr(exp_avg), ptr(exp_avg_base), ptr(exp_avg_sq),
-                                   ptr(exp_avg_sq_base), ptr(steps), _bits(lr), _bits(betas[0]), _bits(betas[1]), _bits(eps),
-                                   _bits(weight_decay), lr_at, _scalar(grad_scale, "grad_scale", device),
-                                   _scalar(found_inf, "found_inf", device), ptr(_counter(device, stream)), stream), "wcn_adamw_step")
+        status = lib().wcn_adamw_step(_at(at_params), _at(at_grads), _at(sizes), _at(slots), _at(step_index), len(params), *codes, ptr(exp_avg),
+                                      ptr(exp_avg_base), ptr(exp_avg_sq), ptr(exp_avg_sq_base), length, ptr(steps), steps.numel(), _bits(lr),
+                                      _bits(betas[0]), _bits(betas[1]), _bits(eps), _bits(weight_decay), lr_at,
+                                      _scalar(grad_scale, "grad_scale", device), _scalar(found_inf, "found_inf", device),
+                                      ptr(_counter(device, stream)), stream)
+    if status == _BOUNDS:
+        raise ValueError(f"the tensors need more than the {length} elements of the moments or the {steps.numel()} of steps")
+    check(status, "wcn_adamw_step")
     torch.autograd.graph.increment_version(params)
 
 
