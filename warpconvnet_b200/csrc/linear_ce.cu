@@ -15,7 +15,7 @@
 // products at a time.
 #include "linear_ce.cuh"
 
-int wcn_ce_logits_splits(int rows, int classes);
+int wcn_ce_logits_parts(int rows, int classes);
 int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st);
 int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias);
 int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
@@ -426,7 +426,7 @@ int fp32_product(const wcn_ce_product& q, bool transposed, cudaStream_t st) {
 // ------------------------------------------------------------------ plans
 
 int logit_parts(int64_t n, int64_t v, int dtype) {
-  return dtype == WCN_F32 ? (int)((v + TILE - 1) / TILE) : 2 * wcn_ce_logits_splits((int)n, (int)v);
+  return dtype == WCN_F32 ? (int)((v + TILE - 1) / TILE) : wcn_ce_logits_parts((int)n, (int)v);
 }
 int loss_blocks(int64_t n) {
   const int64_t want = (n + THREADS / 8 - 1) / (THREADS / 8), most = 8 * (int64_t)wcn_num_sms();

@@ -16,7 +16,7 @@ struct wcn_ce_piece {
   int64_t x_ld, w_ld;
   int rows, classes, channels;
   const float* bias2;       // bias / ln 2 from the first class on, -inf from the last class to a multiple of 256; null: none
-  // forward: [2 * splits][rows] of (largest, sum of 2^(z - largest)), z in units of ln 2
+  // forward: [parts][rows] of (largest, sum of 2^(z - largest)), z in units of ln 2
   float2* part;
   // backward
   const float* lse2;        // of the piece's rows, in units of ln 2

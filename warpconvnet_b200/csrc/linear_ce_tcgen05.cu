@@ -1,12 +1,12 @@
 // The matrix products of the linear cross entropy in 16 bits on the tensor cores.
 //
 // ce_logits_kernel computes tiles of 128 rows x up to 256 classes of z = x w^T + b and uses them as they leave tensor memory:
-//   forward   running (largest, sum of exponentials) of each row over the classes of a unit, one pair per half tile column;
+//   forward   running (largest, sum of exponentials) of each row over the classes of a unit, one pair per quarter of a tile's columns;
 //   backward  g = (softmax - onehot) in 16 bits, a piece of the gradient of the logits, from the saved log-sum-exp.
 // ce_product_kernel multiplies such a piece by the weights (dX = g W) or by the rows (dW = g^T X).
 //
 // Logits are kept in units of ln 2, so that an exponential is one instruction.  Both kernels are persistent: one thread issues
-// TMA tile loads into a ring, one the matrix instructions, eight warps empty one of two accumulators while the other is filled.
+// TMA tile loads into a ring, one the matrix instructions, eight or sixteen warps empty one of two accumulators while the other is filled.
 // Where they fit, the rows of a tile (up to 384 channels) or the classes (up to 256 of them) stay in shared memory and only the
 // other operand passes: a multiprocessor receives about 80 bytes a clock, and a tile whose operands both arrived anew would
 // wait for them (192 KB against 2 048 clocks of matrix instructions at 256 channels).
@@ -22,7 +22,9 @@ namespace {
 constexpr int TILE_M = 128, SLICE = 64;                   // rows of a tile; channels (elements of k) of a stage
 constexpr int A_BYTES = TILE_M * SLICE * 2;
 constexpr int MAX_STAGES = 12;
-constexpr int EPI_WARPS = 8, EPI_WARP0 = 2, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+constexpr int EPI_WARP0 = 2;
+constexpr int PARTS = 4, LOGIT_WARPS = 4 * PARTS, LOGIT_THREADS = (EPI_WARP0 + LOGIT_WARPS) * 32;   // four warps a lane quarter share a tile's columns
+constexpr int EPI_WARPS = 8, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int SMEM_BUDGET = 222 * 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -74,7 +76,7 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
 }
 
 // Barriers, tensor memory and the look at the status word that both kernels begin with; false: an earlier launch gave up.
-__device__ __forceinline__ bool begin(Control* ctl, int stages, int tmem_cols, int32_t* dev_status) {
+__device__ __forceinline__ bool begin(Control* ctl, int stages, int tmem_cols, int epi_warps, int32_t* dev_status) {
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)dev_status;
   __syncthreads();
@@ -83,7 +85,7 @@ __device__ __forceinline__ bool begin(Control* ctl, int stages, int tmem_cols, i
     for (int s = 0; s < stages; ++s) { mbar_init(bar(&ctl->full[s]), 1); mbar_init(bar(&ctl->empty[s]), 1); }
     mbar_init(bar(&ctl->res_full), 1);
     mbar_init(bar(&ctl->res_empty), 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), EPI_WARPS); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)epi_warps); }
     mbar_init(bar(&ctl->done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -173,7 +175,7 @@ template <int W, bool BF16> __device__ __forceinline__ void gradients(const wcn_
 }
 
 template <int RES, bool GRAD, bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(LOGIT_THREADS, 1)
 ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ LogitParams p) {
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -183,7 +185,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t res = base + (uint32_t)(p.stages * stage_bytes);
   Control* ctl = reinterpret_cast<Control*>(smem_raw + (base - smem_u32(smem_raw)) + p.stages * stage_bytes + (RES == NOTHING ? 0 : p.KB * res_slice));
-  if (!begin(ctl, p.stages, p.tmem_cols, p.dev_status)) return;
+  if (!begin(ctl, p.stages, p.tmem_cols, LOGIT_WARPS, p.dev_status)) return;
   const uint32_t tmem = ctl->tmem_holder;
   bool ok = true;
 
@@ -260,8 +262,8 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
-    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;   // of 16 columns
+    const int quarter = warp & 3, part = (warp - EPI_WARP0) >> 2;
+    const int pieces = p.NT / 16, first = pieces * part / PARTS, last = pieces * (part + 1) / PARTS;   // of 16 columns
     int ab = 0, aphase = 0;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
       const int m = u % p.m_tiles, split = u / p.m_tiles, n0 = split * p.per, n1 = min(n0 + p.per, p.n_tiles);
@@ -320,7 +322,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
         if (++ab == 2) { ab = 0; aphase ^= 1; }
       }
       if (!ok) break;
-      if (!GRAD && live) p.q.part[(int64_t)(split * 2 + half) * p.q.rows + row] = make_float2(top, sum);
+      if (!GRAD && live) p.q.part[(int64_t)(split * PARTS + part) * p.q.rows + row] = make_float2(top, sum);
     }
   }
   tc_fence_before();
@@ -367,7 +369,7 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
     for (int i = threadIdx.x; i < CHUNK / 4; i += THREADS) reinterpret_cast<uint32_t*>(gen)[i] = one;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (!begin(ctl, p.stages, p.tmem_cols, p.dev_status)) { mark(); return; }
+  if (!begin(ctl, p.stages, p.tmem_cols, EPI_WARPS, p.dev_status)) { mark(); return; }
   const uint32_t tmem = ctl->tmem_holder;
   bool ok = true;
 
@@ -526,7 +528,7 @@ struct HeadControl {
 constexpr int ONES_BYTES = 16 * 128;
 
 template <bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(LOGIT_THREADS, 1)
 ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -541,7 +543,7 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     if (!p.dx) return;
     const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x)
-      for (int i = threadIdx.x; i < TILE_M * p.q.channels; i += THREADS) {
+      for (int i = threadIdx.x; i < TILE_M * p.q.channels; i += LOGIT_THREADS) {
         const int row = t * TILE_M + i / p.q.channels;
         if (row < p.q.rows) reinterpret_cast<uint16_t*>(p.dx)[(int64_t)row * p.q.channels + i % p.q.channels] = nan;
       }
@@ -553,15 +555,15 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->x_full[i]), 1); mbar_init(bar(&ctl->x_empty[i]), 1); }
     mbar_init(bar(&ctl->w_full), 1);
     mbar_init(bar(&ctl->s_full), 1);
-    mbar_init(bar(&ctl->g_full), EPI_WARPS);
+    mbar_init(bar(&ctl->g_full), LOGIT_WARPS);
     mbar_init(bar(&ctl->g_empty), 1);
     mbar_init(bar(&ctl->dx_full), 1);
-    mbar_init(bar(&ctl->dx_read), EPI_WARPS);
+    mbar_init(bar(&ctl->dx_read), LOGIT_WARPS);
     mbar_init(bar(&ctl->acc_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   const uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u;
-  for (int i = threadIdx.x; i < ONES_BYTES / 4; i += THREADS) reinterpret_cast<uint32_t*>(gen + ones_at)[i] = one;
+  for (int i = threadIdx.x; i < ONES_BYTES / 4; i += LOGIT_THREADS) reinterpret_cast<uint32_t*>(gen + ones_at)[i] = one;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
   tc_fence_before();
@@ -650,10 +652,10 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2, in_tile = quarter * 32 + lane;
+    const int quarter = warp & 3, part = (warp - EPI_WARP0) >> 2, in_tile = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;
-    const int c_pieces = p.CN / 16, c_first = half ? (c_pieces + 1) / 2 : 0, c_last = half ? c_pieces : (c_pieces + 1) / 2;
+    const int pieces = p.NT / 16, first = pieces * part / PARTS, last = pieces * (part + 1) / PARTS;
+    const int c_pieces = p.CN / 16, c_first = c_pieces * part / PARTS, c_last = c_pieces * (part + 1) / PARTS;
     float scale = 0.f;
     if (p.dx) {
       const int count = p.scale.count ? *p.scale.count : 1;
@@ -733,7 +735,7 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
             st_global_32B(to + c * 16, r);
             st_global_32B(to + c * 16 + 8, r + 8);
           }
-          if (with_ones && half) {
+          if (with_ones && part == PARTS - 1) {
             uint32_t r[16];
             __syncwarp();
             tmem_ld16(lanes + (uint32_t)(p.acc + p.MB * p.CN + m * 16), r);
@@ -804,7 +806,7 @@ int launch_logits(LogitParams& p, size_t fixed, cudaStream_t st) {
   constexpr auto kern = ce_logits_kernel<RES, GRAD, BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
-  kern<<<p.units < sms ? p.units : sms, THREADS, fixed + kept + (size_t)p.stages * stage, st>>>(xm, wm, p);
+  kern<<<p.units < sms ? p.units : sms, LOGIT_THREADS, fixed + kept + (size_t)p.stages * stage, st>>>(xm, wm, p);
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -873,7 +875,7 @@ template <bool BF16> int launch_head(HeadParams& p, size_t smem, int blocks, cud
     return WCN_ERR_UNSUPPORTED_CONFIG;
   constexpr auto kern = ce_head_kernel<BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
-  kern<<<blocks, THREADS, smem, st>>>(xm, wm, p);
+  kern<<<blocks, LOGIT_THREADS, smem, st>>>(xm, wm, p);
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -899,10 +901,11 @@ int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, floa
   return dtype == WCN_BF16 ? launch_head<true>(p, smem, blocks, st) : launch_head<false>(p, smem, blocks, st);
 }
 
-int wcn_ce_logits_splits(int rows, int classes) {
+// Pairs of (largest, sum) that the forward kernel leaves for each row.
+int wcn_ce_logits_parts(int rows, int classes) {
   LogitParams p = {};
   plan_logits(rows, classes, &p);
-  return p.splits;
+  return p.splits * PARTS;
 }
 
 int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st) {
