@@ -21,7 +21,10 @@ int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias);
 int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
                 int32_t* dev_status, cudaStream_t st);
 int wcn_ce_product_splits(int m, int n, int k);
-int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, int dtype, int32_t* dev_status, cudaStream_t st);
+int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st);
+bool wcn_ce_rows_taken(int channels);
+void wcn_ce_rows_plan(int rows, int classes, int* chunk, int* slots);
+int wcn_ce_rows(const wcn_ce_piece& q, float* slab, int dtype, float lift, int32_t* dev_status, cudaStream_t st);
 
 namespace {
 
@@ -184,6 +187,7 @@ struct JoinParams {
   int n, ld, splits;
   wcn_ce_scale scale;
   const int32_t* dev_status;
+  int n_tiles, chunk;      // splits of a row as ce_rows_kernel leaves them (chunk 0: `splits` for all)
 };
 
 template <typename TO, int SIDE>
@@ -196,8 +200,13 @@ __global__ void __launch_bounds__(THREADS) ce_join_kernel(const __grid_constant_
   double v[4] = {0, 0, 0, 0};
   if (q < all) {
     const float4* const from = reinterpret_cast<const float4*>(p.slab) + q;
+    int splits = p.splits;
+    if (p.chunk) {
+      const int64_t first = q / quads / 128 * p.n_tiles;
+      splits = (int)((first + p.n_tiles - 1) / p.chunk - first / p.chunk) + 1;
+    }
 #pragma unroll 4
-    for (int s = side; s < p.splits; s += SIDE) {
+    for (int s = side; s < splits; s += SIDE) {
       const float4 t = __ldg(from + (int64_t)s * all);
       v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
     }
@@ -441,6 +450,7 @@ struct Pieces {
   int rows, classes, row_pieces, class_pieces;
   int64_t g, slab_x, slab_w, slab_b, acc_x, acc_w, acc_b, bytes;
   int64_t g_ld;
+  bool fused;            // g and dx are one kernel's
   int head;              // blocks of the kernel that needs no pieces (few classes), 0: not taken
 };
 
@@ -460,9 +470,10 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
     p.bytes = at;
     return p;
   }
+  p.fused = dtype != WCN_F32 && v > 256 && wcn_ce_rows_taken(c);
   p.row_pieces = (int)((n + PIECE_ROWS - 1) / PIECE_ROWS);
-  if (v <= 1024) {   // few classes: all of them with as many rows as there is room for
-    const int64_t most = PIECE_BYTES / (e * ((v + 63) / 64 * 64)) / 128 * 128;
+  if (v <= 1024 || p.fused) {   // as many rows as there is room for with all classes or a good many
+    const int64_t few = v <= 1024 ? (v + 63) / 64 * 64 : 1024, most = PIECE_BYTES / (e * few) / 128 * 128;
     p.row_pieces = (int)((n + most - 1) / most);
   }
   p.rows = wcn_ce_round((n + p.row_pieces - 1) / p.row_pieces, 128);
@@ -479,12 +490,15 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 2; ++j) {
       const int64_t r = i ? n - (int64_t)(p.row_pieces - 1) * p.rows : p.rows, k = j ? v - (int64_t)(p.class_pieces - 1) * p.classes : p.classes;
-      const int64_t fx = product_splits((int)r, c, (int)k, dtype) * r * p.ld * 4, s = product_splits((int)k, c, (int)r, dtype);
+      int chunk, slots;
+      if (p.fused) wcn_ce_rows_plan((int)r, (int)k, &chunk, &slots);
+      else slots = product_splits((int)r, c, (int)k, dtype);
+      const int64_t fx = slots * r * p.ld * 4, s = product_splits((int)k, c, (int)r, dtype);
       if (fx > sx) sx = fx;
       if (s * k * p.ld * 4 > sw) sw = s * k * p.ld * 4;
       if (s * k * 4 > sb) sb = s * k * 4;
     }
-  p.g = take((int64_t)p.rows * p.g_ld * e);
+  p.g = take(p.fused ? (w || b ? (int64_t)wcn_ce_round(p.rows, 128) * wcn_ce_round(p.classes, 128) * e : 0) : (int64_t)p.rows * p.g_ld * e);
   p.slab_x = take(x ? sx : 0);
   p.slab_w = take(w || b ? sw : 0);
   p.slab_b = take(b ? (sb + 15) / 16 * 16 : 0);
@@ -600,17 +614,26 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
       q.row_scale = row_max ? grad + r0 : nullptr; q.row_max = row_max;
       q.g = ws + p.g; q.g_ld = p.g_ld;
       int rc = WCN_OK;
-      if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q);
+      if (p.fused) {
+        int chunk, slots;
+        wcn_ce_rows_plan(rows, vs, &chunk, &slots);
+        if (!dw && !dbias) q.g = nullptr;
+        float* const slab = dx ? (float*)(ws + p.slab_x) : nullptr;
+        rc = wcn_ce_rows(q, slab, dtype, lift, dev_status, st);
+        if (rc == WCN_OK && dx)
+          rc = join({slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? (char*)dx + r0 * channels * e : nullptr, rows, channels, p.ld, slots, scale, dev_status,
+                     (vs + 127) / 128, chunk}, dtype, st);
+      } else if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q);
       else rc = wcn_ce_logits(q, dtype, true, lift, dev_status, st);
       if (rc != WCN_OK) return rc;
-      if (dx) {
+      if (dx && !p.fused) {
         wcn_ce_product d = {};
         d.a = q.g; d.a_ld = p.g_ld; d.b = q.w; d.b_ld = w_ld; d.m = rows; d.n = channels; d.k = vs;
         d.splits = product_splits(rows, channels, vs, dtype); d.slab = (float*)(ws + p.slab_x); d.scale = scale;
         char* const out = (char*)dx + r0 * channels * e;
         const bool whole = p.class_pieces == 1 && d.splits == 1 && dtype != WCN_F32;
         if (whole) d.out = out;
-        rc = dtype == WCN_F32 ? fp32_product(d, false, st) : wcn_ce_product_run(d, false, dtype, dev_status, st);
+        rc = dtype == WCN_F32 ? fp32_product(d, false, st) : wcn_ce_product_run(d, false, false, dtype, dev_status, st);
         if (rc != WCN_OK) return rc;
         if (!whole) {
           JoinParams jp = {d.slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? out : nullptr, rows, channels, p.ld, d.splits, scale, dev_status};
@@ -620,10 +643,10 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
       }
       if (dw || dbias) {
         wcn_ce_product d = {};
-        d.a = q.g; d.a_ld = p.g_ld; d.b = q.x; d.b_ld = x_ld; d.m = vs; d.n = channels; d.k = rows;
+        d.a = q.g; d.a_ld = p.fused ? (vs + 127) / 128 : p.g_ld; d.b = q.x; d.b_ld = x_ld; d.m = vs; d.n = channels; d.k = rows;
         d.splits = product_splits(vs, channels, rows, dtype); d.slab = (float*)(ws + p.slab_w); d.scale = scale;
         d.slab_ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
-        rc = dtype == WCN_F32 ? fp32_product(d, true, st) : wcn_ce_product_run(d, true, dtype, dev_status, st);
+        rc = dtype == WCN_F32 ? fp32_product(d, true, st) : wcn_ce_product_run(d, true, p.fused, dtype, dev_status, st);
         if (rc != WCN_OK) return rc;
         const bool done = i == p.row_pieces - 1;
         if (dw) {

@@ -340,7 +340,8 @@ struct ProductParams {
   int32_t* dev_status;
 };
 
-template <bool TRANS, bool BF16>
+// BLOCKED: A is g as ce_rows_kernel leaves it, images of [128 rows][64 classes] with which a stage is filled as it is.
+template <bool TRANS, bool BLOCKED, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ ProductParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -383,7 +384,11 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
           if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
           const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
           mbar_expect_tx(full, (uint32_t)stage_bytes);
-          if (TRANS) {
+          if (BLOCKED) {   // 64 rows of two images
+            const char* const from = reinterpret_cast<const char*>(p.q.a) + ((int64_t)(k >> 1) * p.q.a_ld + m / TILE_M) * (2 * A_BYTES) + (k & 1) * CHUNK;
+            bulk_copy_g2s(at, from, CHUNK, full);
+            bulk_copy_g2s(at + CHUNK, from + A_BYTES, CHUNK, full);
+          } else if (TRANS) {
             tma_load_2d(at, &a_map, m, k * SLICE, full);
             tma_load_2d(at + CHUNK, &a_map, m + 64, k * SLICE, full);
           } else {
@@ -754,12 +759,224 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
   if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) mark();
 }
 
-template <auto KERNEL> bool allow_smem() {
+// ------------------------------------------------------------------ gradients of many classes
+
+// g and dx = g w in one kernel, for up to 256 channels: the rows of a tile stay in shared memory, classes pass in tiles of 128;
+// a tile's z = x w^T is computed in one of two accumulators while the epilogue warps turn the other into g, an operand tile in
+// shared memory, of which dx += g w is made (in columns that stay in tensor memory for all classes of a row tile) and which one
+// bulk copy leaves in global memory for dw, as it is: [128 rows][64 classes] images.  The (row tile, class tile) pairs are one
+// sequence that is divided evenly among the blocks; where a row tile's classes are several blocks', each leaves its dx apart.
+// As two kernels, the second of which read g again in rows of 128 bytes, 15 000 rows x 6 656 classes x 256 channels bf16 took
+// 85 (g) + 62 us (dx).
+struct RowsParams {
+  wcn_ce_piece q;         // g: images, or null (no dw)
+  float* slab;            // [slots][rows][channels rounded up to 16], or null (no dx)
+  int KB, CN;
+  int n_tiles, total, chunk;   // class tiles; pairs in all, and of a block
+  float lift;
+  int32_t* dev_status;
+};
+
+struct RowsControl {
+  uint64_t x_full, x_empty, w_full[2], w_empty[2], s_full[2], g_full, g_empty, dx_full, dx_read, done;
+  uint32_t tmem_holder;
+  int32_t skip;
+};
+
+constexpr int STORE_WARP = 2, ROWS_WARP0 = 3, ROWS_THREADS = (ROWS_WARP0 + LOGIT_WARPS) * 32;
+constexpr int ROWS_SMEM = 227 * 1024;
+
+template <bool BF16>
+__global__ void __launch_bounds__(ROWS_THREADS, 1)
+ce_rows_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ RowsParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slices = p.KB * A_BYTES;                       // a tile of 128 rows, or of 128 classes
+  const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
+  const int x_at = 0, w_at = slices, g_at = 3 * slices;
+  uint8_t* const gen = smem_raw + pad;
+  const uint32_t base = smem_u32(smem_raw) + pad;
+  RowsControl* ctl = reinterpret_cast<RowsControl*>(gen + g_at + 2 * A_BYTES);
+  const bool want_x = p.slab != nullptr, want_w = p.q.g != nullptr;
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) return;
+  if (threadIdx.x == 0) {
+    mbar_init(bar(&ctl->x_full), 1);
+    mbar_init(bar(&ctl->x_empty), 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(&ctl->w_full[i]), 1); mbar_init(bar(&ctl->w_empty[i]), 1); mbar_init(bar(&ctl->s_full[i]), 1); }
+    mbar_init(bar(&ctl->g_full), LOGIT_WARPS);
+    mbar_init(bar(&ctl->g_empty), 2);                      // the products that read g, and the copy of it
+    mbar_init(bar(&ctl->dx_full), 1);
+    mbar_init(bar(&ctl->dx_read), LOGIT_WARPS);
+    mbar_init(bar(&ctl->done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), 512u);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_holder, dx_col = 256;
+  const int begin_at = (int)blockIdx.x * p.chunk, end_at = min(begin_at + p.chunk, p.total);
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int i = 0, segments = 0;
+      for (int t = begin_at; t < end_at; ++t, ++i) {
+        const int m = t / p.n_tiles, n = t - m * p.n_tiles;
+        if (i == 0 || n == 0) {
+          if (!mbar_wait(bar(&ctl->x_empty), (segments & 1) ^ 1, p.dev_status)) { ok = false; break; }
+          ++segments;
+          mbar_expect_tx(bar(&ctl->x_full), (uint32_t)slices);
+          for (int s = 0; s < p.KB; ++s) tma_load_2d(base + x_at + (uint32_t)(s * A_BYTES), &x_map, s * SLICE, m * TILE_M, bar(&ctl->x_full));
+        }
+        if (!mbar_wait(bar(&ctl->w_empty[i & 1]), ((i >> 1) & 1) ^ 1, p.dev_status)) { ok = false; break; }
+        const uint32_t full = bar(&ctl->w_full[i & 1]);
+        mbar_expect_tx(full, (uint32_t)slices);
+        for (int s = 0; s < p.KB; ++s) tma_load_2d(base + w_at + (uint32_t)((i & 1) * slices + s * A_BYTES), &w_map, s * SLICE, n * TILE_M, full);
+      }
+      if (!ok) {   // what has been issued lands before the block's shared memory is given back
+        if (segments)
+          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->x_full), (uint32_t)((segments - 1) & 1)); ++k) {}
+        for (int j = i - 2 < 0 ? 0 : i - 2; j < i; ++j)
+          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->w_full[j & 1]), (uint32_t)((j >> 1) & 1)); ++k) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t flags = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(TILE_M >> 4) << 24);
+      const uint32_t id_s = flags | ((uint32_t)(TILE_M >> 3) << 17), id_dx = flags | (1u << 16) | ((uint32_t)(p.CN >> 3) << 17);
+      const uint64_t x_k = smem_desc<128>(base + x_at), w_k = smem_desc<128>(base + w_at), w_mn = smem_desc_mn<128>(base + w_at, A_BYTES), g_k = smem_desc<128>(base + g_at);
+      int segments = 0;
+      auto logits = [&](int i) {
+        const int t = begin_at + i, n = t % p.n_tiles;
+        if (i == 0 || n == 0) {
+          if (!mbar_wait(bar(&ctl->x_full), segments & 1, p.dev_status)) { ok = false; return; }
+          ++segments;
+        }
+        if (!mbar_wait(bar(&ctl->w_full[i & 1]), (i >> 1) & 1, p.dev_status)) { ok = false; return; }
+        tc_fence_after();
+        const uint64_t w = w_k + (uint64_t)(((i & 1) * slices) >> 4);
+        for (int s = 0; s < p.KB; ++s)
+#pragma unroll
+          for (int k = 0; k < SLICE / 16; ++k)
+            umma_f16(tmem + (uint32_t)((i & 1) * TILE_M), x_k + (uint64_t)((s * A_BYTES) >> 4) + (uint64_t)(k * 2), w + (uint64_t)((s * A_BYTES) >> 4) + (uint64_t)(k * 2), id_s,
+                     (s | k) ? 1u : 0u);
+        umma_commit(bar(&ctl->s_full[i & 1]));
+        if (t + 1 < end_at && n == p.n_tiles - 1) umma_commit(bar(&ctl->x_empty));   // the rows' last logits
+      };
+      const int count = end_at - begin_at;
+      if (count > 0) logits(0);
+      int done_segments = 0;
+      for (int i = 0; i < count && ok; ++i) {
+        if (i + 1 < count) logits(i + 1);                  // (its accumulator was read before g of tile i - 1 was complete)
+        if (!ok) break;
+        const int n = (begin_at + i) % p.n_tiles;
+        const bool opens = i == 0 || n == 0, closes = i + 1 == count || n == p.n_tiles - 1;
+        if (!mbar_wait(bar(&ctl->g_full), i & 1, p.dev_status)) { ok = false; break; }
+        if (want_x) {
+          if (opens && done_segments && !mbar_wait(bar(&ctl->dx_read), (done_segments - 1) & 1, p.dev_status)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t w = w_mn + (uint64_t)(((i & 1) * slices) >> 4);
+#pragma unroll
+          for (int k = 0; k < TILE_M / 16; ++k)
+            umma_f16(tmem + dx_col, g_k + (uint64_t)(((k >> 2) * A_BYTES) >> 4) + (uint64_t)((k & 3) * 2), w + (uint64_t)(k * 128), id_dx, (!opens || k) ? 1u : 0u);
+        }
+        umma_commit(bar(&ctl->w_empty[i & 1]));
+        umma_commit(bar(&ctl->g_empty));
+        if (want_x && closes) {
+          umma_commit(bar(&ctl->dx_full));
+          ++done_segments;
+        }
+      }
+      umma_commit(bar(&ctl->done));
+      (void)mbar_wait(bar(&ctl->done), 0, p.dev_status);
+    }
+    __syncwarp();
+  } else if (warp == STORE_WARP) {
+    if (elect_one()) {
+      const int count = end_at - begin_at;
+      for (int i = 0; i < count; ++i) {
+        if (!mbar_wait(bar(&ctl->g_full), i & 1, p.dev_status)) break;
+        if (want_w) {
+          void* const to = reinterpret_cast<char*>(p.q.g) + (int64_t)(begin_at + i) * (2 * A_BYTES);
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::"l"(to),
+                       "r"(base + (uint32_t)g_at), "r"(2 * A_BYTES)
+                       : "memory");
+        }
+        mbar_arrive(bar(&ctl->g_empty));
+      }
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, part = (warp - ROWS_WARP0) >> 2, in_tile = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int c_pieces = p.CN / 16, c_first = c_pieces * part / PARTS, c_last = c_pieces * (part + 1) / PARTS;
+    RowGrad rg = {};
+    int i = 0, segments = 0;
+    for (int t = begin_at; t < end_at; ++t, ++i) {
+      const int m = t / p.n_tiles, n = t - m * p.n_tiles, row = m * TILE_M + in_tile;
+      if (i == 0 || n == 0) rg = row_grad(p.q, row, p.lift);
+      if (ok) ok = mbar_wait(bar(&ctl->s_full[i & 1]), (i >> 1) & 1, p.dev_status);
+      if (ok && i) ok = mbar_wait(bar(&ctl->g_empty), (i - 1) & 1, p.dev_status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      {   // 32 of the tile's 128 columns
+        uint32_t r[32], out[16];
+        float z[32];
+        const int col = n * TILE_M + part * 32;
+        tmem_ld32(lanes + (uint32_t)((i & 1) * TILE_M + part * 32), r);
+        tmem_ld_wait();
+        to_logits<32>(p.q, r, col, z);
+        gradients<32, BF16>(p.q, rg, z, out);
+        uint8_t* const chunk = gen + g_at + (part >> 1) * A_BYTES;
+        const int piece = (part & 1) * 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(chunk + tile_offset<128>(in_tile, piece + k)) = make_uint4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+        const int in = rg.label - col;
+        if (in >= 0 && in < 32)
+          reinterpret_cast<uint16_t*>(chunk + tile_offset<128>(in_tile, piece + (in >> 3)))[in & 7] = label_grad<BF16>(p.q, rg, row, p.lift);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->g_full));
+      if (!want_x || !(t + 1 == end_at || n == p.n_tiles - 1)) continue;
+      if (ok) ok = mbar_wait(bar(&ctl->dx_full), segments & 1, p.dev_status);
+      ++segments;
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      const int slot = (int)blockIdx.x - m * p.n_tiles / p.chunk;
+      float* const to = p.slab + ((int64_t)slot * p.q.rows + row) * p.CN;
+      for (int c = c_first; c < c_last; ++c) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld16(lanes + dx_col + (uint32_t)(c * 16), r);
+        tmem_ld_wait();
+        if (row >= p.q.rows) continue;
+        st_global_32B(to + c * 16, r);
+        st_global_32B(to + c * 16 + 8, r + 8);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->dx_read));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512u);
+}
+
+template <auto KERNEL, int BYTES = SMEM_BUDGET> bool allow_smem() {
   static bool configured[64] = {};   // per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET) != cudaSuccess) {
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) != cudaSuccess) {
       (void)cudaGetLastError();
       return false;
     }
@@ -818,7 +1035,7 @@ template <bool GRAD, bool BF16> int by_resident(LogitParams& p, cudaStream_t st)
   return launch_logits<NOTHING, GRAD, BF16>(p, fixed, st);
 }
 
-template <bool TRANS, bool BF16>
+template <bool TRANS, bool BLOCKED, bool BF16>
 int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st) {
   ProductParams p = {};
   p.q = q;
@@ -841,10 +1058,10 @@ int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st
   p.stages = (int)((SMEM_BUDGET - fixed) / stage);
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   CUtensorMap am, bm;
-  if (!matrix_map(&am, q.a, TRANS ? q.k : q.m, TRANS ? q.m : q.k, q.a_ld * 2, TRANS ? SLICE : TILE_M, BF16) ||
-      !matrix_map(&bm, q.b, q.k, q.n, q.b_ld * 2, SLICE, BF16))
-    return WCN_ERR_UNSUPPORTED_CONFIG;
-  constexpr auto kern = ce_product_kernel<TRANS, BF16>;
+  if (!matrix_map(&bm, q.b, q.k, q.n, q.b_ld * 2, SLICE, BF16)) return WCN_ERR_UNSUPPORTED_CONFIG;
+  if (BLOCKED) am = bm;   // (not read)
+  else if (!matrix_map(&am, q.a, TRANS ? q.k : q.m, TRANS ? q.m : q.k, q.a_ld * 2, TRANS ? SLICE : TILE_M, BF16)) return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = ce_product_kernel<TRANS, BLOCKED, BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
   kern<<<p.units < sms ? p.units : sms, THREADS, fixed + (size_t)p.stages * stage, st>>>(am, bm, p);
@@ -879,7 +1096,41 @@ template <bool BF16> int launch_head(HeadParams& p, size_t smem, int blocks, cud
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
+size_t rows_smem(int channels) { return 1024 + (size_t)(3 * ((channels + SLICE - 1) / SLICE) + 2) * A_BYTES + sizeof(RowsControl) + 128; }
+
+template <bool BF16> int launch_rows(RowsParams& p, cudaStream_t st) {
+  CUtensorMap xm, wm;
+  if (!matrix_map(&xm, p.q.x, p.q.rows, p.q.channels, p.q.x_ld * 2, TILE_M, BF16) ||
+      !matrix_map(&wm, p.q.w, p.q.classes, p.q.channels, p.q.w_ld * 2, TILE_M, BF16))
+    return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = ce_rows_kernel<BF16>;
+  if (!allow_smem<kern, ROWS_SMEM>()) return WCN_ERR_INITIALIZATION;
+  kern<<<(p.total + p.chunk - 1) / p.chunk, ROWS_THREADS, rows_smem(p.q.channels), st>>>(xm, wm, p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
 }  // namespace
+
+// Whether g and dx are one kernel's, and how the (row tile, class tile) pairs of a piece are divided among blocks: `chunk` pairs
+// each, so that a row tile has at most `slots` of them.
+bool wcn_ce_rows_taken(int channels) { return channels <= 256 && rows_smem(channels) <= (size_t)ROWS_SMEM; }
+void wcn_ce_rows_plan(int rows, int classes, int* chunk, int* slots) {
+  const int64_t n_tiles = (classes + TILE_M - 1) / TILE_M, total = n_tiles * ((rows + TILE_M - 1) / TILE_M), sms = wcn_num_sms();
+  *chunk = (int)((total + sms - 1) / sms);
+  *slots = (int)((n_tiles - 1) / *chunk) + 2;
+}
+
+int wcn_ce_rows(const wcn_ce_piece& q, float* slab, int dtype, float lift, int32_t* dev_status, cudaStream_t st) {
+  RowsParams p = {};
+  int slots;
+  p.q = q; p.slab = slab; p.lift = lift; p.dev_status = dev_status;
+  p.KB = (q.channels + SLICE - 1) / SLICE;
+  p.CN = wcn_ce_round(q.channels, 16);
+  p.n_tiles = (q.classes + TILE_M - 1) / TILE_M;
+  p.total = p.n_tiles * ((q.rows + TILE_M - 1) / TILE_M);
+  wcn_ce_rows_plan(q.rows, q.classes, &p.chunk, &slots);
+  return dtype == WCN_BF16 ? launch_rows<true>(p, st) : launch_rows<false>(p, st);
+}
 
 // Blocks, and with them slabs, of the kernel for few classes; 0: not taken.
 int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias) {
@@ -928,13 +1179,14 @@ int wcn_ce_product_splits(int m, int n, int k) {
     const int per = (ksteps + s - 1) / s;
     if ((ksteps + per - 1) / per != s) continue;
     // rounds of the grid in steps of k, a unit's start and its sums' way out and back counted as some more
-    const double cost = (double)((tiles * (int64_t)s + sms - 1) / sms) * (per + 6) + 0.02 * tiles * s;
+    const double cost = (double)((tiles * (int64_t)s + sms - 1) / sms) * (per + 12);
     if (cost < least) { least = cost; best = s; }
   }
   return best;
 }
 
-int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, int dtype, int32_t* dev_status, cudaStream_t st) {
-  if (dtype == WCN_BF16) return transposed ? launch_product<true, true>(q, dev_status, st) : launch_product<false, true>(q, dev_status, st);
-  return transposed ? launch_product<true, false>(q, dev_status, st) : launch_product<false, false>(q, dev_status, st);
+int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st) {
+  if (blocked) return dtype == WCN_BF16 ? launch_product<true, true, true>(q, dev_status, st) : launch_product<true, true, false>(q, dev_status, st);
+  if (dtype == WCN_BF16) return transposed ? launch_product<true, false, true>(q, dev_status, st) : launch_product<false, false, true>(q, dev_status, st);
+  return transposed ? launch_product<true, false, false>(q, dev_status, st) : launch_product<false, false, false>(q, dev_status, st);
 }
