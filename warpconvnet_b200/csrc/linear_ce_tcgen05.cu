@@ -340,14 +340,16 @@ struct ProductParams {
   int32_t* dev_status;
 };
 
-// BLOCKED: A is g as ce_rows_kernel leaves it, images of [128 rows][64 classes] with which a stage is filled as it is.
+// BLOCKED: A is g as ce_rows_kernel leaves it, images of [128 rows][64 classes] with which a stage is filled as it is, for 256
+// classes at a time: what arrives in shared memory is then 64 bytes a clock of the matrix instructions, with 128 classes 96.
 template <bool TRANS, bool BLOCKED, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ ProductParams p) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int CHUNK = SLICE * 128;                      // 64 rows of k x 64 columns
+  constexpr int MB = BLOCKED ? 2 : 1;                     // blocks of 128 rows of a tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int stage_bytes = A_BYTES + p.NB * CHUNK;
+  const int stage_bytes = MB * A_BYTES + p.NB * CHUNK;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t ones = base + (uint32_t)(p.stages * stage_bytes);
   uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw)) + p.stages * stage_bytes;
@@ -360,8 +362,8 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
     if (!p.q.out) return;
     const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x)
-      for (int i = threadIdx.x; i < TILE_M * p.NT; i += THREADS) {
-        const int row = m_of(u) * TILE_M + i / p.NT, col = n_of(u) * p.NT + i % p.NT;
+      for (int i = threadIdx.x; i < MB * TILE_M * p.NT; i += THREADS) {
+        const int row = m_of(u) * MB * TILE_M + i / p.NT, col = n_of(u) * p.NT + i % p.NT;
         if (row < p.q.m && col < p.q.n) reinterpret_cast<uint16_t*>(p.q.out)[(int64_t)row * p.q.n + col] = nan;
       }
   };
@@ -379,22 +381,26 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
       Ring r{0, 0, p.stages};
       int issued = 0;
       for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
-        const int m = m_of(u) * TILE_M, n = n_of(u) * p.NT, k0 = split_of(u) * p.per, k1 = min(k0 + p.per, p.ksteps);
+        const int m = m_of(u) * MB * TILE_M, n = n_of(u) * p.NT, k0 = split_of(u) * p.per, k1 = min(k0 + p.per, p.ksteps);
         for (int k = k0; k < k1; ++k) {
           if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
           const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
           mbar_expect_tx(full, (uint32_t)stage_bytes);
-          if (BLOCKED) {   // 64 rows of two images
-            const char* const from = reinterpret_cast<const char*>(p.q.a) + ((int64_t)(k >> 1) * p.q.a_ld + m / TILE_M) * (2 * A_BYTES) + (k & 1) * CHUNK;
-            bulk_copy_g2s(at, from, CHUNK, full);
-            bulk_copy_g2s(at + CHUNK, from + A_BYTES, CHUNK, full);
+          if (BLOCKED) {   // 64 rows of two images for each block of 128 classes (the last one again where there is no other)
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+              const int64_t tile = min((int64_t)(m / TILE_M + j), p.q.a_ld - 1);
+              const char* const from = reinterpret_cast<const char*>(p.q.a) + ((int64_t)(k >> 1) * p.q.a_ld + tile) * (2 * A_BYTES) + (k & 1) * CHUNK;
+              bulk_copy_g2s(at + j * A_BYTES, from, CHUNK, full);
+              bulk_copy_g2s(at + j * A_BYTES + CHUNK, from + A_BYTES, CHUNK, full);
+            }
           } else if (TRANS) {
             tma_load_2d(at, &a_map, m, k * SLICE, full);
             tma_load_2d(at + CHUNK, &a_map, m + 64, k * SLICE, full);
           } else {
             tma_load_2d(at, &a_map, k * SLICE, m, full);
           }
-          for (int c = 0; c < p.NB; ++c) tma_load_2d(at + A_BYTES + (uint32_t)(c * CHUNK), &b_map, n + 64 * c, k * SLICE, full);
+          for (int c = 0; c < p.NB; ++c) tma_load_2d(at + MB * A_BYTES + (uint32_t)(c * CHUNK), &b_map, n + 64 * c, k * SLICE, full);
           r.advance();
           ++issued;
         }
@@ -407,7 +413,7 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
       const uint32_t flags = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | (TRANS ? 1u << 15 : 0u) | (1u << 16) |
                              ((uint32_t)(TILE_M >> 4) << 24);
       const uint32_t idesc = flags | ((uint32_t)(p.NT >> 3) << 17), idesc_ones = flags | ((uint32_t)(16 >> 3) << 17);
-      const uint64_t a0 = TRANS ? smem_desc_mn<128>(base, CHUNK) : smem_desc<128>(base), b0 = smem_desc_mn<128>(base + A_BYTES, CHUNK);
+      const uint64_t a0 = TRANS ? smem_desc_mn<128>(base, CHUNK) : smem_desc<128>(base), b0 = smem_desc_mn<128>(base + MB * A_BYTES, CHUNK);
       const uint64_t ones0 = smem_desc_mn<128>(ones, CHUNK);
       constexpr int A_STEP = TRANS ? 128 : 2;             // 16 of k further, in units of 16 bytes
       Ring r{0, 0, p.stages};
@@ -417,18 +423,23 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
         const bool sums = with_ones && n_of(u) == 0;
         if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(ab * p.stride);
+        const uint32_t d0 = tmem + (uint32_t)(ab * MB * p.stride);
         for (int k = k0; k < k1; ++k) {
           if (!mbar_wait(bar(&ctl->full[r.slot]), r.phase, p.dev_status)) { ok = false; break; }
           tc_fence_after();
           const uint64_t at = (uint64_t)((r.slot * stage_bytes) >> 4);
 #pragma unroll
-          for (int i = 0; i < SLICE / 16; ++i)
-            umma_f16(d, a0 + at + (uint64_t)(i * A_STEP), b0 + at + (uint64_t)(i * 128), idesc, (k > k0 || i) ? 1u : 0u);
-          if (sums)
+          for (int j = 0; j < MB; ++j) {
+            const uint64_t a = a0 + at + (uint64_t)((j * A_BYTES) >> 4);
+            const uint32_t d = d0 + (uint32_t)(j * p.stride);
 #pragma unroll
             for (int i = 0; i < SLICE / 16; ++i)
-              umma_f16(d + (uint32_t)p.NT, a0 + at + (uint64_t)(i * A_STEP), ones0 + (uint64_t)(i * 128), idesc_ones, (k > k0 || i) ? 1u : 0u);
+              umma_f16(d, a + (uint64_t)(i * A_STEP), b0 + at + (uint64_t)(i * 128), idesc, (k > k0 || i) ? 1u : 0u);
+            if (sums)
+#pragma unroll
+              for (int i = 0; i < SLICE / 16; ++i)
+                umma_f16(d + (uint32_t)p.NT, a + (uint64_t)(i * A_STEP), ones0 + (uint64_t)(i * 128), idesc_ones, (k > k0 || i) ? 1u : 0u);
+          }
           umma_commit(bar(&ctl->empty[r.slot]));
           r.advance();
         }
@@ -454,39 +465,43 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
       if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       tc_fence_after();
-      const int row = m_of(u) * TILE_M + quarter * 32 + lane, n = n_of(u) * p.NT, split = split_of(u);
-      const bool live = row < p.q.m;
-      const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.stride);
-      float* const slab = p.q.slab + ((int64_t)split * p.q.m + row) * slab_ld + n;
-      uint16_t* const out = reinterpret_cast<uint16_t*>(p.q.out) + (int64_t)row * p.q.n + n;
-      for (int c = first; c < last; ++c) {
-        uint32_t r[16];
-        __syncwarp();
-        tmem_ld16(t + (uint32_t)(c * 16), r);
-        tmem_ld_wait();
-        if (!live) continue;
-        if (p.q.out) {
-          uint32_t v[8];
+      const int n = n_of(u) * p.NT, split = split_of(u);
+#pragma unroll 1
+      for (int j = 0; j < MB; ++j) {
+        const int row = (m_of(u) * MB + j) * TILE_M + quarter * 32 + lane;
+        const bool live = row < p.q.m;
+        const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((ab * MB + j) * p.stride);
+        float* const slab = p.q.slab + ((int64_t)split * p.q.m + row) * slab_ld + n;
+        uint16_t* const out = reinterpret_cast<uint16_t*>(p.q.out) + (int64_t)row * p.q.n + n;
+        for (int c = first; c < last; ++c) {
+          uint32_t r[16];
+          __syncwarp();
+          tmem_ld16(t + (uint32_t)(c * 16), r);
+          tmem_ld_wait();
+          if (!live) continue;
+          if (p.q.out) {
+            uint32_t v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = pack2<BF16>(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
-          if (p.vec && n + c * 16 + 16 <= p.q.n) {
-            st_global_32B(out + c * 16, v);
-          } else {
+            for (int i = 0; i < 8; ++i) v[i] = pack2<BF16>(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
+            if (p.vec && n + c * 16 + 16 <= p.q.n) {
+              st_global_32B(out + c * 16, v);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n + c * 16 + i < p.q.n) out[c * 16 + i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+              for (int i = 0; i < 16; ++i)
+                if (n + c * 16 + i < p.q.n) out[c * 16 + i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+            }
+          } else if (n + c * 16 < slab_ld) {
+            st_global_32B(slab + c * 16, r);
+            st_global_32B(slab + c * 16 + 8, r + 8);
           }
-        } else if (n + c * 16 < slab_ld) {
-          st_global_32B(slab + c * 16, r);
-          st_global_32B(slab + c * 16 + 8, r + 8);
         }
-      }
-      if (with_ones && n == 0 && half) {
-        uint32_t r[16];
-        __syncwarp();
-        tmem_ld16(t + (uint32_t)p.NT, r);
-        tmem_ld_wait();
-        if (live) p.q.slab_ones[(int64_t)split * p.q.m + row] = __uint_as_float(r[0]);
+        if (with_ones && n == 0 && half) {
+          uint32_t r[16];
+          __syncwarp();
+          tmem_ld16(t + (uint32_t)p.NT, r);
+          tmem_ld_wait();
+          if (live) p.q.slab_ones[(int64_t)split * p.q.m + row] = __uint_as_float(r[0]);
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -921,10 +936,9 @@ ce_rows_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       const int m = t / p.n_tiles, n = t - m * p.n_tiles, row = m * TILE_M + in_tile;
       if (i == 0 || n == 0) rg = row_grad(p.q, row, p.lift);
       if (ok) ok = mbar_wait(bar(&ctl->s_full[i & 1]), (i >> 1) & 1, p.dev_status);
-      if (ok && i) ok = mbar_wait(bar(&ctl->g_empty), (i - 1) & 1, p.dev_status);
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       tc_fence_after();
-      {   // 32 of the tile's 128 columns
+      {   // 32 of the tile's 128 columns, while g of the tile before is still multiplied
         uint32_t r[32], out[16];
         float z[32];
         const int col = n * TILE_M + part * 32;
@@ -932,6 +946,8 @@ ce_rows_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
         tmem_ld_wait();
         to_logits<32>(p.q, r, col, z);
         gradients<32, BF16>(p.q, rg, z, out);
+        if (i) ok = mbar_wait(bar(&ctl->g_empty), (i - 1) & 1, p.dev_status);
+        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
         uint8_t* const chunk = gen + g_at + (part >> 1) * A_BYTES;
         const int piece = (part & 1) * 4;
 #pragma unroll
@@ -1037,6 +1053,7 @@ template <bool GRAD, bool BF16> int by_resident(LogitParams& p, cudaStream_t st)
 
 template <bool TRANS, bool BLOCKED, bool BF16>
 int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st) {
+  constexpr int MB = BLOCKED ? 2 : 1;
   ProductParams p = {};
   p.q = q;
   p.dev_status = dev_status;
@@ -1044,17 +1061,17 @@ int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st
   p.n_tiles = (q.n + most - 1) / most;
   p.NT = wcn_ce_round((q.n + p.n_tiles - 1) / p.n_tiles, 16);
   p.NB = (p.NT + 63) / 64;
-  p.m_tiles = (q.m + TILE_M - 1) / TILE_M;
+  p.m_tiles = (q.m + MB * TILE_M - 1) / (MB * TILE_M);
   p.ksteps = (q.k + SLICE - 1) / SLICE;
   p.per = (p.ksteps + q.splits - 1) / q.splits;
   if ((p.ksteps + p.per - 1) / p.per != q.splits) return WCN_ERR_INVALID_PARAMETERS;
   p.units = p.m_tiles * p.n_tiles * q.splits;
   p.stride = p.NT + (q.slab_ones ? 16 : 0);
-  p.accs = 2 * p.stride <= 512 ? 2 : 1;
-  p.tmem_cols = columns_pow2(p.accs * p.stride);
+  p.accs = 2 * MB * p.stride <= 512 ? 2 : 1;
+  p.tmem_cols = columns_pow2(p.accs * MB * p.stride);
   p.vec = q.out && reinterpret_cast<uintptr_t>(q.out) % 32 == 0 && (q.n * 2) % 32 == 0;
   const size_t fixed = sizeof(Control) + 1024 + 128 + SLICE * 128;
-  const int stage = A_BYTES + p.NB * SLICE * 128;
+  const int stage = MB * A_BYTES + p.NB * SLICE * 128;
   p.stages = (int)((SMEM_BUDGET - fixed) / stage);
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   CUtensorMap am, bm;
@@ -1171,8 +1188,8 @@ int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, i
 }
 
 // Splits of k with which the product's tiles keep every multiprocessor busy.
-int wcn_ce_product_splits(int m, int n, int k) {
-  const int tiles = ((m + TILE_M - 1) / TILE_M) * ((n + 239) / 240), ksteps = (k + SLICE - 1) / SLICE, sms = wcn_num_sms();
+int wcn_ce_product_splits(int m, int n, int k, bool blocked) {
+  const int tile = blocked ? 2 * TILE_M : TILE_M, tiles = ((m + tile - 1) / tile) * ((n + 239) / 240), ksteps = (k + SLICE - 1) / SLICE, sms = wcn_num_sms();
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= sms && s <= ksteps; ++s) {

@@ -118,7 +118,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, bias: Option
     dtype); ``bias [V]`` may be of any of the three.  ``labels`` are N integers: a row labelled ``ignore_index`` does not count.
     A label that names no class counts as one and is reported by ``check_device_status``.  ``reduction``: ``"mean"`` over the rows that
     count, ``"sum"``, or ``"none"`` for the row losses.  Gradients come in the inputs' dtypes; that of the logits is made and used
-    in pieces of at most 256 MB (in 16 bits rounded to x's dtype, before the factor of the reduction)."""
+    in pieces of at most 512 MB (in 16 bits rounded to x's dtype, before the factor of the reduction)."""
     how = check_reduction(reduction)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or not weight.numel():
         raise ValueError(f"x must be [N, C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")
