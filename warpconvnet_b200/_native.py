@@ -136,7 +136,7 @@ KERNELS_PER_CALL = {
     "wcn_gather_rows": 1, "wcn_scatter_add_rows": 1, "wcn_conv_pack_weight": 1, "wcn_conv_fwd": 1,
     "wcn_selftest_bounded_wait": 1, "wcn_brick_build": 3, "wcn_kmap_search_bricks": 1,
     "wcn_conv_rows_fwd": 1, "wcn_batch_norm_train": 2, "wcn_column_sums": 2, "wcn_batch_norm_backward": 2, "wcn_conv_pack_weight_from": 1, "wcn_cells_build": 4, "wcn_kmap_search_cells": 1, "wcn_kmap_scan_host": 2, "wcn_unique_counts": 2, "wcn_morton_sort": 1, "wcn_pyramid": 2, "wcn_level_maps": 5,
-    "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1,  # (of up to 250 scenes)
+    "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1,  # (of up to 320 scenes)
     "wcn_linear_ce": 2, "wcn_linear_ce_backward": 5,  # (of one piece)
 }
 LAUNCH_COUNTS: Counter = Counter()

@@ -27,7 +27,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int BLOCKS_FORWARD = 2, BLOCKS_BACKWARD = 2;   // of a multiprocessor (128 registers a thread)
-constexpr int SCENES = 250;                      // of a launch: 2 KB of parameters
+constexpr int SCENES = 320;                      // of a launch: 4 KB of parameters
 constexpr int MAX_C = 4096;
 
 enum Act { NONE = 0, RELU = 1, SILU = 2, GELU = 3 };
@@ -702,7 +702,7 @@ template <typename F> int in_launches(const int64_t* offsets, int64_t scenes, bo
     int count = 0;   // scenes with rows
     for (; q.j < scenes && count < SCENES; ++q.j) count += offsets[q.j + 1] > offsets[q.j];
     const int64_t n = offsets[q.j] - offsets[i], side = (int64_t)tys * (back ? BLOCKS_BACKWARD : BLOCKS_FORWARD) * wcn_num_sms(), per = (n + side - 1) / side;
-    const int most = back ? 32 : 64, least = 2;
+    const int most = back ? 32 : 64, least = 4;
     q.rows = (int)(per < least ? least : per > most ? most : per) * tys;
     for (int64_t k = i; k < q.j; ++k) {
       const int tiles = (int)((offsets[k + 1] - offsets[k] + q.rows - 1) / q.rows);
@@ -743,7 +743,7 @@ template <typename T, int V, int ACT, int SUB, bool BACK> int all_launches(Param
     p.rows = q.rows;
     p.each = q.rows / tys;
     p.tiles = q.tiles;
-    const int lag = q.most + grid_most * 5 / 8;   // (two items for each tile: what was claimed a grid of items ago is done)
+    const int lag = q.most + grid_most;   // (what was claimed a grid of tiles ago is done: blocks hardly ever wait)
     p.lag = lag < q.tiles ? lag : q.tiles;
     p.x = reinterpret_cast<const T*>(base.x) + r * p.x_ld;
     if (BACK) p.dy = reinterpret_cast<const T*>(base.dy) + r * p.dy_ld;
