@@ -178,6 +178,25 @@ def test_infinities_and_what_is_no_number(dtype):
     check_device_status(DEV)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [40, 300])
+def test_gradients_that_are_no_numbers_stay_with_their_rows(dtype, v):
+    x, w, labels, _ = (None if t is None else t.to(DEV) for t in inputs(200, 32, v, dtype, False, ignored=0.0))
+    x = x.requires_grad_(True)
+    grad = torch.randn(200, device=DEV)
+    row = linear_cross_entropy(x, w, labels, reduction="none")
+    (want,) = torch.autograd.grad(row, [x], grad, retain_graph=True)
+    bad = grad.clone()
+    bad[3], bad[70] = float("inf"), float("nan")
+    (got,) = torch.autograd.grad(row, [x], bad, retain_graph=True)
+    fine = torch.ones(200, dtype=torch.bool, device=DEV)
+    fine[[3, 70]] = False
+    # (the others are divided by the largest of them and multiplied again: two roundings of fp32, or of one in 16 bits otherwise)
+    assert off(got[fine], want[fine]) <= TOL[dtype] and not torch.isfinite(got[3]).all() and torch.isnan(got[70]).all()
+    (none,) = torch.autograd.grad(row, [x], torch.zeros_like(grad))
+    assert not none.any()
+
+
 def test_certain_rows_and_large_logits():
     """Losses that round to zero are not negative; logits of hundreds do not overflow."""
     for dtype in DTYPES:
@@ -246,6 +265,17 @@ def test_second_derivatives():
     (gr,) = torch.autograd.grad(row.sum() / counts.sum(), [r], create_graph=True)
     (gga,), (ggr,) = torch.autograd.grad(ga.square().sum(), [a]), torch.autograd.grad(gr.square().sum(), [r])
     assert off(ga, gr) <= 1e-5 and off(gga, ggr) <= 1e-5
+
+
+def test_labels_of_no_class_in_a_graph_of_the_gradient():
+    x, w, labels, _ = (None if t is None else t.to(DEV) for t in inputs(30, 8, 11, torch.float32, False))
+    wrong = labels.clone()
+    wrong[0] = 11
+    labels[0] = -100
+    x = x.requires_grad_(True)
+    grads = [torch.autograd.grad(linear_cross_entropy(x, w, t), [x], create_graph=True)[0] for t in (wrong, labels)]
+    assert torch.equal(*grads)
+    device_status(DEV).zero_()
 
 
 def test_captured_and_on_a_stream_of_its_own():

@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(THREADS) ce_logits_fp32_kernel(const __grid_co
       float scale = 1.f;
       if (q.row_scale) {
         const float most = __ldg(q.row_max);
-        scale = most > 0.f ? __ldg(&q.row_scale[row]) / most : most == most ? 0.f : most;
+        scale = __ldg(&q.row_scale[row]) / (most > 0.f ? most : 1.f);
       }
       const float lse2 = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
 #pragma unroll

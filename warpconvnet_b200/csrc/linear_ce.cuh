@@ -22,7 +22,7 @@ struct wcn_ce_piece {
   const float* lse2;        // of the piece's rows, in units of ln 2
   const float* loss;
   const int64_t* labels;
-  const float* row_scale;   // gradient of each row's loss (null: 1), divided by *row_max
+  const float* row_scale;   // gradient of each row's loss (null: 1), divided by *row_max (0: all of them are 0 or no numbers)
   const float* row_max;
   int64_t ignore, first_class, all_classes;
   void* g;                  // [rows][g_ld]

@@ -156,7 +156,7 @@ __device__ __forceinline__ RowGrad row_grad(const wcn_ce_piece& q, int row, floa
   g.label = in >= 0 && in < q.classes ? (int)in : -1;
   if (q.row_scale) {
     const float most = __ldg(q.row_max);
-    g.scale = most > 0.f ? __ldg(&q.row_scale[row]) / most : most == most ? 0.f : most;
+    g.scale = __ldg(&q.row_scale[row]) / (most > 0.f ? most : 1.f);
   }
   return g;
 }

@@ -22,17 +22,17 @@ def check_reduction(reduction: str) -> int:
         raise ValueError(f"reduction is one of {list(_REDUCTIONS)}, got {reduction!r}") from None
 
 
-def _matrix(t: Tensor):
+def _matrix(t: Tensor, c: int = 0):
     """``t`` as the kernels read it (unit stride along the channels; in 16 bits rows on 16-byte boundaries) and the elements from
-    row to row.  Copied where it is not so already."""
-    n, c = t.shape
+    row to row.  Copied where it is not so already.  ``c``: the channels of a copy that this function has made (rows may be longer)."""
+    n, c = t.shape[0], c or t.shape[1]
     whole = 1 if t.dtype == torch.float32 else 8
     padded = -(-c // whole) * whole
     one_row = n == 1
     if (t.stride(1) == 1 or c == 1) and (one_row or (t.stride(0) >= c and t.stride(0) % whole == 0)) and t.data_ptr() % (2 * whole) == 0:
         return t, padded if one_row else t.stride(0)
     rows = torch.empty((n, padded), dtype=t.dtype, device=t.device)
-    rows[:, :c].copy_(t)
+    rows[:, :c].copy_(t[:, :c])
     return rows, padded
 
 
@@ -47,7 +47,8 @@ def _kept(n: int, v: int, bias: bool):
 
 
 def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: int):
-    """(loss or losses, what the backward pass needs: log-sum-exp and loss of each row, the count, the bias in units of ln 2)"""
+    """(loss or losses, what the backward pass needs: log-sum-exp and loss of each row, the count, the bias in units of ln 2; the
+    matrices as the kernels read them)"""
     (n, c), v, dev = x.shape, weight.shape[0], x.device
     code, stream = dtype_code(x.dtype), stream_ptr(dev)
     x, x_ld = _matrix(x)
@@ -62,12 +63,13 @@ def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], 
                                   ptr(labels), ignore_index, code, reduction, base, base + 4 * n, base + 4 * at_bias if bias is not None else None,
                                   base + 4 * at_count, ptr(loss), ptr(ws), ws.numel(), ptr(_counter(dev, stream)), ptr(device_status(dev)), stream),
               "wcn_linear_ce")
-    return (loss if reduction else kept[n:2 * n]), kept
+    return (loss if reduction else kept[n:2 * n]), kept, x, weight
 
 
 def formula(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: str) -> Tensor:
     """The same through torch, logits and all: for a graph of the gradient, forward-mode differentiation and function transforms."""
     z = x.float() @ weight.float().t()
+    labels = torch.where((labels >= 0) & (labels < weight.shape[0]), labels, ignore_index)
     return torch.nn.functional.cross_entropy(z if bias is None else z + bias.float(), labels, ignore_index=ignore_index, reduction=reduction)
 
 
@@ -75,14 +77,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], labels: Tensor, ignore_index: int, reduction: str):
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        loss, kept = _forward(x.detach(), weight.detach(), labels, None if bias is None else bias.detach().contiguous(),
-                              ignore_index, _REDUCTIONS[reduction])
-        ctx.save_for_backward(x, weight, bias, labels, kept)
+        loss, kept, x_rows, w_rows = _forward(x.detach(), weight.detach(), labels, None if bias is None else bias.detach().contiguous(),
+                                              ignore_index, _REDUCTIONS[reduction])
+        # (matrices that had to be copied are kept with them: there are not two copies to be made)
+        copied = tuple(None if rows.data_ptr() == given.data_ptr() else rows for rows, given in ((x_rows, x), (w_rows, weight)))
+        ctx.save_for_backward(x, weight, bias, labels, kept, *copied)
         return loss.clone() if reduction == "none" else loss   # (the row losses are kept: the caller's are its own)
 
     @staticmethod
     def backward(ctx, grad: Tensor):
-        x, weight, bias, labels, kept = ctx.saved_tensors
+        x, weight, bias, labels, kept, x_rows, w_rows = ctx.saved_tensors
         if torch.is_grad_enabled():  # a graph of the gradient is wanted
             loss = formula(x, weight, labels, bias, ctx.ignore_index, ctx.reduction)
             wanted = [t for t, need in zip((x, weight, bias), ctx.needs_input_grad) if need]
@@ -97,9 +101,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         grad = grad.float().contiguous()
         at_count, at_bias, _ = _kept(n, v, bias is not None)
         base = kept.data_ptr()
-        row_max = grad.abs().amax() if ctx.reduction == "none" else None
-        x, x_ld = _matrix(x)
-        weight, w_ld = _matrix(weight)
+        # (numbers beside which the others keep their precision: what is no number stays with its row)
+        row_max = torch.where(torch.isfinite(grad), grad.abs(), 0.0).amax() if ctx.reduction == "none" else None
+        x, x_ld = _matrix(x if x_rows is None else x_rows, c)
+        weight, w_ld = _matrix(weight if w_rows is None else w_rows, c)
         ws = _workspace(n, c, v, code, need_x + 2 * need_w + 4 * need_b, dev)
         with on_device(dev):
             check(lib().wcn_linear_ce_backward(ptr(x), x_ld, n, c, ptr(weight), w_ld, v, base + 4 * at_bias if bias is not None else None,
