@@ -281,7 +281,7 @@ __device__ __forceinline__ void tile_stats(const Params& p, const Place& at, con
   const T* const x = reinterpret_cast<const T*>(p.x);
   for (int pc = at.tx; pc - at.tx < at.pieces; pc += at.txs) {
     if (at.ty < at.tys && pc < at.pieces) {
-      // About the thread's first row: at most 64 rows, of which a far first one spoils the others' distances by no more than
+      // About the thread's first row: at most 67 rows, of which a far first one spoils the others' distances by no more than
       // its own distance counts for.
       constexpr int P = (V + 1) / 2;
       float2 first[P], s1[P], s2[P];     // (its negative)
@@ -361,7 +361,7 @@ __device__ __forceinline__ void join_stats(const Params& p, const Tile& t, int n
     float about = 0.f;
     if (g < p.G) {
       about = __ldcg(&p.part[(int64_t)t.first * p.G + g]).x;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = t.first + lane; i < t.last; i += width) {
         const float2 v = __ldcg(&p.part[(int64_t)i * p.G + g]);
         const double k = (double)(i == t.last - 1 ? n_last : p.rows), d = (double)v.x - (double)about;
@@ -388,7 +388,7 @@ __device__ __forceinline__ void join_grad_sums(const Params& p, const Tile& t, i
   per_group(p.G, [&](int g, int lane, int width) {
     double a = 0, b = 0;
     if (g < p.G)
-#pragma unroll 4
+#pragma unroll 8
       for (int i = t.first + lane; i < t.last; i += width) {
         const float2 v = __ldcg(&p.part[(int64_t)i * p.G + g]);
         a += (double)v.x;
@@ -413,17 +413,27 @@ template <int V, int SUB> __device__ __forceinline__ float2 of_pair(const float 
   return make_float2(v[2 * i * SUB / V], v[V == 1 ? 0 : (2 * i + 1) * SUB / V]);
 }
 
-template <typename T, int V, int ACT, int SUB>
-__device__ __forceinline__ void tile_apply(const Params& p, const Place& at, const Tile& t, bool ok) {
+// ready(): waits for the scene's sums (all threads); what does not depend on them is asked for before.
+template <typename T, int V, int ACT, int SUB, typename R>
+__device__ __forceinline__ void tile_apply(const Params& p, const Place& at, const Tile& t, R&& ready) {
   constexpr int P = (V + 1) / 2;
-  if (at.ty >= at.tys) return;
+  bool ok = false, asked = false;
   const int rows = rows_of(p, at, t.hi - t.lo);
   const int64_t step = (int64_t)at.tys * p.x_ld, out_step = (int64_t)at.tys * p.C;
-  for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
+  for (int pc = at.tx; pc < at.pieces || !asked; pc += at.txs) {
+    const int c0 = min(pc, at.pieces - 1) * V;
     const T* const from = reinterpret_cast<const T*>(p.x) + (int64_t)(t.lo + at.ty) * p.x_ld + pc * V;
     T* const to = reinterpret_cast<T*>(p.out) + (int64_t)(t.lo + at.ty) * p.C + pc * V;
     float mean[SUB], rstd[SUB];
     float2 scale[P], beta[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      scale[i] = pair_at<V>(p.gamma, c0 + 2 * i, 1.f);
+      beta[i] = pair_at<V>(p.beta, c0 + 2 * i, 0.f);
+    }
+    if (!asked) ok = ready();
+    asked = true;
+    if (at.ty >= at.tys || pc >= at.pieces) return;
 #pragma unroll
     for (int k = 0; k < SUB; ++k) {
       const int g = (pc * V + k * (V / SUB)) / p.per;
@@ -433,8 +443,7 @@ __device__ __forceinline__ void tile_apply(const Params& p, const Place& at, con
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), pair_at<V>(p.gamma, pc * V + 2 * i, 1.f));
-      beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
+      scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), scale[i]);
       const float2 m = of_pair<V, SUB>(mean, i);
       if (sizeof(T) == 2) beta[i] = __ffma2_rn(make_float2(-m.x, -m.y), scale[i], beta[i]);
     }
@@ -539,8 +548,9 @@ __device__ __forceinline__ void tile_grad_sums(const Params& p, const Place& at,
   });
 }
 
-template <typename T, int V, int ACT, int SUB>
-__device__ __forceinline__ void tile_grad_apply(const Params& p, const Place& at, const Tile& t, bool ok) {
+template <typename T, int V, int ACT, int SUB, typename R>
+__device__ __forceinline__ void tile_grad_apply(const Params& p, const Place& at, const Tile& t, R&& ready) {
+  const bool ok = ready();   // (asking for more before that costs registers, and with SiLU 6 %)
   if (at.ty >= at.tys) return;
   const int64_t step = (int64_t)at.tys * p.x_ld, dy_step = (int64_t)at.tys * p.dy_ld, out_step = (int64_t)at.tys * p.C;
   for (int pc = at.tx; pc < at.pieces; pc += at.txs) {
@@ -632,28 +642,32 @@ __global__ void __launch_bounds__(THREADS, BACK ? BLOCKS_BACKWARD : BLOCKS_FORWA
       if (it.kind == 0) {
         if constexpr (BACK) tile_grad_sums<T, V, ACT, SUB>(p, at, t, it.at, smem);
         else tile_stats<T, V>(p, at, t, it.at, smem);
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) s_last = atomicAdd(&p.sync->tiles[t.scene], 1) == t.last - t.first - 1;
+        if (threadIdx.x == 0) {
+          __threadfence();   // (of what the block has written)
+          s_last = atomicAdd(&p.sync->tiles[t.scene], 1) == t.last - t.first - 1;
+        }
         __syncthreads();
         if (s_last) {
           __threadfence();
           const int n = scenes.row0[t.scene + 1] - scenes.row0[t.scene];
           if constexpr (BACK) join_grad_sums(p, t, n);
           else join_stats<T, V>(p, t, n);
-          __threadfence();
           __syncthreads();
           if (threadIdx.x == 0) {
-            store_release(&p.sync->flag[t.scene], 1);
             __threadfence();
+            store_release(&p.sync->flag[t.scene], 1);
             atomicAdd(&p.sync->scenes, 1);
           }
         }
       } else {
-        if (threadIdx.x == 0) s_ok = wait_for(&p.sync->flag[t.scene], 1, p.dev_status);
-        __syncthreads();
-        if constexpr (BACK) tile_grad_apply<T, V, ACT, SUB>(p, at, t, s_ok);
-        else tile_apply<T, V, ACT, SUB>(p, at, t, s_ok);
+        auto ready = [&]() -> bool {
+          if (threadIdx.x == 0) s_ok = wait_for(&p.sync->flag[t.scene], 1, p.dev_status);
+          __syncthreads();
+          return s_ok;
+        };
+        if constexpr (BACK) tile_grad_apply<T, V, ACT, SUB>(p, at, t, ready);
+        else tile_apply<T, V, ACT, SUB>(p, at, t, ready);
       }
     }
     __syncthreads();
@@ -694,20 +708,26 @@ size_t sums_smem(int C, int vec) {
 // Scenes [i, j) of a launch.
 struct Part { int64_t i, j; int rows, tiles, most; };   // rows of a tile; tiles of all scenes and of the longest one
 
-// f(part) for each launch.  Tiles of up to 64 rows a thread (32 backward, where there are two numbers for each), fewer where
-// there would not be one for each block.
+// f(part) for each launch.  Tiles of up to 64 rows a thread (32 backward, where there are two numbers for each), of such a size
+// that the blocks have whole rounds of them (8 x 150 000 x 96 fp16: seven rounds of 64 rows or eight of 49 for both looks).
 template <typename F> int in_launches(const int64_t* offsets, int64_t scenes, bool back, int tys, F&& f) {
   for (int64_t i = 0; i < scenes;) {
     Part q = {i, i, 0, 0, 0};
     int count = 0;   // scenes with rows
     for (; q.j < scenes && count < SCENES; ++q.j) count += offsets[q.j + 1] > offsets[q.j];
-    const int64_t n = offsets[q.j] - offsets[i], side = (int64_t)tys * (back ? BLOCKS_BACKWARD : BLOCKS_FORWARD) * wcn_num_sms(), per = (n + side - 1) / side;
-    const int most = back ? 32 : 64, least = 4;
-    q.rows = (int)(per < least ? least : per > most ? most : per) * tys;
-    for (int64_t k = i; k < q.j; ++k) {
-      const int tiles = (int)((offsets[k + 1] - offsets[k] + q.rows - 1) / q.rows);
-      q.tiles += tiles;
-      if (tiles > q.most) q.most = tiles;
+    const int64_t n = offsets[q.j] - offsets[i], blocks = (back ? BLOCKS_BACKWARD : BLOCKS_FORWARD) * wcn_num_sms(), side = tys * blocks;
+    const int64_t most = back ? 32 : 64, least = 4, rounds = (n + side * most - 1) / (side * most);
+    int64_t per = rounds ? (n + side * rounds - 1) / (side * rounds) : least;
+    if (per < least) per = least;
+    for (int tries = 0;; ++tries, ++per) {
+      q.rows = (int)per * tys;
+      q.tiles = q.most = 0;
+      for (int64_t k = i; k < q.j; ++k) {
+        const int tiles = (int)((offsets[k + 1] - offsets[k] + q.rows - 1) / q.rows);
+        q.tiles += tiles;
+        if (tiles > q.most) q.most = tiles;
+      }
+      if (q.tiles <= rounds * blocks || tries == 3 || count > 16) break;   // (the scenes' last tiles are smaller ones)
     }
     i = q.j;
     const int rc = q.tiles ? f(q) : WCN_OK;
