@@ -16,7 +16,8 @@
 #include "linear_ce.cuh"
 
 int wcn_ce_logits_parts(int rows, int classes);
-int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st);
+int wcn_ce_whole_blocks(int rows, int classes, int channels);
+int wcn_ce_logits(const wcn_ce_piece& q, const wcn_ce_result* out, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st);
 int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias);
 int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
                 int32_t* dev_status, cudaStream_t st);
@@ -190,8 +191,7 @@ struct JoinParams {
   int n_tiles, chunk;      // splits of a row as ce_rows_kernel leaves them (chunk 0: `splits` for all)
 };
 
-template <typename TO, int SIDE>
-__global__ void __launch_bounds__(THREADS) ce_join_kernel(const __grid_constant__ JoinParams p) {
+template <typename TO, int SIDE> __device__ __forceinline__ void join_quads(const JoinParams& p) {
   constexpr int QUADS = THREADS / SIDE;
   __shared__ double part[SIDE > 1 ? THREADS : 1][4];
   const int side = threadIdx.x / QUADS, at = threadIdx.x % QUADS;
@@ -250,12 +250,15 @@ __global__ void __launch_bounds__(THREADS) ce_join_kernel(const __grid_constant_
   }
 }
 
+template <typename TO, int SIDE>
+__global__ void __launch_bounds__(THREADS) ce_join_kernel(const __grid_constant__ JoinParams p) { join_quads<TO, SIDE>(p); }
+
 // The same of one number a class: 32 classes a block, eight threads that share the splits.
 template <typename TO>
-__global__ void __launch_bounds__(THREADS) ce_join_sums_kernel(const __grid_constant__ JoinParams p) {
+__device__ __forceinline__ void join_sums(const JoinParams& p, int block) {
   __shared__ double part[THREADS / 32][33];
   const int lane = threadIdx.x & 31, side = threadIdx.x >> 5;
-  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t i = (int64_t)block * 32 + lane;
   double v = 0;
   if (i < p.m)
 #pragma unroll 4
@@ -275,6 +278,16 @@ __global__ void __launch_bounds__(THREADS) ce_join_sums_kernel(const __grid_cons
   reinterpret_cast<TO*>(p.out)[i] = wcn_from_float<TO>((float)v * scale);
 }
 
+template <typename TO>
+__global__ void __launch_bounds__(THREADS) ce_join_sums_kernel(const __grid_constant__ JoinParams p) { join_sums<TO>(p, blockIdx.x); }
+
+// Both of a small head in one launch: the blocks behind the first `blocks` do the second one's.
+template <typename TO>
+__global__ void __launch_bounds__(THREADS) ce_join_both_kernel(const __grid_constant__ JoinParams p, const __grid_constant__ JoinParams sums, int blocks) {
+  if ((int)blockIdx.x < blocks) join_quads<TO, 8>(p);
+  else join_sums<TO>(sums, blockIdx.x - blocks);
+}
+
 template <typename TO> int join_as(const JoinParams& p, cudaStream_t st) {
   if (p.ld == 1) {
     ce_join_sums_kernel<TO><<<(unsigned)((p.m + 31) / 32), THREADS, 0, st>>>(p);
@@ -289,6 +302,15 @@ int join(const JoinParams& p, int dtype, cudaStream_t st) {
   if (dtype == WCN_F32) return join_as<float>(p, st);
   if (dtype == WCN_F16) return join_as<__half>(p, st);
   return join_as<__nv_bfloat16>(p, st);
+}
+
+template <typename TO> int join_both_as(const JoinParams& p, const JoinParams& sums, cudaStream_t st) {
+  const int blocks = (int)((p.m * (p.ld / 4) + THREADS / 8 - 1) / (THREADS / 8));
+  ce_join_both_kernel<TO><<<(unsigned)(blocks + (sums.m + 31) / 32), THREADS, 0, st>>>(p, sums, blocks);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+int join_both(const JoinParams& p, const JoinParams& sums, int dtype, cudaStream_t st) {
+  return dtype == WCN_F16 ? join_both_as<__half>(p, sums, st) : dtype == WCN_F32 ? join_both_as<float>(p, sums, st) : join_both_as<__nv_bfloat16>(p, sums, st);
 }
 
 // ------------------------------------------------------------------ fp32
@@ -543,6 +565,14 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   wcn_linear_ce_workspace_bytes(n, channels, classes, dtype, 0, &need);
   if (need > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   cudaStream_t st = wcn_stream(stream);
+  if (const int blocks = dtype == WCN_F32 || classes > 256 ? 0 : wcn_ce_whole_blocks((int)n, (int)classes, channels)) {
+    wcn_ce_piece q = {};
+    q.x = x; q.w = w; q.x_ld = x_ld; q.w_ld = w_ld; q.rows = (int)n; q.classes = (int)classes; q.channels = channels;
+    q.labels = labels; q.ignore = ignore; q.all_classes = classes;
+    double* const sums = (double*)workspace;
+    const wcn_ce_result out = {bias, bias_dtype, reduction, bias2, lse2, loss_rows, reduction ? loss : nullptr, count, sums, (int32_t*)(sums + blocks), counter};
+    return wcn_ce_logits(q, &out, dtype, false, 0.f, dev_status, st);
+  }
   if (bias) {
     const int64_t padded = (classes + 255) / 256 * 256 + 256;
     const unsigned blocks = (unsigned)((padded + THREADS - 1) / THREADS < 1024 ? (padded + THREADS - 1) / THREADS : 1024);
@@ -558,7 +588,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   if (dtype == WCN_F32) {
     ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)((classes + TILE - 1) / TILE)), THREADS, 0, st>>>(q);
   } else {
-    const int rc = wcn_ce_logits(q, dtype, false, 0.f, dev_status, st);
+    const int rc = wcn_ce_logits(q, nullptr, dtype, false, 0.f, dev_status, st);
     if (rc != WCN_OK) return rc;
   }
   LossParams p = {};
@@ -599,8 +629,10 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
     q.row_scale = row_max ? grad : nullptr; q.row_max = row_max;
     float *const slab = dw || dbias ? (float*)(ws + p.slab_w) : nullptr, *const ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
     int rc = wcn_ce_head(q, scale, dx, slab, ones, dtype, lift, dev_status, st);
-    if (rc == WCN_OK && dw) rc = join({slab, nullptr, false, dw, classes, channels, p.ld, p.head, scale, dev_status}, dtype, st);
-    if (rc == WCN_OK && dbias) rc = join({ones, nullptr, false, dbias, classes, 1, 1, p.head, scale, dev_status}, bias_dtype, st);
+    const JoinParams for_w = {slab, nullptr, false, dw, classes, channels, p.ld, p.head, scale, dev_status}, for_b = {ones, nullptr, false, dbias, classes, 1, 1, p.head, scale, dev_status};
+    if (rc == WCN_OK && dw && dbias && bias_dtype == dtype) return join_both(for_w, for_b, dtype, st);
+    if (rc == WCN_OK && dw) rc = join(for_w, dtype, st);
+    if (rc == WCN_OK && dbias) rc = join(for_b, bias_dtype, st);
     return rc;
   }
   for (int i = 0; i < p.row_pieces; ++i) {
@@ -626,7 +658,7 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
           rc = join({slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? (char*)dx + r0 * channels * e : nullptr, rows, channels, p.ld, slots, scale, dev_status,
                      (vs + 127) / 128, chunk}, dtype, st);
       } else if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q);
-      else rc = wcn_ce_logits(q, dtype, true, lift, dev_status, st);
+      else rc = wcn_ce_logits(q, nullptr, dtype, true, lift, dev_status, st);
       if (rc != WCN_OK) return rc;
       if (dx && !p.fused) {
         wcn_ce_product d = {};
@@ -651,6 +683,12 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
         rc = dtype == WCN_F32 ? fp32_product(d, true, st) : wcn_ce_product_run(d, true, p.fused, dtype, dev_status, st);
         if (rc != WCN_OK) return rc;
         const bool done = i == p.row_pieces - 1;
+        if (dw && dbias && p.row_pieces == 1 && dtype == bias_dtype && d.splits >= 16) {
+          rc = join_both({d.slab, nullptr, false, (char*)dw + v0 * channels * e, vs, channels, p.ld, d.splits, scale, dev_status},
+                         {d.slab_ones, nullptr, false, (char*)dbias + v0 * e, vs, 1, 1, d.splits, scale, dev_status}, dtype, st);
+          if (rc != WCN_OK) return rc;
+          continue;
+        }
         if (dw) {
           JoinParams jp = {d.slab, (float*)(ws + p.acc_w) + v0 * p.ld, i > 0, done ? (char*)dw + v0 * channels * e : nullptr, vs, channels, p.ld, d.splits, scale, dev_status};
           rc = join(jp, dtype, st);

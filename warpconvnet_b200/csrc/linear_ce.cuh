@@ -29,6 +29,20 @@ struct wcn_ce_piece {
   int64_t g_ld;
 };
 
+// Where the forward pass leaves its results when all classes of a row are one tile's (linear_ce.cu does it otherwise).
+struct wcn_ce_result {
+  const void* bias;         // as given, of bias_dtype (null: none)
+  int bias_dtype, reduction;
+  float* bias2;             // [classes rounded up to 256, + 256]
+  float* lse2;
+  float* loss_rows;
+  float* loss;              // null: none wanted
+  int32_t* count;
+  double* block_sums;       // [blocks]
+  int32_t* block_counts;
+  unsigned* counter;
+};
+
 // D[m][n] = sum over k of A[m][k] B[k][n]: the sums of each split of k, or the finished result.
 struct wcn_ce_product {
   const void* a;            // [k][m] (transposed) or [m][k]

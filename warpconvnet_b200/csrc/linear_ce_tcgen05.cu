@@ -111,6 +111,7 @@ enum Resident { NOTHING = 0, ROWS = 1, CLASSES = 2 };
 
 struct LogitParams {
   wcn_ce_piece q;
+  wcn_ce_result out;      // forward with the classes resident
   int KB;                 // slices of 64 channels
   int NT;                 // classes of a tile
   int m_tiles, n_tiles, splits, per, units, stages, tmem_cols;
@@ -123,7 +124,7 @@ template <int W> __device__ __forceinline__ void to_logits(const wcn_ce_piece& q
   if (q.bias2) {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const float4 b = __ldg(reinterpret_cast<const float4*>(q.bias2 + col + i));
+      const float4 b = *reinterpret_cast<const float4*>(q.bias2 + col + i);
       z[i] = fmaf(__uint_as_float(r[i]), LOG2E, b.x);
       z[i + 1] = fmaf(__uint_as_float(r[i + 1]), LOG2E, b.y);
       z[i + 2] = fmaf(__uint_as_float(r[i + 2]), LOG2E, b.z);
@@ -174,6 +175,54 @@ template <int W, bool BF16> __device__ __forceinline__ void gradients(const wcn_
   }
 }
 
+// What the parts of a row come to together, in shared memory (forward with the classes resident: a tile has whole rows).
+struct WholeRows {
+  float bias2[256];
+  float4 part[2][PARTS][TILE_M];      // (largest, sum, the label's logit if it is this part's); tiles in turns
+  uint64_t full[2], empty[2];
+  double sums[4];
+  int counts[4];
+  int last;
+};
+
+__device__ __forceinline__ float bias_at(const wcn_ce_result& o, int i) {
+  if (o.bias_dtype == WCN_F32) return reinterpret_cast<const float*>(o.bias)[i];
+  if (o.bias_dtype == WCN_F16) return __half2float(reinterpret_cast<const __half*>(o.bias)[i]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(o.bias)[i]);
+}
+
+// The block's sum of losses, and of the last block to get here the mean or the sum (in a fixed order).
+__device__ void finish_loss(const wcn_ce_result& o, WholeRows* w, bool failed) {
+  if (threadIdx.x == 0) {
+    double total = 0;
+    int counted = 0;
+    for (int i = 0; i < 4; ++i) { total += w->sums[i]; counted += w->counts[i]; }
+    o.block_sums[blockIdx.x] = failed ? (double)__int_as_float(0x7FC00000) : total;
+    o.block_counts[blockIdx.x] = counted;
+    __threadfence();
+    w->last = atomicAdd(o.counter, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!w->last || threadIdx.x >= 32) return;
+  __threadfence();
+  double total = 0;
+  int counted = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 32) {
+    total += __ldcg(&o.block_sums[i]);
+    counted += __ldcg(&o.block_counts[i]);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+    counted += __shfl_xor_sync(0xFFFFFFFFu, counted, d);
+  }
+  if (threadIdx.x == 0) {
+    *o.loss = (float)(o.reduction == 1 ? total / (double)counted : total);
+    *o.count = counted;
+    *o.counter = 0;
+  }
+}
+
 template <int RES, bool GRAD, bool BF16>
 __global__ void __launch_bounds__(LOGIT_THREADS, 1)
 ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ LogitParams p) {
@@ -185,7 +234,33 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t res = base + (uint32_t)(p.stages * stage_bytes);
   Control* ctl = reinterpret_cast<Control*>(smem_raw + (base - smem_u32(smem_raw)) + p.stages * stage_bytes + (RES == NOTHING ? 0 : p.KB * res_slice));
-  if (!begin(ctl, p.stages, p.tmem_cols, LOGIT_WARPS, p.dev_status)) return;
+  constexpr bool WHOLE = RES == CLASSES && !GRAD;           // losses are finished here
+  WholeRows* const whole = reinterpret_cast<WholeRows*>(reinterpret_cast<uint8_t*>(ctl) + (sizeof(Control) + 15) / 16 * 16);
+  auto mark = [&]() {   // no losses of this block's rows
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x)
+      for (int r = threadIdx.x; r < TILE_M; r += LOGIT_THREADS)
+        if (u * TILE_M + r < p.q.rows) p.out.lse2[u * TILE_M + r] = p.out.loss_rows[u * TILE_M + r] = __int_as_float(0x7FC00000);
+  };
+  wcn_ce_piece q = p.q;
+  if (WHOLE) {
+    if (threadIdx.x < 4) { whole->sums[threadIdx.x] = 0; whole->counts[threadIdx.x] = 0; }
+    if (threadIdx.x == 0)
+      for (int i = 0; i < 2; ++i) { mbar_init(bar(&whole->full[i]), LOGIT_WARPS); mbar_init(bar(&whole->empty[i]), 4); }
+    if (p.out.bias) {
+      for (int i = threadIdx.x; i < 256; i += LOGIT_THREADS) whole->bias2[i] = i < q.classes ? bias_at(p.out, i) * LOG2E : -INFINITY;
+      if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < 512; i += LOGIT_THREADS) p.out.bias2[i] = i < q.classes ? bias_at(p.out, i) * LOG2E : -INFINITY;
+      q.bias2 = whole->bias2;
+    }
+  }
+  if (!begin(ctl, p.stages, p.tmem_cols, LOGIT_WARPS, p.dev_status)) {
+    if (WHOLE) {
+      mark();
+      __syncthreads();
+      if (p.out.loss) finish_loss(p.out, whole, true);
+    }
+    return;
+  }
   const uint32_t tmem = ctl->tmem_holder;
   bool ok = true;
 
@@ -264,7 +339,9 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
   } else {
     const int quarter = warp & 3, part = (warp - EPI_WARP0) >> 2;
     const int pieces = p.NT / 16, first = pieces * part / PARTS, last = pieces * (part + 1) / PARTS;   // of 16 columns
-    int ab = 0, aphase = 0;
+    int ab = 0, aphase = 0, tiles = 0, counted = 0;
+    double total = 0;
+    bool bad = false;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
       const int m = u % p.m_tiles, split = u / p.m_tiles, n0 = split * p.per, n1 = min(n0 + p.per, p.n_tiles);
       const int row = m * TILE_M + quarter * 32 + lane;
@@ -272,6 +349,10 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
       float top = -INFINITY, sum = 0.f;                  // forward
       RowGrad rg = {};                                   // backward
       if (GRAD) rg = row_grad(p.q, row, p.lift);
+      const int64_t y = WHOLE && live ? __ldg(&p.q.labels[row]) : p.q.ignore;
+      const bool counts = WHOLE && y != p.q.ignore && y >= 0 && y < p.q.all_classes;
+      const int label = counts ? (int)y : -1;
+      float z_label = -INFINITY;
       for (int n = n0; n < n1; ++n) {
         if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
@@ -285,7 +366,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
           tmem_ld_wait();
           float z[W];
           const int col = col0 + c;
-          to_logits<W>(p.q, r, col, z);
+          to_logits<W>(q, r, col, z);
           if (!GRAD) {
             float m8[8];
 #pragma unroll
@@ -302,6 +383,10 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
             for (int i = 0; i < W; ++i) s4[i & 3] += exp2_fast(z[i] - by);
             sum = fmaf(sum, exp2_fast(top - by), (s4[0] + s4[1]) + (s4[2] + s4[3]));
             top = now;
+            if (WHOLE) {
+#pragma unroll
+              for (int i = 0; i < W; ++i) z_label = col + i == label ? z[i] : z_label;
+            }
           } else {
             uint32_t out[W / 2];
             gradients<W, BF16>(p.q, rg, z, out);
@@ -322,12 +407,68 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
         if (++ab == 2) { ab = 0; aphase ^= 1; }
       }
       if (!ok) break;
-      if (!GRAD && live) p.q.part[(int64_t)(split * PARTS + part) * p.q.rows + row] = make_float2(top, sum);
+      if (WHOLE) {
+        const int turn = tiles & 1, phase = (tiles >> 1) & 1;
+        if (tiles > 1) ok = mbar_wait(bar(&whole->empty[turn]), phase ^ 1, p.dev_status);
+        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+        whole->part[turn][part][quarter * 32 + lane] = make_float4(top, sum, z_label, label >= 0 && label / 16 >= first && label / 16 < last ? 1.f : 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(&whole->full[turn]));
+        if (part == 0) {
+          ok = mbar_wait(bar(&whole->full[turn]), phase, p.dev_status);
+          if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+        }
+        if (part == 0 && live) {
+          float all = -INFINITY, s = 0.f, z = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k) all = fmaxf(all, whole->part[turn][k][quarter * 32 + lane].x);
+          const float by = all == -INFINITY ? 0.f : all;
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k) {
+            const float4 v = whole->part[turn][k][quarter * 32 + lane];
+            s += v.y * exp2f(v.x - by);
+            if (v.w != 0.f) z = v.z;
+          }
+          const float lse2 = all + log2f(s);
+          float loss = 0.f;
+          if (counts) {
+            loss = (lse2 - z) * 0.69314718055994531f;
+            if (loss < 0.f) loss = 0.f;                    // (roundings of a probability of one)
+          }
+          bad |= y != p.q.ignore && !counts;
+          p.out.lse2[row] = lse2;
+          p.out.loss_rows[row] = loss;
+          total += (double)loss;
+          counted += counts;
+        }
+        __syncwarp();
+        if (part == 0 && lane == 0) mbar_arrive(bar(&whole->empty[turn]));
+        ++tiles;
+      } else if (!GRAD && live) {
+        p.q.part[(int64_t)(split * PARTS + part) * p.q.rows + row] = make_float2(top, sum);
+      }
+    }
+    if (WHOLE && part == 0) {
+      if (bad) wcn_report_bounds(p.dev_status);
+      __syncwarp();
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+        counted += __shfl_xor_sync(0xFFFFFFFFu, counted, o);
+      }
+      if (lane == 0) { whole->sums[quarter] = total; whole->counts[quarter] = counted; }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  if (WHOLE) {
+    if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+    __syncthreads();
+    const bool failed = ctl->skip == (int)WCN_ERR_WAIT_EXPIRED;
+    if (failed) mark();
+    if (p.out.loss) finish_loss(p.out, whole, failed);
+  }
 }
 
 // ------------------------------------------------------------------ products
@@ -1043,10 +1184,16 @@ int launch_logits(LogitParams& p, size_t fixed, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
+constexpr size_t FIXED = sizeof(Control) + 1024 + 128, FIXED_WHOLE = FIXED + sizeof(WholeRows) + 16;
+
+// Whether the forward kernel finishes the losses: all classes one tile that stays in shared memory.
+bool whole_rows(const LogitParams& p) { return p.n_tiles == 1 && p.KB * (int64_t)p.NT * SLICE * 2 + 4 * A_BYTES + (int64_t)FIXED_WHOLE <= SMEM_BUDGET; }
+
 template <bool GRAD, bool BF16> int by_resident(LogitParams& p, cudaStream_t st) {
-  const size_t fixed = sizeof(Control) + 1024 + 128;
+  const size_t fixed = FIXED;
   const int64_t b_bytes = (int64_t)p.NT * SLICE * 2;
-  if (p.n_tiles == 1 && p.KB * b_bytes + 4 * A_BYTES + (int64_t)fixed <= SMEM_BUDGET) return launch_logits<CLASSES, GRAD, BF16>(p, fixed, st);
+  if (!GRAD && whole_rows(p)) return launch_logits<CLASSES, GRAD, BF16>(p, FIXED_WHOLE, st);
+  if (GRAD && p.n_tiles == 1 && p.KB * b_bytes + 4 * A_BYTES + (int64_t)fixed <= SMEM_BUDGET) return launch_logits<CLASSES, GRAD, BF16>(p, fixed, st);
   if (p.KB * (int64_t)A_BYTES + 3 * b_bytes + (int64_t)fixed <= SMEM_BUDGET) return launch_logits<ROWS, GRAD, BF16>(p, fixed, st);
   return launch_logits<NOTHING, GRAD, BF16>(p, fixed, st);
 }
@@ -1176,9 +1323,19 @@ int wcn_ce_logits_parts(int rows, int classes) {
   return p.splits * PARTS;
 }
 
-int wcn_ce_logits(const wcn_ce_piece& q, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st) {
+// Blocks of a forward kernel that finishes the losses itself; 0: it leaves parts.
+int wcn_ce_whole_blocks(int rows, int classes, int channels) {
+  LogitParams p = {};
+  p.KB = (channels + SLICE - 1) / SLICE;
+  plan_logits(rows, classes, &p);
+  const int sms = wcn_num_sms();
+  return whole_rows(p) ? (p.units < sms ? p.units : sms) : 0;
+}
+
+int wcn_ce_logits(const wcn_ce_piece& q, const wcn_ce_result* out, int dtype, bool gradient, float lift, int32_t* dev_status, cudaStream_t st) {
   LogitParams p = {};
   p.q = q;
+  if (out) p.out = *out;
   p.lift = lift;
   p.dev_status = dev_status;
   p.KB = (q.channels + SLICE - 1) / SLICE;
