@@ -21,7 +21,7 @@ int wcn_ce_logits(const wcn_ce_piece& q, const wcn_ce_result* out, int dtype, bo
 int wcn_ce_head_blocks(int64_t rows, int channels, int classes, bool bias);
 int wcn_ce_head(const wcn_ce_piece& q, const wcn_ce_scale& scale, void* dx, float* slab, float* slab_ones, int dtype, float lift,
                 int32_t* dev_status, cudaStream_t st);
-int wcn_ce_product_splits(int m, int n, int k, bool blocked);
+int wcn_ce_product_splits(int m, int n, int k, bool blocked, bool ones);
 int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st);
 bool wcn_ce_rows_taken(int channels);
 void wcn_ce_rows_plan(int rows, int classes, int* chunk, int* slots);
@@ -463,8 +463,8 @@ int loss_blocks(int64_t n) {
   const int64_t want = (n + THREADS / 8 - 1) / (THREADS / 8), most = 8 * (int64_t)wcn_num_sms();
   return (int)(want < most ? want : most);
 }
-int product_splits(int m, int n, int k, int dtype, bool blocked = false) {
-  return dtype == WCN_F32 ? fp32_splits(m, n, k) : wcn_ce_product_splits(m, n, k, blocked);
+int product_splits(int m, int n, int k, int dtype, bool blocked = false, bool ones = false) {
+  return dtype == WCN_F32 ? fp32_splits(m, n, k) : wcn_ce_product_splits(m, n, k, blocked, ones);
 }
 
 // How the gradient of the logits is cut into pieces, and where everything is in the workspace.
@@ -517,7 +517,7 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
       int chunk, slots;
       if (p.fused) wcn_ce_rows_plan((int)r, (int)k, &chunk, &slots);
       else slots = product_splits((int)r, c, (int)k, dtype);
-      const int64_t fx = slots * r * p.ld * 4, s = product_splits((int)k, c, (int)r, dtype, p.fused);
+      const int64_t fx = slots * r * p.ld * 4, s = product_splits((int)k, c, (int)r, dtype, p.fused, b);
       if (fx > sx) sx = fx;
       if (s * k * p.ld * 4 > sw) sw = s * k * p.ld * 4;
       if (s * k * 4 > sb) sb = s * k * 4;
@@ -678,7 +678,7 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
       if (dw || dbias) {
         wcn_ce_product d = {};
         d.a = q.g; d.a_ld = p.fused ? (vs + 127) / 128 : p.g_ld; d.b = q.x; d.b_ld = x_ld; d.m = vs; d.n = channels; d.k = rows;
-        d.splits = product_splits(vs, channels, rows, dtype, p.fused); d.slab = (float*)(ws + p.slab_w); d.scale = scale;
+        d.splits = product_splits(vs, channels, rows, dtype, p.fused, dbias); d.slab = (float*)(ws + p.slab_w); d.scale = scale;
         d.slab_ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
         rc = dtype == WCN_F32 ? fp32_product(d, true, st) : wcn_ce_product_run(d, true, p.fused, dtype, dev_status, st);
         if (rc != WCN_OK) return rc;

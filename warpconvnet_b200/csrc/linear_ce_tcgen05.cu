@@ -1198,13 +1198,16 @@ template <bool GRAD, bool BF16> int by_resident(LogitParams& p, cudaStream_t st)
   return launch_logits<NOTHING, GRAD, BF16>(p, fixed, st);
 }
 
+// Columns of a tile: with the sums of A's rows beside them.
+int most_columns(bool ones) { return ones ? 240 : 256; }
+
 template <bool TRANS, bool BLOCKED, bool BF16>
 int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st) {
   constexpr int MB = BLOCKED ? 2 : 1;
   ProductParams p = {};
   p.q = q;
   p.dev_status = dev_status;
-  const int most = q.slab_ones ? 240 : 256;
+  const int most = most_columns(q.slab_ones);
   p.n_tiles = (q.n + most - 1) / most;
   p.NT = wcn_ce_round((q.n + p.n_tiles - 1) / p.n_tiles, 16);
   p.NB = (p.NT + 63) / 64;
@@ -1345,8 +1348,8 @@ int wcn_ce_logits(const wcn_ce_piece& q, const wcn_ce_result* out, int dtype, bo
 }
 
 // Splits of k with which the product's tiles keep every multiprocessor busy.
-int wcn_ce_product_splits(int m, int n, int k, bool blocked) {
-  const int tile = blocked ? 2 * TILE_M : TILE_M, tiles = ((m + tile - 1) / tile) * ((n + 239) / 240), ksteps = (k + SLICE - 1) / SLICE, sms = wcn_num_sms();
+int wcn_ce_product_splits(int m, int n, int k, bool blocked, bool ones) {
+  const int tile = blocked ? 2 * TILE_M : TILE_M, most = most_columns(ones), tiles = ((m + tile - 1) / tile) * ((n + most - 1) / most), ksteps = (k + SLICE - 1) / SLICE, sms = wcn_num_sms();
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= sms && s <= ksteps; ++s) {
