@@ -4,6 +4,8 @@
 // in fp32 whatever the parameters' and gradients' type; a parameter in 16 bits is rounded to nearest once, as it is stored.
 //
 // Bound by HBM: p, g, m and v are read and p, m, v written once, 28 bytes a parameter in fp32.  With moments in 8 bits it is 16.
+// Measured for 38 M parameters in 188 tensors, fp32: 170 us, 6.2 TB/s, with moments in 32 bits; 165 us with 8 bits, where the
+// integer pipe is 64 % busy with hashes and codes and 550 MB of HBM traffic are not the limit (decoding both moments: 57 us).
 //
 // 8-bit moments are codes of a logarithmic scale: the code k > 0 of a block of 256 elements stands for the fp32 number with the
 // bits (k + base) << 20, i.e. 8 values to an octave, the code 0 for zero.  The block's base puts its largest magnitude at the

@@ -12,7 +12,9 @@
 // of 2^-28 is still a normal number.)
 //
 // 16-bit types run on the tensor cores (linear_ce_tcgen05.cu); fp32 on the FMA pipes here, in tiles of 64 x 64, sums of 128
-// products at a time.
+// products at a time.  20 000 rows x 64 channels x 40 classes fp32, forward and backward: 79 us on the device in eight launches of
+// 2 to 20 us (the host's part makes that 150; 40 of a tile's 64 classes are used).  30 000 x 256 x 32 768 classes bf16 forward and
+// backward: 1.95 to 2.25 ms as the power cap sets the clock, 0.9 to 1.0 PFLOP/s of products (logits twice, dx and dw).
 #include "linear_ce.cuh"
 
 int wcn_ce_logits_parts(int rows, int classes);

@@ -11,6 +11,11 @@
 // other operand passes: a multiprocessor receives about 80 bytes a clock, and a tile whose operands both arrived anew would
 // wait for them (192 KB against 2 048 clocks of matrix instructions at 256 channels).
 //
+// Measured: logits and sums of 30 000 rows x 256 channels x 32 768 classes bf16 in 388 to 436 us, 1.2 to 1.3 PFLOP/s, where matrix
+// instructions and the power cap bound them; of 60 000 x 128 x 4 096 fp16 in 94 us, 0.67 PFLOP/s, where the exponentials do (the
+// special-function pipe is 73 % busy, the tensor pipe 35 %).  dw of 15 000 x 256 x 16 384 in 105 to 113 us, 1.1 to 1.2 PFLOP/s; with half as
+// many splits, from an estimate by narrower tiles than it had, it took 178.
+//
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix
 // instructions and frees its tensor memory; what was to come of it is then filled with NaN (linear_ce.cu).
 #include "linear_ce.cuh"
@@ -665,7 +670,9 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
 // tile; dx = g w and dw += g^T x, the latter in accumulators that stay in tensor memory until the block's last tile.  The same
 // images in shared memory serve every product: a tile of rows whose channels (classes) run along 128-byte lines is a K-major
 // operand with its rows on the M / N side, or an MN-major one with its rows on the K side.
-// 240 000 x 96 x 200 classes bf16: pieces of g through global memory took 64 (g) + 39 (dx) + 33 us (dw).
+// 240 000 x 96 x 200 classes bf16: 70 us, after 41 for the forward pass (reading and writing 92 MB would take 14); pieces of g
+// through global memory took 64 (g) + 39 (dx) + 33 us (dw).  What bounds it is the chain of a tile, z -> g -> both products, of
+// which tensor memory holds one set: 23 % of the tensor pipe and 59 MB of HBM traffic are used in that time.
 struct HeadParams {
   wcn_ce_piece q;
   wcn_ce_scale scale;
@@ -923,7 +930,9 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 // bulk copy leaves in global memory for dw, as it is: [128 rows][64 classes] images.  The (row tile, class tile) pairs are one
 // sequence that is divided evenly among the blocks; where a row tile's classes are several blocks', each leaves its dx apart.
 // As two kernels, the second of which read g again in rows of 128 bytes, 15 000 rows x 6 656 classes x 256 channels bf16 took
-// 85 (g) + 62 us (dx).
+// 85 (g) + 62 us (dx); 15 000 x 16 384 x 256 takes 248 to 283, 0.9 to 1.0 PFLOP/s, with the tensor pipe 46 % busy: a tile's g has one
+// place in shared memory, where the products of one tile and the exponentials of the next meet.  (g handed over in halves of 64
+// classes, for more of the two at a time, made the whole call 2 % longer.)
 struct RowsParams {
   wcn_ce_piece q;         // g: images, or null (no dw)
   float* slab;            // [slots][rows][channels rounded up to 16], or null (no dx)
