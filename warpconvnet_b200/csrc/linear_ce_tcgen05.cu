@@ -13,7 +13,7 @@
 //
 // Measured: logits and sums of 30 000 rows x 256 channels x 32 768 classes bf16 in 388 to 436 us, 1.2 to 1.3 PFLOP/s, where matrix
 // instructions and the power cap bound them; of 60 000 x 128 x 4 096 fp16 in 94 us, 0.67 PFLOP/s, where the exponentials do (the
-// special-function pipe is 73 % busy, the tensor pipe 35 %).  dw of 15 000 x 256 x 16 384 in 105 to 113 us, 1.1 to 1.2 PFLOP/s; with half as
+// special-function pipe is 73 % busy, the tensor pipe 35 %; a quarter of them as polynomials on the FMA pipe gained 2 %, more lost).  dw of 15 000 x 256 x 16 384 in 105 to 113 us, 1.1 to 1.2 PFLOP/s; with half as
 // many splits, from an estimate by narrower tiles than it had, it took 178.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix
