@@ -620,7 +620,7 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
  * backward: gradients of x [n, channels] and w [classes, channels] (contiguous, 16-byte aligned, of dtype) and of the bias (of
  * bias_dtype), each of which may be NULL.  grad: one number; or, with row_max (the largest magnitude of the finite ones), one a row's loss.
  * count: of a mean, else NULL.  Few launches for small problems, some for every piece of 512 MB of the logits' gradient.
- * workspace: 16-byte aligned; `what` of the query: 0 forward, else the sum of 1 (dx), 2 (dw), 4 (dbias).
+ * workspace: 16-byte aligned, that of backward 32-byte aligned; `what` of the query: 0 forward, else the sum of 1 (dx), 2 (dw), 4 (dbias).
  * Stands for a 1x1x1 convolution to classes (examples/mink_unet.py:405-413) and torch.nn.functional.cross_entropy behind it. */
 int wcn_linear_ce_workspace_bytes(int64_t n, int32_t channels, int64_t classes, int dtype, int what, int64_t* bytes);
 int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t channels, const void* w, int64_t w_ld, int64_t classes,

@@ -1,0 +1,24 @@
+"""What the C entry points of group norm, linear cross entropy and AdamW refuse on the host: nothing is launched, the addresses are
+made up."""
+from array import array
+
+import pytest
+
+from warpconvnet_b200 import _native
+
+BASE = 1 << 20   # stands for aligned device memory
+INVALID, BOUNDS = -5, -8
+
+
+def backward(workspace, n=256, c=64, v=40, dtype=_native.WCN_BF16):
+    size = _native.query_bytes("wcn_linear_ce_workspace_bytes", n, c, v, dtype, 7)
+    return _native.lib().wcn_linear_ce_backward(BASE, c, n, c, BASE, c, v, None, BASE, -100, dtype, BASE, BASE, BASE, BASE, None, BASE, BASE, BASE, dtype,
+                                                workspace, size, BASE, None)
+
+
+@pytest.mark.parametrize("n,c,v", [(256, 64, 40), (256, 64, 1000), (256, 512, 1000)])   # a kernel for each: few classes, many, wide rows
+@pytest.mark.parametrize("dtype", [_native.WCN_F32, _native.WCN_F16, _native.WCN_BF16])
+def test_workspace_of_the_cross_entropys_gradients_starts_on_32_bytes(n, c, v, dtype):
+    """Sums go there in pieces of 32 bytes."""
+    for off in (4, 8, 16, 48):
+        assert backward(BASE + off, n, c, v, dtype) == INVALID

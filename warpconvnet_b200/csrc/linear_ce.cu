@@ -545,6 +545,7 @@ bool matrix_ok(const void* p, int64_t ld, int c, int dtype) {
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool on32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }   // (what is written in pieces of 32 bytes)
 
 }  // namespace
 
@@ -613,7 +614,7 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
                                       const float* row_max, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
                                       int64_t workspace_bytes, int32_t* dev_status, void* stream) {
   if (!sizes_ok(n, channels, classes, dtype) || !matrix_ok(x, x_ld, channels, dtype) || !matrix_ok(w, w_ld, channels, dtype) || !labels ||
-      !lse2 || !loss_rows || !grad || !workspace || !on16(workspace) || !on16(dx) || !on16(dw) || !dev_status || bias_dtype < WCN_F32 ||
+      !lse2 || !loss_rows || !grad || !workspace || !on32(workspace) || !on16(dx) || !on16(dw) || !dev_status || bias_dtype < WCN_F32 ||
       bias_dtype > WCN_BF16)
     return WCN_ERR_INVALID_PARAMETERS;
   if (!dx && !dw && !dbias) return WCN_OK;
