@@ -22,3 +22,19 @@ def test_workspace_of_the_cross_entropys_gradients_starts_on_32_bytes(n, c, v, d
     """Sums go there in pieces of 32 bytes."""
     for off in (4, 8, 16, 48):
         assert backward(BASE + off, n, c, v, dtype) == INVALID
+
+
+def step(sizes, slots, length):
+    count = len(sizes)
+    at, sizes, slots = array("q", [BASE] * count), array("q", sizes), array("q", slots)
+    address = lambda a: a.buffer_info()[0]   # noqa: E731
+    return _native.lib().wcn_adamw_step(address(at), address(at), address(sizes), address(slots), None, count, 0, 0, BASE, None, BASE, None, length, BASE, count,
+                                        0, 0, 0, 0, 0, None, None, None, BASE, None)
+
+
+@pytest.mark.parametrize("slot", [512, 1 << 40, (1 << 63) - 512, (1 << 63) - 256])
+def test_moments_beyond_their_end_are_refused(slot):
+    """Also where a slot and a size come to more than 2^63."""
+    assert step([300], [slot], 512) == BOUNDS
+    assert step([5, 300], [0, slot], 512) == BOUNDS
+    assert step([(1 << 63) - 1], [0], 512) == BOUNDS

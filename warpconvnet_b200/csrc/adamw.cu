@@ -336,8 +336,10 @@ extern "C" int wcn_adamw_step(const int64_t* params, const int64_t* grads, const
     if (n < 0 || (n && (!params[i] || !grads[i])) || params[i] % wcn_dtype_size(dtype) || grads[i] % wcn_dtype_size(grad_dtype) || slot < 0 ||
         slot % CODES || at < 0 || at > 0x7FFFFFFF)
       return WCN_ERR_INVALID_PARAMETERS;
-    slot += (n + CODES - 1) / CODES * CODES;
-    if (slot > length || at >= num_steps) return WCN_ERR_BOUNDS;
+    // (in blocks: the sum of a slot and a size may be beyond 63 bits)
+    const int64_t end = slot / CODES + n / CODES + (n % CODES != 0);
+    if (end > length / CODES || at >= num_steps) return WCN_ERR_BOUNDS;
+    slot = end * CODES;
   }
   const Given a = {params, grads, sizes, slots, step_at, count};
   Hyper h = {};
