@@ -19,7 +19,9 @@
 // What an item waits for has been claimed before it, by blocks that are running: there is always one that can go on.  Waits are
 // bounded all the same; one that runs out sets the status word, and what could not be computed is filled with NaN.
 // Variances are never differences of large numbers: a thread's few rows of a tile have a mean of their own, about the first of
-// them, and means are put together by their differences.  A row far from all others or a mean that is large against the spread costs no precision.
+// them, and means are put together by their differences: neither a row far from all others nor a mean that is large against the
+// spread costs them precision.  Of a large mean its own rounding to fp32 is left in x - mean: up to 2^-24 |mean| / std in a
+// result before gamma (nothing where the mean is a number of fp32, as in a constant group).
 #include <string.h>
 
 #include <type_traits>
@@ -406,11 +408,10 @@ __device__ __forceinline__ void join_grad_sums(const Params& p, const Tile& t, i
   });
 }
 
+// x - mean, before anything is scaled: x / std - mean / std would be a difference of numbers that are rounded at the size of
+// mean / std (of a constant group of 1000 with eps 1e-5: 3e5, and results off by 0.016 where they are beta).
+__device__ __forceinline__ float2 less(float2 x, float2 mean) { return __fadd2_rn(x, make_float2(-mean.x, -mean.y)); }
 // A piece has SUB groups side by side (V / SUB channels of one group each; V: any).
-// (x - mean) * scale: of 16-bit numbers as one multiplication and addition, whose rounding is far below theirs.
-template <typename T> __device__ __forceinline__ float2 centred(float2 x, float2 mean, float2 scale, float2 minus) {
-  return sizeof(T) == 2 ? __ffma2_rn(x, scale, minus) : __fmul2_rn(__fadd2_rn(x, make_float2(-mean.x, -mean.y)), scale);
-}
 // The values of a pair of channels, which may be of two of a piece's SUB groups.
 template <int V, int SUB> __device__ __forceinline__ float2 of_pair(const float (&v)[SUB], int i) {
   return make_float2(v[2 * i * SUB / V], v[V == 1 ? 0 : (2 * i + 1) * SUB / V]);
@@ -445,20 +446,11 @@ __device__ __forceinline__ void tile_apply(const Params& p, const Place& at, con
       rstd[k] = v.y;
     }
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), scale[i]);
-      const float2 m = of_pair<V, SUB>(mean, i);
-      if (sizeof(T) == 2) beta[i] = __ffma2_rn(make_float2(-m.x, -m.y), scale[i], beta[i]);
-    }
+    for (int i = 0; i < P; ++i) scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), scale[i]);
     walk<4>(rows, [&](int j) { return load_last<T, V>(from + j * step); }, [&](int j, const Piece<T, V>& q) {
       float2 o[P];
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        float2 x = pair_of<T, V>(q, i);
-        const float2 m = of_pair<V, SUB>(mean, i);
-        if (sizeof(T) == 4) x = __fadd2_rn(x, make_float2(-m.x, -m.y));
-        o[i] = activate<ACT>(__ffma2_rn(x, scale[i], beta[i]));
-      }
+      for (int i = 0; i < P; ++i) o[i] = activate<ACT>(__ffma2_rn(less(pair_of<T, V>(q, i), of_pair<V, SUB>(mean, i)), scale[i], beta[i]));
       store_piece<T, V>(to + j * out_step, rounded<T, V>(o));
     });
   }
@@ -479,34 +471,34 @@ __device__ __forceinline__ void tile_grad_sums(const Params& p, const Place& at,
       const T* const dy = reinterpret_cast<const T*>(p.dy) + (int64_t)(t.lo + at.ty) * p.dy_ld + pc * V;
       const int64_t step = (int64_t)at.tys * p.x_ld, dy_step = (int64_t)at.tys * p.dy_ld;
       constexpr int P = (V + 1) / 2;
-      float2 a[P], b[P], gamma[P], beta[P];
-      float mean[SUB], rstd[SUB], minus[SUB];
+      float2 a[P], b[P], scale[P], beta[P];   // (b: of x - mean, multiplied by 1 / std at the end)
+      float mean[SUB], rstd[SUB];
 #pragma unroll
       for (int k = 0; k < SUB; ++k) {
         const int64_t g = (int64_t)t.place * p.G + (pc * V + k * (V / SUB)) / p.per;
         mean[k] = __ldg(&p.mean[g]);
         rstd[k] = __ldg(&p.rstd[g]);
-        minus[k] = -mean[k] * rstd[k];
       }
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         a[i] = b[i] = both(0.f);
-        gamma[i] = pair_at<V>(p.gamma, pc * V + 2 * i, 1.f);
+        scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), pair_at<V>(p.gamma, pc * V + 2 * i, 1.f));
         beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
       }
       walk<2>(rows_of(p, at, t.hi - t.lo), [&](int j) { return Pair<T, V>{load_piece<T, V>(x + j * step), load_piece<T, V>(dy + j * dy_step)}; },
               [&](int, const Pair<T, V>& q) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float2 xhat = centred<T>(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i), of_pair<V, SUB>(rstd, i), of_pair<V, SUB>(minus, i));
-          const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(xhat, gamma[i], beta[i]));
+          const float2 d = less(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i));
+          const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(d, scale[i], beta[i]));
           a[i] = __fadd2_rn(a[i], dz);
-          b[i] = __ffma2_rn(dz, xhat, b[i]);
+          b[i] = __ffma2_rn(dz, d, b[i]);
         }
       });
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const int c = at.ty * W + at.tx * V + 2 * i;
+        b[i] = __fmul2_rn(b[i], of_pair<V, SUB>(rstd, i));
         s_a[c] = a[i].x;
         s_b[c] = b[i].x;
         if (V > 1) {
@@ -561,32 +553,30 @@ __device__ __forceinline__ void tile_grad_apply(const Params& p, const Place& at
     const T* const dy = reinterpret_cast<const T*>(p.dy) + (int64_t)(t.lo + at.ty) * p.dy_ld + pc * V;
     T* const dx = reinterpret_cast<T*>(p.out) + (int64_t)(t.lo + at.ty) * p.C + pc * V;
     constexpr int P = (V + 1) / 2;
-    float mean[SUB], rstd[SUB], minus[SUB], a[SUB], b[SUB];   // (the sums' negatives)
-    float2 gamma[P], beta[P];
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      gamma[i] = pair_at<V>(p.gamma, pc * V + 2 * i, 1.f);
-      beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
-    }
+    float mean[SUB], rstd[SUB], a[SUB], b[SUB];   // (the sums' negatives over std, over its square)
+    float2 scale[P], beta[P];
 #pragma unroll
     for (int k = 0; k < SUB; ++k) {
       const int g = (pc * V + k * (V / SUB)) / p.per;
       mean[k] = __ldg(&p.mean[(int64_t)t.place * p.G + g]);
       rstd[k] = __ldg(&p.rstd[(int64_t)t.place * p.G + g]);
-      minus[k] = -mean[k] * rstd[k];
       const float2 v = ok ? __ldcg(&p.whole[(int64_t)t.scene * p.G + g]) : make_float2(__int_as_float(0x7FC00000), 0.f);
-      a[k] = -v.x;
-      b[k] = -v.y;
+      a[k] = -rstd[k] * v.x;
+      b[k] = -rstd[k] * (rstd[k] * v.y);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      scale[i] = __fmul2_rn(of_pair<V, SUB>(rstd, i), pair_at<V>(p.gamma, pc * V + 2 * i, 1.f));
+      beta[i] = pair_at<V>(p.beta, pc * V + 2 * i, 0.f);
     }
     walk<2>(rows_of(p, at, t.hi - t.lo), [&](int j) { return Pair<T, V>{load_last<T, V>(x + j * step), load_last<T, V>(dy + j * dy_step)}; },
             [&](int j, const Pair<T, V>& q) {
       float2 o[P];
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const float2 r = of_pair<V, SUB>(rstd, i);
-        const float2 xhat = centred<T>(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i), r, of_pair<V, SUB>(minus, i));
-        const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(xhat, gamma[i], beta[i]));
-        o[i] = __fmul2_rn(r, __ffma2_rn(xhat, of_pair<V, SUB>(b, i), __ffma2_rn(gamma[i], dz, of_pair<V, SUB>(a, i))));
+        const float2 d = less(pair_of<T, V>(q.x, i), of_pair<V, SUB>(mean, i));
+        const float2 dz = through<ACT>(pair_of<T, V>(q.dy, i), __ffma2_rn(d, scale[i], beta[i]));
+        o[i] = __ffma2_rn(d, of_pair<V, SUB>(b, i), __ffma2_rn(scale[i], dz, of_pair<V, SUB>(a, i)));
       }
       store_piece<T, V>(dx + j * out_step, rounded<T, V>(o));
     });
