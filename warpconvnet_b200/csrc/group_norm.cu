@@ -17,7 +17,8 @@
 // distances from it per group (backward: two sums, and two per channel); the block that leaves a scene's last tile puts the
 // tiles together, in their order and in double, and raises the scene's flag: the same bits on every run.
 // What an item waits for has been claimed before it, by blocks that are running: there is always one that can go on.  Waits are
-// bounded all the same; one that runs out sets the status word, and what could not be computed is filled with NaN.
+// bounded all the same; one that runs out sets the status word, and what could not be computed is filled with NaN: all of the
+// results of a launch that finds the word set by an earlier one.
 // Variances are never differences of large numbers: a thread's few rows of a tile have a mean of their own, about the first of
 // them, and means are put together by their differences: neither a row far from all others nor a mean that is large against the
 // spread costs them precision.  Of a large mean its own rounding to fp32 is left in x - mean: up to 2^-24 |mean| / std in a
@@ -615,10 +616,13 @@ __device__ __forceinline__ Item item_of(const Params& p, int k, bool apply) {
 template <typename T, int V, int ACT, int SUB, bool BACK>
 __global__ void __launch_bounds__(THREADS, BACK ? BLOCKS_BACKWARD : BLOCKS_FORWARD) group_norm_kernel(const __grid_constant__ Scenes scenes, const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ int s_item, s_last, s_ok;
+  __shared__ int s_item, s_last, s_ok, s_failed;
   const bool apply = p.out != nullptr;
   const Place at(p.C, V);
-  if (threadIdx.x == 0) s_item = atomicAdd(&p.sync->ticket, 1);
+  if (threadIdx.x == 0) {
+    s_item = atomicAdd(&p.sync->ticket, 1);
+    s_failed = *(volatile int32_t*)p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;   // (an earlier launch gave up: no results)
+  }
   __syncthreads();
   for (;;) {
     const int k = s_item;
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, BACK ? BLOCKS_BACKWARD : BLOCKS_FORWA
     if (threadIdx.x == 0) next = atomicAdd(&p.sync->ticket, 1);   // (arrives while this item is worked on)
     const Item it = item_of(p, k, apply);
     if (it.kind == 2) {
-      if (threadIdx.x == 0) s_ok = wait_for(&p.sync->scenes, scenes.count, p.dev_status);
+      if (threadIdx.x == 0) s_ok = !s_failed && wait_for(&p.sync->scenes, scenes.count, p.dev_status);
       __syncthreads();
       join_channels(p, it.at * JOINED, s_ok, smem);
     } else {
@@ -655,7 +659,7 @@ __global__ void __launch_bounds__(THREADS, BACK ? BLOCKS_BACKWARD : BLOCKS_FORWA
         }
       } else {
         auto ready = [&]() -> bool {
-          if (threadIdx.x == 0) s_ok = wait_for(&p.sync->flag[t.scene], 1, p.dev_status);
+          if (threadIdx.x == 0) s_ok = !s_failed && wait_for(&p.sync->flag[t.scene], 1, p.dev_status);
           __syncthreads();
           return s_ok;
         };
