@@ -7,9 +7,9 @@
 // comparison each).  Backward: z again, piece by piece of rows x classes; a piece's g goes to the workspace in x's type and is
 // multiplied by w and by x from there.  Products whose sums over k are divided, or that several pieces add to, are put together
 // in fp32 in a fixed order: the same bits on every run.
-// g is rounded to 16 bits as softmax - onehot, without the rows' factor, which the results are multiplied by in fp32: labels'
+// g is rounded to 16 bits as softmax - onehot, without the factor of a mean, which the results are multiplied by in fp32: labels'
 // entries are the largest ones and keep 8 (11) bits whatever the number of rows.  (In fp16 it is raised by 2^14: a probability
-// of 2^-28 is still a normal number.)
+// of 2^-28 is still a normal number.)  Weights of single rows, over the largest of them, are in g; not in that of dx in fp16.
 //
 // 16-bit types run on the tensor cores (linear_ce_tcgen05.cu); fp32 on the FMA pipes here, in tiles of 64 x 64, sums of 128
 // products at a time.  20 000 rows x 64 channels x 40 classes fp32, forward and backward: 79 us on the device in eight launches of
@@ -233,8 +233,7 @@ template <typename TO, int SIDE> __device__ __forceinline__ void join_quads(cons
     reinterpret_cast<float4*>(p.acc)[q] = make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
     return;
   }
-  const int count = p.scale.count ? *p.scale.count : 1;
-  float scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
+  float scale = p.scale.rows ? wcn_ce_row_factor(p.scale, row) : wcn_ce_factor(p.scale);
   if (*p.dev_status == (int)WCN_ERR_WAIT_EXPIRED) scale = __int_as_float(0x7FC00000);
   TO* const out = reinterpret_cast<TO*>(p.out) + row * p.n + col;
   __align__(16) TO r[4];
@@ -274,8 +273,7 @@ __device__ __forceinline__ void join_sums(const JoinParams& p, int block) {
     p.acc[i] = (float)v;
     return;
   }
-  const int count = p.scale.count ? *p.scale.count : 1;
-  float scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
+  float scale = wcn_ce_factor(p.scale);
   if (*p.dev_status == (int)WCN_ERR_WAIT_EXPIRED) scale = __int_as_float(0x7FC00000);
   reinterpret_cast<TO*>(p.out)[i] = wcn_from_float<TO>((float)v * scale);
 }
@@ -618,18 +616,27 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
       bias_dtype > WCN_BF16)
     return WCN_ERR_INVALID_PARAMETERS;
   if (!dx && !dw && !dbias) return WCN_OK;
+  // Rows of their own weight in fp16: g of a row times its weight over the largest one would be subnormal where that is below 2^-28.
+  // dx takes the weights in fp32 at its end, from a g without them; dw and dbias, which add rows up, from a g with them.
+  const bool late = row_max && dtype == WCN_F16 && dx;
+  if (late && (dw || dbias)) {
+    const int rc = wcn_linear_ce_backward(x, x_ld, n, channels, w, w_ld, classes, bias2, labels, ignore, dtype, lse2, loss_rows, count, grad, row_max, nullptr,
+                                          dw, dbias, bias_dtype, workspace, workspace_bytes, dev_status, stream);
+    if (rc != WCN_OK) return rc;
+    dw = dbias = nullptr;
+  }
   const Pieces p = cut(n, channels, classes, dtype, dx, dw, dbias);
   if (p.bytes > workspace_bytes) return WCN_ERR_SCRATCH_TOO_SMALL;
   cudaStream_t st = wcn_stream(stream);
   char* const ws = (char*)workspace;
   const int e = wcn_dtype_size(dtype);
   const float lift = lift_of(dtype);
-  const wcn_ce_scale scale = {row_max ? row_max : grad, count, dtype == WCN_F16 ? 1.f / 16384.f : 1.f};
+  wcn_ce_scale scale = {row_max ? row_max : grad, count, dtype == WCN_F16 ? 1.f / 16384.f : 1.f, late ? grad : nullptr, labels, ignore, classes};
   if (p.head) {
     wcn_ce_piece q = {};
     q.x = x; q.w = w; q.x_ld = x_ld; q.w_ld = w_ld; q.rows = (int)n; q.classes = (int)classes; q.channels = channels; q.bias2 = bias2;
     q.lse2 = lse2; q.loss = loss_rows; q.labels = labels; q.ignore = ignore; q.all_classes = classes;
-    q.row_scale = row_max ? grad : nullptr; q.row_max = row_max;
+    q.row_scale = row_max && !late ? grad : nullptr; q.row_max = row_max;
     float *const slab = dw || dbias ? (float*)(ws + p.slab_w) : nullptr, *const ones = dbias ? (float*)(ws + p.slab_b) : nullptr;
     int rc = wcn_ce_head(q, scale, dx, slab, ones, dtype, lift, dev_status, st);
     const JoinParams for_w = {slab, nullptr, false, dw, classes, channels, p.ld, p.head, scale, dev_status}, for_b = {ones, nullptr, false, dbias, classes, 1, 1, p.head, scale, dev_status};
@@ -648,7 +655,8 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
       q.x = (const char*)x + r0 * x_ld * e; q.w = (const char*)w + v0 * w_ld * e; q.x_ld = x_ld; q.w_ld = w_ld;
       q.rows = rows; q.classes = vs; q.channels = channels; q.bias2 = bias2 ? bias2 + v0 : nullptr;
       q.lse2 = lse2 + r0; q.loss = loss_rows + r0; q.labels = labels + r0; q.ignore = ignore; q.first_class = v0; q.all_classes = classes;
-      q.row_scale = row_max ? grad + r0 : nullptr; q.row_max = row_max;
+      q.row_scale = row_max && !late ? grad + r0 : nullptr; q.row_max = row_max;
+      if (late) { scale.rows = grad + r0; scale.labels = labels + r0; }
       q.g = ws + p.g; q.g_ld = p.g_ld;
       int rc = WCN_OK;
       if (p.fused) {

@@ -2,12 +2,27 @@
 #pragma once
 #include "wcn_common.cuh"
 
-// What a gradient is multiplied by as it is finished: *g / *count * factor (0 where no row counts).
+// What a gradient is multiplied by as it is finished: *g / *count * factor (0 where no row counts); or, with `rows`, the gradient of
+// each row's loss (0 of a row that does not count) * factor.
 struct wcn_ce_scale {
   const float* g;
   const int32_t* count;   // null: 1
   float factor;
+  const float* rows;      // null: one number for all
+  const int64_t* labels;  // (with rows)
+  int64_t ignore, classes;
 };
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float wcn_ce_factor(const wcn_ce_scale& s) {
+  const int count = s.count ? *s.count : 1;
+  return count ? *s.g / (float)count * s.factor : 0.f;
+}
+__device__ __forceinline__ float wcn_ce_row_factor(const wcn_ce_scale& s, int64_t row) {
+  const int64_t y = __ldg(&s.labels[row]);
+  return y != s.ignore && y >= 0 && y < s.classes ? __ldg(&s.rows[row]) * s.factor : 0.f;
+}
+#endif
 
 // The logits of a piece of rows x classes, as they are used: sums of exponentials (forward) or gradients (backward).
 struct wcn_ce_piece {

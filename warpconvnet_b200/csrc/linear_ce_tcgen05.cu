@@ -120,7 +120,7 @@ struct LogitParams {
   int KB;                 // slices of 64 channels
   int NT;                 // classes of a tile
   int m_tiles, n_tiles, splits, per, units, stages, tmem_cols;
-  float lift;             // exponent that gradients are raised by (fp16: see wcn_ce_lift)
+  float lift;             // exponent that gradients are raised by (fp16: 14)
   int32_t* dev_status;
 };
 
@@ -601,11 +601,7 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
     const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
     const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, last = half ? pieces : (pieces + 1) / 2;
     const int64_t slab_ld = wcn_ce_round(p.q.n, 16);
-    float scale = 0.f;
-    if (p.q.out) {
-      const int count = p.q.scale.count ? *p.q.scale.count : 1;
-      scale = count ? *p.q.scale.g / (float)count * p.q.scale.factor : 0.f;
-    }
+    float scale = p.q.out && !p.q.scale.rows ? wcn_ce_factor(p.q.scale) : 0.f;
     int ab = 0, aphase = 0;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
       if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
@@ -616,6 +612,7 @@ ce_product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_consta
       for (int j = 0; j < MB; ++j) {
         const int row = (m_of(u) * MB + j) * TILE_M + quarter * 32 + lane;
         const bool live = row < p.q.m;
+        if (p.q.out && p.q.scale.rows && live) scale = wcn_ce_row_factor(p.q.scale, row);
         const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((ab * MB + j) * p.stride);
         float* const slab = p.q.slab + ((int64_t)split * p.q.m + row) * slab_ld + n;
         uint16_t* const out = reinterpret_cast<uint16_t*>(p.q.out) + (int64_t)row * p.q.n + n;
@@ -824,11 +821,7 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const int pieces = p.NT / 16, first = pieces * part / PARTS, last = pieces * (part + 1) / PARTS;
     const int c_pieces = p.CN / 16, c_first = c_pieces * part / PARTS, c_last = c_pieces * (part + 1) / PARTS;
-    float scale = 0.f;
-    if (p.dx) {
-      const int count = p.scale.count ? *p.scale.count : 1;
-      scale = count ? *p.scale.g / (float)count * p.scale.factor : 0.f;
-    }
+    float scale = p.dx && !p.scale.rows ? wcn_ce_factor(p.scale) : 0.f;
     int i = 0;
     RowGrad next = row_grad(p.q, (int)blockIdx.x * TILE_M + in_tile, p.lift);
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
@@ -860,6 +853,7 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(&ctl->g_full));
       if (!p.dx) continue;
+      if (p.scale.rows && row < p.q.rows) scale = wcn_ce_row_factor(p.scale, row);
       if (ok) ok = mbar_wait(bar(&ctl->dx_full), i & 1, p.dev_status);
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       tc_fence_after();
