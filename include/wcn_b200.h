@@ -618,7 +618,7 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
  * Left for the backward pass: lse2 [n] (log-sum-exp in units of ln 2), loss_rows, count, and with a bias bias2
  * [classes rounded up to 256, + 256] (16-byte aligned).  counter: one zero word, zero again afterwards (one per stream).
  * backward: gradients of x [n, channels] and w [classes, channels] (contiguous, 16-byte aligned, of dtype) and of the bias (of
- * bias_dtype), each of which may be NULL.  grad: one number; or, with row_max (the largest magnitude of the finite ones), one a row's loss.
+ * bias_dtype), each of which may be NULL.  grad: one number; or, with row_max (the largest magnitude of the finite ones of rows that count), one a row's loss.
  * count: of a mean, else NULL.  Few launches for small problems, some for every piece of 512 MB of the logits' gradient.
  * workspace: 16-byte aligned, that of backward 32-byte aligned; `what` of the query: 0 forward, else the sum of 1 (dx), 2 (dw), 4 (dbias).
  * Stands for a 1x1x1 convolution to classes (examples/mink_unet.py:405-413) and torch.nn.functional.cross_entropy behind it. */

@@ -69,3 +69,18 @@ def test_weights_of_unlike_size(dtype, n, c, v):
     assert off(got[1], want[1]) <= TOL[dtype] and off(got[2], want[2]) <= TOL[dtype]
     alone = gradients(x, w, labels, b, grad, (1, 2))
     assert torch.equal(alone[0], got[1]) and torch.equal(alone[1], got[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c,v", SIZES)
+def test_weights_of_rows_that_do_not_count(dtype, n, c, v):
+    """Whatever they are, also far above the others."""
+    x, w, labels, b = problem(n, c, v, dtype, seed=2)
+    labels[5], labels[60] = -100, -100
+    grad = torch.randn(n, generator=torch.Generator().manual_seed(3))
+    clean = gradients(x, w, labels, b, grad)
+    want = exact(x, w, labels, b, grad)
+    grad[5], grad[60] = 2.0 ** 60, -1e30
+    got = gradients(x, w, labels, b, grad)
+    assert all(off(p, q) <= TOL[dtype] for p, q in zip(got, want))
+    assert all(torch.equal(p, q) for p, q in zip(got, clean))

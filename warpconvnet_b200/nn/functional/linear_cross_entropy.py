@@ -101,8 +101,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         grad = grad.float().contiguous()
         at_count, at_bias, _ = _kept(n, v, bias is not None)
         base = kept.data_ptr()
-        # (numbers beside which the others keep their precision: what is no number stays with its row)
-        row_max = torch.where(torch.isfinite(grad), grad.abs(), 0.0).amax() if ctx.reduction == "none" else None
+        # (numbers beside which the others keep their precision: what is no number stays with its row, as does a row that does not count)
+        row_max = torch.where(torch.isfinite(grad) & (labels != ctx.ignore_index), grad.abs(), 0.0).amax() if ctx.reduction == "none" else None
         x, x_ld = _matrix(x if x_rows is None else x_rows, c)
         weight, w_ld = _matrix(weight if w_rows is None else w_rows, c)
         ws = _workspace(n, c, v, code, need_x + 2 * need_w + 4 * need_b, dev)
