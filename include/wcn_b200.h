@@ -615,7 +615,7 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
  * w_ld elements apart; in 16 bits: 16-byte aligned, the distances multiples of 8), bias [classes] of bias_dtype or NULL, one
  * int64 label a row; z is not kept.  A row whose label is `ignore` has the loss 0; so has one whose label names no class, for
  * which WCN_ERR_BOUNDS is stored.  reduction: 0 none, 1 mean over the *count rows that count, 2 sum (*loss).
- * Left for the backward pass: lse2 [n] (log-sum-exp in units of ln 2), loss_rows, count, and with a bias bias2
+ * Left for the backward pass: lse2 [n] (log-sum-exp, in 16 bits in units of ln 2), loss_rows, count, and with a bias bias2
  * [classes rounded up to 256, + 256] (16-byte aligned).  counter: one zero word, zero again afterwards (one per stream).
  * backward: gradients of x [n, channels] and w [classes, channels] (contiguous, 16-byte aligned, of dtype) and of the bias (of
  * bias_dtype), each of which may be NULL.  grad: one number; or, with row_max (the largest magnitude of the finite ones of rows that count), one a row's loss.

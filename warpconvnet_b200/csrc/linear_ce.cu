@@ -2,9 +2,9 @@
 //     loss_i = log sum_j exp(z_ij) - z_iy                       over rows whose label is not `ignore`: mean, sum, or each
 //     g = s_i (softmax(z_i) - onehot(y_i))      dx = g w      dw = g^T x      db = sums of g's columns
 //
-// Forward: one pass over tiles of z, of which each row keeps a running (largest, sum of exponentials); then a warp a row puts
-// the pieces of its classes together and takes z_iy from a product of its own, in fp32 (the label's logit would cost the tiles a
-// comparison each).  Backward: z again, piece by piece of rows x classes; a piece's g goes to the workspace in x's type and is
+// Forward: one pass over tiles of z, of which each row keeps a running (largest, sum of exponentials); then eight lanes a row put
+// the pieces of its classes together and take z_iy from a product of their own (in 16 bits, where the label's logit would cost the
+// tiles a comparison each; fp32 tiles leave it: another order of its sum would be an error of the small losses).  Backward: z again, piece by piece of rows x classes; a piece's g goes to the workspace in x's type and is
 // multiplied by w and by x from there.  Products whose sums over k are divided, or that several pieces add to, are put together
 // in fp32 in a fixed order: the same bits on every run.
 // g is rounded to 16 bits as softmax - onehot, without the factor of a mean, which the results are multiplied by in fp32: labels'
@@ -42,9 +42,9 @@ inline float lift_of(int dtype) { return dtype == WCN_F16 ? 14.f : 0.f; }
 // ------------------------------------------------------------------ around the products
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) ce_bias_kernel(const T* bias, int64_t v, int64_t padded, float* bias2) {
+__global__ void __launch_bounds__(THREADS) ce_bias_kernel(const T* bias, int64_t v, int64_t padded, float unit, float* bias2) {
   for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < padded; i += (int64_t)gridDim.x * THREADS)
-    bias2[i] = i < v ? wcn_to_float<T>(bias[i]) * LOG2E : -INFINITY;
+    bias2[i] = i < v ? wcn_to_float<T>(bias[i]) * unit : -INFINITY;
 }
 
 struct LossParams {
@@ -57,7 +57,7 @@ struct LossParams {
   int64_t ignore;
   const float2* part;      // [parts][n]
   float* lse2;
-  float* loss_rows;
+  float* loss_rows;        // (fp32: before that, the labels' logits)
   float* loss;
   int32_t* count;
   double* block_sums;      // [blocks]
@@ -66,21 +66,16 @@ struct LossParams {
   int32_t* dev_status;
 };
 
-// The product of a row and its label's weights: eight lanes share it in pieces of 16 bytes (VEC: rows start on such boundaries).
-template <typename T, bool VEC> __device__ __forceinline__ float share_of_dot(const T* x, const T* w, int c, int lane) {
+// The product of a row and its label's weights: eight lanes share it in pieces of 16 bytes.
+template <typename T> __device__ __forceinline__ float share_of_dot(const T* x, const T* w, int c, int lane) {
   constexpr int N = 16 / (int)sizeof(T);
   float dot = 0.f;
   int i = lane * N;
 #pragma unroll 4
   for (; i + N <= c; i += 8 * N) {
     __align__(16) T a[N], b[N];
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(x + i));
-      *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(w + i));
-    } else {
-#pragma unroll
-      for (int k = 0; k < N; ++k) { a[k] = x[i + k]; b[k] = w[i + k]; }
-    }
+    *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(x + i));
+    *reinterpret_cast<uint4*>(b) = __ldg(reinterpret_cast<const uint4*>(w + i));
 #pragma unroll
     for (int k = 0; k < N; ++k) dot = fmaf(wcn_to_float<T>(a[k]), wcn_to_float<T>(b[k]), dot);
   }
@@ -88,8 +83,13 @@ template <typename T, bool VEC> __device__ __forceinline__ float share_of_dot(co
   return dot;
 }
 
+// Exponential and logarithm of logits as they are kept: of rows in 16 bits in units of ln 2, where an exponential is one
+// instruction; of fp32 rows as they are, since each rounding of a logit in other units would be one of |z| 2^-24 of its probability.
+template <typename T> __device__ __forceinline__ float exp_of(float z) { return sizeof(T) == 4 ? expf(z) : exp2f(z); }
+template <typename T> __device__ __forceinline__ float log_of(float s) { return sizeof(T) == 4 ? logf(s) : log2f(s); }
+
 // Eight lanes a row: its loss from the sums of its classes' pieces and its label's logit.
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant__ LossParams p) {
   __shared__ double s_sum[THREADS / 32];
   __shared__ int s_count[THREADS / 32];
@@ -106,14 +106,16 @@ __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant_
     const int64_t ahead = r + step < p.n ? __ldg(&p.labels[r + step]) : p.ignore;
     const bool live = r < p.n, counts = live && y != p.ignore && y >= 0 && y < p.v;
     bad |= live && y != p.ignore && !counts;
-    float dot = counts ? share_of_dot<T, VEC>(reinterpret_cast<const T*>(p.x) + r * p.x_ld, reinterpret_cast<const T*>(p.w) + y * p.w_ld, p.c, l) : 0.f;
+    float dot = 0.f;   // (fp32: the label's logit, of one lane)
+    if constexpr (sizeof(T) == 4) dot = counts && l == 0 ? p.loss_rows[r] : 0.f;
+    else if (counts) dot = share_of_dot<T>(reinterpret_cast<const T*>(p.x) + r * p.x_ld, reinterpret_cast<const T*>(p.w) + y * p.w_ld, p.c, l);
     float top = -INFINITY, sum = 0.f;
     if (live)
 #pragma unroll 4
       for (int i = l; i < p.parts; i += 8) {
         const float2 q = __ldg(&p.part[(int64_t)i * p.n + r]);
         const float now = fmaxf(top, q.x), by = now == -INFINITY ? 0.f : now;
-        sum = sum * exp2f(top - by) + q.y * exp2f(q.x - by);
+        sum = sum * exp_of<T>(top - by) + q.y * exp_of<T>(q.x - by);
         top = now;
       }
 #pragma unroll
@@ -121,14 +123,18 @@ __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant_
       dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
       const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
       const float now = fmaxf(top, t), by = now == -INFINITY ? 0.f : now;
-      sum = sum * exp2f(top - by) + s * exp2f(t - by);
+      sum = sum * exp_of<T>(top - by) + s * exp_of<T>(t - by);
       top = now;
     }
-    const float lse2 = top + log2f(sum);
+    const float more = log_of<T>(sum), lse2 = top + more;
     float loss = 0.f;
     if (counts) {
-      const float z = p.bias2 ? fmaf(dot, LOG2E, __ldg(&p.bias2[y])) : dot * LOG2E;
-      loss = (lse2 - z) * (float)LN2;
+      if constexpr (sizeof(T) == 4) {
+        loss = (top - dot) + more;
+      } else {
+        const float z = p.bias2 ? fmaf(dot, LOG2E, __ldg(&p.bias2[y])) : dot * LOG2E;
+        loss = (lse2 - z) * (float)LN2;
+      }
       if (loss < 0.f) loss = 0.f;                       // (roundings of a probability of one)
     }
     if (failed) loss = __int_as_float(0x7FC00000);
@@ -383,21 +389,27 @@ __global__ void __launch_bounds__(THREADS) ce_logits_fp32_kernel(const __grid_co
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int col = n0 + tx * 4 + j;
-      z[i][j] = col >= q.classes ? -INFINITY : q.bias2 ? fmaf(z[i][j], LOG2E, __ldg(&q.bias2[col])) : z[i][j] * LOG2E;
+      z[i][j] = col >= q.classes ? -INFINITY : q.bias2 ? z[i][j] + __ldg(&q.bias2[col]) : z[i][j];
     }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = m0 + ty * 4 + i;
     if (!GRAD) {
+      if (row < q.rows) {
+        const int64_t in = __ldg(&q.labels[row]) - (n0 + tx * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (in == j && n0 + tx * 4 + j < q.classes) q.label_logits[row] = z[i][j];
+      }
       float top = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3])), by = top == -INFINITY ? 0.f : top, sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += exp2f(z[i][j] - by);
+      for (int j = 0; j < 4; ++j) sum += expf(z[i][j] - by);
 #pragma unroll
       for (int o = 8; o; o >>= 1) {   // the 16 threads of a row
         const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         const float now = fmaxf(top, t);
         by = now == -INFINITY ? 0.f : now;
-        sum = sum * exp2f(top - by) + s * exp2f(t - by);
+        sum = sum * expf(top - by) + s * expf(t - by);
         top = now;
       }
       if (tx == 0 && row < q.rows) q.part[(int64_t)blockIdx.y * q.rows + row] = make_float2(top, sum);
@@ -409,13 +421,13 @@ __global__ void __launch_bounds__(THREADS) ce_logits_fp32_kernel(const __grid_co
         const float most = __ldg(q.row_max);
         scale = __ldg(&q.row_scale[row]) / (most > 0.f ? most : 1.f);
       }
-      const float lse2 = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
+      const float lse = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = n0 + tx * 4 + j;
         if (col >= q.classes) continue;
         float g = 0.f;
-        if (counts) g = scale * (y - q.first_class == col ? expm1f(-loss) : exp2f(z[i][j] - lse2));
+        if (counts) g = scale * (y - q.first_class == col ? expm1f(-loss) : expf(z[i][j] - lse));
         reinterpret_cast<float*>(q.g)[(int64_t)row * q.g_ld + col] = g;
       }
     }
@@ -577,15 +589,18 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   if (bias) {
     const int64_t padded = (classes + 255) / 256 * 256 + 256;
     const unsigned blocks = (unsigned)((padded + THREADS - 1) / THREADS < 1024 ? (padded + THREADS - 1) / THREADS : 1024);
-    if (bias_dtype == WCN_F32) ce_bias_kernel<float><<<blocks, THREADS, 0, st>>>((const float*)bias, classes, padded, bias2);
-    else if (bias_dtype == WCN_F16) ce_bias_kernel<__half><<<blocks, THREADS, 0, st>>>((const __half*)bias, classes, padded, bias2);
-    else ce_bias_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>((const __nv_bfloat16*)bias, classes, padded, bias2);
+    const float unit = dtype == WCN_F32 ? 1.f : LOG2E;
+    if (bias_dtype == WCN_F32) ce_bias_kernel<float><<<blocks, THREADS, 0, st>>>((const float*)bias, classes, padded, unit, bias2);
+    else if (bias_dtype == WCN_F16) ce_bias_kernel<__half><<<blocks, THREADS, 0, st>>>((const __half*)bias, classes, padded, unit, bias2);
+    else ce_bias_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>((const __nv_bfloat16*)bias, classes, padded, unit, bias2);
   }
   const int parts = logit_parts(n, classes, dtype);
   wcn_ce_piece q = {};
   q.x = x; q.w = w; q.x_ld = x_ld; q.w_ld = w_ld; q.rows = (int)n; q.classes = (int)classes; q.channels = channels;
   q.bias2 = bias ? bias2 : nullptr;
   q.part = (float2*)workspace;
+  q.labels = labels; q.ignore = ignore; q.all_classes = classes;
+  q.label_logits = loss_rows;
   if (dtype == WCN_F32) {
     ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)((classes + TILE - 1) / TILE)), THREADS, 0, st>>>(q);
   } else {
@@ -599,10 +614,9 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   const int blocks = loss_blocks(n);
   p.block_sums = (double*)((char*)workspace + aligned((int64_t)parts * n * 8));
   p.block_counts = (int32_t*)(p.block_sums + blocks);
-  if (dtype == WCN_F16) ce_loss_kernel<__half, true><<<blocks, THREADS, 0, st>>>(p);
-  else if (dtype == WCN_BF16) ce_loss_kernel<__nv_bfloat16, true><<<blocks, THREADS, 0, st>>>(p);
-  else if (on16(x) && on16(w) && x_ld % 4 == 0 && w_ld % 4 == 0) ce_loss_kernel<float, true><<<blocks, THREADS, 0, st>>>(p);
-  else ce_loss_kernel<float, false><<<blocks, THREADS, 0, st>>>(p);
+  if (dtype == WCN_F16) ce_loss_kernel<__half><<<blocks, THREADS, 0, st>>>(p);
+  else if (dtype == WCN_BF16) ce_loss_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>(p);
+  else ce_loss_kernel<float><<<blocks, THREADS, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 

@@ -30,11 +30,12 @@ struct wcn_ce_piece {
   const void* w;            // first class
   int64_t x_ld, w_ld;
   int rows, classes, channels;
-  const float* bias2;       // bias / ln 2 from the first class on, -inf from the last class to a multiple of 256; null: none
-  // forward: [parts][rows] of (largest, sum of 2^(z - largest)), z in units of ln 2
+  const float* bias2;       // bias / ln 2 (fp32: bias) from the first class on, -inf from the last class to a multiple of 256; null: none
+  // forward: [parts][rows] of (largest, sum of exp(z - largest)), z in units of ln 2 (fp32: as it is)
   float2* part;
+  float* label_logits;      // of each row, where its label names a class (fp32)
   // backward
-  const float* lse2;        // of the piece's rows, in units of ln 2
+  const float* lse2;        // of the piece's rows, in the logits' units
   const float* loss;
   const int64_t* labels;
   const float* row_scale;   // gradient of each row's loss (null: 1), divided by *row_max (0: all of them are 0 or no numbers)
