@@ -38,3 +38,13 @@ def test_moments_beyond_their_end_are_refused(slot):
     assert step([300], [slot], 512) == BOUNDS
     assert step([5, 300], [0, slot], 512) == BOUNDS
     assert step([(1 << 63) - 1], [0], 512) == BOUNDS
+
+
+@pytest.mark.parametrize("dtype,size", [(_native.WCN_F32, 4), (_native.WCN_BF16, 2)])
+@pytest.mark.parametrize("n", [1, 130, 3000])
+def test_the_logits_gradient_has_pieces_of_512_mb_at_most(dtype, size, n):
+    """Whatever the classes are: with it a piece's gradients of the weights in fp32, for up to 23 divisions of 3000 rows."""
+    for v in (70_000, 4_300_000, 40_000_000):
+        piece = min(v, max(1024, (512 << 20) // (size * n) + 256))
+        parts = -(-n // 128)
+        assert _native.query_bytes("wcn_linear_ce_workspace_bytes", n, 8, v, dtype, 2) <= (512 << 20) + parts * piece * 16 * 4 + 4 * 16 * v + (1 << 20)

@@ -379,59 +379,74 @@ __device__ __forceinline__ void fp32_tile(const float* a, int64_t a_ld, const fl
   }
 }
 
+// A block has `per` tiles of classes side by side (GRAD: one), of which each row leaves one (largest, sum).
 template <bool GRAD>
-__global__ void __launch_bounds__(THREADS) ce_logits_fp32_kernel(const __grid_constant__ wcn_ce_piece q) {
-  const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float z[4][4], unused[4];
-  fp32_tile<LOGITS>((const float*)q.x, q.x_ld, (const float*)q.w, q.w_ld, m0, n0, q.rows, q.classes, 0, q.channels, z, unused);
+__global__ void __launch_bounds__(THREADS, 4) ce_logits_fp32_kernel(const __grid_constant__ wcn_ce_piece q, int per) {
+  const int m0 = blockIdx.x * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n_tiles = (q.classes + TILE - 1) / TILE;
+  __shared__ float2 so_far[TILE];   // of each row, its first thread's alone
+  if (!GRAD && threadIdx.x < TILE) so_far[threadIdx.x] = make_float2(-INFINITY, 0.f);   // (barriers follow)
+  for (int n = GRAD ? blockIdx.y : blockIdx.y * per, last = GRAD ? n + 1 : min(n + per, n_tiles); n < last; ++n) {
+    const int n0 = n * TILE;
+    float z[4][4], unused[4];
+    fp32_tile<LOGITS>((const float*)q.x, q.x_ld, (const float*)q.w, q.w_ld, m0, n0, q.rows, q.classes, 0, q.channels, z, unused);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + tx * 4 + j;
-      z[i][j] = col >= q.classes ? -INFINITY : q.bias2 ? z[i][j] + __ldg(&q.bias2[col]) : z[i][j];
-    }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + ty * 4 + i;
-    if (!GRAD) {
-      if (row < q.rows) {
-        const int64_t in = __ldg(&q.labels[row]) - (n0 + tx * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (in == j && n0 + tx * 4 + j < q.classes) q.label_logits[row] = z[i][j];
-      }
-      float top = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3])), by = top == -INFINITY ? 0.f : top, sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum += expf(z[i][j] - by);
-#pragma unroll
-      for (int o = 8; o; o >>= 1) {   // the 16 threads of a row
-        const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        const float now = fmaxf(top, t);
-        by = now == -INFINITY ? 0.f : now;
-        sum = sum * expf(top - by) + s * expf(t - by);
-        top = now;
-      }
-      if (tx == 0 && row < q.rows) q.part[(int64_t)blockIdx.y * q.rows + row] = make_float2(top, sum);
-    } else if (row < q.rows) {
-      const int64_t y = __ldg(&q.labels[row]);
-      const bool counts = y != q.ignore && y >= 0 && y < q.all_classes;
-      float scale = 1.f;
-      if (q.row_scale) {
-        const float most = __ldg(q.row_max);
-        scale = __ldg(&q.row_scale[row]) / (most > 0.f ? most : 1.f);
-      }
-      const float lse = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = n0 + tx * 4 + j;
-        if (col >= q.classes) continue;
-        float g = 0.f;
-        if (counts) g = scale * (y - q.first_class == col ? expm1f(-loss) : expf(z[i][j] - lse));
-        reinterpret_cast<float*>(q.g)[(int64_t)row * q.g_ld + col] = g;
+        z[i][j] = col >= q.classes ? -INFINITY : q.bias2 ? z[i][j] + __ldg(&q.bias2[col]) : z[i][j];
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = m0 + ty * 4 + i;
+      if (!GRAD) {
+        if (row < q.rows) {
+          const int64_t in = __ldg(&q.labels[row]) - (n0 + tx * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (in == j && n0 + tx * 4 + j < q.classes) q.label_logits[row] = z[i][j];
+        }
+        float top = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3])), by = top == -INFINITY ? 0.f : top, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += expf(z[i][j] - by);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) {   // the 16 threads of a row
+          const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o), s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+          const float now = fmaxf(top, t);
+          by = now == -INFINITY ? 0.f : now;
+          sum = sum * expf(top - by) + s * expf(t - by);
+          top = now;
+        }
+        if (tx == 0) {
+          const float2 old = so_far[ty * 4 + i];
+          const float now = fmaxf(old.x, top);
+          by = now == -INFINITY ? 0.f : now;
+          so_far[ty * 4 + i] = make_float2(now, old.y * expf(old.x - by) + sum * expf(top - by));
+        }
+      } else if (row < q.rows) {
+        const int64_t y = __ldg(&q.labels[row]);
+        const bool counts = y != q.ignore && y >= 0 && y < q.all_classes;
+        float scale = 1.f;
+        if (q.row_scale) {
+          const float most = __ldg(q.row_max);
+          scale = __ldg(&q.row_scale[row]) / (most > 0.f ? most : 1.f);
+        }
+        const float lse = __ldg(&q.lse2[row]), loss = __ldg(&q.loss[row]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = n0 + tx * 4 + j;
+          if (col >= q.classes) continue;
+          float g = 0.f;
+          if (counts) g = scale * (y - q.first_class == col ? expm1f(-loss) : expf(z[i][j] - lse));
+          reinterpret_cast<float*>(q.g)[(int64_t)row * q.g_ld + col] = g;
+        }
       }
     }
   }
+  if (GRAD || tx) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (m0 + ty * 4 + i < q.rows) q.part[(int64_t)blockIdx.y * q.rows + m0 + ty * 4 + i] = so_far[ty * 4 + i];
 }
 
 template <bool TRANS>
@@ -468,8 +483,12 @@ int fp32_product(const wcn_ce_product& q, bool transposed, cudaStream_t st) {
 
 // ------------------------------------------------------------------ plans
 
+// Tiles of a block of fp32 losses: a row has at most 256 (largest, sum), 2 KB, as in 16 bits.
+int tiles_a_part(int64_t v) { return (int)((v + 256 * TILE - 1) / (256 * TILE)); }
+
 int logit_parts(int64_t n, int64_t v, int dtype) {
-  return dtype == WCN_F32 ? (int)((v + TILE - 1) / TILE) : wcn_ce_logits_parts((int)n, (int)v);
+  const int64_t part = (int64_t)TILE * tiles_a_part(v);
+  return dtype == WCN_F32 ? (int)((v + part - 1) / part) : wcn_ce_logits_parts((int)n, (int)v);
 }
 int loss_blocks(int64_t n) {
   const int64_t want = (n + THREADS / 8 - 1) / (THREADS / 8), most = 8 * (int64_t)wcn_num_sms();
@@ -515,8 +534,9 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
   p.rows = wcn_ce_round((n + p.row_pieces - 1) / p.row_pieces, 128);
   p.row_pieces = (int)((n + p.rows - 1) / p.rows);
   if (p.rows > n) p.rows = (int)n;
-  int64_t most = PIECE_BYTES / ((int64_t)p.rows * e) / 256 * 256;
+  int64_t most = PIECE_BYTES / ((int64_t)(p.fused ? wcn_ce_round(p.rows, 128) : p.rows) * e) / 256 * 256;   // (fused: whole tiles of g)
   if (most < 1024) most = 1024;
+  if (dtype == WCN_F32 && most > 65535 / 4 * 4 * TILE) most = 65535 / 4 * 4 * TILE;   // (a grid has 65 535 tiles in y)
   p.class_pieces = (int)((v + most - 1) / most);
   p.classes = p.class_pieces == 1 ? (int)v : wcn_ce_round((v + p.class_pieces - 1) / p.class_pieces, 256);
   p.class_pieces = (int)((v + p.classes - 1) / p.classes);
@@ -546,7 +566,7 @@ Pieces cut(int64_t n, int c, int64_t v, int dtype, bool x, bool w, bool b) {
 }
 
 bool sizes_ok(int64_t n, int32_t c, int64_t v, int dtype) {
-  return n > 0 && n < 0x7FFFFF00ll && v > 0 && v < 0x7FFFFF00ll && v / TILE < 65535 && c > 0 && c <= 32768 && dtype >= WCN_F32 && dtype <= WCN_BF16;
+  return n > 0 && n < 0x7FFFFF00ll && v > 0 && v < 0x7FFFFF00ll && c > 0 && c <= 32768 && dtype >= WCN_F32 && dtype <= WCN_BF16;
 }
 
 bool matrix_ok(const void* p, int64_t ld, int c, int dtype) {
@@ -602,7 +622,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   q.labels = labels; q.ignore = ignore; q.all_classes = classes;
   q.label_logits = loss_rows;
   if (dtype == WCN_F32) {
-    ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)((classes + TILE - 1) / TILE)), THREADS, 0, st>>>(q);
+    ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)parts), THREADS, 0, st>>>(q, tiles_a_part(classes));
   } else {
     const int rc = wcn_ce_logits(q, nullptr, dtype, false, 0.f, dev_status, st);
     if (rc != WCN_OK) return rc;
@@ -682,7 +702,7 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
         if (rc == WCN_OK && dx)
           rc = join({slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? (char*)dx + r0 * channels * e : nullptr, rows, channels, p.ld, slots, scale, dev_status,
                      (vs + 127) / 128, chunk}, dtype, st);
-      } else if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q);
+      } else if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q, 1);
       else rc = wcn_ce_logits(q, nullptr, dtype, true, lift, dev_status, st);
       if (rc != WCN_OK) return rc;
       if (dx && !p.fused) {
