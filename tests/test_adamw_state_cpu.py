@@ -1,0 +1,57 @@
+"""States that the optimizer refuses, and what is left of its own then."""
+import copy
+
+import pytest
+import torch
+
+from warpconvnet_b200.optim import AdamW
+
+
+def parameters():
+    return [torch.nn.Parameter(torch.arange(3.0)), torch.nn.Parameter(torch.ones(2, 2))]
+
+
+def stepped(cls=torch.optim.AdamW, **kw):
+    """The state of an optimizer of torch's after a step."""
+    params = parameters()
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = cls(params, lr=0.5, **kw)
+    opt.step()
+    return opt.state_dict()
+
+
+def wrong_size():
+    saved = copy.deepcopy(stepped())
+    saved["state"][1]["exp_avg"] = torch.zeros(5)
+    return saved
+
+
+def wrong_group():
+    saved = copy.deepcopy(stepped())
+    saved["param_groups"][0]["params"] = [0]
+    del saved["state"][1]
+    return saved
+
+
+def two_groups():
+    saved = copy.deepcopy(stepped())
+    saved["param_groups"].append({**saved["param_groups"][0], "params": []})
+    return saved
+
+
+@pytest.mark.parametrize("saved", [lambda: stepped(amsgrad=True), wrong_size, wrong_group, two_groups, stepped],
+                         ids=["amsgrad", "wrong_size", "wrong_group", "two_groups", "parameters_on_the_host"])
+def test_a_refused_state_leaves_everything_as_it_was(saved):
+    params = parameters()
+    opt = AdamW(params, lr=0.1, betas=(0.5, 0.6))
+    kept = {p: {"exp_avg": torch.full_like(p, 7.0)} for p in params}   # (stands for what a step leaves: that needs a device)
+    arenas = {p: object() for p in params}
+    opt.state.update(kept)
+    opt._arena_of.update(arenas)
+    before = {k: v for k, v in opt.param_groups[0].items() if k != "params"}
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved())
+    assert {k: v for k, v in opt.param_groups[0].items() if k != "params"} == before
+    assert opt.param_groups[0]["params"] == params and opt._arena_of == arenas
+    assert all(opt.state[p] is kept[p] for p in params)

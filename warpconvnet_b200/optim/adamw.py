@@ -215,16 +215,18 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise ValueError(f"all groups of this optimizer have moments of {self.state_bits} bits")
 
-    def _make_room(self, params: Sequence[Tensor]) -> None:
-        """Moments for the parameters that have none."""
+    def _rooms(self, params: Sequence[Tensor]) -> dict:
+        """``{parameter: its arena}``, new ones."""
         by_device: dict = {}
         for p in params:
             by_device.setdefault(p.device, []).append(p)
-        for group in by_device.values():
-            arena = _Arena(group, self.state_bits)
-            for p in group:
-                self._arena_of[p] = arena
-                self.state[p] = arena.state(p)
+        return {p: arena for group in by_device.values() for arena in (_Arena(group, self.state_bits),) for p in group}
+
+    def _make_room(self, params: Sequence[Tensor]) -> None:
+        """Moments for the parameters that have none."""
+        for p, arena in self._rooms(params).items():
+            self._arena_of[p] = arena
+            self.state[p] = arena.state(p)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -252,17 +254,15 @@ class AdamW(torch.optim.Optimizer):
 
     # -- what is kept travels as the views of ``state``: copies are put into flat tensors again
 
-    def _take_state(self, state: dict) -> None:
-        """Moments and steps from ``{parameter: entries}``."""
-        self._arena_of = {}
-        self.state.clear()
+    def _filled(self, state: dict) -> dict:
+        """``{parameter: its arena}`` with the moments and steps of ``{parameter: entries}``; what is kept so far stays as it is."""
         known = [p for g in self.param_groups for p in g["params"] if p in state]
         for p in known:
             if not p.is_cuda:
                 raise ValueError("move the parameters to their device before their optimizer's state is loaded")
-        self._make_room(known)
+        rooms = self._rooms(known)
         for p in known:
-            mine = self.state[p]
+            mine = rooms[p].state(p)
             if set(mine) != set(state[p]):
                 raise ValueError(f"state with {sorted(state[p])} cannot be loaded into an optimizer with moments of {self.state_bits} bits")
             for name, view in mine.items():
@@ -270,24 +270,36 @@ class AdamW(torch.optim.Optimizer):
                 if value.numel() != view.numel():
                     raise ValueError(f"{name} of a parameter with {p.numel()} elements has {value.numel()}")
                 view.copy_(value.to(view.device).view(view.shape))
+        return rooms
+
+    def _put(self, rooms: dict) -> None:
+        """Arenas in the place of those so far."""
+        self._arena_of = rooms
+        self.state.clear()
+        for p, arena in rooms.items():
+            self.state[p] = arena.state(p)
 
     def load_state_dict(self, state_dict):
-        """Takes the state of an optimizer of this class with the same ``state_bits``, and with 32 bits one of ``torch.optim.AdamW``."""
-        params = [p for g in self.param_groups for p in g["params"]]
-        names = [i for g in state_dict["param_groups"] for i in g["params"]]
-        entries = {p: state_dict["state"][i] for p, i in zip(params, names) if i in state_dict["state"]}
-        bits = {g.get("state_bits", 32) for g in state_dict["param_groups"]}
+        """Takes the state of an optimizer of this class with the same ``state_bits``, and with 32 bits one of ``torch.optim.AdamW``.
+        A state that is refused leaves everything as it was."""
+        saved = state_dict["param_groups"]
+        if len(saved) != len(self.param_groups):
+            raise ValueError("loaded state dict has a different number of parameter groups")
+        if any(len(own["params"]) != len(g["params"]) for own, g in zip(self.param_groups, saved)):
+            raise ValueError("loaded state dict contains a parameter group that doesn't match the size of optimizer's group")
+        bits = {g.get("state_bits", 32) for g in saved}
         if bits - {self.state_bits}:
             raise ValueError(f"moments of {sorted(bits)} bits cannot be loaded into an optimizer with moments of {self.state_bits} bits")
-        groups = [{**own, **g} for own, g in zip(({k: v for k, v in g.items() if k != "params"} for g in self.param_groups), state_dict["param_groups"])]
-        if len(groups) != len(self.param_groups) or len(state_dict["param_groups"]) != len(self.param_groups):
-            raise ValueError("loaded state dict has a different number of parameter groups")
+        params = [p for g in self.param_groups for p in g["params"]]
+        names = [i for g in saved for i in g["params"]]
+        rooms = self._filled({p: state_dict["state"][i] for p, i in zip(params, names) if i in state_dict["state"]})
+        groups = [{**{k: v for k, v in own.items() if k != "params"}, **g} for own, g in zip(self.param_groups, saved)]
         super().load_state_dict({"state": {}, "param_groups": groups})
-        self._take_state(entries)
+        self._put(rooms)
 
     def __setstate__(self, state):
         super().__setstate__(state)
         self.state_bits = self.defaults["state_bits"]
         self._arena_of = {}
         if "state" in state:
-            self._take_state({p: dict(entries) for p, entries in self.state.items()})
+            self._put(self._filled({p: dict(entries) for p, entries in self.state.items()}))
