@@ -55,3 +55,27 @@ def test_a_refused_state_leaves_everything_as_it_was(saved):
     assert {k: v for k, v in opt.param_groups[0].items() if k != "params"} == before
     assert opt.param_groups[0]["params"] == params and opt._arena_of == arenas
     assert all(opt.state[p] is kept[p] for p in params)
+
+
+@pytest.mark.parametrize("saved", [lambda: stepped(maximize=True), lambda: stepped(torch.optim.Adam, weight_decay=0.1),
+                                   lambda: torch.optim.AdamW(parameters(), maximize=True).state_dict(), lambda: torch.optim.AdamW(parameters(), amsgrad=True).state_dict()],
+                         ids=["maximize", "adam", "maximize_before_a_step", "amsgrad_before_a_step"])
+def test_states_of_another_rule_are_refused(saved):
+    """What would be loaded and then not followed."""
+    opt = AdamW(parameters(), lr=0.1)
+    with pytest.raises(ValueError, match="maximize|amsgrad|decoupled"):
+        opt.load_state_dict(saved())
+    assert opt.param_groups[0]["lr"] == 0.1 and "maximize" not in opt.param_groups[0]
+
+
+def test_groups_of_another_rule_are_refused():
+    p, q = parameters()
+    for kw in ({"maximize": True}, {"amsgrad": True}, {"decoupled_weight_decay": False}):
+        with pytest.raises(ValueError, match="maximize|amsgrad|decoupled"):
+            AdamW([{"params": [p], **kw}])
+        opt = AdamW([p])
+        with pytest.raises(ValueError, match="maximize|amsgrad|decoupled"):
+            opt.add_param_group({"params": [q], **kw})
+        assert len(opt.param_groups) == 1
+    AdamW([{"params": [p], "maximize": False, "amsgrad": False, "fused": True, "decoupled_weight_decay": True}])
+    AdamW(parameters()).load_state_dict(torch.optim.AdamW(parameters(), lr=0.5).state_dict())

@@ -155,6 +155,13 @@ def decode_moments(exp_avg: Tensor, exp_avg_base: Tensor, exp_avg_sq: Tensor, ex
     return m, v
 
 
+def _check_rule(group: dict) -> None:
+    """Flags of torch's optimizers for steps that this one does not make."""
+    asked = [k for k, plain in (("maximize", False), ("amsgrad", False), ("decoupled_weight_decay", True)) if group.get(k, plain) != plain]
+    if asked:
+        raise ValueError(f"a group with {', '.join(f'{k}={group[k]}' for k in asked)} is not AdamW's")
+
+
 class _Arena:
     """The flat moments and step counts of some parameters."""
 
@@ -211,9 +218,13 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        if self.param_groups[-1]["state_bits"] != self.state_bits:
+        try:
+            if self.param_groups[-1]["state_bits"] != self.state_bits:
+                raise ValueError(f"all groups of this optimizer have moments of {self.state_bits} bits")
+            _check_rule(self.param_groups[-1])
+        except ValueError:
             self.param_groups.pop()
-            raise ValueError(f"all groups of this optimizer have moments of {self.state_bits} bits")
+            raise
 
     def _rooms(self, params: Sequence[Tensor]) -> dict:
         """``{parameter: its arena}``, new ones."""
@@ -290,6 +301,8 @@ class AdamW(torch.optim.Optimizer):
         bits = {g.get("state_bits", 32) for g in saved}
         if bits - {self.state_bits}:
             raise ValueError(f"moments of {sorted(bits)} bits cannot be loaded into an optimizer with moments of {self.state_bits} bits")
+        for g in saved:
+            _check_rule(g)
         params = [p for g in self.param_groups for p in g["params"]]
         names = [i for g in saved for i in g["params"]]
         rooms = self._filled({p: state_dict["state"][i] for p, i in zip(params, names) if i in state_dict["state"]})
