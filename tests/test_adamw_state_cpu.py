@@ -79,3 +79,17 @@ def test_groups_of_another_rule_are_refused():
         assert len(opt.param_groups) == 1
     AdamW([{"params": [p], "maximize": False, "amsgrad": False, "fused": True, "decoupled_weight_decay": True}])
     AdamW(parameters()).load_state_dict(torch.optim.AdamW(parameters(), lr=0.5).state_dict())
+
+
+def test_a_scalers_numbers_go_to_the_device_of_each_parameter(monkeypatch):
+    """A GradScaler leaves its scale and its flag on one device; parameters may be on several."""
+    seen = []
+    monkeypatch.setattr("warpconvnet_b200.optim.adamw.adamw_step",
+                        lambda params, grads, *a, grad_scale, found_inf, **kw: seen.append((params[0].device, grad_scale.device, found_inf.device)))
+    params = [torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3, device="meta"))]
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    opt = AdamW(params)
+    opt.grad_scale, opt.found_inf = torch.ones(1), torch.zeros(1)
+    opt.step()
+    assert len(seen) == 2 and all(p == scale == found for p, scale, found in seen)

@@ -162,6 +162,11 @@ def _check_rule(group: dict) -> None:
         raise ValueError(f"a group with {', '.join(f'{k}={group[k]}' for k in asked)} is not AdamW's")
 
 
+def _beside(t: Optional[Tensor], p: Tensor) -> Optional[Tensor]:
+    """``t`` on the device of ``p`` (a scaler has one number for all devices)."""
+    return t if t is None or t.device == p.device else t.to(p.device, non_blocking=True)
+
+
 class _Arena:
     """The flat moments and step counts of some parameters."""
 
@@ -260,7 +265,7 @@ class AdamW(torch.optim.Optimizer):
                 adamw_step(some, [p.grad for p in some], arena.exp_avg, arena.exp_avg_sq, arena.steps, lr=group["lr"], betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"], exp_avg_base=arena.exp_avg_base,
                            exp_avg_sq_base=arena.exp_avg_sq_base, slots=[s for _, s in places], step_index=[i for i, _ in places],
-                           grad_scale=scale, found_inf=found)
+                           grad_scale=_beside(scale, some[0]), found_inf=_beside(found, some[0]))
         return loss
 
     # -- what is kept travels as the views of ``state``: copies are put into flat tensors again
