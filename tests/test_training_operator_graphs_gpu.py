@@ -1,0 +1,17 @@
+"""Group norm and linear cross entropy in graphs: of gradients, of CUDA, and under autocast with function transforms."""
+import pytest
+import torch
+
+from warpconvnet_b200 import SegmentedGroupNorm, Voxels, linear_cross_entropy, segmented_group_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("which", [(1, 1, 1), (0, 1, 0), (0, 0, 1), (1, 0, 1)])
+def test_a_graph_of_the_norms_gradient_without_rows(which):
+    x, w, b = torch.zeros(0, 8, device=DEV), torch.ones(8, device=DEV), torch.ones(8, device=DEV)
+    leaves = [t for t, need in zip((x, w, b), which) if t.requires_grad_(bool(need)).requires_grad]
+    y = segmented_group_norm(x, [0, 0], 2, w, b)
+    grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, leaves))
