@@ -15,3 +15,16 @@ def test_a_graph_of_the_norms_gradient_without_rows(which):
     y = segmented_group_norm(x, [0, 0], 2, w, b)
     grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
     assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, leaves))
+
+
+@pytest.mark.parametrize("low", [torch.float16, torch.bfloat16])
+def test_transforms_under_autocast_are_in_32_bits_too(low):
+    """Inputs are brought to autocast's type once; what is computed from them is not."""
+    g = torch.Generator().manual_seed(0)
+    x, w, labels = torch.randn(200, 64, generator=g).to(DEV), torch.randn(30, 64, generator=g).to(DEV), torch.randint(0, 30, (200,), generator=g).to(DEV)
+    want = linear_cross_entropy(x.to(low).double().float(), w.to(low).double().float(), labels)
+    with torch.autocast("cuda", dtype=low):
+        plain = linear_cross_entropy(x, w, labels)
+        got, tangent = torch.func.jvp(lambda t: linear_cross_entropy(t, w, labels), (x,), (torch.ones_like(x),))
+    # (sums of 64 products in another order)
+    assert abs(float(plain) - float(want)) <= 2e-5 and abs(float(got) - float(want)) <= 2e-5

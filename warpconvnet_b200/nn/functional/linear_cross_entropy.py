@@ -68,7 +68,8 @@ def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], 
 
 def formula(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: str) -> Tensor:
     """The same through torch, logits and all: for a graph of the gradient, forward-mode differentiation and function transforms."""
-    z = x.float() @ weight.float().t()
+    with torch.autocast("cuda", enabled=False):   # (what the inputs were brought to counts, not what a product would be)
+        z = x.float() @ weight.float().t()
     labels = torch.where((labels >= 0) & (labels < weight.shape[0]), labels, ignore_index)
     return torch.nn.functional.cross_entropy(z if bias is None else z + bias.float(), labels, ignore_index=ignore_index, reduction=reduction)
 
