@@ -84,3 +84,9 @@ def test_weights_of_rows_that_do_not_count(dtype, n, c, v):
     got = gradients(x, w, labels, b, grad)
     assert all(off(p, q) <= TOL[dtype] for p, q in zip(got, want))
     assert all(torch.equal(p, q) for p, q in zip(got, clean))
+
+
+def test_row_losses_hold_no_more_than_themselves():
+    x, w, labels, b = (t.to(DEV) for t in problem(1000, 64, 40, torch.bfloat16))
+    for rows in (linear_cross_entropy(x, w, labels, b, reduction="none"), linear_cross_entropy(x.requires_grad_(True), w, labels, b, reduction="none").detach()):
+        assert rows.untyped_storage().nbytes() == 4 * 1000

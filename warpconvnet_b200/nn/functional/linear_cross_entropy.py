@@ -46,7 +46,7 @@ def _kept(n: int, v: int, bias: bool):
     return 2 * n, at_bias, at_bias + (-(-v // 256) * 256 + 256 if bias else 0)
 
 
-def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: int):
+def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: int, keep: bool):
     """(loss or losses, what the backward pass needs: log-sum-exp and loss of each row, the count, the bias in units of ln 2; the
     matrices as the kernels read them)"""
     (n, c), v, dev = x.shape, weight.shape[0], x.device
@@ -56,14 +56,15 @@ def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], 
     at_count, at_bias, length = _kept(n, v, bias is not None)
     kept = torch.empty(length, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
+    rows = torch.empty(n, dtype=torch.float32, device=dev) if not (keep or reduction) else kept[n:2 * n]   # (a result holds no more than itself)
     base = kept.data_ptr()
     ws = _workspace(n, c, v, code, 0, dev)
     with on_device(dev):
         check(lib().wcn_linear_ce(ptr(x), x_ld, n, c, ptr(weight), w_ld, v, ptr(bias), dtype_code(bias.dtype) if bias is not None else 0,
-                                  ptr(labels), ignore_index, code, reduction, base, base + 4 * n, base + 4 * at_bias if bias is not None else None,
+                                  ptr(labels), ignore_index, code, reduction, base, ptr(rows), base + 4 * at_bias if bias is not None else None,
                                   base + 4 * at_count, ptr(loss), ptr(ws), ws.numel(), ptr(_counter(dev, stream)), ptr(device_status(dev)), stream),
               "wcn_linear_ce")
-    return (loss if reduction else kept[n:2 * n]), kept, x, weight
+    return (loss if reduction else rows), kept, x, weight
 
 
 def formula(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], ignore_index: int, reduction: str) -> Tensor:
@@ -79,7 +80,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], labels: Tensor, ignore_index: int, reduction: str):
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         loss, kept, x_rows, w_rows = _forward(x.detach(), weight.detach(), labels, None if bias is None else bias.detach().contiguous(),
-                                              ignore_index, _REDUCTIONS[reduction])
+                                              ignore_index, _REDUCTIONS[reduction], True)
         # (matrices that had to be copied are kept with them: there are not two copies to be made)
         copied = tuple(None if rows.data_ptr() == given.data_ptr() else rows for rows, given in ((x_rows, x), (w_rows, weight)))
         ctx.save_for_backward(x, weight, bias, labels, kept, *copied)
@@ -148,4 +149,4 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, bias: Option
         return formula(x, weight, labels, bias, ignore_index, reduction)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LinearCrossEntropy.apply(x, weight, bias, labels, ignore_index, reduction)
-    return _forward(x, weight, labels, None if bias is None else bias.contiguous(), ignore_index, how)[0]
+    return _forward(x, weight, labels, None if bias is None else bias.contiguous(), ignore_index, how, False)[0]
