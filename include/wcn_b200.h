@@ -609,6 +609,9 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
                             const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
                             int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream);
 
+/* Kernels that this thread's last wcn_group_norm*, wcn_linear_ce* (not the queries) or wcn_adamw_step launched. */
+int wcn_training_launches(void);
+
 /* ------------------------------------------------------------------ cross entropy of a linear layer */
 
 /* loss_rows[i] = log sum_j exp(z_ij) - z_iy of z = x w^T + bias, x [n, channels], w [classes, channels] of one dtype (rows x_ld and

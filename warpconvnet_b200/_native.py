@@ -92,6 +92,7 @@ SIGNATURES = {
     "wcn_net_run": [_c_vp, _c_i32, _c_vp, _c_vp, _c_vp, _c_i32, _c_vp, _c_vp],
     "wcn_group_norm_workspace_bytes": [_c_vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp],
     "wcn_group_norm_sync_bytes": [_p_i64],
+    "wcn_training_launches": [],
     "wcn_group_norm": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp,
                        _c_vp, _c_i64, _c_vp, _c_vp, _c_vp],
     "wcn_group_norm_backward": [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp,
@@ -136,8 +137,7 @@ KERNELS_PER_CALL = {
     "wcn_gather_rows": 1, "wcn_scatter_add_rows": 1, "wcn_conv_pack_weight": 1, "wcn_conv_fwd": 1,
     "wcn_selftest_bounded_wait": 1, "wcn_brick_build": 3, "wcn_kmap_search_bricks": 1,
     "wcn_conv_rows_fwd": 1, "wcn_batch_norm_train": 2, "wcn_column_sums": 2, "wcn_batch_norm_backward": 2, "wcn_conv_pack_weight_from": 1, "wcn_cells_build": 4, "wcn_kmap_search_cells": 1, "wcn_kmap_scan_host": 2, "wcn_unique_counts": 2, "wcn_morton_sort": 1, "wcn_pyramid": 2, "wcn_level_maps": 5,
-    "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1,  # (of up to 320 scenes)
-    "wcn_linear_ce": 2, "wcn_linear_ce_backward": 5,  # (of one piece)
+    "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1, "wcn_linear_ce": 1, "wcn_linear_ce_backward": 1,
 }
 LAUNCH_COUNTS: Counter = Counter()
 
@@ -179,6 +179,11 @@ def count_f32_launches(name: str) -> None:
     """Corrects what the call just made was counted as: with a workspace ``wcn_conv_fwd`` launches one or two kernels,
     ``wcn_conv_wgrad_f32`` two or three."""
     LAUNCH_COUNTS[name] += lib().wcn_conv_f32_launches() - KERNELS_PER_CALL[name]
+
+
+def count_training_launches(name: str) -> None:
+    """The same for group norm, linear cross entropy and AdamW, which launch as many kernels as their sizes ask for."""
+    LAUNCH_COUNTS[name] += lib().wcn_training_launches() - KERNELS_PER_CALL[name]
 
 
 def launches_total() -> int:

@@ -261,6 +261,7 @@ int launch(const Tensor* t, Hyper& h, int count, unsigned blocks, cudaStream_t s
   memcpy(table.t, t, sizeof(Tensor) * count);
   h.count = count;
   adamw_kernel<P, G, EIGHT, MAX><<<blocks, THREADS, 0, st>>>(table, h);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -324,6 +325,7 @@ extern "C" int wcn_adamw_step(const int64_t* params, const int64_t* grads, const
                               void* exp_avg_sq, int16_t* exp_avg_sq_base, int64_t length, int32_t* steps, int64_t num_steps,
                               int64_t lr_bits, int64_t beta1_bits, int64_t beta2_bits, int64_t eps_bits, int64_t weight_decay_bits,
                               const float* lr, const float* grad_scale, const float* found_inf, uint32_t* counter, void* stream) {
+  wcn_launched = 0;
   if (count < 0 || (count && (!params || !grads || !sizes || !counter || (length && (!exp_avg || !exp_avg_sq)) || (num_steps && !steps))) || dtype < WCN_F32 ||
       dtype > WCN_BF16 || grad_dtype < WCN_F32 || grad_dtype > WCN_BF16 || !on32(exp_avg) || !on32(exp_avg_sq) || !exp_avg_base != !exp_avg_sq_base)
     return WCN_ERR_INVALID_PARAMETERS;

@@ -29,6 +29,7 @@ int wcn_conv_fp32_fwd(const void* feats, int64_t num_in, int64_t feats_ld, const
 // conv_split_tcgen05.cu
 bool wcn_conv_split_supported(int K, int c_in, int c_out);
 thread_local int wcn_f32_launches = 0;   // see wcn_conv_f32_launches
+thread_local int wcn_launched = 0;       // see wcn_training_launches
 int64_t wcn_conv_split_workspace(int64_t num_in, int K, int c_in, int c_out);
 int wcn_conv_split_fwd(const void* feats, int64_t num_in, int64_t feats_ld, const void* weight, const int32_t* nbr,
                        const int32_t* out_rows, int64_t M, int K, int c_in, int c_out, const float* scale, const float* shift,
@@ -136,6 +137,7 @@ extern "C" int wcn_conv_f32_workspace_bytes(int64_t num_in, int64_t num_out, int
 }
 
 extern "C" int wcn_conv_f32_launches(void) { return wcn_f32_launches; }
+extern "C" int wcn_training_launches(void) { return wcn_launched; }
 
 extern "C" int wcn_conv_fwd(int algo, const void* feats, int64_t num_in, int64_t feats_ld, const void* weight,
                             const void* packed_weight, const int32_t* nbr, const int32_t* out_rows,

@@ -769,6 +769,7 @@ template <typename T, int V, int ACT, int SUB, bool BACK> int all_launches(Param
     p.rstd = base.rstd ? base.rstd + q.i * p.G : nullptr;
     p.items = (p.out ? 2 : 1) * q.tiles + (p.sums ? (2 * p.C + JOINED - 1) / JOINED : 0);
     kern<<<p.items < grid_most ? p.items : grid_most, THREADS, smem, st>>>(s, p);
+    ++wcn_launched;
     p.add = 1;
     return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
   });
@@ -855,6 +856,7 @@ extern "C" int wcn_group_norm_sync_bytes(int64_t* bytes) {
 extern "C" int wcn_group_norm(const void* x, int64_t x_ld, const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups,
                               int dtype, const float* gamma, const float* beta, uint32_t eps_bits, int act, void* y, float* mean,
                               float* rstd, void* workspace, int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
   if (!norm_ok(scenes, offsets, channels, groups, dtype) || act < NONE || act > GELU || x_ld < channels || !mean != !rstd)
     return WCN_ERR_INVALID_PARAMETERS;
   if (!offsets[scenes]) return WCN_OK;
@@ -874,6 +876,7 @@ extern "C" int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* 
                                        int64_t scenes, int32_t channels, int32_t groups, int dtype, const float* gamma,
                                        const float* beta, const float* mean, const float* rstd, int act, void* dx, float* sums,
                                        void* workspace, int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
   if (!norm_ok(scenes, offsets, channels, groups, dtype) || act < NONE || act > GELU || x_ld < channels || dy_ld < channels)
     return WCN_ERR_INVALID_PARAMETERS;
   cudaStream_t st = wcn_stream(stream);

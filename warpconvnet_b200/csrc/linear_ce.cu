@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(THREADS) ce_join_both_kernel(const __grid_cons
 }
 
 template <typename TO> int join_as(const JoinParams& p, cudaStream_t st) {
+  ++wcn_launched;
   if (p.ld == 1) {
     ce_join_sums_kernel<TO><<<(unsigned)((p.m + 31) / 32), THREADS, 0, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
@@ -313,6 +314,7 @@ int join(const JoinParams& p, int dtype, cudaStream_t st) {
 template <typename TO> int join_both_as(const JoinParams& p, const JoinParams& sums, cudaStream_t st) {
   const int blocks = (int)((p.m * (p.ld / 4) + THREADS / 8 - 1) / (THREADS / 8));
   ce_join_both_kernel<TO><<<(unsigned)(blocks + (sums.m + 31) / 32), THREADS, 0, st>>>(p, sums, blocks);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 int join_both(const JoinParams& p, const JoinParams& sums, int dtype, cudaStream_t st) {
@@ -478,6 +480,7 @@ int fp32_product(const wcn_ce_product& q, bool transposed, cudaStream_t st) {
   const dim3 grid((q.m + TILE - 1) / TILE, (q.n + TILE - 1) / TILE, q.splits);
   if (transposed) ce_product_fp32_kernel<true><<<grid, THREADS, 0, st>>>(q, per);
   else ce_product_fp32_kernel<false><<<grid, THREADS, 0, st>>>(q, per);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -590,6 +593,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
                              const void* bias, int bias_dtype, const int64_t* labels, int64_t ignore, int dtype, int reduction,
                              float* lse2, float* loss_rows, float* bias2, int32_t* count, float* loss, void* workspace,
                              int64_t workspace_bytes, uint32_t* counter, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
   if (!sizes_ok(n, channels, classes, dtype) || !matrix_ok(x, x_ld, channels, dtype) || !matrix_ok(w, w_ld, channels, dtype) || !labels ||
       !lse2 || !loss_rows || !workspace || !on16(workspace) || !counter || !dev_status || (bias && (!bias2 || !on16(bias2))) ||
       reduction < 0 || reduction > 2 || (reduction && (!loss || !count)) || bias_dtype < WCN_F32 || bias_dtype > WCN_BF16)
@@ -613,6 +617,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
     if (bias_dtype == WCN_F32) ce_bias_kernel<float><<<blocks, THREADS, 0, st>>>((const float*)bias, classes, padded, unit, bias2);
     else if (bias_dtype == WCN_F16) ce_bias_kernel<__half><<<blocks, THREADS, 0, st>>>((const __half*)bias, classes, padded, unit, bias2);
     else ce_bias_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>((const __nv_bfloat16*)bias, classes, padded, unit, bias2);
+    ++wcn_launched;
   }
   const int parts = logit_parts(n, classes, dtype);
   wcn_ce_piece q = {};
@@ -623,6 +628,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   q.label_logits = loss_rows;
   if (dtype == WCN_F32) {
     ce_logits_fp32_kernel<false><<<dim3((unsigned)((n + TILE - 1) / TILE), (unsigned)parts), THREADS, 0, st>>>(q, tiles_a_part(classes));
+    ++wcn_launched;
   } else {
     const int rc = wcn_ce_logits(q, nullptr, dtype, false, 0.f, dev_status, st);
     if (rc != WCN_OK) return rc;
@@ -637,6 +643,7 @@ extern "C" int wcn_linear_ce(const void* x, int64_t x_ld, int64_t n, int32_t cha
   if (dtype == WCN_F16) ce_loss_kernel<__half><<<blocks, THREADS, 0, st>>>(p);
   else if (dtype == WCN_BF16) ce_loss_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>(p);
   else ce_loss_kernel<float><<<blocks, THREADS, 0, st>>>(p);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -645,6 +652,7 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
                                       const float* lse2, const float* loss_rows, const int32_t* count, const float* grad,
                                       const float* row_max, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
                                       int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
   if (!sizes_ok(n, channels, classes, dtype) || !matrix_ok(x, x_ld, channels, dtype) || !matrix_ok(w, w_ld, channels, dtype) || !labels ||
       !lse2 || !loss_rows || !grad || !workspace || !on32(workspace) || !on16(dx) || !on16(dw) || !dev_status || bias_dtype < WCN_F32 ||
       bias_dtype > WCN_BF16)
@@ -702,8 +710,10 @@ extern "C" int wcn_linear_ce_backward(const void* x, int64_t x_ld, int64_t n, in
         if (rc == WCN_OK && dx)
           rc = join({slab, (float*)(ws + p.acc_x), j > 0, j == p.class_pieces - 1 ? (char*)dx + r0 * channels * e : nullptr, rows, channels, p.ld, slots, scale, dev_status,
                      (vs + 127) / 128, chunk}, dtype, st);
-      } else if (dtype == WCN_F32) ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q, 1);
-      else rc = wcn_ce_logits(q, nullptr, dtype, true, lift, dev_status, st);
+      } else if (dtype == WCN_F32) {
+        ce_logits_fp32_kernel<true><<<dim3((rows + TILE - 1) / TILE, (vs + TILE - 1) / TILE), THREADS, 0, st>>>(q, 1);
+        ++wcn_launched;
+      } else rc = wcn_ce_logits(q, nullptr, dtype, true, lift, dev_status, st);
       if (rc != WCN_OK) return rc;
       if (dx && !p.fused) {
         wcn_ce_product d = {};

@@ -1184,6 +1184,7 @@ int launch_logits(LogitParams& p, size_t fixed, cudaStream_t st) {
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
   kern<<<p.units < sms ? p.units : sms, LOGIT_THREADS, fixed + kept + (size_t)p.stages * stage, st>>>(xm, wm, p);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -1235,6 +1236,7 @@ int launch_product(const wcn_ce_product& q, int32_t* dev_status, cudaStream_t st
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
   kern<<<p.units < sms ? p.units : sms, THREADS, fixed + (size_t)p.stages * stage, st>>>(am, bm, p);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -1263,6 +1265,7 @@ template <bool BF16> int launch_head(HeadParams& p, size_t smem, int blocks, cud
   constexpr auto kern = ce_head_kernel<BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   kern<<<blocks, LOGIT_THREADS, smem, st>>>(xm, wm, p);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
@@ -1276,6 +1279,7 @@ template <bool BF16> int launch_rows(RowsParams& p, cudaStream_t st) {
   constexpr auto kern = ce_rows_kernel<BF16>;
   if (!allow_smem<kern, ROWS_SMEM>()) return WCN_ERR_INITIALIZATION;
   kern<<<(p.total + p.chunk - 1) / p.chunk, ROWS_THREADS, rows_smem(p.q.channels), st>>>(xm, wm, p);
+  ++wcn_launched;
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 

@@ -128,6 +128,9 @@ static inline int wcn_num_sms() {
   return cached[dev];
 }
 
+// Kernels launched by the call that this thread is in, or by its last one (calls that launch as many as their sizes ask for).
+extern thread_local int wcn_launched;
+
 // Where a unique workspace keeps the number of distinct rows (hash_kmap.cu).
 const int* wcn_unique_total(const void* workspace, int64_t n);
 

@@ -10,7 +10,7 @@ from typing import Optional, Sequence, Union
 import torch
 from torch import Tensor
 
-from ..._native import check, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import _bits, _counter, reverse_mode_only
 
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
@@ -73,6 +73,7 @@ def _forward(x: Tensor, offsets: array, groups: int, weight, bias, eps: float, a
         check(lib().wcn_group_norm(ptr(x), ld, offsets.buffer_info()[0], scenes, c, groups, dc, ptr(weight), ptr(bias), _bits(eps), act, ptr(y),
                                    at, at + 4 * scenes * groups if keep else None, ptr(ws), ws.numel(), ptr(_sync(dev, stream)),
                                    ptr(device_status(dev)), stream), "wcn_group_norm")
+        count_training_launches("wcn_group_norm")
     return y, saved
 
 
@@ -120,6 +121,7 @@ class _SegmentedGroupNorm(torch.autograd.Function):
             check(lib().wcn_group_norm_backward(ptr(x), x_ld, ptr(dy), dy_ld, ctx.offsets.buffer_info()[0], scenes, c, ctx.groups, dc, ptr(gamma),
                                                 ptr(beta), at, at + 4 * scenes * ctx.groups, _ACTIVATIONS[ctx.activation], ptr(dx), ptr(sums),
                                                 ptr(ws), ws.numel(), ptr(_sync(dev, stream)), ptr(device_status(dev)), stream), "wcn_group_norm_backward")
+            count_training_launches("wcn_group_norm_backward")
         return (dx, sums[1].to(weight.dtype) if need_w else None, sums[0].to(bias.dtype) if need_b else None) + (None,) * 4
 
 

@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from ..._native import check, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import _counter, reverse_mode_only
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -64,6 +64,7 @@ def _forward(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor], 
                                   ptr(labels), ignore_index, code, reduction, base, ptr(rows), base + 4 * at_bias if bias is not None else None,
                                   base + 4 * at_count, ptr(loss), ptr(ws), ws.numel(), ptr(_counter(dev, stream)), ptr(device_status(dev)), stream),
               "wcn_linear_ce")
+        count_training_launches("wcn_linear_ce")
     return (loss if reduction else rows), kept, x, weight
 
 
@@ -114,6 +115,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                                                base + 4 * at_count if ctx.reduction == "mean" else None, ptr(grad),
                                                ptr(row_max), ptr(dx), ptr(dw), ptr(db), dtype_code(bias.dtype) if need_b else 0, ptr(ws),
                                                ws.numel(), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear_ce_backward")
+            count_training_launches("wcn_linear_ce_backward")
         return dx, dw, db, None, None, None
 
 

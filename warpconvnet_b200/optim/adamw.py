@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 from torch import Tensor
 
-from .._native import check, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
+from .._native import check, count_training_launches, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
 from ..nn.functional.batch_norm import _counter
 
 BLOCK = 256
@@ -137,6 +137,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Tenso
                                       _bits(betas[0]), _bits(betas[1]), _bits(eps), _bits(weight_decay), lr_at,
                                       _scalar(grad_scale, "grad_scale", device), _scalar(found_inf, "found_inf", device),
                                       ptr(_counter(device, stream)), stream)
+    count_training_launches("wcn_adamw_step")
     if status == _BOUNDS:
         raise ValueError(f"the tensors need more than the {length} elements of the moments or the {steps.numel()} of steps")
     check(status, "wcn_adamw_step")
