@@ -129,11 +129,16 @@ __global__ void __launch_bounds__(THREADS) ce_loss_kernel(const __grid_constant_
     const float more = log_of<T>(sum), lse2 = top + more;
     float loss = 0.f;
     if (counts) {
+      // (a difference of logits, not of one and the log-sum-exp as it is rounded)
       if constexpr (sizeof(T) == 4) {
         loss = (top - dot) + more;
       } else {
-        const float z = p.bias2 ? fmaf(dot, LOG2E, __ldg(&p.bias2[y])) : dot * LOG2E;
-        loss = (lse2 - z) * (float)LN2;
+        // The product is summed in another order than the tile's, and up to 2e-5 beside it: more than the loss of a row that is sure of
+        // its class.  Where all exponentials but the largest come to less than a half, any other class is more than one below the
+        // largest (in units of ln 2): a label that is not is the largest, whose logit is known.
+        float z = p.bias2 ? fmaf(dot, LOG2E, __ldg(&p.bias2[y])) : dot * LOG2E;
+        if (sum < 1.5f && top - z < 0.5f) z = top;
+        loss = ((top - z) + more) * (float)LN2;
       }
       if (loss < 0.f) loss = 0.f;                       // (roundings of a probability of one)
     }

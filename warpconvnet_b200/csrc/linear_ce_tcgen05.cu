@@ -434,14 +434,14 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constan
             s += v.y * exp2f(v.x - by);
             if (v.w != 0.f) z = v.z;
           }
-          const float lse2 = all + log2f(s);
+          const float more = log2f(s);
           float loss = 0.f;
           if (counts) {
-            loss = (lse2 - z) * 0.69314718055994531f;
+            loss = ((all - z) + more) * 0.69314718055994531f;
             if (loss < 0.f) loss = 0.f;                    // (roundings of a probability of one)
           }
           bad |= y != p.q.ignore && !counts;
-          p.out.lse2[row] = lse2;
+          p.out.lse2[row] = all + more;
           p.out.loss_rows[row] = loss;
           total += (double)loss;
           counted += counts;
