@@ -596,7 +596,7 @@ int wcn_batch_norm_backward(const void* x, const void* dy, const void* y, int64_
  * pass; those of empty scenes are not written.
  * backward: dx contiguous (may be NULL), sums [2, channels] = d beta, d gamma (may be NULL).
  * workspace: 16-byte aligned, the bytes that the query gives.  sync: zeroed device memory of the size that its query gives, zero
- * again afterwards (one per stream).  At most 4096 channels and 2^31 - 2^16 rows.  A launch for every 320 scenes that have rows.
+ * again afterwards (one per stream).  At most 4096 channels and 2^31 - 2^16 rows.  A launch for every 1280 scenes that have rows.
  * The reference normalises per row (warpconvnet/nn/modules/normalizations.py) and has segment statistics as torch operations. */
 int wcn_group_norm_workspace_bytes(const int64_t* offsets, int64_t scenes, int32_t channels, int32_t groups, int dtype,
                                    int backward, int64_t* bytes);

@@ -36,9 +36,9 @@ def test_linear_cross_entropy(n, c, v, dtype, bias, forward, backward, of_x):
     assert counted("wcn_linear_ce_backward", lambda: torch.autograd.grad(loss, [x]))[0] == of_x
 
 
-@pytest.mark.parametrize("scenes,launches", [(0, 0), (1, 1), (320, 1), (321, 2), (1000, 4)])
+@pytest.mark.parametrize("scenes,launches", [(0, 0), (1, 1), (1280, 1), (1281, 2), (4000, 4)])
 def test_group_norm(scenes, launches):
-    """A launch for every 320 scenes that have rows."""
+    """A launch for every 1280 scenes that have rows."""
     offsets = [0, 0] + [3 * i for i in range(1, scenes + 1)]
     x = torch.randn(offsets[-1], 8, device=DEV, requires_grad=True)
     launched, y = counted("wcn_group_norm", lambda: segmented_group_norm(x, offsets, 2))
