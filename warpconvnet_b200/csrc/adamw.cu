@@ -93,10 +93,11 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int64_t left,
   }
 }
 
-// m / (sqrt(v) * root + eps), to one part in 2^21 of an update.
+// m / (sqrt(v) * root + eps), to one part in 2^21 of an update.  (Second moments below 2^-126 are numbers: gradients of 1e-18 have
+// such ones, and with an epsilon below them an update as large as any.)
 __device__ __forceinline__ float quotient(float m, float v, float root, float eps) {
   float s, r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(v));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(s, root, eps)));
   return m * r;
 }
