@@ -12,6 +12,7 @@ from torch import Tensor
 from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import _counter, reverse_mode_only
 
+_MOST, _MOST_CHANNELS = 0x7FFFFEFF, 32768   # rows, classes; channels (row numbers of the kernels are 32-bit)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -121,7 +122,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, bias: Optional[Tensor] = None, ignore_index: int = -100,
                          reduction: str = "mean") -> Tensor:
-    """``cross_entropy(x @ weight.T + bias, labels)`` in fp32 without the logits, for any number of classes.
+    """``cross_entropy(x @ weight.T + bias, labels)`` in fp32 without the logits, for any number of classes
+    (below 2^31, as the rows; at most 32 768 channels).
 
     ``x [N, C]`` and ``weight [V, C]`` are float32, float16 or bfloat16 and of one dtype (under autocast they are brought to its
     dtype); ``bias [V]`` may be of any of the three.  ``labels`` are N integers: a row labelled ``ignore_index`` does not count.
@@ -131,6 +133,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, bias: Option
     how = check_reduction(reduction)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or not weight.numel():
         raise ValueError(f"x must be [N, C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if max(x.shape[0], weight.shape[0]) > _MOST or x.shape[1] > _MOST_CHANNELS:
+        raise ValueError(f"at most {_MOST} rows and classes and {_MOST_CHANNELS} channels are taken, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if labels.shape != x.shape[:1] or labels.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"labels must be {x.shape[0]} integers, got {tuple(labels.shape)} {labels.dtype}")
     if bias is not None and bias.shape != weight.shape[:1]:
