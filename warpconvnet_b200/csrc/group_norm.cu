@@ -9,10 +9,10 @@
 // following its first one at a distance of `lag` tiles, so that it finds the rows in L2 while other blocks are at the next
 // scene's first look: HBM sees the rows once (those of scenes that do not fit L2 twice) and no multiprocessor waits between
 // looks.  (A launch a look and group of scenes of 48 MB took 529 us instead of the 869 of many short tiles for 8 x 150 000 rows
-// of 96 channels fp16, forward and backward, of which the launches' starts and ends were half.)  This one takes 150 + 268 us there,
-// 3.1 and 2.6 TB/s of what has to move: neither HBM (30 to 43 %) nor the issue slots (32 to 39 %) are full, the 16 warps that 128
+// of 96 channels fp16, forward and backward, of which the launches' starts and ends were half.)  This one takes 163 + 256 us there,
+// 2.8 and 2.7 TB/s of what has to move: neither HBM (30 to 43 %) nor the issue slots (31 to 40 %) are full, the 16 warps that 128
 // registers leave a multiprocessor wait for an item's loads and its turn.  More warps of fewer registers, other distances between
-// the looks and other tile sizes took as long or longer.  4 x 60 000 rows x 64 channels bf16 with ReLU: 33 + 45 us.
+// the looks and other tile sizes took as long or longer.  4 x 60 000 rows x 64 channels bf16 with ReLU: 31 + 46 us.
 // A thread owns 16 bytes of channels and walks the rows of a tile of its scene; a tile leaves one mean and one sum of squared
 // distances from it per group (backward: two sums, and two per channel); the block that leaves a scene's last tile puts the
 // tiles together, in their order and in double, and raises the scene's flag: the same bits on every run.

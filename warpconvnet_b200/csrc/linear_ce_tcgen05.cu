@@ -13,8 +13,10 @@
 //
 // Measured: logits and sums of 30 000 rows x 256 channels x 32 768 classes bf16 in 388 to 436 us, 1.2 to 1.3 PFLOP/s, where matrix
 // instructions and the power cap bound them; of 60 000 x 128 x 4 096 fp16 in 94 us, 0.67 PFLOP/s, where the exponentials do (the
-// special-function pipe is 73 % busy, the tensor pipe 35 %; a quarter of them as polynomials on the FMA pipe gained 2 %, more lost).  dw of 15 000 x 256 x 16 384 in 105 to 113 us, 1.1 to 1.2 PFLOP/s; with half as
-// many splits, from an estimate by narrower tiles than it had, it took 178.
+// special-function pipe is 73 % busy, the tensor pipe 35 %; a quarter of them as polynomials on the FMA pipe gained 2 %, more lost;
+// the label's logit, row by row or by a comparison of each number, 6 to 8 %: see ce_loss_kernel for how it is had).  dw of 15 000 x
+// 256 x 16 384 in 105 to 113 us, 1.1 to 1.2 PFLOP/s; with half as many splits, from an estimate by narrower tiles than it had, it
+// took 178.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix
 // instructions and frees its tensor memory; what was to come of it is then filled with NaN (linear_ce.cu).
@@ -924,7 +926,7 @@ ce_head_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant_
 // bulk copy leaves in global memory for dw, as it is: [128 rows][64 classes] images.  The (row tile, class tile) pairs are one
 // sequence that is divided evenly among the blocks; where a row tile's classes are several blocks', each leaves its dx apart.
 // As two kernels, the second of which read g again in rows of 128 bytes, 15 000 rows x 6 656 classes x 256 channels bf16 took
-// 85 (g) + 62 us (dx); 15 000 x 16 384 x 256 takes 248 to 283, 0.9 to 1.0 PFLOP/s, with the tensor pipe 46 % busy: a tile's g has one
+// 85 (g) + 62 us (dx); 15 000 x 16 384 x 256 takes 248 to 298, 0.85 to 1.0 PFLOP/s, with the tensor pipe 46 % busy: a tile's g has one
 // place in shared memory, where the products of one tile and the exponentials of the next meet.  (g handed over in halves of 64
 // classes, for more of the two at a time, made the whole call 2 % longer.)
 struct RowsParams {

@@ -128,8 +128,11 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, bias: Option
     ``x [N, C]`` and ``weight [V, C]`` are float32, float16 or bfloat16 and of one dtype (under autocast they are brought to its
     dtype); ``bias [V]`` may be of any of the three.  ``labels`` are N integers: a row labelled ``ignore_index`` does not count.
     A label that names no class counts as one and is reported by ``check_device_status``.  ``reduction``: ``"mean"`` over the rows that
-    count, ``"sum"``, or ``"none"`` for the row losses.  Gradients come in the inputs' dtypes; that of the logits is made and used
-    in pieces of at most 512 MB (in 16 bits rounded to x's dtype, before the factor of the reduction)."""
+    count, ``"sum"``, or ``"none"`` for the row losses.  Gradients come in the inputs' dtypes.  With up to 256 classes and a few
+    hundred channels in 16 bits that of the logits is in no memory; else it is made and used in pieces of at most 512 MB, beside
+    which the sums of a piece take fp32 memory of about two copies of its rows (240 000 rows x 256 channels x 1 000 classes bf16:
+    955 MB in all).  In 16 bits it is rounded to x's dtype before the factor of the reduction, with the rows' weights over the
+    largest of those that count (in fp16 ``x``'s gradient takes them afterwards)."""
     how = check_reduction(reduction)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or not weight.numel():
         raise ValueError(f"x must be [N, C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")

@@ -25,7 +25,7 @@ class BatchNorm(BaseSpatialModule):
 class SegmentedGroupNorm(BaseSpatialModule):
     """Group norm with statistics per scene: over all rows of a scene and the channels of a group, then the activation
     (None, ``"relu"``, ``"silu"`` or ``"gelu"``).  What a scene becomes does not depend on the others of its batch, in training
-    and evaluation alike.  (The reference's ``GroupNorm`` is ``nn.GroupNorm`` of ``[N, C]`` rows: statistics per row.)"""
+    and evaluation alike, but for the last bits: its sums are divided by the size of the whole batch.  (The reference's ``GroupNorm`` is ``nn.GroupNorm`` of ``[N, C]`` rows: statistics per row.)"""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, activation: Optional[str] = None):
         super().__init__()
