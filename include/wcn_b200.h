@@ -609,7 +609,7 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
                             const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
                             int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream);
 
-/* Kernels that this thread's last wcn_group_norm*, wcn_linear_ce* (not the queries) or wcn_adamw_step launched. */
+/* Kernels that this thread's last wcn_group_norm*, wcn_linear_ce* (not the queries), wcn_adamw_step or wcn_rms_norm_backward launched. */
 int wcn_training_launches(void);
 
 /* ------------------------------------------------------------------ cross entropy of a linear layer */
@@ -657,6 +657,32 @@ int wcn_adamw_step(const int64_t* params, const int64_t* grads, const int64_t* s
 /* The numbers that n codes of either moment stand for (n: a multiple of 256). */
 int wcn_adamw_decode(const void* exp_avg, const int16_t* exp_avg_base, const void* exp_avg_sq, const int16_t* exp_avg_sq_base,
                      int64_t n, float* exp_avg_out, float* exp_avg_sq_out, void* stream);
+
+/* ------------------------------------------------------------------ RMS norm, codes of rows, dropout */
+
+/* h = x + residual rounded to dtype (residual NULL: h = x, and the argument h is not used), y = h s weight with
+ * s = 1 / sqrt(mean of a row's h^2 + eps), of [n, channels] rows (x_ld and residual_ld elements apart; h and y contiguous); weight: fp32
+ * [channels] or NULL; eps (the bits of a float): at least 1e-30.  rstd [n] (may be NULL): s, for the backward pass.  In the place of y:
+ * q, e4m3 codes of y / scale, with scale [n] = max(largest |y| of a row / 448, 2^-126); a row with a number that is not finite has NaN.
+ * wcn_quantize_rows: the same of x itself.
+ * backward: dx (contiguous; may be NULL), the gradient of x and of the residual, from that of y and of h (dh; may be NULL); dweight
+ * fp32 [channels] (may be NULL), for which the workspace is (4-byte aligned, the bytes that the query gives).
+ * At most 8192 channels and 2^31 - 257 rows.  The reference normalises with nn.LayerNorm and torch operations
+ * (warpconvnet/nn/modules/normalizations.py). */
+int wcn_rms_norm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t n, int32_t channels, int dtype,
+                 const float* weight, uint32_t eps_bits, void* h, void* y, float* rstd, void* q, float* scale, void* stream);
+int wcn_rms_norm_workspace_bytes(int64_t n, int32_t channels, int64_t* bytes);
+int wcn_rms_norm_backward(const void* h, int64_t h_ld, const void* dy, int64_t dy_ld, const void* dh, int64_t dh_ld, int64_t n,
+                          int32_t channels, int dtype, const float* weight, const float* rstd, void* dx, float* dweight,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int wcn_quantize_rows(const void* x, int64_t x_ld, int64_t n, int32_t channels, int dtype, void* q, float* scale, void* stream);
+
+/* y = residual + keep x 65536 / (65536 - least) of [n, channels] rows (residual may be NULL; y contiguous); the gradient is the same of
+ * dy.  keep: 16 bits of Philox4x32-10 are not below `least`; its key is the seed (*seed_at, device memory, where that is not NULL), its
+ * counter (column / 8, row, row >> 32, 0), the piece column % 8 of the 128 bits, low halves of words first.  What is dropped is 0
+ * whatever it was.  Stands for nn.Dropout. */
+int wcn_dropout(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t n, int32_t channels, int dtype,
+                int32_t least, int64_t seed, const int64_t* seed_at, void* y, void* stream);
 
 /* ------------------------------------------------------------------ self test */
 
