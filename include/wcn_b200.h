@@ -609,7 +609,7 @@ int wcn_group_norm_backward(const void* x, int64_t x_ld, const void* dy, int64_t
                             const float* mean, const float* rstd, int act, void* dx, float* sums, void* workspace,
                             int64_t workspace_bytes, void* sync, int32_t* dev_status, void* stream);
 
-/* Kernels that this thread's last wcn_group_norm*, wcn_linear_ce* (not the queries), wcn_adamw_step or wcn_rms_norm_backward launched. */
+/* Kernels that this thread's last wcn_group_norm*, wcn_linear_ce* (not the queries), wcn_adamw_step, wcn_rms_norm_backward or wcn_linear* (not the query) launched. */
 int wcn_training_launches(void);
 
 /* ------------------------------------------------------------------ cross entropy of a linear layer */
@@ -683,6 +683,28 @@ int wcn_quantize_rows(const void* x, int64_t x_ld, int64_t n, int32_t channels, 
  * whatever it was.  Stands for nn.Dropout. */
 int wcn_dropout(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t n, int32_t channels, int dtype,
                 int32_t least, int64_t seed, const int64_t* seed_at, void* y, void* stream);
+
+/* ------------------------------------------------------------------ linear layers */
+
+/* y = residual + dropout(act(x w^T + bias)), x [n, k], w [m, k], residual (may be NULL), y [n, m] (contiguous) and bias [m] (may be NULL) of
+ * one dtype, fp32 sums, rounded once; act: 0 none, 1 ReLU, 2 SiLU, 3 GELU (of the error function); dropout as wcn_dropout (least 0:
+ * none).  In 16 bits the rows of x and w are 16-byte aligned and their distances multiples of 8, in 8 bits of 16.
+ * wcn_linear_8bit: x and w e4m3 with a scale a row (wcn_quantize_rows), the others of out_dtype (16 bits), no dropout.
+ * backward: gradients of x (contiguous), of w [m, k] and of the bias, each of dtype and each of which may be NULL; the residual's is dy.
+ * Without activation and dropout dy is read as x is and wants the same alignment.
+ * workspace: 32-byte aligned; `what` of the query: the sum of 1 (dx), 2 (dw), 4 (dbias); direct: neither activation nor dropout.
+ * At most 32768 inputs, 2^20 outputs, 2^31 - 257 rows.  The reference has nn.Linear and its neighbours
+ * (warpconvnet/nn/modules/mlp.py). */
+int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype, const void* bias,
+               int act, const void* residual, int64_t residual_ld, int32_t least, int64_t seed, const int64_t* seed_at, void* y,
+               int32_t* dev_status, void* stream);
+int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale, int64_t n, int32_t k, const void* w, int64_t w_ld,
+                    const float* w_scale, int32_t m, int out_dtype, const void* bias, int act, const void* residual,
+                    int64_t residual_ld, void* y, int32_t* dev_status, void* stream);
+int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int32_t direct, int64_t* bytes);
+int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype,
+                        const void* bias, int act, const void* dy, int64_t dy_ld, int32_t least, int64_t seed, const int64_t* seed_at,
+                        void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
 
 /* ------------------------------------------------------------------ self test */
 

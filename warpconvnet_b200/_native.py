@@ -111,6 +111,13 @@ SIGNATURES = {
                               _c_i64, _c_vp],
     "wcn_quantize_rows": [_c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp],
     "wcn_dropout": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_vp, _c_vp, _c_vp],
+    "wcn_linear": [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_i64, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_i32, _c_i64, _c_vp, _c_vp,
+                   _c_vp, _c_vp],
+    "wcn_linear_8bit": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_i64, _c_vp, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_vp, _c_vp,
+                        _c_vp],
+    "wcn_linear_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _p_i64],
+    "wcn_linear_backward": [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_i64, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_i32, _c_i64, _c_vp,
+                            _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp],
     "wcn_selftest_bounded_wait": [_c_i64, _c_vp, _c_vp, _c_vp],
     "wcn_conv_rows_supported": [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp],
     "wcn_conv_rows_fwd": [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp,
@@ -144,7 +151,7 @@ KERNELS_PER_CALL = {
     "wcn_selftest_bounded_wait": 1, "wcn_brick_build": 3, "wcn_kmap_search_bricks": 1,
     "wcn_conv_rows_fwd": 1, "wcn_batch_norm_train": 2, "wcn_column_sums": 2, "wcn_batch_norm_backward": 2, "wcn_conv_pack_weight_from": 1, "wcn_cells_build": 4, "wcn_kmap_search_cells": 1, "wcn_kmap_scan_host": 2, "wcn_unique_counts": 2, "wcn_morton_sort": 1, "wcn_pyramid": 2, "wcn_level_maps": 5,
     "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1, "wcn_linear_ce": 1, "wcn_linear_ce_backward": 1,
-    "wcn_rms_norm": 1, "wcn_rms_norm_backward": 1, "wcn_quantize_rows": 1, "wcn_dropout": 1,
+    "wcn_rms_norm": 1, "wcn_rms_norm_backward": 1, "wcn_quantize_rows": 1, "wcn_dropout": 1, "wcn_linear": 1, "wcn_linear_8bit": 1, "wcn_linear_backward": 1,
 }
 LAUNCH_COUNTS: Counter = Counter()
 
@@ -189,7 +196,7 @@ def count_f32_launches(name: str) -> None:
 
 
 def count_training_launches(name: str) -> None:
-    """The same for group norm, linear cross entropy and AdamW, which launch as many kernels as their sizes ask for."""
+    """The same for group norm, linear cross entropy, AdamW, the gradient of RMS norm and linear layers, which launch as many kernels as their sizes ask for."""
     LAUNCH_COUNTS[name] += lib().wcn_training_launches() - KERNELS_PER_CALL[name]
 
 

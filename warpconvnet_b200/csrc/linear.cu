@@ -1,0 +1,318 @@
+// Linear layers over rows, y = residual + dropout(act(x W^T + bias)) with x [n, k], W [m, k], and their gradients, with z = x W^T + bias:
+//     dz = dropout'(dy) act'(z),   dx = dz W,   dW = dz^T x,   dbias = column sums of dz,   dresidual = dy.
+//
+// z is computed again in the backward pass, not kept: for rows as wide as these a product costs less than writing z and reading it (at
+// 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  dz, rounded to the inputs' type, goes to the
+// workspace, in pieces of rows that stay in L2; each piece is multiplied by W (dx) and by x (dW), whose sums over the rows are divided
+// among the multiprocessors and joined in a fixed order and in double: the same bits on every run.
+//
+// 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 on the
+// FMA pipes here, in tiles of 64 x 64.
+#include "fp32_tile.cuh"
+#include "linear.cuh"
+#include "linear_ce.cuh"
+
+int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st);
+int wcn_ce_product_splits(int m, int n, int k, bool blocked, bool ones);
+int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st);
+
+namespace {
+
+constexpr int THREADS = FP32_THREADS;
+constexpr int MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;
+constexpr int64_t PIECE_BYTES = 64ll << 20;    // of dz
+
+// ------------------------------------------------------------------ fp32
+
+__device__ __forceinline__ float activate(int act, float z) {
+  switch (act) {
+    case WCN_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+    case WCN_ACT_SILU: return z / (1.f + expf(-z));
+    case WCN_ACT_GELU: return z * normcdff(z);
+    default: return z;
+  }
+}
+// dy act'(z)
+__device__ __forceinline__ float through(int act, float dy, float z) {
+  switch (act) {
+    case WCN_ACT_RELU: return z > 0.f ? dy : 0.f;
+    case WCN_ACT_SILU: {
+      const float p = 1.f / (1.f + expf(-z));
+      return dy * (p * (1.f + z * (1.f - p)));
+    }
+    case WCN_ACT_GELU: return dy * (normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z)));
+    default: return dy;
+  }
+}
+
+__device__ __forceinline__ bool kept(const wcn_drop& d, uint64_t seed, int64_t row, int col) {
+  const uint4 w = philox_eight(seed, (uint32_t)col / 8, (uint64_t)row);
+  const int at = col % 8 / 2;
+  const uint32_t word = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
+  return (col & 1 ? word >> 16 : word & 0xFFFFu) >= d.least;
+}
+
+template <int LAYOUT>
+__global__ void __launch_bounds__(THREADS) linear_fp32_kernel(const __grid_constant__ wcn_linear_product q) {
+  const int m_tiles = (q.m + TILE - 1) / TILE;
+  const int m0 = (int)(blockIdx.x % m_tiles) * TILE, n0 = (int)(blockIdx.x / m_tiles) * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float z[4][4], unused[4];
+  fp32_tile<LAYOUT>((const float*)q.a, q.a_ld, (const float*)q.b, q.b_ld, m0, n0, q.m, q.n, 0, q.k, z, unused);
+  const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
+  const float* const add = (const float*)q.add;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m0 + ty * 4 + i;
+    if (row >= q.m) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = n0 + tx * 4 + j;
+      if (col >= q.n) continue;
+      float v = z[i][j];
+      if (q.bias) v += __ldg((const float*)q.bias + col);
+      const bool keep = !q.drop.least || kept(q.drop, seed, q.row0 + row, col);
+      const float by = q.drop.least ? q.drop.scale : 1.f;
+      if (q.grad) {
+        const float g = __ldg(add + row * q.add_ld + col);
+        v = through(q.act, keep ? g * by : 0.f, v);
+      } else {
+        v = activate(q.act, v);
+        v = keep ? v * by : 0.f;
+        if (add) v += __ldg(add + row * q.add_ld + col);
+      }
+      reinterpret_cast<float*>(q.out)[row * q.out_ld + col] = v;
+    }
+  }
+}
+
+int fp32_run(const wcn_linear_product& q, bool by_k, cudaStream_t st) {
+  const int64_t tiles = (int64_t)((q.m + TILE - 1) / TILE) * ((q.n + TILE - 1) / TILE);
+  if (by_k) linear_fp32_kernel<ROWS_BY_CLASSES><<<(unsigned)tiles, THREADS, 0, st>>>(q);
+  else linear_fp32_kernel<LOGITS><<<(unsigned)tiles, THREADS, 0, st>>>(q);
+  ++wcn_launched;
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+// The sums over a part of the rows of dz^T x, and of dz.
+__global__ void __launch_bounds__(THREADS) linear_fp32_weight_kernel(const __grid_constant__ wcn_ce_product q, int per) {
+  const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, split = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float d[4][4], sums[4];
+  fp32_tile<CLASSES_BY_ROWS>((const float*)q.a, q.a_ld, (const float*)q.b, q.b_ld, m0, n0, q.m, q.n, split * per, min((split + 1) * per, q.k), d, sums);
+  const int ld = wcn_ce_round(q.n, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m0 + ty * 4 + i;
+    if (row >= q.m) continue;
+    if (n0 + tx * 4 < ld)
+      *reinterpret_cast<float4*>(q.slab + ((int64_t)split * q.m + row) * ld + n0 + tx * 4) = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
+    if (q.slab_ones && n0 == 0 && tx == 0) q.slab_ones[(int64_t)split * q.m + row] = sums[i];
+  }
+}
+
+int fp32_splits(int m, int n, int k) {
+  const int64_t tiles = (int64_t)((m + TILE - 1) / TILE) * ((n + TILE - 1) / TILE), want = (4 * (int64_t)wcn_num_sms() + tiles - 1) / tiles;
+  const int chains = (k + CHAIN - 1) / CHAIN;
+  const int s = (int)(want < chains ? want : chains), per = (chains + s - 1) / s;
+  return (chains + per - 1) / per;
+}
+
+// ------------------------------------------------------------------ sums of the splits
+
+struct JoinParams {
+  const float* slab;        // [splits][m][ld]
+  const float* ones;        // [splits][m]
+  void* dw;                 // [m][n]; null: not wanted
+  void* db;                 // [m]; null: not wanted
+  int m, n, ld, splits;
+  int quads;                // blocks for dw
+  const int32_t* dev_status;   // null: nothing before this waits (fp32)
+};
+
+constexpr int SIDE = 8;     // threads that share the splits
+template <typename T> __global__ void __launch_bounds__(THREADS) linear_join_kernel(const __grid_constant__ JoinParams p) {
+  __shared__ double part[SIDE][THREADS / SIDE][4];
+  const int side = threadIdx.x / (THREADS / SIDE), at = threadIdx.x % (THREADS / SIDE);
+  const bool of_w = (int)blockIdx.x < p.quads;
+  const int64_t all = of_w ? (int64_t)p.m * (p.ld / 4) : p.m, i = (int64_t)(of_w ? blockIdx.x : blockIdx.x - p.quads) * (THREADS / SIDE) + at;
+  double v[4] = {0, 0, 0, 0};
+  if (i < all) {
+    if (of_w) {
+#pragma unroll 4
+      for (int s = side; s < p.splits; s += SIDE) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(p.slab) + (int64_t)s * all + i);
+        v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+      }
+    } else {
+#pragma unroll 4
+      for (int s = side; s < p.splits; s += SIDE) v[0] += __ldg(&p.ones[(int64_t)s * all + i]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) part[side][at][j] = v[j];
+  __syncthreads();
+  if (side || i >= all) return;
+  for (int s = 1; s < SIDE; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += part[s][at][j];
+  const bool failed = p.dev_status && *p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
+  const float nan = __int_as_float(0x7FC00000);
+  if (!of_w) {
+    reinterpret_cast<T*>(p.db)[i] = wcn_from_float<T>(failed ? nan : (float)v[0]);
+    return;
+  }
+  const int64_t row = i / (p.ld / 4);
+  const int col = (int)(i % (p.ld / 4)) * 4;
+  T* const out = reinterpret_cast<T*>(p.dw) + row * p.n + col;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (col + j < p.n) out[j] = wcn_from_float<T>(failed ? nan : (float)v[j]);
+}
+
+int join(JoinParams p, int dtype, cudaStream_t st) {
+  constexpr int per = THREADS / SIDE;
+  p.quads = p.dw ? (int)(((int64_t)p.m * (p.ld / 4) + per - 1) / per) : 0;
+  const unsigned blocks = (unsigned)(p.quads + (p.db ? (p.m + per - 1) / per : 0));
+  if (dtype == WCN_F32) linear_join_kernel<float><<<blocks, THREADS, 0, st>>>(p);
+  else if (dtype == WCN_F16) linear_join_kernel<__half><<<blocks, THREADS, 0, st>>>(p);
+  else linear_join_kernel<__nv_bfloat16><<<blocks, THREADS, 0, st>>>(p);
+  ++wcn_launched;
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+// ------------------------------------------------------------------ plans
+
+int run(const wcn_linear_product& q, int dtype, bool by_k, int32_t* dev_status, cudaStream_t st) {
+  return dtype == WCN_F32 ? fp32_run(q, by_k, st) : wcn_linear_run(q, dtype, dtype == WCN_BF16, by_k, dev_status, st);
+}
+int weight_splits(int m, int k, int rows, int dtype, bool bias) {
+  return dtype == WCN_F32 ? fp32_splits(m, k, rows) : wcn_ce_product_splits(m, k, rows, false, bias);
+}
+
+// The pieces of rows that dz is made in, and the workspace: dz of a piece, sums of dW and of dbias.
+struct Pieces {
+  int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
+  int64_t dz_ld, slab, ones, bytes;
+};
+enum Want { DX = 1, DW = 2, DB = 4 };
+Pieces plan(int64_t n, int k, int m, int dtype, int what, bool direct) {
+  Pieces p = {};
+  const int64_t e = wcn_dtype_size(dtype);
+  auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
+  p.dz_ld = round(m, 16 / e);
+  // (a gradient that dz is the same as needs no pieces)
+  int64_t rows = direct ? n : PIECE_BYTES / (p.dz_ld * e) / 128 * 128;
+  if (rows < 1024) rows = 1024;
+  const int64_t count = (n + rows - 1) / rows;
+  rows = round((n + count - 1) / count, 128);
+  p.rows = (int)(rows < n ? rows : n);
+  p.count = (int)((n + p.rows - 1) / p.rows);
+  int64_t at = direct ? 0 : round(p.rows * p.dz_ld * e, 128);
+  if (what & (DW | DB)) {
+    const int last = (int)(n - (int64_t)(p.count - 1) * p.rows);
+    p.splits = weight_splits(m, k, p.rows, dtype, what & DB);
+    p.last_splits = weight_splits(m, k, last, dtype, what & DB);
+    const int64_t all = (int64_t)p.splits * (p.count - 1) + p.last_splits;
+    p.slab = at;
+    at += all * m * wcn_ce_round(k, 16) * 4;
+    p.ones = at;
+    if (what & DB) at += round(all * m * 4, 16);
+  }
+  p.bytes = at;
+  return p;
+}
+
+bool sizes_taken(int64_t n, int k, int m) { return n >= 0 && n <= 0x7FFFFEFF && k >= 1 && k <= MOST_INPUTS && m >= 1 && m <= MOST_OUTPUTS; }
+bool rows_taken(const void* p, int64_t ld, int64_t rows, int columns, int size) {
+  const int whole = size == 4 ? 1 : 16 / size;
+  return p && reinterpret_cast<uintptr_t>(p) % (size == 4 ? 4 : 16) == 0 && ld % whole == 0 && (rows <= 1 || ld >= columns);
+}
+
+}  // namespace
+
+extern "C" int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype, const void* bias,
+                          int act, const void* residual, int64_t residual_ld, int32_t least, int64_t seed, const int64_t* seed_at, void* y,
+                          int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
+  if (!sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || act < 0 || act > 3 || least < 0 || least > 65536) return WCN_ERR_INVALID_PARAMETERS;
+  if (n == 0) return WCN_OK;
+  const int size = wcn_dtype_size(dtype);
+  if (!rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !y || !dev_status || (residual && n > 1 && residual_ld < m))
+    return WCN_ERR_INVALID_PARAMETERS;
+  wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, y, m, bias, act, false, residual, residual_ld,
+                          wcn_make_drop((uint32_t)least, seed, seed_at), 0};
+  return run(q, dtype, false, dev_status, wcn_stream(stream));
+}
+
+extern "C" int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale, int64_t n, int32_t k, const void* w, int64_t w_ld,
+                               const float* w_scale, int32_t m, int out_dtype, const void* bias, int act, const void* residual,
+                               int64_t residual_ld, void* y, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
+  if (!sizes_taken(n, k, m) || (out_dtype != WCN_F16 && out_dtype != WCN_BF16) || act < 0 || act > 3) return WCN_ERR_INVALID_PARAMETERS;
+  if (n == 0) return WCN_OK;
+  if (!rows_taken(x, x_ld, n, k, 1) || !rows_taken(w, w_ld, m, k, 1) || !x_scale || !w_scale || !y || !dev_status || (residual && n > 1 && residual_ld < m))
+    return WCN_ERR_INVALID_PARAMETERS;
+  wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, x_scale, w_scale, y, m, bias, act, false, residual, residual_ld, wcn_make_drop(0, 0, nullptr), 0};
+  return wcn_linear_run(q, WCN_E4M3, out_dtype == WCN_BF16, false, dev_status, wcn_stream(stream));
+}
+
+extern "C" int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int32_t direct, int64_t* bytes) {
+  if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 1 || what > 7) return WCN_ERR_INVALID_PARAMETERS;
+  *bytes = plan(n, k, m, dtype, what, direct).bytes;
+  return WCN_OK;
+}
+
+extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype,
+                                   const void* bias, int act, const void* dy, int64_t dy_ld, int32_t least, int64_t seed, const int64_t* seed_at,
+                                   void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+  wcn_launched = 0;
+  if (!sizes_taken(n, k, m) || n == 0 || dtype < WCN_F32 || dtype > WCN_BF16 || act < 0 || act > 3 || least < 0 || least > 65536) return WCN_ERR_INVALID_PARAMETERS;
+  const int size = wcn_dtype_size(dtype), what = (dx ? DX : 0) | (dw ? DW : 0) | (db ? DB : 0);
+  const bool direct = act == WCN_ACT_NONE && least == 0;
+  if (!what || !dev_status || !rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !dy || (n > 1 && dy_ld < m)) return WCN_ERR_INVALID_PARAMETERS;
+  if (direct && !rows_taken(dy, dy_ld, n, m, size)) return WCN_ERR_INVALID_PARAMETERS;
+  const Pieces p = plan(n, k, m, dtype, what, direct);
+  if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes)) return WCN_ERR_INVALID_PARAMETERS;
+  char* const ws = reinterpret_cast<char*>(workspace);
+  cudaStream_t st = wcn_stream(stream);
+  const wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at), none = wcn_make_drop(0, 0, nullptr);
+  const int ld = wcn_ce_round(k, 16);
+  for (int i = 0; i < p.count; ++i) {
+    const int64_t r0 = (int64_t)i * p.rows;
+    const int rows = (int)(n - r0 < p.rows ? n - r0 : p.rows);
+    const char *const xp = (const char*)x + r0 * x_ld * size, *const dyp = (const char*)dy + r0 * dy_ld * size;
+    const void* dz = dyp;
+    int64_t dz_ld = dy_ld;
+    if (!direct) {
+      wcn_linear_product q = {xp, w, x_ld, w_ld, rows, m, k, nullptr, nullptr, ws, p.dz_ld, bias, act, true, dyp, dy_ld, drop, r0};
+      const int rc = run(q, dtype, false, dev_status, st);
+      if (rc != WCN_OK) return rc;
+      dz = ws;
+      dz_ld = p.dz_ld;
+    }
+    if (dx) {
+      wcn_linear_product q = {dz, w, dz_ld, w_ld, rows, k, m, nullptr, nullptr, (char*)dx + r0 * k * size, k, nullptr, WCN_ACT_NONE, false, nullptr, 0, none, 0};
+      const int rc = run(q, dtype, true, dev_status, st);
+      if (rc != WCN_OK) return rc;
+    }
+    if (dw || db) {
+      wcn_ce_product q = {};
+      q.a = dz; q.a_ld = dz_ld; q.b = xp; q.b_ld = x_ld;
+      q.m = m; q.n = k; q.k = rows;
+      q.splits = i + 1 < p.count ? p.splits : p.last_splits;
+      q.slab = (float*)(ws + p.slab) + (int64_t)i * p.splits * m * ld;
+      q.slab_ones = db ? (float*)(ws + p.ones) + (int64_t)i * p.splits * m : nullptr;
+      if (dtype == WCN_F32) {
+        const int chains = (rows + CHAIN - 1) / CHAIN, per = (chains + q.splits - 1) / q.splits * CHAIN;
+        linear_fp32_weight_kernel<<<dim3((m + TILE - 1) / TILE, (k + TILE - 1) / TILE, q.splits), THREADS, 0, st>>>(q, per);
+        ++wcn_launched;
+        if (cudaGetLastError() != cudaSuccess) return WCN_ERR_EXECUTION;
+      } else {
+        const int rc = wcn_ce_product_run(q, true, false, dtype, dev_status, st);
+        if (rc != WCN_OK) return rc;
+      }
+    }
+  }
+  if (!dw && !db) return WCN_OK;
+  return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0,
+               dtype == WCN_F32 ? nullptr : dev_status}, dtype, st);
+}

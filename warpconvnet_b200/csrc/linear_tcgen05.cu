@@ -1,0 +1,586 @@
+// Linear layers in 16 and 8 bits on the tensor cores: out = add + dropout(act(A B^T + bias)), and what their gradients need of the
+// same form (see linear.cuh).
+//
+// Persistent blocks work through tiles of 128 rows x NT columns (up to 256): one thread issues TMA tile loads into a ring, one the
+// matrix instructions (fp32 accumulators in tensor memory, as many tiles as fit), sixteen warps empty them.  Each of those takes 32 rows x 32
+// columns at a time, in turns over the tile's columns and over tiles: bias, activation, dropout and the addition are made in
+// registers in fp32 and the sum is rounded once.  What is added (the residual, or the gradient that arrives) comes by TMA into the warp's
+// own 2 KB of shared memory, one piece ahead, and the result leaves from the same place by TMA: rows of 64 bytes per thread
+// would cost the load/store pipe a line each.  Rows that TMA cannot take (pitches that are no multiple of 16 bytes) go the same way
+// through shared memory and from there in elements.
+// Where they fit beside a ring of four tiles, the columns' rows of B stay in shared memory (RESIDENT): a block then has one group of
+// columns, and A alone passes.
+//
+// Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
+// and frees its tensor memory; its results, and those of a launch that finds the word set, are NaN.
+#include "linear.cuh"
+#include "tcgen05_common.cuh"
+#include "tma_common.cuh"
+
+namespace {
+
+constexpr int TILE_M = 128, SLICE_BYTES = 128;             // rows of a tile; bytes of k of a stage
+constexpr int A_BYTES = TILE_M * SLICE_BYTES;
+constexpr int MN_CHUNK = 64 * 128;                         // 64 of k x 64 columns of a B whose columns run along its rows
+constexpr int MAX_STAGES = 12, MAX_ACC = 4;
+constexpr int EPI_WARP0 = 2, PARTS = 4, EPI_WARPS = 4 * PARTS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+constexpr int PIECE = 32, PIECE_BYTES = 32 * PIECE * 2;    // columns of a warp's piece; its 32 rows in shared memory
+constexpr int SMEM_BUDGET = 224 * 1024;
+
+struct Params {
+  wcn_linear_product q;
+  int KB, NT;               // slices of k; columns of a tile (a multiple of 32)
+  int m_tiles, n_tiles, stages, accs, tmem_cols;
+  int b_slice;              // bytes of a slice of B
+  int out_tma, add_tma;
+  int32_t* dev_status;
+};
+
+struct Ring {
+  int slot, phase, depth;
+  __device__ __forceinline__ void advance() {
+    if (++slot == depth) { slot = 0; phase ^= 1; }
+  }
+};
+
+struct Control {
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t b_full;
+  uint64_t acc_full[MAX_ACC], acc_empty[MAX_ACC];
+  uint64_t add_full[EPI_WARPS][2];
+  uint64_t done;
+  uint32_t tmem_holder;
+  int32_t skip;
+  __align__(16) float bias[EPI_WARPS][PIECE], scale[EPI_WARPS][PIECE];   // of a warp's piece
+};
+
+__device__ __forceinline__ uint32_t bar(uint64_t* b) { return smem_u32(b); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+
+// ------------------------------------------------------------------ activations, two numbers at a time
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The larger and the smaller of two numbers; what is no number stays so.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// Normal distribution's function at -u, 0 <= u <= 7, as an exponential of a polynomial: log2 of it is a smooth curve near a parabola,
+// fitted by least largest error (degree 8): within 8e-6 of the value everywhere, an eightieth of half a step of 16-bit results at
+// least.  The error function of the library takes three times the instructions of the pipes that bound this kernel.
+constexpr float GELU_END = 7.f;   // behind which the function, 1e-12, is taken as what it is there
+__device__ __forceinline__ float2 normal_tail(float2 u) {
+  float2 p = both(5.216057985535372e-08f);
+  p = __ffma2_rn(p, u, both(-3.0775302093388746e-06f));
+  p = __ffma2_rn(p, u, both(7.351476233452559e-05f));
+  p = __ffma2_rn(p, u, both(-0.0009893535170704126f));
+  p = __ffma2_rn(p, u, both(0.00866654422134161f));
+  p = __ffma2_rn(p, u, both(-0.05418838933110237f));
+  p = __ffma2_rn(p, u, both(-0.45830658078193665f));
+  p = __ffma2_rn(p, u, both(-1.1512914896011353f));
+  p = __ffma2_rn(p, u, both(-0.9999936819076538f));
+  return make_float2(exp2_fast(p.x), exp2_fast(p.y));
+}
+__device__ __forceinline__ float2 logistic(float2 z) {
+  const float2 e = __fmul2_rn(z, both(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(both(1.f), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+  return make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+}
+
+template <int ACT> __device__ __forceinline__ float2 activate(float2 z) {
+  if (ACT == WCN_ACT_RELU) return make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f));
+  if (ACT == WCN_ACT_SILU) return __fmul2_rn(z, logistic(z));
+  if (ACT == WCN_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const float2 u = make_float2(min_nan(fabsf(z.x), GELU_END), min_nan(fabsf(z.y), GELU_END));
+    return __ffma2_rn(make_float2(-u.x, -u.y), normal_tail(u), make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
+  }
+  return z;
+}
+// dy act'(z)
+template <int ACT> __device__ __forceinline__ float2 through(float2 dy, float2 z) {
+  if (ACT == WCN_ACT_RELU) return make_float2(z.x > 0.f ? dy.x : 0.f, z.y > 0.f ? dy.y : 0.f);
+  if (ACT == WCN_ACT_SILU) {
+    const float2 p = logistic(z), q = __ffma2_rn(p, both(-1.f), both(1.f));
+    return __fmul2_rn(dy, __fmul2_rn(p, __ffma2_rn(z, q, both(1.f))));
+  }
+  if (ACT == WCN_ACT_GELU) {   // Phi(z) + z phi(z)
+    const float2 u = make_float2(min_nan(fabsf(z.x), GELU_END), min_nan(fabsf(z.y), GELU_END));
+    const float2 e = __ffma2_rn(__fmul2_rn(u, u), both(-0.72134752044448170f), both(-1.3257480647361595f));
+    const float2 t = __ffma2_rn(make_float2(-u.x, -u.y), make_float2(exp2_fast(e.x), exp2_fast(e.y)), normal_tail(u));   // of -|z|
+    return __fmul2_rn(dy, make_float2(z.x > 0.f ? 1.f - t.x : t.x, z.y > 0.f ? 1.f - t.y : t.y));
+  }
+  return dy;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float2 v) {
+  if (BF16) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16> __device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <bool BF16> __device__ __forceinline__ float number(uint16_t v) {
+  return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+}
+
+// A piece's numbers of one row: v = A B^T + bias on entry, the result's on exit; add: 32 numbers in 16 bits.
+template <int ACT, bool BF16> __device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[16], const uint4 (&add)[4], int64_t row, int col) {
+  const uint32_t* const a = reinterpret_cast<const uint32_t*>(add);
+  if (q.grad) {
+    float2 g[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = unpack2<BF16>(a[4 * b + i]);
+      if (q.drop.least) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, reinterpret_cast<float*>(g));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * b + i] = through<ACT>(g[i], v[4 * b + i]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * b + i] = activate<ACT>(v[4 * b + i]);
+    if (q.drop.least) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, reinterpret_cast<float*>(&v[4 * b]));
+    if (q.add)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * b + i] = __fadd2_rn(v[4 * b + i], unpack2<BF16>(a[4 * b + i]));
+  }
+}
+
+// The tiles of a block.  RESIDENT: one group of columns, every `step`-th tile of rows; else tiles in order, columns fastest.
+struct Tiles {
+  int m, n, step, i, m_tiles, n_tiles;
+  bool resident;
+  __device__ __forceinline__ bool there() const { return m < m_tiles; }
+  __device__ __forceinline__ void advance() {
+    if (resident) { m += step; return; }
+    i += (int)gridDim.x;
+    m = i / n_tiles;
+    n = i - m * n_tiles;
+  }
+};
+template <bool RESIDENT> __device__ __forceinline__ Tiles first_tile(const Params& p) {
+  Tiles t;
+  t.m_tiles = p.m_tiles; t.n_tiles = p.n_tiles; t.resident = RESIDENT; t.step = 0; t.i = blockIdx.x;
+  if (RESIDENT) {
+    t.n = blockIdx.x % p.n_tiles;
+    t.m = blockIdx.x / p.n_tiles;
+    t.step = ((int)gridDim.x - t.n + p.n_tiles - 1) / p.n_tiles;   // blocks of this group
+  } else {
+    t.m = t.i / p.n_tiles;
+    t.n = t.i - t.m * p.n_tiles;
+  }
+  return t;
+}
+
+// KIND: operands f16, bf16 or e4m3.  B_MN: the columns of the result run along B's rows.
+template <int KIND, bool B_MN, bool RESIDENT, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap out_map,
+              const __grid_constant__ CUtensorMap add_map, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int DEPTH = KIND == WCN_E4M3 ? 128 : 64;       // elements of k of a slice
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stage_bytes = RESIDENT ? A_BYTES : A_BYTES + p.b_slice;
+  const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
+  const uint32_t base = smem_u32(smem_raw) + pad;
+  const uint32_t res = base + (uint32_t)(p.stages * stage_bytes), staging = res + (RESIDENT ? (uint32_t)(p.KB * p.b_slice) : 0u);
+  uint8_t* const staging_at = smem_raw + (staging - smem_u32(smem_raw));
+  Control* const ctl = reinterpret_cast<Control*>(staging_at + EPI_WARPS * 2 * PIECE_BYTES);
+  const wcn_linear_product& q = p.q;
+  uint16_t* const out = reinterpret_cast<uint16_t*>(q.out);
+  auto mark = [&]() {
+    const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
+    for (Tiles t = first_tile<RESIDENT>(p); t.there(); t.advance())
+      for (int i = threadIdx.x; i < TILE_M * p.NT; i += THREADS) {
+        const int row = t.m * TILE_M + i / p.NT, col = t.n * p.NT + i % p.NT;
+        if (row < q.m && col < q.n) out[(int64_t)row * q.out_ld + col] = nan;
+      }
+  };
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) { mark(); return; }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) { mbar_init(bar(&ctl->full[s]), 1); mbar_init(bar(&ctl->empty[s]), 1); }
+    mbar_init(bar(&ctl->b_full), 1);
+    for (int i = 0; i < p.accs; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)(4 * (p.NT / PIECE))); }
+    for (int w = 0; w < EPI_WARPS; ++w)
+      for (int i = 0; i < 2; ++i) mbar_init(bar(&ctl->add_full[w][i]), 1);
+    mbar_init(bar(&ctl->done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_holder;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      Ring r{0, 0, p.stages};
+      int issued = 0;
+      auto load_b = [&](uint32_t to, int s, int n, uint32_t full) {
+        if (B_MN) {
+          for (int c = 0; c * MN_CHUNK < p.b_slice; ++c) tma_load_2d(to + (uint32_t)(c * MN_CHUNK), &b_map, n * p.NT + 64 * c, s * DEPTH, full);
+        } else {
+          tma_load_2d(to, &b_map, s * DEPTH, n * p.NT, full);
+        }
+      };
+      Tiles t = first_tile<RESIDENT>(p);
+      const bool any = t.there();
+      if (RESIDENT && any) {
+        mbar_expect_tx(bar(&ctl->b_full), (uint32_t)(p.KB * p.b_slice));
+        for (int s = 0; s < p.KB; ++s) load_b(res + (uint32_t)(s * p.b_slice), s, t.n, bar(&ctl->b_full));
+      }
+      for (; t.there() && ok; t.advance())
+        for (int s = 0; s < p.KB; ++s) {
+          if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
+          const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
+          mbar_expect_tx(full, (uint32_t)stage_bytes);
+          tma_load_2d(at, &a_map, s * DEPTH, t.m * TILE_M, full);
+          if (!RESIDENT) load_b(at + A_BYTES, s, t.n, full);
+          r.advance();
+          ++issued;
+        }
+      if (!ok) {   // what has been issued lands before the block's shared memory is given back
+        for (int i = 0; i < issued && i < r.depth; ++i) {
+          if (--r.slot < 0) { r.slot = r.depth - 1; r.phase ^= 1; }
+          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->full[r.slot]), (uint32_t)r.phase); ++k) {}
+        }
+        for (int k = 0; RESIDENT && any && k < 100000 && !mbar_try_wait(bar(&ctl->b_full), 0); ++k) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t type = KIND == WCN_BF16 ? 1u : 0u;   // (f16 and e4m3: 0 of their kinds)
+      const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (B_MN ? 1u << 16 : 0u) | ((uint32_t)(p.NT >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+      constexpr int B_STEP = B_MN ? 128 : 2;                  // an instruction's depth further, in units of 16 bytes
+      auto describe_b = [&](uint32_t at) { return B_MN ? smem_desc_mn<128>(at, MN_CHUNK) : smem_desc<128>(at); };
+      const uint64_t a0 = smem_desc<128>(base), b0 = describe_b(RESIDENT ? res : base + A_BYTES);
+      Ring r{0, 0, p.stages};
+      int ab = 0, aphase = 0;
+      Tiles t = first_tile<RESIDENT>(p);
+      if (RESIDENT && t.there()) ok = mbar_wait(bar(&ctl->b_full), 0, p.dev_status);
+      for (; ok && t.there(); t.advance()) {
+        if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(ab * p.NT);
+        for (int s = 0; s < p.KB; ++s) {
+          if (!mbar_wait(bar(&ctl->full[r.slot]), r.phase, p.dev_status)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t slot = (uint64_t)((r.slot * stage_bytes) >> 4);
+          const uint64_t a = a0 + slot, b = b0 + (RESIDENT ? (uint64_t)((s * p.b_slice) >> 4) : slot);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (KIND == WCN_E4M3) umma_f8(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
+            else umma_f16(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
+          }
+          umma_commit(bar(&ctl->empty[r.slot]));
+          r.advance();
+        }
+        if (!ok) break;
+        umma_commit(bar(&ctl->acc_full[ab]));
+        if (++ab == p.accs) { ab = 0; aphase ^= 1; }
+      }
+      umma_commit(bar(&ctl->done));
+      (void)mbar_wait(bar(&ctl->done), 0, p.dev_status);
+    }
+    __syncwarp();
+  } else {
+    // Pieces of the block's tiles are numbered through, columns fastest; a warp has every fourth.  It has then seen the accumulator
+    // before the one that it waits for filled (of tiles of 32, 64 .. columns there are 4, 4 .. accumulators), as waits by parity want.
+    const int ew = warp - EPI_WARP0, quarter = warp & 3, part = ew >> 2, pieces = p.NT / PIECE;
+    const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
+    uint8_t* const mine = staging_at + ew * 2 * PIECE_BYTES;
+    const uint32_t mine_at = staging + (uint32_t)(ew * 2 * PIECE_BYTES);
+    float* const bias = ctl->bias[ew];
+    float* const scale = ctl->scale[ew];
+    struct Place { Tiles t; int tile, piece; };
+    auto next = [&](Place& w, int by) {
+      w.piece += by;
+      while (w.piece >= pieces) { w.piece -= pieces; ++w.tile; w.t.advance(); }
+    };
+    auto wanted = [&](const Place& w) { return w.t.m * TILE_M + quarter * 32 < q.m && w.t.n * p.NT + w.piece * PIECE < q.n; };
+    auto request = [&](const Place& w, int buffer) {   // one lane
+      const uint32_t full = bar(&ctl->add_full[ew][buffer]);
+      mbar_expect_tx(full, PIECE_BYTES);
+      tma_load_2d(mine_at + (uint32_t)(buffer * PIECE_BYTES), &add_map, w.t.n * p.NT + w.piece * PIECE, w.t.m * TILE_M + quarter * 32, full);
+    };
+    const bool by_tma = q.add && p.add_tma;
+    Place now{first_tile<RESIDENT>(p), 0, 0};
+    next(now, part);
+    int turn = 0, loads[2] = {0, 0}, waits[2] = {0, 0};   // pieces with a place in shared memory; copies into each of the two
+    if (by_tma && now.t.there() && wanted(now)) {
+      if (lane == 0) request(now, 0);
+      ++loads[0];
+    }
+    while (now.t.there()) {
+      Place then = now;
+      next(then, PARTS);
+      const int ab = now.tile % p.accs, aphase = now.tile / p.accs & 1;
+      const bool use = wanted(now);
+      const int col = now.t.n * p.NT + now.piece * PIECE, row = now.t.m * TILE_M + quarter * 32 + lane, b = turn & 1;
+      if (use) {
+        const bool there = col + lane < q.n;
+        bias[lane] = q.bias && there ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[col + lane]) : 0.f;
+        if (KIND == WCN_E4M3) scale[lane] = there ? __ldg(&q.b_scale[col + lane]) : 0.f;
+      }
+      const float row_scale = KIND == WCN_E4M3 && use && row < q.m ? __ldg(&q.a_scale[row]) : 0.f;
+      // Places are free once the piece of two turns ago has been read from this one, and, where the next piece's copy goes into the
+      // other one, the last piece from there.
+      if (lane == 0) {
+        if (by_tma) store_wait_read<0>();
+        else store_wait_read<1>();
+      }
+      __syncwarp();
+      if (by_tma && then.t.there() && wanted(then)) {
+        const int other = use ? b ^ 1 : b;
+        if (lane == 0) request(then, other);
+        ++loads[other];
+      }
+      uint4 add[4];
+      uint8_t* const at = mine + b * PIECE_BYTES;
+      auto chunk = [&](int line, int c) { return reinterpret_cast<uint4*>(at + line * 64 + ((c ^ (line >> 1 & 3)) << 4)); };
+      auto element = [&](int line, int c) { return reinterpret_cast<uint16_t*>(chunk(line, c >> 3)) + (c & 7); };
+      if (use && q.add) {
+        if (by_tma) {
+          if (ok) ok = mbar_wait(bar(&ctl->add_full[ew][b]), waits[b] & 1, p.dev_status);
+          if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+          ++waits[b];
+        } else {
+          for (int l = 0; l < 32; ++l) {
+            const int64_t from = (int64_t)(row - lane + l) * q.add_ld + col + lane;
+            *element(l, lane) = row - lane + l < q.m && col + lane < q.n ? reinterpret_cast<const uint16_t*>(q.add)[from] : (uint16_t)0;
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) add[c] = *chunk(lane, c);
+      }
+      if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t r[32];
+      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.NT + now.piece * PIECE), r);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[ab]));
+      if (use) {
+        float2 v[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 t = reinterpret_cast<const float4*>(bias)[i];
+          v[2 * i] = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]));
+          v[2 * i + 1] = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+          if (KIND == WCN_E4M3) {
+            const float4 s = reinterpret_cast<const float4*>(scale)[i];
+            v[2 * i] = __ffma2_rn(__fmul2_rn(v[2 * i], both(row_scale)), make_float2(s.x, s.y), make_float2(t.x, t.y));
+            v[2 * i + 1] = __ffma2_rn(__fmul2_rn(v[2 * i + 1], both(row_scale)), make_float2(s.z, s.w), make_float2(t.z, t.w));
+          } else {
+            v[2 * i] = __fadd2_rn(v[2 * i], make_float2(t.x, t.y));
+            v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(t.z, t.w));
+          }
+        }
+        const int64_t place = q.row0 + row;
+        switch (q.act) {
+          case WCN_ACT_RELU: finish<WCN_ACT_RELU, BF16>(q, seed, v, add, place, col); break;
+          case WCN_ACT_SILU: finish<WCN_ACT_SILU, BF16>(q, seed, v, add, place, col); break;
+          case WCN_ACT_GELU: finish<WCN_ACT_GELU, BF16>(q, seed, v, add, place, col); break;
+          default: finish<WCN_ACT_NONE, BF16>(q, seed, v, add, place, col); break;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *chunk(lane, c) = make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3]));
+        if (p.out_tma) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&out_map, col, row - lane, mine_at + (uint32_t)(b * PIECE_BYTES));
+            store_commit();
+          }
+        } else {
+          __syncwarp();
+          for (int l = 0; l < 32; ++l)
+            if (row - lane + l < q.m && col + lane < q.n) out[(int64_t)(row - lane + l) * q.out_ld + col + lane] = *element(l, lane);
+          __syncwarp();
+        }
+        ++turn;
+      }
+      now = then;
+    }
+    // what is still on its way to or from this warp's places
+    for (int b = 0; b < 2; ++b)
+      for (int k = 0; waits[b] < loads[b] && k < 100000 && !mbar_try_wait(bar(&ctl->add_full[ew][b]), (uint32_t)(waits[b] & 1)); ++k) {}
+    if (lane == 0) store_wait_read<0>();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+  __syncthreads();
+  if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (results on their way are written before what replaces them)
+    __syncthreads();
+    mark();
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+template <auto KERNEL> bool allow_smem() {
+  static bool configured[64] = {};   // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    configured[dev] = true;
+  }
+  return true;
+}
+
+// A row-major matrix of `size`-byte elements read or written in boxes of cols x rows, swizzled over their row's bytes (64 or 128).
+bool box_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
+  EncodeTiledFn encode = encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t step[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                box_cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tma_rows(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
+
+constexpr int FIXED = 1024 + EPI_WARPS * 2 * PIECE_BYTES + (int)sizeof(Control) + 64;
+
+// Columns of a tile, and whether B's stay in shared memory.
+bool plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
+  const int depth = kind == WCN_E4M3 ? 128 : 64, sms = wcn_num_sms();
+  p->KB = (q.k + depth - 1) / depth;
+  p->m_tiles = (q.m + TILE_M - 1) / TILE_M;
+  auto slice = [&](int nt) { return b_mn ? (nt + 63) / 64 * MN_CHUNK : nt * SLICE_BYTES; };
+  auto tiles_of = [&](int nt) { return (q.n + nt - 1) / nt; };
+  auto even = [&](int most) {   // columns of a tile when as few as can be of `most` at the most share them
+    const int tiles = tiles_of(most);
+    return ((q.n + tiles - 1) / tiles + PIECE - 1) / PIECE * PIECE;
+  };
+  bool resident = false;
+  int nt = even(256);
+  for (int most = 256; most >= 128 && !resident; most -= 64) {
+    const int t = even(most);
+    if ((int64_t)p->KB * slice(t) + 4 * A_BYTES + FIXED <= SMEM_BUDGET && tiles_of(t) * 4 <= sms) { resident = true; nt = t; }
+  }
+  // few tiles: narrower ones, for as many multiprocessors
+  while (nt > PIECE && (int64_t)p->m_tiles * tiles_of(nt) * 2 <= sms) nt = even((nt / 2 + PIECE - 1) / PIECE * PIECE);
+  if (!resident || tiles_of(nt) * 4 > sms) resident = (int64_t)p->KB * slice(nt) + 4 * A_BYTES + FIXED <= SMEM_BUDGET && (int64_t)p->m_tiles * tiles_of(nt) <= sms;
+  p->NT = nt;
+  p->n_tiles = tiles_of(nt);
+  p->b_slice = slice(nt);
+  p->accs = 512 / nt < MAX_ACC ? 512 / nt : MAX_ACC;
+  p->tmem_cols = 32;
+  while (p->tmem_cols < p->accs * nt) p->tmem_cols *= 2;
+  return resident;
+}
+
+template <int KIND, bool B_MN, bool RESIDENT, bool BF16> int launch(Params& p, cudaStream_t st) {
+  const wcn_linear_product& q = p.q;
+  constexpr int size = KIND == WCN_E4M3 ? 1 : 2, depth = SLICE_BYTES / size;
+  constexpr CUtensorMapDataType wide = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  constexpr CUtensorMapDataType type = KIND == WCN_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : wide;
+  const int stage = RESIDENT ? A_BYTES : A_BYTES + p.b_slice, kept = RESIDENT ? p.KB * p.b_slice : 0;
+  p.stages = (SMEM_BUDGET - FIXED - kept) / stage;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (p.stages < 2) return WCN_ERR_UNSUPPORTED_CONFIG;
+  CUtensorMap a, b, out, add;
+  bool ok = box_map(&a, type, size, q.a, q.m, q.k, q.a_ld, depth, TILE_M);
+  ok = ok && (B_MN ? box_map(&b, type, size, q.b, q.k, q.n, q.b_ld, 64, 64) : box_map(&b, type, size, q.b, q.n, q.k, q.b_ld, depth, p.NT));
+  out = add = a;   // (not used where they are not made)
+  if (p.out_tma) ok = ok && box_map(&out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
+  if (q.add && p.add_tma) ok = ok && box_map(&add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
+  if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = linear_kernel<KIND, B_MN, RESIDENT, BF16>;
+  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
+  const int sms = wcn_num_sms();
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  kern<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, (size_t)FIXED + kept + (size_t)p.stages * stage, st>>>(a, b, out, add, p);
+  ++wcn_launched;
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+}
+
+template <int KIND, bool B_MN, bool BF16> int by_plan(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
+  Params p = {};
+  p.q = q;
+  p.dev_status = dev_status;
+  p.out_tma = tma_rows(q.out, q.out_ld, 2);
+  p.add_tma = q.add && tma_rows(q.add, q.add_ld, 2);
+  return plan(q, KIND, B_MN, &p) ? launch<KIND, B_MN, true, BF16>(p, st) : launch<KIND, B_MN, false, BF16>(p, st);
+}
+
+}  // namespace
+
+// kind: WCN_F16, WCN_BF16 (the type of all) or WCN_E4M3 (of A and B; `bf16`: the others').  by_k: B is [k][n].  Rows of A and B start
+// on 16-byte boundaries.
+int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st) {
+  const int size = kind == WCN_E4M3 ? 1 : 2;
+  if (!tma_rows(q.a, q.a_ld, size) || !tma_rows(q.b, q.b_ld, size)) return WCN_ERR_INVALID_PARAMETERS;
+  if (kind == WCN_E4M3) return bf16 ? by_plan<WCN_E4M3, false, true>(q, dev_status, st) : by_plan<WCN_E4M3, false, false>(q, dev_status, st);
+  if (kind == WCN_BF16) return by_k ? by_plan<WCN_BF16, true, true>(q, dev_status, st) : by_plan<WCN_BF16, false, true>(q, dev_status, st);
+  return by_k ? by_plan<WCN_F16, true, false>(q, dev_status, st) : by_plan<WCN_F16, false, false>(q, dev_status, st);
+}

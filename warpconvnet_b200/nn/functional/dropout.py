@@ -53,7 +53,7 @@ def kept_factor(seed: Union[int, Tensor], n: int, c: int, least: int, device: to
         a, b, d, e = ((v >> 32) & _WORD) ^ b ^ k0, v & _WORD, ((u >> 32) & _WORD) ^ e ^ k1, u & _WORD
         k0, k1 = (k0 + 0x9E3779B9) & _WORD, (k1 + 0xBB67AE85) & _WORD
     words = torch.stack([a, b, d, e], dim=2)
-    bits = torch.stack([words & 0xFFFF, words >> 16], dim=3).view(n, -1)[:, :c]
+    bits = torch.stack([words & 0xFFFF, words >> 16], dim=3).view(n, 8 * a.shape[1])[:, :c]
     return torch.where(bits >= least, 65536 / max(1, 65536 - least), 0.0).float()
 
 

@@ -1,0 +1,184 @@
+"""Linear layers over feature rows with bias, activation, dropout and residual in one native kernel (``csrc/linear.cu``), in fp32, 16
+bits and, for inference, of operands in 8 bits.
+
+An addition to the reference, whose ``Linear`` and MLP blocks (warpconvnet/nn/modules/mlp.py) run torch's layers one after the other."""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+from torch import Tensor
+
+from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from .batch_norm import reverse_mode_only
+from .dropout import check_probability, check_seed, kept_factor, new_seed
+from .group_norm import _ACTIVATIONS, _rows, check_activation
+from .linear_cross_entropy import _matrix
+from .rms_norm import E4M3, check_residual, no_gradient
+
+_MOST, _MOST_INPUTS, _MOST_OUTPUTS = 0x7FFFFEFF, 32768, 1 << 20
+
+
+def _check_shapes(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or not weight.numel():
+        raise ValueError(f"x must be [N, K] and weight [M, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.shape[0] > _MOST or x.shape[1] > _MOST_INPUTS or weight.shape[0] > _MOST_OUTPUTS:
+        raise ValueError(f"at most {_MOST} rows, {_MOST_INPUTS} inputs and {_MOST_OUTPUTS} outputs are taken, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    require_cuda(x, "x")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if any(t.device != x.device for t in (weight,) + (() if bias is None else (bias,))):
+        raise ValueError(f"all tensors must be on {x.device}")
+
+
+def _seed_arguments(seed: Union[int, Tensor]):
+    return (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
+
+
+def _forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: int, residual: Optional[Tensor], least: int, seed):
+    """(y, the matrices as the kernels read them)"""
+    (n, k), m, dev = x.shape, weight.shape[0], x.device
+    x, x_ld = _matrix(x)
+    weight, w_ld = _matrix(weight)
+    y = torch.empty((n, m), dtype=x.dtype, device=dev)
+    res_ld = 0
+    if residual is not None:
+        residual, res_ld = _rows(residual)
+    number, at = _seed_arguments(seed)
+    with on_device(dev):
+        check(lib().wcn_linear(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, dtype_code(x.dtype), ptr(bias), act, ptr(residual), res_ld, least, number, at,
+                               ptr(y), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear")
+        count_training_launches("wcn_linear")
+    return y, x, weight
+
+
+def formula(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], residual: Optional[Tensor], least: int, seed) -> Tensor:
+    """The same through torch: for a graph of the gradient, forward-mode differentiation and function transforms."""
+    with torch.autocast("cuda", enabled=False):
+        z = x.float() @ weight.float().t()
+    z = z if bias is None else z + bias.float()
+    y = {None: lambda t: t, "relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}[activation](z)
+    if least:
+        factor = kept_factor(seed, *z.shape, least, z.device)
+        y = torch.where(factor > 0, y * factor, 0.0)
+    return (y if residual is None else y + residual.float()).to(x.dtype)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: Optional[str], least: int, seed):
+        y, x_rows, w_rows = _forward(x.detach(), weight.detach(), None if bias is None else bias.detach().contiguous(), _ACTIVATIONS[activation],
+                                     None if residual is None else residual.detach(), least, seed)
+        ctx.activation, ctx.least, ctx.seed = activation, least, None if isinstance(seed, Tensor) else seed
+        # (matrices that had to be copied are kept with them: there are not two copies to be made)
+        copied = tuple(None if rows.data_ptr() == given.data_ptr() else rows for rows, given in ((x_rows, x), (w_rows, weight)))
+        ctx.save_for_backward(x, weight, bias, seed if isinstance(seed, Tensor) else None, *copied)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy: Tensor):
+        x, weight, bias, seed, x_rows, w_rows = ctx.saved_tensors
+        seed = ctx.seed if seed is None else seed
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        d_residual = dy if need_r else None
+        if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+            y = formula(x, weight, bias, ctx.activation, None, ctx.least, seed)
+            wanted = [t for t, need in zip((x, weight, bias), (need_x, need_w, need_b)) if need]
+            got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True) if wanted else ())
+            return tuple(next(got) if need else None for need in (need_x, need_w, need_b)) + (d_residual, None, None, None)
+        if not (need_x or need_w or need_b):
+            return None, None, None, d_residual, None, None, None
+        (n, k), m, dev = x.shape, weight.shape[0], x.device
+        code, act = dtype_code(x.dtype), _ACTIVATIONS[ctx.activation]
+        dx = torch.empty((n, k), dtype=x.dtype, device=dev) if need_x else None
+        dw = torch.empty((m, k), dtype=x.dtype, device=dev) if need_w else None
+        db = torch.empty(m, dtype=x.dtype, device=dev) if need_b else None
+        direct = not act and not ctx.least
+        dy, dy_ld = _matrix(dy) if direct else _rows(dy)
+        x, x_ld = _matrix(x if x_rows is None else x_rows, k)
+        weight, w_ld = _matrix(weight if w_rows is None else w_rows, k)
+        bias = None if bias is None else bias.contiguous()
+        number, at = _seed_arguments(seed)
+        ws = torch.empty(query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, int(direct)), dtype=torch.uint8, device=dev)
+        with on_device(dev):
+            check(lib().wcn_linear_backward(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, code, ptr(bias), act, ptr(dy), dy_ld, ctx.least, number, at,
+                                            ptr(dx), ptr(dw), ptr(db), ptr(ws), ws.numel(), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear_backward")
+            count_training_launches("wcn_linear_backward")
+        return dx, dw, db, d_residual, None, None, None
+
+
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, residual: Optional[Tensor] = None,
+           dropout_p: float = 0.0, seed: Union[int, Tensor, None] = None) -> Tensor:
+    """``residual + dropout(act(x @ weight.T + bias))`` of ``x [N, K]`` and ``weight [M, K]``, summed in fp32 and rounded once.
+
+    All tensors are of one dtype, float32, float16 or bfloat16 (under autocast they are brought to its dtype).  ``activation``: None,
+    ``"relu"``, ``"silu"`` or ``"gelu"`` (of the error function).  ``dropout_p`` and ``seed`` as in :func:`dropout`; a probability of 0
+    drops nothing.  The gradient computes the activation's argument again; beside its results it takes the gradient behind the
+    activation for pieces of at most 64 MB, and fp32 sums of ``weight``'s gradient.  In 16 bits that gradient is rounded to ``x``'s
+    dtype before its products.  At most 32 768 inputs and 2^20 outputs."""
+    check_activation(activation)
+    least = check_probability(dropout_p)
+    _check_shapes(x, weight, bias)
+    if torch.is_autocast_enabled():
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight = x.to(dtype), weight.to(dtype)
+        bias, residual = (t if t is None else t.to(dtype) for t in (bias, residual))
+    dtype_code(x.dtype)
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise TypeError(f"x is {x.dtype}, weight {weight.dtype}{'' if bias is None else f', bias {bias.dtype}'}: they must be of one dtype")
+    check_residual(residual, (x.shape[0], weight.shape[0]), x.dtype, x.device)
+    check_seed(seed, x.device)
+    seed = new_seed(x.device) if least and seed is None else 0 if not least else seed
+    if not reverse_mode_only() or not x.shape[0]:
+        return formula(x, weight, bias, activation, residual, least, seed)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _Linear.apply(x, weight, bias, residual, activation, least, seed)
+    return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed)[0]
+
+
+def _codes(t: Tensor):
+    """8-bit rows as the kernels read them, and the bytes from row to row."""
+    n, k = t.shape
+    if (t.stride(1) == 1 or k == 1) and t.data_ptr() % 16 == 0 and (n == 1 or (t.stride(0) >= k and t.stride(0) % 16 == 0)):
+        return t, t.stride(0) if n > 1 else -(-k // 16) * 16
+    rows = torch.empty((n, -(-k // 16) * 16), dtype=torch.uint8, device=t.device)
+    rows[:, :k].copy_(t.view(torch.uint8))
+    return rows, rows.shape[1]
+
+
+def _check_scale(scale: Tensor, rows: int, device: torch.device, name: str) -> None:
+    if scale.shape != (rows,) or scale.dtype != torch.float32 or scale.device != device:
+        raise ValueError(f"{name} must be {rows} float32 numbers on {device}, got {tuple(scale.shape)} {scale.dtype} on {scale.device}")
+
+
+def linear_8bit(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
+                residual: Optional[Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """:func:`linear` of e4m3 numbers with a scale a row, as ``rms_norm_8bit`` and ``quantize_rows`` give them: products in 8 bits, summed in
+    fp32, times the scales.  ``residual`` and the result are of ``out_dtype`` (float16 or bfloat16), to which the bias is brought.  No
+    gradient."""
+    act = check_activation(activation)
+    _check_shapes(x, weight, bias)
+    if x.dtype != E4M3 or weight.dtype != E4M3:
+        raise TypeError(f"x and weight must be {E4M3}, got {x.dtype} and {weight.dtype}")
+    if out_dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"out_dtype must be float16 or bfloat16, got {out_dtype}")
+    (n, k), m, dev = x.shape, weight.shape[0], x.device
+    _check_scale(x_scale, n, dev, "x_scale")
+    _check_scale(weight_scale, m, dev, "weight_scale")
+    check_residual(residual, (n, m), out_dtype, dev)
+    no_gradient("linear_8bit", x, x_scale, weight, weight_scale, bias, residual)
+    y = torch.empty((n, m), dtype=out_dtype, device=dev)
+    if not n:
+        return y
+    x, x_ld = _codes(x)
+    weight, w_ld = _codes(weight)
+    res_ld = 0
+    if residual is not None:
+        residual, res_ld = _rows(residual)
+    bias = None if bias is None else bias.to(out_dtype).contiguous()
+    x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    with on_device(dev):
+        check(lib().wcn_linear_8bit(ptr(x), x_ld, ptr(x_scale), n, k, ptr(weight), w_ld, ptr(weight_scale), m, dtype_code(out_dtype), ptr(bias), act,
+                                    ptr(residual), res_ld, ptr(y), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear_8bit")
+        count_training_launches("wcn_linear_8bit")
+    return y
