@@ -134,6 +134,28 @@ def test_activations_over_their_whole_range(dtype, act):
     assert float(y[0, 0]) == float("inf") and torch.isnan(y[0, 1])
 
 
+@pytest.mark.parametrize("act,p", [(None, 0.0), ("gelu", 0.0), ("relu", 0.2)])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n,k,m", [(60001, 64, 32), (45000, 40, 20), (60000, 96, 96), (45003, 128, 160), (30000, 264, 136), (40000, 72, 400), (9000, 512, 1100)])
+def test_several_tiles_a_multiprocessor(n, k, m, residual, act, p):
+    """More tiles than multiprocessors, of one to eight pieces of columns, a group of columns a block and not: gradients too."""
+    x, w, b, r, dy = make(n, k, m, torch.bfloat16)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = linear(*leaves, act, r if residual else None, p, 6)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    keep = dropout(torch.ones(n, m, device=DEV), p, 6).double()
+    z = x.double() @ w.double().t() + b.double()
+    a, slope = act64(z, act)
+    want = a * keep + (r.double() if residual else 0)
+    h = half(torch.bfloat16)
+    within(y.detach(), want, h * want.abs() + keep * (1.13 * (sums(k, x.double().abs() @ w.double().abs().t(), torch.bfloat16) + 2 * U * z.abs()) + 2e-5 * a.abs() + 1e-11) + 4 * U * want.abs())
+    dz = dy.double() * keep * slope
+    assert off(dx, dz @ w.double()) <= h and off(dw, dz.t() @ x.double()) <= h and off(db, dz.sum(0)) <= h
+    rows = torch.linspace(0, n - 1, 500, device=DEV).long()   # every row is its own
+    assert off(dx[rows], (dz @ w.double())[rows]) <= 1.3 * h
+    check_device_status(DEV)
+
+
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(3)
     n, k, m = 37, 20, 24

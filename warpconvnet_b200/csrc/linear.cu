@@ -13,6 +13,8 @@
 #include "linear_ce.cuh"
 
 int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st);
+int wcn_dropout_rows(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, int64_t n, int c, int dtype, const wcn_drop& drop, int64_t row0, void* y,
+                     int64_t y_ld, cudaStream_t st);
 int wcn_ce_product_splits(int m, int n, int k, bool blocked, bool ones);
 int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st);
 
@@ -284,7 +286,7 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
     int64_t dz_ld = dy_ld;
     if (!direct) {
       wcn_linear_product q = {xp, w, x_ld, w_ld, rows, m, k, nullptr, nullptr, ws, p.dz_ld, bias, act, true, dyp, dy_ld, drop, r0};
-      const int rc = run(q, dtype, false, dev_status, st);
+      const int rc = act ? run(q, dtype, false, dev_status, st) : wcn_dropout_rows(dyp, dy_ld, nullptr, 0, rows, m, dtype, drop, r0, ws, p.dz_ld, st);
       if (rc != WCN_OK) return rc;
       dz = ws;
       dz_ld = p.dz_ld;

@@ -8,7 +8,7 @@
 // own 2 KB of shared memory, one piece ahead, and the result leaves from the same place by TMA: rows of 64 bytes per thread
 // would cost the load/store pipe a line each.  Rows that TMA cannot take (pitches that are no multiple of 16 bytes) go the same way
 // through shared memory and from there in elements.
-// Where they fit beside a ring of four tiles, the columns' rows of B stay in shared memory (RESIDENT): a block then has one group of
+// Where they fit beside a ring of four tiles, the columns' rows of B stay in shared memory: a block then has one group of
 // columns, and A alone passes.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
@@ -25,14 +25,16 @@ constexpr int MN_CHUNK = 64 * 128;                         // 64 of k x 64 colum
 constexpr int MAX_STAGES = 12, MAX_ACC = 4;
 constexpr int EPI_WARP0 = 2, PARTS = 4, EPI_WARPS = 4 * PARTS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int PIECE = 32, PIECE_BYTES = 32 * PIECE * 2;    // columns of a warp's piece; its 32 rows in shared memory
-constexpr int SMEM_BUDGET = 224 * 1024;
+constexpr int LASTING = 1024;                              // columns whose bias is kept
+constexpr int SMEM_BUDGET = 226 * 1024;
 
 struct Params {
   wcn_linear_product q;
   int KB, NT;               // slices of k; columns of a tile (a multiple of 32)
   int m_tiles, n_tiles, stages, accs, tmem_cols;
   int b_slice;              // bytes of a slice of B
-  int out_tma, add_tma;
+  int out_tma, add_tma, resident;
+  int lasting;              // bias and scales are in shared memory from the start on: of the block's columns, or of all
   int32_t* dev_status;
 };
 
@@ -51,7 +53,7 @@ struct Control {
   uint64_t done;
   uint32_t tmem_holder;
   int32_t skip;
-  __align__(16) float bias[EPI_WARPS][PIECE], scale[EPI_WARPS][PIECE];   // of a warp's piece
+  __align__(16) float bias[LASTING], scale[LASTING];   // of all columns that this block has, or of each warp's piece
 };
 
 __device__ __forceinline__ uint32_t bar(uint64_t* b) { return smem_u32(b); }
@@ -82,6 +84,15 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_shared(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // ------------------------------------------------------------------ activations, two numbers at a time
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
@@ -95,33 +106,30 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The larger and the smaller of two numbers; what is no number stays so.
+// The larger of two numbers; what is no number stays so.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float y;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-// Normal distribution's function at -u, 0 <= u <= 7, as an exponential of a polynomial: log2 of it is a smooth curve near a parabola,
-// fitted by least largest error (degree 8): within 8e-6 of the value everywhere, an eightieth of half a step of 16-bit results at
-// least.  The error function of the library takes three times the instructions of the pipes that bound this kernel.
-constexpr float GELU_END = 7.f;   // behind which the function, 1e-12, is taken as what it is there
-__device__ __forceinline__ float2 normal_tail(float2 u) {
-  float2 p = both(5.216057985535372e-08f);
-  p = __ffma2_rn(p, u, both(-3.0775302093388746e-06f));
-  p = __ffma2_rn(p, u, both(7.351476233452559e-05f));
-  p = __ffma2_rn(p, u, both(-0.0009893535170704126f));
-  p = __ffma2_rn(p, u, both(0.00866654422134161f));
-  p = __ffma2_rn(p, u, both(-0.05418838933110237f));
-  p = __ffma2_rn(p, u, both(-0.45830658078193665f));
-  p = __ffma2_rn(p, u, both(-1.1512914896011353f));
-  p = __ffma2_rn(p, u, both(-0.9999936819076538f));
+// Normal distribution's function at v <= 0 as an exponential of a polynomial: log2 of it is a smooth curve near a parabola, fitted by
+// least largest error (degree 7) from -6.5 on: within 9e-6 of the value, a fiftieth of half a step of 16-bit results at least.  Before
+// that, where it is below 4e-11, the polynomial falls as the function does, to 0.  (The library's error function takes three times the
+// instructions, of which this kernel has its fill.)
+constexpr float GELU_END = -64.f;   // where it is 0, and so that infinity times it is none
+__device__ __forceinline__ float2 normal_tail(float2 v) {
+  float2 p = both(1.75778337e-06f);
+  p = __ffma2_rn(p, v, both(5.99367486e-05f));
+  p = __ffma2_rn(p, v, both(0.000916364603f));
+  p = __ffma2_rn(p, v, both(0.00844739377f));
+  p = __ffma2_rn(p, v, both(0.0538245253f));
+  p = __ffma2_rn(p, v, both(-0.458615661f));
+  p = __ffma2_rn(p, v, both(1.15118015f));
+  p = __ffma2_rn(p, v, both(-1.00000381f));
   return make_float2(exp2_fast(p.x), exp2_fast(p.y));
 }
+// -|z|, the polynomial's end at least; what is no number stays so.
+__device__ __forceinline__ float2 below_zero(float2 z) { return make_float2(max_nan(-fabsf(z.x), GELU_END), max_nan(-fabsf(z.y), GELU_END)); }
 __device__ __forceinline__ float2 logistic(float2 z) {
   const float2 e = __fmul2_rn(z, both(-1.4426950408889634f));
   const float2 d = __fadd2_rn(both(1.f), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
@@ -132,8 +140,8 @@ template <int ACT> __device__ __forceinline__ float2 activate(float2 z) {
   if (ACT == WCN_ACT_RELU) return make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f));
   if (ACT == WCN_ACT_SILU) return __fmul2_rn(z, logistic(z));
   if (ACT == WCN_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-    const float2 u = make_float2(min_nan(fabsf(z.x), GELU_END), min_nan(fabsf(z.y), GELU_END));
-    return __ffma2_rn(make_float2(-u.x, -u.y), normal_tail(u), make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
+    const float2 v = below_zero(z);
+    return __ffma2_rn(v, normal_tail(v), make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
   }
   return z;
 }
@@ -145,9 +153,9 @@ template <int ACT> __device__ __forceinline__ float2 through(float2 dy, float2 z
     return __fmul2_rn(dy, __fmul2_rn(p, __ffma2_rn(z, q, both(1.f))));
   }
   if (ACT == WCN_ACT_GELU) {   // Phi(z) + z phi(z)
-    const float2 u = make_float2(min_nan(fabsf(z.x), GELU_END), min_nan(fabsf(z.y), GELU_END));
-    const float2 e = __ffma2_rn(__fmul2_rn(u, u), both(-0.72134752044448170f), both(-1.3257480647361595f));
-    const float2 t = __ffma2_rn(make_float2(-u.x, -u.y), make_float2(exp2_fast(e.x), exp2_fast(e.y)), normal_tail(u));   // of -|z|
+    const float2 v = below_zero(z);
+    const float2 e = __ffma2_rn(__fmul2_rn(v, v), both(-0.72134752044448170f), both(-1.3257480647361595f));
+    const float2 t = __ffma2_rn(v, make_float2(exp2_fast(e.x), exp2_fast(e.y)), normal_tail(v));   // of -|z|
     return __fmul2_rn(dy, make_float2(z.x > 0.f ? 1.f - t.x : t.x, z.y > 0.f ? 1.f - t.y : t.y));
   }
   return dy;
@@ -170,76 +178,61 @@ template <bool BF16> __device__ __forceinline__ float number(uint16_t v) {
 }
 
 // A piece's numbers of one row: v = A B^T + bias on entry, the result's on exit; add: 32 numbers in 16 bits.
-template <int ACT, bool BF16> __device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[16], const uint4 (&add)[4], int64_t row, int col) {
-  const uint32_t* const a = reinterpret_cast<const uint32_t*>(add);
-  if (q.grad) {
-    float2 g[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = unpack2<BF16>(a[4 * b + i]);
-      if (q.drop.least) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, reinterpret_cast<float*>(g));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * b + i] = through<ACT>(g[i], v[4 * b + i]);
-    }
-    return;
-  }
+template <int ACT, bool GRAD, bool BF16>
+__device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[16], const uint4 (&add)[4], int64_t row, int col) {
+  const bool drop = q.drop.least != 0, sum = !GRAD && q.add;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
+    const uint32_t a[4] = {add[b].x, add[b].y, add[b].z, add[b].w};
+    float2 t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[4 * b + i] = activate<ACT>(v[4 * b + i]);
-    if (q.drop.least) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, reinterpret_cast<float*>(&v[4 * b]));
-    if (q.add)
+    for (int i = 0; i < 4; ++i) t[i] = GRAD ? unpack2<BF16>(a[i]) : activate<ACT>(v[4 * b + i]);
+    if (drop) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * b + i] = __fadd2_rn(v[4 * b + i], unpack2<BF16>(a[4 * b + i]));
+    for (int i = 0; i < 4; ++i) v[4 * b + i] = GRAD ? through<ACT>(t[i], v[4 * b + i]) : sum ? __fadd2_rn(t[i], unpack2<BF16>(a[i])) : t[i];
   }
 }
 
-// The tiles of a block.  RESIDENT: one group of columns, every `step`-th tile of rows; else tiles in order, columns fastest.
+// The tiles of a block.  With the columns' rows of B in shared memory: one group of columns, a part of its tiles of rows; else all tiles
+// in order, columns fastest.
 struct Tiles {
-  int m, n, step, i, m_tiles, n_tiles;
-  bool resident;
+  int m, n, dm, dn, m_tiles, n_tiles;
+  __device__ __forceinline__ explicit Tiles(const Params& p) : m_tiles(p.m_tiles), n_tiles(p.n_tiles) {
+    const int grid = (int)gridDim.x;
+    m = (int)blockIdx.x / n_tiles;
+    n = (int)blockIdx.x - m * n_tiles;
+    dm = p.resident ? (grid - n + n_tiles - 1) / n_tiles : grid / n_tiles;   // (resident: the blocks of this group)
+    dn = p.resident ? 0 : grid - dm * n_tiles;
+  }
   __device__ __forceinline__ bool there() const { return m < m_tiles; }
   __device__ __forceinline__ void advance() {
-    if (resident) { m += step; return; }
-    i += (int)gridDim.x;
-    m = i / n_tiles;
-    n = i - m * n_tiles;
+    m += dm;
+    n += dn;
+    if (n >= n_tiles) { n -= n_tiles; ++m; }
   }
 };
-template <bool RESIDENT> __device__ __forceinline__ Tiles first_tile(const Params& p) {
-  Tiles t;
-  t.m_tiles = p.m_tiles; t.n_tiles = p.n_tiles; t.resident = RESIDENT; t.step = 0; t.i = blockIdx.x;
-  if (RESIDENT) {
-    t.n = blockIdx.x % p.n_tiles;
-    t.m = blockIdx.x / p.n_tiles;
-    t.step = ((int)gridDim.x - t.n + p.n_tiles - 1) / p.n_tiles;   // blocks of this group
-  } else {
-    t.m = t.i / p.n_tiles;
-    t.n = t.i - t.m * p.n_tiles;
-  }
-  return t;
-}
 
 // KIND: operands f16, bf16 or e4m3.  B_MN: the columns of the result run along B's rows.
-template <int KIND, bool B_MN, bool RESIDENT, bool BF16>
+// ACT, GRAD: what is made of the sums (see linear.cuh); a kernel for each, as one that has all of them waits for its instructions.
+template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap out_map,
               const __grid_constant__ CUtensorMap add_map, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int DEPTH = KIND == WCN_E4M3 ? 128 : 64;       // elements of k of a slice
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int stage_bytes = RESIDENT ? A_BYTES : A_BYTES + p.b_slice;
+  const bool resident = p.resident;
+  const int stage_bytes = resident ? A_BYTES : A_BYTES + p.b_slice;
   const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
   const uint32_t base = smem_u32(smem_raw) + pad;
-  const uint32_t res = base + (uint32_t)(p.stages * stage_bytes), staging = res + (RESIDENT ? (uint32_t)(p.KB * p.b_slice) : 0u);
+  const uint32_t res = base + (uint32_t)(p.stages * stage_bytes), staging = res + (resident ? (uint32_t)(p.KB * p.b_slice) : 0u);
   uint8_t* const staging_at = smem_raw + (staging - smem_u32(smem_raw));
   Control* const ctl = reinterpret_cast<Control*>(staging_at + EPI_WARPS * 2 * PIECE_BYTES);
   const wcn_linear_product& q = p.q;
   uint16_t* const out = reinterpret_cast<uint16_t*>(q.out);
   auto mark = [&]() {
     const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
-    for (Tiles t = first_tile<RESIDENT>(p); t.there(); t.advance())
+    for (Tiles t(p); t.there(); t.advance())
       for (int i = threadIdx.x; i < TILE_M * p.NT; i += THREADS) {
         const int row = t.m * TILE_M + i / p.NT, col = t.n * p.NT + i % p.NT;
         if (row < q.m && col < q.n) out[(int64_t)row * q.out_ld + col] = nan;
@@ -256,6 +249,14 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
       for (int i = 0; i < 2; ++i) mbar_init(bar(&ctl->add_full[w][i]), 1);
     mbar_init(bar(&ctl->done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (p.lasting && !B_MN) {
+    const int first = resident ? (int)blockIdx.x % p.n_tiles * p.NT : 0;
+    for (int i = threadIdx.x; i < p.lasting; i += THREADS) {
+      const bool there = first + i < q.n;
+      ctl->bias[i] = q.bias && there ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[first + i]) : 0.f;
+      if (KIND == WCN_E4M3) ctl->scale[i] = there ? __ldg(&q.b_scale[first + i]) : 0.f;
+    }
   }
   if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
   tc_fence_before();
@@ -275,9 +276,9 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           tma_load_2d(to, &b_map, s * DEPTH, n * p.NT, full);
         }
       };
-      Tiles t = first_tile<RESIDENT>(p);
+      Tiles t(p);
       const bool any = t.there();
-      if (RESIDENT && any) {
+      if (resident && any) {
         mbar_expect_tx(bar(&ctl->b_full), (uint32_t)(p.KB * p.b_slice));
         for (int s = 0; s < p.KB; ++s) load_b(res + (uint32_t)(s * p.b_slice), s, t.n, bar(&ctl->b_full));
       }
@@ -287,7 +288,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
           mbar_expect_tx(full, (uint32_t)stage_bytes);
           tma_load_2d(at, &a_map, s * DEPTH, t.m * TILE_M, full);
-          if (!RESIDENT) load_b(at + A_BYTES, s, t.n, full);
+          if (!resident) load_b(at + A_BYTES, s, t.n, full);
           r.advance();
           ++issued;
         }
@@ -296,7 +297,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           if (--r.slot < 0) { r.slot = r.depth - 1; r.phase ^= 1; }
           for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->full[r.slot]), (uint32_t)r.phase); ++k) {}
         }
-        for (int k = 0; RESIDENT && any && k < 100000 && !mbar_try_wait(bar(&ctl->b_full), 0); ++k) {}
+        for (int k = 0; resident && any && k < 100000 && !mbar_try_wait(bar(&ctl->b_full), 0); ++k) {}
       }
     }
     __syncwarp();
@@ -306,11 +307,11 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
       const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (B_MN ? 1u << 16 : 0u) | ((uint32_t)(p.NT >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
       constexpr int B_STEP = B_MN ? 128 : 2;                  // an instruction's depth further, in units of 16 bytes
       auto describe_b = [&](uint32_t at) { return B_MN ? smem_desc_mn<128>(at, MN_CHUNK) : smem_desc<128>(at); };
-      const uint64_t a0 = smem_desc<128>(base), b0 = describe_b(RESIDENT ? res : base + A_BYTES);
+      const uint64_t a0 = smem_desc<128>(base), b0 = describe_b(resident ? res : base + A_BYTES);
       Ring r{0, 0, p.stages};
       int ab = 0, aphase = 0;
-      Tiles t = first_tile<RESIDENT>(p);
-      if (RESIDENT && t.there()) ok = mbar_wait(bar(&ctl->b_full), 0, p.dev_status);
+      Tiles t(p);
+      if (resident && t.there()) ok = mbar_wait(bar(&ctl->b_full), 0, p.dev_status);
       for (; ok && t.there(); t.advance()) {
         if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
         tc_fence_after();
@@ -319,7 +320,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           if (!mbar_wait(bar(&ctl->full[r.slot]), r.phase, p.dev_status)) { ok = false; break; }
           tc_fence_after();
           const uint64_t slot = (uint64_t)((r.slot * stage_bytes) >> 4);
-          const uint64_t a = a0 + slot, b = b0 + (RESIDENT ? (uint64_t)((s * p.b_slice) >> 4) : slot);
+          const uint64_t a = a0 + slot, b = b0 + (resident ? (uint64_t)((s * p.b_slice) >> 4) : slot);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (KIND == WCN_E4M3) umma_f8(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
@@ -339,92 +340,105 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
   } else {
     // Pieces of the block's tiles are numbered through, columns fastest; a warp has every fourth.  It has then seen the accumulator
     // before the one that it waits for filled (of tiles of 32, 64 .. columns there are 4, 4 .. accumulators), as waits by parity want.
-    const int ew = warp - EPI_WARP0, quarter = warp & 3, part = ew >> 2, pieces = p.NT / PIECE;
+    const int ew = warp - EPI_WARP0, quarter = warp & 3, pieces = p.NT / PIECE;
     const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
     uint8_t* const mine = staging_at + ew * 2 * PIECE_BYTES;
     const uint32_t mine_at = staging + (uint32_t)(ew * 2 * PIECE_BYTES);
-    float* const bias = ctl->bias[ew];
-    float* const scale = ctl->scale[ew];
-    struct Place { Tiles t; int tile, piece; };
-    auto next = [&](Place& w, int by) {
-      w.piece += by;
-      while (w.piece >= pieces) { w.piece -= pieces; ++w.tile; w.t.advance(); }
+    const int rows = q.m - quarter * 32, step = p.NT;    // of this warp's quarters: there is one to do where a tile's first row is less
+    struct Place {
+      int row, n, piece, ab, phase;                      // first row of the tile, its place among the columns' tiles
     };
-    auto wanted = [&](const Place& w) { return w.t.m * TILE_M + quarter * 32 < q.m && w.t.n * p.NT + w.piece * PIECE < q.n; };
+    const Tiles first(p);
+    const int dm = first.dm * TILE_M, dn = first.dn, end = p.m_tiles * TILE_M;
+    auto next = [&](Place& w) {
+      w.piece += PARTS;
+      while (w.piece >= pieces) {
+        w.piece -= pieces;
+        w.row += dm;
+        w.n += dn;
+        if (w.n >= p.n_tiles) { w.n -= p.n_tiles; w.row += TILE_M; }
+        if (++w.ab == p.accs) { w.ab = 0; w.phase ^= 1; }
+      }
+    };
+    auto col_of = [&](const Place& w) { return w.n * step + w.piece * PIECE; };
+    const bool added = GRAD || q.add, by_tma = added && p.add_tma;
     auto request = [&](const Place& w, int buffer) {   // one lane
       const uint32_t full = bar(&ctl->add_full[ew][buffer]);
       mbar_expect_tx(full, PIECE_BYTES);
-      tma_load_2d(mine_at + (uint32_t)(buffer * PIECE_BYTES), &add_map, w.t.n * p.NT + w.piece * PIECE, w.t.m * TILE_M + quarter * 32, full);
+      tma_load_2d(mine_at + (uint32_t)(buffer * PIECE_BYTES), &add_map, col_of(w), w.row + quarter * 32, full);
     };
-    const bool by_tma = q.add && p.add_tma;
-    Place now{first_tile<RESIDENT>(p), 0, 0};
-    next(now, part);
-    int turn = 0, loads[2] = {0, 0}, waits[2] = {0, 0};   // pieces with a place in shared memory; copies into each of the two
-    if (by_tma && now.t.there() && wanted(now)) {
+    Place now{first.m * TILE_M, first.n, (ew >> 2) - PARTS, 0, 0};
+    next(now);
+    int b = 0;                               // this piece's place in shared memory
+    uint32_t pending = 0, phases = 0;        // of each of the two: whether a copy is on its way there, its barrier's phase
+    if (by_tma && now.row < end && now.row < rows && col_of(now) < q.n) {
       if (lane == 0) request(now, 0);
-      ++loads[0];
+      pending = 1;
     }
-    while (now.t.there()) {
+    uint32_t swizzled[4];                    // this lane's row of a piece, 16 bytes at a time
+#pragma unroll
+    for (int c = 0; c < 4; ++c) swizzled[c] = mine_at + (uint32_t)(lane * 64 + ((c ^ (lane >> 1 & 3)) << 4));
+    while (now.row < end) {
       Place then = now;
-      next(then, PARTS);
-      const int ab = now.tile % p.accs, aphase = now.tile / p.accs & 1;
-      const bool use = wanted(now);
-      const int col = now.t.n * p.NT + now.piece * PIECE, row = now.t.m * TILE_M + quarter * 32 + lane, b = turn & 1;
-      if (use) {
+      next(then);
+      const int col = col_of(now), row0 = now.row + quarter * 32, row = row0 + lane;
+      const bool use = now.row < rows && col < q.n;
+      const int kept = p.lasting ? (resident ? now.piece * PIECE : col) : ew * PIECE;
+      if (!p.lasting && !B_MN && use) {
         const bool there = col + lane < q.n;
-        bias[lane] = q.bias && there ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[col + lane]) : 0.f;
-        if (KIND == WCN_E4M3) scale[lane] = there ? __ldg(&q.b_scale[col + lane]) : 0.f;
+        ctl->bias[kept + lane] = q.bias && there ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[col + lane]) : 0.f;
+        if (KIND == WCN_E4M3) ctl->scale[kept + lane] = there ? __ldg(&q.b_scale[col + lane]) : 0.f;
       }
       const float row_scale = KIND == WCN_E4M3 && use && row < q.m ? __ldg(&q.a_scale[row]) : 0.f;
       // Places are free once the piece of two turns ago has been read from this one, and, where the next piece's copy goes into the
       // other one, the last piece from there.
+      const bool ask = by_tma && then.row < end && then.row < rows && col_of(then) < q.n;
+      const int other = use ? b ^ 1 : b;
       if (lane == 0) {
         if (by_tma) store_wait_read<0>();
         else store_wait_read<1>();
+        if (ask) request(then, other);
       }
+      if (ask) pending |= 1u << other;
       __syncwarp();
-      if (by_tma && then.t.there() && wanted(then)) {
-        const int other = use ? b ^ 1 : b;
-        if (lane == 0) request(then, other);
-        ++loads[other];
-      }
       uint4 add[4];
-      uint8_t* const at = mine + b * PIECE_BYTES;
-      auto chunk = [&](int line, int c) { return reinterpret_cast<uint4*>(at + line * 64 + ((c ^ (line >> 1 & 3)) << 4)); };
-      auto element = [&](int line, int c) { return reinterpret_cast<uint16_t*>(chunk(line, c >> 3)) + (c & 7); };
-      if (use && q.add) {
+      const uint32_t place = (uint32_t)(b * PIECE_BYTES);
+      auto element = [&](int line, int c) { return reinterpret_cast<uint16_t*>(mine + place + line * 64 + (((c >> 3) ^ (line >> 1 & 3)) << 4) + (c & 7) * 2); };
+      if (added && use) {
         if (by_tma) {
-          if (ok) ok = mbar_wait(bar(&ctl->add_full[ew][b]), waits[b] & 1, p.dev_status);
+          if (ok) ok = mbar_wait(bar(&ctl->add_full[ew][b]), phases >> b & 1, p.dev_status);
           if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-          ++waits[b];
+          phases ^= 1u << b;
+          pending &= ~(1u << b);
         } else {
-          for (int l = 0; l < 32; ++l) {
-            const int64_t from = (int64_t)(row - lane + l) * q.add_ld + col + lane;
-            *element(l, lane) = row - lane + l < q.m && col + lane < q.n ? reinterpret_cast<const uint16_t*>(q.add)[from] : (uint16_t)0;
-          }
+          for (int l = 0; l < 32; ++l)
+            *element(l, lane) = row0 + l < q.m && col + lane < q.n ? reinterpret_cast<const uint16_t*>(q.add)[(int64_t)(row0 + l) * q.add_ld + col + lane] : (uint16_t)0;
+          __syncwarp();
         }
-        __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) add[c] = *chunk(lane, c);
+        for (int c = 0; c < 4; ++c) add[c] = load_shared(swizzled[c] + place);
       }
-      if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
+      if (ok) ok = mbar_wait(bar(&ctl->acc_full[now.ab]), now.phase, p.dev_status);
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       tc_fence_after();
       uint32_t r[32];
-      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.NT + now.piece * PIECE), r);
+      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(now.ab * step + now.piece * PIECE), r);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[ab]));
+      if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[now.ab]));
       if (use) {
         float2 v[16];
+        const float4* const bias = reinterpret_cast<const float4*>(ctl->bias + kept);
+        const float4* const scale = reinterpret_cast<const float4*>(ctl->scale + kept);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 t = reinterpret_cast<const float4*>(bias)[i];
           v[2 * i] = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]));
           v[2 * i + 1] = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+          if (B_MN) continue;
+          const float4 t = bias[i];
           if (KIND == WCN_E4M3) {
-            const float4 s = reinterpret_cast<const float4*>(scale)[i];
+            const float4 s = scale[i];
             v[2 * i] = __ffma2_rn(__fmul2_rn(v[2 * i], both(row_scale)), make_float2(s.x, s.y), make_float2(t.x, t.y));
             v[2 * i + 1] = __ffma2_rn(__fmul2_rn(v[2 * i + 1], both(row_scale)), make_float2(s.z, s.w), make_float2(t.z, t.w));
           } else {
@@ -432,36 +446,30 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
             v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(t.z, t.w));
           }
         }
-        const int64_t place = q.row0 + row;
-        switch (q.act) {
-          case WCN_ACT_RELU: finish<WCN_ACT_RELU, BF16>(q, seed, v, add, place, col); break;
-          case WCN_ACT_SILU: finish<WCN_ACT_SILU, BF16>(q, seed, v, add, place, col); break;
-          case WCN_ACT_GELU: finish<WCN_ACT_GELU, BF16>(q, seed, v, add, place, col); break;
-          default: finish<WCN_ACT_NONE, BF16>(q, seed, v, add, place, col); break;
-        }
+        finish<ACT, GRAD, BF16>(q, seed, v, add, q.row0 + row, col);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          *chunk(lane, c) = make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3]));
+          store_shared(swizzled[c] + place, make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3])));
         if (p.out_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&out_map, col, row - lane, mine_at + (uint32_t)(b * PIECE_BYTES));
+            tma_store_2d(&out_map, col, row0, mine_at + place);
             store_commit();
           }
         } else {
           __syncwarp();
           for (int l = 0; l < 32; ++l)
-            if (row - lane + l < q.m && col + lane < q.n) out[(int64_t)(row - lane + l) * q.out_ld + col + lane] = *element(l, lane);
+            if (row0 + l < q.m && col + lane < q.n) out[(int64_t)(row0 + l) * q.out_ld + col + lane] = *element(l, lane);
           __syncwarp();
         }
-        ++turn;
+        b ^= 1;
       }
       now = then;
     }
     // what is still on its way to or from this warp's places
-    for (int b = 0; b < 2; ++b)
-      for (int k = 0; waits[b] < loads[b] && k < 100000 && !mbar_try_wait(bar(&ctl->add_full[ew][b]), (uint32_t)(waits[b] & 1)); ++k) {}
+    for (int i = 0; i < 2; ++i)
+      for (int k = 0; (pending >> i & 1) && k < 100000 && !mbar_try_wait(bar(&ctl->add_full[ew][i]), phases >> i & 1); ++k) {}
     if (lane == 0) store_wait_read<0>();
     __syncwarp();
   }
@@ -511,7 +519,7 @@ bool tma_rows(const void* p, int64_t ld, int size) { return reinterpret_cast<uin
 constexpr int FIXED = 1024 + EPI_WARPS * 2 * PIECE_BYTES + (int)sizeof(Control) + 64;
 
 // Columns of a tile, and whether B's stay in shared memory.
-bool plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
+void plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
   const int depth = kind == WCN_E4M3 ? 128 : 64, sms = wcn_num_sms();
   p->KB = (q.k + depth - 1) / depth;
   p->m_tiles = (q.m + TILE_M - 1) / TILE_M;
@@ -534,17 +542,25 @@ bool plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
   p->n_tiles = tiles_of(nt);
   p->b_slice = slice(nt);
   p->accs = 512 / nt < MAX_ACC ? 512 / nt : MAX_ACC;
+  p->resident = resident;
+  const int columns = resident ? nt : p->n_tiles * nt;
+  p->lasting = columns <= LASTING ? columns : 0;
   p->tmem_cols = 32;
   while (p->tmem_cols < p->accs * nt) p->tmem_cols *= 2;
-  return resident;
 }
 
-template <int KIND, bool B_MN, bool RESIDENT, bool BF16> int launch(Params& p, cudaStream_t st) {
-  const wcn_linear_product& q = p.q;
+template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16> int launch(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
+  Params p = {};
+  p.q = q;
+  p.dev_status = dev_status;
+  p.out_tma = tma_rows(q.out, q.out_ld, 2);
+  p.add_tma = q.add && tma_rows(q.add, q.add_ld, 2);
+  plan(q, KIND, B_MN, &p);
+  const bool resident = p.resident;
   constexpr int size = KIND == WCN_E4M3 ? 1 : 2, depth = SLICE_BYTES / size;
   constexpr CUtensorMapDataType wide = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   constexpr CUtensorMapDataType type = KIND == WCN_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : wide;
-  const int stage = RESIDENT ? A_BYTES : A_BYTES + p.b_slice, kept = RESIDENT ? p.KB * p.b_slice : 0;
+  const int stage = resident ? A_BYTES : A_BYTES + p.b_slice, kept = resident ? p.KB * p.b_slice : 0;
   p.stages = (SMEM_BUDGET - FIXED - kept) / stage;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   if (p.stages < 2) return WCN_ERR_UNSUPPORTED_CONFIG;
@@ -555,7 +571,7 @@ template <int KIND, bool B_MN, bool RESIDENT, bool BF16> int launch(Params& p, c
   if (p.out_tma) ok = ok && box_map(&out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
   if (q.add && p.add_tma) ok = ok && box_map(&add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
   if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
-  constexpr auto kern = linear_kernel<KIND, B_MN, RESIDENT, BF16>;
+  constexpr auto kern = linear_kernel<KIND, B_MN, ACT, GRAD, BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
@@ -564,23 +580,24 @@ template <int KIND, bool B_MN, bool RESIDENT, bool BF16> int launch(Params& p, c
   return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
-template <int KIND, bool B_MN, bool BF16> int by_plan(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
-  Params p = {};
-  p.q = q;
-  p.dev_status = dev_status;
-  p.out_tma = tma_rows(q.out, q.out_ld, 2);
-  p.add_tma = q.add && tma_rows(q.add, q.add_ld, 2);
-  return plan(q, KIND, B_MN, &p) ? launch<KIND, B_MN, true, BF16>(p, st) : launch<KIND, B_MN, false, BF16>(p, st);
+template <int KIND, bool GRAD, bool BF16> int by_act(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
+  switch (q.act) {
+    case WCN_ACT_RELU: return launch<KIND, false, WCN_ACT_RELU, GRAD, BF16>(q, dev_status, st);
+    case WCN_ACT_SILU: return launch<KIND, false, WCN_ACT_SILU, GRAD, BF16>(q, dev_status, st);
+    case WCN_ACT_GELU: return launch<KIND, false, WCN_ACT_GELU, GRAD, BF16>(q, dev_status, st);
+    default: return launch<KIND, false, WCN_ACT_NONE, GRAD, BF16>(q, dev_status, st);
+  }
 }
 
 }  // namespace
 
-// kind: WCN_F16, WCN_BF16 (the type of all) or WCN_E4M3 (of A and B; `bf16`: the others').  by_k: B is [k][n].  Rows of A and B start
+// An activation, dropout or bias only with B as [n][k].  kind: WCN_F16, WCN_BF16 (the type of all) or WCN_E4M3 (of A and B; `bf16`: the others').  by_k: B is [k][n].  Rows of A and B start
 // on 16-byte boundaries.
 int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st) {
   const int size = kind == WCN_E4M3 ? 1 : 2;
   if (!tma_rows(q.a, q.a_ld, size) || !tma_rows(q.b, q.b_ld, size)) return WCN_ERR_INVALID_PARAMETERS;
-  if (kind == WCN_E4M3) return bf16 ? by_plan<WCN_E4M3, false, true>(q, dev_status, st) : by_plan<WCN_E4M3, false, false>(q, dev_status, st);
-  if (kind == WCN_BF16) return by_k ? by_plan<WCN_BF16, true, true>(q, dev_status, st) : by_plan<WCN_BF16, false, true>(q, dev_status, st);
-  return by_k ? by_plan<WCN_F16, true, false>(q, dev_status, st) : by_plan<WCN_F16, false, false>(q, dev_status, st);
+  if (kind == WCN_E4M3) return bf16 ? by_act<WCN_E4M3, false, true>(q, dev_status, st) : by_act<WCN_E4M3, false, false>(q, dev_status, st);
+  if (by_k) return kind == WCN_BF16 ? launch<WCN_BF16, true, WCN_ACT_NONE, false, true>(q, dev_status, st) : launch<WCN_F16, true, WCN_ACT_NONE, false, false>(q, dev_status, st);
+  if (q.grad) return kind == WCN_BF16 ? by_act<WCN_BF16, true, true>(q, dev_status, st) : by_act<WCN_F16, true, false>(q, dev_status, st);
+  return kind == WCN_BF16 ? by_act<WCN_BF16, false, true>(q, dev_status, st) : by_act<WCN_F16, false, false>(q, dev_status, st);
 }

@@ -39,14 +39,18 @@ __device__ __forceinline__ uint4 philox_eight(uint64_t seed, uint32_t block, uin
   }
   return make_uint4(c0, c1, c2, c3);
 }
-// Eight numbers of a row, columns 8 * block on: zero (whatever they were) or times the scale.
-__device__ __forceinline__ void drop_eight(const wcn_drop& d, uint64_t seed, uint32_t block, uint64_t row, float* v) {
+// Eight numbers of a row, columns 8 * block on: zero (whatever they were) or times the scale.  (The bits are compared where they
+// stand in a word's upper half: what is below them there decides nothing against a bound that ends in zeros.)
+__device__ __forceinline__ void drop_eight(const wcn_drop& d, uint64_t seed, uint32_t block, uint64_t row, float2 (&v)[4]) {
   const uint4 w = philox_eight(seed, block, row);
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+  const uint32_t bound = d.least << 16;
+  const bool all = d.least >> 16;   // (of all 2^16 values: nothing stays)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = i & 1 ? words[i / 2] >> 16 : words[i / 2] & 0xFFFFu;
-    v[i] = bits >= d.least ? v[i] * d.scale : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = __fmul2_rn(v[i], make_float2(d.scale, d.scale));
+    v[i].x = (words[i] << 16) >= bound && !all ? y.x : 0.f;
+    v[i].y = words[i] >= bound && !all ? y.y : 0.f;
   }
 }
 
