@@ -22,7 +22,7 @@ namespace {
 constexpr int TILE_M = 128, SLICE_BYTES = 128;             // rows of a tile; bytes of k of a stage
 constexpr int A_BYTES = TILE_M * SLICE_BYTES;
 constexpr int MN_CHUNK = 64 * 128;                         // 64 of k x 64 columns of a B whose columns run along its rows
-constexpr int MAX_STAGES = 12, MAX_ACC = 4;
+constexpr int MAX_STAGES = 12, MAX_ACC = 8;
 constexpr int EPI_WARP0 = 2, PARTS = 4, EPI_WARPS = 4 * PARTS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int PIECE = 32, PIECE_BYTES = 32 * PIECE * 2;    // columns of a warp's piece; its 32 rows in shared memory
 constexpr int LASTING = 1024;                              // columns whose bias is kept
@@ -34,6 +34,7 @@ struct Params {
   int m_tiles, n_tiles, stages, accs, tmem_cols;
   int b_slice;              // bytes of a slice of B
   int out_tma, add_tma, resident;
+  int wide, turns;          // pieces of a warp's turn, turns of a tile
   int lasting;              // bias and scales are in shared memory from the start on: of the block's columns, or of all
   int32_t* dev_status;
 };
@@ -130,6 +131,19 @@ __device__ __forceinline__ float2 normal_tail(float2 v) {
 }
 // -|z|, the polynomial's end at least; what is no number stays so.
 __device__ __forceinline__ float2 below_zero(float2 z) { return make_float2(max_nan(-fabsf(z.x), GELU_END), max_nan(-fabsf(z.y), GELU_END)); }
+// -(Phi(v) + v phi(v)) / exp(-v^2 / 2) at v <= 0, the slope of GELU there: a polynomial of degree 7, fitted so that its largest error
+// times the exponential is least (4e-6; the slope itself reaches 1.13).
+__device__ __forceinline__ float2 slope_tail(float2 v) {
+  float2 p = both(-0.000168556944f);
+  p = __ffma2_rn(p, v, both(-0.00231906539f));
+  p = __ffma2_rn(p, v, both(-0.0139235854f));
+  p = __ffma2_rn(p, v, both(-0.0499400012f));
+  p = __ffma2_rn(p, v, both(-0.12582691f));
+  p = __ffma2_rn(p, v, both(-0.247959629f));
+  p = __ffma2_rn(p, v, both(-0.797662377f));
+  p = __ffma2_rn(p, v, both(-0.499996036f));
+  return p;
+}
 __device__ __forceinline__ float2 logistic(float2 z) {
   const float2 e = __fmul2_rn(z, both(-1.4426950408889634f));
   const float2 d = __fadd2_rn(both(1.f), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
@@ -152,11 +166,11 @@ template <int ACT> __device__ __forceinline__ float2 through(float2 dy, float2 z
     const float2 p = logistic(z), q = __ffma2_rn(p, both(-1.f), both(1.f));
     return __fmul2_rn(dy, __fmul2_rn(p, __ffma2_rn(z, q, both(1.f))));
   }
-  if (ACT == WCN_ACT_GELU) {   // Phi(z) + z phi(z)
+  if (ACT == WCN_ACT_GELU) {
     const float2 v = below_zero(z);
-    const float2 e = __ffma2_rn(__fmul2_rn(v, v), both(-0.72134752044448170f), both(-1.3257480647361595f));
-    const float2 t = __ffma2_rn(v, make_float2(exp2_fast(e.x), exp2_fast(e.y)), normal_tail(v));   // of -|z|
-    return __fmul2_rn(dy, make_float2(z.x > 0.f ? 1.f - t.x : t.x, z.y > 0.f ? 1.f - t.y : t.y));
+    const float2 e = __fmul2_rn(__fmul2_rn(v, both(-0.72134752044448170f)), v);
+    const float2 w = __ffma2_rn(make_float2(exp2_fast(e.x), exp2_fast(e.y)), slope_tail(v), both(0.5f));   // slope at |z| - 1/2
+    return __fmul2_rn(dy, __fadd2_rn(make_float2(copysignf(w.x, z.x), copysignf(w.y, z.y)), both(0.5f)));
   }
   return dy;
 }
@@ -177,12 +191,12 @@ template <bool BF16> __device__ __forceinline__ float number(uint16_t v) {
   return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
-// A piece's numbers of one row: v = A B^T + bias on entry, the result's on exit; add: 32 numbers in 16 bits.
-template <int ACT, bool GRAD, bool BF16>
-__device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[16], const uint4 (&add)[4], int64_t row, int col) {
-  const bool drop = q.drop.least != 0, sum = !GRAD && q.add;
+// Sixteen numbers of one row: v = A B^T + bias on entry, the result's on exit; add: as many in 16 bits.
+template <int ACT, bool GRAD, bool BF16, bool MORE>   // MORE: there may be dropout or a sum
+__device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[8], const uint4 (&add)[2], int64_t row, int col) {
+  const bool drop = MORE && q.drop.least != 0, sum = MORE && !GRAD && q.add;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
+  for (int b = 0; b < 2; ++b) {
     const uint32_t a[4] = {add[b].x, add[b].y, add[b].z, add[b].w};
     float2 t[4];
 #pragma unroll
@@ -244,7 +258,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(bar(&ctl->full[s]), 1); mbar_init(bar(&ctl->empty[s]), 1); }
     mbar_init(bar(&ctl->b_full), 1);
-    for (int i = 0; i < p.accs; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)(4 * (p.NT / PIECE))); }
+    for (int i = 0; i < p.accs; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)(4 * p.turns)); }
     for (int w = 0; w < EPI_WARPS; ++w)
       for (int i = 0; i < 2; ++i) mbar_init(bar(&ctl->add_full[w][i]), 1);
     mbar_init(bar(&ctl->done), 1);
@@ -338,30 +352,31 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     }
     __syncwarp();
   } else {
-    // Pieces of the block's tiles are numbered through, columns fastest; a warp has every fourth.  It has then seen the accumulator
-    // before the one that it waits for filled (of tiles of 32, 64 .. columns there are 4, 4 .. accumulators), as waits by parity want.
-    const int ew = warp - EPI_WARP0, quarter = warp & 3, pieces = p.NT / PIECE;
+    // A warp takes one piece at a time where something is added, else two side by side (what a turn costs besides is then shared).
+    // Turns of the block's tiles are numbered through, columns fastest; a warp has every PARTS-th.  It has then seen the accumulator's
+    // last tile but one filled (of tiles of one, two .. turns there are 8, 4 .. accumulators at least), as waits by parity want.
+    const int ew = warp - EPI_WARP0, quarter = warp & 3, pieces = p.NT / PIECE, wide = p.wide, turns = p.turns;
     const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
     uint8_t* const mine = staging_at + ew * 2 * PIECE_BYTES;
     const uint32_t mine_at = staging + (uint32_t)(ew * 2 * PIECE_BYTES);
     const int rows = q.m - quarter * 32, step = p.NT;    // of this warp's quarters: there is one to do where a tile's first row is less
     struct Place {
-      int row, n, piece, ab, phase;                      // first row of the tile, its place among the columns' tiles
+      int row, n, turn, ab, phase;                       // first row of the tile, its place among the columns' tiles
     };
     const Tiles first(p);
     const int dm = first.dm * TILE_M, dn = first.dn, end = p.m_tiles * TILE_M;
     auto next = [&](Place& w) {
-      w.piece += PARTS;
-      while (w.piece >= pieces) {
-        w.piece -= pieces;
+      w.turn += PARTS;
+      while (w.turn >= turns) {
+        w.turn -= turns;
         w.row += dm;
         w.n += dn;
         if (w.n >= p.n_tiles) { w.n -= p.n_tiles; w.row += TILE_M; }
         if (++w.ab == p.accs) { w.ab = 0; w.phase ^= 1; }
       }
     };
-    auto col_of = [&](const Place& w) { return w.n * step + w.piece * PIECE; };
-    const bool added = GRAD || q.add, by_tma = added && p.add_tma;
+    auto col_of = [&](const Place& w) { return w.n * step + w.turn * wide * PIECE; };
+    const bool added = GRAD || q.add, by_tma = added && p.add_tma, more = GRAD ? q.drop.least != 0 : added || q.drop.least;
     auto request = [&](const Place& w, int buffer) {   // one lane
       const uint32_t full = bar(&ctl->add_full[ew][buffer]);
       mbar_expect_tx(full, PIECE_BYTES);
@@ -369,7 +384,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     };
     Place now{first.m * TILE_M, first.n, (ew >> 2) - PARTS, 0, 0};
     next(now);
-    int b = 0;                               // this piece's place in shared memory
+    int b = 0;                               // the next piece's place in shared memory
     uint32_t pending = 0, phases = 0;        // of each of the two: whether a copy is on its way there, its barrier's phase
     if (by_tma && now.row < end && now.row < rows && col_of(now) < q.n) {
       if (lane == 0) request(now, 0);
@@ -381,29 +396,25 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     while (now.row < end) {
       Place then = now;
       next(then);
-      const int col = col_of(now), row0 = now.row + quarter * 32, row = row0 + lane;
-      const bool use = now.row < rows && col < q.n;
-      const int kept = p.lasting ? (resident ? now.piece * PIECE : col) : ew * PIECE;
-      if (!p.lasting && !B_MN && use) {
-        const bool there = col + lane < q.n;
-        ctl->bias[kept + lane] = q.bias && there ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[col + lane]) : 0.f;
-        if (KIND == WCN_E4M3) ctl->scale[kept + lane] = there ? __ldg(&q.b_scale[col + lane]) : 0.f;
-      }
+      const int col0 = col_of(now), row0 = now.row + quarter * 32, row = row0 + lane;
+      const bool use = now.row < rows && col0 < q.n;
       const float row_scale = KIND == WCN_E4M3 && use && row < q.m ? __ldg(&q.a_scale[row]) : 0.f;
-      // Places are free once the piece of two turns ago has been read from this one, and, where the next piece's copy goes into the
-      // other one, the last piece from there.
+      // What the last turn has left has been read from its place, which is this one's or the next copy's.
       const bool ask = by_tma && then.row < end && then.row < rows && col_of(then) < q.n;
       const int other = use ? b ^ 1 : b;
       if (lane == 0) {
-        if (by_tma) store_wait_read<0>();
-        else store_wait_read<1>();
+        store_wait_read<0>();
         if (ask) request(then, other);
       }
       if (ask) pending |= 1u << other;
+      if (!p.lasting && !B_MN && use)
+        for (int j = 0; j < wide; ++j) {
+          const int col = col0 + j * PIECE + lane, at = (ew * 2 + j) * PIECE + lane;
+          ctl->bias[at] = q.bias && col < q.n ? number<BF16>(reinterpret_cast<const uint16_t*>(q.bias)[col]) : 0.f;
+          if (KIND == WCN_E4M3) ctl->scale[at] = col < q.n ? __ldg(&q.b_scale[col]) : 0.f;
+        }
       __syncwarp();
-      uint4 add[4];
-      const uint32_t place = (uint32_t)(b * PIECE_BYTES);
-      auto element = [&](int line, int c) { return reinterpret_cast<uint16_t*>(mine + place + line * 64 + (((c >> 3) ^ (line >> 1 & 3)) << 4) + (c & 7) * 2); };
+      auto element = [&](int line, int c) { return reinterpret_cast<uint16_t*>(mine + b * PIECE_BYTES + line * 64 + (((c >> 3) ^ (line >> 1 & 3)) << 4) + (c & 7) * 2); };
       if (added && use) {
         if (by_tma) {
           if (ok) ok = mbar_wait(bar(&ctl->add_full[ew][b]), phases >> b & 1, p.dev_status);
@@ -412,44 +423,59 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           pending &= ~(1u << b);
         } else {
           for (int l = 0; l < 32; ++l)
-            *element(l, lane) = row0 + l < q.m && col + lane < q.n ? reinterpret_cast<const uint16_t*>(q.add)[(int64_t)(row0 + l) * q.add_ld + col + lane] : (uint16_t)0;
+            *element(l, lane) = row0 + l < q.m && col0 + lane < q.n ? reinterpret_cast<const uint16_t*>(q.add)[(int64_t)(row0 + l) * q.add_ld + col0 + lane] : (uint16_t)0;
           __syncwarp();
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) add[c] = load_shared(swizzled[c] + place);
       }
       if (ok) ok = mbar_wait(bar(&ctl->acc_full[now.ab]), now.phase, p.dev_status);
       if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
       tc_fence_after();
-      uint32_t r[32];
-      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(now.ab * step + now.piece * PIECE), r);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[now.ab]));
-      if (use) {
-        float2 v[16];
+      const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(now.ab * step);
+      const int last = min(now.turn * wide + wide, pieces) - 1;
+#pragma unroll 1
+      for (int piece = now.turn * wide, col = col0; piece <= last; ++piece, col += PIECE) {
+        uint32_t r[32];
+        tmem_ld32(taddr + (uint32_t)(piece * PIECE), r);
+        tmem_ld_wait();
+        if (piece == last) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[now.ab]));
+        }
+        if (!use || col >= q.n) continue;
+        const int kept = p.lasting ? (resident ? piece * PIECE : col) : (ew * 2 + piece - now.turn * wide) * PIECE;
         const float4* const bias = reinterpret_cast<const float4*>(ctl->bias + kept);
         const float4* const scale = reinterpret_cast<const float4*>(ctl->scale + kept);
+        const uint32_t place = (uint32_t)(b * PIECE_BYTES);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[2 * i] = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]));
-          v[2 * i + 1] = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-          if (B_MN) continue;
-          const float4 t = bias[i];
-          if (KIND == WCN_E4M3) {
-            const float4 s = scale[i];
-            v[2 * i] = __ffma2_rn(__fmul2_rn(v[2 * i], both(row_scale)), make_float2(s.x, s.y), make_float2(t.x, t.y));
-            v[2 * i + 1] = __ffma2_rn(__fmul2_rn(v[2 * i + 1], both(row_scale)), make_float2(s.z, s.w), make_float2(t.z, t.w));
-          } else {
-            v[2 * i] = __fadd2_rn(v[2 * i], make_float2(t.x, t.y));
-            v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(t.z, t.w));
+        for (int h = 0; h < 2; ++h) {   // (half a piece at a time, for the registers)
+          float2 v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[2 * i] = make_float2(__uint_as_float(r[16 * h + 4 * i]), __uint_as_float(r[16 * h + 4 * i + 1]));
+            v[2 * i + 1] = make_float2(__uint_as_float(r[16 * h + 4 * i + 2]), __uint_as_float(r[16 * h + 4 * i + 3]));
+            if (B_MN) continue;
+            const float4 t = bias[4 * h + i];
+            if (KIND == WCN_E4M3) {
+              const float4 s = scale[4 * h + i];
+              v[2 * i] = __ffma2_rn(__fmul2_rn(v[2 * i], both(row_scale)), make_float2(s.x, s.y), make_float2(t.x, t.y));
+              v[2 * i + 1] = __ffma2_rn(__fmul2_rn(v[2 * i + 1], both(row_scale)), make_float2(s.z, s.w), make_float2(t.z, t.w));
+            } else {
+              v[2 * i] = __fadd2_rn(v[2 * i], make_float2(t.x, t.y));
+              v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(t.z, t.w));
+            }
           }
-        }
-        finish<ACT, GRAD, BF16>(q, seed, v, add, q.row0 + row, col);
+          uint4 add[2];
+          if (added) {
+            add[0] = load_shared(swizzled[2 * h] + place);
+            add[1] = load_shared(swizzled[2 * h + 1] + place);
+          }
+          if (more) finish<ACT, GRAD, BF16, true>(q, seed, v, add, q.row0 + row, col + 16 * h);
+          else finish<ACT, GRAD, BF16, false>(q, seed, v, add, q.row0 + row, col + 16 * h);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          store_shared(swizzled[c] + place, make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3])));
+          for (int c = 0; c < 2; ++c)
+            store_shared(swizzled[2 * h + c] + place, make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3])));
+        }
         if (p.out_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -543,6 +569,7 @@ void plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
   p->b_slice = slice(nt);
   p->accs = 512 / nt < MAX_ACC ? 512 / nt : MAX_ACC;
   p->resident = resident;
+  p->turns = (nt / PIECE + p->wide - 1) / p->wide;
   const int columns = resident ? nt : p->n_tiles * nt;
   p->lasting = columns <= LASTING ? columns : 0;
   p->tmem_cols = 32;
@@ -555,6 +582,7 @@ template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16> int launch(const w
   p.dev_status = dev_status;
   p.out_tma = tma_rows(q.out, q.out_ld, 2);
   p.add_tma = q.add && tma_rows(q.add, q.add_ld, 2);
+  p.wide = q.add ? 1 : 2;
   plan(q, KIND, B_MN, &p);
   const bool resident = p.resident;
   constexpr int size = KIND == WCN_E4M3 ? 1 : 2, depth = SLICE_BYTES / size;
