@@ -30,7 +30,7 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void load_eight_of(
 
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(THREADS) dropout_kernel(const __grid_constant__ DropParams<T> p) {
-  const uint64_t seed = drop_seed(p.drop);
+  const PhiloxKeys keys = philox_keys(drop_seed(p.drop));
   const int64_t first = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   int64_t row = first / p.across;
   int at = (int)(first - row * p.across);   // piece of the row
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(THREADS) dropout_kernel(const __grid_constant_
       float2 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = make_float2(wcn_to_float<T>(x[j][2 * i]), wcn_to_float<T>(x[j][2 * i + 1]));
-      drop_eight(p.drop, seed, (uint32_t)ats[j], (uint64_t)(p.row0 + rows[j]), v);
+      if (p.drop.least) drop_eight(p.drop, keys, (uint32_t)ats[j], (uint64_t)(p.row0 + rows[j]), v);
       if (p.residual)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __fadd2_rn(v[i], make_float2(wcn_to_float<T>(r[j][2 * i]), wcn_to_float<T>(r[j][2 * i + 1])));

@@ -22,7 +22,7 @@ namespace {
 
 constexpr int THREADS = FP32_THREADS;
 constexpr int MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;
-constexpr int64_t PIECE_BYTES = 64ll << 20;    // of dz
+constexpr int64_t PIECE_BYTES = 512ll << 20;   // of dz
 
 // ------------------------------------------------------------------ fp32
 
@@ -48,7 +48,7 @@ __device__ __forceinline__ float through(int act, float dy, float z) {
 }
 
 __device__ __forceinline__ bool kept(const wcn_drop& d, uint64_t seed, int64_t row, int col) {
-  const uint4 w = philox_eight(seed, (uint32_t)col / 8, (uint64_t)row);
+  const uint4 w = philox_eight(philox_keys(seed), (uint32_t)col / 8, (uint64_t)row);
   const int at = col % 8 / 2;
   const uint32_t word = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
   return (col & 1 ? word >> 16 : word & 0xFFFFu) >= d.least;
@@ -269,9 +269,9 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   wcn_launched = 0;
   if (!sizes_taken(n, k, m) || n == 0 || dtype < WCN_F32 || dtype > WCN_BF16 || act < 0 || act > 3 || least < 0 || least > 65536) return WCN_ERR_INVALID_PARAMETERS;
   const int size = wcn_dtype_size(dtype), what = (dx ? DX : 0) | (dw ? DW : 0) | (db ? DB : 0);
-  const bool direct = act == WCN_ACT_NONE && least == 0;
+  // (rows of a gradient between boundaries are brought to them as others are made)
+  const bool direct = act == WCN_ACT_NONE && least == 0 && rows_taken(dy, dy_ld, n, m, size);
   if (!what || !dev_status || !rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !dy || (n > 1 && dy_ld < m)) return WCN_ERR_INVALID_PARAMETERS;
-  if (direct && !rows_taken(dy, dy_ld, n, m, size)) return WCN_ERR_INVALID_PARAMETERS;
   const Pieces p = plan(n, k, m, dtype, what, direct);
   if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes)) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);

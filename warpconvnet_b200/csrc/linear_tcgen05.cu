@@ -201,7 +201,7 @@ __device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t see
     float2 t[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = GRAD ? unpack2<BF16>(a[i]) : activate<ACT>(v[4 * b + i]);
-    if (drop) drop_eight(q.drop, seed, (uint32_t)col / 8 + b, (uint64_t)row, t);
+    if (drop) drop_eight(q.drop, philox_keys(seed), (uint32_t)col / 8 + b, (uint64_t)row, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[4 * b + i] = GRAD ? through<ACT>(t[i], v[4 * b + i]) : sum ? __fadd2_rn(t[i], unpack2<BF16>(a[i])) : t[i];
   }

@@ -24,33 +24,42 @@ namespace {
 
 __device__ __forceinline__ uint64_t drop_seed(const wcn_drop& d) { return d.at ? (uint64_t)__ldg(d.at) : d.seed; }
 
-__device__ __forceinline__ uint4 philox_eight(uint64_t seed, uint32_t block, uint64_t row) {
+// The keys of the ten rounds: they follow from the seed alone.
+struct PhiloxKeys {
+  uint32_t a[10], b[10];
+};
+__device__ __forceinline__ PhiloxKeys philox_keys(uint64_t seed) {
+  PhiloxKeys k;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    k.a[r] = (uint32_t)seed + r * 0x9E3779B9u;
+    k.b[r] = (uint32_t)(seed >> 32) + r * 0xBB67AE85u;
+  }
+  return k;
+}
+__device__ __forceinline__ uint4 philox_eight(const PhiloxKeys& k, uint32_t block, uint64_t row) {
   uint32_t c0 = block, c1 = (uint32_t)row, c2 = (uint32_t)(row >> 32), c3 = 0;
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k.a[r];
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k.b[r];
     c3 = (uint32_t)p0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
 // Eight numbers of a row, columns 8 * block on: zero (whatever they were) or times the scale.  (The bits are compared where they
-// stand in a word's upper half: what is below them there decides nothing against a bound that ends in zeros.)
-__device__ __forceinline__ void drop_eight(const wcn_drop& d, uint64_t seed, uint32_t block, uint64_t row, float2 (&v)[4]) {
-  const uint4 w = philox_eight(seed, block, row);
+// stand in a word's upper half: what is below them there decides nothing against a bound that ends in ones.)  Not for `least` 0.
+__device__ __forceinline__ void drop_eight(const wcn_drop& d, const PhiloxKeys& keys, uint32_t block, uint64_t row, float2 (&v)[4]) {
+  const uint4 w = philox_eight(keys, block, row);
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-  const uint32_t bound = d.least << 16;
-  const bool all = d.least >> 16;   // (of all 2^16 values: nothing stays)
+  const uint32_t bound = (d.least << 16) - 1u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 y = __fmul2_rn(v[i], make_float2(d.scale, d.scale));
-    v[i].x = (words[i] << 16) >= bound && !all ? y.x : 0.f;
-    v[i].y = words[i] >= bound && !all ? y.y : 0.f;
+    v[i].x = (words[i] << 16) > bound ? y.x : 0.f;
+    v[i].y = words[i] > bound ? y.y : 0.f;
   }
 }
 

@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 from torch import Tensor
 
-from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import WCN_F32, check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import reverse_mode_only
 from .dropout import check_probability, check_seed, kept_factor, new_seed
 from .group_norm import _ACTIVATIONS, _rows, check_activation
@@ -93,8 +93,9 @@ class _Linear(torch.autograd.Function):
         dx = torch.empty((n, k), dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((m, k), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(m, dtype=x.dtype, device=dev) if need_b else None
-        direct = not act and not ctx.least
-        dy, dy_ld = _matrix(dy) if direct else _rows(dy)
+        dy, dy_ld = _rows(dy)
+        whole = 1 if code == WCN_F32 else 8
+        direct = not act and not ctx.least and dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
         x, x_ld = _matrix(x if x_rows is None else x_rows, k)
         weight, w_ld = _matrix(weight if w_rows is None else w_rows, k)
         bias = None if bias is None else bias.contiguous()
