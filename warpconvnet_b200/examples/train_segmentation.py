@@ -1,6 +1,6 @@
 """Training a small voxel network for semantic segmentation with the operators around its convolutions: group norm per scene
 with its activation (``SegmentedGroupNorm``), a head that gives the loss without its logits (``LinearCrossEntropy``) and
-``AdamW`` in one launch, moments in 32 or 8 bits.
+``AdamW`` in one launch, moments in 32 or 8 bits; with ``--blocks`` some feed-forward blocks (``FeedForward``) before the head.
 
     python -m warpconvnet_b200.examples.train_segmentation --scenes 4 --voxels 60000 --classes 200 --state-bits 8
 
@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from .. import LinearCrossEntropy, SegmentedGroupNorm, Sequential, SparseConv3d, Voxels, cat
+from .. import FeedForward, LinearCrossEntropy, SegmentedGroupNorm, Sequential, SparseConv3d, Voxels, cat
 from .._native import check_device_status
 from ..datasets import synthetic
 from ..optim import AdamW
@@ -31,18 +31,19 @@ def _norm(channels: int) -> SegmentedGroupNorm:
 class SegmentationNet(nn.Module):
     """Two levels of a U-Net; ``forward`` gives the loss of a batch, :meth:`features` what the head is applied to."""
 
-    def __init__(self, in_channels: int, num_classes: int, width: int = 32):
+    def __init__(self, in_channels: int, num_classes: int, width: int = 32, blocks: int = 0):
         super().__init__()
         self.stem = Sequential(SparseConv3d(in_channels, width, 3, bias=False), _norm(width))
         self.down = Sequential(SparseConv3d(width, 2 * width, 2, stride=2, bias=False), _norm(2 * width),
                                SparseConv3d(2 * width, 2 * width, 3, bias=False), _norm(2 * width))
         self.up = SparseConv3d(2 * width, width, 2, stride=2, transposed=True, bias=False)
         self.mix = Sequential(SparseConv3d(2 * width, 2 * width, 3, bias=False), _norm(2 * width))
+        self.blocks = nn.Sequential(*(FeedForward(2 * width, 8 * width, dropout=0.1) for _ in range(blocks)))
         self.head = LinearCrossEntropy(2 * width, num_classes)
 
     def features(self, x: Voxels) -> Voxels:
         fine = self.stem(x)
-        return self.mix(cat(self.up(self.down(fine), fine), fine))
+        return self.blocks(self.mix(cat(self.up(self.down(fine), fine), fine)))
 
     def forward(self, x: Voxels, labels: Tensor) -> Tensor:
         return self.head(self.features(x), labels)
@@ -65,10 +66,10 @@ def make_batch(scenes: int, voxels: int, classes: int, seed: int, device) -> Tup
 
 
 def train(scenes: int = 2, voxels: int = 20000, classes: int = 40, steps: int = 30, state_bits: int = 32, dtype=torch.bfloat16,
-          lr: float = 4e-3, seed: int = 0, device="cuda:0") -> Tuple[List[float], float]:
+          lr: float = 4e-3, seed: int = 0, device="cuda:0", blocks: int = 0) -> Tuple[List[float], float]:
     """(loss of every step, milliseconds per step after the first five)"""
     torch.manual_seed(seed)
-    net = SegmentationNet(4, classes).to(device)
+    net = SegmentationNet(4, classes, blocks=blocks).to(device)
     opt = AdamW(net.parameters(), lr=lr, state_bits=state_bits)
     scaler = torch.amp.GradScaler("cuda", enabled=dtype == torch.float16)
     batches = [make_batch(scenes, voxels, classes, seed + 100 * i, device) for i in range(2)]
@@ -97,10 +98,11 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--state-bits", type=int, default=32, choices=(8, 32))
     ap.add_argument("--dtype", default="bf16", choices=("fp32", "fp16", "bf16"))
+    ap.add_argument("--blocks", type=int, default=0)
     a = ap.parse_args()
     dtype = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}[a.dtype]
-    losses, ms = train(a.scenes, a.voxels, a.classes, a.steps, a.state_bits, dtype)
-    print(json.dumps({"scenes": a.scenes, "voxels_per_scene": a.voxels, "classes": a.classes, "state_bits": a.state_bits, "dtype": a.dtype,
+    losses, ms = train(a.scenes, a.voxels, a.classes, a.steps, a.state_bits, dtype, blocks=a.blocks)
+    print(json.dumps({"scenes": a.scenes, "voxels_per_scene": a.voxels, "classes": a.classes, "state_bits": a.state_bits, "dtype": a.dtype, "blocks": a.blocks,
                       "first_loss": round(losses[0], 4), "last_loss": round(losses[-1], 4), "ms_per_step": round(ms, 3)}))
 
 

@@ -1,4 +1,4 @@
-"""Normalisations over geometry features: BatchNorm (warpconvnet/nn/modules/normalizations.py:49-63) and group norm per scene."""
+"""Normalisations over geometry features: BatchNorm (warpconvnet/nn/modules/normalizations.py:49-63), group norm per scene and RMS norm."""
 from typing import Optional
 
 import torch
@@ -6,6 +6,7 @@ import torch.nn as nn
 
 from ...geometry.base.geometry import Geometry
 from ..functional.group_norm import check_activation, segmented_group_norm
+from ..functional.rms_norm import check_eps, rms_norm
 from ..functional.transforms import apply_feature_transform
 from .base_module import BaseSpatialModule
 
@@ -42,3 +43,23 @@ class SegmentedGroupNorm(BaseSpatialModule):
     def forward(self, input: Geometry):
         return apply_feature_transform(input, lambda x: segmented_group_norm(x, input.offsets, self.num_groups, self.weight, self.bias,
                                                                               self.eps, self.activation))
+
+
+class RMSNorm(BaseSpatialModule):
+    """Root-mean-square norm of each row of a geometry's features.  With a second geometry of the same coordinates, the residual, it
+    gives ``(norm, sum)``: the norm of the sum, and the sum."""
+
+    def __init__(self, num_channels: int, eps: float = 1e-6, affine: bool = True):
+        super().__init__()
+        check_eps(eps)
+        self.num_channels, self.eps = num_channels, eps
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+
+    def extra_repr(self):
+        return f"{self.num_channels}, eps={self.eps}, affine={self.weight is not None}"
+
+    def forward(self, input: Geometry, residual: Optional[Geometry] = None):
+        if residual is None:
+            return apply_feature_transform(input, lambda x: rms_norm(x, self.weight, self.eps))
+        y, h = rms_norm(input.feature_tensor, self.weight, self.eps, residual.feature_tensor)
+        return input.replace(batched_features=y), input.replace(batched_features=h)
