@@ -112,7 +112,7 @@ SIGNATURES = {
     "wcn_quantize_rows": [_c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp, _c_vp, _c_vp],
     "wcn_dropout": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_vp, _c_vp, _c_vp],
     "wcn_linear": [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_i64, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_i32, _c_i64, _c_vp, _c_vp,
-                   _c_vp, _c_vp],
+                   _c_vp, _c_i64, _c_vp, _c_vp],
     "wcn_linear_8bit": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_i64, _c_vp, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_vp, _c_vp,
                         _c_vp],
     "wcn_linear_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _p_i64],

@@ -6,8 +6,8 @@
 // workspace, in pieces of rows that stay in L2; each piece is multiplied by W (dx) and by x (dW), whose sums over the rows are divided
 // among the multiprocessors and joined in a fixed order and in double: the same bits on every run.
 //
-// 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 on the
-// FMA pipes here, in tiles of 64 x 64.
+// 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 there too
+// as sums of three bf16 numbers (linear_split_tcgen05.cu), small problems on the FMA pipes here, in tiles of 64 x 64.
 #include "fp32_tile.cuh"
 #include "linear.cuh"
 #include "linear_ce.cuh"
@@ -15,6 +15,11 @@
 int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st);
 int wcn_dropout_rows(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, int64_t n, int c, int dtype, const wcn_drop& drop, int64_t row0, void* y,
                      int64_t y_ld, cudaStream_t st);
+int64_t wcn_linear_parts_bytes(int64_t rows, int cols);
+int wcn_linear_parts(const wcn_linear_matrix* m, int count, cudaStream_t st);
+int wcn_linear_split(const wcn_linear_product& q, bool by_k, const void* a_planes, const void* b_planes, int32_t* dev_status, cudaStream_t st);
+int wcn_linear_split_weight(const wcn_ce_product& c, const void* a_planes, const void* b_planes, int32_t* dev_status, cudaStream_t st);
+int wcn_linear_split_splits(int m, int n, int k);
 int wcn_ce_product_splits(int m, int n, int k, bool blocked, bool ones);
 int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, int dtype, int32_t* dev_status, cudaStream_t st);
 
@@ -127,7 +132,7 @@ struct JoinParams {
   void* db;                 // [m]; null: not wanted
   int m, n, ld, splits;
   int quads;                // blocks for dw
-  const int32_t* dev_status;   // null: nothing before this waits (fp32)
+  const int32_t* dev_status;   // null: nothing before this waits (the FMA pipes)
 };
 
 constexpr int SIDE = 8;     // threads that share the splits
@@ -183,41 +188,59 @@ int join(JoinParams p, int dtype, cudaStream_t st) {
 
 // ------------------------------------------------------------------ plans
 
-int run(const wcn_linear_product& q, int dtype, bool by_k, int32_t* dev_status, cudaStream_t st) {
-  return dtype == WCN_F32 ? fp32_run(q, by_k, st) : wcn_linear_run(q, dtype, dtype == WCN_BF16, by_k, dev_status, st);
+// fp32 on the tensor cores, as sums of three bf16 numbers: where the products are worth the launch that makes the parts.
+constexpr int64_t SPLIT_WORK = 1ll << 22;
+bool in_parts(int64_t n, int k, int m, int dtype) { return dtype == WCN_F32 && n * k * m >= SPLIT_WORK; }
+
+int run(const wcn_linear_product& q, int dtype, bool by_k, const void* a_planes, const void* b_planes, int32_t* dev_status, cudaStream_t st) {
+  if (dtype != WCN_F32) return wcn_linear_run(q, dtype, dtype == WCN_BF16, by_k, dev_status, st);
+  return a_planes ? wcn_linear_split(q, by_k, a_planes, b_planes, dev_status, st) : fp32_run(q, by_k, st);
 }
-int weight_splits(int m, int k, int rows, int dtype, bool bias) {
+int weight_splits(int m, int k, int rows, int dtype, bool bias, bool parts) {
+  if (parts) return wcn_linear_split_splits(m, k, rows);
   return dtype == WCN_F32 ? fp32_splits(m, k, rows) : wcn_ce_product_splits(m, k, rows, false, bias);
 }
 
-// The pieces of rows that dz is made in, and the workspace: dz of a piece, sums of dW and of dbias.
+// The pieces of rows that dz is made in (forward: that x's parts are made in), and the workspace: dz of a piece, parts of x, dz and w, sums
+// of dW and of dbias.
 struct Pieces {
   int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
-  int64_t dz_ld, slab, ones, bytes;
+  bool parts;
+  int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
-enum Want { DX = 1, DW = 2, DB = 4 };
+enum Want { DX = 1, DW = 2, DB = 4 };     // none of them: forward
 Pieces plan(int64_t n, int k, int m, int dtype, int what, bool direct) {
   Pieces p = {};
   const int64_t e = wcn_dtype_size(dtype);
   auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
   p.dz_ld = round(m, 16 / e);
-  // (a gradient that dz is the same as needs no pieces)
-  int64_t rows = direct ? n : PIECE_BYTES / (p.dz_ld * e) / 128 * 128;
+  p.parts = in_parts(n, k, m, dtype);
+  const bool weights = what & (DW | DB), makes_dz = what && !direct;
+  const bool of_x = p.parts && (!what || makes_dz || weights), of_dz = p.parts && what, of_w = p.parts && (!what || makes_dz || (what & DX));
+  const int64_t each = (makes_dz ? p.dz_ld * e : 0) + (of_x ? round(k, 8) * 6 : 0) + (of_dz ? round(m, 8) * 6 : 0);   // bytes of a row of a piece
+  int64_t rows = each ? PIECE_BYTES / each / 128 * 128 : n;
   if (rows < 1024) rows = 1024;
   const int64_t count = (n + rows - 1) / rows;
   rows = round((n + count - 1) / count, 128);
   p.rows = (int)(rows < n ? rows : n);
   p.count = (int)((n + p.rows - 1) / p.rows);
-  int64_t at = direct ? 0 : round(p.rows * p.dz_ld * e, 128);
-  if (what & (DW | DB)) {
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round(bytes, 128);
+    return here;
+  };
+  take(makes_dz ? p.rows * p.dz_ld * e : 0);
+  p.x_parts = take(of_x ? wcn_linear_parts_bytes(p.rows, k) : 0);
+  p.dz_parts = take(of_dz ? wcn_linear_parts_bytes(p.rows, m) : 0);
+  p.w_parts = take(of_w ? wcn_linear_parts_bytes(m, k) : 0);
+  if (weights) {
     const int last = (int)(n - (int64_t)(p.count - 1) * p.rows);
-    p.splits = weight_splits(m, k, p.rows, dtype, what & DB);
-    p.last_splits = weight_splits(m, k, last, dtype, what & DB);
+    p.splits = weight_splits(m, k, p.rows, dtype, what & DB, p.parts);
+    p.last_splits = weight_splits(m, k, last, dtype, what & DB, p.parts);
     const int64_t all = (int64_t)p.splits * (p.count - 1) + p.last_splits;
-    p.slab = at;
-    at += all * m * wcn_ce_round(k, 16) * 4;
-    p.ones = at;
-    if (what & DB) at += round(all * m * 4, 16);
+    p.slab = take(all * m * wcn_ce_round(k, 16) * 4);
+    p.ones = take(what & DB ? all * m * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -233,16 +256,33 @@ bool rows_taken(const void* p, int64_t ld, int64_t rows, int columns, int size) 
 
 extern "C" int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype, const void* bias,
                           int act, const void* residual, int64_t residual_ld, int32_t least, int64_t seed, const int64_t* seed_at, void* y,
-                          int32_t* dev_status, void* stream) {
+                          void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream) {
   wcn_launched = 0;
   if (!sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || act < 0 || act > 3 || least < 0 || least > 65536) return WCN_ERR_INVALID_PARAMETERS;
   if (n == 0) return WCN_OK;
   const int size = wcn_dtype_size(dtype);
   if (!rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !y || !dev_status || (residual && n > 1 && residual_ld < m))
     return WCN_ERR_INVALID_PARAMETERS;
+  cudaStream_t st = wcn_stream(stream);
   wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, y, m, bias, act, false, residual, residual_ld,
                           wcn_make_drop((uint32_t)least, seed, seed_at), 0};
-  return run(q, dtype, false, dev_status, wcn_stream(stream));
+  if (!in_parts(n, k, m, dtype)) return run(q, dtype, false, nullptr, nullptr, dev_status, st);
+  const Pieces p = plan(n, k, m, dtype, 0, false);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes) return WCN_ERR_INVALID_PARAMETERS;
+  char* const ws = reinterpret_cast<char*>(workspace);
+  for (int i = 0; i < p.count; ++i) {
+    const int64_t r0 = (int64_t)i * p.rows;
+    q.m = (int)(n - r0 < p.rows ? n - r0 : p.rows);
+    q.a = (const float*)x + r0 * x_ld;
+    q.out = (float*)y + r0 * m;
+    q.add = residual ? (const float*)residual + r0 * residual_ld : nullptr;
+    q.row0 = r0;
+    const wcn_linear_matrix of[2] = {{(const float*)q.a, ws + p.x_parts, q.m, x_ld, k}, {(const float*)w, ws + p.w_parts, m, w_ld, k}};
+    int rc = wcn_linear_parts(of, i ? 1 : 2, st);
+    if (rc == WCN_OK) rc = run(q, dtype, false, ws + p.x_parts, ws + p.w_parts, dev_status, st);
+    if (rc != WCN_OK) return rc;
+  }
+  return WCN_OK;
 }
 
 extern "C" int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale, int64_t n, int32_t k, const void* w, int64_t w_ld,
@@ -258,8 +298,8 @@ extern "C" int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale
 }
 
 extern "C" int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int32_t direct, int64_t* bytes) {
-  if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 1 || what > 7) return WCN_ERR_INVALID_PARAMETERS;
-  *bytes = plan(n, k, m, dtype, what, direct).bytes;
+  if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 0 || what > 7) return WCN_ERR_INVALID_PARAMETERS;
+  *bytes = what || in_parts(n, k, m, dtype) ? plan(n, k, m, dtype, what, direct).bytes : 0;
   return WCN_OK;
 }
 
@@ -278,22 +318,35 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   cudaStream_t st = wcn_stream(stream);
   const wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at), none = wcn_make_drop(0, 0, nullptr);
   const int ld = wcn_ce_round(k, 16);
+  char *const xs = p.parts ? ws + p.x_parts : nullptr, *const dzs = p.parts ? ws + p.dz_parts : nullptr, *const wsp = p.parts ? ws + p.w_parts : nullptr;
   for (int i = 0; i < p.count; ++i) {
     const int64_t r0 = (int64_t)i * p.rows;
     const int rows = (int)(n - r0 < p.rows ? n - r0 : p.rows);
     const char *const xp = (const char*)x + r0 * x_ld * size, *const dyp = (const char*)dy + r0 * dy_ld * size;
-    const void* dz = dyp;
-    int64_t dz_ld = dy_ld;
+    const void* dz = direct ? (const void*)dyp : (const void*)ws;
+    const int64_t dz_ld = direct ? dy_ld : p.dz_ld;
+    int rc = WCN_OK;
+    if (p.parts) {   // of what is there already
+      wcn_linear_matrix of[3];
+      int count = 0;
+      if (!direct || dw || db) of[count++] = {(const float*)xp, xs, rows, x_ld, k};
+      if (i == 0 && (!direct || dx)) of[count++] = {(const float*)w, wsp, m, w_ld, k};
+      if (direct) of[count++] = {(const float*)dyp, dzs, rows, dy_ld, m};
+      if (count) rc = wcn_linear_parts(of, count, st);
+      if (rc != WCN_OK) return rc;
+    }
     if (!direct) {
       wcn_linear_product q = {xp, w, x_ld, w_ld, rows, m, k, nullptr, nullptr, ws, p.dz_ld, bias, act, true, dyp, dy_ld, drop, r0};
-      const int rc = act ? run(q, dtype, false, dev_status, st) : wcn_dropout_rows(dyp, dy_ld, nullptr, 0, rows, m, dtype, drop, r0, ws, p.dz_ld, st);
+      rc = act ? run(q, dtype, false, xs, wsp, dev_status, st) : wcn_dropout_rows(dyp, dy_ld, nullptr, 0, rows, m, dtype, drop, r0, ws, p.dz_ld, st);
+      if (rc == WCN_OK && p.parts) {
+        const wcn_linear_matrix of = {(const float*)ws, dzs, rows, p.dz_ld, m};
+        rc = wcn_linear_parts(&of, 1, st);
+      }
       if (rc != WCN_OK) return rc;
-      dz = ws;
-      dz_ld = p.dz_ld;
     }
     if (dx) {
       wcn_linear_product q = {dz, w, dz_ld, w_ld, rows, k, m, nullptr, nullptr, (char*)dx + r0 * k * size, k, nullptr, WCN_ACT_NONE, false, nullptr, 0, none, 0};
-      const int rc = run(q, dtype, true, dev_status, st);
+      rc = run(q, dtype, true, dzs, wsp, dev_status, st);
       if (rc != WCN_OK) return rc;
     }
     if (dw || db) {
@@ -303,18 +356,20 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
       q.splits = i + 1 < p.count ? p.splits : p.last_splits;
       q.slab = (float*)(ws + p.slab) + (int64_t)i * p.splits * m * ld;
       q.slab_ones = db ? (float*)(ws + p.ones) + (int64_t)i * p.splits * m : nullptr;
-      if (dtype == WCN_F32) {
+      if (p.parts) {
+        rc = wcn_linear_split_weight(q, dzs, xs, dev_status, st);
+      } else if (dtype == WCN_F32) {
         const int chains = (rows + CHAIN - 1) / CHAIN, per = (chains + q.splits - 1) / q.splits * CHAIN;
         linear_fp32_weight_kernel<<<dim3((m + TILE - 1) / TILE, (k + TILE - 1) / TILE, q.splits), THREADS, 0, st>>>(q, per);
         ++wcn_launched;
-        if (cudaGetLastError() != cudaSuccess) return WCN_ERR_EXECUTION;
+        if (cudaGetLastError() != cudaSuccess) rc = WCN_ERR_EXECUTION;
       } else {
-        const int rc = wcn_ce_product_run(q, true, false, dtype, dev_status, st);
-        if (rc != WCN_OK) return rc;
+        rc = wcn_ce_product_run(q, true, false, dtype, dev_status, st);
       }
+      if (rc != WCN_OK) return rc;
     }
   }
   if (!dw && !db) return WCN_OK;
   return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0,
-               dtype == WCN_F32 ? nullptr : dev_status}, dtype, st);
+               dtype == WCN_F32 && !p.parts ? nullptr : dev_status}, dtype, st);
 }

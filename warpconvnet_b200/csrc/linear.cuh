@@ -23,3 +23,11 @@ struct wcn_linear_product {
   wcn_drop drop;
   int64_t row0;             // place of the first row among all rows (for what is dropped)
 };
+
+// An fp32 matrix and where its parts go (linear_split_tcgen05.cu).
+struct wcn_linear_matrix {
+  const float* x;
+  void* planes;
+  int64_t rows, ld;
+  int cols;
+};

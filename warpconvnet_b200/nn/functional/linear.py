@@ -45,9 +45,12 @@ def _forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: int, residu
     if residual is not None:
         residual, res_ld = _rows(residual)
     number, at = _seed_arguments(seed)
+    code = dtype_code(x.dtype)
+    size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, 0, 0) if code == WCN_F32 else 0
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with on_device(dev):
-        check(lib().wcn_linear(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, dtype_code(x.dtype), ptr(bias), act, ptr(residual), res_ld, least, number, at,
-                               ptr(y), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear")
+        check(lib().wcn_linear(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, code, ptr(bias), act, ptr(residual), res_ld, least, number, at,
+                               ptr(y), ptr(ws), size, ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear")
         count_training_launches("wcn_linear")
     return y, x, weight
 
