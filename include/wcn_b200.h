@@ -691,7 +691,7 @@ int wcn_dropout(const void* x, int64_t x_ld, const void* residual, int64_t resid
  * none).  In 16 bits the rows of x and w are 16-byte aligned and their distances multiples of 8, in 8 bits of 16.
  * wcn_linear_8bit: x and w e4m3 with a scale a row (wcn_quantize_rows), the others of out_dtype (16 bits), no dropout.
  * backward: gradients of x (contiguous), of w [m, k] and of the bias, each of dtype and each of which may be NULL; the residual's is dy.
- * workspace: 32-byte aligned; `what` of the query: 0 forward (0 bytes in 16 bits and for small problems: may be NULL), else the sum of 1 (dx),
+ * workspace: 32-byte aligned; `what` of the query: 0 forward (0 bytes in 16 bits: may be NULL), else the sum of 1 (dx),
  * 2 (dw), 4 (dbias); direct: neither activation nor dropout, and the rows of dy lie as those of x do.
  * At most 32768 inputs, 2^20 outputs, 2^31 - 257 rows.  The reference has nn.Linear and its neighbours
  * (warpconvnet/nn/modules/mlp.py). */

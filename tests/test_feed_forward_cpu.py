@@ -56,3 +56,35 @@ def test_codes_and_dropout_refuse():
     drop = lambda n=4, c=8, ld=8, least=5, dtype=0, y=BASE, res=None, res_ld=0: _native.lib().wcn_dropout(BASE, ld, res, res_ld, n, c, dtype, least, 1, None, y, None)   # noqa: E731
     assert drop(n=0) == 0
     assert all(drop(**b) == INVALID for b in (dict(n=-1), dict(c=0), dict(ld=7), dict(least=-1), dict(least=65537), dict(dtype=5), dict(y=None), dict(res=BASE, res_ld=3)))
+
+
+def layer(n=4, k=8, m=16, dtype=_native.WCN_BF16, act=0, x=BASE, x_ld=8, w_ld=8, y=BASE, least=0, res=None, res_ld=0, ws=None, size=0, status=BASE):
+    return _native.lib().wcn_linear(x, x_ld, n, k, BASE, w_ld, m, dtype, None, act, res, res_ld, least, 1, None, y, ws, size, status, None)
+
+
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=2 ** 31), dict(k=0), dict(k=32769), dict(m=0), dict(m=2 ** 20 + 1), dict(dtype=7), dict(act=4), dict(act=-1), dict(x=None),
+                                 dict(x=BASE + 2), dict(x_ld=12), dict(x_ld=0), dict(w_ld=4), dict(y=None), dict(least=65537), dict(res=BASE, res_ld=15), dict(status=None),
+                                 dict(dtype=_native.WCN_F32), dict(dtype=_native.WCN_F32, ws=BASE + 16, size=1 << 40), dict(dtype=_native.WCN_F32, ws=BASE, size=100)])
+def test_linear_refuses(bad):
+    assert layer(**bad) == INVALID
+    assert layer(n=0) == 0
+
+
+def test_linears_gradient_and_codes_refuse():
+    def gradient(n=100, k=64, m=40, dtype=_native.WCN_BF16, act=1, ws=BASE, less=0, what=7, dy=BASE, dy_ld=40, x_ld=64):
+        size = _native.query_bytes("wcn_linear_workspace_bytes", 100, 64, 40, dtype, 7, 0)
+        out = [BASE if what >> i & 1 else None for i in range(3)]
+        return _native.lib().wcn_linear_backward(BASE, x_ld, n, k, BASE, 64, m, dtype, None, act, dy, dy_ld, 0, 0, None, *out, ws, size - less, BASE, None)
+    for dtype in (_native.WCN_F32, _native.WCN_F16, _native.WCN_BF16):
+        for bad in (dict(n=0), dict(act=9), dict(ws=None), dict(ws=BASE + 16), dict(less=1), dict(what=0), dict(dy=None), dict(dy_ld=39), dict(x_ld=63)):
+            assert gradient(dtype=dtype, **bad) == INVALID
+    eight = lambda x_ld=16, w_ld=16, out=_native.WCN_F16, scale=BASE, n=4, k=16: _native.lib().wcn_linear_8bit(   # noqa: E731
+        BASE, x_ld, scale, n, k, BASE, w_ld, BASE, 8, out, None, 0, None, 0, BASE, BASE, None)
+    assert eight(n=0) == 0
+    assert all(eight(**b) == INVALID for b in (dict(x_ld=8), dict(w_ld=24), dict(out=_native.WCN_F32), dict(scale=None), dict(k=0)))
+    out = ctypes.c_int64()
+    for args in ((0, 8, 8, 1, 1, 0), (10, 0, 8, 1, 1, 0), (10, 8, 8, 5, 1, 0), (10, 8, 8, 1, 8, 0)):
+        assert _native.lib().wcn_linear_workspace_bytes(*args, ctypes.byref(out)) == INVALID
+    # the gradient behind the activation in pieces of 512 MB: whatever the rows are, the workspace stays bounded
+    for dtype in (_native.WCN_F32, _native.WCN_BF16):
+        assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 257, 64, 256, dtype, 1, 0) <= (512 << 20) + (1 << 20)

@@ -18,6 +18,11 @@ def half(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def normal64(z):
+    """(torch.special.ndtr gives 0 on a GPU from -8.34 on, where it is 3.6e-17.)"""
+    return 0.5 * torch.special.erfc(z * -0.5 ** 0.5)
+
+
 def act64(z, act):
     """act(z) and its derivative."""
     one = torch.ones_like(z)
@@ -27,7 +32,7 @@ def act64(z, act):
         s = torch.sigmoid(z)
         return z * s, s + z * s * (1 - s)
     if act == "gelu":
-        p = torch.special.ndtr(z)
+        p = normal64(z)
         return z * p, p + z * torch.exp(-z * z / 2) * 0.3989422804014327
     return z, one
 
@@ -332,7 +337,51 @@ class expired:
         device_status(DEV).zero_()
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_fp32_numbers_of_every_size():
+    """Numbers without three bf16 parts (2^39 and more, infinities), small ones and subnormal ones: as others in their rows and columns."""
+    g = torch.Generator().manual_seed(0)
+    n, k, m = 400, 70, 50
+    x, w = torch.randn(n, k, generator=g), torch.randn(m, k, generator=g) / 8
+    x[3] *= 1e20
+    x[200, 7] = 3e30
+    x[5] *= 1e-30
+    x[6] *= 1e-42
+    w[9] *= 1e25
+    dy = torch.randn(n, m, generator=g)
+    dy[11] *= 1e15
+    lx, lw = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    y = linear(lx, lw)
+    dx, dw = torch.autograd.grad(y, [lx, lw], dy.to(DEV))
+    X, W, D = x.double(), w.double(), dy.double()
+    for got, want, terms, c in ((y, X @ W.t(), X.abs() @ W.t().abs(), k), (dx, D @ W, D.abs() @ W.abs(), m), (dw, D.t() @ X, D.t().abs() @ X.abs(), n)):
+        got = got.detach().cpu()
+        big = terms > 1e38
+        assert not torch.isnan(got[~big]).any()
+        d = (got.double() - want).abs()
+        assert (d <= half(torch.float32) * want.abs() + sums(c, terms, torch.float32) + 2.0 ** -149 * c)[~big].all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_fp32_activations_over_their_whole_range(act):
+    z = torch.cat([torch.linspace(-20, 20, 8001), torch.logspace(-6, 4, 300), -torch.logspace(-6, 4, 300)]).to(DEV)
+    x, w = torch.zeros(1, 8, device=DEV), torch.zeros(len(z), 8, device=DEV)
+    b = z.clone().requires_grad_(True)
+    y = linear(x, w, b, act)
+    slope_got, = torch.autograd.grad(y, [b], torch.ones_like(y))
+    value, slope = act64(z.double(), act)
+    within(y[0].detach(), value, 16 * U * value.abs() + 1e-37)
+    # the slope is f + z f' of the function f that z is multiplied by, which for negative z is a difference: each term is some roundings
+    # (of an exponential, a reciprocal, a polynomial, products) off in itself, and the result may be any part of them
+    Z = z.double()
+    p = torch.sigmoid(Z) if act == "silu" else normal64(Z)
+    terms = p + Z.abs() * (p * torch.sigmoid(-Z) if act == "silu" else torch.exp(-Z * Z / 2) * 0.3989422804014327)
+    within(slope_got, slope, 24 * U * terms + 1e-37)
+    odd = torch.tensor([float("inf"), float("nan")], device=DEV)
+    y = linear(x, w[:2], odd, act)
+    assert float(y[0, 0]) == float("inf") and torch.isnan(y[0, 1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,k,m", [(300, 96, 200), (1, 64, 40), (3000, 1024, 264), (130, 40, 33)])
 def test_where_an_earlier_kernel_gave_up_waiting(dtype, n, k, m):
     x, w, b, r, dy = make(n, k, m, dtype)

@@ -13,7 +13,7 @@ SOURCES = ["api.cu", "hash_kmap.cu", "brick_kmap.cu", "cell_kmap.cu", "morton_so
            "conv_wgrad_tcgen05.cu", "conv_wgrad_split_tcgen05.cu", "conv_wgrad_pairs.cu", "conv_rows_tcgen05.cu",
            "adamw.cu", "group_norm.cu", "linear_ce.cu", "linear_ce_tcgen05.cu",
            "rms_norm.cu", "dropout.cu", "linear.cu", "linear_tcgen05.cu", "linear_split_tcgen05.cu"]
-HEADERS = ["wcn_common.cuh", "tile_order.cuh", "tcgen05_common.cuh", "split_bf16.cuh", "tma_common.cuh", "linear_ce.cuh", "philox.cuh", "fp32_tile.cuh", "linear.cuh", os.path.join("..", "..", "include", "wcn_b200.h")]
+HEADERS = ["wcn_common.cuh", "tile_order.cuh", "tcgen05_common.cuh", "split_bf16.cuh", "tma_common.cuh", "linear_ce.cuh", "philox.cuh", "linear.cuh", "linear_fp32.cuh", os.path.join("..", "..", "include", "wcn_b200.h")]
 LIB = os.path.join(HERE, "libwcn_b200.so")
 FASTCALL_SOURCE, FASTCALL = os.path.join(HERE, "fastcall.c"), os.path.join(HERE, "_fastcall.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -7,8 +7,9 @@
 // among the multiprocessors and joined in a fixed order and in double: the same bits on every run.
 //
 // 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 there too
-// as sums of three bf16 numbers (linear_split_tcgen05.cu), small problems on the FMA pipes here, in tiles of 64 x 64.
-#include "fp32_tile.cuh"
+// as sums of three bf16 numbers (linear_split_tcgen05.cu).  On the FMA pipes in tiles of 64 x 64 fp32 took as long for the smallest problems
+// and up to four times as long for others (us forward, gradients: 500 x 64 -> 64 18, 51 and here 17, 35; 20 000 x 32 -> 32 16, 53 and 19,
+// 40; 100 000 x 96 -> 200 251, 608 and 85, 174).
 #include "linear.cuh"
 #include "linear_ce.cuh"
 
@@ -25,103 +26,9 @@ int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, i
 
 namespace {
 
-constexpr int THREADS = FP32_THREADS;
+constexpr int THREADS = 256;
 constexpr int MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;
 constexpr int64_t PIECE_BYTES = 512ll << 20;   // of dz
-
-// ------------------------------------------------------------------ fp32
-
-__device__ __forceinline__ float activate(int act, float z) {
-  switch (act) {
-    case WCN_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case WCN_ACT_SILU: return z / (1.f + expf(-z));
-    case WCN_ACT_GELU: return z * normcdff(z);
-    default: return z;
-  }
-}
-// dy act'(z)
-__device__ __forceinline__ float through(int act, float dy, float z) {
-  switch (act) {
-    case WCN_ACT_RELU: return z > 0.f ? dy : 0.f;
-    case WCN_ACT_SILU: {
-      const float p = 1.f / (1.f + expf(-z));
-      return dy * (p * (1.f + z * (1.f - p)));
-    }
-    case WCN_ACT_GELU: return dy * (normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z)));
-    default: return dy;
-  }
-}
-
-__device__ __forceinline__ bool kept(const wcn_drop& d, uint64_t seed, int64_t row, int col) {
-  const uint4 w = philox_eight(philox_keys(seed), (uint32_t)col / 8, (uint64_t)row);
-  const int at = col % 8 / 2;
-  const uint32_t word = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
-  return (col & 1 ? word >> 16 : word & 0xFFFFu) >= d.least;
-}
-
-template <int LAYOUT>
-__global__ void __launch_bounds__(THREADS) linear_fp32_kernel(const __grid_constant__ wcn_linear_product q) {
-  const int m_tiles = (q.m + TILE - 1) / TILE;
-  const int m0 = (int)(blockIdx.x % m_tiles) * TILE, n0 = (int)(blockIdx.x / m_tiles) * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float z[4][4], unused[4];
-  fp32_tile<LAYOUT>((const float*)q.a, q.a_ld, (const float*)q.b, q.b_ld, m0, n0, q.m, q.n, 0, q.k, z, unused);
-  const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
-  const float* const add = (const float*)q.add;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + ty * 4 + i;
-    if (row >= q.m) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + tx * 4 + j;
-      if (col >= q.n) continue;
-      float v = z[i][j];
-      if (q.bias) v += __ldg((const float*)q.bias + col);
-      const bool keep = !q.drop.least || kept(q.drop, seed, q.row0 + row, col);
-      const float by = q.drop.least ? q.drop.scale : 1.f;
-      if (q.grad) {
-        const float g = __ldg(add + row * q.add_ld + col);
-        v = through(q.act, keep ? g * by : 0.f, v);
-      } else {
-        v = activate(q.act, v);
-        v = keep ? v * by : 0.f;
-        if (add) v += __ldg(add + row * q.add_ld + col);
-      }
-      reinterpret_cast<float*>(q.out)[row * q.out_ld + col] = v;
-    }
-  }
-}
-
-int fp32_run(const wcn_linear_product& q, bool by_k, cudaStream_t st) {
-  const int64_t tiles = (int64_t)((q.m + TILE - 1) / TILE) * ((q.n + TILE - 1) / TILE);
-  if (by_k) linear_fp32_kernel<ROWS_BY_CLASSES><<<(unsigned)tiles, THREADS, 0, st>>>(q);
-  else linear_fp32_kernel<LOGITS><<<(unsigned)tiles, THREADS, 0, st>>>(q);
-  ++wcn_launched;
-  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
-}
-
-// The sums over a part of the rows of dz^T x, and of dz.
-__global__ void __launch_bounds__(THREADS) linear_fp32_weight_kernel(const __grid_constant__ wcn_ce_product q, int per) {
-  const int m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE, split = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float d[4][4], sums[4];
-  fp32_tile<CLASSES_BY_ROWS>((const float*)q.a, q.a_ld, (const float*)q.b, q.b_ld, m0, n0, q.m, q.n, split * per, min((split + 1) * per, q.k), d, sums);
-  const int ld = wcn_ce_round(q.n, 16);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + ty * 4 + i;
-    if (row >= q.m) continue;
-    if (n0 + tx * 4 < ld)
-      *reinterpret_cast<float4*>(q.slab + ((int64_t)split * q.m + row) * ld + n0 + tx * 4) = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
-    if (q.slab_ones && n0 == 0 && tx == 0) q.slab_ones[(int64_t)split * q.m + row] = sums[i];
-  }
-}
-
-int fp32_splits(int m, int n, int k) {
-  const int64_t tiles = (int64_t)((m + TILE - 1) / TILE) * ((n + TILE - 1) / TILE), want = (4 * (int64_t)wcn_num_sms() + tiles - 1) / tiles;
-  const int chains = (k + CHAIN - 1) / CHAIN;
-  const int s = (int)(want < chains ? want : chains), per = (chains + s - 1) / s;
-  return (chains + per - 1) / per;
-}
 
 // ------------------------------------------------------------------ sums of the splits
 
@@ -132,7 +39,7 @@ struct JoinParams {
   void* db;                 // [m]; null: not wanted
   int m, n, ld, splits;
   int quads;                // blocks for dw
-  const int32_t* dev_status;   // null: nothing before this waits (the FMA pipes)
+  const int32_t* dev_status;
 };
 
 constexpr int SIDE = 8;     // threads that share the splits
@@ -161,7 +68,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) linear_join_ker
   for (int s = 1; s < SIDE; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += part[s][at][j];
-  const bool failed = p.dev_status && *p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
+  const bool failed = *p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
   const float nan = __int_as_float(0x7FC00000);
   if (!of_w) {
     reinterpret_cast<T*>(p.db)[i] = wcn_from_float<T>(failed ? nan : (float)v[0]);
@@ -188,24 +95,19 @@ int join(JoinParams p, int dtype, cudaStream_t st) {
 
 // ------------------------------------------------------------------ plans
 
-// fp32 on the tensor cores, as sums of three bf16 numbers: where the products are worth the launch that makes the parts.
-constexpr int64_t SPLIT_WORK = 1ll << 22;
-bool in_parts(int64_t n, int k, int m, int dtype) { return dtype == WCN_F32 && n * k * m >= SPLIT_WORK; }
-
 int run(const wcn_linear_product& q, int dtype, bool by_k, const void* a_planes, const void* b_planes, int32_t* dev_status, cudaStream_t st) {
   if (dtype != WCN_F32) return wcn_linear_run(q, dtype, dtype == WCN_BF16, by_k, dev_status, st);
-  return a_planes ? wcn_linear_split(q, by_k, a_planes, b_planes, dev_status, st) : fp32_run(q, by_k, st);
+  return wcn_linear_split(q, by_k, a_planes, b_planes, dev_status, st);
 }
-int weight_splits(int m, int k, int rows, int dtype, bool bias, bool parts) {
-  if (parts) return wcn_linear_split_splits(m, k, rows);
-  return dtype == WCN_F32 ? fp32_splits(m, k, rows) : wcn_ce_product_splits(m, k, rows, false, bias);
+int weight_splits(int m, int k, int rows, int dtype, bool bias) {
+  return dtype == WCN_F32 ? wcn_linear_split_splits(m, k, rows) : wcn_ce_product_splits(m, k, rows, false, bias);
 }
 
 // The pieces of rows that dz is made in (forward: that x's parts are made in), and the workspace: dz of a piece, parts of x, dz and w, sums
 // of dW and of dbias.
 struct Pieces {
   int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
-  bool parts;
+  bool parts;                             // fp32: the operands are sums of three bf16 numbers
   int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
 enum Want { DX = 1, DW = 2, DB = 4 };     // none of them: forward
@@ -214,7 +116,7 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, bool direct) {
   const int64_t e = wcn_dtype_size(dtype);
   auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
   p.dz_ld = round(m, 16 / e);
-  p.parts = in_parts(n, k, m, dtype);
+  p.parts = dtype == WCN_F32;
   const bool weights = what & (DW | DB), makes_dz = what && !direct;
   const bool of_x = p.parts && (!what || makes_dz || weights), of_dz = p.parts && what, of_w = p.parts && (!what || makes_dz || (what & DX));
   const int64_t each = (makes_dz ? p.dz_ld * e : 0) + (of_x ? round(k, 8) * 6 : 0) + (of_dz ? round(m, 8) * 6 : 0);   // bytes of a row of a piece
@@ -236,8 +138,8 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, bool direct) {
   p.w_parts = take(of_w ? wcn_linear_parts_bytes(m, k) : 0);
   if (weights) {
     const int last = (int)(n - (int64_t)(p.count - 1) * p.rows);
-    p.splits = weight_splits(m, k, p.rows, dtype, what & DB, p.parts);
-    p.last_splits = weight_splits(m, k, last, dtype, what & DB, p.parts);
+    p.splits = weight_splits(m, k, p.rows, dtype, what & DB);
+    p.last_splits = weight_splits(m, k, last, dtype, what & DB);
     const int64_t all = (int64_t)p.splits * (p.count - 1) + p.last_splits;
     p.slab = take(all * m * wcn_ce_round(k, 16) * 4);
     p.ones = take(what & DB ? all * m * 4 : 0);
@@ -266,7 +168,7 @@ extern "C" int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, con
   cudaStream_t st = wcn_stream(stream);
   wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, y, m, bias, act, false, residual, residual_ld,
                           wcn_make_drop((uint32_t)least, seed, seed_at), 0};
-  if (!in_parts(n, k, m, dtype)) return run(q, dtype, false, nullptr, nullptr, dev_status, st);
+  if (dtype != WCN_F32) return run(q, dtype, false, nullptr, nullptr, dev_status, st);
   const Pieces p = plan(n, k, m, dtype, 0, false);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);
@@ -299,7 +201,7 @@ extern "C" int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale
 
 extern "C" int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int32_t direct, int64_t* bytes) {
   if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 0 || what > 7) return WCN_ERR_INVALID_PARAMETERS;
-  *bytes = what || in_parts(n, k, m, dtype) ? plan(n, k, m, dtype, what, direct).bytes : 0;
+  *bytes = what || dtype == WCN_F32 ? plan(n, k, m, dtype, what, direct).bytes : 0;
   return WCN_OK;
 }
 
@@ -356,20 +258,10 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
       q.splits = i + 1 < p.count ? p.splits : p.last_splits;
       q.slab = (float*)(ws + p.slab) + (int64_t)i * p.splits * m * ld;
       q.slab_ones = db ? (float*)(ws + p.ones) + (int64_t)i * p.splits * m : nullptr;
-      if (p.parts) {
-        rc = wcn_linear_split_weight(q, dzs, xs, dev_status, st);
-      } else if (dtype == WCN_F32) {
-        const int chains = (rows + CHAIN - 1) / CHAIN, per = (chains + q.splits - 1) / q.splits * CHAIN;
-        linear_fp32_weight_kernel<<<dim3((m + TILE - 1) / TILE, (k + TILE - 1) / TILE, q.splits), THREADS, 0, st>>>(q, per);
-        ++wcn_launched;
-        if (cudaGetLastError() != cudaSuccess) rc = WCN_ERR_EXECUTION;
-      } else {
-        rc = wcn_ce_product_run(q, true, false, dtype, dev_status, st);
-      }
+      rc = p.parts ? wcn_linear_split_weight(q, dzs, xs, dev_status, st) : wcn_ce_product_run(q, true, false, dtype, dev_status, st);
       if (rc != WCN_OK) return rc;
     }
   }
   if (!dw && !db) return WCN_OK;
-  return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0,
-               dtype == WCN_F32 && !p.parts ? nullptr : dev_status}, dtype, st);
+  return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0, dev_status}, dtype, st);
 }

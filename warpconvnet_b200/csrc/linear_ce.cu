@@ -17,7 +17,6 @@
 // products at a time.  20 000 rows x 64 channels x 40 classes fp32, forward and backward: 79 us on the device in eight launches of
 // 2 to 20 us (the host's part makes that 150; 40 of a tile's 64 classes are used).  30 000 x 256 x 32 768 classes bf16 forward and
 // backward: 1.92 to 2.29 ms as the power cap sets the clock, 0.9 to 1.05 PFLOP/s of products (logits twice, dx and dw).
-#include "fp32_tile.cuh"
 #include "linear_ce.cuh"
 
 int wcn_ce_logits_parts(int rows, int classes);
@@ -34,7 +33,7 @@ int wcn_ce_rows(const wcn_ce_piece& q, float* slab, int dtype, float lift, int32
 
 namespace {
 
-constexpr int THREADS = FP32_THREADS;
+constexpr int THREADS = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
 constexpr int64_t PIECE_BYTES = 512ll << 20;   // of g
@@ -330,6 +329,64 @@ int join_both(const JoinParams& p, const JoinParams& sums, int dtype, cudaStream
 }
 
 // ------------------------------------------------------------------ fp32
+
+constexpr int TILE = 64, DEPTH = 16, CHAIN = 128;   // a chain of 128 products has a sum of its own
+
+enum Layout { LOGITS = 0, ROWS_BY_CLASSES = 1, CLASSES_BY_ROWS = 2 };   // A[m][k] B[n][k]; A[m][k] B[k][n]; A[k][m] B[k][n]
+
+// One tile of 64 x 64 sums over k in [k0, k1): a thread has rows ty * 4 .. and columns tx * 4 ..; `sums`: A's row sums (tx = 0).
+template <int LAYOUT>
+__device__ __forceinline__ void fp32_tile(const float* a, int64_t a_ld, const float* b, int64_t b_ld, int m0, int n0, int m, int n, int k0, int k1,
+                                          float (&out)[4][4], float (&sums)[4]) {
+  __shared__ __align__(16) float sa[DEPTH][TILE + 4], sb[DEPTH][TILE + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4], part[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sums[i] = part[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = out[i][j] = 0.f;
+  }
+  int chain = 0;
+  for (int k = k0; k < k1; k += DEPTH) {
+#pragma unroll
+    for (int i = threadIdx.x; i < TILE * DEPTH; i += THREADS) {
+      {
+        const int kk = LAYOUT == CLASSES_BY_ROWS ? i / TILE : i % DEPTH, r = LAYOUT == CLASSES_BY_ROWS ? i % TILE : i / DEPTH;
+        const bool in = k + kk < k1 && m0 + r < m;
+        sa[kk][r] = in ? __ldg(LAYOUT == CLASSES_BY_ROWS ? a + (int64_t)(k + kk) * a_ld + m0 + r : a + (int64_t)(m0 + r) * a_ld + k + kk) : 0.f;
+      }
+      {
+        const int kk = LAYOUT == LOGITS ? i % DEPTH : i / TILE, r = LAYOUT == LOGITS ? i / DEPTH : i % TILE;
+        const bool in = k + kk < k1 && n0 + r < n;
+        sb[kk][r] = in ? __ldg(LAYOUT == LOGITS ? b + (int64_t)(n0 + r) * b_ld + k + kk : b + (int64_t)(k + kk) * b_ld + n0 + r) : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < DEPTH; ++kk) {
+      const float4 u = *reinterpret_cast<const float4*>(&sa[kk][ty * 4]), v = *reinterpret_cast<const float4*>(&sb[kk][tx * 4]);
+      const float x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[i] += x[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+      }
+    }
+    __syncthreads();
+    if (++chain == CHAIN / DEPTH || k + DEPTH >= k1) {
+      chain = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sums[i] += part[i];
+        part[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { out[i][j] += acc[i][j]; acc[i][j] = 0.f; }
+      }
+    }
+  }
+}
 
 // A block has `per` tiles of classes side by side (GRAD: one), of which each row leaves one (largest, sum).
 template <bool GRAD>

@@ -3,14 +3,14 @@
 //
 // A first launch writes the parts of the operands, [3][rows][columns] each.  The second works through tiles of 128 rows x up to 128 columns
 // (and, of the weights' gradient, parts of the rows that are summed over): a thread issues TMA loads of 64 of k of all parts into a
-// ring, a thread the 24 matrix instructions of such a slice, small products first, into one of several accumulators; eight warps add every
-// accumulator to sums in their registers (two threads a row), since a tensor core's accumulator cuts what is below its last place
+// ring, a thread the 24 matrix instructions of such a slice, small products first, into one of several accumulators; sixteen warps add every
+// accumulator to sums in their registers (four threads a row), since a tensor core's accumulator cuts what is below its last place
 // instead of rounding it, and finish the tile.  A sum that is not finite, for a number that has no parts (infinite, not a number, 2^39 and
 // more) or for its size, is made again on the FMA pipes from the numbers as they came.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
 // and frees its tensor memory; its results, and those of a launch that finds the word set, are NaN.
-#include "linear.cuh"
+#include "linear_fp32.cuh"
 #include "linear_ce.cuh"
 #include "split_bf16.cuh"
 #include "tcgen05_common.cuh"
@@ -22,7 +22,7 @@ constexpr int TILE_M = 128, MAX_N = 128, SLICE = 64;      // rows, columns of a 
 constexpr int CHUNK = SLICE * 128;                        // 64 of k x 64 columns of an operand whose rows run along k
 constexpr int A_PLANE = TILE_M * 128;
 constexpr int MAX_STAGES = 4, MAX_ACC = 4;
-constexpr int EPI_WARP0 = 2, EPI_WARPS = 8, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+constexpr int EPI_WARP0 = 2, PARTS = 4, EPI_WARPS = 4 * PARTS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int SMEM_BUDGET = 226 * 1024;
 
 struct Params {
@@ -57,27 +57,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
-}
-
-__device__ __forceinline__ float activate(int act, float z) {
-  switch (act) {
-    case WCN_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case WCN_ACT_SILU: return z / (1.f + expf(-z));
-    case WCN_ACT_GELU: return z * normcdff(z);
-    default: return z;
-  }
-}
-// dy act'(z)
-__device__ __forceinline__ float through(int act, float dy, float z) {
-  switch (act) {
-    case WCN_ACT_RELU: return z > 0.f ? dy : 0.f;
-    case WCN_ACT_SILU: {
-      const float p = 1.f / (1.f + expf(-z));
-      return dy * (p * (1.f + z * (1.f - p)));
-    }
-    case WCN_ACT_GELU: return dy * (normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z)));
-    default: return dy;
-  }
 }
 
 // Element (row, col) on the FMA pipes, k in order; `ones`: the sum of A's row.
@@ -209,36 +188,32 @@ linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_cons
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
-    const int pieces = p.NT / 16, first = half ? (pieces + 1) / 2 : 0, mine = half ? pieces / 2 : (pieces + 1) / 2;   // of 16 columns, four at most
-    const PhiloxKeys keys = philox_keys(q.drop.least ? drop_seed(q.drop) : 0);
+    const int quarter = warp & 3, part = (warp - EPI_WARP0) >> 2;
+    const int pieces = p.NT / 16, first = pieces * part / PARTS, mine = pieces * (part + 1) / PARTS - first;   // of 16 columns, two at most
     int ab = 0, aphase = 0;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
       const int split = split_of(u), k0 = split * p.per, k1 = min(k0 + p.per, p.ksteps), n0 = n_of(u) * p.NT + first * 16;
       const int row = m_of(u) * TILE_M + quarter * 32 + lane;
-      const bool live = row < q.m, sums = with_ones && n_of(u) == 0 && half == 0;
-      float sum[64], sum_ones = 0.f;
+      const bool live = row < q.m, sums = with_ones && n_of(u) == 0 && part == 0;
+      float sum[32], sum_ones = 0.f;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sum[i] = 0.f;
+      for (int i = 0; i < 32; ++i) sum[i] = 0.f;
       for (int k = k0; k < k1; ++k) {
         if (ok) ok = mbar_wait(bar(&ctl->acc_full[ab]), aphase, p.dev_status);
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
         tc_fence_after();
         const uint32_t t = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(ab * p.stride);
+        uint32_t r0[16], r1[16];
+        __syncwarp();
+        if (mine > 0) tmem_ld16(t + (uint32_t)(first * 16), r0);
+        if (mine > 1) tmem_ld16(t + (uint32_t)((first + 1) * 16), r1);
+        tmem_ld_wait();
+        if (mine > 0)
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          if (c >= mine) continue;
-          uint32_t r0[16], r1[16];
-          __syncwarp();
-          tmem_ld16(t + (uint32_t)((first + c) * 16), r0);
-          if (c + 1 < mine) tmem_ld16(t + (uint32_t)((first + c + 1) * 16), r1);
-          tmem_ld_wait();
+          for (int i = 0; i < 16; ++i) sum[i] += __uint_as_float(r0[i]);
+        if (mine > 1)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum[c * 16 + i] += __uint_as_float(r0[i]);
-          if (c + 1 < mine)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum[c * 16 + 16 + i] += __uint_as_float(r1[i]);
-        }
+          for (int i = 0; i < 16; ++i) sum[16 + i] += __uint_as_float(r1[i]);
         if (sums) {
           uint32_t r0[16];
           __syncwarp();
@@ -260,7 +235,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_cons
         p.slab_ones[(int64_t)split * q.m + row] = v;
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         if (c >= mine) continue;
 #pragma unroll
         for (int e = 0; e < 16; e += 8) {
@@ -304,7 +279,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_cons
             float2 t[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) t[i] = make_float2(dropped[2 * i], dropped[2 * i + 1]);
-            drop_eight(q.drop, keys, (uint32_t)col / 8, (uint64_t)(q.row0 + row), t);
+            drop_eight(q.drop, philox_keys(drop_seed(q.drop)), (uint32_t)col / 8, (uint64_t)(q.row0 + row), t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) { dropped[2 * i] = t[i].x; dropped[2 * i + 1] = t[i].y; }
           }
