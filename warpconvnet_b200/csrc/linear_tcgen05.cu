@@ -528,9 +528,7 @@ template <auto KERNEL> bool allow_smem() {
 }
 
 // A row-major matrix of `size`-byte elements read or written in boxes of cols x rows, swizzled over their row's bytes (64 or 128).
-bool box_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
-  EncodeTiledFn encode = encode_tiled();
-  if (!encode) return false;
+bool box_map(EncodeTiledFn encode, CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
@@ -593,11 +591,13 @@ template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16> int launch(const w
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   if (p.stages < 2) return WCN_ERR_UNSUPPORTED_CONFIG;
   CUtensorMap a, b, out, add;
-  bool ok = box_map(&a, type, size, q.a, q.m, q.k, q.a_ld, depth, TILE_M);
-  ok = ok && (B_MN ? box_map(&b, type, size, q.b, q.k, q.n, q.b_ld, 64, 64) : box_map(&b, type, size, q.b, q.n, q.k, q.b_ld, depth, p.NT));
+  EncodeTiledFn encode = encode_tiled();
+  if (!encode) return WCN_ERR_UNSUPPORTED_CONFIG;
+  bool ok = box_map(encode, &a, type, size, q.a, q.m, q.k, q.a_ld, depth, TILE_M);
+  ok = ok && (B_MN ? box_map(encode, &b, type, size, q.b, q.k, q.n, q.b_ld, 64, 64) : box_map(encode, &b, type, size, q.b, q.n, q.k, q.b_ld, depth, p.NT));
   out = add = a;   // (not used where they are not made)
-  if (p.out_tma) ok = ok && box_map(&out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
-  if (q.add && p.add_tma) ok = ok && box_map(&add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
+  if (p.out_tma) ok = ok && box_map(encode, &out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
+  if (q.add && p.add_tma) ok = ok && box_map(encode, &add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
   if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
   constexpr auto kern = linear_kernel<KIND, B_MN, ACT, GRAD, BF16>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;

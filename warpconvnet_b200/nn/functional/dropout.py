@@ -67,11 +67,11 @@ def formula(x: Tensor, least: int, seed: Union[int, Tensor], residual: Optional[
 def _run(x: Tensor, least: int, seed: Union[int, Tensor], residual: Optional[Tensor]) -> Tensor:
     n, c = x.shape
     dev = x.device
-    y = torch.empty((n, c), dtype=x.dtype, device=dev)
+    y = x.new_empty((n, c))
     if n and c:
-        x, x_ld = _rows(x)
-        res_ld = 0
-        if residual is not None:
+        x, x_ld = (x, c) if x.is_contiguous() else _rows(x)
+        res_ld = c
+        if residual is not None and not residual.is_contiguous():
             residual, res_ld = _rows(residual)
         number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
         with on_device(dev):

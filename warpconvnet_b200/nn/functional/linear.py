@@ -31,26 +31,29 @@ def _check_shapes(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
         raise ValueError(f"all tensors must be on {x.device}")
 
 
-def _seed_arguments(seed: Union[int, Tensor]):
-    return (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
+def _operand(t: Tensor, whole: int, c: int = 0):
+    """``t`` as the kernels read it and the elements from row to row (``_matrix``, without its questions where they have an answer)."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and t.shape[1] % whole == 0:
+        return t, t.shape[1]
+    return _matrix(t, c)
 
 
-def _forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: int, residual: Optional[Tensor], least: int, seed):
+def _forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: int, residual: Optional[Tensor], least: int, seed, code: int):
     """(y, the matrices as the kernels read them)"""
     (n, k), m, dev = x.shape, weight.shape[0], x.device
-    x, x_ld = _matrix(x)
-    weight, w_ld = _matrix(weight)
-    y = torch.empty((n, m), dtype=x.dtype, device=dev)
-    res_ld = 0
-    if residual is not None:
+    y = x.new_empty((n, m))
+    whole = 1 if code == WCN_F32 else 8
+    x, x_ld = _operand(x, whole)
+    weight, w_ld = _operand(weight, whole)
+    res_ld = m
+    if residual is not None and not residual.is_contiguous():
         residual, res_ld = _rows(residual)
-    number, at = _seed_arguments(seed)
-    code = dtype_code(x.dtype)
+    number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
     size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, 0, 0) if code == WCN_F32 else 0
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with on_device(dev):
-        check(lib().wcn_linear(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, code, ptr(bias), act, ptr(residual), res_ld, least, number, at,
-                               ptr(y), ptr(ws), size, ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear")
+        check(lib().wcn_linear(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, ptr(residual), res_ld, least, number, at,
+                               y.data_ptr(), ptr(ws), size, device_status(dev).data_ptr(), stream_ptr(dev)), "wcn_linear")
         count_training_launches("wcn_linear")
     return y, x, weight
 
@@ -69,13 +72,12 @@ def formula(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optio
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: Optional[str], least: int, seed):
-        y, x_rows, w_rows = _forward(x.detach(), weight.detach(), None if bias is None else bias.detach().contiguous(), _ACTIVATIONS[activation],
-                                     None if residual is None else residual.detach(), least, seed)
-        ctx.activation, ctx.least, ctx.seed = activation, least, None if isinstance(seed, Tensor) else seed
+    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: Optional[str], least: int, seed,
+                code: int):
+        y, x_rows, w_rows = _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)
+        ctx.activation, ctx.least, ctx.seed, ctx.code = activation, least, None if isinstance(seed, Tensor) else seed, code
         # (matrices that had to be copied are kept with them: there are not two copies to be made)
-        copied = tuple(None if rows.data_ptr() == given.data_ptr() else rows for rows, given in ((x_rows, x), (w_rows, weight)))
-        ctx.save_for_backward(x, weight, bias, seed if isinstance(seed, Tensor) else None, *copied)
+        ctx.save_for_backward(x, weight, bias, seed if isinstance(seed, Tensor) else None, None if x_rows is x else x_rows, None if w_rows is weight else w_rows)
         return y
 
     @staticmethod
@@ -88,27 +90,28 @@ class _Linear(torch.autograd.Function):
             y = formula(x, weight, bias, ctx.activation, None, ctx.least, seed)
             wanted = [t for t, need in zip((x, weight, bias), (need_x, need_w, need_b)) if need]
             got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True) if wanted else ())
-            return tuple(next(got) if need else None for need in (need_x, need_w, need_b)) + (d_residual, None, None, None)
+            return tuple(next(got) if need else None for need in (need_x, need_w, need_b)) + (d_residual, None, None, None, None)
         if not (need_x or need_w or need_b):
-            return None, None, None, d_residual, None, None, None
+            return None, None, None, d_residual, None, None, None, None
         (n, k), m, dev = x.shape, weight.shape[0], x.device
-        code, act = dtype_code(x.dtype), _ACTIVATIONS[ctx.activation]
-        dx = torch.empty((n, k), dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty((m, k), dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(m, dtype=x.dtype, device=dev) if need_b else None
-        dy, dy_ld = _rows(dy)
+        code, act = ctx.code, _ACTIVATIONS[ctx.activation]
+        dx = x.new_empty((n, k)) if need_x else None
+        dw = weight.new_empty((m, k)) if need_w else None
+        db = weight.new_empty(m) if need_b else None
+        dy, dy_ld = (dy, m) if dy.is_contiguous() else _rows(dy)
         whole = 1 if code == WCN_F32 else 8
         direct = not act and not ctx.least and dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
-        x, x_ld = _matrix(x if x_rows is None else x_rows, k)
-        weight, w_ld = _matrix(weight if w_rows is None else w_rows, k)
+        x, x_ld = _operand(x if x_rows is None else x_rows, whole, k)
+        weight, w_ld = _operand(weight if w_rows is None else w_rows, whole, k)
         bias = None if bias is None else bias.contiguous()
-        number, at = _seed_arguments(seed)
+        number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
         ws = torch.empty(query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, int(direct)), dtype=torch.uint8, device=dev)
         with on_device(dev):
-            check(lib().wcn_linear_backward(ptr(x), x_ld, n, k, ptr(weight), w_ld, m, code, ptr(bias), act, ptr(dy), dy_ld, ctx.least, number, at,
-                                            ptr(dx), ptr(dw), ptr(db), ptr(ws), ws.numel(), ptr(device_status(dev)), stream_ptr(dev)), "wcn_linear_backward")
+            check(lib().wcn_linear_backward(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, dy.data_ptr(), dy_ld, ctx.least, number, at,
+                                            ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), ws.numel(), device_status(dev).data_ptr(), stream_ptr(dev)),
+                  "wcn_linear_backward")
             count_training_launches("wcn_linear_backward")
-        return dx, dw, db, d_residual, None, None, None
+        return dx, dw, db, d_residual, None, None, None, None
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, residual: Optional[Tensor] = None,
@@ -121,23 +124,25 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     activation for pieces of at most 64 MB, and fp32 sums of ``weight``'s gradient.  In 16 bits that gradient is rounded to ``x``'s
     dtype before its products.  At most 32 768 inputs and 2^20 outputs."""
     check_activation(activation)
-    least = check_probability(dropout_p)
+    least = check_probability(dropout_p) if dropout_p else 0
     _check_shapes(x, weight, bias)
     if torch.is_autocast_enabled():
         dtype = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dtype), weight.to(dtype)
         bias, residual = (t if t is None else t.to(dtype) for t in (bias, residual))
-    dtype_code(x.dtype)
+    code = dtype_code(x.dtype)
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise TypeError(f"x is {x.dtype}, weight {weight.dtype}{'' if bias is None else f', bias {bias.dtype}'}: they must be of one dtype")
-    check_residual(residual, (x.shape[0], weight.shape[0]), x.dtype, x.device)
-    check_seed(seed, x.device)
+    if residual is not None:
+        check_residual(residual, (x.shape[0], weight.shape[0]), x.dtype, x.device)
+    if seed is not None:
+        check_seed(seed, x.device)
     seed = new_seed(x.device) if least and seed is None else 0 if not least else seed
     if not reverse_mode_only() or not x.shape[0]:
         return formula(x, weight, bias, activation, residual, least, seed)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _Linear.apply(x, weight, bias, residual, activation, least, seed)
-    return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed)[0]
+        return _Linear.apply(x, weight, bias, residual, activation, least, seed, code)
+    return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)[0]
 
 
 def _codes(t: Tensor):

@@ -44,7 +44,8 @@ def _check(x: Tensor, weight: Optional[Tensor], eps: float, residual: Optional[T
     check_eps(eps)
     if weight is not None and (weight.shape != x.shape[1:] or weight.device != x.device or not weight.is_floating_point()):
         raise ValueError(f"weight must be {x.shape[1]} floating-point numbers on {x.device}, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
-    check_residual(residual, x.shape, x.dtype, x.device)
+    if residual is not None:
+        check_residual(residual, x.shape, x.dtype, x.device)
     return code
 
 
@@ -52,14 +53,14 @@ def _forward(x: Tensor, weight: Optional[Tensor], eps: float, residual: Optional
     """(y, or codes and scales; h, or None; 1 / root mean square of each row, or None)"""
     n, c = x.shape
     dev = x.device
-    h = torch.empty((n, c), dtype=x.dtype, device=dev) if residual is not None else None
-    y = torch.empty((n, c), dtype=E4M3 if eight else x.dtype, device=dev)
+    h = x.new_empty((n, c)) if residual is not None else None
+    y = torch.empty((n, c), dtype=E4M3, device=dev) if eight else x.new_empty((n, c))
     scale = torch.empty(n, dtype=torch.float32, device=dev) if eight else None
     rstd = torch.empty(n, dtype=torch.float32, device=dev) if keep else None
     if n:
-        x, x_ld = _rows(x)
-        res_ld = 0
-        if residual is not None:
+        x, x_ld = (x, c) if x.is_contiguous() else _rows(x)
+        res_ld = c
+        if residual is not None and not residual.is_contiguous():
             residual, res_ld = _rows(residual)
         with on_device(dev):
             check(lib().wcn_rms_norm(ptr(x), x_ld, ptr(residual), res_ld, n, c, code, ptr(weight), _bits(eps), ptr(h), None if eight else ptr(y),
@@ -101,11 +102,11 @@ class _RMSNorm(torch.autograd.Function):
         n, c = x.shape
         dev, code = x.device, dtype_code(x.dtype)
         h, h_ld = _rows(x if h is None else h)
-        dy, dy_ld = _rows(dy)
-        dh_ld = 0
-        if dh is not None:
+        dy, dy_ld = (dy, c) if dy.is_contiguous() else _rows(dy)
+        dh_ld = c
+        if dh is not None and not dh.is_contiguous():
             dh, dh_ld = _rows(dh)
-        dx = torch.empty((n, c), dtype=x.dtype, device=dev) if need_x or need_r else None
+        dx = x.new_empty((n, c)) if need_x or need_r else None
         dw = (torch.empty if n else torch.zeros)(c, dtype=torch.float32, device=dev) if need_w else None
         if n:
             ws = torch.empty(query_bytes("wcn_rms_norm_workspace_bytes", n, c), dtype=torch.uint8, device=dev) if need_w else None
@@ -114,7 +115,7 @@ class _RMSNorm(torch.autograd.Function):
                 check(lib().wcn_rms_norm_backward(ptr(h), h_ld, ptr(dy), dy_ld, ptr(dh), dh_ld, n, c, code, ptr(gamma), ptr(rstd), ptr(dx), ptr(dw),
                                                   ptr(ws), ws.numel() if need_w else 0, stream_ptr(dev)), "wcn_rms_norm_backward")
                 count_training_launches("wcn_rms_norm_backward")
-        return dx if need_x else None, dx if need_r else None, dw.to(weight.dtype) if need_w else None, None, None
+        return dx if need_x else None, dx if need_r else None, (dw if weight.dtype == torch.float32 else dw.to(weight.dtype)) if need_w else None, None, None
 
 
 def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
