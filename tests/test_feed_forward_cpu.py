@@ -72,7 +72,7 @@ def test_linear_refuses(bad):
 
 def test_linears_gradient_and_codes_refuse():
     def gradient(n=100, k=64, m=40, dtype=_native.WCN_BF16, act=1, ws=BASE, less=0, what=7, dy=BASE, dy_ld=40, x_ld=64):
-        size = _native.query_bytes("wcn_linear_workspace_bytes", 100, 64, 40, dtype, 7, 0)
+        size = _native.query_bytes("wcn_linear_workspace_bytes", 100, 64, 40, dtype, 7, 1, 0, 1)
         out = [BASE if what >> i & 1 else None for i in range(3)]
         return _native.lib().wcn_linear_backward(BASE, x_ld, n, k, BASE, 64, m, dtype, None, act, dy, dy_ld, 0, 0, None, *out, ws, size - less, BASE, None)
     for dtype in (_native.WCN_F32, _native.WCN_F16, _native.WCN_BF16):
@@ -83,8 +83,8 @@ def test_linears_gradient_and_codes_refuse():
     assert eight(n=0) == 0
     assert all(eight(**b) == INVALID for b in (dict(x_ld=8), dict(w_ld=24), dict(out=_native.WCN_F32), dict(scale=None), dict(k=0)))
     out = ctypes.c_int64()
-    for args in ((0, 8, 8, 1, 1, 0), (10, 0, 8, 1, 1, 0), (10, 8, 8, 5, 1, 0), (10, 8, 8, 1, 8, 0)):
+    for args in ((0, 8, 8, 1, 1, 0, 0, 0), (10, 0, 8, 1, 1, 0, 0, 0), (10, 8, 8, 5, 1, 0, 0, 0), (10, 8, 8, 1, 8, 0, 0, 0), (10, 8, 8, 1, 1, 4, 0, 0)):
         assert _native.lib().wcn_linear_workspace_bytes(*args, ctypes.byref(out)) == INVALID
     # the gradient behind the activation in pieces of 512 MB: whatever the rows are, the workspace stays bounded
     for dtype in (_native.WCN_F32, _native.WCN_BF16):
-        assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 257, 64, 256, dtype, 1, 0) <= (512 << 20) + (1 << 20)
+        assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 257, 64, 1000, dtype, 1, 1, 0, 0) <= (512 << 20) + (1 << 20)

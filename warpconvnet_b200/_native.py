@@ -115,7 +115,7 @@ SIGNATURES = {
                    _c_vp, _c_i64, _c_vp, _c_vp],
     "wcn_linear_8bit": [_c_vp, _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_i64, _c_vp, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_vp, _c_vp,
                         _c_vp],
-    "wcn_linear_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _p_i64],
+    "wcn_linear_workspace_bytes": [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _p_i64],
     "wcn_linear_backward": [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_i64, _c_i32, _c_i32, _c_vp, _c_i32, _c_vp, _c_i64, _c_i32, _c_i64, _c_vp,
                             _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp],
     "wcn_selftest_bounded_wait": [_c_i64, _c_vp, _c_vp, _c_vp],

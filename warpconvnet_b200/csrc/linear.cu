@@ -2,8 +2,9 @@
 //     dz = dropout'(dy) act'(z),   dx = dz W,   dW = dz^T x,   dbias = column sums of dz,   dresidual = dy.
 //
 // z is computed again in the backward pass, not kept: for rows as wide as these a product costs less than writing z and reading it (at
-// 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  dz, rounded to the inputs' type, goes to the
-// workspace, in pieces of rows that stay in L2; each piece is multiplied by W (dx) and by x (dW), whose sums over the rows are divided
+// 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  Gradients of narrow layers in 16 bits are one
+// kernel's (linear_backward_tcgen05.cu).  Elsewhere dz, rounded to the inputs' type, goes to the workspace, in pieces of at most 512 MB
+// (pieces that stay in L2 lost more by their launches than they gained: 240 000 x 96 -> 384 in pieces of 64 MB 241 us, whole 196); each is multiplied by W (dx) and by x (dW), whose sums over the rows are divided
 // among the multiprocessors and joined in a fixed order and in double: the same bits on every run.
 //
 // 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 there too
@@ -14,6 +15,8 @@
 #include "linear_ce.cuh"
 
 int wcn_linear_run(const wcn_linear_product& q, int kind, bool bf16, bool by_k, int32_t* dev_status, cudaStream_t st);
+int wcn_linear_backward_blocks(int64_t rows, int k, int n, int act, bool sums);
+int wcn_linear_backward_run(const wcn_linear_product& q, float* slab, float* slab_ones, bool bf16, int32_t* dev_status, cudaStream_t st);
 int wcn_dropout_rows(const void* x, int64_t x_ld, const void* residual, int64_t res_ld, int64_t n, int c, int dtype, const wcn_drop& drop, int64_t row0, void* y,
                      int64_t y_ld, cudaStream_t st);
 int64_t wcn_linear_parts_bytes(int64_t rows, int cols);
@@ -107,14 +110,28 @@ int weight_splits(int m, int k, int rows, int dtype, bool bias) {
 // of dW and of dbias.
 struct Pieces {
   int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
+  int whole;                              // blocks of the kernel that needs no pieces (16 bits, narrow layers); 0: not taken
   bool parts;                             // fp32: the operands are sums of three bf16 numbers
   int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
 enum Want { DX = 1, DW = 2, DB = 4 };     // none of them: forward
-Pieces plan(int64_t n, int k, int m, int dtype, int what, bool direct) {
+// aligned: dy is read as x is.
+Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, bool aligned) {
   Pieces p = {};
   const int64_t e = wcn_dtype_size(dtype);
+  const bool direct = aligned && act == WCN_ACT_NONE && !drops;
   auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
+  if (what && dtype != WCN_F32) p.whole = wcn_linear_backward_blocks(n, k, m, act, what & DB);
+  if (p.whole) {
+    p.rows = (int)n;
+    p.count = 1;
+    p.last_splits = p.whole;
+    p.dz_ld = round(m, 8);
+    p.slab = aligned ? 0 : round(n * p.dz_ld * e, 128);   // (behind dy as the kernel reads it)
+    p.ones = p.slab + (what & (DW | DB) ? round((int64_t)p.whole * m * wcn_ce_round(k, 16) * 4, 128) : 0);
+    p.bytes = p.ones + (what & DB ? (int64_t)p.whole * m * 4 : 0);
+    return p;
+  }
   p.dz_ld = round(m, 16 / e);
   p.parts = dtype == WCN_F32;
   const bool weights = what & (DW | DB), makes_dz = what && !direct;
@@ -169,7 +186,7 @@ extern "C" int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, con
   wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, y, m, bias, act, false, residual, residual_ld,
                           wcn_make_drop((uint32_t)least, seed, seed_at), 0};
   if (dtype != WCN_F32) return run(q, dtype, false, nullptr, nullptr, dev_status, st);
-  const Pieces p = plan(n, k, m, dtype, 0, false);
+  const Pieces p = plan(n, k, m, dtype, 0, act, least, false);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);
   for (int i = 0; i < p.count; ++i) {
@@ -199,9 +216,9 @@ extern "C" int wcn_linear_8bit(const void* x, int64_t x_ld, const float* x_scale
   return wcn_linear_run(q, WCN_E4M3, out_dtype == WCN_BF16, false, dev_status, wcn_stream(stream));
 }
 
-extern "C" int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int32_t direct, int64_t* bytes) {
-  if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 0 || what > 7) return WCN_ERR_INVALID_PARAMETERS;
-  *bytes = what || dtype == WCN_F32 ? plan(n, k, m, dtype, what, direct).bytes : 0;
+extern "C" int wcn_linear_workspace_bytes(int64_t n, int32_t k, int32_t m, int dtype, int32_t what, int act, int32_t least, int32_t aligned, int64_t* bytes) {
+  if (!bytes || n < 1 || !sizes_taken(n, k, m) || dtype < WCN_F32 || dtype > WCN_BF16 || what < 0 || what > 7 || act < 0 || act > 3) return WCN_ERR_INVALID_PARAMETERS;
+  *bytes = what || dtype == WCN_F32 ? plan(n, k, m, dtype, what, act, least != 0, aligned).bytes : 0;
   return WCN_OK;
 }
 
@@ -212,14 +229,22 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   if (!sizes_taken(n, k, m) || n == 0 || dtype < WCN_F32 || dtype > WCN_BF16 || act < 0 || act > 3 || least < 0 || least > 65536) return WCN_ERR_INVALID_PARAMETERS;
   const int size = wcn_dtype_size(dtype), what = (dx ? DX : 0) | (dw ? DW : 0) | (db ? DB : 0);
   // (rows of a gradient between boundaries are brought to them as others are made)
-  const bool direct = act == WCN_ACT_NONE && least == 0 && rows_taken(dy, dy_ld, n, m, size);
+  const bool aligned = rows_taken(dy, dy_ld, n, m, size), direct = act == WCN_ACT_NONE && least == 0 && aligned;
   if (!what || !dev_status || !rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !dy || (n > 1 && dy_ld < m)) return WCN_ERR_INVALID_PARAMETERS;
-  const Pieces p = plan(n, k, m, dtype, what, direct);
+  const Pieces p = plan(n, k, m, dtype, what, act, least != 0, aligned);
   if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes)) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);
   cudaStream_t st = wcn_stream(stream);
   const wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at), none = wcn_make_drop(0, 0, nullptr);
   const int ld = wcn_ce_round(k, 16);
+  if (p.whole) {
+    int rc = aligned ? WCN_OK : wcn_dropout_rows(dy, dy_ld, nullptr, 0, n, m, dtype, none, 0, ws, p.dz_ld, st);
+    if (rc != WCN_OK) return rc;
+    const wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, dx, k, bias, act, true, aligned ? dy : ws, aligned ? dy_ld : p.dz_ld, drop, 0};
+    rc = wcn_linear_backward_run(q, dw || db ? (float*)(ws + p.slab) : nullptr, db ? (float*)(ws + p.ones) : nullptr, dtype == WCN_BF16, dev_status, st);
+    if (rc != WCN_OK || !(dw || db)) return rc;
+    return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.whole, 0, dev_status}, dtype, st);
+  }
   char *const xs = p.parts ? ws + p.x_parts : nullptr, *const dzs = p.parts ? ws + p.dz_parts : nullptr, *const wsp = p.parts ? ws + p.w_parts : nullptr;
   for (int i = 0; i < p.count; ++i) {
     const int64_t r0 = (int64_t)i * p.rows;

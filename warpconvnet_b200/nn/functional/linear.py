@@ -49,7 +49,7 @@ def _forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: int, residu
     if residual is not None and not residual.is_contiguous():
         residual, res_ld = _rows(residual)
     number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
-    size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, 0, 0) if code == WCN_F32 else 0
+    size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, 0, act, least, 0) if code == WCN_F32 else 0
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with on_device(dev):
         check(lib().wcn_linear(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, ptr(residual), res_ld, least, number, at,
@@ -100,15 +100,16 @@ class _Linear(torch.autograd.Function):
         db = weight.new_empty(m) if need_b else None
         dy, dy_ld = (dy, m) if dy.is_contiguous() else _rows(dy)
         whole = 1 if code == WCN_F32 else 8
-        direct = not act and not ctx.least and dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
+        aligned = dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
         x, x_ld = _operand(x if x_rows is None else x_rows, whole, k)
         weight, w_ld = _operand(weight if w_rows is None else w_rows, whole, k)
         bias = None if bias is None else bias.contiguous()
         number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
-        ws = torch.empty(query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, int(direct)), dtype=torch.uint8, device=dev)
+        size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, act, ctx.least, int(aligned))
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         with on_device(dev):
             check(lib().wcn_linear_backward(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, dy.data_ptr(), dy_ld, ctx.least, number, at,
-                                            ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), ws.numel(), device_status(dev).data_ptr(), stream_ptr(dev)),
+                                            ptr(dx), ptr(dw), ptr(db), ptr(ws), size, device_status(dev).data_ptr(), stream_ptr(dev)),
                   "wcn_linear_backward")
             count_training_launches("wcn_linear_backward")
         return dx, dw, db, d_residual, None, None, None, None
