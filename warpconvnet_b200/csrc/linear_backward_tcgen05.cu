@@ -20,7 +20,7 @@ namespace {
 constexpr int TILE_M = 128, CHUNK_N = 128;                // rows of a tile; outputs of a chunk
 constexpr int HALF_BYTES = TILE_M * 128;                  // 64 outputs of dy
 constexpr int EPI_WARP0 = 2, PARTS = 4, EPI_WARPS = 4 * PARTS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
-constexpr int Z_COLUMNS = 128;
+constexpr int Z_COLUMNS = 128, MAX_BUFFERS = 4;            // buffers: chunks of dy in shared memory
 constexpr int SMEM_BUDGET = 226 * 1024;
 
 struct Params {
@@ -28,12 +28,19 @@ struct Params {
   float* slab;              // [blocks][n][ld] (null: not wanted)
   float* slab_ones;         // [blocks][n] (null: not wanted)
   int KS, K16, NB, ld;      // slices of k, columns of dx and dW, chunks of outputs
-  int with_z, acc, tiles, vec;
+  int tiles, vec, buffers;
   int32_t* dev_status;
 };
 
+struct Ring {
+  int slot, phase, depth;
+  __device__ __forceinline__ void advance() {
+    if (++slot == depth) { slot = 0; phase ^= 1; }
+  }
+};
+
 struct Control {
-  uint64_t w_full, x_full[2], x_empty[2], dy_full[2], dz_full[2], dz_empty[2], z_full[2], z_empty[2], dx_full, dx_read, acc_full, done;
+  uint64_t w_full, x_full[2], x_empty[2], dy_full[MAX_BUFFERS], dz_full[MAX_BUFFERS], dz_empty[MAX_BUFFERS], z_full[2], z_empty[2], dx_full, dx_read, acc_full, done;
   uint32_t tmem_holder;
   int32_t skip;
 };
@@ -68,7 +75,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w_slice = p.NB * CHUNK_N * RB, x_slice = TILE_M * RB, x_stage = p.KS * x_slice;
   const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw), base = smem_u32(smem_raw) + pad;
-  const uint32_t w_at = base, x_at = w_at + (uint32_t)(p.KS * w_slice), dy_at = x_at + (uint32_t)(2 * x_stage), end_at = dy_at + 4 * HALF_BYTES;
+  const uint32_t w_at = base, x_at = w_at + (uint32_t)(p.KS * w_slice), dy_at = x_at + (uint32_t)(2 * x_stage), end_at = dy_at + (uint32_t)(p.buffers * 2 * HALF_BYTES);
   uint8_t* const gen = smem_raw + pad;
   float* const sums = reinterpret_cast<float*>(gen + (end_at - base));                         // [4][NB * 128]
   float* const biases = sums + (p.slab_ones ? 4 * p.NB * CHUNK_N : 0);                          // [NB * 128]
@@ -93,11 +100,13 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(&ctl->x_full[i]), 1);
       mbar_init(bar(&ctl->x_empty[i]), 1);
+      mbar_init(bar(&ctl->z_full[i]), 1);
+      mbar_init(bar(&ctl->z_empty[i]), EPI_WARPS / 2);
+    }
+    for (int i = 0; i < p.buffers; ++i) {
       mbar_init(bar(&ctl->dy_full[i]), 1);
       mbar_init(bar(&ctl->dz_full[i]), EPI_WARPS);
       mbar_init(bar(&ctl->dz_empty[i]), 1);
-      mbar_init(bar(&ctl->z_full[i]), 1);
-      mbar_init(bar(&ctl->z_empty[i]), EPI_WARPS / 2);
     }
     mbar_init(bar(&ctl->dx_full), 1);
     mbar_init(bar(&ctl->dx_read), EPI_WARPS);
@@ -123,26 +132,31 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
       mbar_expect_tx(bar(&ctl->w_full), (uint32_t)(p.KS * w_slice));
       for (int s = 0; s < p.KS; ++s)
         for (int j = 0; j < p.NB; ++j) tma_load_2d(w_at + (uint32_t)(s * w_slice + j * CHUNK_N * RB), &w_map, s * DEPTH, j * CHUNK_N, bar(&ctl->w_full));
-      int i = 0, g = 0;       // tiles and chunks so far
+      int i = 0, chunks = 0;  // so far
+      Ring g{0, 0, p.buffers};
       for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++i) {
         if (!mbar_wait(bar(&ctl->x_empty[i & 1]), ((i >> 1) & 1) ^ 1, p.dev_status)) { ok = false; break; }
         mbar_expect_tx(bar(&ctl->x_full[i & 1]), (uint32_t)x_stage);
         for (int s = 0; s < p.KS; ++s) tma_load_2d(x_at + (uint32_t)((i & 1) * x_stage + s * x_slice), &x_map, s * DEPTH, t * TILE_M, bar(&ctl->x_full[i & 1]));
-        for (int j = 0; j < p.NB; ++j, ++g) {
-          if (!mbar_wait(bar(&ctl->dz_empty[g & 1]), ((g >> 1) & 1) ^ 1, p.dev_status)) { ok = false; break; }
-          const uint32_t full = bar(&ctl->dy_full[g & 1]), to = dy_at + (uint32_t)((g & 1) * 2 * HALF_BYTES);
+        for (int j = 0; j < p.NB; ++j) {
+          if (!mbar_wait(bar(&ctl->dz_empty[g.slot]), g.phase ^ 1, p.dev_status)) { ok = false; break; }
+          const uint32_t full = bar(&ctl->dy_full[g.slot]), to = dy_at + (uint32_t)(g.slot * 2 * HALF_BYTES);
           const bool two = 2 * j + 1 < halves;
           mbar_expect_tx(full, (uint32_t)(two ? 2 * HALF_BYTES : HALF_BYTES));
           tma_load_2d(to, &dy_map, j * CHUNK_N, t * TILE_M, full);
           if (two) tma_load_2d(to + HALF_BYTES, &dy_map, j * CHUNK_N + 64, t * TILE_M, full);
+          g.advance();
+          ++chunks;
         }
       }
       if (!ok) {   // what has been issued lands before the block's shared memory is given back
         for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->w_full), 0); ++k) {}
         for (int v = i - 2 < 0 ? 0 : i - 2; v < i; ++v)
           for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->x_full[v & 1]), (uint32_t)((v >> 1) & 1)); ++k) {}
-        for (int v = g - 2 < 0 ? 0 : g - 2; v < g; ++v)
-          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->dy_full[v & 1]), (uint32_t)((v >> 1) & 1)); ++k) {}
+        for (int v = 0; v < chunks && v < g.depth; ++v) {
+          if (--g.slot < 0) { g.slot = g.depth - 1; g.phase ^= 1; }
+          for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->dy_full[g.slot]), (uint32_t)g.phase); ++k) {}
+        }
       }
     }
     __syncwarp();
@@ -155,15 +169,17 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
       const uint64_t x_k = smem_desc<RB>(x_at), x_mn = smem_desc_mn<RB>(x_at, (uint32_t)x_slice);
       const uint64_t dz_k = smem_desc<128>(dy_at), dz_mn = smem_desc_mn<128>(dy_at, HALF_BYTES);
       constexpr int LINES = 16 * RB / 16;                  // 16 lines of x or W further, in units of 16 bytes
-      int i = 0, g = 0, zs[2] = {0, 0};
+      int i = 0;
+      uint32_t zs = 0;       // parities of the two accumulators' uses
+      Ring g{0, 0, p.buffers};
       ok = mbar_wait(bar(&ctl->w_full), 0, p.dev_status);
       for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++i) {
         const uint64_t x_stage_at = (uint64_t)(((i & 1) * x_stage) >> 4);
         if (!mbar_wait(bar(&ctl->x_full[i & 1]), (i >> 1) & 1, p.dev_status)) { ok = false; break; }
         tc_fence_after();
         auto issue_z = [&](int h) {   // 64 outputs
-          if (!mbar_wait(bar(&ctl->z_empty[h & 1]), (zs[h & 1] & 1) ^ 1, p.dev_status)) return false;
-          ++zs[h & 1];
+          if (!mbar_wait(bar(&ctl->z_empty[h & 1]), (zs >> (h & 1) & 1) ^ 1, p.dev_status)) return false;
+          zs ^= 1u << (h & 1);
           tc_fence_after();
           for (int s = 0; s < p.KS; ++s)
 #pragma unroll
@@ -174,10 +190,10 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
           return true;
         };
         auto products = [&](int j) {  // of 128 outputs of dz
-          if (!mbar_wait(bar(&ctl->dz_full[g & 1]), (g >> 1) & 1, p.dev_status)) return false;
+          if (!mbar_wait(bar(&ctl->dz_full[g.slot]), g.phase, p.dev_status)) return false;
           if (j == 0 && i > 0 && q.out && !mbar_wait(bar(&ctl->dx_read), (i - 1) & 1, p.dev_status)) return false;
           tc_fence_after();
-          const uint64_t at = (uint64_t)(((g & 1) * 2 * HALF_BYTES) >> 4);
+          const uint64_t at = (uint64_t)((g.slot * 2 * HALF_BYTES) >> 4);
           if (q.out) {
             const int here = min(2, halves - 2 * j);
             for (int h = 0; h < here; ++h)
@@ -190,8 +206,8 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
 #pragma unroll
             for (int e = 0; e < TILE_M / 16; ++e)
               umma_f16(dw_col + (uint32_t)(j * p.K16), dz_mn + at + (uint64_t)(e * 128), x_mn + x_stage_at + (uint64_t)(e * LINES), idesc_dw, (i | e) ? 1u : 0u);
-          umma_commit(bar(&ctl->dz_empty[g & 1]));
-          ++g;
+          umma_commit(bar(&ctl->dz_empty[g.slot]));
+          g.advance();
           return true;
         };
         for (int j = 0; j < p.NB && ok; ++j) {
@@ -219,12 +235,13 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
     uint32_t place[4];                       // this thread's 32 outputs of its row of dy
 #pragma unroll
     for (int c = 0; c < 4; ++c) place[c] = dy_at + (uint32_t)(side * HALF_BYTES + in_tile * 128 + (((col_half * 4 + c) ^ (in_tile & 7)) << 4));
-    int i = 0, g = 0, zs = 0;
+    int i = 0, zs = 0;
+    Ring g{0, 0, p.buffers};
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
       const int row = t * TILE_M + in_tile;
-      for (int j = 0; j < p.NB; ++j, ++g) {
+      for (int j = 0; j < p.NB; ++j, g.advance()) {
         const bool use = 2 * j + side < halves;
-        if (ok) ok = mbar_wait(bar(&ctl->dy_full[g & 1]), (g >> 1) & 1, p.dev_status);
+        if (ok) ok = mbar_wait(bar(&ctl->dy_full[g.slot]), g.phase, p.dev_status);
         if (ok && with_z && use) ok = mbar_wait(bar(&ctl->z_full[side]), zs & 1, p.dev_status);
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
         if (use) {
@@ -239,7 +256,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
             if (lane == 0) mbar_arrive(bar(&ctl->z_empty[side]));
           }
           const int col = j * CHUNK_N + side * 64 + col_half * 32;
-          const uint32_t buffer = (uint32_t)((g & 1) * 2 * HALF_BYTES);
+          const uint32_t buffer = (uint32_t)(g.slot * 2 * HALF_BYTES);
           const float4* const bias = reinterpret_cast<const float4*>(biases + col);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -269,7 +286,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(&ctl->dz_full[g & 1]));
+        if (lane == 0) mbar_arrive(bar(&ctl->dz_full[g.slot]));
       }
       if (!ok) break;
       if (q.out) {
@@ -343,8 +360,12 @@ bool plan(int k, int n, bool with_z, bool sums, Params* p, size_t* smem) {
   p->ld = p->K16;
   p->NB = (n + CHUNK_N - 1) / CHUNK_N;
   if (k > 256 || (with_z ? Z_COLUMNS : 0) + p->K16 * (p->NB + 1) > 512) return false;
-  *smem = 1024 + (size_t)p->KS * p->NB * CHUNK_N * rb + 2 * (size_t)p->KS * TILE_M * rb + 4 * HALF_BYTES + (size_t)(sums ? 5 : 1) * p->NB * CHUNK_N * 4 + sizeof(Control) + 64;
-  return *smem <= SMEM_BUDGET;
+  const size_t rest = 1024 + (size_t)p->KS * p->NB * CHUNK_N * rb + 2 * (size_t)p->KS * TILE_M * rb + (size_t)(sums ? 5 : 1) * p->NB * CHUNK_N * 4 + sizeof(Control) + 64;
+  for (p->buffers = MAX_BUFFERS; p->buffers >= 2; --p->buffers) {   // dy is on its way for as many chunks
+    *smem = rest + (size_t)p->buffers * 2 * HALF_BYTES;
+    if (*smem <= SMEM_BUDGET) return true;
+  }
+  return false;
 }
 
 template <auto KERNEL> bool allow_smem() {
