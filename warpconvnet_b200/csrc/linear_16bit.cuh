@@ -125,9 +125,9 @@ template <bool BF16> __device__ __forceinline__ float number(uint16_t v) {
   return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
-// Sixteen numbers of one row: v = A B^T + bias on entry, the result's on exit; add: as many in 16 bits.
+// `keys`: in shared memory.  Sixteen numbers of one row: v = A B^T + bias on entry, the result's on exit; add: as many in 16 bits.
 template <int ACT, bool GRAD, bool BF16, bool MORE>   // MORE: there may be dropout or a sum
-__device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t seed, float2 (&v)[8], const uint4 (&add)[2], int64_t row, int col) {
+__device__ __forceinline__ void finish(const wcn_linear_product& q, const PhiloxKeys* keys, float2 (&v)[8], const uint4 (&add)[2], int64_t row, int col) {
   const bool drop = MORE && q.drop.least != 0, sum = MORE && !GRAD && q.add;
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
@@ -135,7 +135,7 @@ __device__ __forceinline__ void finish(const wcn_linear_product& q, uint64_t see
     float2 t[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = GRAD ? unpack2<BF16>(a[i]) : activate<ACT>(v[4 * b + i]);
-    if (drop) drop_eight(q.drop, philox_keys(seed), (uint32_t)col / 8 + b, (uint64_t)row, t);
+    if (drop) drop_eight(q.drop, *keys, (uint32_t)col / 8 + b, (uint64_t)row, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[4 * b + i] = GRAD ? through<ACT>(t[i], v[4 * b + i]) : sum ? __fadd2_rn(t[i], unpack2<BF16>(a[i])) : t[i];
   }

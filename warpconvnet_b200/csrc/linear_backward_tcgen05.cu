@@ -43,6 +43,7 @@ struct Control {
   uint64_t w_full, x_full[2], x_empty[2], dy_full[MAX_BUFFERS], dz_full[MAX_BUFFERS], dz_empty[MAX_BUFFERS], z_full[2], z_empty[2], dx_full, dx_read, acc_full, done;
   uint32_t tmem_holder;
   int32_t skip;
+  PhiloxKeys keys;
 };
 
 // The sums over the warp's rows of 16 columns: each pair of lanes has one column's.
@@ -119,6 +120,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
     if (p.slab_ones)
       for (int s = 0; s < 4; ++s) sums[s * p.NB * CHUNK_N + i] = 0.f;
   }
+  if (threadIdx.x == 32 && q.drop.least) ctl->keys = philox_keys(drop_seed(q.drop));
   if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), 512u);
   tc_fence_before();
   __syncthreads();
@@ -230,7 +232,6 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
   } else {
     const int quarter = warp & 3, part = (warp - EPI_WARP0) >> 2, side = part >> 1, col_half = part & 1;   // side: which half of 64 outputs; which 32 of them
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
     const int in_tile = quarter * 32 + lane;
     uint32_t place[4];                       // this thread's 32 outputs of its row of dy
 #pragma unroll
@@ -272,7 +273,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
                 v[2 * e + 1] = __fadd2_rn(make_float2(__uint_as_float(r[16 * h + 4 * e + 2]), __uint_as_float(r[16 * h + 4 * e + 3])), make_float2(b.z, b.w));
               }
             }
-            finish<ACT, true, BF16, true>(q, seed, v, add, q.row0 + row, col + 16 * h);
+            finish<ACT, true, BF16, true>(q, &ctl->keys, v, add, q.row0 + row, col + 16 * h);
             if (with_z || q.drop.least) {   // (otherwise dy is dz)
               store_shared(place[2 * h] + buffer, make_uint4(pack2<BF16>(v[0]), pack2<BF16>(v[1]), pack2<BF16>(v[2]), pack2<BF16>(v[3])));
               store_shared(place[2 * h + 1] + buffer, make_uint4(pack2<BF16>(v[4]), pack2<BF16>(v[5]), pack2<BF16>(v[6]), pack2<BF16>(v[7])));
@@ -360,7 +361,7 @@ bool plan(int k, int n, bool with_z, bool sums, Params* p, size_t* smem) {
   p->ld = p->K16;
   p->NB = (n + CHUNK_N - 1) / CHUNK_N;
   if (k > 256 || (with_z ? Z_COLUMNS : 0) + p->K16 * (p->NB + 1) > 512) return false;
-  const size_t rest = 1024 + (size_t)p->KS * p->NB * CHUNK_N * rb + 2 * (size_t)p->KS * TILE_M * rb + (size_t)(sums ? 5 : 1) * p->NB * CHUNK_N * 4 + sizeof(Control) + 64;
+  const size_t rest = 1024 + (size_t)p->KS * p->NB * CHUNK_N * rb + 2 * (size_t)p->KS * TILE_M * rb + (size_t)(sums ? 5 : 1) * p->NB * CHUNK_N * 4 + sizeof(Control) + 64;   // (what stands before Control is a multiple of 16 bytes)
   for (p->buffers = MAX_BUFFERS; p->buffers >= 2; --p->buffers) {   // dy is on its way for as many chunks
     *smem = rest + (size_t)p->buffers * 2 * HALF_BYTES;
     if (*smem <= SMEM_BUDGET) return true;

@@ -53,6 +53,7 @@ struct Control {
   uint64_t done;
   uint32_t tmem_holder;
   int32_t skip;
+  PhiloxKeys keys;
   __align__(16) float bias[LASTING], scale[LASTING];   // of all columns that this block has, or of each warp's piece
 };
 
@@ -128,6 +129,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     mbar_init(bar(&ctl->done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x == 32 && q.drop.least) ctl->keys = philox_keys(drop_seed(q.drop));
   if (p.lasting && !B_MN) {
     const int first = resident ? (int)blockIdx.x % p.n_tiles * p.NT : 0;
     for (int i = threadIdx.x; i < p.lasting; i += THREADS) {
@@ -220,7 +222,6 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     // Turns of the block's tiles are numbered through, columns fastest; a warp has every PARTS-th.  It has then seen the accumulator's
     // last tile but one filled (of tiles of one, two .. turns there are 8, 4 .. accumulators at least), as waits by parity want.
     const int ew = warp - EPI_WARP0, quarter = warp & 3, pieces = p.NT / PIECE, wide = p.wide, turns = p.turns;
-    const uint64_t seed = q.drop.least ? drop_seed(q.drop) : 0;
     uint8_t* const mine = staging_at + ew * 2 * PIECE_BYTES;
     const uint32_t mine_at = staging + (uint32_t)(ew * 2 * PIECE_BYTES);
     const int rows = q.m - quarter * 32, step = p.NT;    // of this warp's quarters: there is one to do where a tile's first row is less
@@ -334,8 +335,8 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
             add[0] = load_shared(swizzled[2 * h] + place);
             add[1] = load_shared(swizzled[2 * h + 1] + place);
           }
-          if (more) finish<ACT, GRAD, BF16, true>(q, seed, v, add, q.row0 + row, col + 16 * h);
-          else finish<ACT, GRAD, BF16, false>(q, seed, v, add, q.row0 + row, col + 16 * h);
+          if (more) finish<ACT, GRAD, BF16, true>(q, &ctl->keys, v, add, q.row0 + row, col + 16 * h);
+          else finish<ACT, GRAD, BF16, false>(q, &ctl->keys, v, add, q.row0 + row, col + 16 * h);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
             store_shared(swizzled[2 * h + c] + place, make_uint4(pack2<BF16>(v[4 * c]), pack2<BF16>(v[4 * c + 1]), pack2<BF16>(v[4 * c + 2]), pack2<BF16>(v[4 * c + 3])));

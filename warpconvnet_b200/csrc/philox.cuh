@@ -24,8 +24,8 @@ namespace {
 
 __device__ __forceinline__ uint64_t drop_seed(const wcn_drop& d) { return d.at ? (uint64_t)__ldg(d.at) : d.seed; }
 
-// The keys of the ten rounds: they follow from the seed alone.
-struct PhiloxKeys {
+// The keys of the ten rounds: they follow from the seed alone.  (Where registers are short they are kept in shared memory.)
+struct alignas(16) PhiloxKeys {
   uint32_t a[10], b[10];
 };
 __device__ __forceinline__ PhiloxKeys philox_keys(uint64_t seed) {
