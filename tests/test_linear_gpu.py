@@ -141,7 +141,8 @@ def test_activations_over_their_whole_range(dtype, act):
 
 @pytest.mark.parametrize("act,p", [(None, 0.0), ("gelu", 0.0), ("relu", 0.2)])
 @pytest.mark.parametrize("residual", [False, True])
-@pytest.mark.parametrize("n,k,m", [(60001, 64, 32), (45000, 40, 20), (60000, 96, 96), (45003, 128, 160), (30000, 264, 136), (40000, 72, 400), (9000, 512, 1100)])
+@pytest.mark.parametrize("n,k,m", [(60001, 64, 32), (45000, 40, 20), (60000, 96, 96), (45003, 128, 160), (30000, 264, 136), (40000, 72, 400), (9000, 512, 1100),
+                                   (20001, 800, 512), (9473, 1024, 256), (38000, 1000, 96)])   # (the last ones: pairs of blocks)
 def test_several_tiles_a_multiprocessor(n, k, m, residual, act, p):
     """More tiles than multiprocessors, of one to eight pieces of columns, a group of columns a block and not: gradients too."""
     x, w, b, r, dy = make(n, k, m, torch.bfloat16)
@@ -306,7 +307,7 @@ def test_under_autocast():
     assert all(g.dtype == torch.float32 for g in grads)
 
 
-@pytest.mark.parametrize("n,k,m", [(1, 16, 8), (1, 256, 1024), (300, 96, 384), (257, 100, 13), (129, 384, 96), (64, 1024, 520), (2000, 130, 40), (5, 33, 7)])
+@pytest.mark.parametrize("n,k,m", [(1, 16, 8), (1, 256, 1024), (300, 96, 384), (257, 100, 13), (129, 384, 96), (64, 1024, 520), (2000, 130, 40), (5, 33, 7), (9500, 1536, 512), (20001, 2000, 200)])
 @pytest.mark.parametrize("out_dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("act,residual", [(None, False), ("gelu", True), ("relu", True), ("silu", False)])
 def test_eight_bits(n, k, m, out_dtype, act, residual):

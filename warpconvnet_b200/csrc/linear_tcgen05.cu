@@ -32,7 +32,7 @@ struct Params {
   int KB, NT;               // slices of k; columns of a tile (a multiple of 32)
   int m_tiles, n_tiles, stages, accs, tmem_cols;
   int b_slice;              // bytes of a slice of B
-  int out_tma, add_tma, resident;
+  int out_tma, add_tma, resident, pair;
   int wide, turns;          // pieces of a warp's turn, turns of a tile
   int lasting;              // bias and scales are in shared memory from the start on: of the block's columns, or of all
   int32_t* dev_status;
@@ -65,6 +65,47 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// What two blocks of a cluster do together (PAIR): one matrix instruction has 256 rows, of which each block holds 128, and half of the
+// columns' rows of B from each.
+__device__ __forceinline__ uint32_t of_block(uint32_t at, uint32_t rank) {   // the same place in the shared memory of a block of the cluster
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void arrive_at(uint32_t there) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory"); }
+__device__ __forceinline__ void store_at(uint32_t there, int32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(there), "r"(v) : "memory"); }
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar_of_first) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_of_first)
+               : "memory");
+}
+__device__ __forceinline__ void umma_pair_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar) {   // the barriers at this place in both blocks
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t holder, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src)
                : "memory");
@@ -74,12 +115,12 @@ template <int N> __device__ __forceinline__ void store_wait_read() { asm volatil
 
 // The tiles of a block.  With the columns' rows of B in shared memory: one group of columns, a part of its tiles of rows; else all tiles
 // in order, columns fastest.
-struct Tiles {
+template <bool PAIR> struct Tiles {
   int m, n, dm, dn, m_tiles, n_tiles;
   __device__ __forceinline__ explicit Tiles(const Params& p) : m_tiles(p.m_tiles), n_tiles(p.n_tiles) {
-    const int grid = (int)gridDim.x;
-    m = (int)blockIdx.x / n_tiles;
-    n = (int)blockIdx.x - m * n_tiles;
+    const int grid = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x, block = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x;
+    m = block / n_tiles;
+    n = block - m * n_tiles;
     dm = p.resident ? (grid - n + n_tiles - 1) / n_tiles : grid / n_tiles;   // (resident: the blocks of this group)
     dn = p.resident ? 0 : grid - dm * n_tiles;
   }
@@ -93,14 +134,16 @@ struct Tiles {
 
 // KIND: operands f16, bf16 or e4m3.  B_MN: the columns of the result run along B's rows.
 // ACT, GRAD: what is made of the sums (see linear.cuh); a kernel for each, as one that has all of them waits for its instructions.
-template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16>
+template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap out_map,
               const __grid_constant__ CUtensorMap add_map, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int DEPTH = KIND == WCN_E4M3 ? 128 : 64;       // elements of k of a slice
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool resident = p.resident;
+  constexpr int TILE_ROWS = PAIR ? 2 * TILE_M : TILE_M;
+  const int rank = PAIR ? (int)blockIdx.x & 1 : 0, row_of_block = rank * TILE_M;
+  const bool resident = !PAIR && p.resident;
   const int stage_bytes = resident ? A_BYTES : A_BYTES + p.b_slice;
   const uint32_t pad = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
   const uint32_t base = smem_u32(smem_raw) + pad;
@@ -111,19 +154,29 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
   uint16_t* const out = reinterpret_cast<uint16_t*>(q.out);
   auto mark = [&]() {
     const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
-    for (Tiles t(p); t.there(); t.advance())
+    for (Tiles<PAIR> t(p); t.there(); t.advance())
       for (int i = threadIdx.x; i < TILE_M * p.NT; i += THREADS) {
-        const int row = t.m * TILE_M + i / p.NT, col = t.n * p.NT + i % p.NT;
+        const int row = t.m * TILE_ROWS + row_of_block + i / p.NT, col = t.n * p.NT + i % p.NT;
         if (row < q.m && col < q.n) out[(int64_t)row * q.out_ld + col] = nan;
       }
   };
-  if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
-  __syncthreads();
+  if (!PAIR) {
+    if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
+    __syncthreads();
+  } else {   // (one answer for both blocks, which are both there)
+    cluster_meet();
+    if (threadIdx.x == 0 && rank == 0) {
+      const int32_t status = *(volatile int32_t*)p.dev_status;
+      ctl->skip = status;
+      store_at(of_block(smem_u32(&ctl->skip), 1), status);
+    }
+    cluster_meet();
+  }
   if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) { mark(); return; }
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(bar(&ctl->full[s]), 1); mbar_init(bar(&ctl->empty[s]), 1); }
     mbar_init(bar(&ctl->b_full), 1);
-    for (int i = 0; i < p.accs; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)(4 * p.turns)); }
+    for (int i = 0; i < p.accs; ++i) { mbar_init(bar(&ctl->acc_full[i]), 1); mbar_init(bar(&ctl->acc_empty[i]), (uint32_t)(4 * p.turns * (PAIR ? 2 : 1))); }
     for (int w = 0; w < EPI_WARPS; ++w)
       for (int i = 0; i < 2; ++i) mbar_init(bar(&ctl->add_full[w][i]), 1);
     mbar_init(bar(&ctl->done), 1);
@@ -138,9 +191,13 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
       if (KIND == WCN_E4M3) ctl->scale[i] = there ? __ldg(&q.b_scale[first + i]) : 0.f;
     }
   }
-  if (warp == 1) tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
+    else tmem_alloc(smem_u32(&ctl->tmem_holder), (uint32_t)p.tmem_cols);
+  }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_meet();   // (barriers are there before the other block reaches for them)
   tc_fence_after();
   const uint32_t tmem = ctl->tmem_holder;
   bool ok = true;
@@ -149,14 +206,19 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     if (elect_one()) {
       Ring r{0, 0, p.stages};
       int issued = 0;
-      auto load_b = [&](uint32_t to, int s, int n, uint32_t full) {
+      auto load = [&](uint32_t to, const CUtensorMap* map, int x, int y, uint32_t full) {
+        if (PAIR) tma_load_pair(to, map, x, y, full);
+        else tma_load_2d(to, map, x, y, full);
+      };
+      auto load_b = [&](uint32_t to, int s, int n, uint32_t full) {   // (PAIR: this block's half of the columns)
+        const int col = n * p.NT + (PAIR ? rank * (p.NT / 2) : 0);
         if (B_MN) {
-          for (int c = 0; c * MN_CHUNK < p.b_slice; ++c) tma_load_2d(to + (uint32_t)(c * MN_CHUNK), &b_map, n * p.NT + 64 * c, s * DEPTH, full);
+          for (int c = 0; c * MN_CHUNK < p.b_slice; ++c) load(to + (uint32_t)(c * MN_CHUNK), &b_map, col + 64 * c, s * DEPTH, full);
         } else {
-          tma_load_2d(to, &b_map, s * DEPTH, n * p.NT, full);
+          load(to, &b_map, s * DEPTH, col, full);
         }
       };
-      Tiles t(p);
+      Tiles<PAIR> t(p);
       const bool any = t.there();
       if (resident && any) {
         mbar_expect_tx(bar(&ctl->b_full), (uint32_t)(p.KB * p.b_slice));
@@ -165,14 +227,17 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
       for (; t.there() && ok; t.advance())
         for (int s = 0; s < p.KB; ++s) {
           if (!mbar_wait(bar(&ctl->empty[r.slot]), r.phase ^ 1, p.dev_status)) { ok = false; break; }
-          const uint32_t full = bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
-          mbar_expect_tx(full, (uint32_t)stage_bytes);
-          tma_load_2d(at, &a_map, s * DEPTH, t.m * TILE_M, full);
+          // (PAIR: the first block's barrier counts what both receive)
+          const uint32_t full = PAIR ? of_block(bar(&ctl->full[r.slot]), 0) : bar(&ctl->full[r.slot]), at = base + (uint32_t)(r.slot * stage_bytes);
+          if (rank == 0) mbar_expect_tx(bar(&ctl->full[r.slot]), (uint32_t)(PAIR ? 2 * stage_bytes : stage_bytes));
+          load(at, &a_map, s * DEPTH, t.m * TILE_ROWS + row_of_block, full);
           if (!resident) load_b(at + A_BYTES, s, t.n, full);
           r.advance();
           ++issued;
         }
-      if (!ok) {   // what has been issued lands before the block's shared memory is given back
+      if (!ok && rank) {   // (whose copies the first block's barriers count: time for them to land)
+        for (const long long began = clock64(); clock64() - began < 2000000ll;) {}
+      } else if (!ok) {   // what has been issued lands before the block's shared memory is given back
         for (int i = 0; i < issued && i < r.depth; ++i) {
           if (--r.slot < 0) { r.slot = r.depth - 1; r.phase ^= 1; }
           for (int k = 0; k < 100000 && !mbar_try_wait(bar(&ctl->full[r.slot]), (uint32_t)r.phase); ++k) {}
@@ -182,15 +247,15 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (elect_one()) {
+    if (rank == 0 && elect_one()) {
       constexpr uint32_t type = KIND == WCN_BF16 ? 1u : 0u;   // (f16 and e4m3: 0 of their kinds)
-      const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (B_MN ? 1u << 16 : 0u) | ((uint32_t)(p.NT >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (B_MN ? 1u << 16 : 0u) | ((uint32_t)(p.NT >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
       constexpr int B_STEP = B_MN ? 128 : 2;                  // an instruction's depth further, in units of 16 bytes
       auto describe_b = [&](uint32_t at) { return B_MN ? smem_desc_mn<128>(at, MN_CHUNK) : smem_desc<128>(at); };
       const uint64_t a0 = smem_desc<128>(base), b0 = describe_b(resident ? res : base + A_BYTES);
       Ring r{0, 0, p.stages};
       int ab = 0, aphase = 0;
-      Tiles t(p);
+      Tiles<PAIR> t(p);
       if (resident && t.there()) ok = mbar_wait(bar(&ctl->b_full), 0, p.dev_status);
       for (; ok && t.there(); t.advance()) {
         if (!mbar_wait(bar(&ctl->acc_empty[ab]), aphase ^ 1, p.dev_status)) { ok = false; break; }
@@ -203,17 +268,22 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           const uint64_t a = a0 + slot, b = b0 + (resident ? (uint64_t)((s * p.b_slice) >> 4) : slot);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (KIND == WCN_E4M3) umma_f8(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
+            if (PAIR && KIND == WCN_E4M3) umma_pair_f8(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
+            else if (PAIR) umma_pair_f16(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
+            else if (KIND == WCN_E4M3) umma_f8(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
             else umma_f16(d, a + (uint64_t)(i * 2), b + (uint64_t)(i * B_STEP), idesc, (s | i) ? 1u : 0u);
           }
-          umma_commit(bar(&ctl->empty[r.slot]));
+          if (PAIR) commit_pair(bar(&ctl->empty[r.slot]));
+          else umma_commit(bar(&ctl->empty[r.slot]));
           r.advance();
         }
         if (!ok) break;
-        umma_commit(bar(&ctl->acc_full[ab]));
+        if (PAIR) commit_pair(bar(&ctl->acc_full[ab]));
+        else umma_commit(bar(&ctl->acc_full[ab]));
         if (++ab == p.accs) { ab = 0; aphase ^= 1; }
       }
-      umma_commit(bar(&ctl->done));
+      if (PAIR) commit_pair(bar(&ctl->done));
+      else umma_commit(bar(&ctl->done));
       (void)mbar_wait(bar(&ctl->done), 0, p.dev_status);
     }
     __syncwarp();
@@ -224,19 +294,19 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     const int ew = warp - EPI_WARP0, quarter = warp & 3, pieces = p.NT / PIECE, wide = p.wide, turns = p.turns;
     uint8_t* const mine = staging_at + ew * 2 * PIECE_BYTES;
     const uint32_t mine_at = staging + (uint32_t)(ew * 2 * PIECE_BYTES);
-    const int rows = q.m - quarter * 32, step = p.NT;    // of this warp's quarters: there is one to do where a tile's first row is less
+    const int rows = q.m - row_of_block - quarter * 32, step = p.NT;    // of this warp's quarters: there is one to do where a tile's first row is less
     struct Place {
       int row, n, turn, ab, phase;                       // first row of the tile, its place among the columns' tiles
     };
-    const Tiles first(p);
-    const int dm = first.dm * TILE_M, dn = first.dn, end = p.m_tiles * TILE_M;
+    const Tiles<PAIR> first(p);
+    const int dm = first.dm * TILE_ROWS, dn = first.dn, end = p.m_tiles * TILE_ROWS;
     auto next = [&](Place& w) {
       w.turn += PARTS;
       while (w.turn >= turns) {
         w.turn -= turns;
         w.row += dm;
         w.n += dn;
-        if (w.n >= p.n_tiles) { w.n -= p.n_tiles; w.row += TILE_M; }
+        if (w.n >= p.n_tiles) { w.n -= p.n_tiles; w.row += TILE_ROWS; }
         if (++w.ab == p.accs) { w.ab = 0; w.phase ^= 1; }
       }
     };
@@ -245,9 +315,9 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     auto request = [&](const Place& w, int buffer) {   // one lane
       const uint32_t full = bar(&ctl->add_full[ew][buffer]);
       mbar_expect_tx(full, PIECE_BYTES);
-      tma_load_2d(mine_at + (uint32_t)(buffer * PIECE_BYTES), &add_map, col_of(w), w.row + quarter * 32, full);
+      tma_load_2d(mine_at + (uint32_t)(buffer * PIECE_BYTES), &add_map, col_of(w), w.row + row_of_block + quarter * 32, full);
     };
-    Place now{first.m * TILE_M, first.n, (ew >> 2) - PARTS, 0, 0};
+    Place now{first.m * TILE_ROWS, first.n, (ew >> 2) - PARTS, 0, 0};
     next(now);
     int b = 0;                               // the next piece's place in shared memory
     uint32_t pending = 0, phases = 0;        // of each of the two: whether a copy is on its way there, its barrier's phase
@@ -261,7 +331,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
     while (now.row < end) {
       Place then = now;
       next(then);
-      const int col0 = col_of(now), row0 = now.row + quarter * 32, row = row0 + lane;
+      const int col0 = col_of(now), row0 = now.row + row_of_block + quarter * 32, row = row0 + lane;
       const bool use = now.row < rows && col0 < q.n;
       const float row_scale = KIND == WCN_E4M3 && use && row < q.m ? __ldg(&q.a_scale[row]) : 0.f;
       // What the last turn has left has been read from its place, which is this one's or the next copy's.
@@ -305,7 +375,10 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
         if (piece == last) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(&ctl->acc_empty[now.ab]));
+          if (lane == 0) {
+            if (PAIR && rank) arrive_at(of_block(bar(&ctl->acc_empty[now.ab]), 0));
+            else mbar_arrive(bar(&ctl->acc_empty[now.ab]));
+          }
         }
         if (!use || col >= q.n) continue;
         const int kept = p.lasting ? (resident ? piece * PIECE : col) : (ew * 2 + piece - now.turn * wide) * PIECE;
@@ -366,7 +439,12 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  if (PAIR) {   // (neither block's memory goes while the other one's instructions may reach for it)
+    cluster_meet();
+    if (warp == 1) tmem_dealloc_pair(tmem, (uint32_t)p.tmem_cols);
+  } else if (warp == 1) {
+    tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  }
   if (threadIdx.x == 0) ctl->skip = *(volatile int32_t*)p.dev_status;
   __syncthreads();
   if (ctl->skip == (int)WCN_ERR_WAIT_EXPIRED) {
@@ -431,12 +509,49 @@ void plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
   p->n_tiles = tiles_of(nt);
   p->b_slice = slice(nt);
   p->accs = 512 / nt < MAX_ACC ? 512 / nt : MAX_ACC;
+  // Operands that both pass: two blocks share a tile of 256 rows, each with half of B's rows, where there are tiles for all of them.
+  // What arrives in a block's shared memory is then 64 bytes a clock of the matrix instructions; alone, 96 at 256 columns, it waits.
+  const int pair_tiles = (int)(((int64_t)q.m + 2 * TILE_M - 1) / (2 * TILE_M));
+  p->pair = !resident && nt % (b_mn ? 128 : 32) == 0 && (int64_t)pair_tiles * tiles_of(nt) * 2 >= sms;
+  if (p->pair) {
+    p->m_tiles = pair_tiles;
+    p->b_slice = slice(nt / 2);
+  }
   p->resident = resident;
   p->turns = (nt / PIECE + p->wide - 1) / p->wide;
   const int columns = resident ? nt : p->n_tiles * nt;
   p->lasting = columns <= LASTING ? columns : 0;
   p->tmem_cols = 32;
   while (p->tmem_cols < p->accs * nt) p->tmem_cols *= 2;
+}
+
+template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16, bool PAIR> int launch_as(Params& p, cudaStream_t st) {
+  const wcn_linear_product& q = p.q;
+  constexpr int size = KIND == WCN_E4M3 ? 1 : 2, depth = SLICE_BYTES / size;
+  constexpr CUtensorMapDataType wide = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  constexpr CUtensorMapDataType type = KIND == WCN_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : wide;
+  const int stage = p.resident ? A_BYTES : A_BYTES + p.b_slice, kept = p.resident ? p.KB * p.b_slice : 0;
+  p.stages = (SMEM_BUDGET - FIXED - kept) / stage;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (p.stages < 2) return WCN_ERR_UNSUPPORTED_CONFIG;
+  CUtensorMap a, b, out, add;
+  EncodeTiledFn encode = encode_tiled();
+  if (!encode) return WCN_ERR_UNSUPPORTED_CONFIG;
+  bool ok = box_map(encode, &a, type, size, q.a, q.m, q.k, q.a_ld, depth, TILE_M);
+  ok = ok && (B_MN ? box_map(encode, &b, type, size, q.b, q.k, q.n, q.b_ld, 64, 64) : box_map(encode, &b, type, size, q.b, q.n, q.k, q.b_ld, depth, PAIR ? p.NT / 2 : p.NT));
+  out = add = a;   // (not used where they are not made)
+  if (p.out_tma) ok = ok && box_map(encode, &out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
+  if (q.add && p.add_tma) ok = ok && box_map(encode, &add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
+  if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
+  constexpr auto kern = linear_kernel<KIND, B_MN, ACT, GRAD, BF16, PAIR>;
+  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
+  const size_t smem = (size_t)FIXED + kept + (size_t)p.stages * stage;
+  const int sms = wcn_num_sms();
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  ++wcn_launched;
+  if (PAIR) return wcn_launch(kern, dim3((unsigned)(2 * (tiles < sms / 2 ? tiles : sms / 2))), dim3(THREADS), smem, st, 2, a, b, out, add, p);
+  kern<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, smem, st>>>(a, b, out, add, p);
+  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
 }
 
 template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16> int launch(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
@@ -447,30 +562,7 @@ template <int KIND, bool B_MN, int ACT, bool GRAD, bool BF16> int launch(const w
   p.add_tma = q.add && tma_rows(q.add, q.add_ld, 2);
   p.wide = q.add ? 1 : 2;
   plan(q, KIND, B_MN, &p);
-  const bool resident = p.resident;
-  constexpr int size = KIND == WCN_E4M3 ? 1 : 2, depth = SLICE_BYTES / size;
-  constexpr CUtensorMapDataType wide = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  constexpr CUtensorMapDataType type = KIND == WCN_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : wide;
-  const int stage = resident ? A_BYTES : A_BYTES + p.b_slice, kept = resident ? p.KB * p.b_slice : 0;
-  p.stages = (SMEM_BUDGET - FIXED - kept) / stage;
-  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  if (p.stages < 2) return WCN_ERR_UNSUPPORTED_CONFIG;
-  CUtensorMap a, b, out, add;
-  EncodeTiledFn encode = encode_tiled();
-  if (!encode) return WCN_ERR_UNSUPPORTED_CONFIG;
-  bool ok = box_map(encode, &a, type, size, q.a, q.m, q.k, q.a_ld, depth, TILE_M);
-  ok = ok && (B_MN ? box_map(encode, &b, type, size, q.b, q.k, q.n, q.b_ld, 64, 64) : box_map(encode, &b, type, size, q.b, q.n, q.k, q.b_ld, depth, p.NT));
-  out = add = a;   // (not used where they are not made)
-  if (p.out_tma) ok = ok && box_map(encode, &out, wide, 2, q.out, q.m, q.n, q.out_ld, PIECE, 32);
-  if (q.add && p.add_tma) ok = ok && box_map(encode, &add, wide, 2, q.add, q.m, q.n, q.add_ld, PIECE, 32);
-  if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
-  constexpr auto kern = linear_kernel<KIND, B_MN, ACT, GRAD, BF16>;
-  if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
-  const int sms = wcn_num_sms();
-  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  kern<<<(unsigned)(tiles < sms ? tiles : sms), THREADS, (size_t)FIXED + kept + (size_t)p.stages * stage, st>>>(a, b, out, add, p);
-  ++wcn_launched;
-  return cudaGetLastError() == cudaSuccess ? WCN_OK : WCN_ERR_EXECUTION;
+  return p.pair ? launch_as<KIND, B_MN, ACT, GRAD, BF16, true>(p, st) : launch_as<KIND, B_MN, ACT, GRAD, BF16, false>(p, st);
 }
 
 template <int KIND, bool GRAD, bool BF16> int by_act(const wcn_linear_product& q, int32_t* dev_status, cudaStream_t st) {
