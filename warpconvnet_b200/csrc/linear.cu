@@ -42,6 +42,7 @@ struct JoinParams {
   void* db;                 // [m]; null: not wanted
   int m, n, ld, splits;
   int quads;                // blocks for dw
+  float factor;
   const int32_t* dev_status;
 };
 
@@ -74,7 +75,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) linear_join_ker
   const bool failed = *p.dev_status == (int)WCN_ERR_WAIT_EXPIRED;
   const float nan = __int_as_float(0x7FC00000);
   if (!of_w) {
-    reinterpret_cast<T*>(p.db)[i] = wcn_from_float<T>(failed ? nan : (float)v[0]);
+    reinterpret_cast<T*>(p.db)[i] = wcn_from_float<T>(failed ? nan : (float)v[0] * p.factor);
     return;
   }
   const int64_t row = i / (p.ld / 4);
@@ -82,7 +83,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) linear_join_ker
   T* const out = reinterpret_cast<T*>(p.dw) + row * p.n + col;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (col + j < p.n) out[j] = wcn_from_float<T>(failed ? nan : (float)v[j]);
+    if (col + j < p.n) out[j] = wcn_from_float<T>(failed ? nan : (float)v[j] * p.factor);
 }
 
 int join(JoinParams p, int dtype, cudaStream_t st) {
@@ -235,15 +236,21 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes)) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);
   cudaStream_t st = wcn_stream(stream);
-  const wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at), none = wcn_make_drop(0, 0, nullptr);
+  const wcn_drop none = wcn_make_drop(0, 0, nullptr);
+  wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at);
+  float factor = 1.f;
+  if (act == WCN_ACT_NONE && least && dtype != WCN_F32) {   // dz is dy or nothing, without a rounding: the factor comes to the sums
+    factor = drop.scale;
+    drop.scale = 1.f;
+  }
   const int ld = wcn_ce_round(k, 16);
   if (p.whole) {
     int rc = aligned ? WCN_OK : wcn_dropout_rows(dy, dy_ld, nullptr, 0, n, m, dtype, none, 0, ws, p.dz_ld, st);
     if (rc != WCN_OK) return rc;
-    const wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, dx, k, bias, act, true, aligned ? dy : ws, aligned ? dy_ld : p.dz_ld, drop, 0};
+    const wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, dx, k, bias, act, true, aligned ? dy : ws, aligned ? dy_ld : p.dz_ld, drop, 0, factor};
     rc = wcn_linear_backward_run(q, dw || db ? (float*)(ws + p.slab) : nullptr, db ? (float*)(ws + p.ones) : nullptr, dtype == WCN_BF16, dev_status, st);
     if (rc != WCN_OK || !(dw || db)) return rc;
-    return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.whole, 0, dev_status}, dtype, st);
+    return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.whole, 0, factor, dev_status}, dtype, st);
   }
   char *const xs = p.parts ? ws + p.x_parts : nullptr, *const dzs = p.parts ? ws + p.dz_parts : nullptr, *const wsp = p.parts ? ws + p.w_parts : nullptr;
   for (int i = 0; i < p.count; ++i) {
@@ -272,7 +279,7 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
       if (rc != WCN_OK) return rc;
     }
     if (dx) {
-      wcn_linear_product q = {dz, w, dz_ld, w_ld, rows, k, m, nullptr, nullptr, (char*)dx + r0 * k * size, k, nullptr, WCN_ACT_NONE, false, nullptr, 0, none, 0};
+      wcn_linear_product q = {dz, w, dz_ld, w_ld, rows, k, m, nullptr, nullptr, (char*)dx + r0 * k * size, k, nullptr, WCN_ACT_NONE, false, nullptr, 0, none, 0, factor};
       rc = run(q, dtype, true, dzs, wsp, dev_status, st);
       if (rc != WCN_OK) return rc;
     }
@@ -288,5 +295,5 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
     }
   }
   if (!dw && !db) return WCN_OK;
-  return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0, dev_status}, dtype, st);
+  return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.splits * (p.count - 1) + p.last_splits, 0, factor, dev_status}, dtype, st);
 }

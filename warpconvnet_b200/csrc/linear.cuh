@@ -22,6 +22,7 @@ struct wcn_linear_product {
   int64_t add_ld;
   wcn_drop drop;
   int64_t row0;             // place of the first row among all rows (for what is dropped)
+  float factor;             // of dx (products of gradients alone)
 };
 
 // An fp32 matrix and where its parts go (linear_split_tcgen05.cu).

@@ -303,7 +303,7 @@ linear_backward_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_c
           if (row >= q.m) continue;
           uint32_t v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = pack2<BF16>(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])));
+          for (int e = 0; e < 8; ++e) v[e] = pack2<BF16>(__fmul2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), both(q.factor)));
           if (p.vec && c * 16 + 16 <= q.k) {
             st_global_32B(out + c * 16, v);
           } else {

@@ -325,6 +325,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
       if (lane == 0) request(now, 0);
       pending = 1;
     }
+    const float factor = q.factor;
     uint32_t swizzled[4];                    // this lane's row of a piece, 16 bytes at a time
 #pragma unroll
     for (int c = 0; c < 4; ++c) swizzled[c] = mine_at + (uint32_t)(lane * 64 + ((c ^ (lane >> 1 & 3)) << 4));
@@ -392,7 +393,11 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           for (int i = 0; i < 4; ++i) {
             v[2 * i] = make_float2(__uint_as_float(r[16 * h + 4 * i]), __uint_as_float(r[16 * h + 4 * i + 1]));
             v[2 * i + 1] = make_float2(__uint_as_float(r[16 * h + 4 * i + 2]), __uint_as_float(r[16 * h + 4 * i + 3]));
-            if (B_MN) continue;
+            if (B_MN) {
+              v[2 * i] = __fmul2_rn(v[2 * i], both(factor));
+              v[2 * i + 1] = __fmul2_rn(v[2 * i + 1], both(factor));
+              continue;
+            }
             const float4 t = bias[4 * h + i];
             if (KIND == WCN_E4M3) {
               const float4 s = scale[4 * h + i];

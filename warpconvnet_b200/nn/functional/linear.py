@@ -27,7 +27,7 @@ def _check_shapes(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
     require_cuda(x, "x")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-    if any(t.device != x.device for t in (weight,) + (() if bias is None else (bias,))):
+    if weight.device != x.device or (bias is not None and bias.device != x.device):
         raise ValueError(f"all tensors must be on {x.device}")
 
 
@@ -141,7 +141,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     seed = new_seed(x.device) if least and seed is None else 0 if not least else seed
     if not reverse_mode_only() or not x.shape[0]:
         return formula(x, weight, bias, activation, residual, least, seed)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, activation, least, seed, code)
     return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)[0]
 
