@@ -62,7 +62,7 @@ def layer(n=4, k=8, m=16, dtype=_native.WCN_BF16, act=0, x=BASE, x_ld=8, w_ld=8,
     return _native.lib().wcn_linear(x, x_ld, n, k, BASE, w_ld, m, dtype, None, act, res, res_ld, least, 1, None, y, ws, size, status, None)
 
 
-@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=2 ** 31), dict(k=0), dict(k=32769), dict(m=0), dict(m=2 ** 20 + 1), dict(dtype=7), dict(act=4), dict(act=-1), dict(x=None),
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=2 ** 31 - 2 ** 17 + 1), dict(k=0), dict(k=32769), dict(m=0), dict(m=2 ** 20 + 1), dict(dtype=7), dict(act=4), dict(act=-1), dict(x=None),
                                  dict(x=BASE + 2), dict(x_ld=12), dict(x_ld=0), dict(w_ld=4), dict(y=None), dict(least=65537), dict(res=BASE, res_ld=15), dict(status=None),
                                  dict(dtype=_native.WCN_F32), dict(dtype=_native.WCN_F32, ws=BASE + 16, size=1 << 40), dict(dtype=_native.WCN_F32, ws=BASE, size=100)])
 def test_linear_refuses(bad):
@@ -87,4 +87,4 @@ def test_linears_gradient_and_codes_refuse():
         assert _native.lib().wcn_linear_workspace_bytes(*args, ctypes.byref(out)) == INVALID
     # the gradient behind the activation in pieces of 512 MB: whatever the rows are, the workspace stays bounded
     for dtype in (_native.WCN_F32, _native.WCN_BF16):
-        assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 257, 64, 1000, dtype, 1, 1, 0, 0) <= (512 << 20) + (1 << 20)
+        assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 2 ** 17, 64, 1000, dtype, 1, 1, 0, 0) <= (512 << 20) + (1 << 20)

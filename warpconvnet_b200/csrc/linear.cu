@@ -30,7 +30,7 @@ int wcn_ce_product_run(const wcn_ce_product& q, bool transposed, bool blocked, i
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;
+constexpr int MOST_ROWS = 0x7FFE0000, MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;   // (row numbers, and some tiles behind the last, are 32-bit)
 constexpr int64_t PIECE_BYTES = 512ll << 20;   // of dz
 
 // ------------------------------------------------------------------ sums of the splits
@@ -166,7 +166,7 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, b
   return p;
 }
 
-bool sizes_taken(int64_t n, int k, int m) { return n >= 0 && n <= 0x7FFFFEFF && k >= 1 && k <= MOST_INPUTS && m >= 1 && m <= MOST_OUTPUTS; }
+bool sizes_taken(int64_t n, int k, int m) { return n >= 0 && n <= MOST_ROWS && k >= 1 && k <= MOST_INPUTS && m >= 1 && m <= MOST_OUTPUTS; }
 bool rows_taken(const void* p, int64_t ld, int64_t rows, int columns, int size) {
   const int whole = size == 4 ? 1 : 16 / size;
   return p && reinterpret_cast<uintptr_t>(p) % (size == 4 ? 4 : 16) == 0 && ld % whole == 0 && (rows <= 1 || ld >= columns);

@@ -38,23 +38,23 @@ __device__ __forceinline__ Normal normal(float z) {
   return n;
 }
 
-__device__ __forceinline__ float activate(int act, float z) {
-  if (act == WCN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if (act == WCN_ACT_SILU) return z * reciprocal(1.f + expf(-z));
-  if (act == WCN_ACT_GELU) {
+template <int ACT> __device__ __forceinline__ float activate(float z) {
+  if (ACT == WCN_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (ACT == WCN_ACT_SILU) return z * reciprocal(1.f + expf(-z));
+  if (ACT == WCN_ACT_GELU) {
     const Normal n = normal(z);
     return (z < -14.f ? n.u : z) * n.function;
   }
   return z;
 }
 // dy act'(z)
-__device__ __forceinline__ float through(int act, float dy, float z) {
-  if (act == WCN_ACT_RELU) return z > 0.f ? dy : 0.f;
-  if (act == WCN_ACT_SILU) {
+template <int ACT> __device__ __forceinline__ float through(float dy, float z) {
+  if (ACT == WCN_ACT_RELU) return z > 0.f ? dy : 0.f;
+  if (ACT == WCN_ACT_SILU) {
     const float e = expf(-fabsf(z)), r = reciprocal(1.f + e), p = z > 0.f ? r : e * r, rest = z > 0.f ? e * r : r;   // (1 - p would be z 2^-24 off)
     return dy * (p * fmaf(z, rest, 1.f));
   }
-  if (act == WCN_ACT_GELU) {
+  if (ACT == WCN_ACT_GELU) {
     const Normal n = normal(z);
     return dy * fmaf(n.u, 0.3989422804014327f * n.density, n.function);
   }

@@ -32,7 +32,7 @@ struct Params {
   float* slab_ones;          // [splits][m]: of A alone (null: not wanted)
   int NT, m_tiles, n_tiles, ksteps, per, splits, units, stages, accs, stride, tmem_cols, ld;
   int b_plane;
-  int vec;                   // rows of `out` and of what is added start on 32-byte boundaries
+  int vec, vec_bias;         // rows of `out` and of what is added start on 32-byte boundaries; the bias on a 16-byte one
   int32_t* dev_status;
 };
 
@@ -68,8 +68,9 @@ __device__ __noinline__ float again(const wcn_linear_product& q, int64_t a_k, in
   return v;
 }
 
-// A_MN, B_MN: rows of A (columns of the result) run along the rows of the operand's matrix, which is [k][m] ([k][n]).
-template <bool A_MN, bool B_MN>
+// A_MN, B_MN: rows of A (columns of the result) run along the rows of the operand's matrix, which is [k][m] ([k][n]).  ACT, GRAD: what is
+// made of the sums (a kernel for each: one that has all of them waits for its instructions, 40 us where this takes 2x).
+template <bool A_MN, bool B_MN, int ACT, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -268,13 +269,22 @@ linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_cons
               for (int i = 0; i < 8; ++i) g[i] = col + i < q.n ? __ldg(add + i) : 0.f;
             }
           }
-          if (q.bias)
+          if (q.bias) {
+            __align__(16) float bias[8];
+            if (p.vec_bias && col + 8 <= q.n) {
+              *reinterpret_cast<float4*>(bias) = __ldg(reinterpret_cast<const float4*>((const float*)q.bias + col));
+              *reinterpret_cast<float4*>(bias + 4) = __ldg(reinterpret_cast<const float4*>((const float*)q.bias + col) + 1);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += col + i < q.n ? __ldg((const float*)q.bias + col + i) : 0.f;
-          float* const dropped = q.grad ? g : v;
-          if (!q.grad && q.act)
+              for (int i = 0; i < 8; ++i) bias[i] = col + i < q.n ? __ldg((const float*)q.bias + col + i) : 0.f;
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = activate(q.act, v[i]);
+            for (int i = 0; i < 8; ++i) v[i] += bias[i];
+          }
+          float* const dropped = GRAD ? g : v;
+          if (!GRAD)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = activate<ACT>(v[i]);
           if (q.drop.least) {
             float2 t[4];
 #pragma unroll
@@ -283,9 +293,9 @@ linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) { dropped[2 * i] = t[i].x; dropped[2 * i + 1] = t[i].y; }
           }
-          if (q.grad) {
+          if (GRAD) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = through(q.act, g[i], v[i]);
+            for (int i = 0; i < 8; ++i) v[i] = through<ACT>(g[i], v[i]);
           } else if (q.add) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += g[i];
@@ -383,7 +393,7 @@ int columns_of(int n) {
   return wcn_ce_round((n + tiles - 1) / tiles, 16);
 }
 
-template <bool A_MN, bool B_MN> int launch(Params& p, const void* a_planes, const void* b_planes, cudaStream_t st) {
+template <bool A_MN, bool B_MN, int ACT, bool GRAD> int launch(Params& p, const void* a_planes, const void* b_planes, cudaStream_t st) {
   const wcn_linear_product& q = p.q;
   p.NT = columns_of(q.n);
   p.m_tiles = (q.m + TILE_M - 1) / TILE_M;
@@ -400,6 +410,7 @@ template <bool A_MN, bool B_MN> int launch(Params& p, const void* a_planes, cons
   while (p.tmem_cols < p.accs * p.stride) p.tmem_cols *= 2;
   auto boundary = [](const void* at, int64_t ld) { return !at || (reinterpret_cast<uintptr_t>(at) % 32 == 0 && ld % 8 == 0); };
   p.vec = boundary(q.out, q.out_ld) && boundary(q.add, q.add_ld);
+  p.vec_bias = reinterpret_cast<uintptr_t>(q.bias) % 16 == 0;
   const int fixed = 1024 + (int)sizeof(Control) + 64 + (p.slab_ones ? CHUNK : 0), stage = 3 * (A_PLANE + p.b_plane);
   p.stages = (SMEM_BUDGET - fixed) / stage;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
@@ -407,7 +418,7 @@ template <bool A_MN, bool B_MN> int launch(Params& p, const void* a_planes, cons
   const bool ok = (A_MN ? parts_map(&a, a_planes, q.k, q.m, SLICE) : parts_map(&a, a_planes, q.m, q.k, TILE_M)) &&
                   (B_MN ? parts_map(&b, b_planes, q.k, q.n, SLICE) : parts_map(&b, b_planes, q.n, q.k, p.NT));
   if (!ok) return WCN_ERR_UNSUPPORTED_CONFIG;
-  constexpr auto kern = linear_split_kernel<A_MN, B_MN>;
+  constexpr auto kern = linear_split_kernel<A_MN, B_MN, ACT, GRAD>;
   if (!allow_smem<kern>()) return WCN_ERR_INITIALIZATION;
   const int sms = wcn_num_sms();
   kern<<<(unsigned)(p.units < sms ? p.units : sms), THREADS, (size_t)fixed + (size_t)p.stages * stage, st>>>(a, b, p);
@@ -444,10 +455,17 @@ int wcn_linear_split(const wcn_linear_product& q, bool by_k, const void* a_plane
   p.b_k = 1;
   p.splits = 1;
   p.dev_status = dev_status;
-  if (!by_k) return launch<false, false>(p, a_planes, b_planes, st);
+  if (!by_k) {
+    switch (q.act) {
+      case WCN_ACT_RELU: return q.grad ? launch<false, false, WCN_ACT_RELU, true>(p, a_planes, b_planes, st) : launch<false, false, WCN_ACT_RELU, false>(p, a_planes, b_planes, st);
+      case WCN_ACT_SILU: return q.grad ? launch<false, false, WCN_ACT_SILU, true>(p, a_planes, b_planes, st) : launch<false, false, WCN_ACT_SILU, false>(p, a_planes, b_planes, st);
+      case WCN_ACT_GELU: return q.grad ? launch<false, false, WCN_ACT_GELU, true>(p, a_planes, b_planes, st) : launch<false, false, WCN_ACT_GELU, false>(p, a_planes, b_planes, st);
+      default: return launch<false, false, WCN_ACT_NONE, false>(p, a_planes, b_planes, st);   // (its gradient asks for no z)
+    }
+  }
   p.q.b_ld = 1;
   p.b_k = q.b_ld;
-  return launch<false, true>(p, a_planes, b_planes, st);
+  return launch<false, true, WCN_ACT_NONE, false>(p, a_planes, b_planes, st);
 }
 
 // The sums of parts of the rows of a [k][m] and b [k][n]: a^T b, and those of a.
@@ -461,7 +479,7 @@ int wcn_linear_split_weight(const wcn_ce_product& c, const void* a_planes, const
   p.slab_ones = c.slab_ones;
   p.splits = c.splits;
   p.dev_status = dev_status;
-  return launch<true, true>(p, a_planes, b_planes, st);
+  return launch<true, true, WCN_ACT_NONE, false>(p, a_planes, b_planes, st);
 }
 
 // Parts of the rows with which the tiles keep every multiprocessor busy.

@@ -16,7 +16,7 @@ from .group_norm import _ACTIVATIONS, _rows, check_activation
 from .linear_cross_entropy import _matrix
 from .rms_norm import E4M3, check_residual, no_gradient
 
-_MOST, _MOST_INPUTS, _MOST_OUTPUTS = 0x7FFFFEFF, 32768, 1 << 20
+_MOST, _MOST_INPUTS, _MOST_OUTPUTS = 0x7FFE0000, 32768, 1 << 20
 
 
 def _check_shapes(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
@@ -121,9 +121,10 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
 
     All tensors are of one dtype, float32, float16 or bfloat16 (under autocast they are brought to its dtype).  ``activation``: None,
     ``"relu"``, ``"silu"`` or ``"gelu"`` (of the error function).  ``dropout_p`` and ``seed`` as in :func:`dropout`; a probability of 0
-    drops nothing.  The gradient computes the activation's argument again; beside its results it takes the gradient behind the
-    activation for pieces of at most 64 MB, and fp32 sums of ``weight``'s gradient.  In 16 bits that gradient is rounded to ``x``'s
-    dtype before its products.  At most 32 768 inputs and 2^20 outputs."""
+    drops nothing.  The gradient computes the activation's argument again; beside its results it takes fp32 sums of ``weight``'s
+    gradient and, for wider layers, the gradient behind the activation in pieces of at most 512 MB.  In 16 bits that gradient is
+    rounded to ``x``'s dtype before its products.  In fp32 the operands are made into sums of three bf16 numbers, 6 bytes for each, in
+    pieces of at most 512 MB too.  At most 32 768 inputs and 2^20 outputs."""
     check_activation(activation)
     least = check_probability(dropout_p) if dropout_p else 0
     _check_shapes(x, weight, bias)
