@@ -7,6 +7,9 @@
 // accumulator to sums in their registers (four threads a row), since a tensor core's accumulator cuts what is below its last place
 // instead of rounding it, and finish the tile.  A sum that is not finite, for a number that has no parts (infinite, not a number, 2^39 and
 // more) or for its size, is made again on the FMA pipes from the numbers as they came.
+// Bound by the epilogue and by rounds: 20 000 x 64 -> 256 with SiLU, 314 tiles for 148 multiprocessors, takes 7 us for the parts and 25
+// forward, 33 + 18 + 16 for dz, dx and dW, where bytes allow 4 and products 2 each; the bigger 30 000 x 512 -> 256 with GELU 103 both
+// launches, 0.46 PFLOP/s of the tensor pipe's products in bf16.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
 // and frees its tensor memory; its results, and those of a launch that finds the word set, are NaN.
@@ -69,7 +72,8 @@ __device__ __noinline__ float again(const wcn_linear_product& q, int64_t a_k, in
 }
 
 // A_MN, B_MN: rows of A (columns of the result) run along the rows of the operand's matrix, which is [k][m] ([k][n]).  ACT, GRAD: what is
-// made of the sums (a kernel for each: one that has all of them waits for its instructions, 40 us where this takes 2x).
+// made of the sums (a kernel for each: one that has all of them waits for its instructions; 20 000 x 64 -> 256 with SiLU, both launches,
+// 46 us forward where this takes 33).
 template <bool A_MN, bool B_MN, int ACT, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ Params p) {

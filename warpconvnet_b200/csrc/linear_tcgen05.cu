@@ -9,7 +9,15 @@
 // would cost the load/store pipe a line each.  Rows that TMA cannot take (pitches that are no multiple of 16 bytes) go the same way
 // through shared memory and from there in elements.
 // Where they fit beside a ring of four tiles, the columns' rows of B stay in shared memory: a block then has one group of
-// columns, and A alone passes.
+// columns, and A alone passes.  Elsewhere, with 256 columns and eight slices of k and more, two blocks of a cluster share a tile of 256 rows
+// (one instruction for both, B's rows halved between them): half of B's bytes from L2, which bound the wide layers (100 000 x 1 024 ->
+// 1 024 bf16 196 us with a block a tile, 161 with two; of 8-bit operands 116 and 99).
+//
+// Sixteen warps empty the accumulators: with eight, twelve and 24 the layer below took 98, 82 and 78 us where it takes 72.
+// 240 000 rows, bf16, us: 96 -> 384 40 (5.7 TB/s), with GELU 65, with dropout too 117: issue slots, some 270 arithmetic instructions
+// for a warp's 32 x 32 numbers, 60 % of the cycles busy, and as many again for the generator.  384 -> 96 with residual 46 (6.0 TB/s).
+// 60 000 x 256 -> 1 024 with GELU 82, its dz 95 to 100, its dx 40.  100 000 x 1 024 -> 1 024 of 8 bits 99 (2.1 PFLOP/s), with SiLU and
+// residual 113 to 118.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
 // and frees its tensor memory; its results, and those of a launch that finds the word set, are NaN.
