@@ -1,0 +1,112 @@
+"""Nodes of autograd's graph in the extension (csrc/autograd.cpp): what they pass on to Python, and what stands in for them."""
+import gc
+import os
+
+import pytest
+import torch
+
+from warpconvnet_b200 import _native
+from warpconvnet_b200.nn.functional import dropout as dropout_module
+from warpconvnet_b200.nn.functional import linear as linear_module
+from warpconvnet_b200.nn.functional import rms_norm as norm_module
+
+nodes = _native.graph_nodes()
+built = pytest.mark.skipif(nodes is None, reason="the extension was not built here")
+
+
+def test_the_extension_is_built_where_its_compiler_is():
+    assert nodes is not None or not os.path.isfile(_native.AUTOGRAD_PATH)
+
+
+def test_without_the_extension_functions_in_python_stand_in(monkeypatch, tmp_path):
+    monkeypatch.setattr(_native, "AUTOGRAD_PATH", str(tmp_path / "_autograd.so"))
+    assert _native._load_nodes() is None
+    (tmp_path / "_autograd.so").write_bytes(b"no library")
+    assert _native._load_nodes() is None
+
+
+def leaves(*shapes):
+    torch.manual_seed(0)
+    return [torch.randn(s, requires_grad=True) for s in shapes]
+
+
+def linear(x, w, b, r, act=2):
+    with torch.no_grad():
+        y = linear_module.formula(x, w, b, linear_module._NAMES[act], r, 0, 0)
+    return nodes.linear(y, x, w, b, r, None, None, None, act, 0, 0, 0, 0)
+
+
+@built
+def test_a_graph_of_the_gradient_is_the_formula_s():
+    x, w, b, r = leaves((5, 4), (3, 4), (3,), (5, 3))
+    y = linear(x, w, b, r)
+    assert y.grad_fn.name() == "LinearBackward"
+    first = torch.autograd.grad(y.square().sum(), [x, w, b, r], create_graph=True)
+    want = torch.autograd.grad(linear_module.formula(x, w, b, "silu", r, 0, 0).square().sum(), [x, w, b, r], create_graph=True)
+    for a, e in zip(first, want):
+        torch.testing.assert_close(a, e, rtol=0, atol=0)
+    second = torch.autograd.grad(first[0].square().sum(), [w], create_graph=True)
+    torch.testing.assert_close(second, torch.autograd.grad(want[0].square().sum(), [w], create_graph=True), rtol=2 ** -18, atol=2 ** -18)
+
+
+@built
+def test_norm_and_dropout():
+    x, r, g = leaves((5, 4), (5, 4), (4,))
+    with torch.no_grad():
+        y, h = norm_module.formula(x, g, 1e-6, r)
+    nodes.norm(y, h, x, r, g, torch.ones(5), 1e-6, 0)
+    got = torch.autograd.grad(y.square().sum() + h.sum(), [x, r, g], create_graph=True)
+    a, b = norm_module.formula(x, g, 1e-6, r)
+    torch.testing.assert_close(got, torch.autograd.grad(a.square().sum() + b.sum(), [x, r, g]))
+    with torch.no_grad():
+        y, h = norm_module.formula(x, g, 1e-6, r)
+    nodes.norm(y, h, x, r, g, torch.ones(5), 1e-6, 0)
+    assert all((t == 1).all() for t in torch.autograd.grad(h.sum(), [x, r]))   # the sum alone was used
+    with torch.no_grad():
+        y = dropout_module.formula(x, 20000, 5, r)
+    nodes.dropout(y, x, r, None, 20000, 5, 0)
+    dx, dr = torch.autograd.grad(y.sum(), [x, r], create_graph=True)
+    assert torch.equal(dx, dropout_module.formula(torch.ones(5, 4), 20000, 5, None)) and (dr == 1).all()
+
+
+@built
+def test_errors_are_the_engine_s(monkeypatch):
+    x, w, b, r = leaves((5, 4), (3, 4), (3,), (5, 3))
+    y = linear(x, w, b, r)
+
+    def refuses(*_):
+        raise ValueError("not today")
+    with monkeypatch.context() as m:
+        m.setattr(linear_module, "formula", refuses)
+        with pytest.raises(ValueError, match="not today"):
+            torch.autograd.grad(y.sum(), [x], create_graph=True)
+    y = linear(x, w, b, r)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), [x], create_graph=True)
+    y = linear(x, w, b, r)
+    torch.autograd.grad(y.sum(), [x], create_graph=True, retain_graph=False)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y.sum(), [x], create_graph=True)
+
+
+@built
+def test_what_a_node_keeps_goes_with_it():
+    x, w, b = leaves((5, 4), (3, 4), (3,))
+    kept = [0]
+
+    class Packed:
+        def __init__(self, t):
+            self.t = t
+            kept[0] += 1
+
+        def __del__(self):
+            kept[0] -= 1
+    with torch.autograd.graph.saved_tensors_hooks(Packed, lambda p: p.t):
+        y = linear(x, w, b, None)
+    assert kept[0] == 3
+    torch.autograd.grad(y.sum(), [x], create_graph=True, retain_graph=True)
+    del y
+    gc.collect()
+    assert kept[0] == 0

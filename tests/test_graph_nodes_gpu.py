@@ -1,0 +1,178 @@
+"""Gradients through the nodes of csrc/autograd.cpp and through autograd functions in Python: the same bits, whatever lies how."""
+import threading
+
+import pytest
+import torch
+
+from warpconvnet_b200 import _native
+from warpconvnet_b200.nn.functional import dropout as dropout_module
+from warpconvnet_b200.nn.functional import linear as linear_module
+from warpconvnet_b200.nn.functional import rms_norm as norm_module
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def leaf(*shape, dtype):
+    return torch.randn(*shape, device=DEV).to(dtype).requires_grad_()
+
+
+def wide(t):
+    """The same numbers as a column block of a wider buffer."""
+    buffer = torch.empty(t.shape[0], t.shape[1] + 13, dtype=t.dtype, device=t.device)
+    buffer[:, 5:5 + t.shape[1]] = t.detach()
+    return buffer[:, 5:5 + t.shape[1]].requires_grad_()
+
+
+def both(monkeypatch, call):
+    """``call()``'s results through the nodes and through Python."""
+    assert _native.graph_nodes() is not None
+    one = call()
+    with monkeypatch.context() as m:
+        for module in (linear_module, dropout_module, norm_module):
+            m.setattr(module, "graph_nodes", lambda: None)
+        return one, call()
+
+
+def same(one, two):
+    assert len(one) == len(two)
+    for a, b in zip(one, two):
+        assert (a is None) == (b is None) and (a is None or (a.dtype == b.dtype and torch.equal(a, b)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, k, m", [(1, 8, 8), (300, 96, 20), (257, 13, 200), (130, 64, 384), (200, 384, 96)])
+@pytest.mark.parametrize("lies", ["rows", "wide", "expanded"])
+def test_linear(monkeypatch, dtype, n, k, m, lies):
+    torch.manual_seed(0)
+    x, w, b, r = leaf(n, k, dtype=dtype), leaf(m, k, dtype=dtype), leaf(m, dtype=dtype), leaf(n, m, dtype=dtype)
+    dy = torch.randn(n, m, device=DEV).to(dtype)
+    if lies == "wide":
+        x, w, r, dy = wide(x), wide(w), wide(r), wide(dy).detach()
+    elif lies == "expanded":
+        dy = dy[:1, :1].expand(n, m)
+    for activation, p, seed in ((None, 0.0, None), ("gelu", 0.25, 7), ("silu", 0.1, torch.tensor([11], device=DEV)), (None, 0.5, -3)):
+        for inputs in ([x, w, b, r], [x], [w, b], [r]):
+            same(*both(monkeypatch, lambda: torch.autograd.grad(linear_module.linear(x, w, b, activation, r, p, seed), inputs, dy)))
+        same(*both(monkeypatch, lambda: torch.autograd.grad(linear_module.linear(x, w, None, activation, None, p, seed), [x, w], dy)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, c", [(1, 1), (300, 96), (77, 13), (9, 2048)])
+@pytest.mark.parametrize("lies", ["rows", "wide", "expanded"])
+def test_norm(monkeypatch, dtype, n, c, lies):
+    torch.manual_seed(0)
+    x, r = leaf(n, c, dtype=dtype), leaf(n, c, dtype=dtype)
+    dy, dh = torch.randn(n, c, device=DEV).to(dtype), torch.randn(n, c, device=DEV).to(dtype)
+    if lies == "wide":
+        x, r, dy, dh = wide(x), wide(r), wide(dy).detach(), wide(dh).detach()
+    elif lies == "expanded":
+        dy, dh = dy[:1, :1].expand(n, c), dh[:1, :1].expand(n, c)
+    for w in (leaf(c, dtype=torch.float32), leaf(c, dtype=dtype), None):
+        some = [] if w is None else [w]
+        same(*both(monkeypatch, lambda: torch.autograd.grad(norm_module.rms_norm(x, w), [x] + some, dy)))
+        for inputs in ([x, r] + some, [r], some or [x]):
+            same(*both(monkeypatch, lambda: torch.autograd.grad(norm_module.rms_norm(x, w, residual=r), inputs, [dy, dh])))
+            same(*both(monkeypatch, lambda: torch.autograd.grad(norm_module.rms_norm(x, w, residual=r)[0], inputs, dy)))
+        same(*both(monkeypatch, lambda: torch.autograd.grad(norm_module.rms_norm(x, w, residual=r)[1], [x, r], dh)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, c", [(0, 8), (1, 1), (300, 96), (77, 13)])
+@pytest.mark.parametrize("lies", ["rows", "wide"])
+def test_dropout(monkeypatch, dtype, n, c, lies):
+    torch.manual_seed(0)
+    x, r, dy = leaf(n, c, dtype=dtype), leaf(n, c, dtype=dtype), torch.randn(n, c, device=DEV).to(dtype)
+    if lies == "wide":
+        x, r, dy = wide(x), wide(r), wide(dy).detach()
+    for p, seed in ((0.1, 5), (1.0, 5), (0.5, torch.tensor([-9], device=DEV))):
+        for inputs in ([x, r], [x], [r]):
+            same(*both(monkeypatch, lambda: torch.autograd.grad(dropout_module.dropout(x, p, seed, r), inputs, dy)))
+        same(*both(monkeypatch, lambda: torch.autograd.grad(dropout_module.dropout(x, p, seed), [x], dy)))
+
+
+def block(x, g, w1, b1, w2, seed):
+    t = norm_module.rms_norm(x, g)
+    t = linear_module.linear(t, w1, b1, "gelu", dropout_p=0.1, seed=seed)
+    return dropout_module.dropout(linear_module.linear(t, w2), 0.2, seed, x)
+
+
+def block_leaves(dtype=torch.bfloat16):
+    torch.manual_seed(0)
+    return leaf(500, 64, dtype=dtype), leaf(64, dtype=torch.float32), leaf(256, 64, dtype=dtype), leaf(256, dtype=dtype), leaf(64, 256, dtype=dtype)
+
+
+def test_launches_are_counted():
+    tensors = block_leaves()
+    before = {k: _native.LAUNCH_COUNTS[k] for k in ("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout")}
+    y = block(*tensors, 3)
+    assert _native.LAUNCH_COUNTS["wcn_dropout"] == before["wcn_dropout"] + 1
+    total = _native.launches_total()
+    y.backward(torch.ones_like(y))
+    assert _native.LAUNCH_COUNTS["wcn_dropout"] == before["wcn_dropout"] + 2
+    assert all(_native.LAUNCH_COUNTS[k] > v for k, v in before.items()) and _native.launches_total() >= total + 5
+
+
+def test_kept_graphs_checkpoints_streams_and_threads():
+    tensors = list(block_leaves())
+    dy = torch.randn(500, 64, device=DEV).bfloat16()
+    want = torch.autograd.grad(block(*tensors, 3), tensors, dy)
+    y = block(*tensors, 3)
+    same(torch.autograd.grad(y, tensors, dy, retain_graph=True), want)
+    same(torch.autograd.grad(y, tensors, dy), want)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, tensors, dy)
+    y = torch.utils.checkpoint.checkpoint(block, *tensors, 3, use_reentrant=False)
+    same(torch.autograd.grad(y, tensors, dy), want)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = torch.autograd.grad(block(*tensors, 3), tensors, dy)
+    stream.synchronize()
+    same(got, want)
+    results = [None] * 4
+
+    def work(i):
+        for _ in range(5):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                results[i] = torch.autograd.grad(block(*tensors, 3), tensors, dy)
+                torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for got in results:
+        same(got, want)
+
+
+def test_gradient_of_the_gradient():
+    x, w = leaf(20, 8, dtype=torch.float32), leaf(8, 8, dtype=torch.float32)
+    first, = torch.autograd.grad(linear_module.linear(x, w, activation="gelu").sum(), [x], create_graph=True)
+    got, = torch.autograd.grad(first.square().sum(), [w])
+    first, = torch.autograd.grad(torch.nn.functional.gelu(x.double() @ w.double().t()).sum(), [x], create_graph=True)
+    want, = torch.autograd.grad(first.double().square().sum(), [w])
+    # sums of 20 x 8 terms, each of some ten fp32 operations, first in x's gradient (8 terms) and again in w's (20)
+    assert (got - want).abs().max() <= 400 * 2 ** -24 * want.abs().max()
+
+
+def test_captured_with_a_seed_on_the_device():
+    tensors = block_leaves()
+    seed = torch.tensor([5], device=DEV)
+    dy = torch.randn(500, 64, device=DEV).bfloat16()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            torch.autograd.grad(block(*tensors, seed), tensors, dy)
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(block(*tensors, seed), tensors, dy)
+    for value in (5, 77):
+        seed.fill_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        same(got, torch.autograd.grad(block(*tensors, value), tensors, dy))

@@ -20,6 +20,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libwcn_b200.so")
 FASTCALL_PATH = os.path.join(_HERE, "csrc", "_fastcall.so")
+AUTOGRAD_PATH = os.path.join(_HERE, "csrc", "_autograd.so")
 
 WCN_F32, WCN_F16, WCN_BF16 = 0, 1, 2
 CONV_AUTO, CONV_SIMT, CONV_TCGEN05 = 0, 1, 2
@@ -140,6 +141,7 @@ class NetOp(ctypes.Structure):
 
 
 _lib = None
+_nodes = False   # see graph_nodes; not asked for yet
 
 # Kernels launched by one call of each entry point (0: host-only query).  Used to
 # count this library's launches, e.g. by the benchmark harness.
@@ -153,7 +155,32 @@ KERNELS_PER_CALL = {
     "wcn_adamw_step": 1, "wcn_adamw_decode": 1, "wcn_group_norm": 1, "wcn_group_norm_backward": 1, "wcn_linear_ce": 1, "wcn_linear_ce_backward": 1,
     "wcn_rms_norm": 1, "wcn_rms_norm_backward": 1, "wcn_quantize_rows": 1, "wcn_dropout": 1, "wcn_linear": 1, "wcn_linear_8bit": 1, "wcn_linear_backward": 1,
 }
-LAUNCH_COUNTS: Counter = Counter()
+
+
+class _LaunchCounts(Counter):
+    """Kernels launched through each entry point.  Those of the graph's nodes, which launch without Python, are added when they are asked for."""
+
+    def _with_nodes(self):
+        if _nodes:
+            for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout"), _nodes.launches()):
+                if kernels:
+                    self[name] = self.get(name, 0) + kernels
+        return self
+
+    def __getitem__(self, name):
+        return super(_LaunchCounts, self._with_nodes()).__getitem__(name)
+
+    def items(self):
+        return super(_LaunchCounts, self._with_nodes()).items()
+
+    def values(self):
+        return super(_LaunchCounts, self._with_nodes()).values()
+
+    def clear(self):
+        super(_LaunchCounts, self._with_nodes()).clear()
+
+
+LAUNCH_COUNTS = _LaunchCounts()
 
 
 def _counted(raw, name: str, kernels: Optional[int]):
@@ -162,7 +189,7 @@ def _counted(raw, name: str, kernels: Optional[int]):
         return raw
 
     def fn(*args):
-        LAUNCH_COUNTS[name] += kernels
+        LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + kernels
         return raw(*args)
     return fn
 
@@ -175,6 +202,7 @@ class _Library:
     ``bind`` is None and ctypes makes the same calls."""
 
     def __init__(self, handle, bind):
+        self.handle = handle
         for name, argtypes in SIGNATURES.items():
             fn = getattr(handle, name)
             fn.argtypes, fn.restype = argtypes, ctypes.c_int
@@ -192,12 +220,12 @@ class _Library:
 def count_f32_launches(name: str) -> None:
     """Corrects what the call just made was counted as: with a workspace ``wcn_conv_fwd`` launches one or two kernels,
     ``wcn_conv_wgrad_f32`` two or three."""
-    LAUNCH_COUNTS[name] += lib().wcn_conv_f32_launches() - KERNELS_PER_CALL[name]
+    LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + lib().wcn_conv_f32_launches() - KERNELS_PER_CALL[name]
 
 
 def count_training_launches(name: str) -> None:
     """The same for group norm, linear cross entropy, AdamW, the gradient of RMS norm and linear layers, which launch as many kernels as their sizes ask for."""
-    LAUNCH_COUNTS[name] += lib().wcn_training_launches() - KERNELS_PER_CALL[name]
+    LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + lib().wcn_training_launches() - KERNELS_PER_CALL[name]
 
 
 def launches_total() -> int:
@@ -235,6 +263,35 @@ def _fastcall_bind():
     except ImportError:
         return None
     return fastcall.bind
+
+
+_NODES_CALL = ("wcn_status_string", "wcn_training_launches", "wcn_linear_workspace_bytes", "wcn_linear_backward", "wcn_rms_norm_workspace_bytes",
+               "wcn_rms_norm_backward", "wcn_dropout")
+
+
+def graph_nodes():
+    """The ``_autograd`` extension (csrc/autograd.cpp), whose nodes of autograd's graph call the library's gradients themselves, or None
+    where it was not built or does not load: autograd functions in Python make the same calls."""
+    global _nodes
+    if _nodes is False:
+        _nodes = _load_nodes()
+    return _nodes
+
+
+def _load_nodes():
+    if not os.path.isfile(AUTOGRAD_PATH):
+        return None
+    try:
+        spec = importlib.util.spec_from_file_location("_autograd", AUTOGRAD_PATH)
+        nodes = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(nodes)
+    except ImportError:
+        return None
+    from .nn.functional import dropout, linear, rms_norm  # (names of modules; they import this one)
+    handle = lib().handle
+    nodes.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in _NODES_CALL}, linear.gradients, rms_norm.gradients,
+               dropout.gradients)
+    return nodes
 
 
 def status_string(status: int) -> str:

@@ -1,5 +1,6 @@
-"""Build libwcn_b200.so in this folder with nvcc for sm_100a (no other architecture), and the _fastcall.so extension
-through which Python calls it where that can be built (ctypes makes the calls elsewhere).
+"""Build libwcn_b200.so in this folder with nvcc for sm_100a (no other architecture), and where they can be built the _fastcall.so
+extension through which Python calls it (ctypes makes the calls elsewhere) and the _autograd.so extension whose graph nodes call it
+(autograd functions in Python do elsewhere).
 
 Usage: ``python -m warpconvnet_b200.csrc.build [--force] [--verbose]``
 """
@@ -16,6 +17,7 @@ SOURCES = ["api.cu", "hash_kmap.cu", "brick_kmap.cu", "cell_kmap.cu", "morton_so
 HEADERS = ["wcn_common.cuh", "tile_order.cuh", "tcgen05_common.cuh", "split_bf16.cuh", "tma_common.cuh", "linear_ce.cuh", "philox.cuh", "linear.cuh", "linear_16bit.cuh", "linear_fp32.cuh", os.path.join("..", "..", "include", "wcn_b200.h")]
 LIB = os.path.join(HERE, "libwcn_b200.so")
 FASTCALL_SOURCE, FASTCALL = os.path.join(HERE, "fastcall.c"), os.path.join(HERE, "_fastcall.so")
+AUTOGRAD_SOURCE, AUTOGRAD = os.path.join(HERE, "autograd.cpp"), os.path.join(HERE, "_autograd.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--use_fast_math=false"]
 
@@ -47,8 +49,28 @@ def build_fastcall(force=False):
             print(f"_fastcall.so was not built ({e}): calls go through ctypes")
 
 
+def build_autograd(force=False):
+    header = os.path.join(HERE, "..", "..", "include", "wcn_b200.h")
+    if not force and os.path.isfile(AUTOGRAD) and os.path.getmtime(AUTOGRAD) > max(os.path.getmtime(AUTOGRAD_SOURCE), os.path.getmtime(header)):
+        return
+    try:
+        import torch
+        root = os.path.dirname(torch.__file__)
+        cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *("-I" + i for i in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
+                                    sysconfig.get_paths()["include"])),
+               AUTOGRAD_SOURCE, "-o", AUTOGRAD, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+        subprocess.check_call(cmd)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:  # no compiler, no headers
+        if os.path.isfile(AUTOGRAD):
+            os.remove(AUTOGRAD)  # (of an earlier source)
+        print(f"_autograd.so was not built ({e}): gradients go through Python")
+
+
 def build(force=False, verbose=False, ptxas_info=False):
     build_fastcall(force)
+    build_autograd(force)
     if not force and not needs_build():
         return LIB
     flags = [f for f in NVCC_FLAGS if not f.startswith("--use_fast_math")]

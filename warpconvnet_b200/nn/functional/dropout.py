@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 from torch import Tensor
 
-from ..._native import check, dtype_code, lib, on_device, ptr, require_cuda, stream_ptr
+from ..._native import check, dtype_code, graph_nodes, lib, on_device, ptr, require_cuda, stream_ptr
 from .batch_norm import reverse_mode_only
 from .group_norm import _rows
 from .rms_norm import check_residual
@@ -79,21 +79,28 @@ def _run(x: Tensor, least: int, seed: Union[int, Tensor], residual: Optional[Ten
     return y
 
 
+def gradients(seed: Optional[Tensor], least: int, number: int, needs, dy: Tensor):
+    """Those of x and residual.  ``seed``: a tensor, or None where it is ``number``."""
+    need_x, need_r = needs
+    seed = number if seed is None else seed
+    dx = None
+    if need_x:
+        dx = formula(dy, least, seed, None) if torch.is_grad_enabled() else _run(dy, least, seed, None)
+    return dx, dy if need_r else None
+
+
 class _Dropout(torch.autograd.Function):
+    """What a graph's node of ``csrc/autograd.cpp`` is, where that was not built."""
+
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], least: int, seed: Union[int, Tensor]):
-        ctx.least, ctx.seed = least, None if isinstance(seed, Tensor) else seed
+        ctx.call = least, 0 if isinstance(seed, Tensor) else seed
         ctx.save_for_backward(seed if isinstance(seed, Tensor) else None)   # (one that was changed meanwhile is an error)
         return _run(x, least, seed, residual)
 
     @staticmethod
     def backward(ctx, dy: Tensor):
-        need_x, need_r = ctx.needs_input_grad[:2]
-        seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
-        dx = None
-        if need_x:
-            dx = formula(dy, ctx.least, seed, None) if torch.is_grad_enabled() else _run(dy, ctx.least, seed, None)
-        return dx, dy if need_r else None, None, None
+        return gradients(*ctx.saved_tensors, *ctx.call, ctx.needs_input_grad[:2], dy) + (None, None)
 
 
 def dropout(x: Tensor, p: float = 0.5, seed: Union[int, Tensor, None] = None, residual: Optional[Tensor] = None) -> Tensor:
@@ -118,5 +125,12 @@ def dropout(x: Tensor, p: float = 0.5, seed: Union[int, Tensor, None] = None, re
     if not reverse_mode_only():
         return formula(x, least, seed, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, least, seed)
+        nodes = graph_nodes()
+        if nodes is None:
+            return _Dropout.apply(x, residual, least, seed)
+        with torch.no_grad():
+            y = _run(x, least, seed, residual)
+        at, number = (seed, 0) if isinstance(seed, Tensor) else (None, seed)
+        nodes.dropout(y, x, residual, at, least, number, dtype_code(x.dtype))
+        return y
     return _run(x, least, seed, residual)

@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 from torch import Tensor
 
-from ..._native import WCN_F32, check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import WCN_F32, check, count_training_launches, device_status, dtype_code, graph_nodes, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import reverse_mode_only
 from .dropout import check_probability, check_seed, kept_factor, new_seed
 from .group_norm import _ACTIVATIONS, _rows, check_activation
@@ -17,6 +17,7 @@ from .linear_cross_entropy import _matrix
 from .rms_norm import E4M3, check_residual, no_gradient
 
 _MOST, _MOST_INPUTS, _MOST_OUTPUTS = 0x7FFE0000, 32768, 1 << 20
+_NAMES = {code: name for name, code in _ACTIVATIONS.items()}
 
 
 def _check_shapes(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
@@ -70,49 +71,55 @@ def formula(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optio
     return (y if residual is None else y + residual.float()).to(x.dtype)
 
 
+def gradients(x: Tensor, weight: Tensor, bias: Optional[Tensor], seed, x_rows: Optional[Tensor], w_rows: Optional[Tensor], act: int, least: int,
+              number: int, code: int, needs, dy: Tensor):
+    """Those of x, weight, bias and residual.  ``seed``: a tensor, or None where it is ``number``; ``x_rows``, ``w_rows``: copies that the
+    forward call has made."""
+    seed = number if seed is None else seed
+    need_x, need_w, need_b, need_r = needs
+    d_residual = dy if need_r else None
+    if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+        y = formula(x, weight, bias, _NAMES[act], None, least, seed)
+        wanted = [t for t, need in zip((x, weight, bias), (need_x, need_w, need_b)) if need]
+        got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True) if wanted else ())
+        return tuple(next(got) if need else None for need in (need_x, need_w, need_b)) + (d_residual,)
+    if not (need_x or need_w or need_b):
+        return None, None, None, d_residual
+    (n, k), m, dev = x.shape, weight.shape[0], x.device
+    dx = x.new_empty((n, k)) if need_x else None
+    dw = weight.new_empty((m, k)) if need_w else None
+    db = weight.new_empty(m) if need_b else None
+    dy, dy_ld = (dy, m) if dy.is_contiguous() else _rows(dy)
+    whole = 1 if code == WCN_F32 else 8
+    aligned = dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
+    x, x_ld = _operand(x if x_rows is None else x_rows, whole, k)
+    weight, w_ld = _operand(weight if w_rows is None else w_rows, whole, k)
+    bias = None if bias is None else bias.contiguous()
+    number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
+    size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, act, least, int(aligned))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with on_device(dev):
+        check(lib().wcn_linear_backward(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, dy.data_ptr(), dy_ld, least, number, at,
+                                        ptr(dx), ptr(dw), ptr(db), ptr(ws), size, device_status(dev).data_ptr(), stream_ptr(dev)),
+              "wcn_linear_backward")
+        count_training_launches("wcn_linear_backward")
+    return dx, dw, db, d_residual
+
+
 class _Linear(torch.autograd.Function):
+    """What a graph's node of ``csrc/autograd.cpp`` is, where that was not built."""
+
     @staticmethod
-    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: Optional[str], least: int, seed,
-                code: int):
-        y, x_rows, w_rows = _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)
-        ctx.activation, ctx.least, ctx.seed, ctx.code = activation, least, None if isinstance(seed, Tensor) else seed, code
+    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], act: int, least: int, seed, code: int):
+        y, x_rows, w_rows = _forward(x, weight, None if bias is None else bias.contiguous(), act, residual, least, seed, code)
+        ctx.call = act, least, 0 if isinstance(seed, Tensor) else seed, code
         # (matrices that had to be copied are kept with them: there are not two copies to be made)
         ctx.save_for_backward(x, weight, bias, seed if isinstance(seed, Tensor) else None, None if x_rows is x else x_rows, None if w_rows is weight else w_rows)
         return y
 
     @staticmethod
     def backward(ctx, dy: Tensor):
-        x, weight, bias, seed, x_rows, w_rows = ctx.saved_tensors
-        seed = ctx.seed if seed is None else seed
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        d_residual = dy if need_r else None
-        if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
-            y = formula(x, weight, bias, ctx.activation, None, ctx.least, seed)
-            wanted = [t for t, need in zip((x, weight, bias), (need_x, need_w, need_b)) if need]
-            got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True) if wanted else ())
-            return tuple(next(got) if need else None for need in (need_x, need_w, need_b)) + (d_residual, None, None, None, None)
-        if not (need_x or need_w or need_b):
-            return None, None, None, d_residual, None, None, None, None
-        (n, k), m, dev = x.shape, weight.shape[0], x.device
-        code, act = ctx.code, _ACTIVATIONS[ctx.activation]
-        dx = x.new_empty((n, k)) if need_x else None
-        dw = weight.new_empty((m, k)) if need_w else None
-        db = weight.new_empty(m) if need_b else None
-        dy, dy_ld = (dy, m) if dy.is_contiguous() else _rows(dy)
-        whole = 1 if code == WCN_F32 else 8
-        aligned = dy_ld % whole == 0 and dy.data_ptr() % (2 * whole) == 0
-        x, x_ld = _operand(x if x_rows is None else x_rows, whole, k)
-        weight, w_ld = _operand(weight if w_rows is None else w_rows, whole, k)
-        bias = None if bias is None else bias.contiguous()
-        number, at = (0, seed.data_ptr()) if isinstance(seed, Tensor) else (seed, None)
-        size = query_bytes("wcn_linear_workspace_bytes", n, k, m, code, need_x + 2 * need_w + 4 * need_b, act, ctx.least, int(aligned))
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        with on_device(dev):
-            check(lib().wcn_linear_backward(x.data_ptr(), x_ld, n, k, weight.data_ptr(), w_ld, m, code, ptr(bias), act, dy.data_ptr(), dy_ld, ctx.least, number, at,
-                                            ptr(dx), ptr(dw), ptr(db), ptr(ws), size, device_status(dev).data_ptr(), stream_ptr(dev)),
-                  "wcn_linear_backward")
-            count_training_launches("wcn_linear_backward")
-        return dx, dw, db, d_residual, None, None, None, None
+        return gradients(*ctx.saved_tensors, *ctx.call, ctx.needs_input_grad[:4], dy) + (None, None, None, None)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, residual: Optional[Tensor] = None,
@@ -144,7 +151,14 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
         return formula(x, weight, bias, activation, residual, least, seed)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
-        return _Linear.apply(x, weight, bias, residual, activation, least, seed, code)
+        nodes, act = graph_nodes(), _ACTIVATIONS[activation]
+        if nodes is None:
+            return _Linear.apply(x, weight, bias, residual, act, least, seed, code)
+        with torch.no_grad():
+            y, x_rows, w_rows = _forward(x, weight, None if bias is None else bias.contiguous(), act, residual, least, seed, code)
+        at, number = (seed, 0) if isinstance(seed, Tensor) else (None, seed)
+        return nodes.linear(y, x, weight, bias, residual, at, None if x_rows is x else x_rows, None if w_rows is weight else w_rows, act, least,
+                            number, code, device_status(x.device).data_ptr())
     return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)[0]
 
 

@@ -8,7 +8,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from ..._native import check, count_training_launches, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
+from ..._native import check, count_training_launches, dtype_code, graph_nodes, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
 from .batch_norm import _bits, reverse_mode_only
 from .group_norm import _rows, _vector
 
@@ -77,7 +77,41 @@ def formula(x: Tensor, weight: Optional[Tensor], eps: float, residual: Optional[
     return y if residual is None else (y, h)
 
 
+def gradients(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], h: Optional[Tensor], rstd: Tensor, eps: float, needs, dy: Optional[Tensor],
+              dh: Optional[Tensor] = None):
+    """Those of x, residual and weight."""
+    need_x, need_r, need_w = needs
+    if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+        results = formula(x, weight, eps, residual)
+        pairs = [(t, g) for t, g in zip(results if residual is not None else (results,), (dy, dh)) if g is not None]
+        wanted = [t for t, need in zip((x, residual, weight), (need_x, need_r, need_w)) if need]
+        got = iter(torch.autograd.grad([t for t, _ in pairs], wanted, [g for _, g in pairs], create_graph=True, allow_unused=True) if pairs else
+                   [None] * len(wanted))
+        return tuple(next(got) if need else None for need in (need_x, need_r, need_w))
+    if dy is None:   # the sum alone was used
+        return dh if need_x else None, dh if need_r else None, None
+    n, c = x.shape
+    dev, code = x.device, dtype_code(x.dtype)
+    h, h_ld = _rows(x if h is None else h)
+    dy, dy_ld = (dy, c) if dy.is_contiguous() else _rows(dy)
+    dh_ld = c
+    if dh is not None and not dh.is_contiguous():
+        dh, dh_ld = _rows(dh)
+    dx = x.new_empty((n, c)) if need_x or need_r else None
+    dw = (torch.empty if n else torch.zeros)(c, dtype=torch.float32, device=dev) if need_w else None
+    if n:
+        ws = torch.empty(query_bytes("wcn_rms_norm_workspace_bytes", n, c), dtype=torch.uint8, device=dev) if need_w else None
+        gamma = _vector(weight)
+        with on_device(dev):
+            check(lib().wcn_rms_norm_backward(ptr(h), h_ld, ptr(dy), dy_ld, ptr(dh), dh_ld, n, c, code, ptr(gamma), ptr(rstd), ptr(dx), ptr(dw),
+                                              ptr(ws), ws.numel() if need_w else 0, stream_ptr(dev)), "wcn_rms_norm_backward")
+            count_training_launches("wcn_rms_norm_backward")
+    return dx if need_x else None, dx if need_r else None, (dw if weight.dtype == torch.float32 else dw.to(weight.dtype)) if need_w else None
+
+
 class _RMSNorm(torch.autograd.Function):
+    """What a graph's node of ``csrc/autograd.cpp`` is, where that was not built."""
+
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float, code: int):
         y, h, rstd = _forward(x, _vector(weight), eps, residual, code, False, True)
@@ -88,34 +122,7 @@ class _RMSNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy: Optional[Tensor], dh: Optional[Tensor] = None):
-        x, residual, weight, h, rstd = ctx.saved_tensors
-        need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
-            results = formula(x, weight, ctx.eps, residual)
-            pairs = [(t, g) for t, g in zip(results if residual is not None else (results,), (dy, dh)) if g is not None]
-            wanted = [t for t, need in zip((x, residual, weight), (need_x, need_r, need_w)) if need]
-            got = iter(torch.autograd.grad([t for t, _ in pairs], wanted, [g for _, g in pairs], create_graph=True, allow_unused=True) if pairs else
-                       [None] * len(wanted))
-            return tuple(next(got) if need else None for need in (need_x, need_r, need_w)) + (None, None)
-        if dy is None:   # the sum alone was used
-            return dh if need_x else None, dh if need_r else None, None, None, None
-        n, c = x.shape
-        dev, code = x.device, dtype_code(x.dtype)
-        h, h_ld = _rows(x if h is None else h)
-        dy, dy_ld = (dy, c) if dy.is_contiguous() else _rows(dy)
-        dh_ld = c
-        if dh is not None and not dh.is_contiguous():
-            dh, dh_ld = _rows(dh)
-        dx = x.new_empty((n, c)) if need_x or need_r else None
-        dw = (torch.empty if n else torch.zeros)(c, dtype=torch.float32, device=dev) if need_w else None
-        if n:
-            ws = torch.empty(query_bytes("wcn_rms_norm_workspace_bytes", n, c), dtype=torch.uint8, device=dev) if need_w else None
-            gamma = _vector(weight)
-            with on_device(dev):
-                check(lib().wcn_rms_norm_backward(ptr(h), h_ld, ptr(dy), dy_ld, ptr(dh), dh_ld, n, c, code, ptr(gamma), ptr(rstd), ptr(dx), ptr(dw),
-                                                  ptr(ws), ws.numel() if need_w else 0, stream_ptr(dev)), "wcn_rms_norm_backward")
-                count_training_launches("wcn_rms_norm_backward")
-        return dx if need_x else None, dx if need_r else None, (dw if weight.dtype == torch.float32 else dw.to(weight.dtype)) if need_w else None, None, None
+        return gradients(*ctx.saved_tensors, ctx.eps, ctx.needs_input_grad[:3], dy, dh) + (None, None)
 
 
 def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
@@ -129,7 +136,13 @@ def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, resi
     if not reverse_mode_only():
         return formula(x, weight, eps, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        return _RMSNorm.apply(x, residual, weight, eps, code)
+        nodes = graph_nodes()
+        if nodes is None:
+            return _RMSNorm.apply(x, residual, weight, eps, code)
+        with torch.no_grad():
+            y, h, rstd = _forward(x, _vector(weight), eps, residual, code, False, True)
+        nodes.norm(y, h, x, residual, weight, rstd, eps, code)
+        return y if residual is None else (y, h)
     y, h, _ = _forward(x, _vector(weight), eps, residual, code, False, False)
     return y if residual is None else (y, h)
 
