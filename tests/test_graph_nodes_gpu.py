@@ -176,3 +176,51 @@ def test_captured_with_a_seed_on_the_device():
         graph.replay()
         torch.cuda.synchronize()
         same(got, torch.autograd.grad(block(*tensors, value), tensors, dy))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lies", ["rows", "wide", "off by one"])
+def test_calls_without_gradient(monkeypatch, dtype, lies):
+    """What the extension runs itself and what it leaves to Python is the same."""
+    torch.manual_seed(0)
+    x, w, b, r = (t.detach() for t in (leaf(77, 40, dtype=dtype), leaf(24, 40, dtype=dtype), leaf(24, dtype=dtype), leaf(77, 24, dtype=dtype)))
+    g = torch.rand(40, device=DEV) + 0.5
+    if lies == "wide":
+        x, w, r = (wide(t).detach() for t in (x, w, r))
+    elif lies == "off by one":   # contiguous, but not on a 16-byte boundary
+        x, w, r = (torch.cat([t.flatten()[:1], t.flatten()])[1:].view_as(t) for t in (x, w, r))
+
+    def call():
+        return [linear_module.linear(x, w, b, "gelu", r, 0.3, 9), linear_module.linear(x, w), linear_module.linear(x, w, b, "relu"),
+                norm_module.rms_norm(x, g), *norm_module.rms_norm(x, None, 1e-3, x), dropout_module.dropout(x, 0.4, 2), dropout_module.dropout(x, 0.4, 2, x)]
+    same(*both(monkeypatch, call))
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in call())
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        same(*both(monkeypatch, lambda: [linear_module.linear(x, w, b, "silu")]))
+        assert linear_module.linear(x, w, b).dtype == torch.bfloat16
+
+
+def test_refusals_are_python_s():
+    x, w = leaf(4, 8, dtype=torch.float32), leaf(8, 8, dtype=torch.float32)
+    for bad in (lambda: linear_module.linear(x, w[:, :4]), lambda: linear_module.linear(x, w, residual=x[:2]), lambda: linear_module.linear(x.cpu(), w),
+                lambda: linear_module.linear(x, w, activation="tanh"),
+                lambda: linear_module.linear(x, w, dropout_p=2.0), lambda: linear_module.linear(x, w, dropout_p=0.5, seed=2 ** 63),
+                lambda: norm_module.rms_norm(x, w[0, :4]), lambda: norm_module.rms_norm(x, eps=float("nan")), lambda: norm_module.rms_norm(x, eps=0.0),
+                lambda: norm_module.rms_norm(x, residual=x.double()), lambda: dropout_module.dropout(x, 0.5, 2 ** 63),
+                lambda: dropout_module.dropout(x, 0.5, 1, x[:, :4]), lambda: dropout_module.dropout(x[0], 0.5, 1)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        linear_module.linear(x, w.half())
+    with pytest.raises(TypeError):
+        norm_module.rms_norm(x.double())
+
+
+def test_forward_mode_and_transforms_go_through_torch():
+    x, w = torch.randn(6, 8, device=DEV), torch.randn(8, 8, device=DEV)
+    t = torch.randn(6, 8, device=DEV)
+    _, got = torch.func.jvp(lambda v: linear_module.linear(v, w), (x,), (t,))
+    torch.testing.assert_close(got, t @ w.t(), rtol=2 ** -18, atol=2 ** -18)
+    stacked = torch.vmap(lambda v: norm_module.rms_norm(v))(torch.stack([x, t]))
+    torch.testing.assert_close(stacked[1], norm_module.rms_norm(t), rtol=2 ** -20, atol=2 ** -20)

@@ -158,11 +158,11 @@ KERNELS_PER_CALL = {
 
 
 class _LaunchCounts(Counter):
-    """Kernels launched through each entry point.  Those of the graph's nodes, which launch without Python, are added when they are asked for."""
+    """Kernels launched through each entry point.  Those of the extension, which launches without Python, are added when they are asked for."""
 
     def _with_nodes(self):
         if _nodes:
-            for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout"), _nodes.launches()):
+            for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm"), _nodes.launches()):
                 if kernels:
                     self[name] = self.get(name, 0) + kernels
         return self
@@ -266,7 +266,7 @@ def _fastcall_bind():
 
 
 _NODES_CALL = ("wcn_status_string", "wcn_training_launches", "wcn_linear_workspace_bytes", "wcn_linear_backward", "wcn_rms_norm_workspace_bytes",
-               "wcn_rms_norm_backward", "wcn_dropout")
+               "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm")
 
 
 def graph_nodes():
@@ -353,6 +353,8 @@ def device_status(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     if key not in _status_words:
         _status_words[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        if device.type == "cuda" and graph_nodes() is not None:
+            _nodes.status(key[1], _status_words[key].data_ptr())
     return _status_words[key]
 
 

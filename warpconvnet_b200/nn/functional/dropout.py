@@ -111,6 +111,11 @@ def dropout(x: Tensor, p: float = 0.5, seed: Union[int, Tensor, None] = None, re
     row and column alone); None: one from torch's generator on the host (while a graph is captured, the device's, another one at
     every replay).  Rows of ``x`` and of the residual may be column blocks of wider buffers."""
     least = check_probability(p)
+    nodes, transformed = graph_nodes(), not reverse_mode_only()
+    if nodes is not None and not transformed and least and type(seed) is int and -2 ** 63 <= seed < 2 ** 63 and isinstance(x, Tensor):
+        y = nodes.run_dropout(x, residual, least, seed, _MOST, _MOST_COLUMNS)
+        if y is not None:
+            return y
     if x.dim() != 2:
         raise ValueError(f"x must be [N, C], got {tuple(x.shape)}")
     require_cuda(x, "x")
@@ -122,10 +127,9 @@ def dropout(x: Tensor, p: float = 0.5, seed: Union[int, Tensor, None] = None, re
     if not least and residual is None:
         return x
     seed = new_seed(x.device) if seed is None else seed
-    if not reverse_mode_only():
+    if transformed:
         return formula(x, least, seed, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        nodes = graph_nodes()
         if nodes is None:
             return _Dropout.apply(x, residual, least, seed)
         with torch.no_grad():

@@ -132,8 +132,13 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     gradient and, for wider layers, the gradient behind the activation in pieces of at most 512 MB.  In 16 bits that gradient is
     rounded to ``x``'s dtype before its products.  In fp32 the operands are made into sums of three bf16 numbers, 6 bytes for each, in
     pieces of at most 512 MB too.  At most 32 768 inputs and 2^20 outputs."""
-    check_activation(activation)
+    act = check_activation(activation)
     least = check_probability(dropout_p) if dropout_p else 0
+    nodes, transformed = graph_nodes(), not reverse_mode_only()
+    if nodes is not None and not transformed and (not least or type(seed) is int and -2 ** 63 <= seed < 2 ** 63) and isinstance(x, Tensor):
+        y = nodes.run_linear(x, weight, bias, residual, act, least, seed if least else 0, _MOST, _MOST_INPUTS, _MOST_OUTPUTS)
+        if y is not None:
+            return y
     _check_shapes(x, weight, bias)
     if torch.is_autocast_enabled():
         dtype = torch.get_autocast_dtype("cuda")
@@ -147,11 +152,10 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     if seed is not None:
         check_seed(seed, x.device)
     seed = new_seed(x.device) if least and seed is None else 0 if not least else seed
-    if not reverse_mode_only() or not x.shape[0]:
+    if transformed or not x.shape[0]:
         return formula(x, weight, bias, activation, residual, least, seed)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
-        nodes, act = graph_nodes(), _ACTIVATIONS[activation]
         if nodes is None:
             return _Linear.apply(x, weight, bias, residual, act, least, seed, code)
         with torch.no_grad():
@@ -159,7 +163,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
         at, number = (seed, 0) if isinstance(seed, Tensor) else (None, seed)
         return nodes.linear(y, x, weight, bias, residual, at, None if x_rows is x else x_rows, None if w_rows is weight else w_rows, act, least,
                             number, code, device_status(x.device).data_ptr())
-    return _forward(x, weight, None if bias is None else bias.contiguous(), _ACTIVATIONS[activation], residual, least, seed, code)[0]
+    return _forward(x, weight, None if bias is None else bias.contiguous(), act, residual, least, seed, code)[0]
 
 
 def _codes(t: Tensor):

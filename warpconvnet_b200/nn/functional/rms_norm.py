@@ -132,11 +132,15 @@ def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, resi
     Without a residual ``h`` is ``x`` and the norm is the result.  With one, ``h = x + residual`` rounded to their dtype, and the
     result is ``(norm, h)``: ``h`` is what the next residual connection adds to.  ``eps`` is at least 1e-30.  Rows of ``x`` and of
     the residual may be column blocks of wider buffers."""
+    nodes, transformed = graph_nodes(), not reverse_mode_only()
+    if nodes is not None and not transformed and isinstance(x, Tensor):
+        results = nodes.run_norm(x, weight, eps, residual, _LEAST_EPS, _MOST, _MOST_CHANNELS)
+        if results is not None:
+            return results
     code = _check(x, weight, eps, residual)
-    if not reverse_mode_only():
+    if transformed:
         return formula(x, weight, eps, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        nodes = graph_nodes()
         if nodes is None:
             return _RMSNorm.apply(x, residual, weight, eps, code)
         with torch.no_grad():
