@@ -147,6 +147,21 @@ def test_kept_graphs_checkpoints_streams_and_threads():
         same(got, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_tensor_in_two_places(monkeypatch, dtype):
+    x, w, dy = leaf(100, 64, dtype=dtype), leaf(64, 64, dtype=dtype), torch.randn(100, 64, device=DEV).to(dtype)
+
+    def leaves(call):
+        x.grad = w.grad = None
+        torch.autograd.backward(call(), [dy] * (2 if isinstance(call(), tuple) else 1))
+        return [t for t in (x.grad, w.grad) if t is not None]
+    for call in (lambda: norm_module.rms_norm(x, residual=x), lambda: linear_module.linear(x, w, activation="relu", residual=x), lambda: linear_module.linear(w, w),
+                 lambda: dropout_module.dropout(x, 0.3, 1, x), lambda: norm_module.rms_norm(x * 2, residual=x)):
+        one, two = both(monkeypatch, lambda: leaves(call))
+        same(one, two)
+        assert len({t.data_ptr() for t in one}) == len(one)
+
+
 def test_gradient_of_the_gradient():
     x, w = leaf(20, 8, dtype=torch.float32), leaf(8, 8, dtype=torch.float32)
     first, = torch.autograd.grad(linear_module.linear(x, w, activation="gelu").sum(), [x], create_graph=True)
@@ -205,7 +220,7 @@ def test_refusals_are_python_s():
     x, w = leaf(4, 8, dtype=torch.float32), leaf(8, 8, dtype=torch.float32)
     for bad in (lambda: linear_module.linear(x, w[:, :4]), lambda: linear_module.linear(x, w, residual=x[:2]), lambda: linear_module.linear(x.cpu(), w),
                 lambda: linear_module.linear(x, w, activation="tanh"),
-                lambda: linear_module.linear(x, w, dropout_p=2.0), lambda: linear_module.linear(x, w, dropout_p=0.5, seed=2 ** 63),
+                lambda: linear_module.linear(x, w, dropout_p=2.0), lambda: linear_module.linear(x, w, dropout_p=0.5, seed=2 ** 63), lambda: linear_module.linear(x, w, seed=2 ** 63),
                 lambda: norm_module.rms_norm(x, w[0, :4]), lambda: norm_module.rms_norm(x, eps=float("nan")), lambda: norm_module.rms_norm(x, eps=0.0),
                 lambda: norm_module.rms_norm(x, residual=x.double()), lambda: dropout_module.dropout(x, 0.5, 2 ** 63),
                 lambda: dropout_module.dropout(x, 0.5, 1, x[:, :4]), lambda: dropout_module.dropout(x[0], 0.5, 1)):

@@ -1,12 +1,13 @@
 // Nodes of autograd's graph for RMS norm, dropout and linear layers: what their gradient needs is kept here, and the engine calls the C
 // entry points without Python.  A training step of small layers waits for the host: an autograd function in Python takes some 50 us both
 // ways before it does anything, most of it for the interpreter's lock in the engine's thread (both ways, us, that way and this: linear
-// 2 000 x 96 -> 20 fp16 123, 96; dropout 2 001 x 64 fp32 81, 64; RMS norm 240 000 x 96 bf16 127, 100).  A node runs the gradient of tensors that lie as the kernels read them; all else (rows that have to be copied, a graph of
-// the gradient) goes to the operator's function in Python, which gives the same.
+// 2 000 x 96 -> 20 fp16 123, 96; dropout 2 001 x 64 fp32 81, 64; RMS norm 240 000 x 96 bf16 127, 100).
+// A node runs the gradient of tensors that lie as the kernels read them; all else (rows that have to be copied, a graph of the gradient)
+// goes to the operator's function in Python, which gives the same.
 //
-// The calls themselves are made here too where nothing has to be copied, cast or refused (one row, us of the host:
-// RMS norm 9 to 5, linear 12 to 6; both ways: linear 2 000 x 96 -> 20 fp16 96 to 73, dropout 64 to 52).  The arguments that the functions here do not take get no result, and Python goes on
-// with them.
+// The calls themselves are made here too where nothing has to be copied, cast or refused (us of the host for one row: RMS norm 9, here 5;
+// linear 12, here 6; the three above both ways then take 73, 52 and 78).  Arguments that the functions here do not take get no result, and
+// Python goes on with them.
 //
 // A way of calling and no more: where this extension is not built, autograd functions in Python make the same calls.
 #include <ATen/ATen.h>

@@ -135,7 +135,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     act = check_activation(activation)
     least = check_probability(dropout_p) if dropout_p else 0
     nodes, transformed = graph_nodes(), not reverse_mode_only()
-    if nodes is not None and not transformed and (not least or type(seed) is int and -2 ** 63 <= seed < 2 ** 63) and isinstance(x, Tensor):
+    if nodes is not None and not transformed and isinstance(x, Tensor) and (type(seed) is int and -2 ** 63 <= seed < 2 ** 63 or seed is None and not least):
         y = nodes.run_linear(x, weight, bias, residual, act, least, seed if least else 0, _MOST, _MOST_INPUTS, _MOST_OUTPUTS)
         if y is not None:
             return y
