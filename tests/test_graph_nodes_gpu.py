@@ -153,7 +153,9 @@ def test_one_tensor_in_two_places(monkeypatch, dtype):
 
     def leaves(call):
         x.grad = w.grad = None
-        torch.autograd.backward(call(), [dy] * (2 if isinstance(call(), tuple) else 1))
+        results = call()
+        results = results if isinstance(results, tuple) else (results,)
+        torch.autograd.backward(results, [dy[:len(t)] for t in results])
         return [t for t in (x.grad, w.grad) if t is not None]
     for call in (lambda: norm_module.rms_norm(x, residual=x), lambda: linear_module.linear(x, w, activation="relu", residual=x), lambda: linear_module.linear(w, w),
                  lambda: dropout_module.dropout(x, 0.3, 1, x), lambda: norm_module.rms_norm(x * 2, residual=x)):
@@ -216,11 +218,35 @@ def test_calls_without_gradient(monkeypatch, dtype, lies):
         assert linear_module.linear(x, w, b).dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("k, m", [(64, 24), (40, 24), (13, 7)])
+def test_calls_in_8_bits(monkeypatch, dtype, k, m):
+    torch.manual_seed(0)
+    x, w, r, g = torch.randn(77, k, device=DEV).to(dtype), torch.randn(m, k, device=DEV), torch.randn(77, m, device=DEV).to(dtype), torch.rand(k, device=DEV)
+    (q, s), (wq, ws) = norm_module.quantize_rows(x), norm_module.quantize_rows(w)
+    other = torch.float16 if dtype == torch.bfloat16 else torch.bfloat16
+
+    def call():
+        got = [*norm_module.rms_norm_8bit(x, g), *norm_module.rms_norm_8bit(x, residual=x)]
+        got = [t.view(torch.uint8) if t.dtype == norm_module.E4M3 else t for t in got]
+        return got + [linear_module.linear_8bit(q, s, wq, ws, r[0], "gelu", r, dtype), linear_module.linear_8bit(q, s, wq, ws, out_dtype=dtype),
+                      linear_module.linear_8bit(q, s, wq, ws, r[0], out_dtype=other), linear_module.linear_8bit(q[::2], s[::2], wq, ws, residual=r[::2], out_dtype=dtype)]
+    same(*both(monkeypatch, call))
+    before = _native.LAUNCH_COUNTS["wcn_linear_8bit"]
+    linear_module.linear_8bit(q, s, wq, ws)
+    assert _native.LAUNCH_COUNTS["wcn_linear_8bit"] == before + 1
+    for bad in (lambda: linear_module.linear_8bit(q, s[:3], wq, ws), lambda: linear_module.linear_8bit(q, s.requires_grad_(), wq, ws),
+                lambda: linear_module.linear_8bit(q, s.detach(), wq, ws, residual=r, out_dtype=other)):
+        with pytest.raises(ValueError):
+            bad()
+
+
 def test_refusals_are_python_s():
     x, w = leaf(4, 8, dtype=torch.float32), leaf(8, 8, dtype=torch.float32)
     for bad in (lambda: linear_module.linear(x, w[:, :4]), lambda: linear_module.linear(x, w, residual=x[:2]), lambda: linear_module.linear(x.cpu(), w),
                 lambda: linear_module.linear(x, w, activation="tanh"),
-                lambda: linear_module.linear(x, w, dropout_p=2.0), lambda: linear_module.linear(x, w, dropout_p=0.5, seed=2 ** 63), lambda: linear_module.linear(x, w, seed=2 ** 63),
+                lambda: linear_module.linear(x, w, dropout_p=2.0), lambda: linear_module.linear(x, w, dropout_p=0.5, seed=2 ** 63),
+                lambda: linear_module.linear(x, w, seed=2 ** 63), lambda: norm_module.rms_norm_8bit(x), lambda: norm_module.rms_norm_8bit(x, eps=0.0),
                 lambda: norm_module.rms_norm(x, w[0, :4]), lambda: norm_module.rms_norm(x, eps=float("nan")), lambda: norm_module.rms_norm(x, eps=0.0),
                 lambda: norm_module.rms_norm(x, residual=x.double()), lambda: dropout_module.dropout(x, 0.5, 2 ** 63),
                 lambda: dropout_module.dropout(x, 0.5, 1, x[:, :4]), lambda: dropout_module.dropout(x[0], 0.5, 1)):

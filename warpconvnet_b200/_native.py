@@ -162,7 +162,7 @@ class _LaunchCounts(Counter):
 
     def _with_nodes(self):
         if _nodes:
-            for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm"), _nodes.launches()):
+            for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm", "wcn_linear_8bit"), _nodes.launches()):
                 if kernels:
                     self[name] = self.get(name, 0) + kernels
         return self
@@ -266,7 +266,7 @@ def _fastcall_bind():
 
 
 _NODES_CALL = ("wcn_status_string", "wcn_training_launches", "wcn_linear_workspace_bytes", "wcn_linear_backward", "wcn_rms_norm_workspace_bytes",
-               "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm")
+               "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm", "wcn_linear_8bit")
 
 
 def graph_nodes():

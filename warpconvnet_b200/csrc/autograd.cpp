@@ -6,7 +6,7 @@
 // goes to the operator's function in Python, which gives the same.
 //
 // The calls themselves are made here too where nothing has to be copied, cast or refused (us of the host for one row: RMS norm 9, here 5;
-// linear 12, here 6; the three above both ways then take 73, 52 and 78).  Arguments that the functions here do not take get no result, and
+// linear 12, here 6, of 8-bit operands 15 and 6; the three above both ways then take 73, 52 and 78).  Arguments that the functions here do not take get no result, and
 // Python goes on with them.
 //
 // A way of calling and no more: where this extension is not built, autograd functions in Python make the same calls.
@@ -42,6 +42,7 @@ struct Functions {   // of the loaded library
   decltype(&wcn_linear_workspace_bytes) linear_bytes = nullptr;
   decltype(&wcn_linear_backward) linear = nullptr;
   decltype(&wcn_linear) linear_forward = nullptr;
+  decltype(&wcn_linear_8bit) linear_8bit = nullptr;
   decltype(&wcn_rms_norm) norm_forward = nullptr;
   decltype(&wcn_rms_norm_workspace_bytes) norm_bytes = nullptr;
   decltype(&wcn_rms_norm_backward) norm = nullptr;
@@ -50,7 +51,7 @@ struct Functions {   // of the loaded library
 // The operators' functions in Python, kept for good: a node may outlive the interpreter's lock.
 py::object *linear_in_python, *norm_in_python, *dropout_in_python;
 struct Launched {   // kernels since they were last asked for
-  std::atomic<int64_t> linear{0}, norm{0}, dropout{0}, linear_forward{0}, norm_forward{0};
+  std::atomic<int64_t> linear{0}, norm{0}, dropout{0}, linear_forward{0}, norm_forward{0}, linear_8bit{0};
 } launched;
 
 void check(int status, const char* what) {
@@ -285,14 +286,17 @@ std::optional<Tensor> run_linear(const Tensor& x, const Tensor& weight, const st
   return y;
 }
 
-py::object run_norm(const Tensor& x, const std::optional<Tensor>& weight, double eps, const std::optional<Tensor>& residual, double least_eps,
+// eight: codes and scales in the norm's place, and no graph.
+py::object run_norm(const Tensor& x, const std::optional<Tensor>& weight, double eps, const std::optional<Tensor>& residual, bool eight, double least_eps,
                     int64_t most_rows, int64_t most_channels) {
   int code = 0;
   if (!rows_taken(x, most_rows, most_channels, code) || !(eps >= least_eps) || std::isinf(eps)) return py::none();
   const int64_t n = x.size(0), c = x.size(1);
   if (!same_rows(residual, x, n, c) || (weight && (weight->dim() != 1 || weight->size(0) != c || !plain(*weight, x.device(), at::kFloat)))) return py::none();
   const bool graph = c10::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(residual));
-  Tensor y = rows_like(x, n, c), rstd;
+  if (eight && graph) return py::none();   // (refused there)
+  Tensor y = eight ? at::empty({n, c}, x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false)) : rows_like(x, n, c), rstd, scale;
+  if (eight) scale = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
   std::optional<Tensor> h;
   if (residual) h = rows_like(x, n, c);
   if (graph) rstd = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
@@ -300,12 +304,40 @@ py::object run_norm(const Tensor& x, const std::optional<Tensor>& weight, double
   int32_t bits;
   std::memcpy(&bits, &number, 4);
   check(native.norm_forward(x.data_ptr(), c, residual ? residual->data_ptr() : nullptr, c, n, c, code,
-                            weight ? static_cast<const float*>(weight->data_ptr()) : nullptr, bits, h ? h->data_ptr() : nullptr, y.data_ptr(),
-                            static_cast<float*>(at_of(rstd)), nullptr, nullptr, stream_of(x)),
+                            weight ? static_cast<const float*>(weight->data_ptr()) : nullptr, bits, h ? h->data_ptr() : nullptr, eight ? nullptr : y.data_ptr(),
+                            static_cast<float*>(at_of(rstd)), eight ? y.data_ptr() : nullptr, static_cast<float*>(at_of(scale)), stream_of(x)),
         "wcn_rms_norm");
   launched.norm_forward += 1;
+  if (eight) return h ? py::make_tuple(y, scale, *h) : py::make_tuple(y, scale);
   if (graph) norm(y, h, x, residual, weight, rstd, eps, code);
   return h ? py::object(py::make_tuple(y, *h)) : py::cast(y);
+}
+
+std::optional<Tensor> run_linear_8bit(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias,
+                                      int64_t act, const std::optional<Tensor>& residual, int64_t code, int64_t most_rows, int64_t most_inputs,
+                                      int64_t most_outputs) {
+  if (!x.is_cuda() || x.dim() != 2 || weight.dim() != 2 || x.device().index() >= MOST_DEVICES || x.device().index() != c10::cuda::current_device())
+    return std::nullopt;
+  const int64_t n = x.size(0), k = x.size(1), m = weight.size(0);
+  const at::Device device = x.device();
+  const at::ScalarType type = code == WCN_F16 ? at::kHalf : at::kBFloat16;
+  void* const status = status_words[device.index()];
+  if (!status || n < 1 || n > most_rows || k < 1 || k > most_inputs || m < 1 || m > most_outputs || weight.size(1) != k ||
+      !plain(x, device, at::kFloat8_e4m3fn) || !plain(weight, device, at::kFloat8_e4m3fn) || !on_lines(x, 16) || !on_lines(weight, 16))
+    return std::nullopt;
+  if (x_scale.dim() != 1 || x_scale.size(0) != n || !plain(x_scale, device, at::kFloat) || weight_scale.dim() != 1 || weight_scale.size(0) != m ||
+      !plain(weight_scale, device, at::kFloat) || (bias && (bias->dim() != 1 || bias->size(0) != m || !plain(*bias, device, type))) ||
+      (residual && (residual->dim() != 2 || residual->size(0) != n || residual->size(1) != m || !plain(*residual, device, type))))
+    return std::nullopt;
+  if (c10::GradMode::is_enabled() && (wants(x) || wants(x_scale) || wants(weight) || wants(weight_scale) || wants(bias) || wants(residual)))
+    return std::nullopt;   // (refused there)
+  Tensor y = at::empty({n, m}, x.options().dtype(type).requires_grad(false));
+  check(native.linear_8bit(x.data_ptr(), k, static_cast<const float*>(x_scale.data_ptr()), n, k, weight.data_ptr(), k,
+                           static_cast<const float*>(weight_scale.data_ptr()), m, code, bias ? bias->data_ptr() : nullptr, act,
+                           residual ? residual->data_ptr() : nullptr, residual ? m : 0, y.data_ptr(), static_cast<int32_t*>(status), stream_of(x)),
+        "wcn_linear_8bit");
+  launched.linear_8bit += native.launches();
+  return y;
 }
 
 std::optional<Tensor> run_dropout(const Tensor& x, const std::optional<Tensor>& residual, int64_t least, int64_t number, int64_t most_rows,
@@ -334,6 +366,7 @@ PYBIND11_MODULE(_autograd, m) {
     take(native.linear_bytes, a, "wcn_linear_workspace_bytes");
     take(native.linear, a, "wcn_linear_backward");
     take(native.linear_forward, a, "wcn_linear");
+    take(native.linear_8bit, a, "wcn_linear_8bit");
     take(native.norm_forward, a, "wcn_rms_norm");
     take(native.norm_bytes, a, "wcn_rms_norm_workspace_bytes");
     take(native.norm, a, "wcn_rms_norm_backward");
@@ -341,7 +374,7 @@ PYBIND11_MODULE(_autograd, m) {
     linear_in_python = new py::object(l), norm_in_python = new py::object(n), dropout_in_python = new py::object(d);
   });
   m.def("launches", [] { return py::make_tuple(launched.linear.exchange(0), launched.norm.exchange(0), launched.dropout.exchange(0),
-                                                    launched.linear_forward.exchange(0), launched.norm_forward.exchange(0)); });
+                                                    launched.linear_forward.exchange(0), launched.norm_forward.exchange(0), launched.linear_8bit.exchange(0)); });
   m.def("linear", &linear);
   m.def("norm", &norm);
   m.def("dropout", &dropout);
@@ -349,6 +382,7 @@ PYBIND11_MODULE(_autograd, m) {
     if (device >= 0 && device < MOST_DEVICES) status_words[device] = reinterpret_cast<void*>(word);
   });
   m.def("run_linear", &run_linear);
+  m.def("run_linear_8bit", &run_linear_8bit);
   m.def("run_norm", &run_norm);
   m.def("run_dropout", &run_dropout);
 }

@@ -187,6 +187,11 @@ def linear_8bit(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor
     fp32, times the scales.  ``residual`` and the result are of ``out_dtype`` (float16 or bfloat16), to which the bias is brought.  No
     gradient."""
     act = check_activation(activation)
+    nodes = graph_nodes()
+    if nodes is not None and (out_dtype is torch.bfloat16 or out_dtype is torch.float16) and isinstance(x, Tensor) and reverse_mode_only():
+        y = nodes.run_linear_8bit(x, x_scale, weight, weight_scale, bias, act, residual, dtype_code(out_dtype), _MOST, _MOST_INPUTS, _MOST_OUTPUTS)
+        if y is not None:
+            return y
     _check_shapes(x, weight, bias)
     if x.dtype != E4M3 or weight.dtype != E4M3:
         raise TypeError(f"x and weight must be {E4M3}, got {x.dtype} and {weight.dtype}")

@@ -134,7 +134,7 @@ def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, resi
     the residual may be column blocks of wider buffers."""
     nodes, transformed = graph_nodes(), not reverse_mode_only()
     if nodes is not None and not transformed and isinstance(x, Tensor):
-        results = nodes.run_norm(x, weight, eps, residual, _LEAST_EPS, _MOST, _MOST_CHANNELS)
+        results = nodes.run_norm(x, weight, eps, residual, False, _LEAST_EPS, _MOST, _MOST_CHANNELS)
         if results is not None:
             return results
     code = _check(x, weight, eps, residual)
@@ -161,6 +161,11 @@ def rms_norm_8bit(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6,
 
     ``q [N, C]`` are e4m3 numbers and ``scale [N]`` fp32, the largest magnitude of a row's norm / 448 (2^-126 at least), so that
     ``q * scale`` is the norm.  A row with a number that is not finite is NaN, scale and all.  No gradient."""
+    nodes = graph_nodes()
+    if nodes is not None and isinstance(x, Tensor) and reverse_mode_only():
+        results = nodes.run_norm(x, weight, eps, residual, True, _LEAST_EPS, _MOST, _MOST_CHANNELS)
+        if results is not None:
+            return results
     code = _check(x, weight, eps, residual)
     no_gradient("rms_norm_8bit", x, weight, residual)
     (q, scale), h, _ = _forward(x, _vector(weight), eps, residual, code, True, False)
