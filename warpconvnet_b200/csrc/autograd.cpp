@@ -6,8 +6,8 @@
 // goes to the operator's function in Python, which gives the same.
 //
 // The calls themselves are made here too where nothing has to be copied, cast or refused (us of the host for one row: RMS norm 9, here 5;
-// linear 12, here 6, of 8-bit operands 15 and 6; the three above both ways then take 73, 52 and 78).  Arguments that the functions here do not take get no result, and
-// Python goes on with them.
+// linear 12, here 6, of 8-bit operands 15 and 6; the three above both ways then take 73, 52 and
+// 78).  Arguments that the functions here do not take get no result, and Python goes on with them.
 //
 // A way of calling and no more: where this extension is not built, autograd functions in Python make the same calls.
 #include <ATen/ATen.h>
