@@ -4,8 +4,9 @@
 // z is computed again in the backward pass, not kept: for rows as wide as these a product costs less than writing z and reading it (at
 // 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  Gradients of narrow layers in 16 bits are one
 // kernel's (linear_backward_tcgen05.cu).  Elsewhere dz, rounded to the inputs' type, goes to the workspace, in pieces of at most 512 MB
-// (pieces that stay in L2 lost more by their launches than they gained: 240 000 x 96 -> 384 in pieces of 64 MB 241 us, whole 196); each is multiplied by W (dx) and by x (dW), whose sums over the rows are divided
-// among the multiprocessors and joined in a fixed order and in double: the same bits on every run.
+// (pieces that stay in L2 lost more by their launches than they gained: 240 000 x 96 -> 384 in pieces of 64 MB 241 us, whole 196); each
+// is multiplied by W (dx) and by x (dW), whose sums over the rows are divided among the multiprocessors and joined in a fixed order and
+// in double: the same bits on every run.
 //
 // 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 there too
 // as sums of three bf16 numbers (linear_split_tcgen05.cu).  On the FMA pipes in tiles of 64 x 64 fp32 took as long for the smallest problems
