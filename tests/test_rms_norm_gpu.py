@@ -133,6 +133,46 @@ def test_rows_that_are_not_numbers(dtype):
     assert (scale == 2.0 ** -126).all() and ((q.float() * scale[:, None] - tiny).abs() <= 2.0 ** -136).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [13, 17, 96, 1031, 8192])
+def test_rows_at_the_end_of_the_range(dtype, c):
+    """Numbers as large as the type has, a mask's lowest value among them: their norm, its codes and its gradient are those of other rows."""
+    g = torch.Generator().manual_seed(c)
+    most = torch.finfo(dtype).max
+    rows = torch.stack([torch.full((c,), most), torch.full((c,), -most), most * (torch.rand(c, generator=g) - 0.5) * 2, torch.randn(c, generator=g) * 1e36])
+    x, dy = rows.to(dtype).to(DEV), (torch.randn(4, c, generator=g) * 1e30).to(dtype).to(DEV)
+    w = (torch.rand(c, generator=g) + 0.5).to(DEV)
+    ref, s = norm64(x, w, 1e-6)
+    own = 16 * U + 2.0 ** -149 / s   # (and 1 / root mean square may be a number without all its places)
+    leaf, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = rms_norm(leaf, lw)
+    assert ((y.detach().double() - ref).abs() <= (half(dtype) + own) * ref.abs()).all()
+    if dtype == torch.bfloat16:   # (their errors, 2^-19 at most, lie far below half a step beside 1)
+        assert (rms_norm(x[:1]) == 1).all() and (rms_norm(x[1:2]) == -1).all()
+    assert torch.equal(rms_norm(x, residual=torch.zeros_like(x))[0], rms_norm(x))
+    q, scale = rms_norm_8bit(x, w)
+    t = ref.abs().amax(1, keepdim=True) / 448
+    assert ((scale[:, None].double() - t).abs() <= (own + 4 * U) * t).all()
+    # a code is off by half a step, 2^-4 of the number or 2^-10 of the scale at least
+    assert ((q.double() * scale[:, None].double() - ref).abs() <= (2.0 ** -4 + 2 * own + 4 * U) * ref.abs() + 2.0 ** -10 * t).all()
+    dx, dw = torch.autograd.grad(y, [leaf, lw], dy)
+    xh, u = x.double() * s, dy.double() * w.double()
+    want = s * (u - xh * (u * xh).mean(1, keepdim=True))
+    terms = s * (u.abs() + xh.abs() * (u * xh).abs().mean(1, keepdim=True))
+    assert ((dx.double() - want).abs() <= half(dtype) * want.abs() + (32 * U + 4 * own) * terms).all()
+    each = dy.double() * xh
+    assert ((dw.double() - each.sum(0)).abs() <= ((own + 16 * U) * each.abs()).sum(0)).all()
+
+
+def test_an_eps_that_counts_beside_large_rows():
+    x = torch.randn(9, 96, device=DEV) * 1e20
+    ref = norm64(x, None, 1e38)[0]   # the mean of squares is some 1e40
+    assert ((rms_norm(x, eps=1e38).double() - ref).abs() <= 16 * U * ref.abs()).all()
+    x = torch.full((9, 1), 1.5e19, device=DEV)   # 2.25e38: with eps beyond the end of fp32
+    ref = norm64(x, None, 3e38)[0]
+    assert ((rms_norm(x, eps=3e38).double() - ref).abs() <= (16 * U) * ref.abs()).all()
+
+
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(3)
     x, r, w, dy, dh, u, v = (torch.randn(s, generator=g) for s in ((31, 24), (31, 24), (24,), (31, 24), (31, 24), (31, 24), (24,)))

@@ -7,7 +7,8 @@
 // Bound by HBM: every row is read once and stays in registers.  L threads share a row (2 to 32 of a warp, or a block of up to
 // 1024), V pieces of up to 16 bytes each: the row's sums are a few shuffles.  The norm is that of h as it is written (rounded to the
 // rows' type), so that the gradient, which reads it again, is that of the same numbers.  Sums, 1 / sqrt and products are fp32.
-// A row whose squares pass the end of fp32 is summed again with its numbers times 2^-66.
+// A row whose squares pass the end of fp32 is summed again with its numbers times 2^-80: 8192 of the largest, 2^128 each, then have
+// squares of 2^109 in all, and those that the first sum could not hold, 2^128, are 2^-32.
 // The gradient of w is summed per thread over the rows of a persistent block (tens of them in fp32), then over the block's threads, and
 // over the blocks in double by a second launch: no atomics, the same bits on every run.
 // 240 000 x 96 bf16 with residual 28 us forward (184 MB at 6.6 TB/s, some of what is written still in L2), 46 + 7 backward (161 MB, 4.0
@@ -23,7 +24,7 @@ namespace {
 constexpr int THREADS = 256, MAX_C = 8192, MAX_WARP_C = 512;   // (channels of a warp's row in the gradient)
 constexpr float LEAST_EPS = 1e-30f;            // beside which squares below the end of fp32 are nothing
 constexpr float MOST = 448.f;                  // the largest e4m3 number
-constexpr float SMALL = 1.3552527156068805e-20f;   // 2^-66
+constexpr float SMALL = 8.271806125530277e-25f;   // 2^-80
 
 struct NormParams {
   const void* x;
@@ -187,12 +188,12 @@ __global__ void __launch_bounds__(BLOCK ? most_lanes(E) : THREADS) rms_norm_kern
         }
       return row_sum<BLOCK>((t[0].x + t[0].y) + (t[1].x + t[1].y), lanes, reinterpret_cast<float*>(part));
     };
-    const float sum = squares(1.f);
-    s = 1.f / sqrtf(sum / (float)p.c + p.eps);
-    const bool over = sum == INFINITY;
+    const float mean = squares(1.f) / (float)p.c + p.eps;
+    s = 1.f / sqrtf(mean);
+    const bool over = mean == INFINITY;
     if (BLOCK ? over : __any_sync(0xFFFFFFFFu, over)) {   // (one answer for all threads that sum together)
       const float again = squares(SMALL);
-      if (over) s = SMALL / sqrtf(again / (float)p.c);
+      if (over) s = SMALL / sqrtf(again / (float)p.c + p.eps * SMALL * SMALL);
     }
     if (p.rstd && live && lane == 0) p.rstd[row] = s;
   }
