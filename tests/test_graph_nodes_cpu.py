@@ -69,6 +69,41 @@ def test_norm_and_dropout():
     assert torch.equal(dx, dropout_module.formula(torch.ones(5, 4), 20000, 5, None)) and (dr == 1).all()
 
 
+def norm(x, g, r):
+    with torch.no_grad():
+        results = norm_module.formula(x, g, 1e-6, r)
+    y, h = (results, None) if r is None else results
+    nodes.norm(y, h, x, r, g, torch.ones(x.shape[0]), 1e-6, 0)
+    return results
+
+
+@built
+@pytest.mark.parametrize("inputs", [lambda a, m: (a, a), lambda a, m: (a * 1.5, a), lambda a, m: (a @ m, a), lambda a, m: (a, a @ m)])
+def test_a_graph_of_the_norm_s_gradient_where_inputs_depend_on_each_other(inputs):
+    a, m, g = leaves((5, 4), (4, 4), (4,))
+
+    def gradients(f):
+        x, r = inputs(a, m)
+        y, h = f(x, g, r)
+        first = torch.autograd.grad(y.square().sum() + h.pow(3).sum(), [a, g], create_graph=True)
+        return first + torch.autograd.grad(first[0].square().sum() + first[1].square().sum(), [a, g], create_graph=True)
+    want = gradients(lambda x, g, r: norm_module.formula(x, g, 1e-6, r))
+    for got, e in zip(gradients(norm), want):   # the same sums in fp32, in another order
+        torch.testing.assert_close(got, e, rtol=2 ** -18, atol=2 ** -18 * float(e.abs().max()))
+
+
+@built
+def test_a_graph_of_a_norm_s_gradient_behind_the_same_weight():
+    a, g = leaves((5, 4), (4,))
+
+    def gradients(f):
+        first = torch.autograd.grad(f(f(a, g, None) + a.square(), g, None).pow(3).sum(), [a, g], create_graph=True)
+        return first + torch.autograd.grad(first[0].square().sum() + first[1].square().sum(), [a, g], create_graph=True)
+    want = gradients(lambda x, g, r: norm_module.formula(x, g, 1e-6, r))
+    for got, e in zip(gradients(norm), want):
+        torch.testing.assert_close(got, e, rtol=2 ** -18, atol=2 ** -18 * float(e.abs().max()))
+
+
 @built
 def test_errors_are_the_engine_s(monkeypatch):
     x, w, b, r = leaves((5, 4), (3, 4), (3,), (5, 3))

@@ -40,6 +40,12 @@ def reverse_mode_only() -> bool:
     return forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
 
 
+def apart(*tensors: Optional[Tensor]):
+    """Views of an operator's inputs, for a formula of them that is differentiated within its backward pass: one of them may have been
+    made from another, or be it, and the derivative by an input has to end there (the pass under way goes on behind the input itself)."""
+    return [t if t is None else t.view_as(t) for t in tensors]
+
+
 def bare(*modules: nn.Module) -> bool:
     """Whether calling these modules runs their class's ``forward`` and nothing else: no hooks, on them or on all modules,
     and no ``forward`` of the instance's own."""

@@ -9,7 +9,7 @@ import torch
 from torch import Tensor
 
 from ..._native import check, count_training_launches, dtype_code, graph_nodes, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
-from .batch_norm import _bits, reverse_mode_only
+from .batch_norm import _bits, apart, reverse_mode_only
 from .group_norm import _rows, _vector
 
 _MOST, _MOST_CHANNELS = 0x7FFFFEFF, 8192
@@ -82,6 +82,7 @@ def gradients(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], h
     """Those of x, residual and weight."""
     need_x, need_r, need_w = needs
     if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+        x, residual, weight = apart(x, residual, weight)
         results = formula(x, weight, eps, residual)
         pairs = [(t, g) for t, g in zip(results if residual is not None else (results,), (dy, dh)) if g is not None]
         wanted = [t for t, need in zip((x, residual, weight), (need_x, need_r, need_w)) if need]
