@@ -69,6 +69,25 @@ def test_norm_and_dropout():
     assert torch.equal(dx, dropout_module.formula(torch.ones(5, 4), 20000, 5, None)) and (dr == 1).all()
 
 
+@built
+@pytest.mark.parametrize("f", [lambda layer, a, w: layer(layer(a, w, None, a), w, None, a), lambda layer, a, w: layer(a, a, None, None),
+                               lambda layer, a, w: layer(a, w, w.sum(1), a), lambda layer, a, w: layer(a @ w, w, None, None)],
+                         ids=["one weight twice", "one tensor twice", "a bias of the weight", "rows of the weight"])
+def test_a_graph_of_a_linear_layer_s_gradient_where_inputs_depend_on_each_other(f):
+    a, w = leaves((5, 4), (4, 4))
+
+    def gradients(layer):
+        y = f(layer, a, w)
+        first = torch.autograd.grad(y.square().sum(), [a, w], create_graph=True, allow_unused=True)
+        return first + torch.autograd.grad(sum(t.square().sum() for t in first if t is not None), [a, w], create_graph=True, allow_unused=True)
+    want = gradients(lambda x, w, b, r: linear_module.formula(x, w, b, "silu", r, 0, 0))
+    for got, e in zip(gradients(linear), want):
+        if e is None:
+            assert got is None
+        else:
+            torch.testing.assert_close(got, e, rtol=2 ** -18, atol=2 ** -18 * float(e.abs().max()))
+
+
 def norm(x, g, r):
     with torch.no_grad():
         results = norm_module.formula(x, g, 1e-6, r)

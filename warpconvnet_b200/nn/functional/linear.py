@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 
 from ..._native import WCN_F32, check, count_training_launches, device_status, dtype_code, graph_nodes, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
-from .batch_norm import reverse_mode_only
+from .batch_norm import apart, reverse_mode_only
 from .dropout import check_probability, check_seed, kept_factor, new_seed
 from .group_norm import _ACTIVATIONS, _rows, check_activation
 from .linear_cross_entropy import _matrix
@@ -79,6 +79,7 @@ def gradients(x: Tensor, weight: Tensor, bias: Optional[Tensor], seed, x_rows: O
     need_x, need_w, need_b, need_r = needs
     d_residual = dy if need_r else None
     if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+        x, weight, bias = apart(x, weight, bias)
         y = formula(x, weight, bias, _NAMES[act], None, least, seed)
         wanted = [t for t, need in zip((x, weight, bias), (need_x, need_w, need_b)) if need]
         got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True) if wanted else ())
