@@ -692,7 +692,7 @@ int wcn_dropout(const void* x, int64_t x_ld, const void* residual, int64_t resid
  * wcn_linear_8bit: x and w e4m3 with a scale a row (wcn_quantize_rows), the others of out_dtype (16 bits), no dropout.
  * backward: gradients of x (contiguous), of w [m, k] and of the bias, each of dtype and each of which may be NULL; the residual's is dy.
  * workspace: 32-byte aligned; `what` of the query: 0 forward (0 bytes in 16 bits: may be NULL), else the sum of 1 (dx),
- * 2 (dw), 4 (dbias); aligned: the rows of dy lie as those of x do.
+ * 2 (dw), 4 (dbias); aligned: the rows of dy lie as those of x have to (fp32: whatever is said, they do).
  * At most 32768 inputs, 2^20 outputs, 2^31 - 2^17 rows.  The reference has nn.Linear and its neighbours
  * (warpconvnet/nn/modules/mlp.py). */
 int wcn_linear(const void* x, int64_t x_ld, int64_t n, int32_t k, const void* w, int64_t w_ld, int32_t m, int dtype, const void* bias,

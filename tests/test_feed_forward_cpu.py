@@ -88,3 +88,12 @@ def test_linears_gradient_and_codes_refuse():
     # the gradient behind the activation in pieces of 512 MB: whatever the rows are, the workspace stays bounded
     for dtype in (_native.WCN_F32, _native.WCN_BF16):
         assert _native.query_bytes("wcn_linear_workspace_bytes", 2 ** 31 - 2 ** 17, 64, 1000, dtype, 1, 1, 0, 0) <= (512 << 20) + (1 << 20)
+
+
+@pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64), (2_200_000, 96, 20), (100, 8, 8)])
+def test_a_workspace_for_a_gradient_in_fp32_does_not_go_by_where_it_lies(n, k, m):
+    """The gradient is taken wherever its numbers are: what was asked for one between boundaries has to do for what the call makes of it."""
+    for what in range(1, 8):
+        for act, least in ((0, 0), (0, 100), (3, 0)):
+            sizes = {_native.query_bytes("wcn_linear_workspace_bytes", n, k, m, _native.WCN_F32, what, act, least, aligned) for aligned in (0, 1)}
+            assert len(sizes) == 1

@@ -199,6 +199,21 @@ def test_gradients_in_pieces(dtype):
     assert torch.equal(part, whole[-300:])
 
 
+@pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64)])
+def test_a_gradient_in_fp32_between_boundaries(n, k, m):
+    """What the backward pass of a concatenation gives: contiguous rows that start on any element.  Parts of half a gigabyte."""
+    x, w, b, _, _ = make(n, k, m, torch.float32)
+    wide = torch.randn(n * m + 1, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dy = wide[1:].view(n, m)
+    got = torch.autograd.grad(linear(*leaves), leaves, dy)
+    want = torch.autograd.grad(linear(*leaves), leaves, dy.clone())
+    assert dy.is_contiguous() and all(torch.equal(a, e) for a, e in zip(got, want))
+    x, w = x.detach().double(), w.detach().double()
+    for a, e in zip(got, (dy.double() @ w, dy.double().t() @ x, dy.double().sum(0))):
+        assert off(a, e) <= 2e-6
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strides_and_boundaries(dtype):
     """Column blocks of wider buffers, starts on odd elements, every other row, transposed, repeated: as their copies."""

@@ -112,7 +112,7 @@ struct LinearNode : Node {
     if (need[0]) out[0] = at::empty({n, k}, xt.options().requires_grad(false));
     if (need[1]) out[1] = at::empty({m, k}, wt.options().requires_grad(false));
     if (need[2]) out[2] = at::empty({m}, wt.options().requires_grad(false));
-    const bool aligned = m % whole == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
+    const bool aligned = m % whole == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % (2 * whole) == 0;   // (fp32: always)
     int64_t size = 0;
     check(native.linear_bytes(n, k, m, code, need[0] + 2 * need[1] + 4 * need[2], act, least, aligned, &size), "wcn_linear_workspace_bytes");
     Tensor ws;

@@ -117,9 +117,10 @@ struct Pieces {
   int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
 enum Want { DX = 1, DW = 2, DB = 4 };     // none of them: forward
-// aligned: dy is read as x is.
+// aligned: dy is read as x is (fp32 numbers always are).
 Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, bool aligned) {
   Pieces p = {};
+  aligned = aligned || dtype == WCN_F32;
   const int64_t e = wcn_dtype_size(dtype);
   const bool direct = aligned && act == WCN_ACT_NONE && !drops;
   auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
@@ -232,7 +233,9 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   const int size = wcn_dtype_size(dtype), what = (dx ? DX : 0) | (dw ? DW : 0) | (db ? DB : 0);
   // (rows of a gradient between boundaries are brought to them as others are made)
   const bool aligned = rows_taken(dy, dy_ld, n, m, size), direct = act == WCN_ACT_NONE && least == 0 && aligned;
-  if (!what || !dev_status || !rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !dy || (n > 1 && dy_ld < m)) return WCN_ERR_INVALID_PARAMETERS;
+  if (!what || !dev_status || !rows_taken(x, x_ld, n, k, size) || !rows_taken(w, w_ld, m, k, size) || !dy || reinterpret_cast<uintptr_t>(dy) % size ||
+      (n > 1 && dy_ld < m))
+    return WCN_ERR_INVALID_PARAMETERS;
   const Pieces p = plan(n, k, m, dtype, what, act, least != 0, aligned);
   if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.bytes)) return WCN_ERR_INVALID_PARAMETERS;
   char* const ws = reinterpret_cast<char*>(workspace);
