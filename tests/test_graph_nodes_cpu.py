@@ -25,6 +25,21 @@ def test_without_the_extension_functions_in_python_stand_in(monkeypatch, tmp_pat
     assert _native._load_nodes() is None
 
 
+@built
+def test_the_extension_has_no_cpp_library_of_its_own():
+    """(Two in a process, and the text of the first error ended it.)"""
+    with open(_native.AUTOGRAD_PATH, "rb") as f:
+        assert b"\0libstdc++.so" in f.read()
+
+
+@built
+def test_what_the_library_refuses_is_an_error_with_its_number():
+    x, w = leaves((5, 4), (3, 4))
+    y = nodes.linear(torch.empty(5, 3), x, w, None, None, None, None, None, 9, 0, 0, 0, 0)   # no such activation
+    with pytest.raises(RuntimeError, match=r"invalid parameters \(-5\)"):
+        torch.autograd.grad(y, [x], torch.ones(5, 3))
+
+
 def leaves(*shapes):
     torch.manual_seed(0)
     return [torch.randn(s, requires_grad=True) for s in shapes]

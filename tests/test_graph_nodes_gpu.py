@@ -147,6 +147,16 @@ def test_kept_graphs_checkpoints_streams_and_threads():
         same(got, want)
 
 
+def test_what_the_library_refuses_is_an_error_of_the_engine_s_thread():
+    """A call without a status word is refused on the host; nothing runs."""
+    nodes = _native.graph_nodes()
+    for n, k, m in ((5, 4, 3), (1000, 64, 13)):
+        x, w, b = (torch.randn(s, device=DEV, requires_grad=True) for s in ((n, k), (m, k), (m,)))
+        y = nodes.linear(torch.empty(n, m, device=DEV), x, w, b, None, None, None, None, 0, 0, 0, 0, 0)
+        with pytest.raises(RuntimeError, match=r"wcn_linear_backward failed: invalid parameters \(-5\)"):
+            torch.autograd.grad(y, [x, w, b], torch.randn(n, m, device=DEV))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_tensor_in_two_places(monkeypatch, dtype):
     x, w, dy = leaf(100, 64, dtype=dtype), leaf(64, 64, dtype=dtype), torch.randn(100, 64, device=DEV).to(dtype)

@@ -22,9 +22,12 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <dlfcn.h>
+
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <locale>
 
 #include "../../include/wcn_b200.h"
 
@@ -353,6 +356,14 @@ std::optional<Tensor> run_dropout(const Tensor& x, const std::optional<Tensor>& 
   return y;
 }
 
+// Whether this file has a C++ library of its own in it.  Two of them in a process share some of their objects and not others: a number in
+// the text of an error then ends the process.
+bool own_library() {
+  Dl_info here, there;
+  const std::locale& (*const classic)() = &std::locale::classic;
+  return dladdr(reinterpret_cast<const void*>(&own_library), &here) && dladdr(reinterpret_cast<const void*>(classic), &there) && here.dli_fbase == there.dli_fbase;
+}
+
 template <typename F> void take(F& function, const py::dict& addresses, const char* name) {
   function = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
 }
@@ -360,6 +371,7 @@ template <typename F> void take(F& function, const py::dict& addresses, const ch
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
+  if (own_library()) throw py::import_error("_autograd.so is linked with a C++ library of its own");
   m.def("bind", [](const py::dict& a, py::object l, py::object n, py::object d) {
     take(native.status_string, a, "wcn_status_string");
     take(native.launches, a, "wcn_training_launches");

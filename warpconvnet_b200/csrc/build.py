@@ -60,7 +60,8 @@ def build_autograd(force=False):
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                *("-I" + i for i in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
                                     sysconfig.get_paths()["include"])),
-               AUTOGRAD_SOURCE, "-o", AUTOGRAD, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+               AUTOGRAD_SOURCE, "-o", AUTOGRAD, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+               "-l:libstdc++.so.6"]  # (torch's own: some compilers would link theirs statically, and a process with two of them ends at the first error's text)
         subprocess.check_call(cmd)
     except (ImportError, OSError, subprocess.CalledProcessError) as e:  # no compiler, no headers
         if os.path.isfile(AUTOGRAD):
