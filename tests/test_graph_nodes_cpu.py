@@ -1,6 +1,8 @@
 """Nodes of autograd's graph in the extension (csrc/autograd.cpp): what they pass on to Python, and what stands in for them."""
 import gc
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -23,6 +25,18 @@ def test_without_the_extension_functions_in_python_stand_in(monkeypatch, tmp_pat
     assert _native._load_nodes() is None
     (tmp_path / "_autograd.so").write_bytes(b"no library")
     assert _native._load_nodes() is None
+
+
+@built
+def test_another_torch_does_not_load_it():
+    """Its nodes are laid out as one version of torch has them; a build for another one is made anew."""
+    from warpconvnet_b200.csrc import build
+    assert build._autograd_is_built(torch.__version__) and not build._autograd_is_built("1.2.3")
+    code = "import torch\nfrom warpconvnet_b200 import _native\ntorch.__version__ = {!r}\nprint(_native.graph_nodes() is None)"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(_native.__file__)))
+    for version, refused in ((torch.__version__, "False"), ("1.2.3", "True")):
+        out = subprocess.run([sys.executable, "-c", code.format(str(version))], cwd=root, capture_output=True, text=True, timeout=300)
+        assert out.stdout.strip() == refused, out.stderr
 
 
 @built

@@ -271,7 +271,7 @@ _NODES_CALL = ("wcn_status_string", "wcn_training_launches", "wcn_linear_workspa
 
 def graph_nodes():
     """The ``_autograd`` extension (csrc/autograd.cpp), whose nodes of autograd's graph call the library's gradients themselves, or None
-    where it was not built or does not load: autograd functions in Python make the same calls."""
+    where it was not built or does not load (it refuses any torch but the one that it was compiled with): autograd functions in Python make the same calls."""
     global _nodes
     if _nodes is False:
         _nodes = _load_nodes()

@@ -31,6 +31,11 @@
 
 #include "../../include/wcn_b200.h"
 
+#ifndef WCN_BUILT_WITH   // torch.__version__
+#error "compile with csrc/build.py"
+#endif
+#define WCN_BUILT_WITH_MARK "built with torch " WCN_BUILT_WITH   // (which build.py looks for in the file)
+
 namespace py = pybind11;
 using at::Tensor;
 using torch::autograd::Node;
@@ -371,6 +376,9 @@ template <typename F> void take(F& function, const py::dict& addresses, const ch
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
+  // Nodes and saved variables are laid out as the torch has them that this file was compiled with: no other one may run it.
+  const std::string version = py::str(py::module_::import("torch").attr("__version__"));
+  if (version != WCN_BUILT_WITH) throw py::import_error("_autograd.so was " WCN_BUILT_WITH_MARK ", not " + version);
   if (own_library()) throw py::import_error("_autograd.so is linked with a C++ library of its own");
   m.def("bind", [](const py::dict& a, py::object l, py::object n, py::object d) {
     take(native.status_string, a, "wcn_status_string");

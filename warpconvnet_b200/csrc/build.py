@@ -49,15 +49,24 @@ def build_fastcall(force=False):
             print(f"_fastcall.so was not built ({e}): calls go through ctypes")
 
 
-def build_autograd(force=False):
+def _autograd_is_built(version):
+    """Whether the extension is there, of this source and of this torch."""
     header = os.path.join(HERE, "..", "..", "include", "wcn_b200.h")
-    if not force and os.path.isfile(AUTOGRAD) and os.path.getmtime(AUTOGRAD) > max(os.path.getmtime(AUTOGRAD_SOURCE), os.path.getmtime(header)):
-        return
+    if not os.path.isfile(AUTOGRAD) or os.path.getmtime(AUTOGRAD) <= max(os.path.getmtime(AUTOGRAD_SOURCE), os.path.getmtime(header)):
+        return False
+    with open(AUTOGRAD, "rb") as f:
+        return f"built with torch {version}, not ".encode() in f.read()
+
+
+def build_autograd(force=False):
     try:
         import torch
+        if not force and _autograd_is_built(torch.__version__):
+            return
         root = os.path.dirname(torch.__file__)
         cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DWCN_BUILT_WITH="{torch.__version__}"',
                *("-I" + i for i in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
                                     sysconfig.get_paths()["include"])),
                AUTOGRAD_SOURCE, "-o", AUTOGRAD, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
