@@ -199,6 +199,25 @@ def test_gradients_in_pieces(dtype):
     assert torch.equal(part, whole[-300:])
 
 
+@pytest.mark.parametrize("n,k,m,act", [(5_000_000, 32, 32, None), (2_500_000, 16, 40, "relu"), (250_000, 256, 1024, None), (250_000, 256, 1024, "relu")])
+def test_long_sums_of_one_sign(n, k, m, act):
+    """Numbers of one sign, which a tensor core's accumulator cuts all one way: beside the result's rounding (half a step, 2^-11, of either sign)
+    the weights' gradients may be a quarter of that off in the mean, however many rows there are."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x = ((1 + torch.rand(n, k, device=DEV, generator=g)) * torch.linspace(1, 2, k, device=DEV)).half()   # (results all over a binade)
+    dy = ((1 + torch.rand(n, m, device=DEV, generator=g)) * torch.linspace(1, 2, m, device=DEV) * 1000 / n).half()
+    w, b = torch.rand(m, k, device=DEV, generator=g).half().requires_grad_(), torch.ones(m, device=DEV, dtype=torch.float16, requires_grad=True)
+    dw, db = torch.autograd.grad(linear(x, w, b, act), [w, b], dy)
+    want_w, want_b = torch.zeros(m, k, dtype=torch.float64, device=DEV), torch.zeros(m, dtype=torch.float64, device=DEV)
+    for at in range(0, n, 1 << 18):
+        part = dy[at:at + (1 << 18)].double()
+        want_w += part.t() @ x[at:at + (1 << 18)].double()
+        want_b += part.sum(0)
+    for got, want in ((dw, want_w), (db, want_b)):
+        short = (got.double() - want) / want
+        assert abs(float(short.mean())) <= 2.0 ** -13 and float(short.abs().max()) <= half(torch.float16) + 2.0 ** -13
+
+
 @pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64)])
 def test_a_gradient_in_fp32_between_boundaries(n, k, m):
     """What the backward pass of a concatenation gives: contiguous rows that start on any element.  Parts of half a gigabyte."""

@@ -5,8 +5,8 @@
 // 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  Gradients of narrow layers in 16 bits are one
 // kernel's (linear_backward_tcgen05.cu).  Elsewhere dz, rounded to the inputs' type, goes to the workspace, in pieces of at most 512 MB
 // (pieces that stay in L2 lost more by their launches than they gained: 240 000 x 96 -> 384 in pieces of 64 MB 241 us, whole 196); each
-// is multiplied by W (dx) and by x (dW), whose sums over the rows are divided among the multiprocessors and joined in a fixed order and
-// in double: the same bits on every run.
+// is multiplied by W (dx) and by x (dW), whose sums over the rows are divided among the multiprocessors, in 16 bits into parts of
+// 8192 rows at most too, and joined in a fixed order and in double: the same bits on every run.
 //
 // 16- and 8-bit operands run on the tensor cores (linear_tcgen05.cu; dW: the transposed product of linear_ce_tcgen05.cu), fp32 there too
 // as sums of three bf16 numbers (linear_split_tcgen05.cu).  On the FMA pipes in tiles of 64 x 64 fp32 took as long for the smallest problems
@@ -33,6 +33,10 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int MOST_ROWS = 0x7FFE0000, MOST_INPUTS = 32768, MOST_OUTPUTS = 1 << 20;   // (row numbers, and some tiles behind the last, are 32-bit)
 constexpr int64_t PIECE_BYTES = 512ll << 20;   // of dz
+// Rows that an accumulator of a tensor core sums, at most (16 bits; dW and dbias).  It cuts what lies below its last place instead of
+// rounding: sums of one sign lose 1.4e-7 of themselves for each 16 rows (dW of 1.2 million x 64 -> 64, 8 100 rows a block, came out
+// 7e-5 short, of 10 million 2.4e-4, of 30 million 9e-4, where half a step of fp16 is 2.4e-4 at least).  With these, 7e-5.
+constexpr int MOST_SUMMED = 8192;
 
 // ------------------------------------------------------------------ sums of the splits
 
@@ -105,14 +109,16 @@ int run(const wcn_linear_product& q, int dtype, bool by_k, const void* a_planes,
   return wcn_linear_split(q, by_k, a_planes, b_planes, dev_status, st);
 }
 int weight_splits(int m, int k, int rows, int dtype, bool bias) {
-  return dtype == WCN_F32 ? wcn_linear_split_splits(m, k, rows) : wcn_ce_product_splits(m, k, rows, false, bias);
+  if (dtype == WCN_F32) return wcn_linear_split_splits(m, k, rows);   // (which adds its accumulators to sums in registers)
+  const int splits = wcn_ce_product_splits(m, k, rows, false, bias), least = (int)(((int64_t)rows + MOST_SUMMED - 1) / MOST_SUMMED);
+  return splits > least ? splits : least;
 }
 
 // The pieces of rows that dz is made in (forward: that x's parts are made in), and the workspace: dz of a piece, parts of x, dz and w, sums
 // of dW and of dbias.
 struct Pieces {
   int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
-  int whole;                              // blocks of the kernel that needs no pieces (16 bits, narrow layers); 0: not taken
+  bool whole;                             // the kernel that makes all of them (16 bits, narrow layers); its splits are its blocks
   bool parts;                             // fp32: the operands are sums of three bf16 numbers
   int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
@@ -124,15 +130,20 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, b
   const int64_t e = wcn_dtype_size(dtype);
   const bool direct = aligned && act == WCN_ACT_NONE && !drops;
   auto round = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
-  if (what && dtype != WCN_F32) p.whole = wcn_linear_backward_blocks(n, k, m, act, what & DB);
+  if (what && dtype != WCN_F32) p.whole = wcn_linear_backward_blocks(n, k, m, act, what & DB) > 0;
   if (p.whole) {
-    p.rows = (int)n;
-    p.count = 1;
-    p.last_splits = p.whole;
     p.dz_ld = round(m, 8);
-    p.slab = aligned ? 0 : round(n * p.dz_ld * e, 128);   // (behind dy as the kernel reads it)
-    p.ones = p.slab + (what & (DW | DB) ? round((int64_t)p.whole * m * wcn_ce_round(k, 16) * 4, 128) : 0);
-    p.bytes = p.ones + (what & DB ? (int64_t)p.whole * m * 4 : 0);
+    int64_t most = (int64_t)wcn_num_sms() * MOST_SUMMED;
+    if (!aligned && PIECE_BYTES / (p.dz_ld * e) < most) most = PIECE_BYTES / (p.dz_ld * e) / 128 * 128;   // (a copy of dy as the kernel reads it)
+    const int64_t count = (n + most - 1) / most, rows = round((n + count - 1) / count, 128);
+    p.rows = (int)(rows < n ? rows : n);
+    p.count = (int)((n + p.rows - 1) / p.rows);
+    p.splits = wcn_linear_backward_blocks(p.rows, k, m, act, what & DB);
+    p.last_splits = wcn_linear_backward_blocks(n - (int64_t)(p.count - 1) * p.rows, k, m, act, what & DB);
+    const int64_t all = (int64_t)p.splits * (p.count - 1) + p.last_splits;
+    p.slab = aligned ? 0 : round(p.rows * p.dz_ld * e, 128);
+    p.ones = p.slab + (what & (DW | DB) ? round(all * m * wcn_ce_round(k, 16) * 4, 128) : 0);
+    p.bytes = p.ones + (what & DB ? all * m * 4 : 0);
     return p;
   }
   p.dz_ld = round(m, 16 / e);
@@ -248,14 +259,6 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
     drop.scale = 1.f;
   }
   const int ld = wcn_ce_round(k, 16);
-  if (p.whole) {
-    int rc = aligned ? WCN_OK : wcn_dropout_rows(dy, dy_ld, nullptr, 0, n, m, dtype, none, 0, ws, p.dz_ld, st);
-    if (rc != WCN_OK) return rc;
-    const wcn_linear_product q = {x, w, x_ld, w_ld, (int)n, m, k, nullptr, nullptr, dx, k, bias, act, true, aligned ? dy : ws, aligned ? dy_ld : p.dz_ld, drop, 0, factor};
-    rc = wcn_linear_backward_run(q, dw || db ? (float*)(ws + p.slab) : nullptr, db ? (float*)(ws + p.ones) : nullptr, dtype == WCN_BF16, dev_status, st);
-    if (rc != WCN_OK || !(dw || db)) return rc;
-    return join({(const float*)(ws + p.slab), (const float*)(ws + p.ones), dw, db, m, k, ld, p.whole, 0, factor, dev_status}, dtype, st);
-  }
   char *const xs = p.parts ? ws + p.x_parts : nullptr, *const dzs = p.parts ? ws + p.dz_parts : nullptr, *const wsp = p.parts ? ws + p.w_parts : nullptr;
   for (int i = 0; i < p.count; ++i) {
     const int64_t r0 = (int64_t)i * p.rows;
@@ -264,6 +267,15 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
     const void* dz = direct ? (const void*)dyp : (const void*)ws;
     const int64_t dz_ld = direct ? dy_ld : p.dz_ld;
     int rc = WCN_OK;
+    float *const slab = dw || db ? (float*)(ws + p.slab) + (int64_t)i * p.splits * m * ld : nullptr, *const ones = db ? (float*)(ws + p.ones) + (int64_t)i * p.splits * m : nullptr;
+    if (p.whole) {
+      if (!aligned) rc = wcn_dropout_rows(dyp, dy_ld, nullptr, 0, rows, m, dtype, none, r0, ws, p.dz_ld, st);
+      const wcn_linear_product q = {xp, w, x_ld, w_ld, rows, m, k, nullptr, nullptr, dx ? (char*)dx + r0 * k * size : nullptr, k, bias, act, true, aligned ? dyp : ws,
+                                    aligned ? dy_ld : p.dz_ld, drop, r0, factor};
+      if (rc == WCN_OK) rc = wcn_linear_backward_run(q, slab, ones, dtype == WCN_BF16, dev_status, st);
+      if (rc != WCN_OK) return rc;
+      continue;
+    }
     if (p.parts) {   // of what is there already
       wcn_linear_matrix of[3];
       int count = 0;
@@ -292,8 +304,8 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
       q.a = dz; q.a_ld = dz_ld; q.b = xp; q.b_ld = x_ld;
       q.m = m; q.n = k; q.k = rows;
       q.splits = i + 1 < p.count ? p.splits : p.last_splits;
-      q.slab = (float*)(ws + p.slab) + (int64_t)i * p.splits * m * ld;
-      q.slab_ones = db ? (float*)(ws + p.ones) + (int64_t)i * p.splits * m : nullptr;
+      q.slab = slab;
+      q.slab_ones = ones;
       rc = p.parts ? wcn_linear_split_weight(q, dzs, xs, dev_status, st) : wcn_ce_product_run(q, true, false, dtype, dev_status, st);
       if (rc != WCN_OK) return rc;
     }
