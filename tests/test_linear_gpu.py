@@ -218,6 +218,35 @@ def test_long_sums_of_one_sign(n, k, m, act):
         assert abs(float(short.mean())) <= 2.0 ** -13 and float(short.abs().max()) <= half(torch.float16) + 2.0 ** -13
 
 
+@pytest.mark.parametrize("m,act,p", [(1 << 18, None, 0.0), (1 << 20, "relu", 0.0), (1 << 18, None, 0.5)])
+def test_long_sums_over_outputs(m, act, p):
+    """The gradient of x is a sum over the outputs: half of half a step in the mean, as sums over the most inputs that there may be."""
+    n, k = 300, 64
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x = torch.rand(n, k, device=DEV, generator=g).half().requires_grad_()
+    w = ((1 + torch.rand(m, k, device=DEV, generator=g)) * torch.linspace(1, 2, k, device=DEV)).half()
+    dy = ((1 + torch.rand(n, m, device=DEV, generator=g)) * torch.linspace(1, 2, n, device=DEV)[:, None] * 1000 / m).half()
+    dx, = torch.autograd.grad(linear(x, w, None, act, dropout_p=p, seed=5), [x], dy)
+    dz = dy.double() if not p else dy.double() * dropout(torch.ones(n, m, device=DEV, dtype=torch.float16), p, 5).double()
+    want = dz @ w.double()
+    short = (dx.double() - want) / want
+    assert abs(float(short.mean())) <= 2.0 ** -12 and float(short.abs().max()) <= half(torch.float16) + 2.0 ** -11
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,k,m", [(1, 8, 32769), (130, 33, 40001), (700, 96, 65544)])
+def test_gradients_of_more_outputs_than_inputs_may_be(dtype, n, k, m):
+    x, w, b, _, dy = make(n, k, m, dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    for act, p in ((None, 0.0), ("gelu", 0.25)):
+        got = torch.autograd.grad(linear(*leaves, act, dropout_p=p, seed=4), leaves, dy)
+        x64, w64, b64 = (t.detach().double() for t in leaves)
+        keep = dropout(torch.ones(n, m, device=DEV), p, 4).double() if p else 1.0
+        dz = dy.double() * keep * act64(x64 @ w64.t() + b64, act)[1]
+        for a, e in zip(got, (dz @ w64, dz.t() @ x64, dz.sum(0))):   # dz's rounding and the result's; sums beside them
+            assert off(a, e) <= 2 * half(dtype)
+
+
 @pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64)])
 def test_a_gradient_in_fp32_between_boundaries(n, k, m):
     """What the backward pass of a concatenation gives: contiguous rows that start on any element.  Parts of half a gigabyte."""

@@ -37,6 +37,9 @@ constexpr int64_t PIECE_BYTES = 512ll << 20;   // of dz
 // rounding: sums of one sign lose 1.4e-7 of themselves for each 16 rows (dW of 1.2 million x 64 -> 64, 8 100 rows a block, came out
 // 7e-5 short, of 10 million 2.4e-4, of 30 million 9e-4, where half a step of fp16 is 2.4e-4 at least).  With these, 7e-5.
 constexpr int MOST_SUMMED = 8192;
+// The same of the products that are one launch's, over inputs (which are not more) and over outputs (dx): 2 048 steps, 3e-4.
+constexpr int MOST_TERMS = 32768;
+static_assert(MOST_INPUTS <= MOST_TERMS, "sums over the inputs are not divided");
 
 // ------------------------------------------------------------------ sums of the splits
 
@@ -120,7 +123,8 @@ struct Pieces {
   int rows, count, splits, last_splits;   // of a piece; pieces; splits of a full piece and of the last one
   bool whole;                             // the kernel that makes all of them (16 bits, narrow layers); its splits are its blocks
   bool parts;                             // fp32: the operands are sums of three bf16 numbers
-  int64_t dz_ld, x_parts, dz_parts, w_parts, slab, ones, bytes;
+  int x_splits;                           // of dx: parts of the outputs (0: one launch finishes it)
+  int64_t dz_ld, x_slab, x_parts, dz_parts, w_parts, slab, ones, bytes;
 };
 enum Want { DX = 1, DW = 2, DB = 4 };     // none of them: forward
 // aligned: dy is read as x is (fp32 numbers always are).
@@ -150,7 +154,9 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, b
   p.parts = dtype == WCN_F32;
   const bool weights = what & (DW | DB), makes_dz = what && !direct;
   const bool of_x = p.parts && (!what || makes_dz || weights), of_dz = p.parts && what, of_w = p.parts && (!what || makes_dz || (what & DX));
-  const int64_t each = (makes_dz ? p.dz_ld * e : 0) + (of_x ? round(k, 8) * 6 : 0) + (of_dz ? round(m, 8) * 6 : 0);   // bytes of a row of a piece
+  if (what & DX && dtype != WCN_F32 && m > MOST_TERMS) p.x_splits = (m + MOST_TERMS - 1) / MOST_TERMS;
+  const int64_t x_slab = (int64_t)p.x_splits * wcn_ce_round(k, 16) * 4;
+  const int64_t each = x_slab + (makes_dz ? p.dz_ld * e : 0) + (of_x ? round(k, 8) * 6 : 0) + (of_dz ? round(m, 8) * 6 : 0);   // bytes of a row of a piece
   int64_t rows = each ? PIECE_BYTES / each / 128 * 128 : n;
   if (rows < 1024) rows = 1024;
   const int64_t count = (n + rows - 1) / rows;
@@ -164,6 +170,7 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, b
     return here;
   };
   take(makes_dz ? p.rows * p.dz_ld * e : 0);
+  p.x_slab = take(p.rows * x_slab);
   p.x_parts = take(of_x ? wcn_linear_parts_bytes(p.rows, k) : 0);
   p.dz_parts = take(of_dz ? wcn_linear_parts_bytes(p.rows, m) : 0);
   p.w_parts = take(of_w ? wcn_linear_parts_bytes(m, k) : 0);
@@ -294,7 +301,16 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
       }
       if (rc != WCN_OK) return rc;
     }
-    if (dx) {
+    if (dx && p.x_splits) {
+      wcn_ce_product q = {};
+      q.a = dz; q.a_ld = dz_ld; q.b = w; q.b_ld = w_ld;
+      q.m = rows; q.n = k; q.k = m;
+      q.splits = p.x_splits;
+      q.slab = (float*)(ws + p.x_slab);
+      rc = wcn_ce_product_run(q, false, false, dtype, dev_status, st);
+      if (rc == WCN_OK) rc = join({q.slab, nullptr, (char*)dx + r0 * k * size, nullptr, rows, k, ld, p.x_splits, 0, factor, dev_status}, dtype, st);
+      if (rc != WCN_OK) return rc;
+    } else if (dx) {
       wcn_linear_product q = {dz, w, dz_ld, w_ld, rows, k, m, nullptr, nullptr, (char*)dx + r0 * k * size, k, nullptr, WCN_ACT_NONE, false, nullptr, 0, none, 0, factor};
       rc = run(q, dtype, true, dzs, wsp, dev_status, st);
       if (rc != WCN_OK) return rc;
