@@ -1,0 +1,36 @@
+"""Graphs of gradients (``create_graph=True``) where one input of an operator was made from another, or is it: the derivatives of the
+operators' formulas, each input for itself."""
+import pytest
+import torch
+
+from warpconvnet_b200 import segmented_group_norm
+from warpconvnet_b200.nn.functional import group_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def leaves(*shapes):
+    g = torch.Generator().manual_seed(0)
+    return [torch.randn(s, generator=g).to(DEV).requires_grad_() for s in shapes]
+
+
+def check(f, plain, inputs, bound=1e-5):
+    """First gradients with a graph, and where that has one the gradients of their squares, against those of ``plain``.  (fp32 against fp32 in
+    another order, some 30 roundings of sums of a thousand terms at most.)"""
+    got, want = (torch.autograd.grad(h(*inputs), inputs, create_graph=True) for h in (f, plain))
+    for a, e in zip(got, want):
+        assert float((a - e).norm()) <= bound * float(e.norm())
+    got, want = (torch.autograd.grad(sum(t.square().sum() for t in first), inputs) for first in (got, want))
+    for a, e in zip(got, want):
+        assert float((a - e).norm()) <= 10 * bound * float(e.norm())
+
+
+def test_group_norm():
+    a, w = leaves((60, 8), (8,))
+    offsets = [0, 20, 60]
+
+    def run(norm):
+        return lambda a, w: norm(a + norm(a, w, None), w, w * 0.5).pow(3).sum()
+    check(run(lambda x, w, b: segmented_group_norm(x, offsets, 2, w, b, activation="silu")),
+          run(lambda x, w, b: group_norm.formula(x, offsets, 2, w, b, 1e-5, "silu")), [a, w])

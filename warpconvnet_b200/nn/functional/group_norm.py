@@ -11,7 +11,7 @@ import torch
 from torch import Tensor
 
 from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
-from .batch_norm import _bits, _counter, reverse_mode_only
+from .batch_norm import _bits, _counter, apart, reverse_mode_only
 
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -104,6 +104,7 @@ class _SegmentedGroupNorm(torch.autograd.Function):
     def backward(ctx, dy: Tensor):
         x, weight, bias, saved = ctx.saved_tensors
         if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+            x, weight, bias = apart(x, weight, bias)
             y = formula(x, ctx.offsets, ctx.groups, weight, bias, ctx.eps, ctx.activation)
             wanted = [t for t, need in zip((x, weight, bias), ctx.needs_input_grad) if need]
             got = iter(torch.autograd.grad(y, wanted, dy, create_graph=True))
