@@ -3,8 +3,9 @@ operators' formulas, each input for itself."""
 import pytest
 import torch
 
-from warpconvnet_b200 import segmented_group_norm
+from warpconvnet_b200 import linear_cross_entropy, segmented_group_norm
 from warpconvnet_b200.nn.functional import group_norm
+from warpconvnet_b200.nn.functional.linear_cross_entropy import formula as cross_entropy
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -34,3 +35,9 @@ def test_group_norm():
         return lambda a, w: norm(a + norm(a, w, None), w, w * 0.5).pow(3).sum()
     check(run(lambda x, w, b: segmented_group_norm(x, offsets, 2, w, b, activation="silu")),
           run(lambda x, w, b: group_norm.formula(x, offsets, 2, w, b, 1e-5, "silu")), [a, w])
+
+
+def test_linear_cross_entropy():
+    a, w = leaves((60, 16), (16, 16))
+    labels = torch.randint(0, 16, (60,), generator=torch.Generator().manual_seed(1)).to(DEV)
+    check(lambda a, w: linear_cross_entropy(a @ w, w, labels, w.sum(1)), lambda a, w: cross_entropy(a @ w, w, labels, w.sum(1), -100, "mean"), [a, w])

@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 
 from ..._native import check, count_training_launches, device_status, dtype_code, lib, on_device, ptr, query_bytes, require_cuda, stream_ptr
-from .batch_norm import _counter, reverse_mode_only
+from .batch_norm import _counter, apart, reverse_mode_only
 
 _MOST, _MOST_CHANNELS = 0x7FFFFEFF, 32768   # rows, classes; channels (row numbers of the kernels are 32-bit)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -92,6 +92,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, grad: Tensor):
         x, weight, bias, labels, kept, x_rows, w_rows = ctx.saved_tensors
         if torch.is_grad_enabled():  # a graph of the gradient is wanted
+            x, weight, bias = apart(x, weight, bias)
             loss = formula(x, weight, labels, bias, ctx.ignore_index, ctx.reduction)
             wanted = [t for t, need in zip((x, weight, bias), ctx.needs_input_grad) if need]
             got = iter(torch.autograd.grad(loss, wanted, grad, create_graph=True))
