@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from warpconvnet_b200 import linear_cross_entropy, segmented_group_norm
-from warpconvnet_b200.nn.functional import group_norm
+from warpconvnet_b200.nn.functional import batch_norm, group_norm
 from warpconvnet_b200.nn.functional.linear_cross_entropy import formula as cross_entropy
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,12 @@ def test_linear_cross_entropy():
     a, w = leaves((60, 16), (16, 16))
     labels = torch.randint(0, 16, (60,), generator=torch.Generator().manual_seed(1)).to(DEV)
     check(lambda a, w: linear_cross_entropy(a @ w, w, labels, w.sum(1)), lambda a, w: cross_entropy(a @ w, w, labels, w.sum(1), -100, "mean"), [a, w])
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_batch_norm_with_residual(relu):
+    a, m, dy = leaves((60, 16), (16, 16), (60, 16))
+    bn = torch.nn.BatchNorm1d(16).to(DEV).train()
+    for x in (lambda a, m: a, lambda a, m: a @ m):
+        check(lambda a, m: (batch_norm.batch_norm_act(x(a, m), bn, relu, a) * dy * m.sum()).sum(),
+              lambda a, m: (batch_norm.formula(x(a, m), bn.weight, bn.bias, a, bn.eps, relu) * dy * m.sum()).sum(), [a, m])

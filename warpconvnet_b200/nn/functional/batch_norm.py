@@ -148,6 +148,7 @@ class _BatchNormAct(torch.autograd.Function):
     def backward(ctx, dy: Tensor):
         x, gamma, beta, residual, saved, y = ctx.saved_tensors
         if torch.is_grad_enabled():  # a graph of the gradient is wanted: the same formulas through torch
+            x, gamma, beta, residual = apart(x, gamma, beta, residual)
             z = formula(x, gamma, beta, residual, ctx.eps, ctx.relu)
             wanted = [t for t, need in zip((x, gamma, beta, residual), ctx.needs_input_grad) if need]
             got = iter(torch.autograd.grad(z, wanted, dy, create_graph=True))
