@@ -3,9 +3,10 @@ operators' formulas, each input for itself."""
 import pytest
 import torch
 
-from warpconvnet_b200 import linear_cross_entropy, segmented_group_norm
+from warpconvnet_b200 import SparseConv3d, Voxels, linear_cross_entropy, segmented_group_norm
 from warpconvnet_b200.nn.functional import batch_norm, group_norm
 from warpconvnet_b200.nn.functional.linear_cross_entropy import formula as cross_entropy
+from warpconvnet_b200.nn.functional.sparse_conv import train_layer_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -50,3 +51,26 @@ def test_batch_norm_with_residual(relu):
     for x in (lambda a, m: a, lambda a, m: a @ m):
         check(lambda a, m: (batch_norm.batch_norm_act(x(a, m), bn, relu, a) * dy * m.sum()).sum(),
               lambda a, m: (batch_norm.formula(x(a, m), bn.weight, bn.bias, a, bn.eps, relu) * dy * m.sum()).sum(), [a, m])
+
+
+def test_a_convolution_with_norm_and_its_input_as_residual():
+    g = torch.Generator().manual_seed(0)
+    xyz = torch.unique(torch.randint(0, 12, (700, 3), generator=g, dtype=torch.int32), dim=0)
+    feats, dy = (torch.randn(len(xyz), 32, generator=g).to(DEV) for _ in range(2))
+    torch.manual_seed(0)
+    layer, bn = SparseConv3d(32, 32, 3, bias=False).to(DEV).train(), torch.nn.BatchNorm1d(32).to(DEV).train()
+    x = Voxels(xyz.to(DEV), feats, offsets=torch.tensor([0, len(xyz)]))
+    a = feats.clone().requires_grad_()
+    inputs = [a, layer.weight]
+
+    def together(f):
+        y = train_layer_norm(layer, bn, x.replace(batched_features=f), None, True, f)
+        assert "LayerNorm" in type(y.feature_tensor.grad_fn).__name__
+        return y.feature_tensor
+
+    def apart(f):
+        return batch_norm.formula(layer(x.replace(batched_features=f)).feature_tensor, bn.weight, bn.bias, f, bn.eps, True)
+    for f in (lambda t: t, lambda t: t * 2):
+        got, want = (torch.autograd.grad((h(f(a)) * dy).sum(), inputs, create_graph=True) for h in (together, apart))
+        for p, q in zip(got, want):   # (the same kernels, sums in another order)
+            assert float((p - q).norm()) <= 1e-5 * float(q.norm())

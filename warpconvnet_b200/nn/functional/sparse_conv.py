@@ -1418,6 +1418,7 @@ class _LayerNormFunction(torch.autograd.Function):
         x, weight, gamma, beta, residual, z, stats, y = ctx.saved_tensors
         need = ctx.needs_input_grad[:5]
         if torch.is_grad_enabled():  # a graph of the gradient is wanted: the two steps as they are without this function
+            x, weight, gamma, beta, residual = batch_norm.apart(x, weight, gamma, beta, residual)
             out = batch_norm.formula(_LayerFunction.apply(x, weight, ctx.tables), gamma, beta, residual, ctx.eps, ctx.relu)
             got = iter(torch.autograd.grad(out, [t for t, n in zip((x, weight, gamma, beta, residual), need) if n], dy,
                                            create_graph=True))
