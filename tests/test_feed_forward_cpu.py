@@ -97,3 +97,11 @@ def test_a_workspace_for_a_gradient_in_fp32_does_not_go_by_where_it_lies(n, k, m
         for act, least in ((0, 0), (0, 100), (3, 0)):
             sizes = {_native.query_bytes("wcn_linear_workspace_bytes", n, k, m, _native.WCN_F32, what, act, least, aligned) for aligned in (0, 1)}
             assert len(sizes) == 1
+
+
+@pytest.mark.parametrize("n,k,m,dtype,act,aligned", [(5000, 8, 1 << 20, _native.WCN_BF16, 1, 1), (300, 64, 60_000, _native.WCN_F32, 3, 1), (5000, 64, 1 << 19, _native.WCN_F16, 0, 0),
+                                                     (100_000_000, 8, 13, _native.WCN_F16, 0, 0), (20_000_000, 64, 100, _native.WCN_BF16, 2, 0)])
+def test_workspaces_stay_bounded(n, k, m, dtype, act, aligned):
+    """Pieces of 512 MB (or 128 rows), also for many outputs and for a gradient between boundaries; what the weight's parts take beside them is its own."""
+    size = _native.query_bytes("wcn_linear_workspace_bytes", n, k, m, dtype, 1, act, 0, aligned)
+    assert size <= (512 << 20) + (1 << 20) + (6 * k * m if dtype == _native.WCN_F32 else 0)

@@ -3,7 +3,7 @@
 //
 // z is computed again in the backward pass, not kept: for rows as wide as these a product costs less than writing z and reading it (at
 // 1.4 PFLOP/s and 6.5 TB/s up to some 400 inputs), and a training step holds x alone.  Gradients of narrow layers in 16 bits are one
-// kernel's (linear_backward_tcgen05.cu).  Elsewhere dz, rounded to the inputs' type, goes to the workspace, in pieces of at most 512 MB
+// kernel's (linear_backward_tcgen05.cu).  Elsewhere dz, rounded to the inputs' type, goes to the workspace, in pieces of at most 512 MB (or 128 rows)
 // (pieces that stay in L2 lost more by their launches than they gained: 240 000 x 96 -> 384 in pieces of 64 MB 241 us, whole 196); each
 // is multiplied by W (dx) and by x (dW), whose sums over the rows are divided among the multiprocessors, in 16 bits into parts of
 // 8192 rows at most too, and joined in a fixed order and in double: the same bits on every run.
@@ -158,7 +158,7 @@ Pieces plan(int64_t n, int k, int m, int dtype, int what, int act, bool drops, b
   const int64_t x_slab = (int64_t)p.x_splits * wcn_ce_round(k, 16) * 4;
   const int64_t each = x_slab + (makes_dz ? p.dz_ld * e : 0) + (of_x ? round(k, 8) * 6 : 0) + (of_dz ? round(m, 8) * 6 : 0);   // bytes of a row of a piece
   int64_t rows = each ? PIECE_BYTES / each / 128 * 128 : n;
-  if (rows < 1024) rows = 1024;
+  if (rows < 128) rows = 128;
   const int64_t count = (n + rows - 1) / rows;
   rows = round((n + count - 1) / count, 128);
   p.rows = (int)(rows < n ? rows : n);
