@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from warpconvnet_b200._native import check_device_status, device_status
+from warpconvnet_b200._native import check_device_status, device_status, dtype_code, query_bytes
 from warpconvnet_b200.nn.functional.dropout import dropout
 from warpconvnet_b200.nn.functional.linear import linear, linear_8bit
 from warpconvnet_b200.nn.functional.rms_norm import quantize_rows
@@ -245,6 +245,58 @@ def test_gradients_of_more_outputs_than_inputs_may_be(dtype, n, k, m):
         dz = dy.double() * keep * act64(x64 @ w64.t() + b64, act)[1]
         for a, e in zip(got, (dz @ w64, dz.t() @ x64, dz.sum(0))):   # dz's rounding and the result's; sums beside them
             assert off(a, e) <= 2 * half(dtype)
+
+
+# Wide in 16 bits (pieces of dz, the last one with other splits; dx of it in parts), narrow (rows of one launch; a gradient that is copied), fp32.
+PIECES = [(300_001, 64, 1024, torch.bfloat16), (8_000, 64, 40_000, torch.float16), (1_300_001, 16, 40, torch.float16), (1_250_003, 24, 13, torch.bfloat16), (1_300_001, 64, 8, torch.float32)]
+
+
+@pytest.mark.parametrize("act,p", [(None, 0.3), ("gelu", 0.3), ("gelu", 0.0)])
+@pytest.mark.parametrize("n,k,m,dtype", PIECES)
+def test_gradients_of_more_rows_than_a_piece(n, k, m, dtype, act, p):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x, dy = (torch.randn(n, c, device=DEV, generator=g).to(dtype) for c in (k, m))
+    w, b = (torch.randn(m, k, device=DEV, generator=g) / k ** 0.5).to(dtype), torch.randn(m, device=DEV, generator=g).to(dtype)
+    what, aligned = 7, int(dtype == torch.float32 or m % 8 == 0)
+    one = query_bytes("wcn_linear_workspace_bytes", n // 3, k, m, dtype_code(dtype), what, 3 if act else 0, round(65536 * p), aligned)
+    whole = query_bytes("wcn_linear_workspace_bytes", n, k, m, dtype_code(dtype), what, 3 if act else 0, round(65536 * p), aligned)
+    assert 1.4 * one < whole < 2.1 * one   # two pieces (of one: three times as much, or for sums alone as much)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(linear(*leaves, act, dropout_p=p, seed=77), leaves, dy)
+    keep = dropout(torch.ones(n, m, device=DEV, dtype=torch.bfloat16), p, 77) if p else None
+    w64, b64 = w.detach().double(), b.detach().double()
+    want = [torch.empty(n, k, dtype=torch.float64, device=DEV), torch.zeros(m, k, dtype=torch.float64, device=DEV), torch.zeros(m, dtype=torch.float64, device=DEV)]
+    step = 1 << 13 if m > 10_000 else 1 << 17
+    for at in range(0, n, step):
+        rows = slice(at, at + step)
+        x64 = x[rows].detach().double()
+        dz = dy[rows].double() * act64(x64 @ w64.t() + b64, act)[1]
+        if p:
+            dz *= (keep[rows] != 0) / (1 - round(65536 * p) / 65536)
+        want[0][rows] = dz @ w64
+        want[1] += dz.t() @ x64
+        want[2] += dz.sum(0)
+    # in 16 bits dz is rounded and the result is; in fp32 as at fewer rows
+    bound = 2 * half(dtype) if dtype != torch.float32 else 4e-6
+    for a, e in zip(got, want):
+        assert off(a, e) <= bound
+    for rows in (slice(0, 500), slice(n // 2, n // 2 + 500), slice(n - 500, n)):
+        assert off(got[0][rows], want[0][rows]) <= bound
+
+
+def test_more_rows_than_a_piece_forward_in_fp32():
+    n, k, m = 1_500_001, 64, 8
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, r = torch.randn(n, k, device=DEV, generator=g), torch.randn(n, m, device=DEV, generator=g)
+    w, b = torch.randn(m, k, device=DEV, generator=g) / 8, torch.randn(m, device=DEV, generator=g)
+    one = query_bytes("wcn_linear_workspace_bytes", n // 3, k, m, dtype_code(x.dtype), 0, 3, 20000, 0)
+    assert query_bytes("wcn_linear_workspace_bytes", n, k, m, dtype_code(x.dtype), 0, 3, 20000, 0) < 2.1 * one   # two pieces
+    y = linear(x, w, b, "gelu", r, 20000 / 65536, 3)
+    keep = dropout(torch.ones(n, m, device=DEV), 20000 / 65536, 3) != 0
+    z, _ = act64(x.double() @ w.double().t() + b.double(), "gelu")
+    want = r.double() + torch.where(keep, z * (65536 / 45536), 0.0)
+    # 64 products' sum and its rounding (|x| |w| has the norm of some 8 x 64^0.5 / 8), the activation's 3e-7, the addition's
+    assert ((y.double() - want).abs() <= 64 * U * (1 + want.abs() + x.double().abs() @ w.double().abs().t())).all()
 
 
 @pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64)])
