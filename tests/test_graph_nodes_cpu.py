@@ -1,8 +1,10 @@
 """Nodes of autograd's graph in the extension (csrc/autograd.cpp): what they pass on to Python, and what stands in for them."""
+import copy
 import gc
 import os
 import subprocess
 import sys
+from collections import Counter
 
 import pytest
 import torch
@@ -193,3 +195,35 @@ def test_what_a_node_keeps_goes_with_it():
     del y
     gc.collect()
     assert kept[0] == 0
+
+
+def test_launches_of_the_extension_are_counted_however_they_are_read(monkeypatch):
+    class Nodes:
+        left = 0
+
+        def launches(self):
+            n, self.left = self.left, 0
+            return (0, 0, n, 0, 0, 0)
+    nodes = Nodes()
+    monkeypatch.setattr(_native, "_nodes", nodes)
+    counts = _native.LAUNCH_COUNTS
+    monkeypatch.setattr(_native, "LAUNCH_COUNTS", counts := type(counts)())
+    reads = [lambda: counts["wcn_dropout"], lambda: counts.get("wcn_dropout"), lambda: dict(counts)["wcn_dropout"], lambda: dict(counts.items())["wcn_dropout"],
+             lambda: sum(counts.values()), lambda: counts.total(), lambda: counts.copy()["wcn_dropout"], lambda: (counts - Counter())["wcn_dropout"],
+             lambda: copy.deepcopy(counts)["wcn_dropout"], lambda: counts.most_common(1)[0][1], lambda: {**counts}["wcn_dropout"], lambda: list(counts.elements()).count("wcn_dropout"),
+             lambda: 10 * len(counts), lambda: 10 * ("wcn_dropout" in counts), lambda: 10 * len(list(counts)), lambda: 10 * len(counts.keys()), lambda: counts.pop("wcn_dropout"),
+             _native.launches_total]
+    for read in reads:
+        counts.clear()
+        nodes.left = 3
+        before = counts["wcn_dropout"]   # (3 of them are in)
+        nodes.left = 7
+        assert before == 3 and read() == 10
+    nodes.left = 5
+    taken = counts.copy()
+    nodes.left = 2
+    assert taken["wcn_dropout"] == counts["wcn_dropout"] - 2   # (a copy takes nothing away)
+    counts.clear()
+    nodes.left = 5   # (what was launched before goes with the others)
+    counts.clear()
+    assert counts["wcn_dropout"] == 0

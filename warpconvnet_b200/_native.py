@@ -158,26 +158,47 @@ KERNELS_PER_CALL = {
 
 
 class _LaunchCounts(Counter):
-    """Kernels launched through each entry point.  Those of the extension, which launches without Python, are added when they are asked for."""
+    """Kernels launched through each entry point.  Those of the extension, which launches without Python, are added whenever it is read."""
 
     def _with_nodes(self):
-        if _nodes:
+        if _nodes and self is LAUNCH_COUNTS:   # (a copy has what was counted until then)
             for name, kernels in zip(("wcn_linear_backward", "wcn_rms_norm_backward", "wcn_dropout", "wcn_linear", "wcn_rms_norm", "wcn_linear_8bit"), _nodes.launches()):
                 if kernels:
-                    self[name] = self.get(name, 0) + kernels
-        return self
+                    self[name] = dict.get(self, name, 0) + kernels
+        return super()
 
     def __getitem__(self, name):
-        return super(_LaunchCounts, self._with_nodes()).__getitem__(name)
+        return self._with_nodes().__getitem__(name)
+
+    def __contains__(self, name):
+        return self._with_nodes().__contains__(name)
+
+    def __iter__(self):
+        return self._with_nodes().__iter__()
+
+    def __len__(self):
+        return self._with_nodes().__len__()
+
+    def get(self, name, default=None):
+        return self._with_nodes().get(name, default)
+
+    def keys(self):
+        return self._with_nodes().keys()
 
     def items(self):
-        return super(_LaunchCounts, self._with_nodes()).items()
+        return self._with_nodes().items()
 
     def values(self):
-        return super(_LaunchCounts, self._with_nodes()).values()
+        return self._with_nodes().values()
+
+    def pop(self, *args):
+        return self._with_nodes().pop(*args)
 
     def clear(self):
-        super(_LaunchCounts, self._with_nodes()).clear()
+        self._with_nodes().clear()
+
+    def copy(self):
+        return Counter(dict(self))
 
 
 LAUNCH_COUNTS = _LaunchCounts()
@@ -189,7 +210,7 @@ def _counted(raw, name: str, kernels: Optional[int]):
         return raw
 
     def fn(*args):
-        LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + kernels
+        LAUNCH_COUNTS[name] = dict.get(LAUNCH_COUNTS, name, 0) + kernels
         return raw(*args)
     return fn
 
@@ -220,12 +241,12 @@ class _Library:
 def count_f32_launches(name: str) -> None:
     """Corrects what the call just made was counted as: with a workspace ``wcn_conv_fwd`` launches one or two kernels,
     ``wcn_conv_wgrad_f32`` two or three."""
-    LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + lib().wcn_conv_f32_launches() - KERNELS_PER_CALL[name]
+    LAUNCH_COUNTS[name] = dict.get(LAUNCH_COUNTS, name, 0) + lib().wcn_conv_f32_launches() - KERNELS_PER_CALL[name]
 
 
 def count_training_launches(name: str) -> None:
     """The same for group norm, linear cross entropy, AdamW, the gradient of RMS norm and linear layers, which launch as many kernels as their sizes ask for."""
-    LAUNCH_COUNTS[name] = LAUNCH_COUNTS.get(name, 0) + lib().wcn_training_launches() - KERNELS_PER_CALL[name]
+    LAUNCH_COUNTS[name] = dict.get(LAUNCH_COUNTS, name, 0) + lib().wcn_training_launches() - KERNELS_PER_CALL[name]
 
 
 def launches_total() -> int:
