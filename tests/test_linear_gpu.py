@@ -299,6 +299,23 @@ def test_more_rows_than_a_piece_forward_in_fp32():
     assert ((y.double() - want).abs() <= 64 * U * (1 + want.abs() + x.double().abs() @ w.double().abs().t())).all()
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("n,k,m", [(300, 32, 64), (300, 512, 640)])   # in one kernel, and by way of dz
+def test_large_gradients_in_fp16_under_dropout(n, k, m, act):
+    """What is kept is multiplied by 8: the gradients are in range, though the one behind the activation times 8 is not."""
+    x, w, b, _, dy = make(n, k, m, torch.float16)
+    leaves = [t.requires_grad_() for t in (x * 0.002, w * 2.0 ** -11, b)]
+    dy = (dy.sign() * 30000).half()
+    dx, dw, _ = torch.autograd.grad(linear(*leaves, act, dropout_p=0.875, seed=2), leaves, dy)
+    x64, w64, b64 = (t.detach().double() for t in leaves)
+    keep = (dropout(torch.ones(n, m, device=DEV), 0.875, 2) != 0).double() * 8
+    dz = dy.double() * keep * act64(x64 @ w64.t() + b64, act)[1]
+    want = dz @ w64, dz.t() @ x64
+    assert float(dz.abs().max()) > 2 * 65504 and max(float(e.abs().max()) for e in want) < 65000
+    for a, e in zip((dx, dw), want):   # dz's rounding and the result's
+        assert off(a, e) <= 2 * half(torch.float16)
+
+
 @pytest.mark.parametrize("n,k,m", [(1_000_000, 64, 13), (600_000, 64, 64)])
 def test_a_gradient_in_fp32_between_boundaries(n, k, m):
     """What the backward pass of a concatenation gives: contiguous rows that start on any element.  Parts of half a gigabyte."""

@@ -261,7 +261,9 @@ extern "C" int wcn_linear_backward(const void* x, int64_t x_ld, int64_t n, int32
   const wcn_drop none = wcn_make_drop(0, 0, nullptr);
   wcn_drop drop = wcn_make_drop((uint32_t)least, seed, seed_at);
   float factor = 1.f;
-  if (act == WCN_ACT_NONE && least && dtype != WCN_F32) {   // dz is dy or nothing, without a rounding: the factor comes to the sums
+  // In 16 bits dz is what is kept of dy (times the slope): the factor comes to the fp32 sums.  Without an activation nothing is rounded then; with
+  // one, dz in fp16 does not pass the type's end for the factor's sake.
+  if (least && dtype != WCN_F32) {
     factor = drop.scale;
     drop.scale = 1.f;
   }
