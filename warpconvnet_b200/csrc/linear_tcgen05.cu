@@ -9,9 +9,8 @@
 // would cost the load/store pipe a line each.  Rows that TMA cannot take (pitches that are no multiple of 16 bytes) go the same way
 // through shared memory and from there in elements.
 // Where they fit beside a ring of four tiles, the columns' rows of B stay in shared memory: a block then has one group of
-// columns, and A alone passes.  Elsewhere, with 256 columns and eight slices of k and more, two blocks of a cluster share a tile of 256 rows
-// (one instruction for both, B's rows halved between them): half of B's bytes from L2, which bound the wide layers (100 000 x 1 024 ->
-// 1 024 bf16 196 us with a block a tile, 161 with two; of 8-bit operands 116 and 99).
+// columns, and A alone passes.  Elsewhere, with 192 columns of a tile and six slices of k and more, two blocks of a cluster share a tile of 256
+// rows (one instruction for both, B's rows halved between them): half of B's bytes from L2, which bound the wide layers.
 //
 // Sixteen warps empty the accumulators: with eight, twelve and 24 the layer below took 98, 82 and 78 us where it takes 72.
 // 240 000 rows, bf16, us: 96 -> 384 40 (5.7 TB/s), with GELU 65, with dropout too 117: issue slots, some 270 arithmetic instructions
@@ -524,8 +523,12 @@ void plan(const wcn_linear_product& q, int kind, bool b_mn, Params* p) {
   p->accs = 512 / nt < MAX_ACC ? 512 / nt : MAX_ACC;
   // Operands that both pass: two blocks share a tile of 256 rows, each with half of B's rows, where there are tiles for all of them.
   // What arrives in a block's shared memory is then 64 bytes a clock of the matrix instructions; alone, 96 at 256 columns, it waits.
+  // 100 000 rows bf16, a block a tile and two, us: 1 024 -> 1 024 198, 163; 1 024 -> 256 73, 67; 768 -> 256 60, 54; 384 -> 256 38, 36; 512 -> 200
+  // 46, 40; of 8-bit operands 1 024 -> 1 024 118, 99; 768 -> 256 (six slices) 40, 38.  Narrower tiles have less of B, and short sums wait for
+  // the other block at each tile: 512 -> 96 34, 34; 1 024 -> 64 52, 54; 2 048 -> 32 87, 89, and its dx, one slice, 75, 81; 8 bits, 384 -> 256
+  // (three slices) 26, 27.
   const int pair_tiles = (int)(((int64_t)q.m + 2 * TILE_M - 1) / (2 * TILE_M));
-  p->pair = !resident && nt % (b_mn ? 128 : 32) == 0 && (int64_t)pair_tiles * tiles_of(nt) * 2 >= sms;
+  p->pair = !resident && nt >= 192 && nt % (b_mn ? 128 : 32) == 0 && p->KB >= 6 && (int64_t)pair_tiles * tiles_of(nt) * 2 >= sms;
   if (p->pair) {
     p->m_tiles = pair_tiles;
     p->b_slice = slice(nt / 2);
