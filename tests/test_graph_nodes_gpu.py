@@ -1,5 +1,6 @@
 """Gradients through the nodes of csrc/autograd.cpp and through autograd functions in Python: the same bits, whatever lies how."""
 import threading
+import time
 
 import pytest
 import torch
@@ -145,6 +146,33 @@ def test_kept_graphs_checkpoints_streams_and_threads():
         t.join()
     for got in results:
         same(got, want)
+
+
+def test_other_threads_go_on_while_a_launch_waits():
+    """The GPU is kept busy for half a second, and a thousand launches fill its queue: Python's other threads run meanwhile."""
+    x, w = torch.randn(64, 64, device=DEV).bfloat16(), torch.randn(64, 64, device=DEV).bfloat16()
+    q, s = norm_module.quantize_rows(x)
+    qw, sw = norm_module.quantize_rows(w)
+    for call in (lambda: linear_module.linear(x, w), lambda: norm_module.rms_norm(x), lambda: norm_module.rms_norm_8bit(x), lambda: dropout_module.dropout(x, 0.5, 3),
+                 lambda: linear_module.linear_8bit(q, s, qw, sw)):
+        call()
+        torch.cuda.synchronize()
+        longest, done = 0.0, threading.Event()
+
+        def launch():
+            torch.cuda._sleep(1_000_000_000)
+            for _ in range(1500):
+                call()
+            done.set()
+        thread = threading.Thread(target=launch)
+        thread.start()
+        last = time.perf_counter()
+        while not done.wait(0.002):
+            now = time.perf_counter()
+            longest, last = max(longest, now - last), now
+        thread.join()
+        torch.cuda.synchronize()
+        assert longest < 0.2, longest
 
 
 def test_what_the_library_refuses_is_an_error_of_the_engine_s_thread():

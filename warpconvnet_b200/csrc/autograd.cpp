@@ -303,19 +303,23 @@ py::object run_norm(const Tensor& x, const std::optional<Tensor>& weight, double
   if (!same_rows(residual, x, n, c) || (weight && (weight->dim() != 1 || weight->size(0) != c || !plain(*weight, x.device(), at::kFloat)))) return py::none();
   const bool graph = c10::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(residual));
   if (eight && graph) return py::none();   // (refused there)
-  Tensor y = eight ? at::empty({n, c}, x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false)) : rows_like(x, n, c), rstd, scale;
-  if (eight) scale = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
+  Tensor y, rstd, scale;
   std::optional<Tensor> h;
-  if (residual) h = rows_like(x, n, c);
-  if (graph) rstd = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
-  const float number = static_cast<float>(eps);
-  int32_t bits;
-  std::memcpy(&bits, &number, 4);
-  check(native.norm_forward(x.data_ptr(), c, residual ? residual->data_ptr() : nullptr, c, n, c, code,
-                            weight ? static_cast<const float*>(weight->data_ptr()) : nullptr, bits, h ? h->data_ptr() : nullptr, eight ? nullptr : y.data_ptr(),
-                            static_cast<float*>(at_of(rstd)), eight ? y.data_ptr() : nullptr, static_cast<float*>(at_of(scale)), stream_of(x)),
-        "wcn_rms_norm");
-  launched.norm_forward += 1;
+  {
+    py::gil_scoped_release others;
+    y = eight ? at::empty({n, c}, x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false)) : rows_like(x, n, c);
+    if (eight) scale = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
+    if (residual) h = rows_like(x, n, c);
+    if (graph) rstd = at::empty({n}, x.options().dtype(at::kFloat).requires_grad(false));
+    const float number = static_cast<float>(eps);
+    int32_t bits;
+    std::memcpy(&bits, &number, 4);
+    check(native.norm_forward(x.data_ptr(), c, residual ? residual->data_ptr() : nullptr, c, n, c, code,
+                              weight ? static_cast<const float*>(weight->data_ptr()) : nullptr, bits, h ? h->data_ptr() : nullptr, eight ? nullptr : y.data_ptr(),
+                              static_cast<float*>(at_of(rstd)), eight ? y.data_ptr() : nullptr, static_cast<float*>(at_of(scale)), stream_of(x)),
+          "wcn_rms_norm");
+    launched.norm_forward += 1;
+  }
   if (eight) return h ? py::make_tuple(y, scale, *h) : py::make_tuple(y, scale);
   if (graph) norm(y, h, x, residual, weight, rstd, eps, code);
   return h ? py::object(py::make_tuple(y, *h)) : py::cast(y);
@@ -401,8 +405,9 @@ PYBIND11_MODULE(_autograd, m) {
   m.def("status", [](int64_t device, uintptr_t word) {
     if (device >= 0 && device < MOST_DEVICES) status_words[device] = reinterpret_cast<void*>(word);
   });
-  m.def("run_linear", &run_linear);
-  m.def("run_linear_8bit", &run_linear_8bit);
-  m.def("run_norm", &run_norm);
-  m.def("run_dropout", &run_dropout);
+  // A launch waits where a stream's queue is full, as long as the GPU takes (for another thread's launch, it may be): Python's other threads go on.
+  m.def("run_linear", &run_linear, py::call_guard<py::gil_scoped_release>());
+  m.def("run_linear_8bit", &run_linear_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("run_norm", &run_norm);   // (itself, as its results are Python's)
+  m.def("run_dropout", &run_dropout, py::call_guard<py::gil_scoped_release>());
 }
