@@ -7,9 +7,10 @@
 // inputs (1 + outputs / 128) of 512 columns.  The same images in shared memory serve every product: a tile of rows whose columns run
 // along 128-byte (or, for inputs that are no multiple of 64, 64-byte) lines is a K-major operand with its rows on the M / N side, or an
 // MN-major one with its rows on the K side.  Sums of the blocks are joined by linear.cu.
-// The column sums are made of dz before it is rounded, by exchanges among the lanes.
+// The column sums are made of dz before it is rounded, by exchanges among the lanes.  A launch has 8192 rows a block at most (linear.cu).
 // 240 000 x 96 -> 384 bf16 with GELU 120 us (277 MB at 2.3 TB/s; z, dz, dx and dW in launches of their own took 190), without
-// activation 79, with dropout 175: bound by the issue slots of the slope and the generator; the tensor pipe waits for dz.
+// activation 79, with dropout 175: the time is the slope's and the generator's, a piece of a warp after the other; the tensor pipe waits
+// for dz.
 //
 // Every wait is bounded (tcgen05_common.cuh); a kernel that gives up sets the status word, waits for its copies and matrix instructions
 // and frees its tensor memory; its results, and those of a launch that finds the word set, are NaN (dW and dbias: where they are joined).

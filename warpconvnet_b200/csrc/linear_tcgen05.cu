@@ -13,8 +13,9 @@
 // rows (one instruction for both, B's rows halved between them): half of B's bytes from L2, which bound the wide layers.
 //
 // Sixteen warps empty the accumulators: with eight, twelve and 24 the layer below took 98, 82 and 78 us where it takes 72.
-// 240 000 rows, bf16, us: 96 -> 384 40 (5.7 TB/s), with GELU 65, with dropout too 117: issue slots, some 270 arithmetic instructions
-// for a warp's 32 x 32 numbers, 60 % of the cycles busy, and as many again for the generator.  384 -> 96 with residual 46 (6.0 TB/s).
+// 240 000 rows, bf16, us: 96 -> 384 40 (5.7 TB/s), with GELU 65, with dropout too 117.  GELU is some 270 arithmetic instructions of 430 for a
+// warp's 32 x 32 numbers; issue slots are 60 % busy and HBM half: a warp has one piece at a time and waits between its load from tensor
+// memory and its store.  The generator is as many instructions again.  384 -> 96 with residual 46 (6.0 TB/s).
 // 60 000 x 256 -> 1 024 with GELU 82, its dz 95 to 100, its dx 40.  100 000 x 1 024 -> 1 024 of 8 bits 99 (2.1 PFLOP/s), with SiLU and
 // residual 113 to 118.
 //

@@ -9,8 +9,8 @@
 // rows' type), so that the gradient, which reads it again, is that of the same numbers.  Sums, 1 / sqrt and products are fp32.
 // A row whose squares pass the end of fp32 is summed again with its numbers times 2^-80: 8192 of the largest, 2^128 each, then have
 // squares of 2^109 in all, and those that the first sum could not hold, 2^128, are 2^-32.
-// The gradient of w is summed per thread over the rows of a persistent block (tens of them in fp32), then over the block's threads, and
-// over the blocks in double by a second launch: no atomics, the same bits on every run.
+// The gradient of w is summed in fp32 per thread over the rows of a persistent block (25 of 240 000 x 96 in 16 bits, 130 of 1 200 000; more
+// with more rows), then over the block's threads, and over the blocks in double by a second launch: no atomics, the same bits on every run.
 // 240 000 x 96 bf16 with residual 28 us forward (184 MB at 6.6 TB/s, some of what is written still in L2), 46 + 7 backward (161 MB, 4.0
 // TB/s: the loads in flight are those of 32 warps, a row and the next one each); 1 200 000 x 96 fp16 into 8 bits 120 (811 MB, 6.8 TB/s).
 #include <cuda_fp8.h>
