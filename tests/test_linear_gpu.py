@@ -356,6 +356,20 @@ def test_strides_and_boundaries(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k,m", [(45_000, 40, 13), (30_001, 64, 100), (9_000, 300, 20)])
+def test_a_residual_on_boundaries_beside_a_result_that_is_not(dtype, n, k, m):
+    """Columns of a wider buffer whose rows can be copied as a whole, results whose rows cannot."""
+    x, w, b, r, _ = make(n, k, m, dtype)
+    wide = torch.zeros(n, -(-m // 8) * 8, dtype=dtype, device=DEV)
+    wide[:, :m] = r
+    for act in (None, "gelu"):
+        want = linear(x, w, b, act, r)
+        assert all(torch.equal(linear(x, w, b, act, wide[:, :m]), want) for _ in range(3))
+        z, _ = act64(x.double() @ w.double().t() + b.double(), act)
+        assert off(want, z + r.double()) <= (half(dtype) if dtype != torch.float32 else 2e-6)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_numbers_that_are_none_stay_in_their_rows(dtype):
     x, w, b, r, dy = make(300, 64, 96, dtype)
     clean = linear(x, w, b, "gelu", r)

@@ -438,6 +438,7 @@ linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__
           __syncwarp();
           for (int l = 0; l < 32; ++l)
             if (row0 + l < q.m && col + lane < q.n) out[(int64_t)(row0 + l) * q.out_ld + col + lane] = *element(l, lane);
+          if (by_tma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy of what is added comes to this place)
           __syncwarp();
         }
         b ^= 1;
