@@ -662,7 +662,7 @@ int wcn_adamw_decode(const void* exp_avg, const int16_t* exp_avg_base, const voi
 
 /* h = x + residual rounded to dtype (residual NULL: h = x, and the argument h is not used), y = h s weight with
  * s = 1 / sqrt(mean of a row's h^2 + eps), of [n, channels] rows (x_ld and residual_ld elements apart; h and y contiguous); weight: fp32
- * [channels] or NULL; eps (the bits of a float): at least 1e-30.  rstd [n] (may be NULL): s, for the backward pass.  In the place of y:
+ * [channels] or NULL; eps (the bits of a float): 1e-30 or more, finite.  rstd [n] (may be NULL): s, for the backward pass.  In the place of y:
  * q, e4m3 codes of y / scale, with scale [n] = max(largest |y| of a row / 448, 2^-126); a row with a number that is not finite has NaN.
  * wcn_quantize_rows: the same of x itself.
  * backward: dx (contiguous; may be NULL), the gradient of x and of the residual, from that of y and of h (dh; may be NULL); dweight

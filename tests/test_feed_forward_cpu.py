@@ -8,6 +8,7 @@ import torch
 from warpconvnet_b200 import _native
 from warpconvnet_b200.nn.functional.dropout import dropout, kept_factor
 from warpconvnet_b200.nn.functional.rms_norm import rms_norm
+from warpconvnet_b200.nn.functional.rms_norm import check_eps
 
 BASE = 1 << 20   # stands for aligned device memory
 INVALID = -5
@@ -105,3 +106,11 @@ def test_workspaces_stay_bounded(n, k, m, dtype, act, aligned):
     """Pieces of 512 MB (or 128 rows), also for many outputs and for a gradient between boundaries; what the weight's parts take beside them is its own."""
     size = _native.query_bytes("wcn_linear_workspace_bytes", n, k, m, dtype, 1, act, 0, aligned)
     assert size <= (512 << 20) + (1 << 20) + (6 * k * m if dtype == _native.WCN_F32 else 0)
+
+
+def test_an_eps_that_fp32_does_not_hold_is_refused():
+    assert norm(eps=0x7F800000) == INVALID
+    assert check_eps(3.4e38) == 3.4e38
+    for eps in (3.5e38, float("inf"), float("nan"), 0.9e-30):
+        with pytest.raises(ValueError, match="eps"):
+            check_eps(eps)

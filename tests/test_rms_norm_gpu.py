@@ -173,6 +173,15 @@ def test_an_eps_that_counts_beside_large_rows():
     assert ((rms_norm(x, eps=3e38).double() - ref).abs() <= (16 * U) * ref.abs()).all()
 
 
+def test_an_eps_beyond_fp32_is_refused():
+    x = torch.ones(4, 8, device=DEV)
+    for f in (rms_norm, rms_norm_8bit):
+        for eps in (3.5e38, float("inf")):
+            with pytest.raises(ValueError, match="eps"):
+                f(x, eps=eps)
+    assert torch.isfinite(rms_norm(x, eps=3.4e38)).all()
+
+
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(3)
     x, r, w, dy, dh, u, v = (torch.randn(s, generator=g) for s in ((31, 24), (31, 24), (24,), (31, 24), (31, 24), (31, 24), (24,)))

@@ -25,8 +25,8 @@
 #include <dlfcn.h>
 
 #include <atomic>
-#include <cmath>
 #include <cstring>
+#include <limits>
 #include <locale>
 
 #include "../../include/wcn_b200.h"
@@ -298,7 +298,7 @@ std::optional<Tensor> run_linear(const Tensor& x, const Tensor& weight, const st
 py::object run_norm(const Tensor& x, const std::optional<Tensor>& weight, double eps, const std::optional<Tensor>& residual, bool eight, double least_eps,
                     int64_t most_rows, int64_t most_channels) {
   int code = 0;
-  if (!rows_taken(x, most_rows, most_channels, code) || !(eps >= least_eps) || std::isinf(eps)) return py::none();
+  if (!rows_taken(x, most_rows, most_channels, code) || !(eps >= least_eps) || eps > std::numeric_limits<float>::max()) return py::none();
   const int64_t n = x.size(0), c = x.size(1);
   if (!same_rows(residual, x, n, c) || (weight && (weight->dim() != 1 || weight->size(0) != c || !plain(*weight, x.device(), at::kFloat)))) return py::none();
   const bool graph = c10::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(residual));

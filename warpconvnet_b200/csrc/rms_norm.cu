@@ -502,7 +502,7 @@ extern "C" int wcn_rms_norm(const void* x, int64_t x_ld, const void* residual, i
                             const float* weight, uint32_t eps_bits, void* h, void* y, float* rstd, void* q, float* scale, void* stream) {
   if (!sizes_taken(n, channels, dtype)) return WCN_ERR_INVALID_PARAMETERS;
   if (n == 0) return WCN_OK;
-  if (!(float_of(eps_bits) >= LEAST_EPS)) return WCN_ERR_INVALID_PARAMETERS;
+  if (!(float_of(eps_bits) >= LEAST_EPS) || float_of(eps_bits) == INFINITY) return WCN_ERR_INVALID_PARAMETERS;
   if (!x || (residual && !h) || !y == !q || (q && !scale) || (n > 1 && (x_ld < channels || (residual && residual_ld < channels)))) return WCN_ERR_INVALID_PARAMETERS;
   NormParams p = {x, residual, weight, residual ? h : nullptr, y, (uint8_t*)q, scale, rstd, x_ld, residual_ld, n, channels, 0, float_of(eps_bits), false};
   return norm(p, dtype, wcn_stream(stream));

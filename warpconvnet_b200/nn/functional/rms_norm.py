@@ -13,13 +13,13 @@ from .batch_norm import _bits, apart, reverse_mode_only
 from .group_norm import _rows, _vector
 
 _MOST, _MOST_CHANNELS = 0x7FFFFEFF, 8192
-_LEAST_EPS = 1e-30
+_LEAST_EPS, _MOST_EPS = 1e-30, torch.finfo(torch.float32).max
 E4M3 = torch.float8_e4m3fn
 
 
 def check_eps(eps: float) -> float:
-    if not _LEAST_EPS <= eps < float("inf"):
-        raise ValueError(f"eps must be a number of at least {_LEAST_EPS}, got {eps}")
+    if not _LEAST_EPS <= eps <= _MOST_EPS:
+        raise ValueError(f"eps must be a number of at least {_LEAST_EPS} that fp32 holds, got {eps}")
     return eps
 
 
