@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from warpconvnet_b200._native import check_device_status, device_status, dtype_code, query_bytes
+from warpconvnet_b200._native import check_device_status, device_status
+from warpconvnet_b200._native import dtype_code, query_bytes
 from warpconvnet_b200.nn.functional.dropout import dropout
 from warpconvnet_b200.nn.functional.linear import linear, linear_8bit
 from warpconvnet_b200.nn.functional.rms_norm import quantize_rows
@@ -353,6 +354,26 @@ def test_strides_and_boundaries(dtype):
     lx, lw = wide[:0, :64].clone().requires_grad_(True), w.clone().requires_grad_(True)
     gx, gw = torch.autograd.grad(linear(lx, lw, None, "gelu", dropout_p=0.5).sum(), [lx, lw])
     assert gx.shape == (0, 64) and not gw.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act,p", [(None, 0.0), ("gelu", 0.2)])
+@pytest.mark.parametrize("n,k,m", [(20_001, 512, 400), (9_700, 1000, 776), (38_000, 768, 200)])
+def test_two_blocks_to_a_tile_both_ways(dtype, act, p, n, k, m):
+    """Forward, the gradient behind the activation and that of x, each with tiles cut at the rows' and the columns' end."""
+    x, w, b, r, dy = make(n, k, m, dtype)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = linear(x, w, b, act, r, p, 11)
+    got = torch.autograd.grad(y, leaves, dy)
+    x64, w64, b64, r64 = (t.detach().double() for t in leaves)
+    keep = (dropout(torch.ones(n, m, device=DEV), p, 11) != 0).double() / (1 - round(65536 * p) / 65536) if p else 1.0
+    a, slope = act64(x64 @ w64.t() + b64, act)
+    dz = dy.double() * keep * slope
+    assert off(y.detach(), r64 + keep * a) <= half(dtype)
+    for t, e in zip(got, (dz @ w64, dz.t() @ x64, dz.sum(0), dy.double())):   # dz's rounding and the result's
+        assert off(t, e) <= 2 * half(dtype)
+    assert all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(linear(x, w, b, act, r, p, 11), leaves, dy), got))
+    check_device_status(DEV)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
